@@ -26,6 +26,14 @@ TRIPS_LAYOUT_CHW = 0
 TRIPS_LAYOUT_HWC = 1
 TRIPS_DTYPE_F32 = 0
 TRIPS_DTYPE_F64 = 1
+TRIPS_DTYPE_BF16 = 2
+TRIPS_DTYPE_F16 = 3
+TRIPS_MOMENT_BLOCK = 256
+TRIPS_ADAMW_WORKSPACE_BYTES = 16384
+TRIPS_TABLE_COLUMNS = 0
+TRIPS_TABLE_ROWS = 1
+TRIPS_INDEX_I64 = 0
+TRIPS_INDEX_I32 = 1
 
 
 class TripsView(C.Structure):
@@ -159,6 +167,64 @@ class TripsUnetGrads(C.Structure):
         ("final_weight", C.c_void_p),
         ("final_bias", C.c_void_p),
         ("inputs", C.c_void_p * TRIPS_UNET_MAX_LEVELS),
+    ]
+
+
+class TripsAdamWTensor(C.Structure):
+    """include/trips_optim.h"""
+    _fields_ = [
+        ("weights", C.c_void_p),
+        ("grads", C.c_void_p),
+        ("first_moment", C.c_void_p),
+        ("second_moment", C.c_void_p),
+        ("first_scale", C.c_void_p),
+        ("second_scale", C.c_void_p),
+        ("copy", C.c_void_p),
+        ("step", C.c_void_p),
+        ("n", C.c_int64),
+        ("weight_dtype", C.c_int32),
+        ("grad_dtype", C.c_int32),
+        ("copy_dtype", C.c_int32),
+        ("state_bits", C.c_int32),
+        ("lr", C.c_double),
+        ("beta1", C.c_double),
+        ("beta2", C.c_double),
+        ("eps", C.c_double),
+        ("weight_decay", C.c_double),
+    ]
+
+
+class TripsAdamWOptions(C.Structure):
+    """include/trips_optim.h"""
+    _fields_ = [
+        ("abi_version", C.c_int32),
+        ("seed", C.c_uint32),
+        ("grad_norm", C.c_void_p),
+        ("compute_norm", C.c_int32),
+        ("max_norm", C.c_float),
+        ("loss_scale", C.c_float),
+    ]
+
+
+class TripsGradTensor(C.Structure):
+    """include/trips_optim.h"""
+    _fields_ = [("grads", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32)]
+
+
+class TripsLookupDesc(C.Structure):
+    """include/trips_lookup.h"""
+    _fields_ = [
+        ("abi_version", C.c_int32),
+        ("layout", C.c_int32),
+        ("dtype", C.c_int32),
+        ("index_dtype", C.c_int32),
+        ("num_texels", C.c_int64),
+        ("num_points", C.c_int64),
+        ("num_channels", C.c_int32),
+        ("accumulate", C.c_int32),
+        ("table_stride", C.c_int64),
+        ("values_stride", C.c_int64),
+        ("scale", C.c_float),
     ]
 
 

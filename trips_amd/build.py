@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtrips_splat.so")
 SOURCES = ["trips_splat_abi.hip", "splat_forward.hip", "splat_backward.hip", "misc_kernels.hip", "unet_forward.hip",
-           "unet_backward.hip"]
+           "unet_backward.hip", "adamw_kernels.hip", "lookup_kernels.hip"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
     # packed FP32 instructions are kept out of the generated code on purpose
@@ -24,8 +24,9 @@ def hipcc():
     raise RuntimeError("hipcc not found")
 
 
-HEADERS = ["splat_internal.h", "trips_math.h", "row16.h", "unet_common.h", os.path.join("..", "..", "include", "trips_splat.h"),
-           os.path.join("..", "..", "include", "trips_unet.h")]
+HEADERS = ["splat_internal.h", "trips_math.h", "row16.h", "unet_common.h", "abi_common.h", os.path.join("..", "..", "include", "trips_splat.h"),
+           os.path.join("..", "..", "include", "trips_unet.h"), os.path.join("..", "..", "include", "trips_optim.h"),
+           os.path.join("..", "..", "include", "trips_lookup.h")]
 
 
 def build(verbose=False, incremental=False):

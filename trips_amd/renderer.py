@@ -219,6 +219,36 @@ class SplatContext:
         _lib.check(self.lib.trips_adam_step_points(self.ctx, arr, int(num_points), int(num_channels), _ptr(state),
                                                    _stream_ptr(self.device)))
 
+    def adamw_step(self, tensors, n_tensors, options, workspace):
+        """tensors: an array of abi.TripsAdamWTensor, or its bytes; options: abi.TripsAdamWOptions; workspace: a device
+        tensor of abi.TRIPS_ADAMW_WORKSPACE_BYTES, zero before its first use."""
+        _lib.check(self.lib.trips_adamw_step(self.ctx, tensors, n_tensors, C.byref(options), _ptr(workspace), workspace.numel(),
+                                             _stream_ptr(self.device)))
+
+    def grad_norm(self, tensors, n_tensors, max_norm, loss_scale, out, workspace):
+        """tensors: an array of abi.TripsGradTensor, or its bytes; out: two device floats {norm, factor}."""
+        _lib.check(self.lib.trips_grad_norm(self.ctx, tensors, n_tensors, max_norm, loss_scale, _ptr(out), _ptr(workspace),
+                                            workspace.numel(), _stream_ptr(self.device)))
+
+    # ---- table lookups ----
+    def lookup_forward(self, desc, table, index, values):
+        _lib.check(self.lib.trips_lookup_forward(self.ctx, C.byref(desc), _ptr(table), _ptr(index), _ptr(values),
+                                                 _stream_ptr(self.device)))
+
+    def lookup_plan(self, num_texels, index, index_dtype, order, starts):
+        need = C.c_size_t(0)
+        _lib.check(self.lib.trips_lookup_plan_workspace_size(num_texels, index.numel(), C.byref(need)))
+        workspace = self.alloc_bytes(need.value)
+        _lib.check(self.lib.trips_lookup_plan(self.ctx, num_texels, index.numel(), _ptr(index), index_dtype, _ptr(order), _ptr(starts),
+                                              _ptr(workspace), workspace.numel(), _stream_ptr(self.device)))
+
+    def lookup_backward(self, desc, d_values, order, starts, d_table):
+        need = C.c_size_t(0)
+        _lib.check(self.lib.trips_lookup_backward_workspace_size(C.byref(desc), C.byref(need)))
+        workspace = self.alloc_bytes(need.value) if need.value else None
+        _lib.check(self.lib.trips_lookup_backward(self.ctx, C.byref(desc), _ptr(d_values), _ptr(order), _ptr(starts), _ptr(d_table),
+                                                  _ptr(workspace), need.value, _stream_ptr(self.device)))
+
     def apply_tangent(self, tangent, poses_se3):
         assert tangent.dtype == torch.float64 and poses_se3.dtype == torch.float64
         assert tangent.is_contiguous() and poses_se3.is_contiguous()
