@@ -34,16 +34,19 @@ typedef struct TripsLookupDesc {
     int32_t index_dtype; /* TRIPS_INDEX_* */
     int64_t num_texels;  /* T, below 2^31 - 1 */
     int64_t num_points;  /* N, below 2^31 - 1 */
-    int32_t num_channels; /* C, below 2^20 */
+    int32_t num_channels; /* C, below 2^17 */
     int32_t accumulate;   /* backward: 0 = d_table is written, zeros where no point refers to; 1 = added to */
     int64_t table_stride;  /* of table and d_table */
     int64_t values_stride; /* of values and d_values */
     float scale;
 } TripsLookupDesc;
 
-/* values of point i = scale * (entry index[i] of the table), rounded once; zeros where index[i] is outside [0, T). */
+/* values of point i = scale * (entry index[i] of the table), rounded once; zeros where index[i] is outside [0, T).
+ * `workspace`: trips_lookup_workspace_size bytes (0 in the rows layout), 256-byte aligned, of any content, like those below;
+ * calls that share one must not overlap. */
+int trips_lookup_workspace_size(const TripsLookupDesc* desc, size_t* bytes);
 int trips_lookup_forward(TripsCtx* ctx, const TripsLookupDesc* desc, const void* table, const void* index, void* values,
-                         void* stream);
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* The points in the order of their indexes: order [N] lists the points by (index, point), those with an index outside [0, T)
  * last; those of texel t are order[starts[t]] to order[starts[t + 1] - 1], starts [T + 1]. */

@@ -25,7 +25,7 @@ enum { TRIPS_DTYPE_BF16 = 2, TRIPS_DTYPE_F16 = 3 };
 
 /* Elements that share a scale where moments are held in 8 bits: element i of a tensor belongs to block i / 256. */
 #define TRIPS_MOMENT_BLOCK 256
-#define TRIPS_ADAMW_WORKSPACE_BYTES 16384
+#define TRIPS_GRAD_NORM_WORKSPACE_BYTES 8192
 
 /* One tensor. With a gradient factor f, step count t (from 1), all else per tensor:
  *
@@ -73,9 +73,10 @@ typedef struct TripsAdamWOptions {
     float loss_scale; /* the loss was multiplied by this */
 } TripsAdamWOptions;
 
-/* `tensors` is a HOST array. One launch steps up to 40 tensors of one combination of types (and two launches before it take
- * their norm). `workspace`: TRIPS_ADAMW_WORKSPACE_BYTES, 256-byte aligned, zero-filled before its first use; calls that
- * share it must not overlap. */
+/* `tensors` is a HOST array. All tensors of one combination of types (weights, gradients, state bits) are stepped by one
+ * launch, after a small one per 40 of them, and one or two before those that take the norm. `workspace`:
+ * trips_adamw_workspace_size bytes, 256-byte aligned, of any content; calls that share it must not overlap. */
+int trips_adamw_workspace_size(int n_tensors, size_t* bytes);
 int trips_adamw_step(TripsCtx* ctx, const TripsAdamWTensor* tensors, int n_tensors, const TripsAdamWOptions* options,
                      void* workspace, size_t workspace_bytes, void* stream);
 
@@ -87,8 +88,8 @@ typedef struct TripsGradTensor {
 
 /* grad_norm[0] = sqrt(sum of all squares) / loss_scale, grad_norm[1] = min(1, max_norm / (grad_norm[0] + 1e-6)) / loss_scale
  * (1 / loss_scale where max_norm <= 0; NaN where the norm is not finite). Squares are summed in double, in an order that
- * depends on the sizes alone. `grad_norm`: two device floats. `workspace`: TRIPS_ADAMW_WORKSPACE_BYTES, 256-byte aligned,
- * of any content; its first 256 bytes are left alone, so an optimiser's will do. */
+ * depends on the sizes alone. `grad_norm`: two device floats. `workspace`: TRIPS_GRAD_NORM_WORKSPACE_BYTES, 256-byte
+ * aligned, of any content; calls that share it must not overlap. */
 int trips_grad_norm(TripsCtx* ctx, const TripsGradTensor* tensors, int n_tensors, float max_norm, float loss_scale,
                     float* grad_norm, void* workspace, size_t workspace_bytes, void* stream);
 

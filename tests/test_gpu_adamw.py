@@ -413,6 +413,35 @@ def test_norm_of_large_and_small_numbers_and_of_nonfinite_ones():
     assert grad_norm([torch.zeros(10, device="cuda")], 1.0).tolist() == [0.0, 1.0]
 
 
+def test_hooks_closures_versions_and_schedulers():
+    from trips_amd.adamw import AdamW
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = AdamW([p], lr=0.1)
+    seen = []
+    before, after = opt.register_step_pre_hook(lambda *a: seen.append("before")), opt.register_step_post_hook(lambda *a: seen.append("after"))
+
+    def closure():
+        seen.append("loss")
+        opt.zero_grad()
+        loss = (p * p).sum()
+        loss.backward()
+        return loss
+    assert float(opt.step(closure)) == 8.0 and seen == ["before", "loss", "after"]
+    before.remove(), after.remove()
+    with torch.profiler.profile() as profile:
+        opt.step(closure)
+    assert seen == ["before", "loss", "after", "loss"]
+    assert any("AdamW" in e.name for e in profile.events())
+    scheduler = torch.optim.lr_scheduler.StepLR(opt, 1, 0.5)
+    opt.step(closure)
+    scheduler.step()
+    assert opt.param_groups[0]["lr"] == 0.05
+    loss = (p * p).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_refusals():
     from trips_amd._lib import TripsError
     from trips_amd.adamw import AdamW, grad_norm

@@ -31,22 +31,31 @@ def test_ctypes_mirrors_have_c_sizes(tmp_path):
     prog.write_text('#include <stdio.h>\n#include "trips_lookup.h"\nint main(){printf("%zu %zu %zu %zu %zu %zu %zu %d %d\\n",'
                     "sizeof(TripsAdamWTensor),offsetof(TripsAdamWTensor,lr),sizeof(TripsAdamWOptions),offsetof(TripsAdamWOptions,grad_norm),"
                     "sizeof(TripsGradTensor),sizeof(TripsLookupDesc),offsetof(TripsLookupDesc,scale),"
-                    "TRIPS_ADAMW_WORKSPACE_BYTES,TRIPS_MOMENT_BLOCK);return 0;}\n")
+                    "TRIPS_GRAD_NORM_WORKSPACE_BYTES,TRIPS_MOMENT_BLOCK);return 0;}\n")
     exe = tmp_path / "sizes"
     subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(prog), "-o", str(exe)])
     got = [int(x) for x in subprocess.check_output([str(exe)]).split()]
     assert got == [C.sizeof(abi.TripsAdamWTensor), abi.TripsAdamWTensor.lr.offset, C.sizeof(abi.TripsAdamWOptions),
                    abi.TripsAdamWOptions.grad_norm.offset, C.sizeof(abi.TripsGradTensor), C.sizeof(abi.TripsLookupDesc),
-                   abi.TripsLookupDesc.scale.offset, abi.TRIPS_ADAMW_WORKSPACE_BYTES, abi.TRIPS_MOMENT_BLOCK]
+                   abi.TripsLookupDesc.scale.offset, abi.TRIPS_GRAD_NORM_WORKSPACE_BYTES, abi.TRIPS_MOMENT_BLOCK]
     from trips_amd import adamw
-    assert struct.calcsize("8Qq4i5d") == C.sizeof(abi.TripsAdamWTensor) and struct.calcsize("Qqi4x") == C.sizeof(abi.TripsGradTensor)
-    t = abi.TripsAdamWTensor.from_buffer_copy(adamw._pack_tensor(*range(1, 10), 0, 2, 3, 8, 0.5, 0.25, 0.125, 1.0, 2.0))
+    assert struct.calcsize("8Qq4i") + struct.calcsize("5d") == C.sizeof(abi.TripsAdamWTensor) and struct.calcsize("Qqi4x") == C.sizeof(abi.TripsGradTensor)
+    t = abi.TripsAdamWTensor.from_buffer_copy(adamw._pack_tensor(*range(1, 10), 0, 2, 3, 8) + adamw._pack_options(0.5, 0.25, 0.125, 1.0, 2.0))
     assert (t.weights, t.step, t.n, t.weight_dtype, t.copy_dtype, t.state_bits, t.lr, t.weight_decay) == (1, 8, 9, 0, 3, 8, 0.5, 2.0)
 
 
 # A context stands behind a pointer that is not looked into before all arguments are checked; addresses are never used here.
 CTX = C.create_string_buffer(4096)
 AT = 1 << 20
+
+
+def _step_bytes(n):
+    b = C.c_size_t(0)
+    assert _lib.load().trips_adamw_workspace_size(n, C.byref(b)) == 0
+    return b.value
+
+
+STEP_BYTES = _step_bytes(2)
 
 
 def _tensor(**kw):
@@ -77,14 +86,14 @@ NAN = float("nan")
     ({}, dict(abi_version=1), {}), ({}, dict(compute_norm=1), {}), ({}, dict(max_norm=1.0), {}), ({}, dict(max_norm=NAN), {}),
     ({}, dict(loss_scale=0.0), {}), ({}, dict(loss_scale=NAN), {}), ({}, dict(loss_scale=float("inf")), {}),
     ({}, dict(grad_norm=AT + 1), {}),
-    ({}, {}, dict(workspace=None)), ({}, {}, dict(workspace=AT + 128)), ({}, {}, dict(size=abi.TRIPS_ADAMW_WORKSPACE_BYTES - 1)),
+    ({}, {}, dict(workspace=None)), ({}, {}, dict(workspace=AT + 128)), ({}, {}, dict(size=STEP_BYTES - 1)),
     ({}, {}, dict(ctx=None)), ({}, {}, dict(count=-1)),
 ])
 def test_adamw_refuses(tensor, options, call):
     lib = _lib.load()
     tensors = (abi.TripsAdamWTensor * 2)(_tensor(), _tensor(**tensor))
     rc = lib.trips_adamw_step(call.get("ctx", C.addressof(CTX)), tensors, call.get("count", 2), C.byref(_options(**options)),
-                              call.get("workspace", AT), call.get("size", abi.TRIPS_ADAMW_WORKSPACE_BYTES), None)
+                              call.get("workspace", AT), call.get("size", STEP_BYTES), None)
     assert rc in ERR and lib.trips_last_error_string()
 
 
@@ -99,7 +108,7 @@ def test_norm_refuses(tensor, call):
         setattr(t, k, v)
     tensors = (abi.TripsGradTensor * 1)(t)
     rc = lib.trips_grad_norm(C.addressof(CTX), tensors, call.get("count", 1), call.get("max_norm", 1.0), call.get("loss_scale", 1.0),
-                             call.get("out", AT), call.get("workspace", AT), call.get("size", abi.TRIPS_ADAMW_WORKSPACE_BYTES), None)
+                             call.get("out", AT), call.get("workspace", AT), call.get("size", abi.TRIPS_GRAD_NORM_WORKSPACE_BYTES), None)
     assert rc in ERR and lib.trips_last_error_string()
 
 
@@ -118,17 +127,19 @@ BAD_DESC = [dict(abi_version=1), dict(layout=2), dict(dtype=1), dict(dtype=9), d
 @pytest.mark.parametrize("desc,call", [(d, {}) for d in BAD_DESC] + [
     (dict(values_stride=49), {}), (dict(layout=1, values_stride=3), {}), ({}, dict(table=None)), ({}, dict(table=AT + 2)),
     ({}, dict(index=None)), ({}, dict(index=AT + 2)), (dict(index_dtype=0), dict(index=AT + 4)), ({}, dict(values=None)),
-    (dict(dtype=2), dict(values=AT + 1)), ({}, dict(ctx=None))])
+    (dict(dtype=2), dict(values=AT + 1)), ({}, dict(ctx=None)), ({}, dict(workspace=None)),
+    ({}, dict(workspace=AT + 16)), ({}, dict(size=100))])
 def test_lookup_refuses(desc, call):
     lib = _lib.load()
     rc = lib.trips_lookup_forward(call.get("ctx", C.addressof(CTX)), C.byref(_lookup(**desc)), call.get("table", AT), call.get("index", AT),
-                                  call.get("values", AT), None)
+                                  call.get("values", AT), call.get("workspace", AT), call.get("size", 1 << 30), None)
     assert rc in ERR and lib.trips_last_error_string()
 
 
 @pytest.mark.parametrize("desc,call", [(d, {}) for d in BAD_DESC] + [
     (dict(table_stride=99), {}), (dict(layout=1, table_stride=3), {}), ({}, dict(d_values=None)), ({}, dict(order=None)), ({}, dict(order=AT + 1)),
-    ({}, dict(starts=None)), ({}, dict(d_table=None)), (dict(dtype=3), dict(d_table=AT + 1))])
+    ({}, dict(starts=None)), ({}, dict(d_table=None)), (dict(dtype=3), dict(d_table=AT + 1)), ({}, dict(workspace=None)),
+    ({}, dict(size=700)), (dict(layout=1, table_stride=4, values_stride=4, num_points=1_000_000), dict(size=700))])
 def test_lookup_backward_refuses(desc, call):
     lib = _lib.load()
     rc = lib.trips_lookup_backward(C.addressof(CTX), C.byref(_lookup(**desc)), call.get("d_values", AT), call.get("order", AT),

@@ -24,10 +24,10 @@ UNET_SYMBOLS = ["trips_unet_workspace_size", "trips_unet_saved_size", "trips_une
                 "trips_unet_forward", "trips_unet_forward_hwc", "trips_unet_backward", "trips_unet_flops"]
 
 # every symbol include/trips_optim.h declares
-OPTIM_SYMBOLS = ["trips_adamw_step", "trips_grad_norm"]
+OPTIM_SYMBOLS = ["trips_adamw_workspace_size", "trips_adamw_step", "trips_grad_norm"]
 # every symbol include/trips_lookup.h declares
-LOOKUP_SYMBOLS = ["trips_lookup_forward", "trips_lookup_plan_workspace_size", "trips_lookup_plan",
-                  "trips_lookup_backward_workspace_size", "trips_lookup_backward"]
+LOOKUP_SYMBOLS = ["trips_lookup_workspace_size", "trips_lookup_forward", "trips_lookup_plan_workspace_size",
+                  "trips_lookup_plan", "trips_lookup_backward_workspace_size", "trips_lookup_backward"]
 
 
 class TripsError(RuntimeError):
@@ -82,9 +82,11 @@ def load():
     lib.trips_unet_backward.argtypes = [vp, C.POINTER(abi.TripsUnetDesc), C.POINTER(abi.TripsUnetWeights),
                                         C.POINTER(vp), vp, vp, C.c_float, C.POINTER(abi.TripsUnetGrads), vp,
                                         C.c_size_t, vp]
+    lib.trips_adamw_workspace_size.argtypes = [i32, C.POINTER(C.c_size_t)]
     lib.trips_adamw_step.argtypes = [vp, vp, i32, C.POINTER(abi.TripsAdamWOptions), vp, C.c_size_t, vp]
     lib.trips_grad_norm.argtypes = [vp, vp, i32, C.c_float, C.c_float, vp, vp, C.c_size_t, vp]
-    lib.trips_lookup_forward.argtypes = [vp, C.POINTER(abi.TripsLookupDesc), vp, vp, vp, vp]
+    lib.trips_lookup_workspace_size.argtypes = [C.POINTER(abi.TripsLookupDesc), C.POINTER(C.c_size_t)]
+    lib.trips_lookup_forward.argtypes = [vp, C.POINTER(abi.TripsLookupDesc), vp, vp, vp, vp, C.c_size_t, vp]
     lib.trips_lookup_plan_workspace_size.argtypes = [i64, i64, C.POINTER(C.c_size_t)]
     lib.trips_lookup_plan.argtypes = [vp, i64, i64, vp, i32, vp, vp, vp, C.c_size_t, vp]
     lib.trips_lookup_backward_workspace_size.argtypes = [C.POINTER(abi.TripsLookupDesc), C.POINTER(C.c_size_t)]

@@ -29,7 +29,7 @@ TRIPS_DTYPE_F64 = 1
 TRIPS_DTYPE_BF16 = 2
 TRIPS_DTYPE_F16 = 3
 TRIPS_MOMENT_BLOCK = 256
-TRIPS_ADAMW_WORKSPACE_BYTES = 16384
+TRIPS_GRAD_NORM_WORKSPACE_BYTES = 8192
 TRIPS_TABLE_COLUMNS = 0
 TRIPS_TABLE_ROWS = 1
 TRIPS_INDEX_I64 = 0

@@ -11,47 +11,61 @@ import math
 import struct
 
 import torch
+from torch.autograd import _profiler_enabled
+from torch.autograd.graph import increment_version as _increment_version
+from torch.optim import optimizer as _optimizer
 
 from . import abi
 from .renderer import get_context
 
 _DTYPES = {torch.float32: abi.TRIPS_DTYPE_F32, torch.bfloat16: abi.TRIPS_DTYPE_BF16, torch.float16: abi.TRIPS_DTYPE_F16}
-_pack_tensor = struct.Struct("8Qq4i5d").pack  # TripsAdamWTensor
-_pack_grad = struct.Struct("Qqi4x").pack      # TripsGradTensor
+_pack_tensor, _pack_options = struct.Struct("8Qq4i").pack, struct.Struct("5d").pack  # TripsAdamWTensor up to `lr`, and from there
+_pack_grad = struct.Struct("Qqi4x").pack                                             # TripsGradTensor
 _MOMENTS = {8: (torch.float8_e4m3fn, torch.float8_e5m2), 32: (torch.float32, torch.float32)}
 
 
-def _check_grad(g):
+def _contiguous(g):
+    if g.is_sparse:
+        _refuse(None, g, 0)
+    return g.detach().contiguous()
+
+
+def _refuse(p, g, device):
+    """Says what is wrong with a parameter (or None) and its gradient."""
     if g.is_sparse:
         raise RuntimeError("sparse gradients are not supported")
     if g.dtype not in _DTYPES:
         raise RuntimeError(f"gradients are float32, bfloat16 or float16, not {g.dtype}")
-    return g if g.is_contiguous() else g.contiguous()
-
-
-def _device_of(tensors):
-    device = tensors[0].device
-    if device.type != "cuda":
+    if p is not None and (p.dtype not in _DTYPES or not p.is_contiguous()):
+        raise RuntimeError("AdamW needs contiguous float32, bfloat16 or float16 parameters")
+    if p is not None and g.numel() != p.numel():
+        raise RuntimeError(f"a gradient of {g.numel()} elements for a parameter of {p.numel()}")
+    if device < 0:
         raise RuntimeError("the kernels need tensors on a GPU: there is no CPU implementation")
-    for t in tensors:
-        if t.device != device:
-            raise RuntimeError(f"all tensors of a call must be on one device: {t.device} and {device}")
-    return device
+    raise RuntimeError("all tensors of a call must be on one device")
 
 
-@torch.no_grad()
 def grad_norm(grads, max_norm=0.0, loss_scale=1.0):
     """[norm, factor] of a list of gradients as a float32 tensor on their device: the root of the sum of all their squares
     divided by loss_scale, and what gradients are multiplied by to undo loss_scale and to clip their norm at max_norm
     (0: no clipping); the factor is NaN where the norm is not finite. Nothing is read back. AdamW.step() takes it as `grad_norm`."""
-    grads = [_check_grad(g) for g in grads]
-    if not grads:
+    table, temporary, device = [], [], None
+    for g in grads:
+        dtype, index = _DTYPES.get(g.dtype), g.get_device()
+        if device is None:
+            device = index
+        if dtype is None or index < 0 or index != device:
+            _refuse(None, g, device)
+        if not g.is_contiguous():
+            g = _contiguous(g)
+            temporary.append(g)
+        table.append(_pack_grad(g.data_ptr(), g.numel(), dtype))
+    if not table:
         raise ValueError("grad_norm of no gradients")
-    device = _device_of(grads)
     ctx = get_context(device)
+    device = ctx.device
     out = torch.empty(2, dtype=torch.float32, device=device)
-    table = b"".join([_pack_grad(g.data_ptr(), g.numel(), _DTYPES[g.dtype]) for g in grads])
-    ctx.grad_norm(table, len(grads), max_norm, loss_scale, out, ctx.alloc_bytes(abi.TRIPS_ADAMW_WORKSPACE_BYTES))
+    ctx.grad_norm(b"".join(table), len(table), max_norm, loss_scale, out, ctx.alloc_bytes(abi.TRIPS_GRAD_NORM_WORKSPACE_BYTES))
     return out
 
 
@@ -119,56 +133,76 @@ class AdamW(torch.optim.Optimizer):
             st["second_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
         return st
 
-    @torch.no_grad()
     def step(self, closure=None, grads=None, grad_norm=None):
         """grads: {parameter: gradient}, for gradients in another type than their parameter's, instead of the parameters' own;
         grad_norm: the [norm, factor] to go by, where this optimiser's gradients are only some of those whose norm counts."""
+        if self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _optimizer._global_optimizer_pre_hooks \
+                or _optimizer._global_optimizer_post_hooks or _profiler_enabled():
+            return _watched_step(self, closure, grads, grad_norm)
+        return self._step(closure, grads, grad_norm)
+
+    # The base class would wrap step() for its hooks and the profiler's range: some 10 us a step, as much as the kernels take of
+    # a small net's. Here that way is gone where there is something to call.
+    step.hooked = True
+
+    def _step(self, closure, grads, grad_norm):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        table, keep, device = [], [], None
+        # (An attribute or a call costs 50 to 100 ns, of which a tensor takes a score; what a check finds is said in _refuse.)
+        table, params, temporary, device, copies, states, dtypes = [], [], [], None, self._copies, self.state, _DTYPES
         for group in self.param_groups:
-            (beta1, beta2), lr, eps, decay = group["betas"], group["lr"], group["eps"], group["weight_decay"]
+            options = _pack_options(group["lr"], *group["betas"], group["eps"], group["weight_decay"])
             for p in group["params"]:
                 g = p.grad if grads is None else grads.get(p)
                 if g is None:
                     continue
-                weight_dtype = _DTYPES.get(p.dtype)
-                if weight_dtype is None or not p.is_contiguous():
-                    raise RuntimeError("AdamW needs contiguous float32, bfloat16 or float16 parameters")
-                g = _check_grad(g)
-                n = p.numel()
-                if g.numel() != n:
-                    raise RuntimeError(f"a gradient of {g.numel()} elements for a parameter of {n}")
-                keep += (p, g)
-                st = self.state.get(p) or self._make_state(p, group)
-                first, first_scale = st["first_moment"], st.get("first_scale")
-                copy = self._copies.get(p) if self._copies else None
-                table.append(_pack_tensor(
-                    p.data_ptr(), g.data_ptr(), first.data_ptr(), st["second_moment"].data_ptr(),
-                    0 if first_scale is None else first_scale.data_ptr(), 0 if first_scale is None else st["second_scale"].data_ptr(),
-                    0 if copy is None else copy.data_ptr(), st["step"].data_ptr(), n, weight_dtype, _DTYPES[g.dtype],
-                    0 if copy is None else _DTYPES[copy.dtype], 32 if first_scale is None else 8, lr, beta1, beta2, eps, decay))
-        if not table:
+                n, index = p.numel(), p.get_device()
+                weight_dtype, grad_dtype = dtypes.get(p.dtype), dtypes.get(g.dtype)
+                if device is None:
+                    device = index
+                if weight_dtype is None or grad_dtype is None or index < 0 or index != device or g.get_device() != index \
+                        or g.numel() != n or not p.is_contiguous():
+                    _refuse(p, g, device)
+                if not g.is_contiguous():
+                    g = _contiguous(g)
+                    temporary.append(g)
+                st = states.get(p) or self._make_state(p, group)
+                if "first_scale" in st:
+                    first_scale, second_scale, bits = st["first_scale"].data_ptr(), st["second_scale"].data_ptr(), 8
+                else:
+                    first_scale, second_scale, bits = 0, 0, 32
+                copy_at, copy_dtype = 0, 0
+                if copies:
+                    copy = copies.get(p)
+                    if copy is not None:
+                        copy_at, copy_dtype = copy.data_ptr(), dtypes[copy.dtype]
+                params.append(p)
+                table += (_pack_tensor(p.data_ptr(), g.data_ptr(), st["first_moment"].data_ptr(), st["second_moment"].data_ptr(),
+                                       first_scale, second_scale, copy_at, st["step"].data_ptr(), n, weight_dtype, grad_dtype,
+                                       copy_dtype, bits), options)
+        if not params:
             return loss
-        device = _device_of(keep)
         ctx = get_context(device)
-        if self._workspace is None or self._workspace.device != device:
-            self._workspace = torch.zeros(abi.TRIPS_ADAMW_WORKSPACE_BYTES, dtype=torch.uint8, device=device)
-            self._norm = torch.empty(2, dtype=torch.float32, device=device)
+        if self._workspace is None or self._workspace.device != ctx.device or self._workspace_for < len(params):
+            self._workspace = ctx.alloc_bytes(ctx.adamw_workspace_size(len(params)))
+            self._workspace_for = len(params)
+            self._norm = torch.empty(2, dtype=torch.float32, device=ctx.device)
         max_norm = self.max_grad_norm or 0.0
         compute = grad_norm is None and (max_norm > 0 or self.skip_nonfinite)
-        if grad_norm is not None and (grad_norm.dtype != torch.float32 or grad_norm.numel() != 2 or grad_norm.device != device
+        if grad_norm is not None and (grad_norm.dtype != torch.float32 or grad_norm.numel() != 2 or grad_norm.device != ctx.device
                                       or not grad_norm.is_contiguous()):
             raise ValueError("grad_norm: two float32 numbers on the parameters' device expected")
         self.grad_norm = self._norm if compute else grad_norm
         options = abi.TripsAdamWOptions(abi.TRIPS_ABI_VERSION, self.seed & 0xFFFFFFFF,
                                         None if self.grad_norm is None else self.grad_norm.data_ptr(), int(compute),
                                         max_norm if compute else 0.0, self.loss_scale)
-        ctx.adamw_step(b"".join(table), len(table), options, self._workspace)
+        ctx.adamw_step(b"".join(table), len(params), options, self._workspace)
+        _increment_version(params)  # (a backward pass that needs the old values raises)
         return loss
 
+    @torch.no_grad()
     def moments(self, p):
         """First and second moment of a parameter as float32 tensors of its shape."""
         st = self.state[p]
@@ -190,3 +224,6 @@ class AdamW(torch.optim.Optimizer):
             st = state_dict["state"].get(i)
             if st is not None:
                 self.state[p] = {k: v.detach().to(p.device).clone() if torch.is_tensor(v) else v for k, v in st.items()}
+
+
+_watched_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)

@@ -58,6 +58,18 @@ struct Element<TRIPS_DTYPE_F16>
     static __device__ __forceinline__ unsigned short from_float(float x) { return __builtin_bit_cast(unsigned short, (_Float16)x); }
 };
 
+// Pointers that a kernel finds in memory: said to be global (the compiler would take them for any kind), or to a table that no
+// kernel writes while this one runs (read by scalar loads).
+template <typename T>
+using Global = __attribute__((address_space(1))) T*;
+template <typename T>
+using Constant = const __attribute__((address_space(4))) T*;
+template <typename T>
+__device__ __forceinline__ Global<T> global(T* p)
+{
+    return (Global<T>)p;
+}
+
 // N elements side by side, at any address that their type allows (global memory takes wide accesses there too).
 template <typename T, int N>
 struct Pack

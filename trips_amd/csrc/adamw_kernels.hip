@@ -8,6 +8,7 @@
 #include <cmath>
 
 #include "abi_common.h"
+#include "row16.h"
 
 #pragma clang fp contract(off)
 
@@ -15,15 +16,38 @@ namespace trips
 {
 namespace
 {
-constexpr int kTensors     = 40;   // tensors of a launch: what 4 KB of kernel arguments hold
+constexpr int kTensors     = 40;   // tensors of a table in the kernel's arguments (4 KB)
 constexpr int kGroups      = 8;    // different sets of options among them
+constexpr int kStepTensors = 4096; // tensors of a step's launch
 constexpr int kTileOptim   = 1024; // elements of a tile: four wavefronts with a block of 256 each
-constexpr int kStepGroups  = 2048; // workgroups of a step
-constexpr int kNormTensors = 120;
+constexpr int kStepGroups  = 2048; // workgroups of a step with a tile each
+constexpr int kStepRun     = 2;    // tiles of a workgroup, one behind the other, where there are more tiles
+constexpr int kNormTensors = 140; // of a launch: 4 KB of arguments
 constexpr int kNormTile    = 4096; // elements of a tile of the norm
 constexpr int kNormGroups  = 1024; // workgroups of the norm = partial sums
 static_assert(TRIPS_MOMENT_BLOCK == 256, "a block is four elements a lane");
-static_assert(256 + kNormGroups * sizeof(double) <= TRIPS_ADAMW_WORKSPACE_BYTES, "workspace");
+static_assert(kNormGroups * sizeof(double) <= TRIPS_GRAD_NORM_WORKSPACE_BYTES, "workspace");
+
+// A tensor as the step's kernel reads it, made by the kernel before it from what the host knows (StepTensor) and the step count
+// on the device. (In the step's own arguments, searched by every workgroup entry by entry, the table cost more than the work
+// of a small call: the benchmark's net 10 us, 40 tensors 39.)
+struct StepEntry
+{
+    void* w;
+    const void* g;
+    void* m;
+    void* v;
+    float* ms;
+    float* vs;
+    void* copy;
+    long long n;
+    double b1, c1, b2, c2;        // beta and 1 - beta
+    float fb1, fc1, fb2, fc2;     // the same in float
+    float keep, rate, root, eps;  // 1 - lr decay, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
+    uint32_t key;                 // of the rounding
+    uint32_t first_block;         // of the call, in blocks of 256 elements
+    uint32_t copy_dtype, unused;
+};
 
 struct StepTensor
 {
@@ -36,8 +60,8 @@ struct StepTensor
     void* copy;
     int32_t* step;
     long long n;
-    uint32_t first_tile;   // of this launch
-    uint32_t first_block;  // of the call, in blocks of 256 elements
+    uint32_t first_tile;  // of the step's launch
+    uint32_t first_block;
     uint8_t group, copy_dtype;
 };
 struct StepOptions
@@ -48,13 +72,24 @@ struct StepTable
 {
     StepTensor t[kTensors];
     StepOptions o[kGroups];
-    uint32_t n, tiles;
-    uint32_t seed;
-    float factor;            // where there is no `norm`
-    const float* norm;       // {norm, factor} or NULL
-    uint32_t* ticket;        // workgroups that are done, 0 between launches
+    uint32_t n, seed;
+    float* norm;           // {norm, factor} or NULL
+    const double* sums;    // squares to make the norm of first, or NULL
+    uint32_t groups;       // how many
+    float max_norm, loss_scale;
+    StepEntry* entries;
+    uint32_t* first_tiles;
 };
 static_assert(sizeof(StepTable) <= 4096, "kernel arguments");
+
+struct StepParams
+{
+    const StepEntry* entries;
+    const uint32_t* first_tiles;
+    uint32_t n, tiles, run;  // run: tiles of a workgroup, one behind the other
+    const float* norm;
+    float factor;  // where there is no `norm`
+};
 
 // beta^t by squaring, in double
 __device__ __forceinline__ double power(double beta, uint32_t t)
@@ -80,11 +115,15 @@ __device__ __forceinline__ uint32_t mix(uint32_t x)
     return x;
 }
 
+// Of all lanes, the same for all.
 __device__ __forceinline__ uint32_t wave_max(uint32_t x)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o));
-    return x;
+    x = max(x, (uint32_t)dpp_i<kDppXor1>((int)x));
+    x = max(x, (uint32_t)dpp_i<kDppXor2>((int)x));
+    x = max(x, (uint32_t)dpp_i<kDppHalfMirror>((int)x));
+    x = max(x, (uint32_t)dpp_i<kDppMirror>((int)x));
+    auto of = [&](int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)x, lane); };
+    return max(max(of(0), of(16)), max(of(32), of(48)));
 }
 
 // The high word of |x|, one more where the low word holds something: compares like |x| against numbers of 20 mantissa bits.
@@ -105,14 +144,13 @@ __device__ __forceinline__ int scale_exponent(uint32_t top)
 }
 
 // |x| 2^-k as a code of an 8-bit float with MANTISSA bits and exponent bias BIAS: floor(y / q + (r + 0.5) / 65536) steps q,
-// at most MOST. The bits of a double are such a code, followed by 52 - MANTISSA more and with another bias; the steps are added
-// to those of the high word, whose carry is the rounding (what the low word holds can make no carry: the addend is a multiple
-// of the high word's last place). Below the lowest normal number steps stay as they are: the significand shifts right instead.
+// at most MOST; `hi`: the high word of |x|, finite. The bits of a double are such a code, followed by 52 - MANTISSA more and with
+// another bias; the steps are added to those of the high word, whose carry is the rounding (what the low word holds can make no
+// carry: the addend is a multiple of the high word's last place). Below the lowest normal number steps stay as they are: the
+// significand shifts right instead.
 template <int MANTISSA, int BIAS, int MOST>
-__device__ __forceinline__ uint32_t encode(double x, int k, uint32_t r)
+__device__ __forceinline__ uint32_t encode(uint32_t hi, int k, uint32_t r)
 {
-    const uint32_t hi = (uint32_t)((unsigned long long)__double_as_longlong(x) >> 32) & 0x7fffffffu;
-    if (hi >= 0x7ff00000u) return 0x7fu;  // infinite or no number: no number
     const int t        = (int)hi - (k + 1023 - BIAS) * (1 << 20);
     const int e        = t >> 20;
     const uint32_t sig = 0x100000u | (hi & 0xfffffu);
@@ -121,36 +159,25 @@ __device__ __forceinline__ uint32_t encode(double x, int k, uint32_t r)
     return min((y + ((2u * r + 1u) << (DROP - 17))) >> DROP, (uint32_t)MOST);
 }
 
-// The launch's rates of one tensor at step t.
-struct Rates
+// The new weight. Root and reciprocal are the instructions' own (off by one place each); a root of v below the normal numbers
+// counts as 0, which is nothing beside an eps of 2^-40 or more. Below that they are taken exactly.
+constexpr float kLeastEps = 0x1p-40f;
+template <bool EXACT>
+__device__ __forceinline__ float stepped(Constant<StepEntry> r, float w, float m, float v)
 {
-    double b1, c1, b2, c2;       // beta and 1 - beta
-    float fb1, fc1, fb2, fc2;    // the same in float
-    float keep, rate, root, eps; // 1 - lr decay, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
-};
-__device__ __forceinline__ Rates rates(const StepOptions& o, uint32_t t)
-{
-    Rates r;
-    r.b1 = o.beta1, r.c1 = 1.0 - o.beta1, r.b2 = o.beta2, r.c2 = 1.0 - o.beta2;
-    r.fb1 = (float)r.b1, r.fc1 = (float)r.c1, r.fb2 = (float)r.b2, r.fc2 = (float)r.c2;
-    r.keep = (float)(1.0 - o.lr * o.decay);
-    r.rate = (float)(o.lr / (1.0 - power(o.beta1, t)));
-    r.root = (float)(1.0 / sqrt(1.0 - power(o.beta2, t)));
-    r.eps  = (float)o.eps;
-    return r;
+    if constexpr (EXACT) return fmaf(-r->rate, m / fmaf(sqrtf(v), r->root, r->eps), r->keep * w);
+    const float down = __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(v), r->root, r->eps));
+    return fmaf(-r->rate * m, down, r->keep * w);
 }
 
-__device__ __forceinline__ float stepped(const Rates& r, float w, float m, float v)
-{
-    return fmaf(-r.rate, m / fmaf(sqrtf(v), r.root, r.eps), r.keep * w);
-}
+typedef uint32_t Codes __attribute__((aligned(1)));  // four codes of 8 bits
 
 template <typename T>
-__device__ __forceinline__ void load4(const T* from, bool whole, int count, T (&x)[4])
+__device__ __forceinline__ void load4(Global<const T> from, bool whole, int count, T (&x)[4])
 {
     if (whole)
     {
-        const auto q = __builtin_nontemporal_load(reinterpret_cast<const typename Pack<T, 4>::type*>(from));
+        const auto q = __builtin_nontemporal_load((Global<const typename Pack<T, 4>::type>)from);
         x[0] = q.x, x[1] = q.y, x[2] = q.z, x[3] = q.w;
     }
     else
@@ -160,12 +187,12 @@ __device__ __forceinline__ void load4(const T* from, bool whole, int count, T (&
     }
 }
 template <typename T>
-__device__ __forceinline__ void store4(T* to, bool whole, int count, const T (&x)[4])
+__device__ __forceinline__ void store4(Global<T> to, bool whole, int count, const T (&x)[4])
 {
     if (whole)
     {
         typename Pack<T, 4>::type q = {x[0], x[1], x[2], x[3]};
-        __builtin_nontemporal_store(q, reinterpret_cast<typename Pack<T, 4>::type*>(to));
+        __builtin_nontemporal_store(q, (Global<typename Pack<T, 4>::type>)to);
     }
     else
     {
@@ -175,45 +202,148 @@ __device__ __forceinline__ void store4(T* to, bool whole, int count, const T (&x
     }
 }
 
-// Four elements a lane, a block of 256 a wavefront.
+template <int WD>
+__device__ __forceinline__ void store_weights(Constant<StepEntry> T, long long i0, bool whole, int count, const float (&nw)[4])
+{
+    using W = typename Element<WD>::type;
+    W w4[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w4[i] = Element<WD>::from_float(nw[i]);
+    store4(global(reinterpret_cast<W*>(T->w)) + i0, whole, count, w4);
+    if (!T->copy) return;
+    if (T->copy_dtype == TRIPS_DTYPE_F32)
+        store4(global(reinterpret_cast<float*>(T->copy)) + i0, whole, count, nw);
+    else
+    {
+        const bool bf = T->copy_dtype == TRIPS_DTYPE_BF16;
+        unsigned short c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = bf ? Element<TRIPS_DTYPE_BF16>::from_float(nw[i]) : Element<TRIPS_DTYPE_F16>::from_float(nw[i]);
+        store4(global(reinterpret_cast<unsigned short*>(T->copy)) + i0, whole, count, c);
+    }
+}
+
+// Four elements a lane, a block of 256 a wavefront. Returns whether it was done: not where the block is one for step_any.
 template <int WD, int GD, int BITS>
-__device__ __forceinline__ void step_block(const StepTensor& T, const Rates& r, float factor, uint32_t key, long long block, int lane)
+__device__ __forceinline__ bool step_whole(Constant<StepEntry> T, float factor, long long block, int lane)
 {
     using W = typename Element<WD>::type;
     using G = typename Element<GD>::type;
     const long long i0 = block * TRIPS_MOMENT_BLOCK + lane * 4;
-    const long long left = T.n - i0;
-    const int count      = left >= 4 ? 4 : left > 0 ? (int)left : 0;
-    const bool whole     = count == 4;
     W w4[4];
     G g4[4];
-    load4(reinterpret_cast<const G*>(T.g) + i0, whole, count, g4);
-    load4(reinterpret_cast<const W*>(T.w) + i0, whole, count, w4);
+    load4(global(reinterpret_cast<const G*>(T->g)) + i0, true, 4, g4);
+    load4(global(reinterpret_cast<const W*>(T->w)) + i0, true, 4, w4);
     float nw[4];
     if constexpr (BITS == 32)
     {
         float m[4], v[4];
-        float* mo = reinterpret_cast<float*>(T.m) + i0;
-        float* vo = reinterpret_cast<float*>(T.v) + i0;
+        const auto mo = global(reinterpret_cast<float*>(T->m)) + i0;
+        const auto vo = global(reinterpret_cast<float*>(T->v)) + i0;
+        load4(mo, true, 4, m);
+        load4(vo, true, 4, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            const float g = Element<GD>::to_float(g4[i]) * factor;
+            m[i]  = fmaf(T->fc1, g, T->fb1 * m[i]);
+            v[i]  = fmaf(T->fc2 * g, g, T->fb2 * v[i]);
+            nw[i] = stepped<false>(T, Element<WD>::to_float(w4[i]), m[i], v[i]);
+        }
+        store4(mo, true, 4, m);
+        store4(vo, true, 4, v);
+    }
+    else
+    {
+        // The new moments in double: which code they get must not depend on roundings on the way.
+        const auto mo = (Global<Codes>)(global(reinterpret_cast<unsigned char*>(T->m)) + i0);
+        const auto vo = (Global<Codes>)(global(reinterpret_cast<unsigned char*>(T->v)) + i0);
+        const int mw = (int)__builtin_nontemporal_load(mo), vw = (int)__builtin_nontemporal_load(vo);
+        const double bm = T->b1 * (double)((Constant<float>)T->ms)[block], bv = T->b2 * (double)((Constant<float>)T->vs)[block];
+        const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8(mw, false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8(mw, true);
+        const auto v01 = __builtin_amdgcn_cvt_pk_f32_bf8(vw, false), v23 = __builtin_amdgcn_cvt_pk_f32_bf8(vw, true);
+        const float mf[4] = {m01[0], m01[1], m23[0], m23[1]}, vf[4] = {v01[0], v01[1], v23[0], v23[1]};
+        uint32_t mh[4], vh[4], mtop = 0, vtop = 0;  // the high words of the moments
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            const double g = (double)Element<GD>::to_float(g4[i]) * (double)factor;
+            const double m = fma(T->c1, g, bm * (double)mf[i]);
+            const double v = fma(T->c2 * g, g, bv * (double)vf[i]);
+            nw[i] = stepped<false>(T, Element<WD>::to_float(w4[i]), (float)m, (float)v);
+            mh[i] = (uint32_t)((unsigned long long)__double_as_longlong(m) >> 32);
+            vh[i] = (uint32_t)((unsigned long long)__double_as_longlong(v) >> 32);
+            mtop  = max(mtop, mh[i] & 0x7fffffffu);
+            vtop  = max(vtop, vh[i]);
+        }
+        mtop = wave_max(mtop), vtop = wave_max(vtop);
+        // not finite (or a negative v), or a largest number so near the border of two scales that the low words decide
+        if (mtop >= 0x7ff00000u || vtop >= 0x7ff00000u || (mtop & 0xfffffu) == 0xc0000u || (vtop & 0xfffffu) == 0xc0000u) return false;
+        const int km = scale_exponent<9>(mtop), kv = scale_exponent<16>(vtop);
+        const uint32_t at = (T->first_block + (uint32_t)block) * TRIPS_MOMENT_BLOCK + (uint32_t)lane * 4u;
+        uint32_t mc = 0, vc = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            const uint32_t bits = mix((at + i) ^ T->key);
+            mc |= (encode<3, 7, 0x7e>(mh[i] & 0x7fffffffu, km, bits & 0xffffu) | (mh[i] >> 24 & 0x80u)) << (8 * i);
+            vc |= max(encode<2, 15, 0x7b>(vh[i], kv, bits >> 16), vh[i] ? 1u : 0u) << (8 * i);
+        }
+        __builtin_nontemporal_store(mc, mo);
+        __builtin_nontemporal_store(vc, vo);
+        if (lane == 0)
+        {
+            global(T->ms)[block] = __uint_as_float((uint32_t)(km + 127) << 23);
+            global(T->vs)[block] = __uint_as_float((uint32_t)(kv + 127) << 23);
+        }
+    }
+    store_weights<WD>(T, i0, true, 4, nw);
+    return true;
+}
+
+__device__ __forceinline__ float stepped_any(Constant<StepEntry> T, float w, float m, float v)
+{
+    return T->eps < kLeastEps ? stepped<true>(T, w, m, v) : stepped<false>(T, w, m, v);
+}
+
+// The same for any block: a tensor's last, numbers that are not finite, an eps near zero.
+template <int WD, int GD, int BITS>
+__device__ __forceinline__ void step_any(Constant<StepEntry> T, float factor, long long block, int lane)
+{
+    using W = typename Element<WD>::type;
+    using G = typename Element<GD>::type;
+    const long long i0 = block * TRIPS_MOMENT_BLOCK + lane * 4;
+    const long long left = T->n - i0;
+    const int count      = left >= 4 ? 4 : left > 0 ? (int)left : 0;
+    const bool whole     = count == 4;
+    W w4[4];
+    G g4[4];
+    load4(global(reinterpret_cast<const G*>(T->g)) + i0, whole, count, g4);
+    load4(global(reinterpret_cast<const W*>(T->w)) + i0, whole, count, w4);
+    float nw[4];
+    if constexpr (BITS == 32)
+    {
+        float m[4], v[4];
+        const auto mo = global(reinterpret_cast<float*>(T->m)) + i0;
+        const auto vo = global(reinterpret_cast<float*>(T->v)) + i0;
         load4(mo, whole, count, m);
         load4(vo, whole, count, v);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
         {
             const float g = Element<GD>::to_float(g4[i]) * factor;
-            m[i]  = fmaf(r.fc1, g, r.fb1 * m[i]);
-            v[i]  = fmaf(r.fc2 * g, g, r.fb2 * v[i]);
-            nw[i] = stepped(r, Element<WD>::to_float(w4[i]), m[i], v[i]);
+            m[i]  = fmaf(T->fc1, g, T->fb1 * m[i]);
+            v[i]  = fmaf(T->fc2 * g, g, T->fb2 * v[i]);
+            nw[i] = stepped_any(T, Element<WD>::to_float(w4[i]), m[i], v[i]);
         }
         store4(mo, whole, count, m);
         store4(vo, whole, count, v);
     }
     else
     {
-        // The new moments in double: which code they get must not depend on roundings on the way.
         unsigned char m4[4], v4[4];
-        unsigned char* mo = reinterpret_cast<unsigned char*>(T.m) + i0;
-        unsigned char* vo = reinterpret_cast<unsigned char*>(T.v) + i0;
+        const auto mo = global(reinterpret_cast<unsigned char*>(T->m)) + i0;
+        const auto vo = global(reinterpret_cast<unsigned char*>(T->v)) + i0;
         load4(mo, whole, count, m4);
         load4(vo, whole, count, v4);
         const unsigned mw = m4[0] | m4[1] << 8 | m4[2] << 16 | (unsigned)m4[3] << 24;
@@ -221,28 +351,30 @@ __device__ __forceinline__ void step_block(const StepTensor& T, const Rates& r, 
         const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mw, false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mw, true);
         const auto v01 = __builtin_amdgcn_cvt_pk_f32_bf8((int)vw, false), v23 = __builtin_amdgcn_cvt_pk_f32_bf8((int)vw, true);
         const float mf[4] = {m01[0], m01[1], m23[0], m23[1]}, vf[4] = {v01[0], v01[1], v23[0], v23[1]};
-        const double bm = r.b1 * (double)T.ms[block], bv = r.b2 * (double)T.vs[block];
+        const double bm = T->b1 * (double)global(T->ms)[block], bv = T->b2 * (double)global(T->vs)[block];
         double m[4], v[4];
         uint32_t mtop = 0, vtop = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
         {
             const double g = (double)Element<GD>::to_float(g4[i]) * (double)factor;
-            m[i]  = fma(r.c1, g, bm * (double)mf[i]);
-            v[i]  = fma(r.c2 * g, g, bv * (double)vf[i]);
-            nw[i] = stepped(r, Element<WD>::to_float(w4[i]), (float)m[i], (float)v[i]);
+            m[i]  = fma(T->c1, g, bm * (double)mf[i]);
+            v[i]  = fma(T->c2 * g, g, bv * (double)vf[i]);
+            nw[i] = stepped_any(T, Element<WD>::to_float(w4[i]), (float)m[i], (float)v[i]);
             const uint32_t mh = high_word_up(m[i]), vh = high_word_up(v[i]);
             mtop = max(mtop, mh < 0x7ff00000u ? mh : 0u);
             vtop = max(vtop, vh < 0x7ff00000u ? vh : 0u);
         }
         const int km = scale_exponent<9>(wave_max(mtop)), kv = scale_exponent<16>(wave_max(vtop));
-        const uint32_t at = (T.first_block + (uint32_t)block) * TRIPS_MOMENT_BLOCK + (uint32_t)lane * 4u;
+        const uint32_t at = (T->first_block + (uint32_t)block) * TRIPS_MOMENT_BLOCK + (uint32_t)lane * 4u;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
         {
-            const uint32_t bits = mix((at + i) ^ key);
-            const uint32_t mc = encode<3, 7, 0x7e>(m[i], km, bits & 0xffffu);
-            const uint32_t vc = encode<2, 15, 0x7b>(v[i], kv, bits >> 16);
+            const uint32_t bits = mix((at + i) ^ T->key);
+            const uint32_t mh = (uint32_t)((unsigned long long)__double_as_longlong(m[i]) >> 32) & 0x7fffffffu;
+            const uint32_t vh = (uint32_t)((unsigned long long)__double_as_longlong(v[i]) >> 32) & 0x7fffffffu;
+            const uint32_t mc = mh < 0x7ff00000u ? encode<3, 7, 0x7e>(mh, km, bits & 0xffffu) : 0x7fu;  // (no number)
+            const uint32_t vc = vh < 0x7ff00000u ? encode<2, 15, 0x7b>(vh, kv, bits >> 16) : 0x7fu;
             m4[i] = (unsigned char)(mc | (__double_as_longlong(m[i]) < 0 ? 0x80u : 0u));
             v4[i] = (unsigned char)(v[i] > 0.0 ? max(vc, 1u) : vc);
         }
@@ -250,65 +382,51 @@ __device__ __forceinline__ void step_block(const StepTensor& T, const Rates& r, 
         store4(vo, whole, count, v4);
         if (lane == 0 && count > 0)
         {
-            T.ms[block] = __uint_as_float((uint32_t)(km + 127) << 23);
-            T.vs[block] = __uint_as_float((uint32_t)(kv + 127) << 23);
+            global(T->ms)[block] = __uint_as_float((uint32_t)(km + 127) << 23);
+            global(T->vs)[block] = __uint_as_float((uint32_t)(kv + 127) << 23);
         }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w4[i] = Element<WD>::from_float(nw[i]);
-    store4(reinterpret_cast<W*>(T.w) + i0, whole, count, w4);
-    if (T.copy)
+    store_weights<WD>(T, i0, whole, count, nw);
+}
+
+// The last entry of first_tiles[0..n) that is not behind `tile`, by the whole wavefront; n <= 4096.
+__device__ __forceinline__ uint32_t tensor_of_tile(const uint32_t* first_tiles, uint32_t n, uint32_t tile, int lane)
+{
+    uint32_t base = 0, stride = (n + 63) / 64;
+    if (stride > 1)
     {
-        if (T.copy_dtype == TRIPS_DTYPE_F32)
-            store4(reinterpret_cast<float*>(T.copy) + i0, whole, count, nw);
-        else
-        {
-            const bool bf = T.copy_dtype == TRIPS_DTYPE_BF16;
-            unsigned short c[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                c[i] = bf ? Element<TRIPS_DTYPE_BF16>::from_float(nw[i]) : Element<TRIPS_DTYPE_F16>::from_float(nw[i]);
-            store4(reinterpret_cast<unsigned short*>(T.copy) + i0, whole, count, c);
-        }
+        const uint32_t i = lane * stride;
+        base = ((uint32_t)__popcll(__ballot(i < n && first_tiles[i] <= tile)) - 1u) * stride;
+        const uint32_t j = base + lane;
+        return base + (uint32_t)__popcll(__ballot(lane < (int)stride && j < n && first_tiles[j] <= tile)) - 1u;
     }
+    return (uint32_t)__popcll(__ballot(lane < (int)n && first_tiles[lane] <= tile)) - 1u;
 }
 
 template <int WD, int GD, int BITS>
-__global__ __launch_bounds__(256) void adamw_kernel(const StepTable tab)
+__global__ __launch_bounds__(256) void adamw_kernel(const StepParams p)
 {
-    const float factor = tab.norm ? tab.norm[1] : tab.factor;
-    const bool skip    = !(fabsf(factor) <= FLT_MAX);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (!skip)
+    const float factor = p.norm ? p.norm[1] : p.factor;
+    if (!(fabsf(factor) <= FLT_MAX)) return;  // the step is skipped
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    uint32_t first = 0, behind = 0;
+    Constant<StepEntry> T = (Constant<StepEntry>)p.entries;
+    bool any = false;
+    const uint32_t end = min(p.tiles, (blockIdx.x + 1u) * p.run);
+    for (uint32_t tile = blockIdx.x * p.run; tile < end; ++tile)
     {
-        uint32_t ti = 0, known = ~0u, key = 0;
-        Rates r;
-        for (uint32_t tile = blockIdx.x; tile < tab.tiles; tile += gridDim.x)
+        if (tile >= behind)
         {
-            while (ti + 1 < tab.n && tile >= tab.t[ti + 1].first_tile) ++ti;
-            const StepTensor& T = tab.t[ti];
-            if (ti != known)
-            {
-                const uint32_t t = (uint32_t)*T.step + 1u;
-                r     = rates(tab.o[T.group], t);
-                key   = mix(tab.seed + t * 0x9E3779B9u);
-                known = ti;
-            }
-            const long long block = (long long)(tile - T.first_tile) * (kTileOptim / TRIPS_MOMENT_BLOCK) + wave;
-            if (block * TRIPS_MOMENT_BLOCK < T.n) step_block<WD, GD, BITS>(T, r, factor, key, block, lane);
+            const uint32_t i = (uint32_t)__builtin_amdgcn_readfirstlane((int)tensor_of_tile(p.first_tiles, p.n, tile, lane));
+            T      = (Constant<StepEntry>)p.entries + i;
+            first  = ((Constant<uint32_t>)p.first_tiles)[i];
+            behind = i + 1 < p.n ? ((Constant<uint32_t>)p.first_tiles)[i + 1] : p.tiles;
+            any    = T->eps < kLeastEps;
         }
-    }
-    // The step counts go on when every workgroup has read them: the last one to get here counts. (All that a workgroup does
-    // with the counts ends before its barrier; the ticket orders nothing else.)
-    __shared__ uint32_t s_last;
-    __syncthreads();
-    if (threadIdx.x == 0)
-        s_last = __hip_atomic_fetch_add(tab.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1u ? 1u : 0u;
-    __syncthreads();
-    if (s_last)
-    {
-        if (!skip && threadIdx.x < tab.n) *tab.t[threadIdx.x].step += 1;
-        if (threadIdx.x == 0) *tab.ticket = 0u;
+        const long long block = (long long)(tile - first) * (kTileOptim / TRIPS_MOMENT_BLOCK) + wave;
+        if (block * TRIPS_MOMENT_BLOCK >= T->n) continue;
+        if (any || (block + 1) * TRIPS_MOMENT_BLOCK > T->n || !step_whole<WD, GD, BITS>(T, factor, block, lane))
+            step_any<WD, GD, BITS>(T, factor, block, lane);
     }
 }
 
@@ -318,11 +436,12 @@ struct NormTensor
 {
     const void* g;
     long long n;
-    uint32_t first_tile, dtype;
+    uint32_t dtype;
 };
 struct NormTable
 {
     NormTensor t[kNormTensors];
+    uint32_t first_tiles[kNormTensors];
     uint32_t n, tiles, add;  // add: to the sums of an earlier launch of the call
     double* sums;            // [kNormGroups]
 };
@@ -372,13 +491,18 @@ __device__ __forceinline__ double tile_squares(const NormTensor& T, long long ti
 __global__ __launch_bounds__(256) void grad_squares_kernel(const NormTable tab)
 {
     __shared__ double s[4];
-    double sum  = 0.0;
-    uint32_t ti = 0;
+    double sum = 0.0;
+    uint32_t i = 0, first = 0, behind = 0;
     for (uint32_t tile = blockIdx.x; tile < tab.tiles; tile += gridDim.x)
     {
-        while (ti + 1 < tab.n && tile >= tab.t[ti + 1].first_tile) ++ti;
-        const NormTensor& T    = tab.t[ti];
-        const long long within = tile - T.first_tile;
+        if (tile >= behind)
+        {
+            i      = (uint32_t)__builtin_amdgcn_readfirstlane((int)tensor_of_tile(tab.first_tiles, tab.n, tile, threadIdx.x & 63));
+            first  = tab.first_tiles[i];
+            behind = i + 1 < tab.n ? tab.first_tiles[i + 1] : tab.tiles;
+        }
+        const NormTensor& T    = tab.t[i];
+        const long long within = tile - first;
         if (T.dtype == TRIPS_DTYPE_F32)
             sum += tile_squares<TRIPS_DTYPE_F32>(T, within);
         else if (T.dtype == TRIPS_DTYPE_BF16)
@@ -390,9 +514,8 @@ __global__ __launch_bounds__(256) void grad_squares_kernel(const NormTable tab)
     if (threadIdx.x == 0) tab.sums[blockIdx.x] = tab.add ? tab.sums[blockIdx.x] + sum : sum;
 }
 
-__global__ __launch_bounds__(256) void grad_norm_kernel(const double* sums, int n, float max_norm, float loss_scale, float* out)
+__device__ __forceinline__ void write_norm(const double* sums, int n, float max_norm, float loss_scale, float* out, double* s)
 {
-    __shared__ double s[4];
     double sum = 0.0;
     for (int i = threadIdx.x; i < n; i += 256) sum += sums[i];
     sum = block_sum(sum, s);
@@ -406,12 +529,47 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const double* sums, int 
     }
 }
 
+__global__ __launch_bounds__(256) void grad_norm_kernel(const double* sums, int n, float max_norm, float loss_scale, float* out)
+{
+    __shared__ double s[4];
+    write_norm(sums, n, max_norm, loss_scale, out, s);
+}
+
+// Before a step, one workgroup: the norm of the squares, if they were summed for it; the step counts go on; the step's table.
+__global__ __launch_bounds__(256) void adamw_begin_kernel(const StepTable tab)
+{
+    __shared__ double s[4];
+    if (tab.sums)
+    {
+        write_norm(tab.sums, (int)tab.groups, tab.max_norm, tab.loss_scale, tab.norm, s);
+        __syncthreads();
+    }
+    const uint32_t i = threadIdx.x;
+    if (i >= tab.n) return;
+    // (written by this workgroup, or by another launch)
+    if (tab.norm && !(fabsf(__hip_atomic_load(tab.norm + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)) <= FLT_MAX)) return;
+    const StepTensor& T   = tab.t[i];
+    const StepOptions& o  = tab.o[T.group];
+    const uint32_t t      = (uint32_t)*T.step + 1u;
+    *T.step               = (int32_t)t;
+    StepEntry e;
+    e.w = T.w, e.g = T.g, e.m = T.m, e.v = T.v, e.ms = T.ms, e.vs = T.vs, e.copy = T.copy, e.n = T.n;
+    e.b1 = o.beta1, e.c1 = 1.0 - o.beta1, e.b2 = o.beta2, e.c2 = 1.0 - o.beta2;
+    e.fb1 = (float)e.b1, e.fc1 = (float)e.c1, e.fb2 = (float)e.b2, e.fc2 = (float)e.c2;
+    e.keep = (float)(1.0 - o.lr * o.decay);
+    e.rate = (float)(o.lr / (1.0 - power(o.beta1, t)));
+    e.root = (float)(1.0 / sqrt(1.0 - power(o.beta2, t)));
+    e.eps  = (float)o.eps;
+    e.key  = mix(tab.seed + t * 0x9E3779B9u);
+    e.first_block = T.first_block, e.copy_dtype = T.copy_dtype, e.unused = 0;
+    tab.entries[i]     = e;
+    tab.first_tiles[i] = T.first_tile;
+}
+
 // `get(i)`: the gradients of tensor i of n, as a TripsGradTensor.
 template <typename Get>
-hipError_t launch_norm(const Get& get, int n, float max_norm, float loss_scale, float* out, void* workspace, hipStream_t stream,
-                       Profiler* prof)
+hipError_t launch_squares(const Get& get, int n, double* sums, int& groups, hipStream_t stream)
 {
-    double* sums   = reinterpret_cast<double*>(reinterpret_cast<char*>(workspace) + 256);
     auto tiles_of  = [](long long elements) { return (elements + kNormTile - 1) / kNormTile; };
     long long most = 1;  // tiles of the largest launch: all launches of the call have its grid
     for (int i = 0, used = 0, done = 0; done < n; used = 0)
@@ -422,8 +580,7 @@ hipError_t launch_norm(const Get& get, int n, float max_norm, float loss_scale, 
         most = tiles > most ? tiles : most;
     }
     if (most > 0x7fffffffll) return hipErrorInvalidValue;
-    const int groups = (int)(most < kNormGroups ? most : kNormGroups);
-    ProfScope ps(prof, "grad_norm", stream);
+    groups   = (int)(most < kNormGroups ? most : kNormGroups);
     int done = 0;
     bool add = false;
     do
@@ -434,42 +591,59 @@ hipError_t launch_norm(const Get& get, int n, float max_norm, float loss_scale, 
         {
             const TripsGradTensor T = get(done);
             if (T.n <= 0) continue;
-            tab.t[tab.n++] = NormTensor{T.grads, T.n, tab.tiles, (uint32_t)T.dtype};
+            tab.first_tiles[tab.n] = tab.tiles;
+            tab.t[tab.n++]         = NormTensor{T.grads, T.n, (uint32_t)T.dtype};
             tab.tiles += (uint32_t)tiles_of(T.n);
         }
         hipLaunchKernelGGL(grad_squares_kernel, dim3(groups), dim3(256), 0, stream, tab);
         add = true;
     } while (done < n);
-    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, stream, sums, groups, max_norm, loss_scale, out);
     return hipGetLastError();
 }
 
 template <int WD, int GD>
-void launch_step_of(int bits, const StepTable& tab, int groups, hipStream_t stream)
+void launch_step_of(int bits, const StepParams& p, int groups, hipStream_t stream)
 {
     if (bits == 32)
-        hipLaunchKernelGGL((adamw_kernel<WD, GD, 32>), dim3(groups), dim3(256), 0, stream, tab);
+        hipLaunchKernelGGL((adamw_kernel<WD, GD, 32>), dim3(groups), dim3(256), 0, stream, p);
     else
-        hipLaunchKernelGGL((adamw_kernel<WD, GD, 8>), dim3(groups), dim3(256), 0, stream, tab);
+        hipLaunchKernelGGL((adamw_kernel<WD, GD, 8>), dim3(groups), dim3(256), 0, stream, p);
 }
 template <int WD>
-void launch_step(int gd, int bits, const StepTable& tab, int groups, hipStream_t stream)
+void launch_step(int gd, int bits, const StepParams& p, int groups, hipStream_t stream)
 {
     if (gd == TRIPS_DTYPE_F32)
-        launch_step_of<WD, TRIPS_DTYPE_F32>(bits, tab, groups, stream);
+        launch_step_of<WD, TRIPS_DTYPE_F32>(bits, p, groups, stream);
     else if (gd == TRIPS_DTYPE_BF16)
-        launch_step_of<WD, TRIPS_DTYPE_BF16>(bits, tab, groups, stream);
+        launch_step_of<WD, TRIPS_DTYPE_BF16>(bits, p, groups, stream);
     else
-        launch_step_of<WD, TRIPS_DTYPE_F16>(bits, tab, groups, stream);
+        launch_step_of<WD, TRIPS_DTYPE_F16>(bits, p, groups, stream);
+}
+
+struct StepLayout
+{
+    size_t sums, first_tiles, entries, bytes;
+};
+StepLayout step_layout(int n_tensors)
+{
+    auto up        = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    const size_t n = (size_t)(n_tensors < kStepTensors ? n_tensors : kStepTensors);
+    StepLayout l;
+    l.sums        = 0;
+    l.first_tiles = TRIPS_GRAD_NORM_WORKSPACE_BYTES;
+    l.entries     = l.first_tiles + up(n * sizeof(uint32_t));
+    l.bytes       = l.entries + up(n * sizeof(StepEntry));
+    return l;
 }
 
 int kind_of(const TripsAdamWTensor& t) { return t.weight_dtype * 8 + t.grad_dtype * 2 + (t.state_bits == 8 ? 1 : 0); }
 
-// The tensors of one combination of types, in launches of at most kTensors.
-hipError_t launch_steps(const TripsAdamWTensor* tensors, int n, const TripsAdamWOptions& opt, void* workspace, hipStream_t stream,
-                        Profiler* prof)
+// The tensors of one combination of types in one launch (of at most kStepTensors), their table before it.
+hipError_t launch_steps(const TripsAdamWTensor* tensors, int n, const TripsAdamWOptions& opt, char* workspace, const double* sums, int sum_groups,
+                        hipStream_t stream, Profiler* prof)
 {
-    uint32_t kinds = 0;
+    const StepLayout l = step_layout(n);
+    uint32_t kinds     = 0;
     for (int i = 0; i < n; ++i) kinds |= 1u << kind_of(tensors[i]);
     ProfScope ps(prof, "adamw", stream);
     for (int kind = 0; kind < 32; ++kind)
@@ -479,59 +653,70 @@ hipError_t launch_steps(const TripsAdamWTensor* tensors, int n, const TripsAdamW
         int done       = 0;
         while (done < n)
         {
-            StepTable tab;
-            tab.n = 0, tab.seed = opt.seed, tab.norm = opt.grad_norm, tab.factor = (float)(1.0 / (double)opt.loss_scale);
-            tab.ticket      = reinterpret_cast<uint32_t*>(workspace);
+            StepParams p;
+            p.entries     = reinterpret_cast<const StepEntry*>(workspace + l.entries);
+            p.first_tiles = reinterpret_cast<const uint32_t*>(workspace + l.first_tiles);
+            p.n = 0, p.norm = opt.grad_norm, p.factor = (float)(1.0 / (double)opt.loss_scale);
             long long tiles = 0;
-            int groups      = 0;
-            const TripsAdamWTensor* first = nullptr;
-            for (; done < n && tab.n < kTensors; ++done)
+            while (done < n && p.n < kStepTensors && tiles < (1ll << 31))
             {
-                const TripsAdamWTensor& T = tensors[done];
-                const uint32_t blocks     = (uint32_t)((T.n + TRIPS_MOMENT_BLOCK - 1) / TRIPS_MOMENT_BLOCK);
-                if (kind_of(T) == kind)
+                StepTable tab;
+                tab.n = 0, tab.seed = opt.seed, tab.norm = opt.grad_norm, tab.sums = sums, tab.groups = (uint32_t)sum_groups;
+                tab.max_norm = opt.max_norm, tab.loss_scale = opt.loss_scale;
+                tab.entries     = reinterpret_cast<StepEntry*>(workspace + l.entries) + p.n;
+                tab.first_tiles = reinterpret_cast<uint32_t*>(workspace + l.first_tiles) + p.n;
+                int groups      = 0;
+                for (; done < n && tab.n < kTensors && p.n + tab.n < kStepTensors && tiles < (1ll << 31); ++done)
                 {
-                    first = &T;
-                    const StepOptions o = {T.lr, T.beta1, T.beta2, T.eps, T.weight_decay};
-                    int g = groups - 1;
-                    while (g >= 0 && !(tab.o[g].lr == o.lr && tab.o[g].beta1 == o.beta1 && tab.o[g].beta2 == o.beta2 &&
-                                       tab.o[g].eps == o.eps && tab.o[g].decay == o.decay))
-                        --g;
-                    if (g < 0)
+                    const TripsAdamWTensor& T = tensors[done];
+                    const uint32_t blocks     = (uint32_t)((T.n + TRIPS_MOMENT_BLOCK - 1) / TRIPS_MOMENT_BLOCK);
+                    if (kind_of(T) == kind)
                     {
-                        if (groups == kGroups) break;
-                        g        = groups++;
-                        tab.o[g] = o;
+                        const StepOptions o = {T.lr, T.beta1, T.beta2, T.eps, T.weight_decay};
+                        int g = groups - 1;
+                        while (g >= 0 && !(tab.o[g].lr == o.lr && tab.o[g].beta1 == o.beta1 && tab.o[g].beta2 == o.beta2 &&
+                                           tab.o[g].eps == o.eps && tab.o[g].decay == o.decay))
+                            --g;
+                        if (g < 0)
+                        {
+                            if (groups == kGroups) break;
+                            g        = groups++;
+                            tab.o[g] = o;
+                        }
+                        StepTensor& S = tab.t[tab.n++];
+                        S.w = T.weights, S.g = T.grads, S.m = T.first_moment, S.v = T.second_moment, S.ms = T.first_scale;
+                        S.vs = T.second_scale, S.copy = T.copy, S.step = T.step, S.n = T.n;
+                        S.first_tile = (uint32_t)tiles, S.first_block = block;
+                        S.group = (uint8_t)g, S.copy_dtype = (uint8_t)T.copy_dtype;
+                        tiles += (T.n + kTileOptim - 1) / kTileOptim;
                     }
-                    StepTensor& S = tab.t[tab.n++];
-                    S.w = T.weights, S.g = T.grads, S.m = T.first_moment, S.v = T.second_moment, S.ms = T.first_scale;
-                    S.vs = T.second_scale, S.copy = T.copy, S.step = T.step, S.n = T.n;
-                    S.first_tile = (uint32_t)tiles, S.first_block = block;
-                    S.group = (uint8_t)g, S.copy_dtype = (uint8_t)T.copy_dtype;
-                    tiles += (T.n + kTileOptim - 1) / kTileOptim;
+                    block += blocks;
                 }
-                block += blocks;
+                if (tab.n == 0) continue;
+                hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(256), 0, stream, tab);
+                sums = nullptr;  // (the first one has made the norm)
+                p.n += tab.n;
             }
-            if (tab.n == 0) continue;
-            if (tiles > 0x7fffffffll) return hipErrorInvalidValue;
-            tab.tiles   = (uint32_t)tiles;
-            const int g = tiles < 1 ? 1 : tiles > kStepGroups ? kStepGroups : (int)tiles;
-            if (first->weight_dtype == TRIPS_DTYPE_F32)
-                launch_step<TRIPS_DTYPE_F32>(first->grad_dtype, first->state_bits, tab, g, stream);
-            else if (first->weight_dtype == TRIPS_DTYPE_BF16)
-                launch_step<TRIPS_DTYPE_BF16>(first->grad_dtype, first->state_bits, tab, g, stream);
+            if (tiles == 0) continue;
+            p.tiles     = (uint32_t)tiles;
+            p.run       = tiles > kStepGroups ? kStepRun : 1u;
+            const int g = (int)((tiles + p.run - 1) / p.run);
+            const int wd = kind / 8, gd = kind / 2 % 4, bits = kind & 1 ? 8 : 32;
+            if (wd == TRIPS_DTYPE_F32)
+                launch_step<TRIPS_DTYPE_F32>(gd, bits, p, g, stream);
+            else if (wd == TRIPS_DTYPE_BF16)
+                launch_step<TRIPS_DTYPE_BF16>(gd, bits, p, g, stream);
             else
-                launch_step<TRIPS_DTYPE_F16>(first->grad_dtype, first->state_bits, tab, g, stream);
+                launch_step<TRIPS_DTYPE_F16>(gd, bits, p, g, stream);
         }
     }
     return hipGetLastError();
 }
 
-int check_workspace(const void* workspace, size_t bytes)
+int check_workspace(const void* workspace, size_t bytes, size_t need)
 {
     if (!workspace || !aligned(workspace, 256)) return set_error(TRIPS_ERR_INVALID_ARG, "workspace must be a 256-byte aligned device pointer");
-    if (bytes < TRIPS_ADAMW_WORKSPACE_BYTES)
-        return set_error(TRIPS_ERR_WORKSPACE_SMALL, "workspace has %zu bytes, %d needed", bytes, TRIPS_ADAMW_WORKSPACE_BYTES);
+    if (bytes < need) return set_error(TRIPS_ERR_WORKSPACE_SMALL, "workspace has %zu bytes, %zu needed", bytes, need);
     return TRIPS_OK;
 }
 
@@ -542,7 +727,7 @@ int check_norm(float max_norm, float loss_scale)
     return TRIPS_OK;
 }
 
-constexpr int64_t kMostElements = (int64_t)1 << 38;  // of a tensor: tiles are counted in 32 bits
+constexpr int64_t kMostElements = (int64_t)1 << 38;  // of a tensor: a launch counts less than 2^32 tiles
 }  // namespace
 }  // namespace trips
 
@@ -551,13 +736,13 @@ using namespace trips;
 extern "C" {
 
 int trips_grad_norm(TripsCtx* ctx, const TripsGradTensor* tensors, int n_tensors, float max_norm, float loss_scale,
-                    float* grad_norm, void* workspace, size_t workspace_bytes, void* stream)
+                    float* grad_norm, void* workspace, size_t workspace_bytes, void* stream_)
 {
     if (!ctx) return set_error(TRIPS_ERR_INVALID_ARG, "ctx is NULL");
     if (n_tensors < 0 || (n_tensors > 0 && !tensors)) return set_error(TRIPS_ERR_INVALID_ARG, "tensors");
     if (!grad_norm || !aligned(grad_norm, 4)) return set_error(TRIPS_ERR_INVALID_ARG, "grad_norm must be a device pointer to two floats");
     if (int e = check_norm(max_norm, loss_scale)) return e;
-    if (int e = check_workspace(workspace, workspace_bytes)) return e;
+    if (int e = check_workspace(workspace, workspace_bytes, TRIPS_GRAD_NORM_WORKSPACE_BYTES)) return e;
     for (int i = 0; i < n_tensors; ++i)
     {
         const TripsGradTensor& t = tensors[i];
@@ -567,9 +752,25 @@ int trips_grad_norm(TripsCtx* ctx, const TripsGradTensor* tensors, int n_tensors
     }
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_error(scope.error, "hipSetDevice");
-    hipError_t e = launch_norm([&](int i) { return tensors[i]; }, n_tensors, max_norm, loss_scale, grad_norm, workspace,
-                               reinterpret_cast<hipStream_t>(stream), profiler(ctx));
+    hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    ProfScope ps(profiler(ctx), "grad_norm", stream);
+    double* sums = reinterpret_cast<double*>(workspace);
+    int groups   = 0;
+    hipError_t e = launch_squares([&](int i) { return tensors[i]; }, n_tensors, sums, groups, stream);
+    if (e == hipSuccess)
+    {
+        hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, stream, sums, groups, max_norm, loss_scale, grad_norm);
+        e = hipGetLastError();
+    }
     return e == hipSuccess ? TRIPS_OK : hip_error(e, "norm launch");
+}
+
+int trips_adamw_workspace_size(int n_tensors, size_t* bytes)
+{
+    if (!bytes) return set_error(TRIPS_ERR_INVALID_ARG, "bytes is NULL");
+    if (n_tensors < 0) return set_error(TRIPS_ERR_INVALID_ARG, "n_tensors = %d", n_tensors);
+    *bytes = step_layout(n_tensors).bytes;
+    return TRIPS_OK;
 }
 
 int trips_adamw_step(TripsCtx* ctx, const TripsAdamWTensor* tensors, int n_tensors, const TripsAdamWOptions* options,
@@ -584,7 +785,7 @@ int trips_adamw_step(TripsCtx* ctx, const TripsAdamWTensor* tensors, int n_tenso
     if (!aligned(options->grad_norm, 4)) return set_error(TRIPS_ERR_INVALID_ARG, "grad_norm is not aligned");
     if (int e = check_norm(options->max_norm, options->loss_scale)) return e;
     if (options->max_norm > 0.f && !options->grad_norm) return set_error(TRIPS_ERR_INVALID_ARG, "max_norm without grad_norm");
-    if (int e = check_workspace(workspace, workspace_bytes)) return e;
+    if (int e = check_workspace(workspace, workspace_bytes, step_layout(n_tensors).bytes)) return e;
     for (int i = 0; i < n_tensors; ++i)
     {
         const TripsAdamWTensor& t = tensors[i];
@@ -611,13 +812,18 @@ int trips_adamw_step(TripsCtx* ctx, const TripsAdamWTensor* tensors, int n_tenso
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_error(scope.error, "hipSetDevice");
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+    if (n_tensors == 0) return TRIPS_OK;
+    double* sums = nullptr;
+    int groups   = 0;
     if (options->compute_norm)
     {
+        ProfScope ps(profiler(ctx), "grad_norm", stream);
+        sums         = reinterpret_cast<double*>(workspace);
         auto grads   = [&](int i) { return TripsGradTensor{tensors[i].grads, tensors[i].n, tensors[i].grad_dtype}; };
-        hipError_t e = launch_norm(grads, n_tensors, options->max_norm, options->loss_scale, options->grad_norm, workspace, stream, profiler(ctx));
+        hipError_t e = launch_squares(grads, n_tensors, sums, groups, stream);
         if (e != hipSuccess) return hip_error(e, "norm launch");
     }
-    hipError_t e = launch_steps(tensors, n_tensors, *options, workspace, stream, profiler(ctx));
+    hipError_t e = launch_steps(tensors, n_tensors, *options, reinterpret_cast<char*>(workspace), sums, groups, stream, profiler(ctx));
     return e == hipSuccess ? TRIPS_OK : hip_error(e, "adamw launch");
 }
 

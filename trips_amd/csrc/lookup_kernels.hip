@@ -3,6 +3,7 @@
 // All are bound by memory: the lookup and the gradient by scattered requests (of 4 bytes a channel in the columns layout,
 // of whole rows in the rows layout), the order by the passes of its sort.
 #include <algorithm>
+#include <type_traits>
 
 #include "abi_common.h"
 
@@ -15,7 +16,7 @@ namespace trips
 namespace
 {
 constexpr int64_t kMostEntries = 0x7ffffffell;  // texels or points: positions and T + 1 starts in 32 bits
-constexpr int kMostChannels    = 1 << 20;  // a grid's y holds 65535 groups of 16
+constexpr int kMostChannels    = 1 << 17;  // lanes of 16 bytes that a grid's y holds
 
 template <bool I32>
 __device__ __forceinline__ long long load_index(const void* index, long long i)
@@ -32,19 +33,39 @@ __device__ __forceinline__ long long load_index(bool i32, const void* index, lon
 
 struct LookupParams
 {
-    const void* table;   // or d_values
-    const void* index;   // or NULL
-    void* values;        // or d_table
-    const int32_t* order;
-    const int32_t* starts;
+    const void* table;
+    const void* index;
+    void* values;
     long long texels, points, table_stride, values_stride;
-    int channels, i32, accumulate;
+    int channels, i32, lanes_log2;
     float scale;
 };
 
+// ---- columns to rows ----
+
+// [channels, n] to [n, row] with 16 bytes (8 where two or four channels of 16 bits make no more) a lane: what the kernels below
+// gather is then one request of a point, not one per channel. Bound by memory, read and written once.
+// (row: channels rounded up to whole lanes; the elements added are zeros.)
+template <int D, int V>
+__global__ __launch_bounds__(256) void rows_kernel(const void* columns, void* rows, long long n, long long stride, int channels, int row,
+                                                   uint32_t* clear)
+{
+    using T           = typename Element<D>::type;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (clear && i == 0 && blockIdx.y == 0) *clear = 0u;
+    if (i >= n) return;
+    const int c0   = blockIdx.y * V;
+    const T* from  = reinterpret_cast<const T*>(columns) + i;
+    typename Pack<T, V>::type x;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = c0 + e < channels ? from[(c0 + e) * stride] : T(0);
+    *reinterpret_cast<typename Pack<T, V>::type*>(reinterpret_cast<T*>(rows) + i * row + c0) = x;
+}
+
 // ---- lookup ----
 
-// One point a lane; channels in groups of kColumnGroup along grid.y.
+// One point a lane; channels in groups of kColumnGroup along grid.y. For one channel, and for so few points that turning the
+// table's columns to rows would cost more than it saves.
 constexpr int kColumnGroup = 16;
 template <int D>
 __global__ __launch_bounds__(256) void lookup_columns_kernel(const LookupParams p)
@@ -63,33 +84,67 @@ __global__ __launch_bounds__(256) void lookup_columns_kernel(const LookupParams 
     }
 }
 
-// LANES lanes a point, 16 bytes a lane and step.
-template <int D>
-__global__ __launch_bounds__(256) void lookup_rows_kernel(const LookupParams p, int lanes_log2)
+// V elements a lane, 1 << lanes_log2 lanes a point. OUT_COLUMNS: the values are columns (and the table's rows whole lanes wide).
+template <int D, int V, bool OUT_COLUMNS>
+__global__ __launch_bounds__(256) void lookup_rows_kernel(const LookupParams p)
 {
-    using E         = Element<D>;
-    using T         = typename E::type;
-    constexpr int V = 16 / sizeof(T);
-    const int lanes = 1 << lanes_log2, j = threadIdx.x & (lanes - 1);
-    const long long step = (long long)gridDim.x * (256 >> lanes_log2);
-    for (long long i = (long long)blockIdx.x * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2); i < p.points; i += step)
+    using E = Element<D>;
+    using T = typename E::type;
+    const int lanes = 1 << p.lanes_log2, j = threadIdx.x & (lanes - 1), at_once = 256 >> p.lanes_log2;
+    const T* table       = reinterpret_cast<const T*>(p.table);
+    T* values            = reinterpret_cast<T*>(p.values);
+    constexpr int POINTS = 4;  // whose rows a lane has on the way at a time
+    for (long long base = (long long)blockIdx.x * at_once * POINTS; base < p.points; base += (long long)gridDim.x * at_once * POINTS)
     {
-        const long long t = load_index(p.i32 != 0, p.index, i);
-        const bool in     = t >= 0 && t < p.texels;
-        const T* from     = reinterpret_cast<const T*>(p.table) + (in ? t : 0) * p.table_stride;
-        T* to             = reinterpret_cast<T*>(p.values) + i * p.values_stride;
+        long long t[POINTS];
+#pragma unroll
+        for (int q = 0; q < POINTS; ++q)
+        {
+            const long long i = base + q * at_once + (threadIdx.x >> p.lanes_log2);
+            t[q] = i < p.points ? load_index(p.i32 != 0, p.index, i) : -1;
+            if (t[q] >= p.texels) t[q] = -1;
+        }
         for (int c = j * V; c < p.channels; c += lanes * V)
         {
-            if (c + V <= p.channels)
-            {
-                typename Pack<T, V>::type x = {};
-                if (in) x = *reinterpret_cast<const typename Pack<T, V>::type*>(from + c);
+            const int count = OUT_COLUMNS ? V : min(V, p.channels - c);
+            typename Pack<T, V>::type x[POINTS];
 #pragma unroll
-                for (int e = 0; e < V; ++e) x[e] = in ? E::from_float(E::to_float(x[e]) * p.scale) : T(0);
-                *reinterpret_cast<typename Pack<T, V>::type*>(to + c) = x;
+            for (int q = 0; q < POINTS; ++q)
+            {
+                x[q] = typename Pack<T, V>::type{};
+                if (t[q] < 0) continue;
+                const T* from = table + t[q] * p.table_stride + c;
+                if (count == V)
+                    x[q] = *reinterpret_cast<const typename Pack<T, V>::type*>(from);
+                else
+                {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (e < count) x[q][e] = from[e];
+                }
             }
-            else
-                for (int e = c; e < p.channels; ++e) to[e] = in ? E::from_float(E::to_float(from[e]) * p.scale) : T(0);
+#pragma unroll
+            for (int q = 0; q < POINTS; ++q)
+            {
+                const long long i = base + q * at_once + (threadIdx.x >> p.lanes_log2);
+                if (i >= p.points) continue;
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[q][e] = t[q] >= 0 ? E::from_float(E::to_float(x[q][e]) * p.scale) : T(0);
+                if constexpr (OUT_COLUMNS)
+                {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (c + e < p.channels) values[(c + e) * p.values_stride + i] = x[q][e];
+                }
+                else if (count == V)
+                    *reinterpret_cast<typename Pack<T, V>::type*>(values + i * p.values_stride + c) = x[q];
+                else
+                {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (e < count) values[i * p.values_stride + c + e] = x[q][e];
+                }
+            }
         }
     }
 }
@@ -249,122 +304,331 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortPa
     }
 }
 
-// starts[t] = the first of the sorted keys that is t or more
+// The first of n ascending numbers that is `x` or more, by the whole wavefront: 64 probes a round.
+template <typename T>
+__device__ __forceinline__ uint32_t lower_bound(const T* a, uint32_t n, uint32_t x, int lane)
+{
+    uint32_t lo = 0, len = n;  // in [lo, lo + len]
+    while (len > 0)
+    {
+        const uint32_t step = len / 64 + 1, at = (uint32_t)lane * step;
+        const bool less     = at < len && (uint32_t)a[lo + at] < x;
+        const uint32_t k    = (uint32_t)__popcll(__ballot(less));  // probes below x, the first ones
+        if (k == 0) return lo;
+        const uint32_t from = (k - 1) * step + 1;
+        len = min(k * step, len) - from;
+        lo += from;
+    }
+    return lo;
+}
+
+// starts[t] = the first of the sorted keys that is t or more. A wavefront finds those of its first and its last texel with all
+// lanes; each lane's search goes on between them.
+constexpr int kStartsItems = 4;  // texels of a lane, 64 apart
 __global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t texels, int32_t* starts)
 {
-    const uint32_t t = blockIdx.x * 256u + threadIdx.x;
-    if (t > texels) return;
-    uint32_t lo = 0, hi = n;
-    while (lo < hi)
+    const int lane       = threadIdx.x & 63;
+    const uint32_t first = (blockIdx.x * 4u + (threadIdx.x >> 6)) * (64u * kStartsItems);
+    if (first > texels) return;
+    const uint32_t last = min(texels, first + 64u * kStartsItems - 1u);
+    const uint32_t from = lower_bound(keys, n, first, lane), to = from + lower_bound(keys + from, n - from, last, lane);
+#pragma unroll
+    for (int q = 0; q < kStartsItems; ++q)
     {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (keys[mid] < t)
-            lo = mid + 1;
-        else
-            hi = mid;
+        const uint32_t t = first + q * 64u + lane;
+        if (t > texels) return;
+        uint32_t lo = from, hi = to;
+        while (lo < hi)
+        {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (keys[mid] < t)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        starts[t] = (int32_t)lo;
     }
-    starts[t] = (int32_t)lo;
 }
 
 // ---- the gradient ----
+//
+// The rows of a texel's points are gathered in the order of the plan and added up by the lanes that hold the texel's row. Texels
+// with more than kShort points are listed and left to a second kernel, a workgroup each, and what lies in between is summed
+// beforehand in tiles of the plan's positions that one texel fills, so that no entry of a table, however many points refer to
+// it, is left to one wavefront. Which points are added to which sum first goes by the plan and the sizes alone.
 
-__device__ __forceinline__ void segment(const LookupParams& p, long long t, uint32_t& from, uint32_t& to)
+constexpr int kShort      = 32;
+constexpr int kLongGroups = 2048;  // workgroups for the listed texels
+
+struct GradParams
+{
+    const void* rows;  // gradients [points, row]
+    void* d_table;
+    const int32_t* order;
+    const int32_t* starts;
+    float* tiles;     // [points / tile, padded] sums of the tiles that one texel fills (zeros for the others)
+    uint32_t* listed;  // texels for the second kernel: how many, then 63 words on, which
+    long long texels, table_stride, row;
+    uint32_t points, tile, capacity;
+    int channels, padded, lanes_log2, accumulate;
+    float scale;
+};
+constexpr int kListHead = 64;
+
+__device__ __forceinline__ void segment(const GradParams& p, long long t, uint32_t& from, uint32_t& to)
 {
     // (a plan of another scene must not lead outside)
-    from = min((uint32_t)p.starts[t], (uint32_t)p.points);
-    to   = max(from, min((uint32_t)p.starts[t + 1], (uint32_t)p.points));
+    from = min((uint32_t)p.starts[t], p.points);
+    to   = max(from, min((uint32_t)p.starts[t + 1], p.points));
 }
 
-template <int D>
-__global__ __launch_bounds__(256) void lookup_backward_columns_kernel(const LookupParams p)
+// sum += the rows of the points order[k], k = from, from + step .. below to; V channels from c on
+template <int D, int V>
+__device__ __forceinline__ void add_rows(const GradParams& p, uint32_t from, uint32_t to, uint32_t step, int c, int count, float (&sum)[V])
+{
+    using E       = Element<D>;
+    using T       = typename E::type;
+    const T* rows = reinterpret_cast<const T*>(p.rows) + c;
+    constexpr int AHEAD = 4;
+    for (uint32_t k = from; k < to; k += AHEAD * step)
+    {
+        uint32_t i[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) i[q] = k + q * step < to ? (uint32_t)p.order[k + q * step] : ~0u;
+        typename Pack<T, V>::type x[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q)
+        {
+            x[q] = typename Pack<T, V>::type{};
+            if (i[q] >= p.points) continue;
+            const T* row = rows + (long long)i[q] * p.row;
+            if (count == V)
+                x[q] = *reinterpret_cast<const typename Pack<T, V>::type*>(row);
+            else
+            {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e < count) x[q][e] = row[e];
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q)
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum[e] += E::to_float(x[q][e]);
+    }
+}
+
+template <int D, int V, bool OUT_COLUMNS>
+__device__ __forceinline__ void store_sum(const GradParams& p, long long t, int c, int count, const float (&sum)[V])
 {
     using E = Element<D>;
     using T = typename E::type;
-    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (t >= p.texels) return;
-    uint32_t from, to;
-    segment(p, t, from, to);
-    const int c0 = blockIdx.y * kColumnGroup;
-    float sum[kColumnGroup];
-#pragma unroll
-    for (int c = 0; c < kColumnGroup; ++c) sum[c] = 0.f;
-    for (uint32_t k = from; k < to; ++k)
+    T* to             = reinterpret_cast<T*>(p.d_table) + (OUT_COLUMNS ? c * p.table_stride + t : t * p.table_stride + c);
+    const long long s = OUT_COLUMNS ? p.table_stride : 1;
+    if (!OUT_COLUMNS && count == V && !p.accumulate)
     {
-        const uint32_t i = (uint32_t)p.order[k];
-        if (i >= (uint32_t)p.points) continue;
+        typename Pack<T, V>::type x;
 #pragma unroll
-        for (int c = 0; c < kColumnGroup; ++c)
-            if (c0 + c < p.channels) sum[c] += E::to_float(reinterpret_cast<const T*>(p.table)[(c0 + c) * p.values_stride + i]);
+        for (int e = 0; e < V; ++e) x[e] = E::from_float(p.scale * sum[e]);
+        *reinterpret_cast<typename Pack<T, V>::type*>(to) = x;
+        return;
     }
 #pragma unroll
-    for (int c = 0; c < kColumnGroup; ++c)
-    {
-        if (c0 + c >= p.channels) break;
-        T* to_ = reinterpret_cast<T*>(p.values) + (c0 + c) * p.table_stride + t;
-        if (p.accumulate)
-        {
-            if (from < to) *to_ = E::from_float(E::to_float(*to_) + p.scale * sum[c]);
-        }
-        else
-            *to_ = E::from_float(p.scale * sum[c]);
-    }
+    for (int e = 0; e < V; ++e)
+        if (c + e < p.channels) to[e * s] = E::from_float(p.accumulate ? E::to_float(to[e * s]) + p.scale * sum[e] : p.scale * sum[e]);
 }
 
-template <int D>
-__global__ __launch_bounds__(256) void lookup_backward_rows_kernel(const LookupParams p, int lanes_log2)
+// OUT_COLUMNS: the table's gradient is columns, and the rows were made of columns (whole lanes wide).
+template <int D, int V, bool OUT_COLUMNS>
+__global__ __launch_bounds__(256) void lookup_backward_kernel(const GradParams p)
 {
-    using E         = Element<D>;
-    using T         = typename E::type;
-    constexpr int V = 16 / sizeof(T);
-    const int lanes = 1 << lanes_log2, j = threadIdx.x & (lanes - 1);
-    const long long step = (long long)gridDim.x * (256 >> lanes_log2);
-    for (long long t = (long long)blockIdx.x * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2); t < p.texels; t += step)
+    const int lanes = 1 << p.lanes_log2, j = threadIdx.x & (lanes - 1), at_once = 256 >> p.lanes_log2, lane = threadIdx.x & 63;
+    for (long long base = (long long)blockIdx.x * at_once; base < p.texels; base += (long long)gridDim.x * at_once)
     {
-        uint32_t from, to;
-        segment(p, t, from, to);
-        if (p.accumulate && from == to) continue;
-        T* out = reinterpret_cast<T*>(p.values) + t * p.table_stride;
+        const long long t = base + (threadIdx.x >> p.lanes_log2);
+        uint32_t from = 0, to = 0;
+        if (t < p.texels) segment(p, t, from, to);
+        const bool later = to - from > kShort;
+        const unsigned long long mask = __ballot(later && j == 0);
+        if (mask)
+        {
+            uint32_t at = 0;
+            if (lane == 0) at = atomicAdd(p.listed, (uint32_t)__popcll(mask));
+            at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(mask & ((1ull << lane) - 1ull));
+            if (later && j == 0 && at < p.capacity) p.listed[kListHead + at] = (uint32_t)t;
+        }
+        if (t >= p.texels || later || (p.accumulate && from == to)) continue;
         for (int c = j * V; c < p.channels; c += lanes * V)
         {
-            const int count = min(V, p.channels - c);
+            const int count = OUT_COLUMNS ? V : min(V, p.channels - c);
             float sum[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) sum[e] = 0.f;
-            for (uint32_t k = from; k < to; ++k)
-            {
-                const uint32_t i = (uint32_t)p.order[k];
-                if (i >= (uint32_t)p.points) continue;
-                const T* row = reinterpret_cast<const T*>(p.table) + (long long)i * p.values_stride + c;
-                if (count == V)
-                {
-                    const auto x = *reinterpret_cast<const typename Pack<T, V>::type*>(row);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) sum[e] += E::to_float(x[e]);
-                }
-                else
-                {
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (e < count) sum[e] += E::to_float(row[e]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (e < count) out[c + e] = E::from_float(p.accumulate ? E::to_float(out[c + e]) + p.scale * sum[e] : p.scale * sum[e]);
+            add_rows<D, V>(p, from, to, 1, c, count, sum);
+            store_sum<D, V, OUT_COLUMNS>(p, t, c, count, sum);
         }
+    }
+}
+
+// The sums of the threads of one column (threadIdx.x >> lanes_log2 counts them), in their order; valid in the first `lanes` threads.
+template <int V>
+__device__ __forceinline__ void add_threads(float (&sum)[V], float* s, int lanes_log2)
+{
+    const int lanes = 1 << lanes_log2;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e * 256 + threadIdx.x] = sum[e];
+    __syncthreads();
+    for (int half = 128; half >= lanes; half >>= 1)
+    {
+        if ((int)threadIdx.x < half)
+        {
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e * 256 + threadIdx.x] += s[e * 256 + threadIdx.x + half];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[e] = s[e * 256 + threadIdx.x];
+}
+
+// One workgroup a tile of the plan's positions (and a group of lanes' channels). Clears the list's length as well.
+template <int D, int V, bool OUT_COLUMNS>
+__global__ __launch_bounds__(256) void lookup_tiles_kernel(const GradParams p)
+{
+    __shared__ float s[V * 256];
+    __shared__ uint32_t s_in;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.listed = 0u;
+    const uint32_t from = blockIdx.x * p.tile, to = from + p.tile;
+    if (to > p.points) return;  // (the last positions, and the workgroup of a plan with no whole tile)
+    if (threadIdx.x < 64)
+    {
+        // the last texel that begins at `from` or before, and whether it ends behind the tile
+        const uint32_t t = lower_bound(reinterpret_cast<const uint32_t*>(p.starts), (uint32_t)p.texels + 1u, from + 1u, threadIdx.x);
+        if (threadIdx.x == 0) s_in = t > 0 && t <= (uint32_t)p.texels && (uint32_t)p.starts[t] >= to ? 1u : 0u;
+    }
+    __syncthreads();
+    const int lanes = 1 << p.lanes_log2, j = threadIdx.x & (lanes - 1), r = threadIdx.x >> p.lanes_log2;
+    const int c     = (blockIdx.y * lanes + j) * V;
+    float sum[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[e] = 0.f;
+    if (s_in && c < p.channels) add_rows<D, V>(p, from + r, to, 256 >> p.lanes_log2, c, OUT_COLUMNS ? V : min(V, p.channels - c), sum);
+    add_threads(sum, s, p.lanes_log2);
+    if ((int)threadIdx.x < lanes && c < p.padded)
+    {
+#pragma unroll
+        for (int e = 0; e < V; ++e) p.tiles[(long long)blockIdx.x * p.padded + c + e] = sum[e];
+    }
+}
+
+// One workgroup a listed texel (and a group of lanes' channels): the points before its first whole tile, those behind its last
+// one, and the tiles.
+template <int D, int V, bool OUT_COLUMNS>
+__global__ __launch_bounds__(256) void lookup_backward_long_kernel(const GradParams p)
+{
+    __shared__ float s[V * 256];
+    const int lanes = 1 << p.lanes_log2, j = threadIdx.x & (lanes - 1), r = threadIdx.x >> p.lanes_log2;
+    const uint32_t rows = 256u >> p.lanes_log2;
+    const int c         = (blockIdx.y * lanes + j) * V;
+    const int count     = OUT_COLUMNS ? V : min(V, p.channels - c);
+    const uint32_t n    = min(*p.listed, p.capacity);
+    for (uint32_t at = blockIdx.x; at < n; at += gridDim.x)
+    {
+        const long long t = p.listed[kListHead + at];
+        uint32_t from, to;
+        segment(p, t, from, to);
+        const uint32_t first = (from + p.tile - 1) / p.tile, last = to / p.tile;
+        float sum[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] = 0.f;
+        if (c < p.channels)
+        {
+            if (first < last)
+            {
+                add_rows<D, V>(p, from + r, first * p.tile, rows, c, count, sum);
+                for (uint32_t k = first + r; k < last; k += rows)
+                {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) sum[e] += p.tiles[(long long)k * p.padded + c + e];
+                }
+                add_rows<D, V>(p, last * p.tile + r, to, rows, c, count, sum);
+            }
+            else
+                add_rows<D, V>(p, from + r, to, rows, c, count, sum);
+        }
+        add_threads(sum, s, p.lanes_log2);
+        if ((int)threadIdx.x < lanes && c < p.channels) store_sum<D, V, OUT_COLUMNS>(p, t, c, count, sum);
     }
 }
 
 // ---- host ----
 
 constexpr long long kMostRowGroups = 1 << 20;  // a launch has less than 2^32 threads
+constexpr size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-int lanes_log2_of(int channels, int dtype)
+// How a row of channels is spread over lanes: 16 bytes a lane, or 8 where all of a row in columns fits them.
+struct RowShape
 {
-    const int v = 16 / dtype_bytes(dtype), chunks = (channels + v - 1) / v;
-    int l = 0;
-    while ((1 << l) < chunks && l < 6) ++l;
-    return l;
+    int lane_bytes, lanes_log2, groups, padded;  // groups of lanes a row; padded: channels in whole lanes
+};
+RowShape row_shape(const TripsLookupDesc& d)
+{
+    const int size = dtype_bytes(d.dtype);
+    RowShape r;
+    r.lane_bytes    = d.layout == TRIPS_TABLE_COLUMNS && d.num_channels * size <= 8 ? 8 : 16;
+    const int v     = r.lane_bytes / size, chunks = (d.num_channels + v - 1) / v;
+    r.lanes_log2    = 0;
+    while ((1 << r.lanes_log2) < chunks && r.lanes_log2 < 6) ++r.lanes_log2;
+    r.groups = (chunks + (1 << r.lanes_log2) - 1) >> r.lanes_log2;
+    r.padded = chunks * v;
+    return r;
+}
+
+// f(type, elements of a lane, whether columns) with all three as constants
+template <typename F>
+void with_types(int dtype, int lane_bytes, bool columns, const F& f)
+{
+    auto with_columns = [&](auto d, auto v)
+    {
+        if (columns)
+            f(d, v, std::true_type{});
+        else
+            f(d, v, std::false_type{});
+    };
+    auto with_lane = [&](auto d)
+    {
+        constexpr int size = decltype(d)::value == TRIPS_DTYPE_F32 ? 4 : 2;
+        if (lane_bytes == 8)
+            f(d, std::integral_constant<int, 8 / size>{}, std::true_type{});  // (columns alone)
+        else
+            with_columns(d, std::integral_constant<int, 16 / size>{});
+    };
+    if (dtype == TRIPS_DTYPE_F32)
+        with_lane(std::integral_constant<int, TRIPS_DTYPE_F32>{});
+    else if (dtype == TRIPS_DTYPE_BF16)
+        with_lane(std::integral_constant<int, TRIPS_DTYPE_BF16>{});
+    else
+        with_lane(std::integral_constant<int, TRIPS_DTYPE_F16>{});
+}
+
+// Columns [channels, n] to rows [n, padded].
+void launch_rows(const TripsLookupDesc& d, const RowShape& r, const void* columns, void* rows, int64_t n, int64_t stride, hipStream_t stream)
+{
+    const int v = r.lane_bytes / dtype_bytes(d.dtype);
+    const dim3 grid((unsigned)((n + 255) / 256), (unsigned)(r.padded / v));
+    with_types(d.dtype, r.lane_bytes, true, [&](auto D, auto V, auto) {
+        hipLaunchKernelGGL((rows_kernel<decltype(D)::value, decltype(V)::value>), grid, dim3(256), 0, stream, columns, rows, n, stride,
+                           d.num_channels, r.padded, (uint32_t*)nullptr);
+    });
+}
+
+// Whether a lookup in columns turns the table to rows first. Scattered requests are what a lookup costs, one a point and channel
+// in columns, one a point in rows (6M points and four channels of 1.5M texels in no order: 350 us and 88); turning the table
+// costs its bytes twice, as much as about an eighth of a request a texel.
+bool turns_table(const TripsLookupDesc& d)
+{
+    return d.layout == TRIPS_TABLE_COLUMNS && d.num_channels > 1 && d.num_points >= d.num_texels / 8;
 }
 
 int key_bits(int64_t texels)
@@ -380,7 +644,7 @@ struct PlanLayout
 };
 PlanLayout plan_layout(int64_t points)
 {
-    auto up            = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    auto up            = up256;
     const size_t tiles = (size_t)((points + kSortTile - 1) / kSortTile);
     PlanLayout l;
     size_t o  = 0;
@@ -417,7 +681,7 @@ hipError_t launch_plan(int64_t texels, int64_t points, const void* index, int in
         hipLaunchKernelGGL(sort_scatter_kernel, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
         shift += p.bits;
     }
-    hipLaunchKernelGGL(starts_kernel, dim3((unsigned)(texels / 256 + 1)), dim3(256), 0, stream, p.keys_out, (uint32_t)points,
+    hipLaunchKernelGGL(starts_kernel, dim3((unsigned)(texels / (256 * kStartsItems) + 1)), dim3(256), 0, stream, p.keys_out, (uint32_t)points,
                        (uint32_t)texels, starts);
     return hipGetLastError();
 }
@@ -435,6 +699,14 @@ int check_lookup(const TripsLookupDesc* d)
     return TRIPS_OK;
 }
 
+int check_workspace(const void* workspace, size_t bytes, size_t need)
+{
+    if (need == 0) return TRIPS_OK;
+    if (!workspace || !aligned(workspace, 256)) return set_error(TRIPS_ERR_INVALID_ARG, "workspace must be a 256-byte aligned device pointer");
+    if (bytes < need) return set_error(TRIPS_ERR_WORKSPACE_SMALL, "workspace has %zu bytes, %zu needed", bytes, need);
+    return TRIPS_OK;
+}
+
 // Strides of what is written must keep its rows apart; what is read may repeat a row.
 int check_stride(const char* name, int64_t stride, int64_t row, int64_t rows, bool written)
 {
@@ -443,67 +715,92 @@ int check_stride(const char* name, int64_t stride, int64_t row, int64_t rows, bo
     return TRIPS_OK;
 }
 
-hipError_t launch_lookup(const TripsLookupDesc& d, const LookupParams& p, hipStream_t stream, Profiler* prof)
+size_t lookup_bytes(const TripsLookupDesc& d)
+{
+    return turns_table(d) ? up256((size_t)d.num_texels * (size_t)row_shape(d).padded * dtype_bytes(d.dtype)) : 0;
+}
+
+hipError_t launch_lookup(const TripsLookupDesc& d, const void* table, const void* index, void* values, void* workspace, hipStream_t stream,
+                         Profiler* prof)
 {
     ProfScope ps(prof, "lookup", stream);
-    if (d.layout == TRIPS_TABLE_COLUMNS)
+    const RowShape r = row_shape(d);
+    LookupParams p;
+    p.table = table, p.index = index, p.values = values, p.texels = d.num_texels, p.points = d.num_points;
+    p.table_stride = d.table_stride, p.values_stride = d.values_stride, p.channels = d.num_channels;
+    p.i32 = d.index_dtype == TRIPS_INDEX_I32, p.lanes_log2 = r.lanes_log2, p.scale = d.scale;
+    const bool columns = d.layout == TRIPS_TABLE_COLUMNS;
+    if (columns && !turns_table(d))
     {
         const dim3 grid((unsigned)((d.num_points + 255) / 256), (unsigned)((d.num_channels + kColumnGroup - 1) / kColumnGroup));
-        if (d.dtype == TRIPS_DTYPE_F32)
-            hipLaunchKernelGGL(lookup_columns_kernel<TRIPS_DTYPE_F32>, grid, dim3(256), 0, stream, p);
-        else if (d.dtype == TRIPS_DTYPE_BF16)
-            hipLaunchKernelGGL(lookup_columns_kernel<TRIPS_DTYPE_BF16>, grid, dim3(256), 0, stream, p);
-        else
-            hipLaunchKernelGGL(lookup_columns_kernel<TRIPS_DTYPE_F16>, grid, dim3(256), 0, stream, p);
+        with_types(d.dtype, 16, true, [&](auto D, auto, auto) {
+            hipLaunchKernelGGL(lookup_columns_kernel<decltype(D)::value>, grid, dim3(256), 0, stream, p);
+        });
+        return hipGetLastError();
     }
-    else
+    if (columns)
     {
-        const int l = lanes_log2_of(d.num_channels, d.dtype);
-        const dim3 grid((unsigned)std::min<long long>(((d.num_points << l) + 255) / 256, kMostRowGroups));
-        if (d.dtype == TRIPS_DTYPE_F32)
-            hipLaunchKernelGGL(lookup_rows_kernel<TRIPS_DTYPE_F32>, grid, dim3(256), 0, stream, p, l);
-        else if (d.dtype == TRIPS_DTYPE_BF16)
-            hipLaunchKernelGGL(lookup_rows_kernel<TRIPS_DTYPE_BF16>, grid, dim3(256), 0, stream, p, l);
-        else
-            hipLaunchKernelGGL(lookup_rows_kernel<TRIPS_DTYPE_F16>, grid, dim3(256), 0, stream, p, l);
+        if (d.num_texels > 0) launch_rows(d, r, table, workspace, d.num_texels, d.table_stride, stream);
+        p.table = workspace, p.table_stride = r.padded;
     }
+    const long long at_once = 4ll * (256 >> r.lanes_log2);
+    const dim3 grid((unsigned)std::min<long long>((d.num_points + at_once - 1) / at_once, kMostRowGroups));
+    with_types(d.dtype, r.lane_bytes, columns, [&](auto D, auto V, auto C) {
+        hipLaunchKernelGGL((lookup_rows_kernel<decltype(D)::value, decltype(V)::value, decltype(C)::value>), grid, dim3(256), 0, stream, p);
+    });
     return hipGetLastError();
 }
 
-hipError_t launch_lookup_backward(const TripsLookupDesc& d, const LookupParams& p, hipStream_t stream, Profiler* prof)
+struct GradLayout
+{
+    size_t rows, tiles, listed, bytes;
+    uint32_t tile, count, capacity;  // positions of a tile, tiles, texels of the list
+};
+GradLayout grad_layout(const TripsLookupDesc& d)
+{
+    const RowShape r = row_shape(d);
+    GradLayout l;
+    l.tile = 256;
+    while ((int64_t)l.tile * 4096 < d.num_points) l.tile *= 2;
+    l.count    = (uint32_t)(d.num_points / l.tile);
+    l.capacity = (uint32_t)(d.num_points / (kShort + 1));
+    size_t o   = 0;
+    l.rows     = o;
+    if (d.layout == TRIPS_TABLE_COLUMNS) o += up256((size_t)d.num_points * (size_t)r.padded * dtype_bytes(d.dtype));
+    l.tiles = o, o += up256((size_t)l.count * (size_t)r.padded * sizeof(float));
+    l.listed = o, o += up256((kListHead + (size_t)l.capacity) * sizeof(uint32_t));
+    l.bytes = o;
+    return l;
+}
+
+hipError_t launch_lookup_backward(const TripsLookupDesc& d, const void* d_values, const int32_t* order, const int32_t* starts, void* d_table,
+                                  char* ws, hipStream_t stream, Profiler* prof)
 {
     ProfScope ps(prof, "lookup_backward", stream);
-    if (d.layout == TRIPS_TABLE_COLUMNS)
+    const RowShape r   = row_shape(d);
+    const GradLayout l = grad_layout(d);
+    const bool columns = d.layout == TRIPS_TABLE_COLUMNS;
+    GradParams p;
+    p.rows = d_values, p.row = d.values_stride, p.d_table = d_table, p.order = order, p.starts = starts;
+    p.tiles = reinterpret_cast<float*>(ws + l.tiles), p.listed = reinterpret_cast<uint32_t*>(ws + l.listed);
+    p.texels = d.num_texels, p.table_stride = d.table_stride, p.points = (uint32_t)d.num_points, p.tile = l.tile, p.capacity = l.capacity;
+    p.channels = d.num_channels, p.padded = r.padded, p.lanes_log2 = r.lanes_log2, p.accumulate = d.accumulate != 0, p.scale = d.scale;
+    if (columns && d.num_points > 0)
     {
-        const dim3 grid((unsigned)((d.num_texels + 255) / 256), (unsigned)((d.num_channels + kColumnGroup - 1) / kColumnGroup));
-        if (d.dtype == TRIPS_DTYPE_F32)
-            hipLaunchKernelGGL(lookup_backward_columns_kernel<TRIPS_DTYPE_F32>, grid, dim3(256), 0, stream, p);
-        else if (d.dtype == TRIPS_DTYPE_BF16)
-            hipLaunchKernelGGL(lookup_backward_columns_kernel<TRIPS_DTYPE_BF16>, grid, dim3(256), 0, stream, p);
-        else
-            hipLaunchKernelGGL(lookup_backward_columns_kernel<TRIPS_DTYPE_F16>, grid, dim3(256), 0, stream, p);
+        launch_rows(d, r, d_values, ws + l.rows, d.num_points, d.values_stride, stream);
+        p.rows = ws + l.rows, p.row = r.padded;
     }
-    else
-    {
-        const int l = lanes_log2_of(d.num_channels, d.dtype);
-        const dim3 grid((unsigned)std::min<long long>(((d.num_texels << l) + 255) / 256, kMostRowGroups));
-        if (d.dtype == TRIPS_DTYPE_F32)
-            hipLaunchKernelGGL(lookup_backward_rows_kernel<TRIPS_DTYPE_F32>, grid, dim3(256), 0, stream, p, l);
-        else if (d.dtype == TRIPS_DTYPE_BF16)
-            hipLaunchKernelGGL(lookup_backward_rows_kernel<TRIPS_DTYPE_BF16>, grid, dim3(256), 0, stream, p, l);
-        else
-            hipLaunchKernelGGL(lookup_backward_rows_kernel<TRIPS_DTYPE_F16>, grid, dim3(256), 0, stream, p, l);
-    }
+    const long long at_once = 256 >> r.lanes_log2;
+    const dim3 grid((unsigned)std::min<long long>((d.num_texels + at_once - 1) / at_once, kMostRowGroups));
+    const dim3 tiles(l.count > 0 ? l.count : 1, r.groups), longs(std::min<uint32_t>(l.capacity, kLongGroups), r.groups);
+    with_types(d.dtype, r.lane_bytes, columns, [&](auto D, auto V, auto C) {
+        constexpr int kD = decltype(D)::value, kV = decltype(V)::value;
+        constexpr bool kC = decltype(C)::value;
+        if (l.capacity > 0) hipLaunchKernelGGL((lookup_tiles_kernel<kD, kV, kC>), tiles, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((lookup_backward_kernel<kD, kV, kC>), grid, dim3(256), 0, stream, p);
+        if (l.capacity > 0) hipLaunchKernelGGL((lookup_backward_long_kernel<kD, kV, kC>), longs, dim3(256), 0, stream, p);
+    });
     return hipGetLastError();
-}
-
-LookupParams params_of(const TripsLookupDesc& d)
-{
-    LookupParams p;
-    p.table = p.index = nullptr, p.values = nullptr, p.order = p.starts = nullptr;
-    p.texels = d.num_texels, p.points = d.num_points, p.table_stride = d.table_stride, p.values_stride = d.values_stride;
-    p.channels = d.num_channels, p.i32 = d.index_dtype == TRIPS_INDEX_I32, p.accumulate = d.accumulate != 0, p.scale = d.scale;
-    return p;
 }
 }  // namespace
 }  // namespace trips
@@ -512,7 +809,16 @@ using namespace trips;
 
 extern "C" {
 
-int trips_lookup_forward(TripsCtx* ctx, const TripsLookupDesc* desc, const void* table, const void* index, void* values, void* stream)
+int trips_lookup_workspace_size(const TripsLookupDesc* desc, size_t* bytes)
+{
+    if (!bytes) return set_error(TRIPS_ERR_INVALID_ARG, "bytes is NULL");
+    if (int e = check_lookup(desc)) return e;
+    *bytes = lookup_bytes(*desc);
+    return TRIPS_OK;
+}
+
+int trips_lookup_forward(TripsCtx* ctx, const TripsLookupDesc* desc, const void* table, const void* index, void* values,
+                         void* workspace, size_t workspace_bytes, void* stream)
 {
     if (!ctx) return set_error(TRIPS_ERR_INVALID_ARG, "ctx is NULL");
     if (int e = check_lookup(desc)) return e;
@@ -525,11 +831,10 @@ int trips_lookup_forward(TripsCtx* ctx, const TripsLookupDesc* desc, const void*
     if (!index || !aligned(index, d.index_dtype == TRIPS_INDEX_I32 ? 4 : 8)) return set_error(TRIPS_ERR_INVALID_ARG, "index is NULL or not aligned");
     if ((!table && d.num_texels > 0) || !aligned(table, size)) return set_error(TRIPS_ERR_INVALID_ARG, "table is NULL or not aligned");
     if (!values || !aligned(values, size)) return set_error(TRIPS_ERR_INVALID_ARG, "values is NULL or not aligned");
+    if (int e = check_workspace(workspace, workspace_bytes, lookup_bytes(d))) return e;
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_error(scope.error, "hipSetDevice");
-    LookupParams p = params_of(d);
-    p.table = table, p.index = index, p.values = values;
-    hipError_t e = launch_lookup(d, p, reinterpret_cast<hipStream_t>(stream), profiler(ctx));
+    hipError_t e = launch_lookup(d, table, index, values, workspace, reinterpret_cast<hipStream_t>(stream), profiler(ctx));
     return e == hipSuccess ? TRIPS_OK : hip_error(e, "lookup launch");
 }
 
@@ -554,8 +859,7 @@ int trips_lookup_plan(TripsCtx* ctx, int64_t num_texels, int64_t num_points, con
     {
         if (!index || !aligned(index, index_dtype == TRIPS_INDEX_I32 ? 4 : 8)) return set_error(TRIPS_ERR_INVALID_ARG, "index is NULL or not aligned");
         if (!order || !aligned(order, 4)) return set_error(TRIPS_ERR_INVALID_ARG, "order is NULL or not aligned");
-        if (!workspace || !aligned(workspace, 256)) return set_error(TRIPS_ERR_INVALID_ARG, "workspace must be a 256-byte aligned device pointer");
-        if (workspace_bytes < need) return set_error(TRIPS_ERR_WORKSPACE_SMALL, "workspace has %zu bytes, %zu needed", workspace_bytes, need);
+        if (int e = check_workspace(workspace, workspace_bytes, need)) return e;
     }
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_error(scope.error, "hipSetDevice");
@@ -568,7 +872,7 @@ int trips_lookup_backward_workspace_size(const TripsLookupDesc* desc, size_t* by
 {
     if (!bytes) return set_error(TRIPS_ERR_INVALID_ARG, "bytes is NULL");
     if (int e = check_lookup(desc)) return e;
-    *bytes = 0;
+    *bytes = grad_layout(*desc).bytes;
     return TRIPS_OK;
 }
 
@@ -587,15 +891,11 @@ int trips_lookup_backward(TripsCtx* ctx, const TripsLookupDesc* desc, const void
     if (!d_table || !aligned(d_table, size)) return set_error(TRIPS_ERR_INVALID_ARG, "d_table is NULL or not aligned");
     if (d.num_points > 0 && (!order || !aligned(order, 4) || !d_values || !aligned(d_values, size)))
         return set_error(TRIPS_ERR_INVALID_ARG, "order or d_values is NULL or not aligned");
-    size_t need = 0;
-    if (int e = trips_lookup_backward_workspace_size(desc, &need)) return e;
-    if (need > 0 && (!workspace || !aligned(workspace, 256))) return set_error(TRIPS_ERR_INVALID_ARG, "workspace must be a 256-byte aligned device pointer");
-    if (workspace_bytes < need) return set_error(TRIPS_ERR_WORKSPACE_SMALL, "workspace has %zu bytes, %zu needed", workspace_bytes, need);
+    if (int e = check_workspace(workspace, workspace_bytes, grad_layout(d).bytes)) return e;
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_error(scope.error, "hipSetDevice");
-    LookupParams p = params_of(d);
-    p.table = d_values, p.values = d_table, p.order = order, p.starts = starts;
-    hipError_t e = launch_lookup_backward(d, p, reinterpret_cast<hipStream_t>(stream), profiler(ctx));
+    hipError_t e = launch_lookup_backward(d, d_values, order, starts, d_table, reinterpret_cast<char*>(workspace),
+                                          reinterpret_cast<hipStream_t>(stream), profiler(ctx));
     return e == hipSuccess ? TRIPS_OK : hip_error(e, "lookup backward launch");
 }
 

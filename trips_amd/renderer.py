@@ -219,9 +219,14 @@ class SplatContext:
         _lib.check(self.lib.trips_adam_step_points(self.ctx, arr, int(num_points), int(num_channels), _ptr(state),
                                                    _stream_ptr(self.device)))
 
+    def adamw_workspace_size(self, n_tensors):
+        b = C.c_size_t(0)
+        _lib.check(self.lib.trips_adamw_workspace_size(n_tensors, C.byref(b)))
+        return b.value
+
     def adamw_step(self, tensors, n_tensors, options, workspace):
         """tensors: an array of abi.TripsAdamWTensor, or its bytes; options: abi.TripsAdamWOptions; workspace: a device
-        tensor of abi.TRIPS_ADAMW_WORKSPACE_BYTES, zero before its first use."""
+        tensor of adamw_workspace_size bytes."""
         _lib.check(self.lib.trips_adamw_step(self.ctx, tensors, n_tensors, C.byref(options), _ptr(workspace), workspace.numel(),
                                              _stream_ptr(self.device)))
 
@@ -232,8 +237,11 @@ class SplatContext:
 
     # ---- table lookups ----
     def lookup_forward(self, desc, table, index, values):
-        _lib.check(self.lib.trips_lookup_forward(self.ctx, C.byref(desc), _ptr(table), _ptr(index), _ptr(values),
-                                                 _stream_ptr(self.device)))
+        need = C.c_size_t(0)
+        _lib.check(self.lib.trips_lookup_workspace_size(C.byref(desc), C.byref(need)))
+        workspace = self.alloc_bytes(need.value) if need.value else None
+        _lib.check(self.lib.trips_lookup_forward(self.ctx, C.byref(desc), _ptr(table), _ptr(index), _ptr(values), _ptr(workspace),
+                                                 need.value, _stream_ptr(self.device)))
 
     def lookup_plan(self, num_texels, index, index_dtype, order, starts):
         need = C.c_size_t(0)
