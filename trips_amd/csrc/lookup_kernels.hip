@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(const LookupParams p)
                 {
 #pragma unroll
                     for (int e = 0; e < V; ++e)
-                        if (c + e < p.channels) values[(c + e) * p.values_stride + i] = x[q][e];
+                        if (c + e < p.channels) __builtin_nontemporal_store(x[q][e], values + (c + e) * p.values_stride + i);
                 }
                 else if (count == V)
                     *reinterpret_cast<typename Pack<T, V>::type*>(values + i * p.values_stride + c) = x[q];
@@ -151,8 +151,12 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(const LookupParams p)
 
 // ---- the order of the points: a stable radix sort, least significant digit first ----
 
-constexpr int kSortThreads = 256, kSortItems = 16, kSortTile = kSortThreads * kSortItems;
+// A tile: 4096 points, or 2048 below a million (20k points 31 us and 37, 1M 57 and 58; 6M the other way round).
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int64_t kManyPoints = 1 << 20;
+constexpr int sort_items(int64_t points) { return points < kManyPoints ? 2 : 4; }
 constexpr int kDigits = 256;
+constexpr uint32_t kFewTiles = 32;  // so few that each tile's workgroup sums the counts of the others itself: a launch less a pass
 
 struct SortParams
 {
@@ -175,12 +179,15 @@ __device__ __forceinline__ uint32_t sort_key(const SortParams& p, uint32_t i)
     return t >= 0 && t < (long long)p.texels ? (uint32_t)t : p.texels;
 }
 
+template <int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortParams p)
 {
+    constexpr int kSortItems = ITEMS, kSortTile = kSortThreads * ITEMS;
     __shared__ uint32_t s[kDigits];
-    s[threadIdx.x] = 0;
+    if (threadIdx.x < kDigits) s[threadIdx.x] = 0;
     __syncthreads();
     const uint32_t mask = (1u << p.bits) - 1u;
+#pragma unroll
     for (int k = 0; k < kSortItems; ++k)
     {
         const uint32_t i = blockIdx.x * (uint32_t)kSortTile + k * kSortThreads + threadIdx.x;
@@ -190,7 +197,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortPara
     if (threadIdx.x <= mask) p.hist[(size_t)threadIdx.x * p.tiles + blockIdx.x] = s[threadIdx.x];
 }
 
-// Sum over the threads of the workgroup up to this one, itself included; s: 4 words.
+// Sum over the threads of the workgroup up to this one, itself included; s: a word a wavefront.
 __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* s)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -207,19 +214,20 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* s)
     return x;
 }
 
+constexpr int kScanThreads = 1024;
 // One workgroup a digit: its counts become the sums of the tiles before.
-__global__ __launch_bounds__(kSortThreads) void sort_scan_kernel(const SortParams p)
+__global__ __launch_bounds__(kScanThreads) void sort_scan_kernel(const SortParams p)
 {
-    __shared__ uint32_t s[4], s_sum;
-    uint32_t* row  = p.hist + (size_t)blockIdx.x * p.tiles;
+    __shared__ uint32_t s[kScanThreads / 64], s_sum;
+    uint32_t* row   = p.hist + (size_t)blockIdx.x * p.tiles;
     uint32_t before = 0;
-    for (uint32_t base = 0; base < p.tiles; base += kSortThreads)
+    for (uint32_t base = 0; base < p.tiles; base += kScanThreads)
     {
         const uint32_t i = base + threadIdx.x;
         const uint32_t x = i < p.tiles ? row[i] : 0u;
         const uint32_t y = block_scan(x, s);
         if (i < p.tiles) row[i] = before + y - x;
-        if (threadIdx.x == kSortThreads - 1) s_sum = y;
+        if (threadIdx.x == kScanThreads - 1) s_sum = y;
         __syncthreads();
         before += s_sum;
         __syncthreads();
@@ -227,69 +235,104 @@ __global__ __launch_bounds__(kSortThreads) void sort_scan_kernel(const SortParam
     if (threadIdx.x == 0) p.totals[blockIdx.x] = before;
 }
 
-// A tile's keys go to their places. A wavefront takes 64 keys after the other, the keys of equal digit found by ballots; the
-// tile is put in order in LDS first, so that each digit's keys leave side by side.
+// Ranks of a wavefront's keys among its keys of the same digit: ITEMS rounds of 64 keys, the keys of a round that share a digit
+// found by ballots. The first of them adds their number to the digit's count in LDS; LDS serves a wavefront in order, so no round
+// waits for the one before. `count`: the wavefront's counts, zeros before, its keys of each digit behind a barrier.
+template <int ITEMS>
+__device__ __forceinline__ void rank_keys(const uint32_t (&key)[ITEMS], uint32_t valid, int shift, int bits, uint32_t* count, uint32_t (&rank)[ITEMS])
+{
+    const int lane      = threadIdx.x & 63;
+    const uint32_t mask = (1u << bits) - 1u;
+    uint32_t base[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+    {
+        const bool in        = k * 64u + lane < valid;
+        const uint32_t digit = (key[k] >> shift) & mask;
+        const unsigned long long all = __ballot(in);
+        uint32_t low = (uint32_t)all, high = (uint32_t)(all >> 32);
+#pragma unroll 1
+        for (int b = 0; b < bits; ++b)
+        {
+            const uint32_t set         = (uint32_t)__builtin_amdgcn_sbfe((int)digit, (uint32_t)b, 1u);  // all ones or zeros
+            const unsigned long long v = __ballot(set != 0u);
+            low &= ~((uint32_t)v ^ set);
+            high &= ~((uint32_t)(v >> 32) ^ set);
+        }
+        const unsigned long long same = (unsigned long long)high << 32 | low;
+        const uint32_t before = (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
+        rank[k] = before | (((uint32_t)__ffsll((long long)same) - 1u) & 63u) << 8;  // and the lane of the first of them
+        base[k] = 0;
+        if (in && before == 0)
+            base[k] = __hip_atomic_fetch_add(count + digit, (uint32_t)__popcll(same), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) rank[k] = (rank[k] & 255u) + (uint32_t)__shfl((int)base[k], (int)(rank[k] >> 8));
+}
+
+// A tile's keys go to their places; the tile is put in order in LDS first, so that each digit's keys leave side by side.
+template <int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortParams p)
 {
-    __shared__ uint32_t s_count[4][kDigits];  // keys of a digit in each wavefront, then those of the tile before them
-    __shared__ uint32_t s_place[kDigits];     // of the tile's first key of a digit: its place, less its place in the tile
+    constexpr int kSortItems = ITEMS, kSortTile = kSortThreads * ITEMS;
+    __shared__ uint32_t s_count[kSortWaves][kDigits];  // keys of a digit in each wavefront, then those of the tile before them
+    __shared__ uint32_t s_place[kDigits];              // of the tile's first key of a digit: its place, less its place in the tile
     __shared__ uint32_t s_key[kSortTile];
     __shared__ int32_t s_point[kSortTile];
-    __shared__ uint32_t s_scan[4];
+    __shared__ uint32_t s_scan[kSortWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t mask  = (1u << p.bits) - 1u;
     const uint32_t begin = blockIdx.x * (uint32_t)kSortTile;
     const uint32_t count = min((uint32_t)kSortTile, p.n - begin);
-    for (int w = 0; w < 4; ++w) s_count[w][threadIdx.x] = 0;
-    __syncthreads();
+    for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) s_count[0][i] = 0;
     uint32_t key[kSortItems], rank[kSortItems];
     int32_t point[kSortItems];
-    const uint32_t mine = wave * (uint32_t)(kSortTile / 4) + lane;
+    const uint32_t mine = wave * 64u * kSortItems, valid = count > mine ? count - mine : 0u;
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k)
     {
-        const uint32_t i = mine + k * 64;
+        const uint32_t i = mine + k * 64 + lane;
         key[k]   = i < count ? sort_key(p, begin + i) : ~0u;
         point[k] = i < count ? (p.first ? (int32_t)(begin + i) : p.points_in[begin + i]) : 0;
     }
-#pragma unroll
-    for (int k = 0; k < kSortItems; ++k)
-    {
-        const bool in        = mine + k * 64 < count;
-        const uint32_t digit = (key[k] >> p.shift) & mask;
-        unsigned long long same = __ballot(in);
-        for (int b = 0; b < p.bits; ++b)
-        {
-            const bool set = (digit >> b) & 1u;
-            const unsigned long long v = __ballot(set);
-            same &= set ? v : ~v;
-        }
-        const uint32_t before = (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
-        uint32_t base = 0;
-        if (in) base = s_count[wave][digit];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (in && before == 0) s_count[wave][digit] = base + (uint32_t)__popcll(same);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        rank[k] = base + before;
-    }
+    __syncthreads();
+    rank_keys(key, valid, p.shift, p.bits, s_count[wave], rank);
     __syncthreads();
     {
-        const int d = threadIdx.x;
-        uint32_t c[4], sum = 0;
-        for (int w = 0; w < 4; ++w) c[w] = s_count[w][d], sum += c[w];
+        const int d    = threadIdx.x;
+        const bool has = d <= (int)mask;
+        uint32_t sum   = 0;
+        if (has)
+            for (int w = 0; w < kSortWaves; ++w) sum += s_count[w][d];
         const uint32_t in_tile = block_scan(sum, s_scan) - sum;  // the tile's keys of lower digits
-        for (uint32_t w = 0, x = in_tile; w < 4; ++w) s_count[w][d] = x, x += c[w];
-        const uint32_t total = d <= (int)mask ? p.totals[d] : 0u;
+        // of all keys, those of the digit, and of the tiles before this one
+        uint32_t total = 0, before = 0;
+        if (has && p.tiles > kFewTiles)
+            total = p.totals[d], before = p.hist[(size_t)d * p.tiles + blockIdx.x];
+        else if (has)
+            for (uint32_t t = 0; t < p.tiles; ++t)
+            {
+                const uint32_t c = p.hist[(size_t)d * p.tiles + t];
+                total += c;
+                before += t < blockIdx.x ? c : 0u;
+            }
         const uint32_t below = block_scan(total, s_scan) - total;  // all keys of lower digits
-        if (d <= (int)mask) s_place[d] = below + p.hist[(size_t)d * p.tiles + blockIdx.x] - in_tile;
+        if (has)
+        {
+            s_place[d] = below + before - in_tile;
+            for (uint32_t w = 0, x = in_tile; w < kSortWaves; ++w)
+            {
+                const uint32_t c = s_count[w][d];
+                s_count[w][d]    = x;
+                x += c;
+            }
+        }
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k)
     {
-        if (mine + k * 64 >= count) continue;
+        if (k * 64u + lane >= valid) continue;
         const uint32_t at = s_count[wave][(key[k] >> p.shift) & mask] + rank[k];
         s_key[at]   = key[k];
         s_point[at] = point[k];
@@ -301,6 +344,74 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortPa
         const uint32_t to = s_place[(k >> p.shift) & mask] + at;
         p.keys_out[to]    = k;
         p.points_out[to]  = s_point[at];
+    }
+}
+
+// Few points: a point's place is the number of keys below its own and of equal ones before it, counted outright. All keys in LDS,
+// 32 points a workgroup, each by 32 threads with a 32nd of the keys. One launch, on all of the card, where the sort's passes are
+// launches in a row. Bound by the LDS that every key of every workgroup is read from (3.4 us of 11 at 8191 points) and the
+// pairs' two instructions (as much).
+// Behind the points' places, if `starts`: the keys below each t.
+constexpr int kCountThreads = 1024, kCountItems = 32;
+constexpr int64_t kSmallPoints = 8192;             // a workgroup a CU (8192 of 5000 texels 12.5 us, 12288 24; by passes 21 and 22)
+constexpr int64_t kSmallPairs  = (int64_t)1 << 27; // keys and starts
+constexpr uint32_t small_part(uint32_t n) { return ((n + 31u) / 32u + 31u) & ~31u; }  // keys of a thread, whole words of signs
+__global__ __launch_bounds__(kCountThreads) void sort_small_kernel(const SortParams p, int32_t* starts)
+{
+    extern __shared__ uint4 s_keys[];
+    __shared__ uint32_t s_rank[kCountItems];
+    uint32_t* s_key     = reinterpret_cast<uint32_t*>(s_keys);
+    const uint32_t part = small_part(p.n);
+    const uint32_t from = (threadIdx.x >> 5) * part, to = from + part;
+    // (four words between the parts: a wavefront reads two of them at a time, from other banks)
+    const uint32_t shift = (threadIdx.x >> 5) * 4u;
+    for (uint32_t j = from + (threadIdx.x & 31u); j < to; j += 32) s_key[j + shift] = j < p.n ? sort_key(p, j) : 0x7fffffffu;  // (no key is that)
+    if (threadIdx.x < kCountItems) s_rank[threadIdx.x] = 0u;
+    __syncthreads();
+    // (the points' workgroups first, then those of the starts)
+    const uint32_t point_groups = (p.n + kCountItems - 1) / kCountItems;
+    const bool of_points = blockIdx.x < point_groups;
+    const uint32_t i0 = (of_points ? blockIdx.x : blockIdx.x - point_groups) * kCountItems, i = i0 + (threadIdx.x & 31u);
+    const uint32_t mine = of_points ? (i < p.n ? sort_key(p, i) : 0u) : i;
+    // The signs of 32 differences in a word: a subtraction and a shift a pair, where the carry of a comparison must be waited for.
+    auto less = [&](uint32_t j, uint32_t limit)
+    {
+        uint32_t signs = 0;
+#pragma unroll
+        for (uint32_t q = 0; q < 32; q += 4)
+        {
+            const uint4 k = s_keys[(j + q + shift) / 4];
+            signs = __builtin_amdgcn_alignbit(signs, k.x - limit, 31u);
+            signs = __builtin_amdgcn_alignbit(signs, k.y - limit, 31u);
+            signs = __builtin_amdgcn_alignbit(signs, k.z - limit, 31u);
+            signs = __builtin_amdgcn_alignbit(signs, k.w - limit, 31u);
+        }
+        return signs;
+    };
+    uint32_t below = 0;
+    for (uint32_t j = from; j < to; j += 32)
+    {
+        // equal keys count where they lie before the point
+        const uint32_t signs = less(j, mine + (of_points && j < i0 ? 1u : 0u));
+        below += (uint32_t)__popc(signs);
+        if (of_points && __ballot(j == i0))
+        {
+            const uint32_t equal = less(j, mine + 1u) & ~signs & ~(~0u >> (i & 31u));  // (the word's first keys are its highest bits)
+            below += j == i0 ? (uint32_t)__popc(equal) : 0u;
+        }
+    }
+    atomicAdd(&s_rank[threadIdx.x & 31u], below);
+    __syncthreads();
+    if (threadIdx.x >= kCountItems) return;
+    const uint32_t at = s_rank[threadIdx.x];
+    if (!of_points)
+    {
+        if (i <= p.texels) starts[i] = (int32_t)at;
+    }
+    else if (i < p.n)
+    {
+        p.points_out[at] = (int32_t)i;
+        if (p.keys_out) p.keys_out[at] = mine;
     }
 }
 
@@ -322,32 +433,70 @@ __device__ __forceinline__ uint32_t lower_bound(const T* a, uint32_t n, uint32_t
     return lo;
 }
 
-// starts[t] = the first of the sorted keys that is t or more. A wavefront finds those of its first and its last texel with all
-// lanes; each lane's search goes on between them.
-constexpr int kStartsItems = 4;  // texels of a lane, 64 apart
+// starts[t] = the first of the sorted keys that is t or more, for kStartsTexels texels a workgroup. Two wavefronts find the keys
+// that belong to them; where these are about as many as the texels, each key that differs from the one before is noted in LDS
+// and the texels in between take the next one's; where they are many more, each texel is searched for. ITEMS texels a thread: 8,
+// or 1 where there are more than two points a texel.
+template <int ITEMS>
 __global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t texels, int32_t* starts)
 {
-    const int lane       = threadIdx.x & 63;
-    const uint32_t first = (blockIdx.x * 4u + (threadIdx.x >> 6)) * (64u * kStartsItems);
-    if (first > texels) return;
-    const uint32_t last = min(texels, first + 64u * kStartsItems - 1u);
-    const uint32_t from = lower_bound(keys, n, first, lane), to = from + lower_bound(keys + from, n - from, last, lane);
-#pragma unroll
-    for (int q = 0; q < kStartsItems; ++q)
+    constexpr int kStartsItems = ITEMS, kStartsTexels = 256 * ITEMS;
+    __shared__ uint32_t s_range[2], s_first[kStartsTexels], s_next[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t first = blockIdx.x * (uint32_t)kStartsTexels, count = min((uint32_t)kStartsTexels, texels + 1u - first);
+    if (wave < 2)
     {
-        const uint32_t t = first + q * 64u + lane;
-        if (t > texels) return;
-        uint32_t lo = from, hi = to;
-        while (lo < hi)
-        {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (keys[mid] < t)
-                lo = mid + 1;
-            else
-                hi = mid;
-        }
-        starts[t] = (int32_t)lo;
+        const uint32_t at = lower_bound(keys, n, wave == 0 ? first : first + count, lane);
+        if (lane == 0) s_range[wave] = at;
     }
+#pragma unroll
+    for (int q = 0; q < kStartsItems; ++q) s_first[q * 256 + threadIdx.x] = ~0u;
+    __syncthreads();
+    const uint32_t from = s_range[0], to = s_range[1];
+    if (to - from > 8u * kStartsTexels)
+    {
+        for (uint32_t t = threadIdx.x; t < count; t += 256)
+        {
+            uint32_t lo = from, hi = to;
+            while (lo < hi)
+            {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                if (keys[mid] < first + t)
+                    lo = mid + 1;
+                else
+                    hi = mid;
+            }
+            starts[first + t] = (int32_t)lo;
+        }
+        return;
+    }
+    for (uint32_t k = from + threadIdx.x; k < to; k += 256)
+    {
+        const uint32_t key = keys[k];
+        if (k == from || keys[k - 1] != key) s_first[key - first] = k;
+    }
+    __syncthreads();
+    // the least of a thread's texels' and all that follow
+    uint32_t at[kStartsItems], least = ~0u;
+#pragma unroll
+    for (int q = kStartsItems - 1; q >= 0; --q) at[q] = least = min(least, s_first[threadIdx.x * kStartsItems + q]);
+    uint32_t behind = least;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+    {
+        const uint32_t y = (uint32_t)__shfl_down((int)behind, o);
+        if (lane + o < 64) behind = min(behind, y);
+    }
+    if (lane == 0) s_next[wave] = behind;
+    behind = (uint32_t)__shfl_down((int)behind, 1);
+    if (lane == 63) behind = ~0u;
+    __syncthreads();
+    for (int w = wave + 1; w < 4; ++w) behind = min(behind, s_next[w]);
+    behind = min(behind, to);
+#pragma unroll
+    for (int q = 0; q < kStartsItems; ++q) s_first[threadIdx.x * kStartsItems + q] = min(at[q], behind);
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < count; t += 256) starts[first + t] = (int32_t)s_first[t];
 }
 
 // ---- the gradient ----
@@ -359,6 +508,7 @@ __global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict_
 
 constexpr int kShort      = 32;
 constexpr int kLongGroups = 2048;  // workgroups for the listed texels
+constexpr int kWideThreads = 1024; // of a workgroup that adds up rows of more than eight lanes; 256 for others
 
 struct GradParams
 {
@@ -477,26 +627,26 @@ __device__ __forceinline__ void add_threads(float (&sum)[V], float* s, int lanes
     const int lanes = 1 << lanes_log2;
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < V; ++e) s[e * 256 + threadIdx.x] = sum[e];
+    for (int e = 0; e < V; ++e) s[e * blockDim.x + threadIdx.x] = sum[e];
     __syncthreads();
-    for (int half = 128; half >= lanes; half >>= 1)
+    for (int half = (int)blockDim.x / 2; half >= lanes; half >>= 1)
     {
         if ((int)threadIdx.x < half)
         {
 #pragma unroll
-            for (int e = 0; e < V; ++e) s[e * 256 + threadIdx.x] += s[e * 256 + threadIdx.x + half];
+            for (int e = 0; e < V; ++e) s[e * blockDim.x + threadIdx.x] += s[e * blockDim.x + threadIdx.x + half];
         }
         __syncthreads();
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) sum[e] = s[e * 256 + threadIdx.x];
+    for (int e = 0; e < V; ++e) sum[e] = s[e * blockDim.x + threadIdx.x];
 }
 
 // One workgroup a tile of the plan's positions (and a group of lanes' channels). Clears the list's length as well.
 template <int D, int V, bool OUT_COLUMNS>
-__global__ __launch_bounds__(256) void lookup_tiles_kernel(const GradParams p)
+__global__ __launch_bounds__(kWideThreads) void lookup_tiles_kernel(const GradParams p)
 {
-    __shared__ float s[V * 256];
+    extern __shared__ float s[];  // [V][threads]
     __shared__ uint32_t s_in;
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.listed = 0u;
     const uint32_t from = blockIdx.x * p.tile, to = from + p.tile;
@@ -513,7 +663,7 @@ __global__ __launch_bounds__(256) void lookup_tiles_kernel(const GradParams p)
     float sum[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[e] = 0.f;
-    if (s_in && c < p.channels) add_rows<D, V>(p, from + r, to, 256 >> p.lanes_log2, c, OUT_COLUMNS ? V : min(V, p.channels - c), sum);
+    if (s_in && c < p.channels) add_rows<D, V>(p, from + r, to, blockDim.x >> p.lanes_log2, c, OUT_COLUMNS ? V : min(V, p.channels - c), sum);
     add_threads(sum, s, p.lanes_log2);
     if ((int)threadIdx.x < lanes && c < p.padded)
     {
@@ -525,11 +675,11 @@ __global__ __launch_bounds__(256) void lookup_tiles_kernel(const GradParams p)
 // One workgroup a listed texel (and a group of lanes' channels): the points before its first whole tile, those behind its last
 // one, and the tiles.
 template <int D, int V, bool OUT_COLUMNS>
-__global__ __launch_bounds__(256) void lookup_backward_long_kernel(const GradParams p)
+__global__ __launch_bounds__(kWideThreads) void lookup_backward_long_kernel(const GradParams p)
 {
-    __shared__ float s[V * 256];
+    extern __shared__ float s[];  // [V][threads]
     const int lanes = 1 << p.lanes_log2, j = threadIdx.x & (lanes - 1), r = threadIdx.x >> p.lanes_log2;
-    const uint32_t rows = 256u >> p.lanes_log2;
+    const uint32_t rows = blockDim.x >> p.lanes_log2;
     const int c         = (blockIdx.y * lanes + j) * V;
     const int count     = OUT_COLUMNS ? V : min(V, p.channels - c);
     const uint32_t n    = min(*p.listed, p.capacity);
@@ -645,7 +795,8 @@ struct PlanLayout
 PlanLayout plan_layout(int64_t points)
 {
     auto up            = up256;
-    const size_t tiles = (size_t)((points + kSortTile - 1) / kSortTile);
+    const int tile     = kSortThreads * sort_items(points);
+    const size_t tiles = (size_t)((points + tile - 1) / tile);
     PlanLayout l;
     size_t o  = 0;
     l.keys[0] = o, o += up((size_t)points * 4);
@@ -664,25 +815,50 @@ hipError_t launch_plan(int64_t texels, int64_t points, const void* index, int in
     const int bits     = key_bits(texels), passes = (bits + 7) / 8;
     SortParams p;
     p.index = index, p.i32 = index_dtype == TRIPS_INDEX_I32, p.n = (uint32_t)points, p.texels = (uint32_t)texels;
-    p.tiles = (uint32_t)((points + kSortTile - 1) / kSortTile);
+    const int tile = kSortThreads * sort_items(points);
+    p.tiles        = (uint32_t)((points + tile - 1) / tile);
     p.hist = reinterpret_cast<uint32_t*>(ws + l.hist), p.totals = reinterpret_cast<uint32_t*>(ws + l.totals);
     p.keys_out = nullptr, p.points_out = nullptr;
     ProfScope ps(prof, "lookup_plan", stream);
+    if (points > 0 && points <= kSmallPoints)
+    {
+        const bool whole = (texels + 1) * points <= kSmallPairs;
+        p.first = 1, p.shift = 0, p.bits = 0, p.keys_in = nullptr, p.points_in = nullptr;
+        p.keys_out   = whole ? nullptr : reinterpret_cast<uint32_t*>(ws + l.keys[0]);
+        p.points_out = order;
+        const size_t lds      = 32 * sizeof(uint32_t) * (small_part(p.n) + 4);
+        const unsigned groups = (p.n + kCountItems - 1) / kCountItems, more = whole ? (unsigned)(texels + kCountItems) / kCountItems : 0u;
+        if (lds > 64 * 1024)
+        {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&sort_small_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL(sort_small_kernel, dim3(groups + more), dim3(kCountThreads), lds, stream, p, starts);
+        if (whole) return hipGetLastError();
+    }
     int shift = 0;
-    for (int pass = 0; pass < passes && points > 0; ++pass)
+    for (int pass = 0; pass < passes && points > kSmallPoints; ++pass)
     {
         p.first = pass == 0, p.shift = shift, p.bits = (bits - shift + passes - pass - 1) / (passes - pass);
         p.keys_in    = p.keys_out;
         p.points_in  = p.points_out;
         p.keys_out   = reinterpret_cast<uint32_t*>(ws + l.keys[pass & 1]);
         p.points_out = (passes - 1 - pass) % 2 == 0 ? order : reinterpret_cast<int32_t*>(ws + l.points);
-        hipLaunchKernelGGL(sort_count_kernel, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
-        hipLaunchKernelGGL(sort_scan_kernel, dim3(1 << p.bits), dim3(kSortThreads), 0, stream, p);
-        hipLaunchKernelGGL(sort_scatter_kernel, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
+        if (sort_items(points) == 2)
+            hipLaunchKernelGGL(sort_count_kernel<2>, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
+        else
+            hipLaunchKernelGGL(sort_count_kernel<4>, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
+        if (p.tiles > kFewTiles) hipLaunchKernelGGL(sort_scan_kernel, dim3(1 << p.bits), dim3(kScanThreads), 0, stream, p);
+        if (sort_items(points) == 2)
+            hipLaunchKernelGGL(sort_scatter_kernel<2>, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
+        else
+            hipLaunchKernelGGL(sort_scatter_kernel<4>, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
         shift += p.bits;
     }
-    hipLaunchKernelGGL(starts_kernel, dim3((unsigned)(texels / (256 * kStartsItems) + 1)), dim3(256), 0, stream, p.keys_out, (uint32_t)points,
-                       (uint32_t)texels, starts);
+    if (points > 2 * texels)
+        hipLaunchKernelGGL(starts_kernel<1>, dim3((unsigned)(texels / 256 + 1)), dim3(256), 0, stream, p.keys_out, (uint32_t)points, (uint32_t)texels, starts);
+    else
+        hipLaunchKernelGGL(starts_kernel<8>, dim3((unsigned)(texels / 2048 + 1)), dim3(256), 0, stream, p.keys_out, (uint32_t)points, (uint32_t)texels, starts);
     return hipGetLastError();
 }
 
@@ -796,9 +972,11 @@ hipError_t launch_lookup_backward(const TripsLookupDesc& d, const void* d_values
     with_types(d.dtype, r.lane_bytes, columns, [&](auto D, auto V, auto C) {
         constexpr int kD = decltype(D)::value, kV = decltype(V)::value;
         constexpr bool kC = decltype(C)::value;
-        if (l.capacity > 0) hipLaunchKernelGGL((lookup_tiles_kernel<kD, kV, kC>), tiles, dim3(256), 0, stream, p);
+        const int threads = r.lanes_log2 > 3 ? kWideThreads : 256;
+        const size_t lds  = (size_t)kV * threads * sizeof(float);
+        if (l.capacity > 0) hipLaunchKernelGGL((lookup_tiles_kernel<kD, kV, kC>), tiles, dim3(threads), lds, stream, p);
         hipLaunchKernelGGL((lookup_backward_kernel<kD, kV, kC>), grid, dim3(256), 0, stream, p);
-        if (l.capacity > 0) hipLaunchKernelGGL((lookup_backward_long_kernel<kD, kV, kC>), longs, dim3(256), 0, stream, p);
+        if (l.capacity > 0) hipLaunchKernelGGL((lookup_backward_long_kernel<kD, kV, kC>), longs, dim3(threads), lds, stream, p);
     });
     return hipGetLastError();
 }
