@@ -53,6 +53,7 @@ class LookupPlan:
             raise ValueError("a plan is two contiguous int32 tensors: order [N] and starts [T + 1]")
         self.order, self.starts = order, starts
         self.index = index
+        self._own = None
         self.version = None if index is None or index.is_inference() else index._version
 
     def check(self, index, texels):
@@ -63,6 +64,20 @@ class LookupPlan:
         if own is not None and (own.data_ptr() != index.data_ptr() or own.dtype != index.dtype or own.stride() != index.stride()
                                 or (None if index.is_inference() else index._version) != self.version):
             raise ValueError("the plan was made of another index, or the index was changed since")
+
+
+    def own_index(self, index):
+        """own_index() of the plan's index, made once."""
+        self.check(index, self.starts.numel() - 1)
+        if self._own is None:
+            self._own = own_index(index, self.starts.numel() - 1)
+        return self._own
+
+
+def own_index(index, num_texels):
+    """The number of each point, -1 where its index is outside [0, num_texels): int32, in the index's shape."""
+    own = torch.arange(index.numel(), dtype=torch.int32, device=index.device).reshape(index.shape)
+    return torch.where((index >= 0) & (index < num_texels), own, -1)
 
 
 @torch.no_grad()

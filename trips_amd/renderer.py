@@ -11,7 +11,9 @@ Same names and argument meaning as the reference (paths relative to the referenc
 torch is used for device memory, streams and the autograd graph only; all computation happens in
 libtrips_splat.so. There is no fallback path: without the library (or without a GPU) these calls raise.
 """
+import copy
 import ctypes as C
+import functools
 from dataclasses import dataclass, field
 from typing import List, Optional
 
@@ -317,6 +319,10 @@ class RenderParams:
     background_mode: int = abi.TRIPS_BG_REFERENCE
     max_pixels_per_list: int = 16
     floor_layer_sizes: bool = False  # network_version == "MultiScaleUnet2d" (PointRenderer.cu:385-394)
+    # not in the reference either: descriptors and confidences that points share (t_index names a texel more than once) are
+    # looked up per point before the splat, and their gradients summed in the order of the points, the same bits every time.
+    # The splat by itself adds them with float atomics. NeuralScene.plan_texels() keeps the order from step to step.
+    shared_texels_in_order: bool = False
 
 
 class PointRendererCache:
@@ -473,8 +479,31 @@ class PointRender(torch.autograd.Function):
                 grads["d_intrinsics"], d_conf, None, d_layer, None)
 
 
+def _with_own_texels(info):
+    """`info` for a scene in which every point has a texel of its own, looked up from those that t_index names."""
+    from . import lookup
+    sc = info.scene
+    if info.cache is None:
+        info.cache = PointRendererCache()
+    points, index = sc.point_cloud_cuda, sc.point_cloud_cuda.t_index
+    plan = getattr(sc, "texel_plan", None)
+    if plan is None:
+        plan = lookup.lookup_plan(index, int(sc.texture.texture.shape[1])) if info.train else None
+    # a point whose texel is outside the table is left out, and reported, as ever
+    own = lookup.own_index(index, int(sc.texture.texture.shape[1])) if plan is None else plan.own_index(index)
+    look = functools.partial(lookup.lookup, index=index, layout=lookup.COLUMNS, plan=plan)
+    scene, inner = copy.copy(sc), copy.copy(info)
+    scene.texture = _Namespace(texture=look(sc.texture.texture), background_color=sc.texture.background_color,
+                               confidence_value_of_point=look(sc.texture.confidence_value_of_point.reshape(1, -1)))
+    scene.point_cloud_cuda = _Namespace(t_position=points.t_position, t_point_size=points.t_point_size, t_index=own)
+    inner.scene = scene
+    return inner
+
+
 def BlendPointCloud(info: NeuralRenderInfo):
     """Render the scene into a batch of image pyramids (RenderInfo.cpp:27-40)."""
+    if info.params.shared_texels_in_order:
+        info = _with_own_texels(info)
     sc = info.scene
     inputs = (sc.texture.texture, sc.texture.background_color, sc.point_cloud_cuda.t_position, sc.poses.tangent_poses,
               sc.intrinsics.intrinsics, sc.texture.confidence_value_of_point, sc.dynamic_refinement_t,
@@ -514,6 +543,13 @@ class NeuralScene:
         self.poses = _Namespace(poses_se3=poses_se3, tangent_poses=tangent_poses)
         self.intrinsics = _Namespace(intrinsics=intrinsics)
         self.dynamic_refinement_t = torch.zeros(1, device=dev)
+        self.texel_plan = None
+
+    def plan_texels(self):
+        """Keeps the order of the points by their texels for RenderParams.shared_texels_in_order; to be called again after
+        t_index or the number of texels has changed (an old plan is refused)."""
+        from . import lookup
+        self.texel_plan = lookup.lookup_plan(self.point_cloud_cuda.t_index, int(self.texture.texture.shape[1]))
 
     @staticmethod
     def from_arrays(scene, device="cuda", requires_grad=False):
