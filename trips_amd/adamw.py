@@ -7,65 +7,43 @@ step counts, so that a step may be captured into a HIP graph.
 
 A graph's backward pass must not be captured while an eager graph of the same leaves is alive (torch ends the process).
 """
+import functools
 import math
-import struct
 
 import torch
 from torch.autograd import _profiler_enabled
-from torch.autograd.graph import increment_version as _increment_version
 from torch.optim import optimizer as _optimizer
 
-from . import abi
-from .renderer import get_context
+from . import _lib, abi
+from .renderer import _stream_ptr, get_context
 
-_DTYPES = {torch.float32: abi.TRIPS_DTYPE_F32, torch.bfloat16: abi.TRIPS_DTYPE_BF16, torch.float16: abi.TRIPS_DTYPE_F16}
-_pack_tensor, _pack_options = struct.Struct("8Qq4i").pack, struct.Struct("5d").pack  # TripsAdamWTensor up to `lr`, and from there
-_pack_grad = struct.Struct("Qqi4x").pack                                             # TripsGradTensor
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _MOMENTS = {8: (torch.float8_e4m3fn, torch.float8_e5m2), 32: (torch.float32, torch.float32)}
 
 
-def _contiguous(g):
-    if g.is_sparse:
-        _refuse(None, g, 0)
-    return g.detach().contiguous()
-
-
-def _refuse(p, g, device):
-    """Says what is wrong with a parameter (or None) and its gradient."""
-    if g.is_sparse:
-        raise RuntimeError("sparse gradients are not supported")
-    if g.dtype not in _DTYPES:
-        raise RuntimeError(f"gradients are float32, bfloat16 or float16, not {g.dtype}")
-    if p is not None and (p.dtype not in _DTYPES or not p.is_contiguous()):
-        raise RuntimeError("AdamW needs contiguous float32, bfloat16 or float16 parameters")
-    if p is not None and g.numel() != p.numel():
-        raise RuntimeError(f"a gradient of {g.numel()} elements for a parameter of {p.numel()}")
-    if device < 0:
-        raise RuntimeError("the kernels need tensors on a GPU: there is no CPU implementation")
-    raise RuntimeError("all tensors of a call must be on one device")
+@functools.lru_cache(maxsize=None)
+def _host():
+    """The extension that collects what the C ABI takes of each tensor."""
+    _lib.load()
+    try:
+        from . import _trips_host
+    except ImportError as e:
+        raise RuntimeError("trips_amd/_trips_host.so is missing: build it with `python -m trips_amd.build`") from e
+    return _trips_host
 
 
 def grad_norm(grads, max_norm=0.0, loss_scale=1.0):
     """[norm, factor] of a list of gradients as a float32 tensor on their device: the root of the sum of all their squares
     divided by loss_scale, and what gradients are multiplied by to undo loss_scale and to clip their norm at max_norm
     (0: no clipping); the factor is NaN where the norm is not finite. Nothing is read back. AdamW.step() takes it as `grad_norm`."""
-    table, temporary, device = [], [], None
-    for g in grads:
-        dtype, index = _DTYPES.get(g.dtype), g.get_device()
-        if device is None:
-            device = index
-        if dtype is None or index < 0 or index != device:
-            _refuse(None, g, device)
-        if not g.is_contiguous():
-            g = _contiguous(g)
-            temporary.append(g)
-        table.append(_pack_grad(g.data_ptr(), g.numel(), dtype))
-    if not table:
+    table = _host().NormTable()
+    count, device = table.collect(grads)
+    if not count:
         raise ValueError("grad_norm of no gradients")
     ctx = get_context(device)
-    device = ctx.device
-    out = torch.empty(2, dtype=torch.float32, device=device)
-    ctx.grad_norm(b"".join(table), len(table), max_norm, loss_scale, out, ctx.alloc_bytes(abi.TRIPS_GRAD_NORM_WORKSPACE_BYTES))
+    out = torch.empty(2, dtype=torch.float32, device=ctx.device)
+    _lib.check(table.norm(ctx.ctx.value, max_norm, loss_scale, out, ctx.alloc_bytes(abi.TRIPS_GRAD_NORM_WORKSPACE_BYTES),
+                          _stream_ptr(ctx.device)))
     return out
 
 
@@ -150,44 +128,14 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        # (An attribute or a call costs 50 to 100 ns, of which a tensor takes a score; what a check finds is said in _refuse.)
-        table, params, temporary, device, copies, states, dtypes = [], [], [], None, self._copies, self.state, _DTYPES
-        for group in self.param_groups:
-            options = _pack_options(group["lr"], *group["betas"], group["eps"], group["weight_decay"])
-            for p in group["params"]:
-                g = p.grad if grads is None else grads.get(p)
-                if g is None:
-                    continue
-                n, index = p.numel(), p.get_device()
-                weight_dtype, grad_dtype = dtypes.get(p.dtype), dtypes.get(g.dtype)
-                if device is None:
-                    device = index
-                if weight_dtype is None or grad_dtype is None or index < 0 or index != device or g.get_device() != index \
-                        or g.numel() != n or not p.is_contiguous():
-                    _refuse(p, g, device)
-                if not g.is_contiguous():
-                    g = _contiguous(g)
-                    temporary.append(g)
-                st = states.get(p) or self._make_state(p, group)
-                if "first_scale" in st:
-                    first_scale, second_scale, bits = st["first_scale"].data_ptr(), st["second_scale"].data_ptr(), 8
-                else:
-                    first_scale, second_scale, bits = 0, 0, 32
-                copy_at, copy_dtype = 0, 0
-                if copies:
-                    copy = copies.get(p)
-                    if copy is not None:
-                        copy_at, copy_dtype = copy.data_ptr(), dtypes[copy.dtype]
-                params.append(p)
-                table += (_pack_tensor(p.data_ptr(), g.data_ptr(), st["first_moment"].data_ptr(), st["second_moment"].data_ptr(),
-                                       first_scale, second_scale, copy_at, st["step"].data_ptr(), n, weight_dtype, grad_dtype,
-                                       copy_dtype, bits), options)
-        if not params:
+        table = _host().StepTable()
+        count, device = table.collect(self.param_groups, self.state, self._copies, grads, self._make_state)
+        if not count:
             return loss
         ctx = get_context(device)
-        if self._workspace is None or self._workspace.device != ctx.device or self._workspace_for < len(params):
-            self._workspace = ctx.alloc_bytes(ctx.adamw_workspace_size(len(params)))
-            self._workspace_for = len(params)
+        if self._workspace is None or self._workspace.device != ctx.device or self._workspace_for < count:
+            self._workspace = ctx.alloc_bytes(ctx.adamw_workspace_size(count))
+            self._workspace_for = count
             self._norm = torch.empty(2, dtype=torch.float32, device=ctx.device)
         max_norm = self.max_grad_norm or 0.0
         compute = grad_norm is None and (max_norm > 0 or self.skip_nonfinite)
@@ -195,11 +143,8 @@ class AdamW(torch.optim.Optimizer):
                                       or not grad_norm.is_contiguous()):
             raise ValueError("grad_norm: two float32 numbers on the parameters' device expected")
         self.grad_norm = self._norm if compute else grad_norm
-        options = abi.TripsAdamWOptions(abi.TRIPS_ABI_VERSION, self.seed & 0xFFFFFFFF,
-                                        None if self.grad_norm is None else self.grad_norm.data_ptr(), int(compute),
-                                        max_norm if compute else 0.0, self.loss_scale)
-        ctx.adamw_step(b"".join(table), len(params), options, self._workspace)
-        _increment_version(params)  # (a backward pass that needs the old values raises)
+        _lib.check(table.step(ctx.ctx.value, self.seed & 0xFFFFFFFF, self.grad_norm, compute, max_norm if compute else 0.0, self.loss_scale,
+                              self._workspace, _stream_ptr(ctx.device)))
         return loss
 
     @torch.no_grad()

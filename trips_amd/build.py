@@ -58,11 +58,11 @@ def build(verbose=False, incremental=False):
 
 SHIM_DIR = os.path.join(CSRC, "torch_shim")
 SHIM_LIB = os.path.join(HERE, "_trips_torch.so")
+HOST_LIB = os.path.join(HERE, "_trips_host.so")
 
 
-def build_torch_shim(verbose=False):
-    """Builds the libtorch host side (PointRender / NeuralRenderInfo / MyAdam in C++) with a pybind11 test driver.
-    Plain g++: the shim holds no device code, it only calls the C ABI of libtrips_splat.so."""
+def _torch_flags(name):
+    """(compiler flags, linker flags) of a libtorch extension that calls the C ABI of libtrips_splat.so."""
     import sysconfig
 
     import torch
@@ -71,31 +71,53 @@ def build_torch_shim(verbose=False):
     inc = [f"-I{p}" for p in ce.include_paths()] + [f"-I{sysconfig.get_paths()['include']}", "-I/opt/rocm/include"]
     abi_flag = f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
     flags = (["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-variable", abi_flag, "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-              "-DTORCH_EXTENSION_NAME=_trips_torch", "-DTORCH_API_INCLUDE_EXTENSION_H"] + inc)
-    sources = ("trips_torch.cpp", "trips_unet_torch.cpp", "trips_scene_io.cpp", "trips_torch_py.cpp")
+              f"-DTORCH_EXTENSION_NAME={name}", "-DTORCH_API_INCLUDE_EXTENSION_H"] + inc)
+    return flags, [f"-L{tlib}", f"-L{HERE}", "-ltrips_splat", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
+                   "-ltorch_python", f"-Wl,-rpath,{tlib}", "-Wl,-rpath,$ORIGIN"]
+
+
+def _build_torch_extension(name, sources, lib, verbose, incremental=False):
+    """Plain g++, one process per translation unit, side by side: these hold no device code."""
+    flags, libs = _torch_flags(name)
     objdir = os.path.join(SHIM_DIR, "_obj")
     os.makedirs(objdir, exist_ok=True)
-    procs = []
-    for f in sources:  # one compiler process per translation unit, side by side
-        obj = os.path.join(objdir, f.replace(".cpp", ".o"))
-        cmd = ["g++"] + flags + ["-c", os.path.join(SHIM_DIR, f), "-o", obj]
+    include = os.path.join(HERE, "..", "include")
+    headers = [os.path.join(d, f) for d in (SHIM_DIR, include) for f in os.listdir(d) if f.endswith(".h")]
+    newest_header = max(os.path.getmtime(h) for h in headers)
+    procs, objs = [], []
+    for f in sources:
+        path, obj = os.path.join(SHIM_DIR, f), os.path.join(objdir, f.replace(".cpp", ".o"))
+        objs.append(obj)
+        if incremental and os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(path), newest_header):
+            continue
+        cmd = ["g++"] + flags + ["-c", path, "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
-        procs.append((cmd, obj, subprocess.Popen(cmd)))
-    for cmd, obj, pr in procs:
+        procs.append((cmd, subprocess.Popen(cmd)))
+    for cmd, pr in procs:
         if pr.wait() != 0:
             raise subprocess.CalledProcessError(pr.returncode, cmd)
-    link = (["g++", "-shared"] + [obj for _, obj, _ in procs] +
-            [f"-L{tlib}", f"-L{HERE}", "-ltrips_splat", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
-             "-ltorch_python", f"-Wl,-rpath,{tlib}", "-Wl,-rpath,$ORIGIN", "-o", SHIM_LIB])
+    link = ["g++", "-shared"] + objs + libs + ["-o", lib]
     if verbose:
         print(" ".join(link), flush=True)
     subprocess.check_call(link)
-    return SHIM_LIB
+    return lib
+
+
+def build_host(verbose=False, incremental=False):
+    """Builds _trips_host.so, the host side of trips_amd/adamw.py; after build(), whose library it links."""
+    return _build_torch_extension("_trips_host", ("trips_host.cpp",), HOST_LIB, verbose, incremental)
+
+
+def build_torch_shim(verbose=False):
+    """Builds the libtorch host side (PointRender / NeuralRenderInfo / MyAdam in C++) with a pybind11 test driver."""
+    sources = ("trips_torch.cpp", "trips_unet_torch.cpp", "trips_scene_io.cpp", "trips_torch_py.cpp")
+    return _build_torch_extension("_trips_torch", sources, SHIM_LIB, verbose)
 
 
 if __name__ == "__main__":
     build(verbose=True, incremental="--incremental" in sys.argv)
     print(LIB)
+    print(build_host(verbose=True, incremental="--incremental" in sys.argv))
     if "--shim" in sys.argv:
         print(build_torch_shim(verbose=True))

@@ -1,0 +1,188 @@
+// The host side of an optimiser step and of the gradients' norm for Python: what the C ABI takes of each tensor, collected from
+// the objects that torch keeps. In Python a tensor's score of attributes and checks took 1.3 to 2 us, more than its share of the
+// kernels' time in a step over a net (18 tensors 31 us, 40 with copies 80; here 5 and 9).
+#include <torch/csrc/DynamicTypes.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/extension.h>
+
+#include <string>
+#include <vector>
+
+#include "../../../include/trips_optim.h"
+
+namespace py = pybind11;
+
+namespace
+{
+// TRIPS_DTYPE_* of a tensor, or -1
+int dtype_of(const at::Tensor& t)
+{
+    switch (t.scalar_type())
+    {
+        case at::kFloat: return TRIPS_DTYPE_F32;
+        case at::kBFloat16: return TRIPS_DTYPE_BF16;
+        case at::kHalf: return TRIPS_DTYPE_F16;
+        default: return -1;
+    }
+}
+
+const at::Tensor& tensor_of(PyObject* o, const char* what)
+{
+    if (!o || !THPVariable_Check(o)) throw py::type_error(std::string(what) + ": a tensor expected");
+    return THPVariable_Unpack(o);
+}
+
+// One device for all tensors of a call, a GPU.
+void check_device(const at::Tensor& t, int& device)
+{
+    const int own = t.is_cuda() ? (int)t.get_device() : -1;
+    if (device >= 0 && own != device) throw std::runtime_error("all tensors of a call must be on one device");
+    if (own < 0) throw std::runtime_error("the kernels need tensors on a GPU: there is no CPU implementation");
+    device = own;
+}
+
+// A gradient as the kernels read it; a copy is kept in `temporaries`.
+at::Tensor readable(const at::Tensor& g, std::vector<at::Tensor>& temporaries)
+{
+    if (g.layout() != at::kStrided) throw std::runtime_error("sparse gradients are not supported");
+    if (dtype_of(g) < 0) throw std::runtime_error("gradients are float32, bfloat16 or float16, not " + std::string(torch::getTHPDtype(g.scalar_type())->name));
+    if (g.is_contiguous()) return g;
+    temporaries.push_back(g.detach().contiguous());
+    return temporaries.back();
+}
+
+PyObject* item(PyObject* dict, PyObject* key)  // borrowed, or NULL
+{
+    PyObject* v = PyDict_GetItemWithError(dict, key);
+    if (!v && PyErr_Occurred()) throw py::error_already_set();
+    return v;
+}
+
+// A tensor of the optimiser's state, as the kernels expect it.
+void* state_ptr(PyObject* st, const char* name, at::ScalarType type, int64_t n, int device)
+{
+    const at::Tensor& t = tensor_of(PyDict_GetItemString(st, name), name);
+    if (t.scalar_type() != type || t.numel() != n || !t.is_contiguous() || !t.is_cuda() || t.get_device() != device)
+        throw std::runtime_error(std::string("state of a parameter: ") + name + " is not a contiguous tensor of its type and size on the parameter's device");
+    return t.data_ptr();
+}
+
+class StepTable
+{
+   public:
+    // Everything that the step takes of the parameters with a gradient; (how many, their device or -1).
+    std::pair<int, int> collect(const py::list& groups, const py::dict& state, const py::dict& copies, const py::object& grads, const py::function& make_state)
+    {
+        clear();
+        int device        = -1;
+        const bool own    = grads.is_none();
+        const bool plain  = !own && PyDict_Check(grads.ptr());
+        const bool copied = !copies.empty();
+        for (const py::handle& g_ : groups)
+        {
+            const py::dict group = py::reinterpret_borrow<py::dict>(g_);
+            const py::tuple betas(group["betas"]);
+            const double lr = group["lr"].cast<double>(), b1 = betas[0].cast<double>(), b2 = betas[1].cast<double>(), eps = group["eps"].cast<double>(),
+                         decay = group["weight_decay"].cast<double>();
+            for (const py::handle& o : py::list(group["params"]))
+            {
+                const at::Tensor& p = tensor_of(o.ptr(), "a parameter");
+                at::Tensor g;
+                if (own)
+                    g = p.grad();
+                else
+                {
+                    py::object v = plain ? py::reinterpret_borrow<py::object>(item(grads.ptr(), o.ptr()) ? item(grads.ptr(), o.ptr()) : Py_None) : grads.attr("get")(o);
+                    if (!v.is_none()) g = tensor_of(v.ptr(), "a gradient");
+                }
+                if (!g.defined()) continue;
+                g = readable(g, temporaries);
+                TripsAdamWTensor t;
+                t.weight_dtype = dtype_of(p), t.grad_dtype = dtype_of(g), t.n = p.numel();
+                if (t.weight_dtype < 0 || !p.is_contiguous()) throw std::runtime_error("AdamW needs contiguous float32, bfloat16 or float16 parameters");
+                if (g.numel() != t.n) throw std::runtime_error("a gradient of " + std::to_string(g.numel()) + " elements for a parameter of " + std::to_string(t.n));
+                check_device(p, device);
+                check_device(g, device);
+                py::object st = py::reinterpret_borrow<py::object>(item(state.ptr(), o.ptr()));
+                if (!st || !PyDict_Check(st.ptr()) || PyDict_Size(st.ptr()) == 0) st = make_state(o, group);
+                const bool eight = PyDict_GetItemString(st.ptr(), "first_scale") != nullptr;
+                t.state_bits     = eight ? 8 : 32;
+                t.first_moment   = state_ptr(st.ptr(), "first_moment", eight ? at::kFloat8_e4m3fn : at::kFloat, t.n, device);
+                t.second_moment  = state_ptr(st.ptr(), "second_moment", eight ? at::kFloat8_e5m2 : at::kFloat, t.n, device);
+                const int64_t blocks = (t.n + TRIPS_MOMENT_BLOCK - 1) / TRIPS_MOMENT_BLOCK;
+                t.first_scale    = eight ? (float*)state_ptr(st.ptr(), "first_scale", at::kFloat, blocks, device) : nullptr;
+                t.second_scale   = eight ? (float*)state_ptr(st.ptr(), "second_scale", at::kFloat, blocks, device) : nullptr;
+                t.step           = (int32_t*)state_ptr(st.ptr(), "step", at::kInt, 1, device);
+                t.weights = p.data_ptr(), t.grads = g.data_ptr(), t.copy = nullptr, t.copy_dtype = 0;
+                if (PyObject* c = copied ? item(copies.ptr(), o.ptr()) : nullptr)
+                {
+                    const at::Tensor& copy = tensor_of(c, "a copy");
+                    t.copy = copy.data_ptr(), t.copy_dtype = dtype_of(copy);
+                    if (copy.numel() != t.n) throw std::runtime_error("a copy of " + std::to_string(copy.numel()) + " elements for a parameter of " + std::to_string(t.n));
+                }
+                t.lr = lr, t.beta1 = b1, t.beta2 = b2, t.eps = eps, t.weight_decay = decay;
+                tensors.push_back(t);
+                params.push_back(p);
+            }
+        }
+        return {(int)tensors.size(), device};
+    }
+
+    // trips_adamw_step for what was collected; its return value.
+    int step(uintptr_t ctx, uint32_t seed, const std::optional<at::Tensor>& grad_norm, bool compute_norm, float max_norm, float loss_scale, const at::Tensor& workspace,
+             uintptr_t stream)
+    {
+        TripsAdamWOptions o;
+        o.abi_version = TRIPS_ABI_VERSION, o.seed = seed, o.grad_norm = grad_norm ? (float*)grad_norm->data_ptr() : nullptr;
+        o.compute_norm = compute_norm, o.max_norm = max_norm, o.loss_scale = loss_scale;
+        const int rc = trips_adamw_step(reinterpret_cast<TripsCtx*>(ctx), tensors.data(), (int)tensors.size(), &o, workspace.data_ptr(), workspace.nbytes(),
+                                        reinterpret_cast<void*>(stream));
+        if (rc == TRIPS_OK)  // (a backward pass that needs the old values raises)
+            for (const at::Tensor& p : params)
+                if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+        clear();
+        return rc;
+    }
+
+    void clear() { tensors.clear(), params.clear(), temporaries.clear(); }
+
+   private:
+    std::vector<TripsAdamWTensor> tensors;
+    std::vector<at::Tensor> params, temporaries;
+};
+
+class NormTable
+{
+   public:
+    std::pair<int, int> collect(const py::iterable& grads)
+    {
+        clear();
+        int device = -1;
+        for (const py::handle& o : grads)
+        {
+            const at::Tensor g = readable(tensor_of(o.ptr(), "a gradient"), temporaries);
+            check_device(g, device);
+            tensors.push_back(TripsGradTensor{g.data_ptr(), g.numel(), dtype_of(g)});
+        }
+        return {(int)tensors.size(), device};
+    }
+    int norm(uintptr_t ctx, float max_norm, float loss_scale, const at::Tensor& out, const at::Tensor& workspace, uintptr_t stream)
+    {
+        const int rc = trips_grad_norm(reinterpret_cast<TripsCtx*>(ctx), tensors.data(), (int)tensors.size(), max_norm, loss_scale, (float*)out.data_ptr(),
+                                       workspace.data_ptr(), workspace.nbytes(), reinterpret_cast<void*>(stream));
+        clear();
+        return rc;
+    }
+    void clear() { tensors.clear(), temporaries.clear(); }
+
+   private:
+    std::vector<TripsGradTensor> tensors;
+    std::vector<at::Tensor> temporaries;
+};
+}  // namespace
+
+PYBIND11_MODULE(_trips_host, m)
+{
+    py::class_<StepTable>(m, "StepTable").def(py::init<>()).def("collect", &StepTable::collect).def("step", &StepTable::step).def("clear", &StepTable::clear);
+    py::class_<NormTable>(m, "NormTable").def(py::init<>()).def("collect", &NormTable::collect).def("norm", &NormTable::norm).def("clear", &NormTable::clear);
+}

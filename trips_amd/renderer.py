@@ -226,17 +226,6 @@ class SplatContext:
         _lib.check(self.lib.trips_adamw_workspace_size(n_tensors, C.byref(b)))
         return b.value
 
-    def adamw_step(self, tensors, n_tensors, options, workspace):
-        """tensors: an array of abi.TripsAdamWTensor, or its bytes; options: abi.TripsAdamWOptions; workspace: a device
-        tensor of adamw_workspace_size bytes."""
-        _lib.check(self.lib.trips_adamw_step(self.ctx, tensors, n_tensors, C.byref(options), _ptr(workspace), workspace.numel(),
-                                             _stream_ptr(self.device)))
-
-    def grad_norm(self, tensors, n_tensors, max_norm, loss_scale, out, workspace):
-        """tensors: an array of abi.TripsGradTensor, or its bytes; out: two device floats {norm, factor}."""
-        _lib.check(self.lib.trips_grad_norm(self.ctx, tensors, n_tensors, max_norm, loss_scale, _ptr(out), _ptr(workspace),
-                                            workspace.numel(), _stream_ptr(self.device)))
-
     # ---- table lookups ----
     def lookup_forward(self, desc, table, index, values):
         need = C.c_size_t(0)
