@@ -363,6 +363,84 @@ def test_captured_step_replays_with_its_counts(bits):
         del junk
 
 
+def test_first_steps_cannot_be_captured_and_captured_ones_outlive_larger_steps():
+    """A captured step of one parameter of two; an eager step of both in between, and much else allocated."""
+    from trips_amd.adamw import AdamW
+    params, gs = _tensors((3000, 5000), "f32", "f32", 17)
+    opt = AdamW(params, max_grad_norm=0.5)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step(grads={params[0]: gs[0]})
+        graph.capture_end()
+    torch.cuda.synchronize()
+    opt.step(grads={params[0]: gs[0]})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        opt.step(grads={params[0]: gs[0]})
+    opt.step(grads=dict(zip(params, gs)))
+    opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(4, device="cuda")) for _ in range(100)]))
+    for p in opt.param_groups[1]["params"]:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    junk = [torch.full((64, 1024), float("nan"), device="cuda") for _ in range(50)]
+    for t in (3, 4):
+        before = _state(opt, params[:1])
+        graph.replay()
+        torch.cuda.synchronize()
+        norm = np.sqrt((_numbers(gs[0]) ** 2).sum())
+        _check_step(opt, before, params[:1], gs[:1], t, factor=float(np.float32(min(1.0, 0.5 / (norm + 1e-6)))))
+    assert all(torch.isnan(j).all() for j in junk)
+
+
+def test_copies_of_the_optimiser():
+    import copy
+    from trips_amd.adamw import AdamW
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    p.grad = torch.full_like(p, 0.5)
+    opt = AdamW([p], max_grad_norm=0.25, state_bits=8, min_8bit_size=0, seed=6)
+    opt.step()
+    twin = copy.deepcopy(opt)
+    q = twin.param_groups[0]["params"][0]
+    assert q is not p and torch.equal(p, q) and (twin.max_grad_norm, twin.seed) == (0.25, 6)
+    q.grad = p.grad.clone()
+    opt.step(), twin.step()
+    assert torch.equal(p, q) and all(torch.equal(a, b) for a, b in zip(opt.moments(p), twin.moments(q)))
+
+
+def test_a_tensor_of_more_than_2_31_elements():
+    """The last elements of 2^31 + 1000, the others zeros: offsets pass 32 bits, places of the rounding wrap at 2^32 no sooner."""
+    from trips_amd.adamw import AdamW
+    n, tail = (1 << 31) + 1000, 1300
+    w, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    rng = torch.Generator().manual_seed(18)
+    w[-tail:], g[-tail:] = (torch.randn(tail, generator=rng).to(torch.bfloat16).cuda() for _ in range(2))
+    p = torch.nn.Parameter(w)
+    opt = AdamW([p], state_bits=8, max_grad_norm=1.0, seed=3)
+    before = w[-tail:].double().cpu().numpy()
+    opt.step(grads={p: g})
+    gd = g[-tail:].double().cpu().numpy()
+    norm = np.sqrt((gd ** 2).sum())
+    got = opt.grad_norm.cpu().numpy()
+    assert abs(got[0] - norm) <= 1.01 * U * norm
+    want, m, v, terms = ref.step(before, gd, np.zeros(tail), np.zeros(tail), 1, 1e-3, (0.9, 0.999), 1e-8, 1e-2, float(got[1]))
+    bound = U * (3 * np.abs(before) + 21 * terms + np.abs(want)) + _half_step(torch.bfloat16, want)
+    assert (np.abs(w[-tail:].double().cpu().numpy() - want) <= bound).all()
+    # the moments of the last whole block and of the rest, rounded by their places
+    first = n - n % 256 - 256
+    skip = tail - (n - first)
+    bits = ref.mix(np.arange(first, n, dtype=np.uint64) ^ ref.mix(3 + 0x9E3779B9))
+    for name, x, r, kind in (("first", m, bits & np.uint64(0xFFFF), (3, 7, 448.0, False)), ("second", v, bits >> np.uint64(16), (2, 15, 57344.0, True))):
+        codes, scales, margin = ref.encode(x[skip:], r.astype(np.float64), *kind)
+        assert margin > 2.0 ** -30
+        st = opt.state[p]
+        np.testing.assert_array_equal(st[name + "_scale"][-2:].cpu().numpy(), scales)
+        np.testing.assert_array_equal(st[name + "_moment"].view(torch.uint8)[first:].cpu().numpy(), codes)
+    assert not w[:100_000].any() and not w[1 << 30:(1 << 30) + 100_000].any()
+
+
 def test_another_stream():
     from trips_amd.adamw import AdamW
     params, gs = _tensors((5000, 200_000), "f32", "f32", 15)

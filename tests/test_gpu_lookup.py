@@ -323,6 +323,37 @@ def test_captured_lookup_and_gradient_replay(layout):
         torch.cuda.synchronize()
 
 
+def test_offsets_that_pass_32_bits():
+    """Tables and gradients of more than 2^32 elements: their last and first entries."""
+    texels = (1 << 22) + 5
+    index = torch.tensor([0, texels - 1, 5, texels - 1, texels, texels - 2], dtype=torch.int64, device="cuda")
+    table = torch.zeros((texels, 1024), dtype=torch.bfloat16, device="cuda")
+    for i in (0, 5, texels - 2, texels - 1):
+        table[i] = torch.arange(1024, device="cuda").remainder(13) + i % 7
+    got = lk.lookup(table, index, 2.0, lk.ROWS)
+    assert torch.equal(got[[0, 1, 2, 3, 5]], table[index[[0, 1, 2, 3, 5]]] * 2) and not got[4].any()
+    grad = got.clone()
+    del table
+    d_table = lk.lookup_backward(grad, index, texels, 1.0, lk.ROWS)
+    assert torch.equal(d_table[0], grad[0]) and torch.equal(d_table[5], grad[2]) and torch.equal(d_table[texels - 2], grad[5])
+    assert torch.equal(d_table[texels - 1], (grad[1].float() + grad[3].float()).to(torch.bfloat16))
+    assert not d_table[6:100].any() and not d_table[texels - 100:texels - 2].any()
+    del d_table
+    texels = (1 << 30) + 3
+    index = torch.tensor([texels - 1, 0, texels - 1, -1, texels, 1 << 29], dtype=torch.int32, device="cuda")
+    table = torch.zeros((5, texels), dtype=torch.float16, device="cuda")
+    table[:, texels - 1] = torch.arange(1, 6, device="cuda")
+    table[:, 0], table[:, 1 << 29] = 7, 9
+    got = lk.lookup(table, index, 0.5)
+    want = torch.stack([torch.arange(1, 6) * 0.5, torch.full((5,), 3.5), torch.arange(1, 6) * 0.5, torch.zeros(5), torch.zeros(5),
+                        torch.full((5,), 4.5)], 1).to(torch.float16).cuda()
+    assert torch.equal(got, want)
+    del table
+    d_table = lk.lookup_backward(want, index, texels, 1.0)
+    assert torch.equal(d_table[:, texels - 1], want[:, 0] * 2) and torch.equal(d_table[:, 0], want[:, 1])
+    assert torch.equal(d_table[:, 1 << 29], want[:, 5]) and not d_table[:, 1:1000].any() and not d_table[4, texels - 1000:texels - 1].any()
+
+
 def test_another_stream():
     rng = np.random.default_rng(9)
     index, grad = _index(rng, 500, 60_000, "skewed"), _matrix(rng, 4, 60_000, "f32")

@@ -58,8 +58,8 @@ class AdamW(torch.optim.Optimizer):
     over by the next step) if it was computed.
 
     State per parameter: step (int32, on the device), first_moment, second_moment, and with 8 bits first_scale and second_scale;
-    moments() gives the moments as numbers. A captured step replays with the learning rates of its capture; a step that is
-    captured must not be the first (which makes the state)."""
+    moments() gives the moments as numbers. A captured step replays with the learning rates of its capture; a parameter's first
+    step, which makes its state, cannot be captured. Steps of one optimiser must not overlap."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_size=4096,
                  max_grad_norm=0.0, skip_nonfinite=False, loss_scale=1.0, seed=0):
@@ -84,6 +84,7 @@ class AdamW(torch.optim.Optimizer):
         self.seed = seed
         self.grad_norm = None
         self._workspace = None
+        self._kept = []
         self._copies = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size))
@@ -99,6 +100,8 @@ class AdamW(torch.optim.Optimizer):
         self._copies[p] = copy
 
     def _make_state(self, p, group):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a parameter's first step makes its state and cannot be captured into a graph")
         bits = 8 if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"] else 32
         first, second = _MOMENTS[bits]
         st = self.state[p]
@@ -134,9 +137,7 @@ class AdamW(torch.optim.Optimizer):
             return loss
         ctx = get_context(device)
         if self._workspace is None or self._workspace.device != ctx.device or self._workspace_for < count:
-            self._workspace = ctx.alloc_bytes(ctx.adamw_workspace_size(count))
-            self._workspace_for = count
-            self._norm = torch.empty(2, dtype=torch.float32, device=ctx.device)
+            self._make_workspace(ctx)
         max_norm = self.max_grad_norm or 0.0
         compute = grad_norm is None and (max_norm > 0 or self.skip_nonfinite)
         if grad_norm is not None and (grad_norm.dtype != torch.float32 or grad_norm.numel() != 2 or grad_norm.device != ctx.device
@@ -146,6 +147,24 @@ class AdamW(torch.optim.Optimizer):
         _lib.check(table.step(ctx.ctx.value, self.seed & 0xFFFFFFFF, self.grad_norm, compute, max_norm if compute else 0.0, self.loss_scale,
                               self._workspace, _stream_ptr(ctx.device)))
         return loss
+
+    def _make_workspace(self, ctx):
+        # For all parameters, whichever have a gradient this time. What an earlier one was captured with stays alive with it.
+        if self._workspace is not None:
+            self._kept.append((self._workspace, self._norm))
+        self._workspace_for = sum(len(g["params"]) for g in self.param_groups)
+        self._workspace = ctx.alloc_bytes(ctx.adamw_workspace_size(self._workspace_for))
+        self._norm = torch.empty(2, dtype=torch.float32, device=ctx.device)
+
+    _OWN = ("max_grad_norm", "skip_nonfinite", "loss_scale", "seed")
+
+    def __getstate__(self):
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in self._OWN}}
+
+    def __setstate__(self, state):
+        # (a copy has its own workspace, and no copies of parameters yet)
+        self.grad_norm, self._workspace, self._kept, self._copies = None, None, [], {}
+        super().__setstate__(state)
 
     @torch.no_grad()
     def moments(self, p):

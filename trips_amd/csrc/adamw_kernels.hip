@@ -5,6 +5,7 @@
 // kernel's arguments; a workgroup finds the tensor of each of its tiles there.
 #include <float.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "abi_common.h"
@@ -21,7 +22,8 @@ constexpr int kGroups      = 8;    // different sets of options among them
 constexpr int kStepTensors = 4096; // tensors of a step's launch
 constexpr int kTileOptim   = 1024; // elements of a tile: four wavefronts with a block of 256 each
 constexpr int kStepGroups  = 2048; // workgroups of a step with a tile each
-constexpr int kStepRun     = 2;    // tiles of a workgroup, one behind the other, where there are more tiles
+constexpr int kStepRun     = 2;    // tiles of a workgroup, one behind the other, where there are more tiles (60M elements in
+                                   // 8 bits, us: 1 tile 181, 2 169, 4 178, 8 188; 2048 workgroups in turn 194. In 32: 297 to 305, 331)
 constexpr int kNormTensors = 140; // of a launch: 4 KB of arguments
 constexpr int kNormTile    = 4096; // elements of a tile of the norm
 constexpr int kNormGroups  = 1024; // workgroups of the norm = partial sums
@@ -699,7 +701,7 @@ hipError_t launch_steps(const TripsAdamWTensor* tensors, int n, const TripsAdamW
             }
             if (tiles == 0) continue;
             p.tiles     = (uint32_t)tiles;
-            p.run       = tiles > kStepGroups ? kStepRun : 1u;
+            p.run       = tiles <= kStepGroups ? 1u : (uint32_t)std::max<long long>(kStepRun, (tiles >> 23) + 1);  // (less than 2^32 threads)
             const int g = (int)((tiles + p.run - 1) / p.run);
             const int wd = kind / 8, gd = kind / 2 % 4, bits = kind & 1 ? 8 : 32;
             if (wd == TRIPS_DTYPE_F32)

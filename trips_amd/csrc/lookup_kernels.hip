@@ -663,8 +663,11 @@ __global__ __launch_bounds__(kWideThreads) void lookup_tiles_kernel(const GradPa
     float sum[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[e] = 0.f;
-    if (s_in && c < p.channels) add_rows<D, V>(p, from + r, to, blockDim.x >> p.lanes_log2, c, OUT_COLUMNS ? V : min(V, p.channels - c), sum);
-    add_threads(sum, s, p.lanes_log2);
+    if (s_in)
+    {
+        if (c < p.channels) add_rows<D, V>(p, from + r, to, blockDim.x >> p.lanes_log2, c, OUT_COLUMNS ? V : min(V, p.channels - c), sum);
+        add_threads(sum, s, p.lanes_log2);
+    }
     if ((int)threadIdx.x < lanes && c < p.padded)
     {
 #pragma unroll
