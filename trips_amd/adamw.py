@@ -7,7 +7,6 @@ step counts, so that a step may be captured into a HIP graph.
 
 A graph's backward pass must not be captured while an eager graph of the same leaves is alive (torch ends the process).
 """
-import functools
 import math
 
 import torch
@@ -15,21 +14,11 @@ from torch.autograd import _profiler_enabled
 from torch.optim import optimizer as _optimizer
 
 from . import _lib, abi
+from ._host import host as _host
 from .renderer import _stream_ptr, get_context
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _MOMENTS = {8: (torch.float8_e4m3fn, torch.float8_e5m2), 32: (torch.float32, torch.float32)}
-
-
-@functools.lru_cache(maxsize=None)
-def _host():
-    """The extension that collects what the C ABI takes of each tensor."""
-    _lib.load()
-    try:
-        from . import _trips_host
-    except ImportError as e:
-        raise RuntimeError("trips_amd/_trips_host.so is missing: build it with `python -m trips_amd.build`") from e
-    return _trips_host
 
 
 def grad_norm(grads, max_norm=0.0, loss_scale=1.0):

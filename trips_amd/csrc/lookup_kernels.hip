@@ -436,7 +436,8 @@ __device__ __forceinline__ uint32_t lower_bound(const T* a, uint32_t n, uint32_t
 // starts[t] = the first of the sorted keys that is t or more, for kStartsTexels texels a workgroup. Two wavefronts find the keys
 // that belong to them; where these are about as many as the texels, each key that differs from the one before is noted in LDS
 // and the texels in between take the next one's; where they are many more, each texel is searched for. ITEMS texels a thread: 8,
-// or 1 where there are more than two points a texel.
+// or 1 where there are more than two points a texel or few texels.
+constexpr int64_t kFewTexels = 1 << 18;
 template <int ITEMS>
 __global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t texels, int32_t* starts)
 {
@@ -858,7 +859,7 @@ hipError_t launch_plan(int64_t texels, int64_t points, const void* index, int in
             hipLaunchKernelGGL(sort_scatter_kernel<4>, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
         shift += p.bits;
     }
-    if (points > 2 * texels)
+    if (points > 2 * texels || texels < kFewTexels)
         hipLaunchKernelGGL(starts_kernel<1>, dim3((unsigned)(texels / 256 + 1)), dim3(256), 0, stream, p.keys_out, (uint32_t)points, (uint32_t)texels, starts);
     else
         hipLaunchKernelGGL(starts_kernel<8>, dim3((unsigned)(texels / 2048 + 1)), dim3(256), 0, stream, p.keys_out, (uint32_t)points, (uint32_t)texels, starts);

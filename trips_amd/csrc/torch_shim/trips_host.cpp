@@ -1,6 +1,6 @@
-// The host side of an optimiser step and of the gradients' norm for Python: what the C ABI takes of each tensor, collected from
-// the objects that torch keeps. In Python a tensor's score of attributes and checks took 1.3 to 2 us, more than its share of the
-// kernels' time in a step over a net (18 tensors 31 us, 40 with copies 80; here 5 and 9).
+// The host side of trips_amd/adamw.py and trips_amd/lookup.py: what the C ABI takes of each tensor, collected from the objects
+// that torch keeps. In Python a tensor's score of attributes and checks took 1.3 to 2 us, more than its share of the kernels'
+// time in a step over a net (18 tensors 32 us a step and 17 so, 40 with copies 68 and 29), and a lookup 10 us.
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/extension.h>
@@ -8,6 +8,7 @@
 #include <string>
 #include <vector>
 
+#include "../../../include/trips_lookup.h"
 #include "../../../include/trips_optim.h"
 
 namespace py = pybind11;
@@ -179,10 +180,123 @@ class NormTable
     std::vector<TripsGradTensor> tensors;
     std::vector<at::Tensor> temporaries;
 };
+
+// ---- table lookups ----
+
+void check(int rc)
+{
+    if (rc != TRIPS_OK) py::module_::import("trips_amd._lib").attr("check")(rc);
+}
+
+int index_dtype_of(const at::Tensor& index)
+{
+    if (index.scalar_type() != at::kInt && index.scalar_type() != at::kLong)
+        throw py::value_error("index: int32 or int64 expected, got " + std::string(torch::getTHPDtype(index.scalar_type())->name));
+    if (!index.is_cuda()) throw std::runtime_error("lookups need tensors on a GPU: there is no CPU implementation");
+    return index.scalar_type() == at::kInt ? TRIPS_INDEX_I32 : TRIPS_INDEX_I64;
+}
+
+// A matrix on the index's device with adjacent elements in a row (a copy of it, if need be), and the distance of its rows.
+at::Tensor rows_of(const char* name, const at::Tensor& t, const at::Tensor& index, int64_t& stride)
+{
+    if (t.dim() != 2 || dtype_of(t) < 0 || t.layout() != at::kStrided || t.device() != index.device())
+        throw py::value_error(std::string(name) + ": a float32, bfloat16 or float16 matrix on the index's device expected");
+    const at::Tensor m = t.stride(1) != 1 && t.size(1) > 1 ? t.detach().contiguous() : t;
+    stride             = m.size(0) > 1 ? m.stride(0) : m.size(1);
+    return m;
+}
+
+at::Tensor bytes(size_t n, const at::Tensor& like)
+{
+    return n ? torch::empty({(int64_t)n}, like.options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
+}
+void* data(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+void check_layout(int layout)
+{
+    if (layout != TRIPS_TABLE_COLUMNS && layout != TRIPS_TABLE_ROWS) throw py::value_error("layout: COLUMNS or ROWS expected, got " + std::to_string(layout));
+}
+
+TripsLookupDesc lookup_desc(int layout, int dtype, int index_dtype, int64_t texels, int64_t points, int64_t channels, float scale)
+{
+    TripsLookupDesc d{};
+    d.abi_version = TRIPS_ABI_VERSION, d.layout = layout, d.dtype = dtype, d.index_dtype = index_dtype;
+    d.num_texels = texels, d.num_points = points, d.num_channels = (int32_t)std::min<int64_t>(channels, INT32_MAX), d.scale = scale;
+    return d;
+}
+
+at::Tensor lookup(uintptr_t ctx, uintptr_t stream, const at::Tensor& table, const at::Tensor& index, float scale, int layout)
+{
+    int64_t stride;
+    check_layout(layout);
+    const int index_dtype = index_dtype_of(index);
+    const at::Tensor t    = rows_of("table", table, index, stride);
+    const bool columns    = layout == TRIPS_TABLE_COLUMNS;
+    const int64_t n = index.numel(), c = t.size(columns ? 0 : 1);
+    TripsLookupDesc d = lookup_desc(layout, dtype_of(t), index_dtype, t.size(columns ? 1 : 0), n, c, scale);
+    at::Tensor values = torch::empty({columns ? c : n, columns ? n : c}, t.options().requires_grad(false));
+    if (c == 0 || n == 0) return values;
+    d.table_stride = stride, d.values_stride = values.size(1);
+    size_t need = 0;
+    check(trips_lookup_workspace_size(&d, &need));
+    const at::Tensor workspace = bytes(need, t), i = index.contiguous();
+    check(trips_lookup_forward(reinterpret_cast<TripsCtx*>(ctx), &d, t.data_ptr(), i.data_ptr(), values.data_ptr(), data(workspace), need, reinterpret_cast<void*>(stream)));
+    return values;
+}
+
+std::pair<at::Tensor, at::Tensor> lookup_plan(uintptr_t ctx, uintptr_t stream, const at::Tensor& index, int64_t texels)
+{
+    const int index_dtype = index_dtype_of(index);
+    if (texels < 0) throw py::value_error("num_texels = " + std::to_string(texels));
+    size_t need = 0;
+    check(trips_lookup_plan_workspace_size(texels, index.numel(), &need));
+    const auto options = index.options().dtype(at::kInt);
+    at::Tensor order = torch::empty({index.numel()}, options), starts = torch::empty({texels + 1}, options);
+    const at::Tensor workspace = bytes(need, index), i = index.contiguous();
+    check(trips_lookup_plan(reinterpret_cast<TripsCtx*>(ctx), texels, index.numel(), i.data_ptr(), index_dtype, (int32_t*)order.data_ptr(), (int32_t*)starts.data_ptr(),
+                            data(workspace), need, reinterpret_cast<void*>(stream)));
+    return {order, starts};
+}
+
+at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& grad, const at::Tensor& index, const at::Tensor& order, const at::Tensor& starts, int64_t texels,
+                           float scale, int layout, const std::optional<at::Tensor>& out)
+{
+    int64_t stride;
+    check_layout(layout);
+    const int index_dtype = index_dtype_of(index);
+    const at::Tensor g    = rows_of("grad", grad, index, stride);
+    const bool columns    = layout == TRIPS_TABLE_COLUMNS;
+    const int64_t n = g.size(columns ? 1 : 0), c = g.size(columns ? 0 : 1);
+    if (n != index.numel()) throw py::value_error("grad: " + std::to_string(n) + " points, index has " + std::to_string(index.numel()));
+    TripsLookupDesc d     = lookup_desc(layout, dtype_of(g), index_dtype, texels, n, c, scale);
+    const int64_t rows = columns ? c : texels, row = columns ? texels : c;
+    at::Tensor d_table;
+    if (out)
+    {
+        d_table = *out;
+        if (d_table.dim() != 2 || d_table.size(0) != rows || d_table.size(1) != row || d_table.scalar_type() != g.scalar_type() || d_table.device() != g.device() ||
+            (d_table.stride(1) != 1 && row > 1) || (rows > 1 && d_table.stride(0) < row))
+            throw py::value_error("out: a tensor of the gradient's type of " + std::to_string(rows) + " x " + std::to_string(row) + " with adjacent elements in a row expected");
+    }
+    else
+        d_table = torch::empty({rows, row}, g.options().requires_grad(false));
+    if (rows == 0 || row == 0) return d_table;
+    d.accumulate = out.has_value(), d.table_stride = rows > 1 ? d_table.stride(0) : row, d.values_stride = stride;
+    size_t need = 0;
+    check(trips_lookup_backward_workspace_size(&d, &need));
+    const at::Tensor workspace = bytes(need, g);
+    check(trips_lookup_backward(reinterpret_cast<TripsCtx*>(ctx), &d, g.data_ptr(), (const int32_t*)order.data_ptr(), (const int32_t*)starts.data_ptr(), d_table.data_ptr(),
+                                data(workspace), need, reinterpret_cast<void*>(stream)));
+    if (out && !d_table.is_inference()) d_table.unsafeGetTensorImpl()->bump_version();
+    return d_table;
+}
 }  // namespace
 
 PYBIND11_MODULE(_trips_host, m)
 {
     py::class_<StepTable>(m, "StepTable").def(py::init<>()).def("collect", &StepTable::collect).def("step", &StepTable::step).def("clear", &StepTable::clear);
     py::class_<NormTable>(m, "NormTable").def(py::init<>()).def("collect", &NormTable::collect).def("norm", &NormTable::norm).def("clear", &NormTable::clear);
+    m.def("lookup", &lookup);
+    m.def("lookup_plan", &lookup_plan);
+    m.def("lookup_backward", &lookup_backward);
 }

@@ -9,38 +9,18 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import abi
-from .renderer import get_context
+from ._host import host as _host
+from .renderer import _stream_ptr, get_context
 
 COLUMNS, ROWS = abi.TRIPS_TABLE_COLUMNS, abi.TRIPS_TABLE_ROWS
-_DTYPES = {torch.float32: abi.TRIPS_DTYPE_F32, torch.bfloat16: abi.TRIPS_DTYPE_BF16, torch.float16: abi.TRIPS_DTYPE_F16}
-_INDEX_DTYPES = {torch.int32: abi.TRIPS_INDEX_I32, torch.int64: abi.TRIPS_INDEX_I64}
 
 
-def _check_index(index):
-    if index.dtype not in _INDEX_DTYPES:
-        raise ValueError(f"index: int32 or int64 expected, got {index.dtype}")
+def _where(index):
+    """The context of the index's device and its current stream, as the extension takes them (it refuses other devices)."""
     if index.device.type != "cuda":
-        raise RuntimeError("lookups need tensors on a GPU: there is no CPU implementation")
-
-
-def _rows_of(name, t, device):
-    """t [A, B] with adjacent elements in a row, and the distance of its rows."""
-    if t.dim() != 2 or t.dtype not in _DTYPES or t.device != device:
-        raise ValueError(f"{name}: a float32, bfloat16 or float16 matrix on the index's device expected, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
-    if (t.stride(1) != 1 and t.shape[1] > 1) or t.stride(0) < 0:
-        t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _desc(layout, dtype, index_dtype, texels, points, channels, table_stride, values_stride, scale, accumulate=False):
-    return abi.TripsLookupDesc(abi.TRIPS_ABI_VERSION, layout, _DTYPES[dtype], _INDEX_DTYPES[index_dtype], texels, points, channels,
-                               int(accumulate), table_stride, values_stride, scale)
-
-
-def _check_layout(layout):
-    if layout not in (COLUMNS, ROWS):
-        raise ValueError(f"layout: COLUMNS or ROWS expected, got {layout!r}")
+        return 0, 0
+    ctx = get_context(index.device)
+    return ctx.ctx.value, _stream_ptr(ctx.device)
 
 
 class LookupPlan:
@@ -61,10 +41,10 @@ class LookupPlan:
             raise ValueError(f"the plan is for {self.order.numel()} points and {self.starts.numel() - 1} texels, not for "
                              f"{index.numel()} and {texels}")
         own = self.index
-        if own is not None and (own.data_ptr() != index.data_ptr() or own.dtype != index.dtype or own.stride() != index.stride()
+        if own is not None and (own.data_ptr() != index.data_ptr() or own.dtype != index.dtype
+                                or (own.stride() != index.stride() and not (own.is_contiguous() and index.is_contiguous()))
                                 or (None if index.is_inference() else index._version) != self.version):
             raise ValueError("the plan was made of another index, or the index was changed since")
-
 
     def own_index(self, index):
         """own_index() of the plan's index, made once."""
@@ -80,66 +60,28 @@ def own_index(index, num_texels):
     return torch.where((index >= 0) & (index < num_texels), own, -1)
 
 
-@torch.no_grad()
 def lookup_plan(index, num_texels):
     """The order of the points by their texel. Indexes outside [0, num_texels) come last and count for no texel."""
-    _check_index(index)
-    if num_texels < 0:
-        raise ValueError(f"num_texels = {num_texels}")
-    ctx = get_context(index.device)
-    order = torch.empty(index.numel(), dtype=torch.int32, device=index.device)
-    starts = torch.empty(num_texels + 1, dtype=torch.int32, device=index.device)
-    ctx.lookup_plan(num_texels, index.contiguous(), _INDEX_DTYPES[index.dtype], order, starts)
-    return LookupPlan(order, starts, index)
+    return LookupPlan(*_host().lookup_plan(*_where(index), index, num_texels), index)
 
 
-def _forward(table, index, scale, layout):
-    table, stride = _rows_of("table", table, index.device)
-    columns = layout == COLUMNS
-    channels, texels = (table.shape[0], table.shape[1]) if columns else (table.shape[1], table.shape[0])
-    points = index.numel()
-    values = torch.empty((channels, points) if columns else (points, channels), dtype=table.dtype, device=index.device)
-    if channels and points:
-        desc = _desc(layout, table.dtype, index.dtype, texels, points, channels, stride, values.shape[1], scale)
-        get_context(index.device).lookup_forward(desc, table, index.contiguous(), values)
-    return values
-
-
-@torch.no_grad()
 def lookup_backward(grad, index, num_texels, scale=1.0, layout=COLUMNS, plan=None, out=None):
     """The table's gradient from that of its looked-up values: [C, T] from [C, N], or [T, C] from [N, C]. plan: lookup_plan of the
     index, where a program keeps it (it is made here otherwise). out: a table gradient to add to, instead of a new one."""
-    _check_layout(layout)
-    _check_index(index)
-    grad, grad_stride = _rows_of("grad", grad, index.device)
-    columns = layout == COLUMNS
-    channels, points = (grad.shape[0], grad.shape[1]) if columns else (grad.shape[1], grad.shape[0])
-    if points != index.numel():
-        raise ValueError(f"grad: {points} points, index has {index.numel()}")
     if plan is None:
         plan = lookup_plan(index, num_texels)
-    plan.check(index, num_texels)
-    shape = (channels, num_texels) if columns else (num_texels, channels)
-    if out is None:
-        d_table, accumulate = torch.empty(shape, dtype=grad.dtype, device=grad.device), False
     else:
-        if tuple(out.shape) != shape or out.dtype != grad.dtype or out.device != grad.device or (out.stride(1) != 1 and shape[1] > 1) \
-                or (shape[0] > 1 and out.stride(0) < shape[1]):
-            raise ValueError(f"out: a {grad.dtype} tensor {shape} with adjacent elements in a row expected")
-        d_table, accumulate = out, True
-    if channels and num_texels:
-        desc = _desc(layout, grad.dtype, index.dtype, num_texels, points, channels, d_table.stride(0) if shape[0] > 1 else shape[1],
-                     grad_stride, scale, accumulate)
-        get_context(index.device).lookup_backward(desc, grad, plan.order, plan.starts, d_table)
-    return d_table
+        plan.check(index, num_texels)
+    return _host().lookup_backward(*_where(index), grad.detach(), index, plan.order, plan.starts, num_texels, scale, layout, out)
 
 
 class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, index, scale, layout, plan):
+        values = _host().lookup(*_where(index), table.detach(), index, scale, layout)
         ctx.save_for_backward(index)
         ctx.args = (table.shape[1] if layout == COLUMNS else table.shape[0], scale, layout, plan)
-        return _forward(table, index, scale, layout)
+        return values
 
     @staticmethod
     @once_differentiable
@@ -153,12 +95,8 @@ def lookup(table, index, scale=1.0, layout=COLUMNS, plan=None):
     """scale times the entries of the table that the index names: [C, N] from a table [C, T] (COLUMNS, a scene's texture), or
     [N, C] from [T, C] (ROWS); N = index.numel(). Zeros where an index is outside the table (padding). Differentiable in the
     table; plan: lookup_plan of the index, for the gradient, where a program keeps it."""
-    _check_layout(layout)
-    _check_index(index)
-    if table.dim() != 2:
-        raise ValueError(f"table: a matrix expected, got {tuple(table.shape)}")
-    if plan is not None:
+    if plan is not None and table.dim() == 2:
         plan.check(index, table.shape[1] if layout == COLUMNS else table.shape[0])
-    if torch.is_grad_enabled() and table.requires_grad:
-        return _Lookup.apply(table, index, float(scale), layout, plan)
-    return _forward(table.detach(), index, scale, layout)
+    if table.requires_grad and torch.is_grad_enabled():
+        return _Lookup.apply(table, index, scale, layout, plan)
+    return _host().lookup(*_where(index), table.detach(), index, scale, layout)

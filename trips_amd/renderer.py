@@ -226,28 +226,6 @@ class SplatContext:
         _lib.check(self.lib.trips_adamw_workspace_size(n_tensors, C.byref(b)))
         return b.value
 
-    # ---- table lookups ----
-    def lookup_forward(self, desc, table, index, values):
-        need = C.c_size_t(0)
-        _lib.check(self.lib.trips_lookup_workspace_size(C.byref(desc), C.byref(need)))
-        workspace = self.alloc_bytes(need.value) if need.value else None
-        _lib.check(self.lib.trips_lookup_forward(self.ctx, C.byref(desc), _ptr(table), _ptr(index), _ptr(values), _ptr(workspace),
-                                                 need.value, _stream_ptr(self.device)))
-
-    def lookup_plan(self, num_texels, index, index_dtype, order, starts):
-        need = C.c_size_t(0)
-        _lib.check(self.lib.trips_lookup_plan_workspace_size(num_texels, index.numel(), C.byref(need)))
-        workspace = self.alloc_bytes(need.value)
-        _lib.check(self.lib.trips_lookup_plan(self.ctx, num_texels, index.numel(), _ptr(index), index_dtype, _ptr(order), _ptr(starts),
-                                              _ptr(workspace), workspace.numel(), _stream_ptr(self.device)))
-
-    def lookup_backward(self, desc, d_values, order, starts, d_table):
-        need = C.c_size_t(0)
-        _lib.check(self.lib.trips_lookup_backward_workspace_size(C.byref(desc), C.byref(need)))
-        workspace = self.alloc_bytes(need.value) if need.value else None
-        _lib.check(self.lib.trips_lookup_backward(self.ctx, C.byref(desc), _ptr(d_values), _ptr(order), _ptr(starts), _ptr(d_table),
-                                                  _ptr(workspace), need.value, _stream_ptr(self.device)))
-
     def apply_tangent(self, tangent, poses_se3):
         assert tangent.dtype == torch.float64 and poses_se3.dtype == torch.float64
         assert tangent.is_contiguous() and poses_se3.is_contiguous()
