@@ -516,10 +516,9 @@ __global__ __launch_bounds__(256) void grad_squares_kernel(const NormTable tab)
     if (threadIdx.x == 0) tab.sums[blockIdx.x] = tab.add ? tab.sums[blockIdx.x] + sum : sum;
 }
 
-__device__ __forceinline__ void write_norm(const double* sums, int n, float max_norm, float loss_scale, float* out, double* s)
+// `sum`: this thread's share of the squares
+__device__ __forceinline__ void write_norm(double sum, float max_norm, float loss_scale, float* out, double* s)
 {
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < n; i += 256) sum += sums[i];
     sum = block_sum(sum, s);
     if (threadIdx.x == 0)
     {
@@ -534,36 +533,47 @@ __device__ __forceinline__ void write_norm(const double* sums, int n, float max_
 __global__ __launch_bounds__(256) void grad_norm_kernel(const double* sums, int n, float max_norm, float loss_scale, float* out)
 {
     __shared__ double s[4];
-    write_norm(sums, n, max_norm, loss_scale, out, s);
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < n; i += 256) sum += sums[i];
+    write_norm(sum, max_norm, loss_scale, out, s);
 }
 
 // Before a step, one workgroup: the norm of the squares, if they were summed for it; the step counts go on; the step's table.
+// All of it waits on memory and on double precision's long chains: what the tensors' rates need comes first, beside the sums.
 __global__ __launch_bounds__(256) void adamw_begin_kernel(const StepTable tab)
 {
     __shared__ double s[4];
+    const uint32_t i    = threadIdx.x;
+    const bool mine     = i < tab.n;
+    const StepTensor& T = tab.t[mine ? i : 0];
+    uint32_t t          = 0;
+    if (mine) t = (uint32_t)*T.step + 1u;
+    double sum = 0.0;
+    if (tab.sums)
+        for (uint32_t k = i; k < tab.groups; k += 256) sum += tab.sums[k];
+    StepEntry e;
+    if (mine)
+    {
+        const StepOptions& o = tab.o[T.group];
+        e.w = T.w, e.g = T.g, e.m = T.m, e.v = T.v, e.ms = T.ms, e.vs = T.vs, e.copy = T.copy, e.n = T.n;
+        e.b1 = o.beta1, e.c1 = 1.0 - o.beta1, e.b2 = o.beta2, e.c2 = 1.0 - o.beta2;
+        e.fb1 = (float)e.b1, e.fc1 = (float)e.c1, e.fb2 = (float)e.b2, e.fc2 = (float)e.c2;
+        e.keep = (float)(1.0 - o.lr * o.decay);
+        e.rate = (float)(o.lr / (1.0 - power(o.beta1, t)));
+        e.root = (float)(1.0 / sqrt(1.0 - power(o.beta2, t)));
+        e.eps  = (float)o.eps;
+        e.key  = mix(tab.seed + t * 0x9E3779B9u);
+        e.first_block = T.first_block, e.copy_dtype = T.copy_dtype, e.unused = 0;
+    }
     if (tab.sums)
     {
-        write_norm(tab.sums, (int)tab.groups, tab.max_norm, tab.loss_scale, tab.norm, s);
+        write_norm(sum, tab.max_norm, tab.loss_scale, tab.norm, s);
         __syncthreads();
     }
-    const uint32_t i = threadIdx.x;
-    if (i >= tab.n) return;
     // (written by this workgroup, or by another launch)
     if (tab.norm && !(fabsf(__hip_atomic_load(tab.norm + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)) <= FLT_MAX)) return;
-    const StepTensor& T   = tab.t[i];
-    const StepOptions& o  = tab.o[T.group];
-    const uint32_t t      = (uint32_t)*T.step + 1u;
-    *T.step               = (int32_t)t;
-    StepEntry e;
-    e.w = T.w, e.g = T.g, e.m = T.m, e.v = T.v, e.ms = T.ms, e.vs = T.vs, e.copy = T.copy, e.n = T.n;
-    e.b1 = o.beta1, e.c1 = 1.0 - o.beta1, e.b2 = o.beta2, e.c2 = 1.0 - o.beta2;
-    e.fb1 = (float)e.b1, e.fc1 = (float)e.c1, e.fb2 = (float)e.b2, e.fc2 = (float)e.c2;
-    e.keep = (float)(1.0 - o.lr * o.decay);
-    e.rate = (float)(o.lr / (1.0 - power(o.beta1, t)));
-    e.root = (float)(1.0 / sqrt(1.0 - power(o.beta2, t)));
-    e.eps  = (float)o.eps;
-    e.key  = mix(tab.seed + t * 0x9E3779B9u);
-    e.first_block = T.first_block, e.copy_dtype = T.copy_dtype, e.unused = 0;
+    if (!mine) return;
+    *T.step            = (int32_t)t;
     tab.entries[i]     = e;
     tab.first_tiles[i] = T.first_tile;
 }

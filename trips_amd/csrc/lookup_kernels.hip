@@ -520,7 +520,7 @@ struct GradParams
     float* tiles;     // [points / tile, padded] sums of the tiles that one texel fills (zeros for the others)
     uint32_t* listed;  // texels for the second kernel: how many, then 63 words on, which
     long long texels, table_stride, row;
-    uint32_t points, tile, capacity;
+    uint32_t points, tile, capacity, longest;  // longest: points of a texel that is not listed
     int channels, padded, lanes_log2, accumulate;
     float scale;
 };
@@ -599,7 +599,7 @@ __global__ __launch_bounds__(256) void lookup_backward_kernel(const GradParams p
         const long long t = base + (threadIdx.x >> p.lanes_log2);
         uint32_t from = 0, to = 0;
         if (t < p.texels) segment(p, t, from, to);
-        const bool later = to - from > kShort;
+        const bool later = to - from > p.longest;
         const unsigned long long mask = __ballot(later && j == 0);
         if (mask)
         {
@@ -943,7 +943,7 @@ GradLayout grad_layout(const TripsLookupDesc& d)
     l.tile = 256;
     while ((int64_t)l.tile * 4096 < d.num_points) l.tile *= 2;
     l.count    = (uint32_t)(d.num_points / l.tile);
-    l.capacity = (uint32_t)(d.num_points / (kShort + 1));
+    l.capacity = d.num_points <= l.tile ? 0u : (uint32_t)(d.num_points / (kShort + 1));  // (few points: none is listed)
     size_t o   = 0;
     l.rows     = o;
     if (d.layout == TRIPS_TABLE_COLUMNS) o += up256((size_t)d.num_points * (size_t)r.padded * dtype_bytes(d.dtype));
@@ -964,6 +964,7 @@ hipError_t launch_lookup_backward(const TripsLookupDesc& d, const void* d_values
     p.rows = d_values, p.row = d.values_stride, p.d_table = d_table, p.order = order, p.starts = starts;
     p.tiles = reinterpret_cast<float*>(ws + l.tiles), p.listed = reinterpret_cast<uint32_t*>(ws + l.listed);
     p.texels = d.num_texels, p.table_stride = d.table_stride, p.points = (uint32_t)d.num_points, p.tile = l.tile, p.capacity = l.capacity;
+    p.longest = l.capacity > 0 ? kShort : l.tile;
     p.channels = d.num_channels, p.padded = r.padded, p.lanes_log2 = r.lanes_log2, p.accumulate = d.accumulate != 0, p.scale = d.scale;
     if (columns && d.num_points > 0)
     {
