@@ -47,12 +47,10 @@ struct LookupParams
 // gather is then one request of a point, not one per channel. Bound by memory, read and written once.
 // (row: channels rounded up to whole lanes; the elements added are zeros.)
 template <int D, int V>
-__global__ __launch_bounds__(256) void rows_kernel(const void* columns, void* rows, long long n, long long stride, int channels, int row,
-                                                   uint32_t* clear)
+__global__ __launch_bounds__(256) void rows_kernel(const void* columns, void* rows, long long n, long long stride, int channels, int row)
 {
     using T           = typename Element<D>::type;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (clear && i == 0 && blockIdx.y == 0) *clear = 0u;
     if (i >= n) return;
     const int c0   = blockIdx.y * V;
     const T* from  = reinterpret_cast<const T*>(columns) + i;
@@ -97,13 +95,19 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(const LookupParams p)
     for (long long base = (long long)blockIdx.x * at_once * POINTS; base < p.points; base += (long long)gridDim.x * at_once * POINTS)
     {
         long long t[POINTS];
+        auto load = [&](auto i32)
+        {
+#pragma unroll
+            for (int q = 0; q < POINTS; ++q)
+                t[q] = load_index<decltype(i32)::value>(p.index, min(base + q * at_once + (threadIdx.x >> p.lanes_log2), p.points - 1));
+        };
+        if (p.i32)  // (not at each load: they would wait for one another)
+            load(std::true_type{});
+        else
+            load(std::false_type{});
 #pragma unroll
         for (int q = 0; q < POINTS; ++q)
-        {
-            const long long i = base + q * at_once + (threadIdx.x >> p.lanes_log2);
-            t[q] = i < p.points ? load_index(p.i32 != 0, p.index, i) : -1;
             if (t[q] >= p.texels) t[q] = -1;
-        }
         for (int c = j * V; c < p.channels; c += lanes * V)
         {
             const int count = OUT_COLUMNS ? V : min(V, p.channels - c);
@@ -168,31 +172,37 @@ struct SortParams
     uint32_t* hist;    // [kDigits][tiles]: of each digit, its keys in each tile; then those in the tiles before
     uint32_t* totals;  // [kDigits]
     uint32_t n, texels, tiles;
-    int first, i32, shift, bits;
+    int shift, bits;
 };
 
+// Where keys come from: the pass before, or the index, of 32 or 64 bits. (A constant of the kernels: with a branch at each load the
+// loads waited for one another, and a pass over 6M points took 34 us and the count before it 9.)
+enum { kFromKeys = 0, kFromI32 = 1, kFromI64 = 2 };
+
 // A point's key: its texel, or T outside the table.
+template <int FROM>
 __device__ __forceinline__ uint32_t sort_key(const SortParams& p, uint32_t i)
 {
-    if (!p.first) return p.keys_in[i];
-    const long long t = load_index(p.i32 != 0, p.index, i);
+    if constexpr (FROM == kFromKeys) return p.keys_in[i];
+    const long long t = load_index<FROM == kFromI32>(p.index, i);
     return t >= 0 && t < (long long)p.texels ? (uint32_t)t : p.texels;
 }
 
-template <int ITEMS>
+template <int ITEMS, int FROM>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortParams p)
 {
     constexpr int kSortItems = ITEMS, kSortTile = kSortThreads * ITEMS;
     __shared__ uint32_t s[kDigits];
+    const uint32_t first = blockIdx.x * (uint32_t)kSortTile + threadIdx.x;
+    uint32_t key[kSortItems];
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) key[k] = sort_key<FROM>(p, min(first + k * kSortThreads, p.n - 1u));
     if (threadIdx.x < kDigits) s[threadIdx.x] = 0;
     __syncthreads();
     const uint32_t mask = (1u << p.bits) - 1u;
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k)
-    {
-        const uint32_t i = blockIdx.x * (uint32_t)kSortTile + k * kSortThreads + threadIdx.x;
-        if (i < p.n) atomicAdd(&s[(sort_key(p, i) >> p.shift) & mask], 1u);
-    }
+        if (first + k * kSortThreads < p.n) atomicAdd(&s[(key[k] >> p.shift) & mask], 1u);
     __syncthreads();
     if (threadIdx.x <= mask) p.hist[(size_t)threadIdx.x * p.tiles + blockIdx.x] = s[threadIdx.x];
 }
@@ -271,7 +281,7 @@ __device__ __forceinline__ void rank_keys(const uint32_t (&key)[ITEMS], uint32_t
 }
 
 // A tile's keys go to their places; the tile is put in order in LDS first, so that each digit's keys leave side by side.
-template <int ITEMS>
+template <int ITEMS, int FROM>
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortParams p)
 {
     constexpr int kSortItems = ITEMS, kSortTile = kSortThreads * ITEMS;
@@ -284,17 +294,17 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortPa
     const uint32_t mask  = (1u << p.bits) - 1u;
     const uint32_t begin = blockIdx.x * (uint32_t)kSortTile;
     const uint32_t count = min((uint32_t)kSortTile, p.n - begin);
-    for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) s_count[0][i] = 0;
     uint32_t key[kSortItems], rank[kSortItems];
     int32_t point[kSortItems];
     const uint32_t mine = wave * 64u * kSortItems, valid = count > mine ? count - mine : 0u;
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k)
     {
-        const uint32_t i = mine + k * 64 + lane;
-        key[k]   = i < count ? sort_key(p, begin + i) : ~0u;
-        point[k] = i < count ? (p.first ? (int32_t)(begin + i) : p.points_in[begin + i]) : 0;
+        const uint32_t i = begin + min(mine + k * 64 + lane, count - 1u);  // (the last lanes' copies of the last key count for nothing)
+        key[k]   = sort_key<FROM>(p, i);
+        point[k] = FROM == kFromKeys ? p.points_in[i] : (int32_t)i;
     }
+    for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) s_count[0][i] = 0;
     __syncthreads();
     rank_keys(key, valid, p.shift, p.bits, s_count[wave], rank);
     __syncthreads();
@@ -342,8 +352,9 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortPa
     {
         const uint32_t k  = s_key[at];
         const uint32_t to = s_place[(k >> p.shift) & mask] + at;
-        p.keys_out[to]    = k;
-        p.points_out[to]  = s_point[at];
+        if (to >= p.n) continue;  // (an index that was written to since it was counted must not lead outside)
+        p.keys_out[to]   = k;
+        p.points_out[to] = s_point[at];
     }
 }
 
@@ -356,6 +367,7 @@ constexpr int kCountThreads = 1024, kCountItems = 32;
 constexpr int64_t kSmallPoints = 8192;             // a workgroup a CU (8192 of 5000 texels 12.5 us, 12288 24; by passes 21 and 22)
 constexpr int64_t kSmallPairs  = (int64_t)1 << 27; // keys and starts
 constexpr uint32_t small_part(uint32_t n) { return ((n + 31u) / 32u + 31u) & ~31u; }  // keys of a thread, whole words of signs
+template <int FROM>
 __global__ __launch_bounds__(kCountThreads) void sort_small_kernel(const SortParams p, int32_t* starts)
 {
     extern __shared__ uint4 s_keys[];
@@ -365,14 +377,14 @@ __global__ __launch_bounds__(kCountThreads) void sort_small_kernel(const SortPar
     const uint32_t from = (threadIdx.x >> 5) * part, to = from + part;
     // (four words between the parts: a wavefront reads two of them at a time, from other banks)
     const uint32_t shift = (threadIdx.x >> 5) * 4u;
-    for (uint32_t j = from + (threadIdx.x & 31u); j < to; j += 32) s_key[j + shift] = j < p.n ? sort_key(p, j) : 0x7fffffffu;  // (no key is that)
+    for (uint32_t j = from + (threadIdx.x & 31u); j < to; j += 32) s_key[j + shift] = j < p.n ? sort_key<FROM>(p, j) : 0x7fffffffu;  // (no key is that)
     if (threadIdx.x < kCountItems) s_rank[threadIdx.x] = 0u;
     __syncthreads();
     // (the points' workgroups first, then those of the starts)
     const uint32_t point_groups = (p.n + kCountItems - 1) / kCountItems;
     const bool of_points = blockIdx.x < point_groups;
     const uint32_t i0 = (of_points ? blockIdx.x : blockIdx.x - point_groups) * kCountItems, i = i0 + (threadIdx.x & 31u);
-    const uint32_t mine = of_points ? (i < p.n ? sort_key(p, i) : 0u) : i;
+    const uint32_t mine = of_points ? (i < p.n ? sort_key<FROM>(p, i) : 0u) : i;
     // The signs of 32 differences in a word: a subtraction and a shift a pair, where the carry of a comparison must be waited for.
     auto less = [&](uint32_t j, uint32_t limit)
     {
@@ -408,7 +420,7 @@ __global__ __launch_bounds__(kCountThreads) void sort_small_kernel(const SortPar
     {
         if (i <= p.texels) starts[i] = (int32_t)at;
     }
-    else if (i < p.n)
+    else if (i < p.n && at < p.n)  // (an index that is written to meanwhile must not lead outside)
     {
         p.points_out[at] = (int32_t)i;
         if (p.keys_out) p.keys_out[at] = mine;
@@ -471,10 +483,11 @@ __global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict_
         }
         return;
     }
+#pragma unroll 4
     for (uint32_t k = from + threadIdx.x; k < to; k += 256)
     {
-        const uint32_t key = keys[k];
-        if (k == from || keys[k - 1] != key) s_first[key - first] = k;
+        const uint32_t key = keys[k], before = keys[max(k, 1u) - 1u];
+        if (k == from || before != key) s_first[key - first] = k;
     }
     __syncthreads();
     // the least of a thread's texels' and all that follow
@@ -540,7 +553,7 @@ __device__ __forceinline__ void add_rows(const GradParams& p, uint32_t from, uin
     using E       = Element<D>;
     using T       = typename E::type;
     const T* rows = reinterpret_cast<const T*>(p.rows) + c;
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = 8;
     for (uint32_t k = from; k < to; k += AHEAD * step)
     {
         uint32_t i[AHEAD];
@@ -773,7 +786,7 @@ void launch_rows(const TripsLookupDesc& d, const RowShape& r, const void* column
     const dim3 grid((unsigned)((n + 255) / 256), (unsigned)(r.padded / v));
     with_types(d.dtype, r.lane_bytes, true, [&](auto D, auto V, auto) {
         hipLaunchKernelGGL((rows_kernel<decltype(D)::value, decltype(V)::value>), grid, dim3(256), 0, stream, columns, rows, n, stride,
-                           d.num_channels, r.padded, (uint32_t*)nullptr);
+                           d.num_channels, r.padded);
     });
 }
 
@@ -818,7 +831,8 @@ hipError_t launch_plan(int64_t texels, int64_t points, const void* index, int in
     const PlanLayout l = plan_layout(points);
     const int bits     = key_bits(texels), passes = (bits + 7) / 8;
     SortParams p;
-    p.index = index, p.i32 = index_dtype == TRIPS_INDEX_I32, p.n = (uint32_t)points, p.texels = (uint32_t)texels;
+    const bool i32 = index_dtype == TRIPS_INDEX_I32;
+    p.index = index, p.n = (uint32_t)points, p.texels = (uint32_t)texels;
     const int tile = kSortThreads * sort_items(points);
     p.tiles        = (uint32_t)((points + tile - 1) / tile);
     p.hist = reinterpret_cast<uint32_t*>(ws + l.hist), p.totals = reinterpret_cast<uint32_t*>(ws + l.totals);
@@ -827,36 +841,44 @@ hipError_t launch_plan(int64_t texels, int64_t points, const void* index, int in
     if (points > 0 && points <= kSmallPoints)
     {
         const bool whole = (texels + 1) * points <= kSmallPairs;
-        p.first = 1, p.shift = 0, p.bits = 0, p.keys_in = nullptr, p.points_in = nullptr;
+        p.shift = 0, p.bits = 0, p.keys_in = nullptr, p.points_in = nullptr;
         p.keys_out   = whole ? nullptr : reinterpret_cast<uint32_t*>(ws + l.keys[0]);
         p.points_out = order;
         const size_t lds      = 32 * sizeof(uint32_t) * (small_part(p.n) + 4);
         const unsigned groups = (p.n + kCountItems - 1) / kCountItems, more = whole ? (unsigned)(texels + kCountItems) / kCountItems : 0u;
-        if (lds > 64 * 1024)
-        {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&sort_small_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            if (e != hipSuccess) return e;
-        }
-        hipLaunchKernelGGL(sort_small_kernel, dim3(groups + more), dim3(kCountThreads), lds, stream, p, starts);
+        if (i32)
+            hipLaunchKernelGGL(sort_small_kernel<kFromI32>, dim3(groups + more), dim3(kCountThreads), lds, stream, p, starts);
+        else
+            hipLaunchKernelGGL(sort_small_kernel<kFromI64>, dim3(groups + more), dim3(kCountThreads), lds, stream, p, starts);
         if (whole) return hipGetLastError();
     }
     int shift = 0;
     for (int pass = 0; pass < passes && points > kSmallPoints; ++pass)
     {
-        p.first = pass == 0, p.shift = shift, p.bits = (bits - shift + passes - pass - 1) / (passes - pass);
+        p.shift      = shift, p.bits = (bits - shift + passes - pass - 1) / (passes - pass);
         p.keys_in    = p.keys_out;
         p.points_in  = p.points_out;
         p.keys_out   = reinterpret_cast<uint32_t*>(ws + l.keys[pass & 1]);
         p.points_out = (passes - 1 - pass) % 2 == 0 ? order : reinterpret_cast<int32_t*>(ws + l.points);
+        auto launch = [&](auto items, auto from)
+        {
+            hipLaunchKernelGGL((sort_count_kernel<decltype(items)::value, decltype(from)::value>), dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
+            if (p.tiles > kFewTiles) hipLaunchKernelGGL(sort_scan_kernel, dim3(1 << p.bits), dim3(kScanThreads), 0, stream, p);
+            hipLaunchKernelGGL((sort_scatter_kernel<decltype(items)::value, decltype(from)::value>), dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
+        };
+        auto launch_from = [&](auto items)
+        {
+            if (pass > 0)
+                launch(items, std::integral_constant<int, kFromKeys>{});
+            else if (i32)
+                launch(items, std::integral_constant<int, kFromI32>{});
+            else
+                launch(items, std::integral_constant<int, kFromI64>{});
+        };
         if (sort_items(points) == 2)
-            hipLaunchKernelGGL(sort_count_kernel<2>, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
+            launch_from(std::integral_constant<int, 2>{});
         else
-            hipLaunchKernelGGL(sort_count_kernel<4>, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
-        if (p.tiles > kFewTiles) hipLaunchKernelGGL(sort_scan_kernel, dim3(1 << p.bits), dim3(kScanThreads), 0, stream, p);
-        if (sort_items(points) == 2)
-            hipLaunchKernelGGL(sort_scatter_kernel<2>, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
-        else
-            hipLaunchKernelGGL(sort_scatter_kernel<4>, dim3(p.tiles), dim3(kSortThreads), 0, stream, p);
+            launch_from(std::integral_constant<int, 4>{});
         shift += p.bits;
     }
     if (points > 2 * texels || texels < kFewTexels)
