@@ -98,7 +98,8 @@ PLANS = [(1, 1, "any"), (1, 5000, "same"), (2, 1, "any"), (7, 64, "outside"), (2
          (1 << 24, 300_000, "any"), ((1 << 31) - 100, 1, "none"), (50_000, 300_000, "same"), (1000, 30_000, "all_outside"), (40_000, 40_000, "once"),
          (0, 100, "all_outside"), (100, 0, "any"), (0, 0, "any"), (5000, 16_385, "skewed"), (33, 8192, "outside"), (33, 8193, "outside"),
          (9000, 8191, "any"), (200_000, 8192, "skewed"), (1000, 1_100_000, "skewed"), (2_000_000, 1_200_000, "outside"), (70_000, 65_536, "any"),
-         (70_000, 65_537, "any"), (500_000, 1_048_575, "any"), (500_000, 1_048_576, "any")]
+         (70_000, 65_537, "any"), (500_000, 1_048_575, "any"), (500_000, 1_048_576, "any"),
+         (3_000_000, 4_194_303, "outside"), (3_000_000, 4_194_304, "outside"), (300, 5_000_000, "skewed")]
 
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])

@@ -155,10 +155,10 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(const LookupParams p)
 
 // ---- the order of the points: a stable radix sort, least significant digit first ----
 
-// A tile: 4096 points, or 2048 below a million (20k points 31 us and 37, 1M 57 and 58; 6M the other way round).
+// A tile: 1024 threads with 2 points each below 2^20 points, with 4 below 2^22, with 6 above (two tiles a CU at a time in any case;
+// us: 20k points 22 with 2 and 31 with 8 of 512 threads, 1M 56 and with 6 59, 2M 68 with 4 and 74 with 6, 6M 147 with 4 and 132 with 6).
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int64_t kManyPoints = 1 << 20;
-constexpr int sort_items(int64_t points) { return points < kManyPoints ? 2 : 4; }
+constexpr int sort_items(int64_t points) { return points < (1 << 20) ? 2 : points < (1 << 22) ? 4 : 6; }
 constexpr int kDigits = 256;
 constexpr uint32_t kFewTiles = 32;  // so few that each tile's workgroup sums the counts of the others itself: a launch less a pass
 
@@ -176,7 +176,7 @@ struct SortParams
 };
 
 // Where keys come from: the pass before, or the index, of 32 or 64 bits. (A constant of the kernels: with a branch at each load the
-// loads waited for one another, and a pass over 6M points took 34 us and the count before it 9.)
+// loads waited for one another: a pass over 6M points 34 us and 32, the count before it 9 and 8.)
 enum { kFromKeys = 0, kFromI32 = 1, kFromI64 = 2 };
 
 // A point's key: its texel, or T outside the table.
@@ -546,14 +546,14 @@ __device__ __forceinline__ void segment(const GradParams& p, long long t, uint32
     to   = max(from, min((uint32_t)p.starts[t + 1], p.points));
 }
 
-// sum += the rows of the points order[k], k = from, from + step .. below to; V channels from c on
-template <int D, int V>
+// sum += the rows of the points order[k], k = from, from + step .. below to; V channels from c on. AHEAD rows are on their way at a
+// time: 8 short ones of columns (6M points of 1.5M texels 157 us, with 4 160), 4 of longer rows (8191 tokens 46 us, with 8 47 to 49).
+template <int D, int V, int AHEAD>
 __device__ __forceinline__ void add_rows(const GradParams& p, uint32_t from, uint32_t to, uint32_t step, int c, int count, float (&sum)[V])
 {
     using E       = Element<D>;
     using T       = typename E::type;
     const T* rows = reinterpret_cast<const T*>(p.rows) + c;
-    constexpr int AHEAD = 8;
     for (uint32_t k = from; k < to; k += AHEAD * step)
     {
         uint32_t i[AHEAD];
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(256) void lookup_backward_kernel(const GradParams p
             float sum[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) sum[e] = 0.f;
-            add_rows<D, V>(p, from, to, 1, c, count, sum);
+            add_rows<D, V, OUT_COLUMNS ? 8 : 4>(p, from, to, 1, c, count, sum);
             store_sum<D, V, OUT_COLUMNS>(p, t, c, count, sum);
         }
     }
@@ -679,7 +679,7 @@ __global__ __launch_bounds__(kWideThreads) void lookup_tiles_kernel(const GradPa
     for (int e = 0; e < V; ++e) sum[e] = 0.f;
     if (s_in)
     {
-        if (c < p.channels) add_rows<D, V>(p, from + r, to, blockDim.x >> p.lanes_log2, c, OUT_COLUMNS ? V : min(V, p.channels - c), sum);
+        if (c < p.channels) add_rows<D, V, OUT_COLUMNS ? 8 : 4>(p, from + r, to, blockDim.x >> p.lanes_log2, c, OUT_COLUMNS ? V : min(V, p.channels - c), sum);
         add_threads(sum, s, p.lanes_log2);
     }
     if ((int)threadIdx.x < lanes && c < p.padded)
@@ -713,16 +713,16 @@ __global__ __launch_bounds__(kWideThreads) void lookup_backward_long_kernel(cons
         {
             if (first < last)
             {
-                add_rows<D, V>(p, from + r, first * p.tile, rows, c, count, sum);
+                add_rows<D, V, OUT_COLUMNS ? 8 : 4>(p, from + r, first * p.tile, rows, c, count, sum);
                 for (uint32_t k = first + r; k < last; k += rows)
                 {
 #pragma unroll
                     for (int e = 0; e < V; ++e) sum[e] += p.tiles[(long long)k * p.padded + c + e];
                 }
-                add_rows<D, V>(p, last * p.tile + r, to, rows, c, count, sum);
+                add_rows<D, V, OUT_COLUMNS ? 8 : 4>(p, last * p.tile + r, to, rows, c, count, sum);
             }
             else
-                add_rows<D, V>(p, from + r, to, rows, c, count, sum);
+                add_rows<D, V, OUT_COLUMNS ? 8 : 4>(p, from + r, to, rows, c, count, sum);
         }
         add_threads(sum, s, p.lanes_log2);
         if ((int)threadIdx.x < lanes && c < p.channels) store_sum<D, V, OUT_COLUMNS>(p, t, c, count, sum);
@@ -877,8 +877,10 @@ hipError_t launch_plan(int64_t texels, int64_t points, const void* index, int in
         };
         if (sort_items(points) == 2)
             launch_from(std::integral_constant<int, 2>{});
-        else
+        else if (sort_items(points) == 4)
             launch_from(std::integral_constant<int, 4>{});
+        else
+            launch_from(std::integral_constant<int, 6>{});
         shift += p.bits;
     }
     if (points > 2 * texels || texels < kFewTexels)
