@@ -109,6 +109,16 @@ def test_plan(texels, points, how, dtype):
     _check_plan(lk.lookup_plan(index, texels), index, texels)
 
 
+@pytest.mark.parametrize("points", [1, 31, 32, 33, 100, 1025])
+@pytest.mark.parametrize("texels", [15_359, 15_360, 30_721, 491_519, 491_520, 130_815, 4_194_303, 4_194_304])
+def test_plan_of_few_points_and_many_texels(texels, points):
+    rng = np.random.default_rng(texels + points)
+    index = _index(rng, texels, points, "any")
+    index[rng.integers(points)] = texels - 1
+    index[rng.integers(points)] = texels
+    _check_plan(lk.lookup_plan(index, texels), index, texels)
+
+
 def test_plan_of_indexes_beyond_32_bits():
     index = torch.tensor([1 << 32, 5, -(1 << 40), (1 << 31) + 5, 0, 5], device="cuda")
     plan = lk.lookup_plan(index, 6)
@@ -144,6 +154,26 @@ def test_lookup_and_gradient(texels, points, channels, dtype, layout, pad):
         out = lk.lookup_backward(grad, index, texels, scale, layout, plan, out=wide[:, :columns])
         _check_grad(out, grad, index, texels, scale, layout, before[:, :columns])
         assert torch.equal(wide[:, columns:], before[:, columns:])
+
+
+@pytest.mark.parametrize("layout", BOTH)
+@pytest.mark.parametrize("channels", [1, 2, 7, 40, 256, 2100])
+@pytest.mark.parametrize("texels,how", [(1, "same"), (4, "any"), (9, "outside"), (40, "skewed"), (5000, "skewed")])
+@pytest.mark.parametrize("points", [32, 33, 64, 65, 255, 256, 257, 512, 513])
+def test_gradient_of_few_points(points, texels, how, channels, layout):
+    """Several texels with many of the points, in one workgroup and in several."""
+    rng = np.random.default_rng(points * 11 + texels + channels)
+    index = _index(rng, texels, points, how)
+    for dtype in ("f32", "f16"):
+        rows, columns = (points, channels) if layout == lk.ROWS else (channels, points)
+        grad = _matrix(rng, rows, columns, dtype, spread=1.0)
+        got = lk.lookup_backward(grad, index, texels, 1.5, layout)
+        _check_grad(got, grad, index, texels, 1.5, layout)
+        rows, columns = (texels, channels) if layout == lk.ROWS else (channels, texels)
+        out = _matrix(rng, rows, columns, dtype)
+        before = out.clone()
+        lk.lookup_backward(grad, index, texels, 1.5, layout, lk.lookup_plan(index, texels), out=out)
+        _check_grad(out, grad, index, texels, 1.5, layout, before)
 
 
 LONG = [(1, 100_000, "same"), (3, 50_000, "any"), (1000, 200_000, "skewed"), (5, 2047, "any"), (2, 2048, "same"), (2, 2049, "same"), (2, 4097, "any"),

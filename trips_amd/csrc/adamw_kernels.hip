@@ -407,6 +407,8 @@ __device__ __forceinline__ uint32_t tensor_of_tile(const uint32_t* first_tiles, 
     return (uint32_t)__popcll(__ballot(lane < (int)n && first_tiles[lane] <= tile)) - 1u;
 }
 
+// 60M weights of 32 bits: moments in 32 bits 300 us (5.6 TB/s), in 8 bits 166 (5.8 TB/s; 7.5e7 vector instructions of wavefronts,
+// 122 us if nothing else were issued: the codes are half of them); four tensors of a net 4.7.
 template <int WD, int GD, int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(const StepParams p)
 {
@@ -492,6 +494,7 @@ __device__ __forceinline__ double tile_squares(const NormTensor& T, long long ti
     return sum;
 }
 
+// 60M elements 38 us (6.3 TB/s), a net of 16,000 elements 4: a launch. At most kNormGroups partial sums, added by one workgroup.
 __global__ __launch_bounds__(256) void grad_squares_kernel(const NormTable tab)
 {
     __shared__ double s[4];

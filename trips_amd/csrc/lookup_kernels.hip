@@ -1,7 +1,11 @@
 // Entries of a table by index, the order of points by their index, and the table's gradient summed in that order (gfx950).
 //
-// All are bound by memory: the lookup and the gradient by scattered requests (of 4 bytes a channel in the columns layout,
-// of whole rows in the rows layout), the order by the passes of its sort.
+//   values[i] = scale table[index[i]]          d_table[t] (+)= scale sum of d_values[i] over the i with index[i] = t, in their order
+//
+// Large calls are bound by memory: lookup and gradient in no order by the lines of 128 bytes that each scattered request moves
+// (7 TB/s of lines), short ones and those of whole rows by latency or by the table's bytes; the order of the points by the three
+// passes of its sort. us a call: 6M points of 1.5M texels in four channels 117, their gradient 157, their order 132; 8191 tokens of
+// a table of 50,000 rows of 1024 bytes 7.5, with order and gradient 46. Below each kernel its own share.
 #include <algorithm>
 #include <type_traits>
 
@@ -44,7 +48,8 @@ struct LookupParams
 // ---- columns to rows ----
 
 // [channels, n] to [n, row] with 16 bytes (8 where two or four channels of 16 bits make no more) a lane: what the kernels below
-// gather is then one request of a point, not one per channel. Bound by memory, read and written once.
+// gather is then one request of a point, not one per channel. Bound by memory, read and written once (6M points in four channels
+// of 32 bits 30 us, 6.4 TB/s).
 // (row: channels rounded up to whole lanes; the elements added are zeros.)
 template <int D, int V>
 __global__ __launch_bounds__(256) void rows_kernel(const void* columns, void* rows, long long n, long long stride, int channels, int row)
@@ -83,6 +88,8 @@ __global__ __launch_bounds__(256) void lookup_columns_kernel(const LookupParams 
 }
 
 // V elements a lane, 1 << lanes_log2 lanes a point. OUT_COLUMNS: the values are columns (and the table's rows whole lanes wide).
+// 6M points of 24 MB of rows in no order: 107 us, 6.0M lines of 128 bytes that no L2 holds (7.1 TB/s of them; an XCD's L2 has 4 MB).
+// 8191 rows of 1024 bytes: 7.9 us, of which the bytes are 3: an index, then its row, with one wave of workgroups on the card.
 template <int D, int V, bool OUT_COLUMNS>
 __global__ __launch_bounds__(256) void lookup_rows_kernel(const LookupParams p)
 {
@@ -188,6 +195,7 @@ __device__ __forceinline__ uint32_t sort_key(const SortParams& p, uint32_t i)
     return t >= 0 && t < (long long)p.texels ? (uint32_t)t : p.texels;
 }
 
+// Bound by memory and by launching: 6M keys 7 us.
 template <int ITEMS, int FROM>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortParams p)
 {
@@ -225,7 +233,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* s)
 }
 
 constexpr int kScanThreads = 1024;
-// One workgroup a digit: its counts become the sums of the tiles before.
+// One workgroup a digit: its counts become the sums of the tiles before. (977 tiles 4.8 us, nearly all of it latency.)
 __global__ __launch_bounds__(kScanThreads) void sort_scan_kernel(const SortParams p)
 {
     __shared__ uint32_t s[kScanThreads / 64], s_sum;
@@ -281,6 +289,7 @@ __device__ __forceinline__ void rank_keys(const uint32_t (&key)[ITEMS], uint32_t
 }
 
 // A tile's keys go to their places; the tile is put in order in LDS first, so that each digit's keys leave side by side.
+// 6M pairs 28 us: vector instructions of the ranks 15 of it, the bytes of pairs 15, both beside barriers and LDS.
 template <int ITEMS, int FROM>
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortParams p)
 {
@@ -362,37 +371,40 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortPa
 // 32 points a workgroup, each by 32 threads with a 32nd of the keys. One launch, on all of the card, where the sort's passes are
 // launches in a row. Bound by the LDS that every key of every workgroup is read from (3.4 us of 11 at 8191 points) and the
 // pairs' two instructions (as much).
-// Behind the points' places, if `starts`: the keys below each t.
+// Behind the points' places, if `starts`: the keys below each t, 1 << starts_log2 of them a workgroup, each by as many threads as that
+// leaves: as many as it takes for about two workgroups a CU (16 points of 643k texels: 32 a workgroup 66 us, 1024 6).
 constexpr int kCountThreads = 1024, kCountItems = 32;
+constexpr int kStartsGroups = 480;
 constexpr int64_t kSmallPoints = 8192;             // a workgroup a CU (8192 of 5000 texels 12.5 us, 12288 24; by passes 21 and 22)
 constexpr int64_t kSmallPairs  = (int64_t)1 << 27; // keys and starts
 constexpr uint32_t small_part(uint32_t n) { return ((n + 31u) / 32u + 31u) & ~31u; }  // keys of a thread, whole words of signs
 template <int FROM>
-__global__ __launch_bounds__(kCountThreads) void sort_small_kernel(const SortParams p, int32_t* starts)
+__global__ __launch_bounds__(kCountThreads) void sort_small_kernel(const SortParams p, int32_t* starts, int starts_log2)
 {
     extern __shared__ uint4 s_keys[];
-    __shared__ uint32_t s_rank[kCountItems];
+    __shared__ uint32_t s_rank[kCountThreads];
     uint32_t* s_key     = reinterpret_cast<uint32_t*>(s_keys);
     const uint32_t part = small_part(p.n);
-    const uint32_t from = (threadIdx.x >> 5) * part, to = from + part;
     // (four words between the parts: a wavefront reads two of them at a time, from other banks)
-    const uint32_t shift = (threadIdx.x >> 5) * 4u;
-    for (uint32_t j = from + (threadIdx.x & 31u); j < to; j += 32) s_key[j + shift] = j < p.n ? sort_key<FROM>(p, j) : 0x7fffffffu;  // (no key is that)
-    if (threadIdx.x < kCountItems) s_rank[threadIdx.x] = 0u;
+    const uint32_t first = (threadIdx.x >> 5) * part, shift = (threadIdx.x >> 5) * 4u;
+    for (uint32_t j = first + (threadIdx.x & 31u); j < first + part; j += 32)
+        s_key[j + shift] = j < p.n ? sort_key<FROM>(p, j) : 0x7fffffffu;  // (no key is that)
+    s_rank[threadIdx.x] = 0u;
     __syncthreads();
     // (the points' workgroups first, then those of the starts)
     const uint32_t point_groups = (p.n + kCountItems - 1) / kCountItems;
-    const bool of_points = blockIdx.x < point_groups;
-    const uint32_t i0 = (of_points ? blockIdx.x : blockIdx.x - point_groups) * kCountItems, i = i0 + (threadIdx.x & 31u);
+    const bool of_points        = blockIdx.x < point_groups;
+    const uint32_t items_log2   = of_points ? 5u : (uint32_t)starts_log2, at_item = threadIdx.x & ((1u << items_log2) - 1u);
+    const uint32_t i0 = (of_points ? blockIdx.x : blockIdx.x - point_groups) << items_log2, i = i0 + at_item;
     const uint32_t mine = of_points ? (i < p.n ? sort_key<FROM>(p, i) : 0u) : i;
     // The signs of 32 differences in a word: a subtraction and a shift a pair, where the carry of a comparison must be waited for.
-    auto less = [&](uint32_t j, uint32_t limit)
+    auto less = [&](uint32_t at, uint32_t limit)
     {
         uint32_t signs = 0;
 #pragma unroll
         for (uint32_t q = 0; q < 32; q += 4)
         {
-            const uint4 k = s_keys[(j + q + shift) / 4];
+            const uint4 k = s_keys[(at + q) / 4];
             signs = __builtin_amdgcn_alignbit(signs, k.x - limit, 31u);
             signs = __builtin_amdgcn_alignbit(signs, k.y - limit, 31u);
             signs = __builtin_amdgcn_alignbit(signs, k.z - limit, 31u);
@@ -401,20 +413,22 @@ __global__ __launch_bounds__(kCountThreads) void sort_small_kernel(const SortPar
         return signs;
     };
     uint32_t below = 0;
-    for (uint32_t j = from; j < to; j += 32)
-    {
-        // equal keys count where they lie before the point
-        const uint32_t signs = less(j, mine + (of_points && j < i0 ? 1u : 0u));
-        below += (uint32_t)__popc(signs);
-        if (of_points && __ballot(j == i0))
+    const uint32_t parts = 1u << (items_log2 - 5u);  // of a thread
+    for (uint32_t k = (threadIdx.x >> items_log2) * parts, last = k + parts; k < last && k * part < p.n; ++k)
+        for (uint32_t j = k * part; j < (k + 1) * part; j += 32)
         {
-            const uint32_t equal = less(j, mine + 1u) & ~signs & ~(~0u >> (i & 31u));  // (the word's first keys are its highest bits)
-            below += j == i0 ? (uint32_t)__popc(equal) : 0u;
+            // equal keys count where they lie before the point
+            const uint32_t signs = less(j + k * 4u, mine + (of_points && j < i0 ? 1u : 0u));
+            below += (uint32_t)__popc(signs);
+            if (of_points && __ballot(j == i0))
+            {
+                const uint32_t equal = less(j + k * 4u, mine + 1u) & ~signs & ~(~0u >> (i & 31u));  // (the word's first keys are its highest bits)
+                below += j == i0 ? (uint32_t)__popc(equal) : 0u;
+            }
         }
-    }
-    atomicAdd(&s_rank[threadIdx.x & 31u], below);
+    atomicAdd(&s_rank[at_item], below);
     __syncthreads();
-    if (threadIdx.x >= kCountItems) return;
+    if (threadIdx.x >> items_log2) return;
     const uint32_t at = s_rank[threadIdx.x];
     if (!of_points)
     {
@@ -448,7 +462,7 @@ __device__ __forceinline__ uint32_t lower_bound(const T* a, uint32_t n, uint32_t
 // starts[t] = the first of the sorted keys that is t or more, for kStartsTexels texels a workgroup. Two wavefronts find the keys
 // that belong to them; where these are about as many as the texels, each key that differs from the one before is noted in LDS
 // and the texels in between take the next one's; where they are many more, each texel is searched for. ITEMS texels a thread: 8,
-// or 1 where there are more than two points a texel or few texels.
+// or 1 where there are more than two points a texel or few texels. 6M keys of 1.5M texels 18 us with 1, of 6M texels 20 with 8.
 constexpr int64_t kFewTexels = 1 << 18;
 template <int ITEMS>
 __global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t texels, int32_t* starts)
@@ -521,6 +535,7 @@ __global__ __launch_bounds__(256) void starts_kernel(const uint32_t* __restrict_
 // it, is left to one wavefront. Which points are added to which sum first goes by the plan and the sizes alone.
 
 constexpr int kShort      = 32;
+constexpr int kShortOfFew = 64;
 constexpr int kLongGroups = 2048;  // workgroups for the listed texels
 constexpr int kWideThreads = 1024; // of a workgroup that adds up rows of more than eight lanes; 256 for others
 
@@ -533,7 +548,7 @@ struct GradParams
     float* tiles;     // [points / tile, padded] sums of the tiles that one texel fills (zeros for the others)
     uint32_t* listed;  // texels for the second kernel: how many, then 63 words on, which
     long long texels, table_stride, row;
-    uint32_t points, tile, capacity, longest;  // longest: points of a texel that is not listed
+    uint32_t points, tile, capacity;
     int channels, padded, lanes_log2, accumulate;
     float scale;
 };
@@ -602,38 +617,6 @@ __device__ __forceinline__ void store_sum(const GradParams& p, long long t, int 
         if (c + e < p.channels) to[e * s] = E::from_float(p.accumulate ? E::to_float(to[e * s]) + p.scale * sum[e] : p.scale * sum[e]);
 }
 
-// OUT_COLUMNS: the table's gradient is columns, and the rows were made of columns (whole lanes wide).
-template <int D, int V, bool OUT_COLUMNS>
-__global__ __launch_bounds__(256) void lookup_backward_kernel(const GradParams p)
-{
-    const int lanes = 1 << p.lanes_log2, j = threadIdx.x & (lanes - 1), at_once = 256 >> p.lanes_log2, lane = threadIdx.x & 63;
-    for (long long base = (long long)blockIdx.x * at_once; base < p.texels; base += (long long)gridDim.x * at_once)
-    {
-        const long long t = base + (threadIdx.x >> p.lanes_log2);
-        uint32_t from = 0, to = 0;
-        if (t < p.texels) segment(p, t, from, to);
-        const bool later = to - from > p.longest;
-        const unsigned long long mask = __ballot(later && j == 0);
-        if (mask)
-        {
-            uint32_t at = 0;
-            if (lane == 0) at = atomicAdd(p.listed, (uint32_t)__popcll(mask));
-            at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(mask & ((1ull << lane) - 1ull));
-            if (later && j == 0 && at < p.capacity) p.listed[kListHead + at] = (uint32_t)t;
-        }
-        if (t >= p.texels || later || (p.accumulate && from == to)) continue;
-        for (int c = j * V; c < p.channels; c += lanes * V)
-        {
-            const int count = OUT_COLUMNS ? V : min(V, p.channels - c);
-            float sum[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) sum[e] = 0.f;
-            add_rows<D, V, OUT_COLUMNS ? 8 : 4>(p, from, to, 1, c, count, sum);
-            store_sum<D, V, OUT_COLUMNS>(p, t, c, count, sum);
-        }
-    }
-}
-
 // The sums of the threads of one column (threadIdx.x >> lanes_log2 counts them), in their order; valid in the first `lanes` threads.
 template <int V>
 __device__ __forceinline__ void add_threads(float (&sum)[V], float* s, int lanes_log2)
@@ -656,7 +639,76 @@ __device__ __forceinline__ void add_threads(float (&sum)[V], float* s, int lanes
     for (int e = 0; e < V; ++e) sum[e] = s[e * blockDim.x + threadIdx.x];
 }
 
-// One workgroup a tile of the plan's positions (and a group of lanes' channels). Clears the list's length as well.
+// OUT_COLUMNS: the table's gradient is columns, and the rows were made of columns (whole lanes wide). 6M points of 1.5M texels in
+// no order: 118 us, 6.3M lines of 128 bytes (6.8 TB/s of them). 8191 tokens: 20 us, the 102 MB of 50,000 rows, mostly zeros, 5.2 TB/s.
+// Groups of lanes' channels go along grid.y where there are few texels, and one behind the other. FEW: so few points that no texel is listed: those with more than
+// kShortOfFew are added up by all of the workgroup that they belong to, one behind the other (at most seven, 1.4 us each).
+template <int D, int V, bool OUT_COLUMNS, bool FEW>
+__global__ __launch_bounds__(256) void lookup_backward_kernel(const GradParams p)
+{
+    extern __shared__ float s[];  // [V][threads] if FEW
+    __shared__ uint32_t s_later[FEW ? 256 : 1], s_count;
+    const int lanes = 1 << p.lanes_log2, j = threadIdx.x & (lanes - 1), at_once = 256 >> p.lanes_log2, lane = threadIdx.x & 63;
+    const int c0 = (int)blockIdx.y * lanes * V, c_step = (int)gridDim.y * lanes * V;
+    if (FEW)
+    {
+        if (threadIdx.x == 0) s_count = 0u;
+        __syncthreads();
+    }
+    for (long long base = (long long)blockIdx.x * at_once; base < p.texels; base += (long long)gridDim.x * at_once)
+    {
+        const long long t = base + (threadIdx.x >> p.lanes_log2);
+        uint32_t from = 0, to = 0;
+        if (t < p.texels) segment(p, t, from, to);
+        const bool later = to - from > (FEW ? kShortOfFew : kShort);
+        if (FEW)
+        {
+            if (later && j == 0) s_later[atomicAdd(&s_count, 1u)] = (uint32_t)t;
+        }
+        else if (const unsigned long long mask = __ballot(later && j == 0 && blockIdx.y == 0))
+        {
+            uint32_t at = 0;
+            if (lane == 0) at = atomicAdd(p.listed, (uint32_t)__popcll(mask));
+            at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(mask & ((1ull << lane) - 1ull));
+            if (later && j == 0 && at < p.capacity) p.listed[kListHead + at] = (uint32_t)t;
+        }
+        float sum[V];
+        if (t < p.texels && !later && !(p.accumulate && from == to))
+        {
+            for (int c = c0 + j * V; c < p.channels; c += c_step)
+            {
+                const int count = OUT_COLUMNS ? V : min(V, p.channels - c);
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[e] = 0.f;
+                add_rows<D, V, OUT_COLUMNS ? 8 : 4>(p, from, to, 1, c, count, sum);
+                store_sum<D, V, OUT_COLUMNS>(p, t, c, count, sum);
+            }
+        }
+        if (!FEW) continue;
+        __syncthreads();
+        const uint32_t n = s_count;
+        for (uint32_t k = 0; k < n; ++k)
+        {
+            const long long tk = s_later[k];
+            segment(p, tk, from, to);
+            for (int first = c0; first < p.channels; first += c_step)
+            {
+                const int c = first + j * V, count = OUT_COLUMNS ? V : min(V, p.channels - c);
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[e] = 0.f;
+                if (c < p.channels) add_rows<D, V, OUT_COLUMNS ? 8 : 4>(p, from + (threadIdx.x >> p.lanes_log2), to, at_once, c, count, sum);
+                add_threads(sum, s, p.lanes_log2);
+                if ((int)threadIdx.x < lanes && c < p.channels) store_sum<D, V, OUT_COLUMNS>(p, tk, c, count, sum);
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) s_count = 0u;
+        __syncthreads();
+    }
+}
+
+// One workgroup a tile of the plan's positions (and a group of lanes' channels). Clears the list's length as well. Where no texel
+// fills a tile it reads the tile's ends and stores zeros: 3 to 7 us.
 template <int D, int V, bool OUT_COLUMNS>
 __global__ __launch_bounds__(kWideThreads) void lookup_tiles_kernel(const GradParams p)
 {
@@ -690,7 +742,8 @@ __global__ __launch_bounds__(kWideThreads) void lookup_tiles_kernel(const GradPa
 }
 
 // One workgroup a listed texel (and a group of lanes' channels): the points before its first whole tile, those behind its last
-// one, and the tiles.
+// one, and the tiles. 4 us with nothing listed; 8191 tokens, most frequent ones a few hundred times, 8: a texel's sum is one
+// workgroup's chain.
 template <int D, int V, bool OUT_COLUMNS>
 __global__ __launch_bounds__(kWideThreads) void lookup_backward_long_kernel(const GradParams p)
 {
@@ -732,9 +785,11 @@ __global__ __launch_bounds__(kWideThreads) void lookup_backward_long_kernel(cons
 // ---- host ----
 
 constexpr long long kMostRowGroups = 1 << 20;  // a launch has less than 2^32 threads
+constexpr long long kFewRowGroups  = 4096;     // (8191 points of 50,000 texels in 1024 bfloat16 channels 31 us, with twice as many groups 34)
 constexpr size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// How a row of channels is spread over lanes: 16 bytes a lane, or 8 where all of a row in columns fits them.
+// How a row of channels is spread over lanes: 16 bytes a lane, 8 where all of a row in columns fits them, or the one channel that
+// a column has.
 struct RowShape
 {
     int lane_bytes, lanes_log2, groups, padded;  // groups of lanes a row; padded: channels in whole lanes
@@ -743,7 +798,7 @@ RowShape row_shape(const TripsLookupDesc& d)
 {
     const int size = dtype_bytes(d.dtype);
     RowShape r;
-    r.lane_bytes    = d.layout == TRIPS_TABLE_COLUMNS && d.num_channels * size <= 8 ? 8 : 16;
+    r.lane_bytes    = d.layout == TRIPS_TABLE_ROWS || d.num_channels * size > 8 ? 16 : d.num_channels > 1 ? 8 : size;
     const int v     = r.lane_bytes / size, chunks = (d.num_channels + v - 1) / v;
     r.lanes_log2    = 0;
     while ((1 << r.lanes_log2) < chunks && r.lanes_log2 < 6) ++r.lanes_log2;
@@ -766,7 +821,9 @@ void with_types(int dtype, int lane_bytes, bool columns, const F& f)
     auto with_lane = [&](auto d)
     {
         constexpr int size = decltype(d)::value == TRIPS_DTYPE_F32 ? 4 : 2;
-        if (lane_bytes == 8)
+        if (lane_bytes == size)
+            f(d, std::integral_constant<int, 1>{}, std::true_type{});  // (columns alone)
+        else if (lane_bytes == 8)
             f(d, std::integral_constant<int, 8 / size>{}, std::true_type{});  // (columns alone)
         else
             with_columns(d, std::integral_constant<int, 16 / size>{});
@@ -791,8 +848,8 @@ void launch_rows(const TripsLookupDesc& d, const RowShape& r, const void* column
 }
 
 // Whether a lookup in columns turns the table to rows first. Scattered requests are what a lookup costs, one a point and channel
-// in columns, one a point in rows (6M points and four channels of 1.5M texels in no order: 350 us and 88); turning the table
-// costs its bytes twice, as much as about an eighth of a request a texel.
+// in columns, one a point in rows (6M points and four channels of 1.5M texels in no order: 350 us and 107); turning the table
+// costs its bytes twice (9), as much as about an eighth of a request a texel.
 bool turns_table(const TripsLookupDesc& d)
 {
     return d.layout == TRIPS_TABLE_COLUMNS && d.num_channels > 1 && d.num_points >= d.num_texels / 8;
@@ -840,16 +897,18 @@ hipError_t launch_plan(int64_t texels, int64_t points, const void* index, int in
     ProfScope ps(prof, "lookup_plan", stream);
     if (points > 0 && points <= kSmallPoints)
     {
-        const bool whole = (texels + 1) * points <= kSmallPairs;
+        const bool whole = (texels + 1) * std::max<int64_t>(points, 32) <= kSmallPairs;
         p.shift = 0, p.bits = 0, p.keys_in = nullptr, p.points_in = nullptr;
         p.keys_out   = whole ? nullptr : reinterpret_cast<uint32_t*>(ws + l.keys[0]);
         p.points_out = order;
         const size_t lds      = 32 * sizeof(uint32_t) * (small_part(p.n) + 4);
-        const unsigned groups = (p.n + kCountItems - 1) / kCountItems, more = whole ? (unsigned)(texels + kCountItems) / kCountItems : 0u;
+        int log2 = 5;
+        while (log2 < 10 && (texels >> log2) >= kStartsGroups) ++log2;
+        const unsigned groups = (p.n + kCountItems - 1) / kCountItems, more = whole ? (unsigned)(texels >> log2) + 1u : 0u;
         if (i32)
-            hipLaunchKernelGGL(sort_small_kernel<kFromI32>, dim3(groups + more), dim3(kCountThreads), lds, stream, p, starts);
+            hipLaunchKernelGGL(sort_small_kernel<kFromI32>, dim3(groups + more), dim3(kCountThreads), lds, stream, p, starts, log2);
         else
-            hipLaunchKernelGGL(sort_small_kernel<kFromI64>, dim3(groups + more), dim3(kCountThreads), lds, stream, p, starts);
+            hipLaunchKernelGGL(sort_small_kernel<kFromI64>, dim3(groups + more), dim3(kCountThreads), lds, stream, p, starts, log2);
         if (whole) return hipGetLastError();
     }
     int shift = 0;
@@ -919,6 +978,13 @@ int check_stride(const char* name, int64_t stride, int64_t row, int64_t rows, bo
     return TRIPS_OK;
 }
 
+// Rows of one channel, one behind the other, are a column. (It needs no more workspace than they do.)
+TripsLookupDesc as_columns(TripsLookupDesc d)
+{
+    if (d.num_channels == 1 && d.table_stride == 1 && d.values_stride == 1) d.layout = TRIPS_TABLE_COLUMNS;
+    return d;
+}
+
 size_t lookup_bytes(const TripsLookupDesc& d)
 {
     return turns_table(d) ? up256((size_t)d.num_texels * (size_t)row_shape(d).padded * dtype_bytes(d.dtype)) : 0;
@@ -955,6 +1021,9 @@ hipError_t launch_lookup(const TripsLookupDesc& d, const void* table, const void
     return hipGetLastError();
 }
 
+// Points that are few: those of one texel are 16 rounds of loads of its workgroup, at most. (500 points of 300,000 texels in four
+// channels 9.4 us, with the two launches for listed texels 14; 8192 points of 100 texels by the texels' workgroups 141, listed 18.)
+constexpr int64_t few_points(int lanes_log2) { return lanes_log2 < 6 ? 512 : 256; }
 struct GradLayout
 {
     size_t rows, tiles, listed, bytes;
@@ -967,10 +1036,10 @@ GradLayout grad_layout(const TripsLookupDesc& d)
     l.tile = 256;
     while ((int64_t)l.tile * 4096 < d.num_points) l.tile *= 2;
     l.count    = (uint32_t)(d.num_points / l.tile);
-    l.capacity = d.num_points <= l.tile ? 0u : (uint32_t)(d.num_points / (kShort + 1));  // (few points: none is listed)
+    l.capacity = d.num_points <= few_points(r.lanes_log2) ? 0u : (uint32_t)(d.num_points / (kShort + 1));
     size_t o   = 0;
     l.rows     = o;
-    if (d.layout == TRIPS_TABLE_COLUMNS) o += up256((size_t)d.num_points * (size_t)r.padded * dtype_bytes(d.dtype));
+    if (d.layout == TRIPS_TABLE_COLUMNS && d.num_channels > 1) o += up256((size_t)d.num_points * (size_t)r.padded * dtype_bytes(d.dtype));
     l.tiles = o, o += up256((size_t)l.count * (size_t)r.padded * sizeof(float));
     l.listed = o, o += up256((kListHead + (size_t)l.capacity) * sizeof(uint32_t));
     l.bytes = o;
@@ -988,15 +1057,17 @@ hipError_t launch_lookup_backward(const TripsLookupDesc& d, const void* d_values
     p.rows = d_values, p.row = d.values_stride, p.d_table = d_table, p.order = order, p.starts = starts;
     p.tiles = reinterpret_cast<float*>(ws + l.tiles), p.listed = reinterpret_cast<uint32_t*>(ws + l.listed);
     p.texels = d.num_texels, p.table_stride = d.table_stride, p.points = (uint32_t)d.num_points, p.tile = l.tile, p.capacity = l.capacity;
-    p.longest = l.capacity > 0 ? kShort : l.tile;
     p.channels = d.num_channels, p.padded = r.padded, p.lanes_log2 = r.lanes_log2, p.accumulate = d.accumulate != 0, p.scale = d.scale;
-    if (columns && d.num_points > 0)
+    if (columns && d.num_channels == 1)
+        p.row = 1;
+    else if (columns && d.num_points > 0)
     {
         launch_rows(d, r, d_values, ws + l.rows, d.num_points, d.values_stride, stream);
         p.rows = ws + l.rows, p.row = r.padded;
     }
     const long long at_once = 256 >> r.lanes_log2;
-    const dim3 grid((unsigned)std::min<long long>((d.num_texels + at_once - 1) / at_once, kMostRowGroups));
+    const long long across  = std::min((d.num_texels + at_once - 1) / at_once, kMostRowGroups);
+    const dim3 grid((unsigned)across, (unsigned)std::max(1ll, std::min<long long>(r.groups, kFewRowGroups / across)));
     const dim3 tiles(l.count > 0 ? l.count : 1, r.groups), longs(std::min<uint32_t>(l.capacity, kLongGroups), r.groups);
     with_types(d.dtype, r.lane_bytes, columns, [&](auto D, auto V, auto C) {
         constexpr int kD = decltype(D)::value, kV = decltype(V)::value;
@@ -1004,7 +1075,10 @@ hipError_t launch_lookup_backward(const TripsLookupDesc& d, const void* d_values
         const int threads = r.lanes_log2 > 3 ? kWideThreads : 256;
         const size_t lds  = (size_t)kV * threads * sizeof(float);
         if (l.capacity > 0) hipLaunchKernelGGL((lookup_tiles_kernel<kD, kV, kC>), tiles, dim3(threads), lds, stream, p);
-        hipLaunchKernelGGL((lookup_backward_kernel<kD, kV, kC>), grid, dim3(256), 0, stream, p);
+        if (l.capacity > 0)
+            hipLaunchKernelGGL((lookup_backward_kernel<kD, kV, kC, false>), grid, dim3(256), 0, stream, p);
+        else
+            hipLaunchKernelGGL((lookup_backward_kernel<kD, kV, kC, true>), grid, dim3(256), kV * 256 * sizeof(float), stream, p);
         if (l.capacity > 0) hipLaunchKernelGGL((lookup_backward_long_kernel<kD, kV, kC>), longs, dim3(threads), lds, stream, p);
     });
     return hipGetLastError();
@@ -1041,7 +1115,7 @@ int trips_lookup_forward(TripsCtx* ctx, const TripsLookupDesc* desc, const void*
     if (int e = check_workspace(workspace, workspace_bytes, lookup_bytes(d))) return e;
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_error(scope.error, "hipSetDevice");
-    hipError_t e = launch_lookup(d, table, index, values, workspace, reinterpret_cast<hipStream_t>(stream), profiler(ctx));
+    hipError_t e = launch_lookup(as_columns(d), table, index, values, workspace, reinterpret_cast<hipStream_t>(stream), profiler(ctx));
     return e == hipSuccess ? TRIPS_OK : hip_error(e, "lookup launch");
 }
 
@@ -1101,7 +1175,7 @@ int trips_lookup_backward(TripsCtx* ctx, const TripsLookupDesc* desc, const void
     if (int e = check_workspace(workspace, workspace_bytes, grad_layout(d).bytes)) return e;
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_error(scope.error, "hipSetDevice");
-    hipError_t e = launch_lookup_backward(d, d_values, order, starts, d_table, reinterpret_cast<char*>(workspace),
+    hipError_t e = launch_lookup_backward(as_columns(d), d_values, order, starts, d_table, reinterpret_cast<char*>(workspace),
                                           reinterpret_cast<hipStream_t>(stream), profiler(ctx));
     return e == hipSuccess ? TRIPS_OK : hip_error(e, "lookup backward launch");
 }

@@ -258,8 +258,9 @@ std::pair<at::Tensor, at::Tensor> lookup_plan(uintptr_t ctx, uintptr_t stream, c
     return {order, starts};
 }
 
-at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& grad, const at::Tensor& index, const at::Tensor& order, const at::Tensor& starts, int64_t texels,
-                           float scale, int layout, const std::optional<at::Tensor>& out)
+// order, starts: of the plan, or neither: it is made here.
+at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& grad, const at::Tensor& index, std::optional<at::Tensor> order,
+                           std::optional<at::Tensor> starts, int64_t texels, float scale, int layout, const std::optional<at::Tensor>& out)
 {
     int64_t stride;
     check_layout(layout);
@@ -268,7 +269,8 @@ at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& gr
     const bool columns    = layout == TRIPS_TABLE_COLUMNS;
     const int64_t n = g.size(columns ? 1 : 0), c = g.size(columns ? 0 : 1);
     if (n != index.numel()) throw py::value_error("grad: " + std::to_string(n) + " points, index has " + std::to_string(index.numel()));
-    TripsLookupDesc d     = lookup_desc(layout, dtype_of(g), index_dtype, texels, n, c, scale);
+    if (!order) std::tie(order, starts) = lookup_plan(ctx, stream, index, texels);
+    TripsLookupDesc d  = lookup_desc(layout, dtype_of(g), index_dtype, texels, n, c, scale);
     const int64_t rows = columns ? c : texels, row = columns ? texels : c;
     at::Tensor d_table;
     if (out)
@@ -285,7 +287,7 @@ at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& gr
     size_t need = 0;
     check(trips_lookup_backward_workspace_size(&d, &need));
     const at::Tensor workspace = bytes(need, g);
-    check(trips_lookup_backward(reinterpret_cast<TripsCtx*>(ctx), &d, g.data_ptr(), (const int32_t*)order.data_ptr(), (const int32_t*)starts.data_ptr(), d_table.data_ptr(),
+    check(trips_lookup_backward(reinterpret_cast<TripsCtx*>(ctx), &d, g.data_ptr(), (const int32_t*)order->data_ptr(), (const int32_t*)starts->data_ptr(), d_table.data_ptr(),
                                 data(workspace), need, reinterpret_cast<void*>(stream)));
     if (out && !d_table.is_inference()) d_table.unsafeGetTensorImpl()->bump_version();
     return d_table;

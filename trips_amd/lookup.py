@@ -68,11 +68,10 @@ def lookup_plan(index, num_texels):
 def lookup_backward(grad, index, num_texels, scale=1.0, layout=COLUMNS, plan=None, out=None):
     """The table's gradient from that of its looked-up values: [C, T] from [C, N], or [T, C] from [N, C]. plan: lookup_plan of the
     index, where a program keeps it (it is made here otherwise). out: a table gradient to add to, instead of a new one."""
-    if plan is None:
-        plan = lookup_plan(index, num_texels)
-    else:
+    if plan is not None:
         plan.check(index, num_texels)
-    return _host().lookup_backward(*_where(index), grad.detach(), index, plan.order, plan.starts, num_texels, scale, layout, out)
+    order, starts = (None, None) if plan is None else (plan.order, plan.starts)
+    return _host().lookup_backward(*_where(index), grad.detach(), index, order, starts, num_texels, scale, layout, out)
 
 
 class _Lookup(torch.autograd.Function):
