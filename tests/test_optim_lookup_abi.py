@@ -134,7 +134,7 @@ def test_lookup_refuses(desc, call):
 @pytest.mark.parametrize("desc,call", [(d, {}) for d in BAD_DESC] + [
     (dict(table_stride=99), {}), (dict(layout=1, table_stride=3), {}), ({}, dict(d_values=None)), ({}, dict(order=None)), ({}, dict(order=AT + 1)),
     ({}, dict(starts=None)), ({}, dict(d_table=None)), (dict(dtype=3), dict(d_table=AT + 1)), ({}, dict(workspace=None)),
-    ({}, dict(size=700)), (dict(layout=1, table_stride=4, values_stride=4, num_points=1_000_000), dict(size=700))])
+    ({}, dict(size=255)), (dict(num_points=1000), dict(size=700)), (dict(layout=1, table_stride=4, values_stride=4, num_points=1_000_000), dict(size=700))])
 def test_lookup_backward_refuses(desc, call):
     lib = _lib.load()
     rc = lib.trips_lookup_backward(C.addressof(CTX), C.byref(_lookup(**desc)), call.get("d_values", AT), call.get("order", AT),

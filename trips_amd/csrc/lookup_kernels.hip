@@ -541,7 +541,7 @@ constexpr int kWideThreads = 1024; // of a workgroup that adds up rows of more t
 
 struct GradParams
 {
-    const void* rows;  // gradients [points, row]
+    const void* rows;  // gradients [points, row], or columns [channels, row]
     void* d_table;
     const int32_t* order;
     const int32_t* starts;
@@ -563,12 +563,13 @@ __device__ __forceinline__ void segment(const GradParams& p, long long t, uint32
 
 // sum += the rows of the points order[k], k = from, from + step .. below to; V channels from c on. AHEAD rows are on their way at a
 // time: 8 short ones of columns (6M points of 1.5M texels 157 us, with 4 160), 4 of longer rows (8191 tokens 46 us, with 8 47 to 49).
-template <int D, int V, int AHEAD>
+// FROM_COLUMNS: they are columns still (those of the channels behind the last one are the last one's, and go nowhere).
+template <int D, int V, int AHEAD, bool FROM_COLUMNS = false>
 __device__ __forceinline__ void add_rows(const GradParams& p, uint32_t from, uint32_t to, uint32_t step, int c, int count, float (&sum)[V])
 {
     using E       = Element<D>;
     using T       = typename E::type;
-    const T* rows = reinterpret_cast<const T*>(p.rows) + c;
+    const T* rows = reinterpret_cast<const T*>(p.rows) + (FROM_COLUMNS ? 0 : c);
     for (uint32_t k = from; k < to; k += AHEAD * step)
     {
         uint32_t i[AHEAD];
@@ -580,6 +581,12 @@ __device__ __forceinline__ void add_rows(const GradParams& p, uint32_t from, uin
         {
             x[q] = typename Pack<T, V>::type{};
             if (i[q] >= p.points) continue;
+            if (FROM_COLUMNS)
+            {
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[q][e] = rows[min(c + e, p.channels - 1) * p.row + i[q]];
+                continue;
+            }
             const T* row = rows + (long long)i[q] * p.row;
             if (count == V)
                 x[q] = *reinterpret_cast<const typename Pack<T, V>::type*>(row);
@@ -639,7 +646,7 @@ __device__ __forceinline__ void add_threads(float (&sum)[V], float* s, int lanes
     for (int e = 0; e < V; ++e) sum[e] = s[e * blockDim.x + threadIdx.x];
 }
 
-// OUT_COLUMNS: the table's gradient is columns, and the rows were made of columns (whole lanes wide). 6M points of 1.5M texels in
+// OUT_COLUMNS: the table's gradient is columns, and the rows were made of columns (whole lanes wide; not if FEW). 6M points of 1.5M texels in
 // no order: 118 us, 6.3M lines of 128 bytes (6.8 TB/s of them). 8191 tokens: 20 us, the 102 MB of 50,000 rows, mostly zeros, 5.2 TB/s.
 // Groups of lanes' channels go along grid.y where there are few texels, and one behind the other. FEW: so few points that no texel is listed: those with more than
 // kShortOfFew are added up by all of the workgroup that they belong to, one behind the other (at most seven, 1.4 us each).
@@ -680,7 +687,7 @@ __global__ __launch_bounds__(256) void lookup_backward_kernel(const GradParams p
                 const int count = OUT_COLUMNS ? V : min(V, p.channels - c);
 #pragma unroll
                 for (int e = 0; e < V; ++e) sum[e] = 0.f;
-                add_rows<D, V, OUT_COLUMNS ? 8 : 4>(p, from, to, 1, c, count, sum);
+                add_rows<D, V, OUT_COLUMNS && !FEW ? 8 : 4, OUT_COLUMNS && FEW>(p, from, to, 1, c, count, sum);
                 store_sum<D, V, OUT_COLUMNS>(p, t, c, count, sum);
             }
         }
@@ -696,7 +703,7 @@ __global__ __launch_bounds__(256) void lookup_backward_kernel(const GradParams p
                 const int c = first + j * V, count = OUT_COLUMNS ? V : min(V, p.channels - c);
 #pragma unroll
                 for (int e = 0; e < V; ++e) sum[e] = 0.f;
-                if (c < p.channels) add_rows<D, V, OUT_COLUMNS ? 8 : 4>(p, from + (threadIdx.x >> p.lanes_log2), to, at_once, c, count, sum);
+                if (c < p.channels) add_rows<D, V, OUT_COLUMNS && !FEW ? 8 : 4, OUT_COLUMNS && FEW>(p, from + (threadIdx.x >> p.lanes_log2), to, at_once, c, count, sum);
                 add_threads(sum, s, p.lanes_log2);
                 if ((int)threadIdx.x < lanes && c < p.channels) store_sum<D, V, OUT_COLUMNS>(p, tk, c, count, sum);
             }
@@ -1039,7 +1046,7 @@ GradLayout grad_layout(const TripsLookupDesc& d)
     l.capacity = d.num_points <= few_points(r.lanes_log2) ? 0u : (uint32_t)(d.num_points / (kShort + 1));
     size_t o   = 0;
     l.rows     = o;
-    if (d.layout == TRIPS_TABLE_COLUMNS && d.num_channels > 1) o += up256((size_t)d.num_points * (size_t)r.padded * dtype_bytes(d.dtype));
+    if (d.layout == TRIPS_TABLE_COLUMNS && d.num_channels > 1 && l.capacity > 0) o += up256((size_t)d.num_points * (size_t)r.padded * dtype_bytes(d.dtype));
     l.tiles = o, o += up256((size_t)l.count * (size_t)r.padded * sizeof(float));
     l.listed = o, o += up256((kListHead + (size_t)l.capacity) * sizeof(uint32_t));
     l.bytes = o;
@@ -1060,7 +1067,7 @@ hipError_t launch_lookup_backward(const TripsLookupDesc& d, const void* d_values
     p.channels = d.num_channels, p.padded = r.padded, p.lanes_log2 = r.lanes_log2, p.accumulate = d.accumulate != 0, p.scale = d.scale;
     if (columns && d.num_channels == 1)
         p.row = 1;
-    else if (columns && d.num_points > 0)
+    else if (columns && l.capacity > 0)
     {
         launch_rows(d, r, d_values, ws + l.rows, d.num_points, d.values_stride, stream);
         p.rows = ws + l.rows, p.row = r.padded;

@@ -244,13 +244,19 @@ at::Tensor lookup(uintptr_t ctx, uintptr_t stream, const at::Tensor& table, cons
     return values;
 }
 
-std::pair<at::Tensor, at::Tensor> lookup_plan(uintptr_t ctx, uintptr_t stream, const at::Tensor& index, int64_t texels)
+size_t plan_bytes(const at::Tensor& index, int64_t texels)
 {
-    const int index_dtype = index_dtype_of(index);
     if (texels < 0) throw py::value_error("num_texels = " + std::to_string(texels));
     size_t need = 0;
     check(trips_lookup_plan_workspace_size(texels, index.numel(), &need));
-    const auto options = index.options().dtype(at::kInt);
+    return need;
+}
+
+std::pair<at::Tensor, at::Tensor> lookup_plan(uintptr_t ctx, uintptr_t stream, const at::Tensor& index, int64_t texels)
+{
+    const int index_dtype = index_dtype_of(index);
+    const size_t need     = plan_bytes(index, texels);
+    const auto options    = index.options().dtype(at::kInt);
     at::Tensor order = torch::empty({index.numel()}, options), starts = torch::empty({texels + 1}, options);
     const at::Tensor workspace = bytes(need, index), i = index.contiguous();
     check(trips_lookup_plan(reinterpret_cast<TripsCtx*>(ctx), texels, index.numel(), i.data_ptr(), index_dtype, (int32_t*)order.data_ptr(), (int32_t*)starts.data_ptr(),
@@ -259,8 +265,8 @@ std::pair<at::Tensor, at::Tensor> lookup_plan(uintptr_t ctx, uintptr_t stream, c
 }
 
 // order, starts: of the plan, or neither: it is made here.
-at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& grad, const at::Tensor& index, std::optional<at::Tensor> order,
-                           std::optional<at::Tensor> starts, int64_t texels, float scale, int layout, const std::optional<at::Tensor>& out)
+at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& grad, const at::Tensor& index, const std::optional<at::Tensor>& order,
+                           const std::optional<at::Tensor>& starts, int64_t texels, float scale, int layout, const std::optional<at::Tensor>& out)
 {
     int64_t stride;
     check_layout(layout);
@@ -269,7 +275,7 @@ at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& gr
     const bool columns    = layout == TRIPS_TABLE_COLUMNS;
     const int64_t n = g.size(columns ? 1 : 0), c = g.size(columns ? 0 : 1);
     if (n != index.numel()) throw py::value_error("grad: " + std::to_string(n) + " points, index has " + std::to_string(index.numel()));
-    if (!order) std::tie(order, starts) = lookup_plan(ctx, stream, index, texels);
+    const size_t plan = order ? 0 : plan_bytes(index, texels);
     TripsLookupDesc d  = lookup_desc(layout, dtype_of(g), index_dtype, texels, n, c, scale);
     const int64_t rows = columns ? c : texels, row = columns ? texels : c;
     at::Tensor d_table;
@@ -286,9 +292,22 @@ at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& gr
     d.accumulate = out.has_value(), d.table_stride = rows > 1 ? d_table.stride(0) : row, d.values_stride = stride;
     size_t need = 0;
     check(trips_lookup_backward_workspace_size(&d, &need));
-    const at::Tensor workspace = bytes(need, g);
-    check(trips_lookup_backward(reinterpret_cast<TripsCtx*>(ctx), &d, g.data_ptr(), (const int32_t*)order->data_ptr(), (const int32_t*)starts->data_ptr(), d_table.data_ptr(),
-                                data(workspace), need, reinterpret_cast<void*>(stream)));
+    // one piece of memory for it, and for the plan that is made here
+    auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    const size_t at_starts = up(need), at_order = at_starts + (order ? 0 : up((texels + 1) * 4)), at_plan = at_order + (order ? 0 : up(n * 4));
+    const at::Tensor workspace = bytes(at_plan + plan, g);
+    char* w                    = (char*)data(workspace);
+    const int32_t *order_at, *starts_at;
+    if (order)
+        order_at = (const int32_t*)order->data_ptr(), starts_at = (const int32_t*)starts->data_ptr();
+    else
+    {
+        const at::Tensor i = index.contiguous();
+        order_at = (int32_t*)(w + at_order), starts_at = (int32_t*)(w + at_starts);
+        check(trips_lookup_plan(reinterpret_cast<TripsCtx*>(ctx), texels, n, i.data_ptr(), index_dtype, (int32_t*)(w + at_order), (int32_t*)(w + at_starts), w + at_plan, plan,
+                                reinterpret_cast<void*>(stream)));
+    }
+    check(trips_lookup_backward(reinterpret_cast<TripsCtx*>(ctx), &d, g.data_ptr(), order_at, starts_at, d_table.data_ptr(), w, need, reinterpret_cast<void*>(stream)));
     if (out && !d_table.is_inference()) d_table.unsafeGetTensorImpl()->bump_version();
     return d_table;
 }
