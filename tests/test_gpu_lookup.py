@@ -119,6 +119,15 @@ def test_plan_of_few_points_and_many_texels(texels, points):
     _check_plan(lk.lookup_plan(index, texels), index, texels)
 
 
+@pytest.mark.parametrize("how", ["any", "skewed", "outside", "same", "all_outside", "once"])
+@pytest.mark.parametrize("points", [1, 63, 64, 65, 1023, 1025, 8192, 8193, 16_385, 24_577, 32_768, 32_769])
+@pytest.mark.parametrize("texels", [1, 2, 255, 256, 257, 511, 20_000, 65_535, 245_759, 245_760])
+def test_plan_in_one_launch(texels, points, how):
+    """About the sizes at which the kernel, its rounds or the texels of a workgroup change."""
+    index = _index(np.random.default_rng(texels + 3 * points), texels, points, how, torch.int64 if points % 2 else torch.int32)
+    _check_plan(lk.lookup_plan(index, texels), index, texels)
+
+
 def test_plan_of_indexes_beyond_32_bits():
     index = torch.tensor([1 << 32, 5, -(1 << 40), (1 << 31) + 5, 0, 5], device="cuda")
     plan = lk.lookup_plan(index, 6)

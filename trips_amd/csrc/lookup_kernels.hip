@@ -367,16 +367,17 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortPa
     }
 }
 
-// Few points: a point's place is the number of keys below its own and of equal ones before it, counted outright. All keys in LDS,
-// 32 points a workgroup, each by 32 threads with a 32nd of the keys. One launch, on all of the card, where the sort's passes are
-// launches in a row. Bound by the LDS that every key of every workgroup is read from (3.4 us of 11 at 8191 points) and the
-// pairs' two instructions (as much).
+// Few points of a large table: a point's place is the number of keys below its own and of equal ones before it, counted outright. All
+// keys in LDS, 32 points a workgroup, each by 32 threads with a 32nd of the keys. One launch, on all of the card, where the sort's
+// passes are launches in a row. Bound by the LDS that every key of every workgroup is read from (3.4 us of 11 at 8191 points) and
+// the pairs' two instructions (as much).
 // Behind the points' places, if `starts`: the keys below each t, 1 << starts_log2 of them a workgroup, each by as many threads as that
 // leaves: as many as it takes for about two workgroups a CU (16 points of 643k texels: 32 a workgroup 66 us, 1024 6).
 constexpr int kCountThreads = 1024, kCountItems = 32;
 constexpr int kStartsGroups = 480;
-constexpr int64_t kSmallPoints = 8192;             // a workgroup a CU (8192 of 5000 texels 12.5 us, 12288 24; by passes 21 and 22)
-constexpr int64_t kSmallPairs  = (int64_t)1 << 27; // keys and starts
+constexpr int64_t kSmallPoints = 8192;             // a workgroup a CU (8192 of 500,000 texels 12.4 us; 20,000 by passes 29)
+constexpr int64_t kSmallPairs  = (int64_t)1 << 25; // keys and starts (16 points of 980,000 texels 7.5 us, by a launch of its own 9.8;
+                                                   // 500 of 260,000 12.5, 9.5)
 constexpr uint32_t small_part(uint32_t n) { return ((n + 31u) / 32u + 31u) & ~31u; }  // keys of a thread, whole words of signs
 template <int FROM>
 __global__ __launch_bounds__(kCountThreads) void sort_small_kernel(const SortParams p, int32_t* starts, int starts_log2)
@@ -438,6 +439,93 @@ __global__ __launch_bounds__(kCountThreads) void sort_small_kernel(const SortPar
     {
         p.points_out[at] = (int32_t)i;
         if (p.keys_out) p.keys_out[at] = mine;
+    }
+}
+
+// A medium number of points, in one launch: each workgroup takes a range of the texels and reads all keys for it. What lies below the
+// range counts for where its points begin; its own keys are counted by wavefront and texel, each wavefront having a piece of the
+// points, and then put to their places in order. The starts come out of it for nothing. Every workgroup reads every key (from L2),
+// on its way while the counts are cleared, and compares it twice: latency and vector instructions bound it. us: 20,000 points of
+// 5000 texels 10.3 (by passes 22), 8191 of 60,000 8.5 (counted outright and by a launch for the starts 12.5), 32,768 13 (23.5) or, all
+// of one texel, 17.7 (14.5); 65,536, with 64 rounds, no better than the passes.
+constexpr int kRangeThreads = 1024, kRangeWaves = kRangeThreads / 64;
+constexpr int64_t kRangePoints = 1 << 15;
+constexpr int64_t kRangeGroups = 256;  // a workgroup a CU
+constexpr int64_t kMostRange   = 960;  // texels of a workgroup: 60 KB of counts
+template <int ROUNDS, int FROM>
+__global__ __launch_bounds__(kRangeThreads) void sort_range_kernel(const SortParams p, int32_t* starts, uint32_t range, int bits)
+{
+    extern __shared__ uint32_t s_counts[];  // [wavefronts][range]
+    __shared__ uint32_t s_scan[kRangeWaves], s_below;
+    const int lane       = threadIdx.x & 63;
+    const uint32_t lo    = blockIdx.x * range, rounds = (p.n + kRangeThreads - 1) / kRangeThreads;
+    const uint32_t first = (threadIdx.x >> 6) * rounds * 64u + lane;
+    uint32_t* count      = s_counts + (threadIdx.x >> 6) * range;
+    uint32_t key[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) key[r] = sort_key<FROM>(p, min(first + r * 64u, p.n - 1u));
+    for (uint32_t i = threadIdx.x; i < kRangeWaves * range; i += kRangeThreads) s_counts[i] = 0u;
+    if (threadIdx.x == 0) s_below = 0u;
+    __syncthreads();
+    uint32_t below = 0;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+    {
+        if ((uint32_t)r >= rounds || first + r * 64u >= p.n) key[r] = ~0u;
+        below += key[r] < lo ? 1u : 0u;
+        const uint32_t d = key[r] - lo;
+        const unsigned long long mine = __ballot(d < range);
+        if (!mine) continue;
+        // (one addition where they are all of one texel: 64 to one word would be 64 in a row)
+        const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)d, __ffsll((long long)mine) - 1);
+        if (__ballot(d == d0) == mine)
+        {
+            if (lane == 0) atomicAdd(&count[d0], (uint32_t)__popcll(mine));
+        }
+        else if (d < range)
+            atomicAdd(&count[d], 1u);
+    }
+    for (int o = 32; o > 0; o >>= 1) below += (uint32_t)__shfl_xor((int)below, o);
+    if (lane == 0) atomicAdd(&s_below, below);
+    __syncthreads();
+    uint32_t total = 0;
+    if (threadIdx.x < range)
+        for (int w = 0; w < kRangeWaves; ++w)
+        {
+            const uint32_t k = s_counts[w * range + threadIdx.x];
+            s_counts[w * range + threadIdx.x] = total;
+            total += k;
+        }
+    const uint32_t start = s_below + block_scan(total, s_scan) - total;
+    if (threadIdx.x < range)
+    {
+        if (lo + threadIdx.x <= p.texels) starts[lo + threadIdx.x] = (int32_t)start;
+        for (int w = 0; w < kRangeWaves; ++w) s_counts[w * range + threadIdx.x] += start;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+    {
+        const uint32_t d = key[r] - lo;
+        const bool mine  = d < range;
+        unsigned long long same = __ballot(mine);
+        if (!same) continue;
+        // the wavefront's keys of the same texel
+        const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)d, __ffsll((long long)same) - 1);
+        if (__ballot(d == d0) != same)
+        {
+#pragma unroll 1
+            for (int b = 0; b < bits; ++b)
+            {
+                const unsigned long long set = __ballot((d >> b) & 1u);
+                same &= (d >> b) & 1u ? set : ~set;
+            }
+        }
+        const uint32_t before = (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
+        uint32_t at = 0;
+        if (mine && before == 0) at = atomicAdd(&count[d], (uint32_t)__popcll(same));
+        at = (uint32_t)__shfl((int)at, mine ? __ffsll((long long)same) - 1 : 0) + before;
+        if (mine && at < p.n) p.points_out[at] = (int32_t)(first + r * 64u);
     }
 }
 
@@ -902,6 +990,34 @@ hipError_t launch_plan(int64_t texels, int64_t points, const void* index, int in
     p.hist = reinterpret_cast<uint32_t*>(ws + l.hist), p.totals = reinterpret_cast<uint32_t*>(ws + l.totals);
     p.keys_out = nullptr, p.points_out = nullptr;
     ProfScope ps(prof, "lookup_plan", stream);
+    if (points > 0 && points <= kRangePoints && texels + 1 <= kRangeGroups * kMostRange)
+    {
+        const uint32_t range = (uint32_t)((texels + kRangeGroups) / kRangeGroups), groups = (uint32_t)(texels / range) + 1u;
+        const size_t lds     = sizeof(uint32_t) * kRangeWaves * range;
+        const int range_bits = range > 1 ? key_bits(range - 1) : 0;
+        p.points_out         = order;
+        auto launch = [&](auto rounds, auto from)
+        {
+            hipLaunchKernelGGL((sort_range_kernel<decltype(rounds)::value, decltype(from)::value>), dim3(groups), dim3(kRangeThreads), lds, stream, p, starts,
+                               range, range_bits);
+        };
+        auto launch_from = [&](auto rounds)
+        {
+            if (i32)
+                launch(rounds, std::integral_constant<int, kFromI32>{});
+            else
+                launch(rounds, std::integral_constant<int, kFromI64>{});
+        };
+        if (points <= 8 * kRangeThreads)
+            launch_from(std::integral_constant<int, 8>{});
+        else if (points <= 16 * kRangeThreads)
+            launch_from(std::integral_constant<int, 16>{});
+        else if (points <= 24 * kRangeThreads)
+            launch_from(std::integral_constant<int, 24>{});
+        else
+            launch_from(std::integral_constant<int, 32>{});
+        return hipGetLastError();
+    }
     if (points > 0 && points <= kSmallPoints)
     {
         const bool whole = (texels + 1) * std::max<int64_t>(points, 32) <= kSmallPairs;
