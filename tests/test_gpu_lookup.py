@@ -315,6 +315,23 @@ def test_a_plan_with_wild_numbers_stays_inside(layout):
     assert torch.isfinite(got).all() and float(got.max()) <= n
 
 
+@pytest.mark.parametrize("layout", BOTH)
+@pytest.mark.parametrize("points", [40, 400, 5000])
+def test_a_plan_in_which_every_other_texel_has_all_points(points, layout):
+    """More long texels than a sound plan can have: those that find no room are left out, nothing else happens."""
+    t = 3000
+    order = torch.arange(points, dtype=torch.int32, device="cuda")
+    starts = torch.where(torch.arange(t + 1, device="cuda") % 2 == 0, 0, points).to(torch.int32)
+    for channels in (1, 4):
+        grad = torch.ones((points, channels) if layout == lk.ROWS else (channels, points), device="cuda")
+        index = torch.zeros(points, dtype=torch.int32, device="cuda")
+        out = torch.zeros((t, channels) if layout == lk.ROWS else (channels, t), device="cuda")
+        lk.lookup_backward(grad, index, t, layout=layout, plan=lk.LookupPlan(order, starts), out=out)
+        rows = out if layout == lk.ROWS else out.t()
+        assert (rows[1::2] == 0).all()
+        assert ((rows[::2] == points) | (rows[::2] == 0)).all()
+
+
 def test_refusals():
     index = torch.zeros(4, dtype=torch.int32, device="cuda")
     table = torch.zeros(3, 5, device="cuda")
@@ -359,6 +376,30 @@ def test_captured_lookup_and_gradient_replay(layout):
         assert torch.equal(values, lk.lookup(table, index, 2.0, layout))
         assert torch.equal(d_table, lk.lookup_backward(grad, index, texels, 2.0, layout))
         _check_grad(d_table, grad, index, texels, 2.0, layout)
+        torch.randn(50_000, device="cuda").sort()
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("layout", BOTH)
+@pytest.mark.parametrize("texels,points,channels", [(30, 300, 4), (9000, 7000, 1), (400_000, 600, 6), (500, 50_000, 5)])
+def test_captured_calls_of_other_sizes_replay(texels, points, channels, layout):
+    rng = np.random.default_rng(points)
+    index = _index(rng, texels, points, "skewed", torch.int64)
+    grad = _matrix(rng, *((points, channels) if layout == lk.ROWS else (channels, points)), "bf16").contiguous()
+    lk.lookup_backward(grad, index, texels, 1.0, layout)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        plan = lk.lookup_plan(index, texels)
+        d_table = lk.lookup_backward(grad, index, texels, 1.0, layout)
+    for k in range(3):
+        index.copy_(_index(rng, texels, points, ("any", "same", "outside")[k]))
+        grad.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_plan(plan, index, texels)
+        _check_grad(d_table, grad, index, texels, 1.0, layout)
+        assert torch.equal(d_table, lk.lookup_backward(grad, index, texels, 1.0, layout))
         torch.randn(50_000, device="cuda").sort()
         torch.cuda.synchronize()
 

@@ -5,7 +5,7 @@
 // Large calls are bound by memory: lookup and gradient in no order by the lines of 128 bytes that each scattered request moves
 // (7 TB/s of lines), short ones and those of whole rows by latency or by the table's bytes; the order of the points by the three
 // passes of its sort. us a call: 6M points of 1.5M texels in four channels 117, their gradient 157, their order 132; 8191 tokens of
-// a table of 50,000 rows of 1024 bytes 7.5, with order and gradient 46. Below each kernel its own share.
+// a table of 50,000 rows of 1024 bfloat16 numbers 7.5, with order and gradient 42. Below each kernel its own share.
 #include <algorithm>
 #include <type_traits>
 
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void lookup_columns_kernel(const LookupParams 
 
 // V elements a lane, 1 << lanes_log2 lanes a point. OUT_COLUMNS: the values are columns (and the table's rows whole lanes wide).
 // 6M points of 24 MB of rows in no order: 107 us, 6.0M lines of 128 bytes that no L2 holds (7.1 TB/s of them; an XCD's L2 has 4 MB).
-// 8191 rows of 1024 bytes: 7.9 us, of which the bytes are 3: an index, then its row, with one wave of workgroups on the card.
+// 8191 rows of 1024 bfloat16 numbers: 7.9 us where it starts alone, 5.4 for the bytes: an index, then its row, in one wave of workgroups.
 template <int D, int V, bool OUT_COLUMNS>
 __global__ __launch_bounds__(256) void lookup_rows_kernel(const LookupParams p)
 {
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(const LookupParams p)
 // ---- the order of the points: a stable radix sort, least significant digit first ----
 
 // A tile: 1024 threads with 2 points each below 2^20 points, with 4 below 2^22, with 6 above (two tiles a CU at a time in any case;
-// us: 20k points 22 with 2 and 31 with 8 of 512 threads, 1M 56 and with 6 59, 2M 68 with 4 and 74 with 6, 6M 147 with 4 and 132 with 6).
+// us: 20k points, by passes, 22 with 2 and 31 with 8 of 512 threads, 1M 56 and with 6 59, 2M 68 with 4 and 74 with 6, 6M 147 with 4 and 132 with 6).
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int sort_items(int64_t points) { return points < (1 << 20) ? 2 : points < (1 << 22) ? 4 : 6; }
 constexpr int kDigits = 256;
@@ -650,7 +650,7 @@ __device__ __forceinline__ void segment(const GradParams& p, long long t, uint32
 }
 
 // sum += the rows of the points order[k], k = from, from + step .. below to; V channels from c on. AHEAD rows are on their way at a
-// time: 8 short ones of columns (6M points of 1.5M texels 157 us, with 4 160), 4 of longer rows (8191 tokens 46 us, with 8 47 to 49).
+// time: 8 short ones of columns (6M points of 1.5M texels 157 us, with 4 160), 4 of longer rows (8191 tokens with 8 1 to 3 us more).
 // FROM_COLUMNS: they are columns still (those of the channels behind the last one are the last one's, and go nowhere).
 template <int D, int V, int AHEAD, bool FROM_COLUMNS = false>
 __device__ __forceinline__ void add_rows(const GradParams& p, uint32_t from, uint32_t to, uint32_t step, int c, int count, float (&sum)[V])
