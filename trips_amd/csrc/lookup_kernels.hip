@@ -98,7 +98,9 @@ __global__ __launch_bounds__(256) void lookup_rows_kernel(const LookupParams p)
     const int lanes = 1 << p.lanes_log2, j = threadIdx.x & (lanes - 1), at_once = 256 >> p.lanes_log2;
     const T* table       = reinterpret_cast<const T*>(p.table);
     T* values            = reinterpret_cast<T*>(p.values);
-    constexpr int POINTS = 4;  // whose rows a lane has on the way at a time
+    // whose rows a lane has on the way at a time (of eight columns the addresses of four points took 188 registers: 2M points of 500,000
+    // texels in 16 bfloat16 channels 62 us, with two 57)
+    constexpr int POINTS = OUT_COLUMNS && V == 8 ? 2 : 4;
     for (long long base = (long long)blockIdx.x * at_once * POINTS; base < p.points; base += (long long)gridDim.x * at_once * POINTS)
     {
         long long t[POINTS];
@@ -902,8 +904,8 @@ RowShape row_shape(const TripsLookupDesc& d)
     return r;
 }
 
-// f(type, elements of a lane, whether columns) with all three as constants
-template <typename F>
+// f(type, elements of a lane, whether columns) with all three as constants; SINGLE: with the one channel of a lane, too
+template <bool SINGLE, typename F>
 void with_types(int dtype, int lane_bytes, bool columns, const F& f)
 {
     auto with_columns = [&](auto d, auto v)
@@ -916,9 +918,9 @@ void with_types(int dtype, int lane_bytes, bool columns, const F& f)
     auto with_lane = [&](auto d)
     {
         constexpr int size = decltype(d)::value == TRIPS_DTYPE_F32 ? 4 : 2;
-        if (lane_bytes == size)
-            f(d, std::integral_constant<int, 1>{}, std::true_type{});  // (columns alone)
-        else if (lane_bytes == 8)
+        if constexpr (SINGLE)
+            if (lane_bytes == size) return f(d, std::integral_constant<int, 1>{}, std::true_type{});  // (columns alone)
+        if (lane_bytes == 8)
             f(d, std::integral_constant<int, 8 / size>{}, std::true_type{});  // (columns alone)
         else
             with_columns(d, std::integral_constant<int, 16 / size>{});
@@ -936,7 +938,7 @@ void launch_rows(const TripsLookupDesc& d, const RowShape& r, const void* column
 {
     const int v = r.lane_bytes / dtype_bytes(d.dtype);
     const dim3 grid((unsigned)((n + 255) / 256), (unsigned)(r.padded / v));
-    with_types(d.dtype, r.lane_bytes, true, [&](auto D, auto V, auto) {
+    with_types<false>(d.dtype, r.lane_bytes, true, [&](auto D, auto V, auto) {
         hipLaunchKernelGGL((rows_kernel<decltype(D)::value, decltype(V)::value>), grid, dim3(256), 0, stream, columns, rows, n, stride,
                            d.num_channels, r.padded);
     });
@@ -1126,7 +1128,7 @@ hipError_t launch_lookup(const TripsLookupDesc& d, const void* table, const void
     if (columns && !turns_table(d))
     {
         const dim3 grid((unsigned)((d.num_points + 255) / 256), (unsigned)((d.num_channels + kColumnGroup - 1) / kColumnGroup));
-        with_types(d.dtype, 16, true, [&](auto D, auto, auto) {
+        with_types<false>(d.dtype, 16, true, [&](auto D, auto, auto) {
             hipLaunchKernelGGL(lookup_columns_kernel<decltype(D)::value>, grid, dim3(256), 0, stream, p);
         });
         return hipGetLastError();
@@ -1138,7 +1140,7 @@ hipError_t launch_lookup(const TripsLookupDesc& d, const void* table, const void
     }
     const long long at_once = 4ll * (256 >> r.lanes_log2);
     const dim3 grid((unsigned)std::min<long long>((d.num_points + at_once - 1) / at_once, kMostRowGroups));
-    with_types(d.dtype, r.lane_bytes, columns, [&](auto D, auto V, auto C) {
+    with_types<false>(d.dtype, r.lane_bytes, columns, [&](auto D, auto V, auto C) {
         hipLaunchKernelGGL((lookup_rows_kernel<decltype(D)::value, decltype(V)::value, decltype(C)::value>), grid, dim3(256), 0, stream, p);
     });
     return hipGetLastError();
@@ -1192,7 +1194,7 @@ hipError_t launch_lookup_backward(const TripsLookupDesc& d, const void* d_values
     const long long across  = std::min((d.num_texels + at_once - 1) / at_once, kMostRowGroups);
     const dim3 grid((unsigned)across, (unsigned)std::max(1ll, std::min<long long>(r.groups, kFewRowGroups / across)));
     const dim3 tiles(l.count > 0 ? l.count : 1, r.groups), longs(std::min<uint32_t>(l.capacity, kLongGroups), r.groups);
-    with_types(d.dtype, r.lane_bytes, columns, [&](auto D, auto V, auto C) {
+    with_types<true>(d.dtype, r.lane_bytes, columns, [&](auto D, auto V, auto C) {
         constexpr int kD = decltype(D)::value, kV = decltype(V)::value;
         constexpr bool kC = decltype(C)::value;
         const int threads = r.lanes_log2 > 3 ? kWideThreads : 256;
