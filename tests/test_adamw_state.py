@@ -1,0 +1,39 @@
+"""What AdamW keeps besides its kernels, on the CPU: its fields over load_state_dict, copies and refusals before a step."""
+import pytest
+import torch
+
+from trips_amd.adamw import AdamW
+
+
+def _optimiser(n=300, **kw):
+    """An optimiser with the state that a first step would have made."""
+    p = torch.nn.Parameter(torch.ones(n))
+    opt = AdamW([p], **kw)
+    opt.state[p] = dict(step=torch.ones((), dtype=torch.int32), first_moment=torch.full((n,), 0.25), second_moment=torch.full((n,), 0.5))
+    return opt, p
+
+
+def test_load_state_dict_keeps_copies_and_workspaces():
+    opt, p = _optimiser()
+    copy = torch.zeros(300, dtype=torch.bfloat16)
+    opt.set_copy(p, copy)
+    workspace, older, norm = torch.zeros(8), torch.zeros(4), torch.zeros(2)
+    opt._workspace, opt._workspace_for, opt._norm, opt.grad_norm = workspace, 1, norm, norm
+    opt._kept.append((older, norm))
+    opt.load_state_dict(opt.state_dict())
+    assert opt._copies[p] is copy
+    assert opt._workspace is workspace and opt._norm is norm and opt.grad_norm is norm
+    assert any(older is t for kept in opt._kept for t in kept)
+
+
+def test_a_copied_optimiser_has_a_workspace_of_its_own():
+    import copy
+    import pickle
+    opt, p = _optimiser(max_grad_norm=0.5, seed=3)
+    opt.set_copy(p, torch.zeros(300))
+    opt._workspace, opt._workspace_for, opt._norm, opt.grad_norm = torch.zeros(8), 1, torch.zeros(2), torch.zeros(2)
+    for twin in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert twin._workspace is None and twin.grad_norm is None and twin._kept == [] and twin._copies == {}
+        assert (twin.max_grad_norm, twin.seed) == (0.5, 3)
+        q = twin.param_groups[0]["params"][0]
+        assert q is not p and torch.equal(twin.state[q]["first_moment"], opt.state[p]["first_moment"])

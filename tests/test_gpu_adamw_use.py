@@ -1,0 +1,30 @@
+"""AdamW as programs use it: resumed, captured, with copies that the forward reads, on other streams."""
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_adamw import TYPES, _check_step, _places, _state, _tensors
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_and_captured_workspaces_after_load_state_dict(bits):
+    """set_copy, then a checkpoint: later steps still write the copy; nor does what was captured lose its workspace."""
+    from trips_amd.adamw import AdamW
+    params, gs = _tensors((300, 5000), "f32", "f32", 21)
+    given = dict(zip(params, gs))
+    opt = AdamW(params, state_bits=bits, min_8bit_size=0, max_grad_norm=0.5)
+    copies = [p.detach().to(torch.bfloat16) for p in params]
+    for p, c in zip(params, copies):
+        opt.set_copy(p, c)
+    opt.step(grads=given)
+    workspace, norm = opt._workspace.data_ptr(), opt.grad_norm.data_ptr()
+    saved = opt.state_dict()
+    opt.load_state_dict(saved)
+    assert opt._workspace.data_ptr() == workspace and opt.grad_norm.data_ptr() == norm
+    before = _state(opt, params)
+    opt.step(grads=given)
+    _check_step(opt, before, params, gs, 2, factor=float(opt.grad_norm[1]), places=_places(params))
+    for p, c, w in zip(params, copies, before):
+        assert torch.equal(c, p.detach().to(torch.bfloat16)) and not np.array_equal(p.detach().double().cpu().numpy(), w[0])

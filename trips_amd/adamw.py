@@ -80,7 +80,7 @@ class AdamW(torch.optim.Optimizer):
 
     def set_copy(self, p, copy):
         """Every step writes the new value of parameter `p` to `copy` as well (a contiguous tensor of its size, in any of the
-        three types), before it is rounded to p's own type. None ends that."""
+        three types), before it is rounded to p's own type. None ends that. A copied or unpickled optimiser has no copies yet."""
         if copy is None:
             self._copies.pop(p, None)
             return
@@ -151,8 +151,10 @@ class AdamW(torch.optim.Optimizer):
         return {**super().__getstate__(), **{k: getattr(self, k) for k in self._OWN}}
 
     def __setstate__(self, state):
-        # (a copy has its own workspace, and no copies of parameters yet)
-        self.grad_norm, self._workspace, self._kept, self._copies = None, None, [], {}
+        # Of an optimiser that is being copied or unpickled, which has none of these yet: a workspace of its own, and no copies
+        # of its parameters. load_state_dict() ends here as well, where what there is stays.
+        for name, value in (("grad_norm", None), ("_workspace", None), ("_kept", []), ("_copies", {})):
+            self.__dict__.setdefault(name, value)
         super().__setstate__(state)
 
     @torch.no_grad()
