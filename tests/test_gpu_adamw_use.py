@@ -28,3 +28,38 @@ def test_copies_and_captured_workspaces_after_load_state_dict(bits):
     _check_step(opt, before, params, gs, 2, factor=float(opt.grad_norm[1]), places=_places(params))
     for p, c, w in zip(params, copies, before):
         assert torch.equal(c, p.detach().to(torch.bfloat16)) and not np.array_equal(p.detach().double().cpu().numpy(), w[0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_backward_pass_that_needs_an_older_copy_raises(bits):
+    """A step writes the copy: what autograd saved of it is gone, as with the parameter itself."""
+    from trips_amd.adamw import AdamW
+    params, gs = _tensors((300,), "f32", "f32", 22)
+    opt = AdamW(params, state_bits=bits, min_8bit_size=0)
+    copy = params[0].detach().to(torch.bfloat16)
+    opt.set_copy(params[0], copy)
+    opt.step(grads={params[0]: gs[0]})
+    x = torch.ones(300, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    loss = (x * copy).sum()
+    version = copy._version
+    opt.step(grads={params[0]: gs[0]})
+    assert copy._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        copy = params[0].detach().to(torch.float16)
+    opt.set_copy(params[0], copy)
+    opt.step(grads={params[0]: gs[0]})  # (has no version)
+    assert torch.equal(copy, params[0].detach().to(torch.float16))
+
+
+def test_a_backward_pass_that_needs_an_older_norm_raises():
+    from trips_amd.adamw import AdamW
+    params, gs = _tensors((300,), "f32", "f32", 23)
+    opt = AdamW(params, max_grad_norm=0.5)
+    opt.step(grads={params[0]: gs[0]})
+    x = torch.ones(2, device="cuda", requires_grad=True)
+    loss = (x * opt.grad_norm).sum()
+    opt.step(grads={params[0]: gs[0]})
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

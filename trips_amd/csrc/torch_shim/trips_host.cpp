@@ -120,10 +120,11 @@ class StepTable
                     const at::Tensor& copy = tensor_of(c, "a copy");
                     t.copy = copy.data_ptr(), t.copy_dtype = dtype_of(copy);
                     if (copy.numel() != t.n) throw std::runtime_error("a copy of " + std::to_string(copy.numel()) + " elements for a parameter of " + std::to_string(t.n));
+                    written.push_back(copy);
                 }
                 t.lr = lr, t.beta1 = b1, t.beta2 = b2, t.eps = eps, t.weight_decay = decay;
                 tensors.push_back(t);
-                params.push_back(p);
+                written.push_back(p);
             }
         }
         return {(int)tensors.size(), device};
@@ -138,18 +139,19 @@ class StepTable
         o.compute_norm = compute_norm, o.max_norm = max_norm, o.loss_scale = loss_scale;
         const int rc = trips_adamw_step(reinterpret_cast<TripsCtx*>(ctx), tensors.data(), (int)tensors.size(), &o, workspace.data_ptr(), workspace.nbytes(),
                                         reinterpret_cast<void*>(stream));
+        if (compute_norm && grad_norm) written.push_back(*grad_norm);
         if (rc == TRIPS_OK)  // (a backward pass that needs the old values raises)
-            for (const at::Tensor& p : params)
-                if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+            for (const at::Tensor& t : written)
+                if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
         clear();
         return rc;
     }
 
-    void clear() { tensors.clear(), params.clear(), temporaries.clear(); }
+    void clear() { tensors.clear(), written.clear(), temporaries.clear(); }
 
    private:
     std::vector<TripsAdamWTensor> tensors;
-    std::vector<at::Tensor> params, temporaries;
+    std::vector<at::Tensor> written, temporaries;  // parameters, their copies and the norm
 };
 
 class NormTable
