@@ -1,0 +1,82 @@
+"""Lookups as programs use them: in front of the splat, under modes that torch has to see, with plans that are kept."""
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_operator import _info
+from tests.test_gpu_shared_texels import _scene
+from trips_amd import lookup as lk
+
+pytestmark = pytest.mark.gpu
+
+
+def _shared(seed, kept=False, **kw):
+    from trips_amd.renderer import NeuralScene
+    sc = _scene(seed, n=600)
+    ns = NeuralScene.from_arrays(sc)
+    if kept:
+        ns.plan_texels()
+    return ns, _info(sc, ns, shared_texels_in_order=True, **kw)
+
+
+def _render_of(ns, info):
+    from trips_amd.renderer import BlendPointCloud
+
+    def render(t):
+        ns.texture.texture = t
+        return tuple(BlendPointCloud(info))
+    return render
+
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("train", [False, True])
+def test_forward_mode_of_shared_texels_is_refused(train, kept):
+    import torch.autograd.forward_ad as fwad
+    from trips_amd.renderer import BlendPointCloud
+    ns, info = _shared(61, kept, train=train)
+    plain = ns.texture.texture
+    with torch.no_grad(), fwad.dual_level():
+        ns.texture.texture = fwad.make_dual(plain, torch.ones_like(plain))
+        with pytest.raises(NotImplementedError):
+            BlendPointCloud(info)
+        ns.texture.texture = plain
+        confidence = ns.texture.confidence_value_of_point
+        ns.texture.confidence_value_of_point = fwad.make_dual(confidence, torch.ones_like(confidence))
+        with pytest.raises(NotImplementedError):
+            BlendPointCloud(info)
+
+
+@pytest.mark.parametrize("transform", ["vmap", "grad", "jvp", "functionalize"])
+def test_functional_transforms_of_shared_texels_are_refused(transform):
+    ns, info = _shared(62, train=False)
+    render, texture, f = _render_of(ns, info), ns.texture.texture.detach(), torch.func
+    call = dict(vmap=lambda: f.vmap(render)(texture[None]), grad=lambda: f.grad(lambda t: render(t)[0].sum())(texture),
+                jvp=lambda: f.jvp(render, (texture,), (texture,)), functionalize=lambda: f.functionalize(render)(texture))[transform]
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        call()
+
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("train", [False, True])
+def test_a_trace_of_shared_texels_renders_what_it_is_given(train, kept):
+    ns, info = _shared(63, kept, train=train)
+    render, texture = _render_of(ns, info), ns.texture.texture.detach().clone()
+    with torch.no_grad():
+        traced = torch.jit.trace(render, (texture,), check_trace=False)
+        want, got = render(2 * texture), traced(2 * texture)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and float(want[0].abs().max()) > 0
+
+
+def test_lookups_without_a_graph_under_modes():
+    import torch.autograd.forward_ad as fwad
+    index = torch.tensor([2, 0, -1, 3], dtype=torch.int32, device="cuda")
+    table = torch.randn(4, 3, device="cuda")
+    look = lambda t: lk.lookup(t, index, 2.0, lk.ROWS)
+    with torch.no_grad():
+        traced = torch.jit.trace(look, (table,), check_trace=False)
+        assert torch.equal(traced(3 * table), look(3 * table))
+        with fwad.dual_level(), pytest.raises(NotImplementedError):
+            look(fwad.make_dual(table, table))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(look)(table[None])
+        assert torch.equal(torch.func.vmap(lambda x: x + look(table).sum())(torch.zeros(2, device="cuda")), look(table).sum().expand(2))

@@ -5,12 +5,15 @@ A scene's texture [C,T] read by t_index (which the splat otherwise does inside i
 adds up with atomics where points share a texel), or any other table of learned rows. The gradient of a shared entry is
 summed in the order of its points: the same bits every time.
 """
+import contextlib
+
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import abi
 from ._host import host as _host
-from .renderer import _stream_ptr, get_context
+from .renderer import _stream_ptr, _untraced, get_context
 
 COLUMNS, ROWS = abi.TRIPS_TABLE_COLUMNS, abi.TRIPS_TABLE_ROWS
 
@@ -21,6 +24,28 @@ def _where(index):
         return 0, 0
     ctx = get_context(index.device)
     return ctx.ctx.value, _stream_ptr(ctx.device)
+
+
+def _needs_function(table, index):
+    """Whether torch has to see a lookup: to record it (a graph, a trace) or to refuse it (forward-mode duals, a functional
+    transform that follows one of the tensors). The kernels' call by itself would lose the derivative, or leave a trace a constant."""
+    return (table.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(table, index)
+
+
+def _transformed(*tensors):
+    if not torch._C._are_functorch_transforms_active():
+        return False
+    return any(torch._C._functorch.is_functorch_wrapped_tensor(t) or torch._C._functorch.is_functionaltensor(t) for t in tensors)
+
+
+def _refuse_unseen(what, *tensors):
+    """For what has no autograd function: nothing is computed that torch would take for something else."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} is not recorded by a trace: call it before")
+    if _transformed(*tensors):
+        raise RuntimeError(f"{what} of tensors that a functional transform follows is not supported")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 class LookupPlan:
@@ -62,22 +87,32 @@ def own_index(index, num_texels):
 
 def lookup_plan(index, num_texels):
     """The order of the points by their texel. Indexes outside [0, num_texels) come last and count for no texel."""
+    _refuse_unseen("lookup_plan", index)
     return LookupPlan(*_host().lookup_plan(*_where(index), index, num_texels), index)
 
 
 def lookup_backward(grad, index, num_texels, scale=1.0, layout=COLUMNS, plan=None, out=None):
     """The table's gradient from that of its looked-up values: [C, T] from [C, N], or [T, C] from [N, C]. plan: lookup_plan of the
     index, where a program keeps it (it is made here otherwise). out: a table gradient to add to, instead of a new one."""
+    _refuse_unseen("lookup_backward", grad, index)
     if plan is not None:
         plan.check(index, num_texels)
     order, starts = (None, None) if plan is None else (plan.order, plan.starts)
     return _host().lookup_backward(*_where(index), grad.detach(), index, order, starts, num_texels, scale, layout, out)
 
 
+def _check_plan(table, index, layout, plan):
+    if plan is not None and table.dim() == 2:
+        plan.check(index, table.shape[1] if layout == COLUMNS else table.shape[0])
+
+
 class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, index, scale, layout, plan):
-        values = _host().lookup(*_where(index), table.detach(), index, scale, layout)
+        # The plan is checked here for a trace, which may be run with another index; what a trace sees of a function is its call alone.
+        with _untraced() if torch.jit.is_tracing() else contextlib.nullcontext():
+            _check_plan(table, index, layout, plan)
+            values = _host().lookup(*_where(index), table.detach(), index, scale, layout)
         ctx.save_for_backward(index)
         ctx.args = (table.shape[1] if layout == COLUMNS else table.shape[0], scale, layout, plan)
         return values
@@ -94,8 +129,7 @@ def lookup(table, index, scale=1.0, layout=COLUMNS, plan=None):
     """scale times the entries of the table that the index names: [C, N] from a table [C, T] (COLUMNS, a scene's texture), or
     [N, C] from [T, C] (ROWS); N = index.numel(). Zeros where an index is outside the table (padding). Differentiable in the
     table; plan: lookup_plan of the index, for the gradient, where a program keeps it."""
-    if plan is not None and table.dim() == 2:
-        plan.check(index, table.shape[1] if layout == COLUMNS else table.shape[0])
-    if table.requires_grad and torch.is_grad_enabled():
+    if _needs_function(table, index):
         return _Lookup.apply(table, index, scale, layout, plan)
+    _check_plan(table, index, layout, plan)
     return _host().lookup(*_where(index), table.detach(), index, scale, layout)

@@ -11,6 +11,7 @@ Same names and argument meaning as the reference (paths relative to the referenc
 torch is used for device memory, streams and the autograd graph only; all computation happens in
 libtrips_splat.so. There is no fallback path: without the library (or without a GPU) these calls raise.
 """
+import contextlib
 import copy
 import ctypes as C
 import functools
@@ -31,6 +32,17 @@ def _ptr(t):
 def _stream_ptr(device):
     """hipStream_t of torch's current stream on `device` (a torch.device with an index)."""
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+@contextlib.contextmanager
+def _untraced():
+    """What runs inside is no part of a trace."""
+    state = torch._C._get_tracing_state()
+    torch._C._set_tracing_state(None)
+    try:
+        yield
+    finally:
+        torch._C._set_tracing_state(state)
 
 
 class SplatContext:
@@ -454,10 +466,12 @@ def _with_own_texels(info):
         info.cache = PointRendererCache()
     points, index = sc.point_cloud_cuda, sc.point_cloud_cuda.t_index
     plan = getattr(sc, "texel_plan", None)
-    if plan is None:
-        plan = lookup.lookup_plan(index, int(sc.texture.texture.shape[1])) if info.train else None
-    # a point whose texel is outside the table is left out, and reported, as ever
-    own = lookup.own_index(index, int(sc.texture.texture.shape[1])) if plan is None else plan.own_index(index)
+    texels = int(sc.texture.texture.shape[1])
+    with _untraced():  # (to a trace the index is a constant, and so is what is made of it)
+        if plan is None:
+            plan = lookup.lookup_plan(index, texels) if info.train else None
+        # a point whose texel is outside the table is left out, and reported, as ever
+        own = lookup.own_index(index, texels) if plan is None else plan.own_index(index)
     look = functools.partial(lookup.lookup, index=index, layout=lookup.COLUMNS, plan=plan)
     scene, inner = copy.copy(sc), copy.copy(info)
     scene.texture = _Namespace(texture=look(sc.texture.texture), background_color=sc.texture.background_color,
