@@ -80,3 +80,27 @@ def test_lookups_without_a_graph_under_modes():
         with pytest.raises(RuntimeError):
             torch.func.vmap(look)(table[None])
         assert torch.equal(torch.func.vmap(lambda x: x + look(table).sum())(torch.zeros(2, device="cuda")), look(table).sum().expand(2))
+
+
+@pytest.mark.parametrize("by_scene", [True, False])
+def test_a_render_between_a_capture_and_its_first_replay(by_scene):
+    """The first render with a plan is captured; an eager one before the replay, and the replays, give the same images."""
+    from trips_amd.renderer import BlendPointCloud, NeuralScene
+    sc = _scene(64, n=600)
+    ns = NeuralScene.from_arrays(sc)
+    with torch.no_grad():
+        want = [o.clone() for o in BlendPointCloud(_info(sc, ns, train=False, shared_texels_in_order=True))]
+        if by_scene:
+            ns.plan_texels()
+        else:
+            ns.texel_plan = lk.lookup_plan(ns.point_cloud_cuda.t_index, ns.texture.texture.shape[1])
+        captured, eager = (_info(sc, ns, train=False, shared_texels_in_order=True) for _ in range(2))
+        torch.cuda.synchronize()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=side):
+            got = BlendPointCloud(captured)
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(BlendPointCloud(eager), want))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))

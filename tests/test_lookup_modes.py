@@ -22,7 +22,7 @@ class _Host:
 
     @staticmethod
     def lookup_plan(ctx, stream, index, texels):
-        i = index.numpy()
+        i = index.numpy().reshape(-1)
         return (torch.from_numpy(np.argsort(i, kind="stable").astype(np.int32)),
                 torch.from_numpy(np.searchsorted(np.sort(i), np.arange(texels + 1)).astype(np.int32)))
 

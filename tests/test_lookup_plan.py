@@ -1,0 +1,37 @@
+"""What a LookupPlan keeps, on the CPU; what the kernels would return is stood in for."""
+import pytest
+import torch
+
+from tests.test_lookup_modes import _Host
+from trips_amd import lookup as lk
+
+
+@pytest.fixture(autouse=True)
+def host(monkeypatch):
+    monkeypatch.setattr(lk, "_host", lambda: _Host)
+
+
+def test_a_plans_own_index_is_kept_only_where_the_program_made_it():
+    """A tensor that a render makes on the way (in a capture, on its own stream) is no one else's."""
+    index = torch.tensor([2, 0, -1, 3], dtype=torch.int32)
+    plan = lk.LookupPlan(torch.tensor([1, 0, 3, 2], dtype=torch.int32), torch.tensor([0, 1, 1, 2, 3], dtype=torch.int32), index)
+    first, second = plan.own_index(index), plan.own_index(index)
+    assert first.tolist() == second.tolist() == [0, 1, -1, 3]
+    assert first.data_ptr() != second.data_ptr()
+    plan.keep_own_index()
+    kept = plan.own_index(index)
+    assert kept.tolist() == [0, 1, -1, 3] and plan.own_index(index) is kept
+    index[1] = 2
+    with pytest.raises(ValueError, match="changed"):
+        plan.own_index(index)
+
+
+def test_plan_texels_keeps_it():
+    from trips_amd.renderer import NeuralScene
+    scene = NeuralScene(texture=torch.zeros(2, 4), background_color=torch.zeros(2), confidence=torch.zeros(1, 4), position=torch.zeros(4, 4),
+                        point_size=torch.zeros(4, 1), index=torch.tensor([[2], [0], [2], [3]], dtype=torch.int32),
+                        poses_se3=torch.zeros(1, 7, dtype=torch.float64), intrinsics=torch.zeros(1, 13))
+    scene.plan_texels()
+    index = scene.point_cloud_cuda.t_index
+    assert scene.texel_plan.own_index(index) is scene.texel_plan.own_index(index)
+    assert scene.texel_plan.own_index(index).tolist() == [[0], [1], [2], [3]]

@@ -50,7 +50,7 @@ def _refuse_unseen(what, *tensors):
 
 class LookupPlan:
     """The points of an index in the order of their texels: order [N] and starts [T + 1] (int32; see trips_lookup_plan).
-    It belongs to the index that it was made of, as it was then."""
+    It belongs to the index that it was made of, as it was then; made in a capture, it holds nothing before the first replay."""
 
     def __init__(self, order, starts, index=None):
         if order.dtype != torch.int32 or starts.dtype != torch.int32 or not order.is_contiguous() or not starts.is_contiguous() \
@@ -71,12 +71,15 @@ class LookupPlan:
                                 or (None if index.is_inference() else index._version) != self.version):
             raise ValueError("the plan was made of another index, or the index was changed since")
 
+    def keep_own_index(self):
+        """Makes own_index() of the plan's index, on the current stream, like the plan itself, for all that use the plan."""
+        self._own = own_index(self.index, self.starts.numel() - 1)
+
     def own_index(self, index):
-        """own_index() of the plan's index, made once."""
+        """own_index() of the plan's index: the one that keep_own_index() made, or a new one (a call that made and kept it on the way
+        would leave it to others before its capture was replayed, or to another stream before it was written)."""
         self.check(index, self.starts.numel() - 1)
-        if self._own is None:
-            self._own = own_index(index, self.starts.numel() - 1)
-        return self._own
+        return own_index(index, self.starts.numel() - 1) if self._own is None else self._own
 
 
 def own_index(index, num_texels):

@@ -528,9 +528,11 @@ class NeuralScene:
 
     def plan_texels(self):
         """Keeps the order of the points by their texels for RenderParams.shared_texels_in_order; to be called again after
-        t_index or the number of texels has changed (an old plan is refused)."""
+        t_index or the number of texels has changed (an old plan is refused). What it keeps is written on the current stream."""
         from . import lookup
-        self.texel_plan = lookup.lookup_plan(self.point_cloud_cuda.t_index, int(self.texture.texture.shape[1]))
+        plan = lookup.lookup_plan(self.point_cloud_cuda.t_index, int(self.texture.texture.shape[1]))
+        plan.keep_own_index()
+        self.texel_plan = plan
 
     @staticmethod
     def from_arrays(scene, device="cuda", requires_grad=False):
