@@ -104,3 +104,31 @@ def test_a_render_between_a_capture_and_its_first_replay(by_scene):
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("layout", [lk.COLUMNS, lk.ROWS])
+def test_gradients_with_a_kept_plan_under_save_on_cpu(layout):
+    rng = np.random.default_rng(7)
+    index = torch.as_tensor(rng.integers(-1, 50, 3000), dtype=torch.int32, device="cuda")
+    table = torch.randn((4, 50) if layout == lk.COLUMNS else (50, 4), device="cuda", requires_grad=True)
+    weights = torch.randn((4, 3000) if layout == lk.COLUMNS else (3000, 4), device="cuda")
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            plan = lk.lookup_plan(index, 50)
+        want = torch.autograd.grad((lk.lookup(table, index, 2.0, layout) * weights).sum(), table)[0]
+        with torch.autograd.graph.save_on_cpu():
+            out = lk.lookup(table, index, 2.0, layout, plan)
+        assert torch.equal(torch.autograd.grad((out * weights).sum(), table)[0], want)
+        checkpointed = torch.utils.checkpoint.checkpoint(lambda t: lk.lookup(t, index, 2.0, layout, plan), table, use_reentrant=False)
+        assert torch.equal(torch.autograd.grad((checkpointed * weights).sum(), table)[0], want)
+
+
+def test_hooks_that_hand_back_something_else_are_refused():
+    index = torch.zeros(8, dtype=torch.int32, device="cuda")
+    table = torch.ones(4, 5, device="cuda", requires_grad=True)
+    plan = lk.lookup_plan(index, 5)
+    for back in (lambda t: t.cpu(), lambda t: t.long() if t is not index else t, lambda t: t[:-1]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+            out = lk.lookup(table, index, 1.0, lk.COLUMNS, plan)
+        with pytest.raises((ValueError, RuntimeError)):
+            out.sum().backward()

@@ -35,3 +35,25 @@ def test_plan_texels_keeps_it():
     index = scene.point_cloud_cuda.t_index
     assert scene.texel_plan.own_index(index) is scene.texel_plan.own_index(index)
     assert scene.texel_plan.own_index(index).tolist() == [[0], [1], [2], [3]]
+
+
+def test_gradients_with_a_kept_plan_under_saved_tensor_hooks():
+    """Hooks that hand back another tensor than the one that was saved (kept on the host, packed to disk)."""
+    index = torch.tensor([2, 0, 2, 3], dtype=torch.int32)
+    plan = lk.lookup_plan(index, 4)
+    table = torch.randn(4, 3, requires_grad=True)
+    want = torch.autograd.grad(lk.lookup(table, index, 2.0, lk.ROWS, plan).sum(), table)[0]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.numpy().copy() if not t.requires_grad else t, lambda a: torch.from_numpy(a)):
+        out = lk.lookup(table, index, 2.0, lk.ROWS, plan)
+    assert torch.equal(torch.autograd.grad(out.sum(), table)[0], want)
+
+
+def test_gradients_with_a_plan_that_was_written_to_are_refused():
+    index = torch.tensor([2, 0, 2, 3], dtype=torch.int32)
+    table = torch.randn(4, 3, requires_grad=True)
+    for change in (lambda plan: plan.order.add_(0), lambda plan: plan.starts.add_(0), lambda plan: index.add_(0)):
+        plan = lk.lookup_plan(index, 4)
+        out = lk.lookup(table, index, 2.0, lk.ROWS, plan)
+        change(plan)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()

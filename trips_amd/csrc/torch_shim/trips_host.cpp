@@ -266,6 +266,13 @@ std::pair<at::Tensor, at::Tensor> lookup_plan(uintptr_t ctx, uintptr_t stream, c
     return {order, starts};
 }
 
+// A plan's tensor, as the kernels read it.
+void check_plan(const char* name, const at::Tensor& t, int64_t n, const at::Tensor& index)
+{
+    if (t.scalar_type() != at::kInt || t.numel() != n || t.device() != index.device() || !t.is_contiguous())
+        throw py::value_error(std::string("plan: ") + name + " of " + std::to_string(n) + " adjacent int32 numbers on the index's device expected");
+}
+
 // order, starts: of the plan, or neither: it is made here.
 at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& grad, const at::Tensor& index, const std::optional<at::Tensor>& order,
                            const std::optional<at::Tensor>& starts, int64_t texels, float scale, int layout, const std::optional<at::Tensor>& out)
@@ -277,6 +284,7 @@ at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& gr
     const bool columns    = layout == TRIPS_TABLE_COLUMNS;
     const int64_t n = g.size(columns ? 1 : 0), c = g.size(columns ? 0 : 1);
     if (n != index.numel()) throw py::value_error("grad: " + std::to_string(n) + " points, index has " + std::to_string(index.numel()));
+    if (order) check_plan("order", *order, n, index), check_plan("starts", *starts, texels + 1, index);
     const size_t plan = order ? 0 : plan_bytes(index, texels);
     TripsLookupDesc d  = lookup_desc(layout, dtype_of(g), index_dtype, texels, n, c, scale);
     const int64_t rows = columns ? c : texels, row = columns ? texels : c;

@@ -97,10 +97,14 @@ def lookup_plan(index, num_texels):
 def lookup_backward(grad, index, num_texels, scale=1.0, layout=COLUMNS, plan=None, out=None):
     """The table's gradient from that of its looked-up values: [C, T] from [C, N], or [T, C] from [N, C]. plan: lookup_plan of the
     index, where a program keeps it (it is made here otherwise). out: a table gradient to add to, instead of a new one."""
-    _refuse_unseen("lookup_backward", grad, index)
     if plan is not None:
         plan.check(index, num_texels)
     order, starts = (None, None) if plan is None else (plan.order, plan.starts)
+    return _table_gradient(grad, index, order, starts, num_texels, scale, layout, out)
+
+
+def _table_gradient(grad, index, order, starts, num_texels, scale, layout, out=None):
+    _refuse_unseen("lookup_backward", grad, index)
     return _host().lookup_backward(*_where(index), grad.detach(), index, order, starts, num_texels, scale, layout, out)
 
 
@@ -116,16 +120,20 @@ class _Lookup(torch.autograd.Function):
         with _untraced() if torch.jit.is_tracing() else contextlib.nullcontext():
             _check_plan(table, index, layout, plan)
             values = _host().lookup(*_where(index), table.detach(), index, scale, layout)
-        ctx.save_for_backward(index)
-        ctx.args = (table.shape[1] if layout == COLUMNS else table.shape[0], scale, layout, plan)
+        # The plan's tensors are saved like the index, so that the gradient is of the lookup that was made: hooks on what is saved may hand
+        # back other tensors, and one that was written to meanwhile is refused. (Those of inference mode cannot be saved, or written to here.)
+        order, starts = (None, None) if plan is None else (plan.order, plan.starts)
+        saved = plan is not None and not (order.is_inference() or starts.is_inference())
+        ctx.save_for_backward(index, *((order, starts) if saved else ()))
+        ctx.args = (table.shape[1] if layout == COLUMNS else table.shape[0], scale, layout)
+        ctx.plan = None if saved else (order, starts)
         return values
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        index, = ctx.saved_tensors
-        texels, scale, layout, plan = ctx.args
-        return lookup_backward(grad, index, texels, scale, layout, plan), None, None, None, None
+        index, *plan = ctx.saved_tensors
+        return _table_gradient(grad, index, *(ctx.plan or plan), *ctx.args), None, None, None, None
 
 
 def lookup(table, index, scale=1.0, layout=COLUMNS, plan=None):
