@@ -63,3 +63,21 @@ def test_a_backward_pass_that_needs_an_older_norm_raises():
     opt.step(grads={params[0]: gs[0]})
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_copies_that_changed_since_they_were_set_are_refused():
+    from trips_amd.adamw import AdamW
+    params, gs = _tensors((64,), "f32", "f32", 24)
+    opt = AdamW(params)
+    wide = torch.zeros(128, device="cuda")
+    for other in (torch.zeros(64), wide[::2], torch.zeros(63, device="cuda"), torch.zeros(64, device="cuda", dtype=torch.float64)):
+        copy = torch.zeros(64, device="cuda", dtype=other.dtype if other.dtype != torch.float64 else torch.float32)
+        opt.set_copy(params[0], copy)
+        if other.dtype == torch.float64:
+            opt._copies[params[0]] = other
+        else:
+            copy.data = other
+        before = params[0].detach().clone()
+        with pytest.raises(RuntimeError, match="a copy"):
+            opt.step(grads={params[0]: gs[0]})
+        assert torch.equal(params[0], before) and not wide.any()

@@ -119,7 +119,9 @@ class StepTable
                 {
                     const at::Tensor& copy = tensor_of(c, "a copy");
                     t.copy = copy.data_ptr(), t.copy_dtype = dtype_of(copy);
-                    if (copy.numel() != t.n) throw std::runtime_error("a copy of " + std::to_string(copy.numel()) + " elements for a parameter of " + std::to_string(t.n));
+                    // (what set_copy() checked may have changed since)
+                    if (copy.numel() != t.n || t.copy_dtype < 0 || !copy.is_contiguous() || !copy.is_cuda() || copy.get_device() != device)
+                        throw std::runtime_error("a copy is no longer a contiguous float32, bfloat16 or float16 tensor of its parameter's size, on its device");
                     written.push_back(copy);
                 }
                 t.lr = lr, t.beta1 = b1, t.beta2 = b2, t.eps = eps, t.weight_decay = decay;
