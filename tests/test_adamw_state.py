@@ -37,3 +37,19 @@ def test_a_copied_optimiser_has_a_workspace_of_its_own():
         assert (twin.max_grad_norm, twin.seed) == (0.5, 3)
         q = twin.param_groups[0]["params"][0]
         assert q is not p and torch.equal(twin.state[q]["first_moment"], opt.state[p]["first_moment"])
+
+
+def test_state_bits_of_a_group_are_checked():
+    p, q = torch.nn.Parameter(torch.ones(8)), torch.nn.Parameter(torch.ones(8))
+    with pytest.raises(ValueError, match="state_bits"):
+        AdamW([dict(params=[p], state_bits=16)])
+    opt = AdamW([dict(params=[p], state_bits=8)])
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.add_param_group(dict(params=[q], state_bits=4))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[q]))
+    assert [g["state_bits"] for g in opt.param_groups] == [8, 32]
+    opt.param_groups[1]["state_bits"] = 16  # (set behind the optimiser's back: the first step makes no state)
+    with pytest.raises(ValueError, match="state_bits"):
+        opt._make_state(q, opt.param_groups[1])
+    assert not opt.state.get(q)

@@ -36,6 +36,11 @@ def grad_norm(grads, max_norm=0.0, loss_scale=1.0):
     return out
 
 
+def _check_bits(bits):
+    if bits not in _MOMENTS:
+        raise ValueError(f"state_bits must be 32 or 8, not {bits}")
+
+
 class AdamW(torch.optim.Optimizer):
     """Adam with decoupled weight decay: parameters float32, bfloat16 or float16, moments in 32 or in 8 bits.
 
@@ -61,8 +66,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"Invalid beta parameter at index {i}: {beta}")
         if not 0 <= weight_decay < math.inf:
             raise ValueError(f"Invalid weight_decay value: {weight_decay}")
-        if state_bits not in _MOMENTS:
-            raise ValueError(f"state_bits must be 32 or 8, not {state_bits}")
+        _check_bits(state_bits)
         if max_grad_norm is not None and not max_grad_norm >= 0:
             raise ValueError(f"Invalid max_grad_norm: {max_grad_norm}")
         if not 0 < loss_scale < math.inf:
@@ -78,6 +82,11 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size))
 
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict):  # (the base class refuses others)
+            _check_bits(param_group.get("state_bits", self.defaults["state_bits"]))
+        super().add_param_group(param_group)
+
     def set_copy(self, p, copy):
         """Every step writes the new value of parameter `p` to `copy` as well (a contiguous tensor of its size, in any of the
         three types), before it is rounded to p's own type. None ends that. A copied or unpickled optimiser has no copies yet."""
@@ -89,6 +98,7 @@ class AdamW(torch.optim.Optimizer):
         self._copies[p] = copy
 
     def _make_state(self, p, group):
+        _check_bits(group["state_bits"])
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a parameter's first step makes its state and cannot be captured into a graph")
         bits = 8 if group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"] else 32
