@@ -53,3 +53,19 @@ def test_state_bits_of_a_group_are_checked():
     with pytest.raises(ValueError, match="state_bits"):
         opt._make_state(q, opt.param_groups[1])
     assert not opt.state.get(q)
+
+
+def test_a_parameter_twice_in_a_group_is_refused():
+    """Its two steps would run side by side in one launch, on the same weights and the same count."""
+    p, q = torch.nn.Parameter(torch.ones(8)), torch.nn.Parameter(torch.ones(8))
+    for params in ([p, p], [dict(params=[q, p, q])], [("a", p), ("b", p)]):
+        with pytest.raises(ValueError, match="twice"):
+            AdamW(params)
+    opt = AdamW([p])
+    with pytest.raises(ValueError, match="twice"):
+        opt.add_param_group(dict(params=iter([q, q])))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=(x for x in [q])))
+    assert len(opt.param_groups[1]["params"]) == 1
+    with pytest.raises(ValueError):
+        AdamW([dict(params=[p]), dict(params=[p])])  # (the base class)

@@ -86,6 +86,10 @@ class AdamW(torch.optim.Optimizer):
         if isinstance(param_group, dict):  # (the base class refuses others)
             _check_bits(param_group.get("state_bits", self.defaults["state_bits"]))
         super().add_param_group(param_group)
+        params = self.param_groups[-1]["params"]
+        if len(set(params)) != len(params):  # (of which the base class only warns; one in two groups it refuses)
+            del self.param_groups[-1]
+            raise ValueError("a parameter is in its group twice: its steps would run side by side")
 
     def set_copy(self, p, copy):
         """Every step writes the new value of parameter `p` to `copy` as well (a contiguous tensor of its size, in any of the
