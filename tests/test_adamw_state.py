@@ -69,3 +69,52 @@ def test_a_parameter_twice_in_a_group_is_refused():
     assert len(opt.param_groups[1]["params"]) == 1
     with pytest.raises(ValueError):
         AdamW([dict(params=[p]), dict(params=[p])])  # (the base class)
+
+
+def test_load_state_dict_goes_by_its_hooks():
+    """Pre-hooks hand on another dict, post-hooks see the state loaded and may change it; later hooks come behind earlier ones."""
+    opt, p = _optimiser()
+    seen = []
+
+    def first(o, sd):
+        return {**sd, "state": {0: {**sd["state"][0], "step": torch.full((), 4, dtype=torch.int32)}}}
+
+    def second(o, sd):
+        seen.append(int(sd["state"][0]["step"]))
+        return {**sd, "state": {0: {**sd["state"][0], "step": torch.full((), 5, dtype=torch.int32)}}}
+
+    def after(o):
+        seen.append(int(o.state[p]["step"]))
+        o.state[p]["first_moment"].fill_(7.0)
+
+    opt.register_load_state_dict_pre_hook(first), opt.register_load_state_dict_pre_hook(second)
+    opt.register_load_state_dict_post_hook(after)
+    saved = opt.state_dict()
+    for _ in range(2):
+        opt.load_state_dict(saved)
+    assert seen == [4, 5, 4, 5] and int(opt.state[p]["step"]) == 5
+    assert (opt.state[p]["first_moment"] == 7).all() and (saved["state"][0]["first_moment"] == 0.25).all()
+
+
+def test_load_state_dict_keeps_types_and_what_is_no_parameters():
+    p = torch.nn.Parameter(torch.ones(300, dtype=torch.bfloat16))
+    opt = AdamW([p])
+    opt.state[p] = dict(step=torch.ones((), dtype=torch.int32), first_moment=torch.ones(300).to(torch.float8_e4m3fn),
+                        second_moment=torch.ones(300).to(torch.float8_e5m2), first_scale=torch.ones(2), second_scale=torch.ones(2))
+    saved = opt.state_dict()
+    saved["state"]["note"] = "kept"
+    strided = dict(saved["state"][0], first_scale=torch.stack([torch.ones(2), torch.zeros(2)], 1)[:, 0])
+    opt.load_state_dict(dict(saved, state={0: strided, "note": "kept"}))
+    assert opt.state["note"] == "kept"
+    for k, v in saved["state"][0].items():
+        got = opt.state[p][k]
+        assert got.dtype == v.dtype and got.is_contiguous() and got.data_ptr() != v.data_ptr() and torch.equal(got.float(), v.float())
+
+
+def test_a_state_dict_that_does_not_fit_leaves_the_optimiser_alone():
+    opt, p = _optimiser()
+    saved = opt.state_dict()
+    saved["param_groups"][0]["params"] = [0, 1]
+    with pytest.raises(ValueError):
+        opt.load_state_dict(saved)
+    assert (opt.state[p]["first_moment"] == 0.25).all() and len(opt._optimizer_load_state_dict_pre_hooks) == 0

@@ -185,14 +185,27 @@ class AdamW(torch.optim.Optimizer):
         return numbers(first, st["first_scale"]), numbers(second, st["second_scale"])
 
     def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
-        # (the base class casts state to the parameters' type: here it keeps its own)
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(ids, params):
-            st = state_dict["state"].get(i)
-            if st is not None:
-                self.state[p] = {k: v.detach().to(p.device).clone() if torch.is_tensor(v) else v for k, v in st.items()}
+        # The base class would cast the state to the parameters' types. It loads all else here; the state itself, in its own types,
+        # goes in between the hooks: those before have made the dict what it is, those behind find it loaded.
+        loaded, ids = {}, []
+
+        def behind_pre_hooks(_, final):
+            loaded.update(final)
+            ids.extend(i for g in final["param_groups"] for i in g["params"])
+            return {**final, "state": {k: v for k, v in final["state"].items() if k not in ids}}
+
+        def before_post_hooks(_):
+            for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+                if i in loaded["state"]:
+                    self.state[p] = {k: v.detach().to(p.device).clone(memory_format=torch.contiguous_format) if torch.is_tensor(v) else v
+                                     for k, v in loaded["state"][i].items()}
+        handles = (self.register_load_state_dict_pre_hook(behind_pre_hooks),
+                   self.register_load_state_dict_post_hook(before_post_hooks, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for handle in handles:
+                handle.remove()
 
 
 _watched_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)
