@@ -118,3 +118,17 @@ def test_a_state_dict_that_does_not_fit_leaves_the_optimiser_alone():
     with pytest.raises(ValueError):
         opt.load_state_dict(saved)
     assert (opt.state[p]["first_moment"] == 0.25).all() and len(opt._optimizer_load_state_dict_pre_hooks) == 0
+
+
+def test_the_optimisers_own_options_are_in_its_state_dict():
+    """A resumed run rounds with the same seed, and clips and scales as before, whatever it was made with."""
+    opt, p = _optimiser(seed=11, max_grad_norm=0.5, skip_nonfinite=True)
+    opt.loss_scale = 512.0
+    saved = opt.state_dict()
+    other, _ = _optimiser()
+    other.load_state_dict(saved)
+    assert (other.seed, other.max_grad_norm, other.skip_nonfinite, other.loss_scale) == (11, 0.5, True, 512.0)
+    del saved["options"]  # (of a program that kept the rest alone)
+    other, _ = _optimiser(seed=3)
+    other.load_state_dict(saved)
+    assert (other.seed, other.loss_scale) == (3, 1.0) and torch.equal(other.state[other.param_groups[0]["params"][0]]["first_moment"], torch.full((300,), 0.25))

@@ -184,6 +184,11 @@ class AdamW(torch.optim.Optimizer):
             return (codes.reshape(-1).to(torch.float32) * wide).reshape(codes.shape)
         return numbers(first, st["first_scale"]), numbers(second, st["second_scale"])
 
+    def state_dict(self):
+        """The base class's, and under "options" what belongs to the optimiser and not to a group: max_grad_norm, skip_nonfinite,
+        loss_scale and seed. load_state_dict() takes them where they are there."""
+        return {**super().state_dict(), "options": {k: getattr(self, k) for k in self._OWN}}
+
     def load_state_dict(self, state_dict):
         # The base class would cast the state to the parameters' types. It loads all else here; the state itself, in its own types,
         # goes in between the hooks: those before have made the dict what it is, those behind find it loaded.
@@ -199,6 +204,9 @@ class AdamW(torch.optim.Optimizer):
                 if i in loaded["state"]:
                     self.state[p] = {k: v.detach().to(p.device).clone(memory_format=torch.contiguous_format) if torch.is_tensor(v) else v
                                      for k, v in loaded["state"][i].items()}
+            for k, v in loaded.get("options", {}).items():
+                if k in self._OWN:
+                    setattr(self, k, v)
         handles = (self.register_load_state_dict_pre_hook(behind_pre_hooks),
                    self.register_load_state_dict_post_hook(before_post_hooks, prepend=True))
         try:
