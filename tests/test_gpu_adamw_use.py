@@ -81,3 +81,32 @@ def test_copies_that_changed_since_they_were_set_are_refused():
         with pytest.raises(RuntimeError, match="a copy"):
             opt.step(grads={params[0]: gs[0]})
         assert torch.equal(params[0], before) and not wide.any()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_steps_state_outlives_load_state_dict(bits):
+    """What a graph writes is not given to others; it goes on with its own moments, and eager steps with those loaded."""
+    from trips_amd.adamw import AdamW
+    params, gs = _tensors((70_001, 9000), "f32", "f32", 25)
+    given = dict(zip(params, gs))
+    opt = AdamW(params, state_bits=bits, min_8bit_size=0, max_grad_norm=0.5)
+    opt.step(grads=given)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        opt.step(grads=given)
+    captured = {t.data_ptr() for p in params for t in opt.state[p].values()}
+    import copy
+    saved = copy.deepcopy(opt.state_dict())
+    for _ in range(2):
+        opt.load_state_dict(saved)
+    others = [torch.zeros(n, dtype=d, device="cuda") for n in (70_001, 9000, 1, 274, 36) for d in (torch.float32, torch.uint8) for _ in range(20)]
+    assert not captured & {t.data_ptr() for t in others + [t for p in params for t in opt.state[p].values()]}
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert not any(x.any() for x in others)
+    assert all(int(opt.state[p]["step"]) == 1 for p in params)
+    before = _state(opt, params)
+    opt.step(grads=given)
+    _check_step(opt, before, params, gs, 2, factor=float(opt.grad_norm[1]), places=_places(params))

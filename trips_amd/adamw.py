@@ -52,8 +52,9 @@ class AdamW(torch.optim.Optimizer):
     over by the next step) if it was computed.
 
     State per parameter: step (int32, on the device), first_moment, second_moment, and with 8 bits first_scale and second_scale;
-    moments() gives the moments as numbers. A captured step replays with the learning rates of its capture; a parameter's first
-    step, which makes its state, cannot be captured. Steps of one optimiser must not overlap."""
+    moments() gives the moments as numbers. A captured step replays with the learning rates and goes on with the moments of its
+    capture: after load_state_dict() it has to be captured anew. A parameter's first step, which makes its state, cannot be
+    captured. Steps of one optimiser must not overlap."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_size=4096,
                  max_grad_norm=0.0, skip_nonfinite=False, loss_scale=1.0, seed=0):
@@ -77,7 +78,8 @@ class AdamW(torch.optim.Optimizer):
         self.seed = seed
         self.grad_norm = None
         self._workspace = None
-        self._kept = []
+        self._kept = []  # what captured steps write and later ones do not
+        self._captured = False
         self._copies = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_size=min_8bit_size))
@@ -141,6 +143,7 @@ class AdamW(torch.optim.Optimizer):
         ctx = get_context(device)
         if self._workspace is None or self._workspace.device != ctx.device or self._workspace_for < count:
             self._make_workspace(ctx)
+        self._captured = self._captured or torch.cuda.is_current_stream_capturing()
         max_norm = self.max_grad_norm or 0.0
         compute = grad_norm is None and (max_norm > 0 or self.skip_nonfinite)
         if grad_norm is not None and (grad_norm.dtype != torch.float32 or grad_norm.numel() != 2 or grad_norm.device != ctx.device
@@ -167,7 +170,7 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state):
         # Of an optimiser that is being copied or unpickled, which has none of these yet: a workspace of its own, and no copies
         # of its parameters. load_state_dict() ends here as well, where what there is stays.
-        for name, value in (("grad_norm", None), ("_workspace", None), ("_kept", []), ("_copies", {})):
+        for name, value in (("grad_norm", None), ("_workspace", None), ("_kept", []), ("_captured", False), ("_copies", {})):
             self.__dict__.setdefault(name, value)
         super().__setstate__(state)
 
@@ -192,7 +195,7 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         # The base class would cast the state to the parameters' types. It loads all else here; the state itself, in its own types,
         # goes in between the hooks: those before have made the dict what it is, those behind find it loaded.
-        loaded, ids = {}, []
+        loaded, ids, before = {}, [], dict(self.state)
 
         def behind_pre_hooks(_, final):
             loaded.update(final)
@@ -200,6 +203,9 @@ class AdamW(torch.optim.Optimizer):
             return {**final, "state": {k: v for k, v in final["state"].items() if k not in ids}}
 
         def before_post_hooks(_):
+            if self._captured:  # (a graph goes on writing to the state of its capture)
+                self._kept.append(before)
+                self._captured = False
             for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
                 if i in loaded["state"]:
                     self.state[p] = {k: v.detach().to(p.device).clone(memory_format=torch.contiguous_format) if torch.is_tensor(v) else v
