@@ -1,4 +1,6 @@
 """AdamW as programs use it: resumed, captured, with copies that the forward reads, on other streams."""
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -110,3 +112,25 @@ def test_a_captured_steps_state_outlives_load_state_dict(bits):
     before = _state(opt, params)
     opt.step(grads=given)
     _check_step(opt, before, params, gs, 2, factor=float(opt.grad_norm[1]), places=_places(params))
+
+
+def test_an_optimiser_dropped_while_its_step_runs_on_another_stream():
+    """Its workspace, made on one stream, is not given to the next tensor of that stream while another one's step may write it."""
+    from trips_amd.adamw import AdamW
+    params, gs = _tensors((3000, 500), "f32", "f32", 26)
+    opt = AdamW(params, max_grad_norm=0.5)
+    opt.step(grads=dict(zip(params, gs)))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    kept = [(t.data_ptr(), t.data_ptr() + t.nbytes) for t in (opt._workspace, opt._norm)]
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1_000_000_000)  # (some tenths of a second: the step waits behind it)
+        opt.step(grads=dict(zip(params, gs)))
+        done = side.record_event()
+    del opt
+    gc.collect()
+    others = [torch.empty(16384, dtype=torch.uint8, device="cuda") for _ in range(300)]
+    pending = not done.query()  # (a step that has ended by now shows nothing)
+    torch.cuda.synchronize()
+    inside = [t for t in others for a, b in kept if t.data_ptr() < b and a < t.data_ptr() + t.nbytes]
+    assert not pending or not inside

@@ -54,7 +54,7 @@ class AdamW(torch.optim.Optimizer):
     State per parameter: step (int32, on the device), first_moment, second_moment, and with 8 bits first_scale and second_scale;
     moments() gives the moments as numbers. A captured step replays with the learning rates and goes on with the moments of its
     capture: after load_state_dict() it has to be captured anew. A parameter's first step, which makes its state, cannot be
-    captured. Steps of one optimiser must not overlap."""
+    captured. Steps of one optimiser must not overlap, and the optimiser has to outlive the graphs that hold its steps."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, min_8bit_size=4096,
                  max_grad_norm=0.0, skip_nonfinite=False, loss_scale=1.0, seed=0):
@@ -143,6 +143,11 @@ class AdamW(torch.optim.Optimizer):
         ctx = get_context(device)
         if self._workspace is None or self._workspace.device != ctx.device or self._workspace_for < count:
             self._make_workspace(ctx)
+        stream = _stream_ptr(ctx.device)
+        if stream not in self._streams:  # (its memory is not to be given away before this stream is done with it)
+            for t in (self._workspace, self._norm):
+                t.record_stream(torch.cuda.current_stream(ctx.device))
+            self._streams.add(stream)
         self._captured = self._captured or torch.cuda.is_current_stream_capturing()
         max_norm = self.max_grad_norm or 0.0
         compute = grad_norm is None and (max_norm > 0 or self.skip_nonfinite)
@@ -151,7 +156,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("grad_norm: two float32 numbers on the parameters' device expected")
         self.grad_norm = self._norm if compute else grad_norm
         _lib.check(table.step(ctx.ctx.value, self.seed & 0xFFFFFFFF, self.grad_norm, compute, max_norm if compute else 0.0, self.loss_scale,
-                              self._workspace, _stream_ptr(ctx.device)))
+                              self._workspace, stream))
         return loss
 
     def _make_workspace(self, ctx):
@@ -161,6 +166,7 @@ class AdamW(torch.optim.Optimizer):
         self._workspace_for = sum(len(g["params"]) for g in self.param_groups)
         self._workspace = ctx.alloc_bytes(ctx.adamw_workspace_size(self._workspace_for))
         self._norm = torch.empty(2, dtype=torch.float32, device=ctx.device)
+        self._streams = {_stream_ptr(ctx.device)}
 
     _OWN = ("max_grad_norm", "skip_nonfinite", "loss_scale", "seed")
 
