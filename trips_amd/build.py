@@ -61,6 +61,14 @@ SHIM_LIB = os.path.join(HERE, "_trips_torch.so")
 HOST_LIB = os.path.join(HERE, "_trips_host.so")
 
 
+def _has_torch():
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        return False
+    return True
+
+
 def _torch_flags(name):
     """(compiler flags, linker flags) of a libtorch extension that calls the C ABI of libtrips_splat.so."""
     import sysconfig
@@ -118,6 +126,9 @@ def build_torch_shim(verbose=False):
 if __name__ == "__main__":
     build(verbose=True, incremental="--incremental" in sys.argv)
     print(LIB)
-    print(build_host(verbose=True, incremental="--incremental" in sys.argv))
+    if _has_torch():
+        print(build_host(verbose=True, incremental="--incremental" in sys.argv))
+    else:
+        print("no torch: _trips_host.so, which adamw.py and lookup.py need, is left out")
     if "--shim" in sys.argv:
         print(build_torch_shim(verbose=True))
