@@ -57,3 +57,17 @@ def test_gradients_with_a_plan_that_was_written_to_are_refused():
         change(plan)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             out.sum().backward()
+
+
+def test_parameters_of_a_programs_own_kind_need_no_new_field(monkeypatch):
+    """Any object with the fields that the render reads is taken as its parameters, also one without shared_texels_in_order."""
+    from types import SimpleNamespace
+    from trips_amd import renderer
+    scene = renderer.NeuralScene(texture=torch.zeros(2, 4), background_color=torch.zeros(2), confidence=torch.zeros(1, 4), position=torch.zeros(4, 4),
+                                 point_size=torch.zeros(4, 1), index=torch.zeros(4, 1, dtype=torch.int32),
+                                 poses_se3=torch.zeros(1, 7, dtype=torch.float64), intrinsics=torch.zeros(1, 13))
+    params = SimpleNamespace(add_depth_to_network=False, output_background_mask=False)
+    info = renderer.NeuralRenderInfo(scene=scene, params=params)
+    image = torch.zeros(1, 2, 3, 4)
+    monkeypatch.setattr(renderer.PointRender, "render", staticmethod(lambda *a: ([image], None, None, None)))
+    assert renderer.BlendPointCloud(info)[0] is image

@@ -483,7 +483,7 @@ def _with_own_texels(info):
 
 def BlendPointCloud(info: NeuralRenderInfo):
     """Render the scene into a batch of image pyramids (RenderInfo.cpp:27-40)."""
-    if info.params.shared_texels_in_order:
+    if getattr(info.params, "shared_texels_in_order", False):
         info = _with_own_texels(info)
     sc = info.scene
     inputs = (sc.texture.texture, sc.texture.background_color, sc.point_cloud_cuda.t_position, sc.poses.tangent_poses,
