@@ -134,3 +134,37 @@ def test_an_optimiser_dropped_while_its_step_runs_on_another_stream():
     torch.cuda.synchronize()
     inside = [t for t in others for a, b in kept if t.data_ptr() < b and a < t.data_ptr() + t.nbytes]
     assert not pending or not inside
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_workgroups_whose_tiles_belong_to_several_tensors(bits):
+    """More than 2048 tiles, so that a workgroup has two, one behind the other; tensors that end after odd numbers of tiles."""
+    from trips_amd.adamw import AdamW
+    params, gs = _tensors((700_001, 3 * 1024, 1_000_077, 5, 400_000, 1, 1025), "f32", "f32", 27)
+    opt = AdamW(params, state_bits=bits, min_8bit_size=0, seed=8)
+    for t in (1, 2):
+        before = _state(opt, params)
+        opt.step(grads=dict(zip(params, gs)))
+        _check_step(opt, before, params, gs, t, places=_places(params), seed=8)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_tensors_than_a_launch_has_room_for(bits):
+    from trips_amd.adamw import AdamW
+    params, gs = _tensors([1 + i % 3 for i in range(4100)], "f32", "f32", 28)
+    opt = AdamW(params, state_bits=bits, min_8bit_size=0, max_grad_norm=0.5, seed=9)
+    before = _state(opt, params)
+    opt.step(grads=dict(zip(params, gs)))
+    _check_step(opt, before, params, gs, 1, factor=float(opt.grad_norm[1]), places=_places(params), seed=9)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-14])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_eps_so_small_that_roots_are_taken_exactly(bits, eps):
+    from trips_amd.adamw import AdamW
+    params, gs = _tensors((1, 1027, 5000), "f32", "f32", 29)
+    opt = AdamW(params, eps=eps, state_bits=bits, min_8bit_size=0, seed=10)
+    for t in (1, 2):
+        before = _state(opt, params)
+        opt.step(grads=dict(zip(params, gs)))
+        _check_step(opt, before, params, gs, t, places=_places(params), seed=10)

@@ -132,3 +132,13 @@ def test_hooks_that_hand_back_something_else_are_refused():
             out = lk.lookup(table, index, 1.0, lk.COLUMNS, plan)
         with pytest.raises((ValueError, RuntimeError)):
             out.sum().backward()
+
+
+def test_the_order_of_points_of_the_largest_table():
+    texels = (1 << 31) - 2
+    index = torch.tensor([texels - 1, 5, 0, texels, 1 << 30, 5, -1], dtype=torch.int64, device="cuda")
+    plan = lk.lookup_plan(index, texels)
+    assert plan.order.tolist() == [2, 1, 5, 4, 0, 3, 6]
+    for first, behind, points in ((0, 1, 0), (1, 6, 1), (6, (1 << 30) + 1, 3), ((1 << 30) + 1, texels, 4), (texels, texels + 1, 5)):
+        part = plan.starts[first:behind]
+        assert part.numel() == behind - first and int(part.min()) == int(part.max()) == points
