@@ -142,3 +142,16 @@ def test_the_order_of_points_of_the_largest_table():
     for first, behind, points in ((0, 1, 0), (1, 6, 1), (6, (1 << 30) + 1, 3), ((1 << 30) + 1, texels, 4), (texels, texels + 1, 5)):
         part = plan.starts[first:behind]
         assert part.numel() == behind - first and int(part.min()) == int(part.max()) == points
+
+
+def test_a_copied_scene_renders_with_its_plan():
+    import copy
+    from trips_amd.renderer import BlendPointCloud
+    ns, info = _shared(65, kept=True)
+    twin = copy.deepcopy(ns)
+    other = copy.copy(info)
+    other.scene, other.cache = twin, None
+    assert all(torch.equal(a, b) for a, b in zip(BlendPointCloud(info), BlendPointCloud(other)))
+    twin.point_cloud_cuda.t_index[0] = 5
+    with pytest.raises(ValueError, match="changed"):
+        BlendPointCloud(other)

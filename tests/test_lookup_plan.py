@@ -71,3 +71,25 @@ def test_parameters_of_a_programs_own_kind_need_no_new_field(monkeypatch):
     image = torch.zeros(1, 2, 3, 4)
     monkeypatch.setattr(renderer.PointRender, "render", staticmethod(lambda *a: ([image], None, None, None)))
     assert renderer.BlendPointCloud(info)[0] is image
+
+
+def test_copies_of_a_plan_go_with_copies_of_their_index():
+    """A scene that is copied or saved with its plan: the copy's index is what the plan was made of, whatever its version is."""
+    import copy
+    import pickle
+    for changes in (0, 3):
+        index = torch.tensor([2, 0, 2, 3], dtype=torch.int32)
+        for _ in range(changes):
+            index.add_(0)
+        plan = lk.lookup_plan(index, 4)
+        plan.keep_own_index()
+        for twin, own in (copy.deepcopy((plan, index)), pickle.loads(pickle.dumps((plan, index))), (copy.copy(plan), index)):
+            twin.check(own, 4)
+            assert twin.own_index(own).tolist() == [0, 1, 2, 3] and torch.equal(twin.order, plan.order)
+            if own is not index:
+                with pytest.raises(ValueError, match="another index"):
+                    twin.check(index, 4)
+        index.add_(0)
+        for twin, own in (copy.deepcopy((plan, index)), pickle.loads(pickle.dumps((plan, index))), (copy.copy(plan), index)):
+            with pytest.raises(ValueError, match="changed"):  # (the index was written to since: so it is of a copy made now)
+                twin.check(own, 4)

@@ -48,6 +48,10 @@ def _refuse_unseen(what, *tensors):
         raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
+def _version(index):
+    return None if index is None or index.is_inference() else index._version
+
+
 class LookupPlan:
     """The points of an index in the order of their texels: order [N] and starts [T + 1] (int32; see trips_lookup_plan).
     It belongs to the index that it was made of, as it was then; made in a capture, it holds nothing before the first replay."""
@@ -59,7 +63,15 @@ class LookupPlan:
         self.order, self.starts = order, starts
         self.index = index
         self._own = None
-        self.version = None if index is None or index.is_inference() else index._version
+        self.version = _version(index)
+
+    def __getstate__(self):
+        # (a copy of the index counts its versions anew: what goes along is whether the index is still what the plan was made of)
+        return {**self.__dict__, "version": _version(self.index) == self.version}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.version = _version(self.index) if state["version"] else -1
 
     def check(self, index, texels):
         if self.order.numel() != index.numel() or self.starts.numel() != texels + 1 or self.order.device != index.device:
@@ -68,7 +80,7 @@ class LookupPlan:
         own = self.index
         if own is not None and (own.data_ptr() != index.data_ptr() or own.dtype != index.dtype
                                 or (own.stride() != index.stride() and not (own.is_contiguous() and index.is_contiguous()))
-                                or (None if index.is_inference() else index._version) != self.version):
+                                or _version(index) != self.version):
             raise ValueError("the plan was made of another index, or the index was changed since")
 
     def keep_own_index(self):
