@@ -93,3 +93,12 @@ def test_copies_of_a_plan_go_with_copies_of_their_index():
         for twin, own in (copy.deepcopy((plan, index)), pickle.loads(pickle.dumps((plan, index))), (copy.copy(plan), index)):
             with pytest.raises(ValueError, match="changed"):  # (the index was written to since: so it is of a copy made now)
                 twin.check(own, 4)
+
+
+def test_a_plan_without_an_index_keeps_none():
+    index = torch.tensor([2, 0, 2, 3], dtype=torch.int32)
+    of = lk.lookup_plan(index, 4)
+    plan = lk.LookupPlan(of.order, of.starts)
+    with pytest.raises(ValueError, match="index"):
+        plan.keep_own_index()
+    assert plan.own_index(index).tolist() == [0, 1, 2, 3]

@@ -85,6 +85,8 @@ class LookupPlan:
 
     def keep_own_index(self):
         """Makes own_index() of the plan's index, on the current stream, like the plan itself, for all that use the plan."""
+        if self.index is None:
+            raise ValueError("the plan was made without an index")
         self._own = own_index(self.index, self.starts.numel() - 1)
 
     def own_index(self, index):
