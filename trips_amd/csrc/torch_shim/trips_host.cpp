@@ -85,7 +85,9 @@ class StepTable
             const py::tuple betas(group["betas"]);
             const double lr = group["lr"].cast<double>(), b1 = betas[0].cast<double>(), b2 = betas[1].cast<double>(), eps = group["eps"].cast<double>(),
                          decay = group["weight_decay"].cast<double>();
-            for (const py::handle& o : py::list(group["params"]))
+            const py::list listed(group["params"]);
+            tensors.reserve(tensors.size() + listed.size()), written.reserve(written.size() + 2 * listed.size() + 1);
+            for (const py::handle& o : listed)
             {
                 const at::Tensor& p = tensor_of(o.ptr(), "a parameter");
                 at::Tensor g;
