@@ -2,8 +2,8 @@
 
 For what MyAdam's rules do not suit: the reconstruction net (which the reference steps with libtorch's optimiser,
 src/lib/models/Pipeline.cpp:870-882) and any other tensor whose every element is stepped every time. All tensors of one
-combination of types go through one launch per 40 of them; clipping by the global norm stays on the device, and so do the
-step counts, so that a step may be captured into a HIP graph.
+combination of types go through one launch, after a small one per 40 of them; clipping by the global norm stays on the
+device, and so do the step counts, so that a step may be captured into a HIP graph.
 
 A graph's backward pass must not be captured while an eager graph of the same leaves is alive (torch ends the process).
 """

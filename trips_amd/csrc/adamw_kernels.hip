@@ -24,8 +24,10 @@ constexpr int kGroups      = 8;    // different sets of options among them
 constexpr int kStepTensors = 4096; // tensors of a step's launch
 constexpr int kTileOptim   = 1024; // elements of a tile: four wavefronts with a block of 256 each
 constexpr int kStepGroups  = 2048; // workgroups of a step with a tile each
-constexpr int kStepRun     = 2;    // tiles of a workgroup, one behind the other, where there are more tiles (60M elements in
-                                   // 8 bits, us: 1 tile 181, 2 169, 4 178, 8 188; 2048 workgroups in turn 194. In 32: 297 to 305, 331)
+constexpr int kStepRun     = 2;    // tiles of a workgroup, one behind the other, where there are more tiles: moments in 8 bits gain by it
+                                   // (us a step with 1 and 2: 3000 tiles 16.0, 15.4; 8000 29.4, 28.3; 24,000 75.5, 73.7; 60M elements 181,
+                                   // 169, with 4 178, 8 188, 2048 workgroups in turn 194), in 32 bits only the largest steps do (8000 tiles
+                                   // 41.7, 46.1; 24,000 124, 130; 40,000 203, 199; 60M elements 297 to 305, in turn 331)
 constexpr int kNormTensors = 140; // of a launch: 4 KB of arguments
 constexpr int kNormTile    = 2048; // elements of a tile of the norm
 constexpr int kNormGroups  = 1024; // workgroups of the norm = partial sums
@@ -407,7 +409,7 @@ __device__ __forceinline__ uint32_t tensor_of_tile(const uint32_t* first_tiles, 
     return (uint32_t)__popcll(__ballot(lane < (int)n && first_tiles[lane] <= tile)) - 1u;
 }
 
-// 60M weights of 32 bits: moments in 32 bits 300 us (5.6 TB/s), in 8 bits 166 (5.8 TB/s; 7.5e7 vector instructions of wavefronts,
+// 60M weights of 32 bits: moments in 32 bits 300 us (5.6 TB/s), in 8 bits 164 to 166 (5.8 TB/s; the card's clocks as they settle, in passes 10 to 100 up to 225; 7.5e7 vector instructions of wavefronts,
 // 122 us if nothing else were issued: the codes are half of them); the 18 tensors of the benchmark's net 4.7.
 template <int WD, int GD, int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(const StepParams p)
