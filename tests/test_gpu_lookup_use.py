@@ -84,12 +84,14 @@ def test_lookups_without_a_graph_under_modes():
 
 @pytest.mark.parametrize("by_scene", [True, False])
 def test_a_render_between_a_capture_and_its_first_replay(by_scene):
-    """The first render with a plan is captured; an eager one before the replay, and the replays, give the same images."""
+    """The first render with a plan is captured; an eager one before the replay, and the replays, give the same images. (With gradients
+    asked for: without, the texels are not looked up.)"""
     from trips_amd.renderer import BlendPointCloud, NeuralScene
     sc = _scene(64, n=600)
     ns = NeuralScene.from_arrays(sc)
-    with torch.no_grad():
-        want = [o.clone() for o in BlendPointCloud(_info(sc, ns, train=False, shared_texels_in_order=True))]
+    ns.texture.texture.requires_grad_()
+    with torch.enable_grad():
+        want = [o.detach().clone() for o in BlendPointCloud(_info(sc, ns, train=False, shared_texels_in_order=True))]
         if by_scene:
             ns.plan_texels()
         else:
@@ -155,3 +157,33 @@ def test_a_copied_scene_renders_with_its_plan():
     twin.point_cloud_cuda.t_index[0] = 5
     with pytest.raises(ValueError, match="changed"):
         BlendPointCloud(other)
+
+
+@pytest.mark.parametrize("train", [False, True])
+@pytest.mark.parametrize("kept", [False, True])
+def test_a_frame_without_gradients_takes_no_lookups(kept, train, monkeypatch):
+    """The splat reads shared texels by itself: the same images, nothing looked up, ordered or numbered on the way."""
+    from trips_amd import renderer
+    ns, info = _shared(66, kept, train=train)
+    ns.texture.texture.requires_grad_()
+    want = [o.detach() for o in renderer.BlendPointCloud(info)]
+
+    def refuse(*a, **kw):
+        raise AssertionError("a frame needs none of these")
+    for name in ("lookup", "lookup_plan", "own_index"):
+        monkeypatch.setattr(lk, name, refuse)
+    with torch.no_grad():
+        got = renderer.BlendPointCloud(info)
+    ns.texture.texture.requires_grad_(False)
+    again = renderer.BlendPointCloud(info)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, again))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_shared_texels_by_indexes_of_64_bits(grad):
+    from trips_amd.renderer import BlendPointCloud
+    ns, info = _shared(67)
+    ns.texture.texture.requires_grad_(grad)
+    want = BlendPointCloud(info)
+    ns.point_cloud_cuda.t_index = ns.point_cloud_cuda.t_index.long()
+    assert all(torch.equal(a, b) for a, b in zip(BlendPointCloud(info), want))

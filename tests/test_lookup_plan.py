@@ -102,3 +102,18 @@ def test_a_plan_without_an_index_keeps_none():
     with pytest.raises(ValueError, match="index"):
         plan.keep_own_index()
     assert plan.own_index(index).tolist() == [0, 1, 2, 3]
+
+
+def test_tensors_on_two_devices_are_left_to_the_lookup(monkeypatch):
+    """Without gradients too: the splat by itself would take an address for the other device's."""
+    from trips_amd import renderer
+    scene = renderer.NeuralScene(texture=torch.zeros(2, 4), background_color=torch.zeros(2), confidence=torch.zeros(1, 4, device="meta"),
+                                 position=torch.zeros(4, 4), point_size=torch.zeros(4, 1), index=torch.zeros(4, 1, dtype=torch.int32),
+                                 poses_se3=torch.zeros(1, 7, dtype=torch.float64), intrinsics=torch.zeros(1, 13))
+    info = renderer.NeuralRenderInfo(scene=scene, params=renderer.RenderParams(shared_texels_in_order=True), train=False)
+
+    def lookup(*a, **kw):
+        raise ValueError("looked up")
+    monkeypatch.setattr(lk, "lookup", lookup)
+    with pytest.raises(ValueError, match="looked up"):
+        renderer.BlendPointCloud(info)

@@ -459,14 +459,23 @@ class PointRender(torch.autograd.Function):
 
 
 def _with_own_texels(info):
-    """`info` for a scene in which every point has a texel of its own, looked up from those that t_index names."""
+    """`info` for a scene in which every point has a texel of its own, looked up from those that t_index names; `info` itself where no
+    gradient of the texels is asked for, whose images are the same."""
     from . import lookup
     sc = info.scene
-    if info.cache is None:
-        info.cache = PointRendererCache()
     points, index = sc.point_cloud_cuda, sc.point_cloud_cuda.t_index
     plan = getattr(sc, "texel_plan", None)
     texels = int(sc.texture.texture.shape[1])
+    looked_up = sc.texture.texture, sc.texture.confidence_value_of_point
+    asked = torch.is_grad_enabled() and any(t.requires_grad for t in looked_up)
+    # (what is traced may be run with gradients; what the splat does not check is left to the lookup, which takes or refuses it)
+    plain = index.dtype == torch.int32 and all(t.dtype == torch.float32 and t.device == index.device for t in looked_up)
+    if not asked and plain and not torch.jit.is_tracing():
+        if plan is not None:
+            plan.check(index, texels)
+        return info
+    if info.cache is None:
+        info.cache = PointRendererCache()
     with _untraced():  # (to a trace the index is a constant, and so is what is made of it)
         if plan is None:
             plan = lookup.lookup_plan(index, texels) if info.train else None
