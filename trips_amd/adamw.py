@@ -206,7 +206,8 @@ class AdamW(torch.optim.Optimizer):
         def behind_pre_hooks(_, final):
             loaded.update(final)
             ids.extend(i for g in final["param_groups"] for i in g["params"])
-            return {**final, "state": {k: v for k, v in final["state"].items() if k not in ids}}
+            known = set(ids)
+            return {**final, "state": {k: v for k, v in final["state"].items() if k not in known}}
 
         def before_post_hooks(_):
             if self._captured:  # (a graph goes on writing to the state of its capture)
