@@ -104,10 +104,11 @@ def test_a_plan_without_an_index_keeps_none():
     assert plan.own_index(index).tolist() == [0, 1, 2, 3]
 
 
-def test_tensors_on_two_devices_are_left_to_the_lookup(monkeypatch):
-    """Without gradients too: the splat by itself would take an address for the other device's."""
+@pytest.mark.parametrize("confidence", [torch.zeros(1, 4, device="meta"), torch.zeros(1, 3), torch.zeros(1, 4, dtype=torch.float16)])
+def test_what_the_splat_does_not_check_is_left_to_the_lookup(confidence, monkeypatch):
+    """Without gradients too: another device's tensor, one shorter than the texture, one of another type."""
     from trips_amd import renderer
-    scene = renderer.NeuralScene(texture=torch.zeros(2, 4), background_color=torch.zeros(2), confidence=torch.zeros(1, 4, device="meta"),
+    scene = renderer.NeuralScene(texture=torch.zeros(2, 4), background_color=torch.zeros(2), confidence=confidence,
                                  position=torch.zeros(4, 4), point_size=torch.zeros(4, 1), index=torch.zeros(4, 1, dtype=torch.int32),
                                  poses_se3=torch.zeros(1, 7, dtype=torch.float64), intrinsics=torch.zeros(1, 13))
     info = renderer.NeuralRenderInfo(scene=scene, params=renderer.RenderParams(shared_texels_in_order=True), train=False)

@@ -469,7 +469,8 @@ def _with_own_texels(info):
     looked_up = sc.texture.texture, sc.texture.confidence_value_of_point
     asked = torch.is_grad_enabled() and any(t.requires_grad for t in looked_up)
     # (what is traced may be run with gradients; what the splat does not check is left to the lookup, which takes or refuses it)
-    plain = index.dtype == torch.int32 and all(t.dtype == torch.float32 and t.device == index.device for t in looked_up)
+    plain = index.dtype == torch.int32 and looked_up[1].numel() == texels and \
+        all(t.dtype == torch.float32 and t.device == index.device for t in looked_up)
     if not asked and plain and not torch.jit.is_tracing():
         if plan is not None:
             plan.check(index, texels)
