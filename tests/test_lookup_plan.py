@@ -118,3 +118,12 @@ def test_what_the_splat_does_not_check_is_left_to_the_lookup(confidence, monkeyp
     monkeypatch.setattr(lk, "lookup", lookup)
     with pytest.raises(ValueError, match="looked up"):
         renderer.BlendPointCloud(info)
+
+
+def test_a_plan_of_other_elements_at_the_same_address_is_refused():
+    base = torch.tensor([0, 1, 2, 3, 0, 1, 2, 3, 0, 1, 2, 3], dtype=torch.int32)
+    index, other = base.as_strided((4, 2), (3, 1)), base.as_strided((2, 4), (3, 1))
+    plan = lk.LookupPlan(torch.arange(8, dtype=torch.int32), torch.zeros(5, dtype=torch.int32), index)
+    plan.check(base.as_strided((4, 2), (3, 1)), 4)
+    with pytest.raises(ValueError, match="another index"):
+        plan.check(other, 4)

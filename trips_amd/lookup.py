@@ -79,7 +79,7 @@ class LookupPlan:
                              f"{index.numel()} and {texels}")
         own = self.index
         if own is not None and (own.data_ptr() != index.data_ptr() or own.dtype != index.dtype
-                                or (own.stride() != index.stride() and not (own.is_contiguous() and index.is_contiguous()))
+                                or ((own.stride() != index.stride() or own.shape != index.shape) and not (own.is_contiguous() and index.is_contiguous()))
                                 or _version(index) != self.version):
             raise ValueError("the plan was made of another index, or the index was changed since")
 
