@@ -1,4 +1,4 @@
-"""Loads _trips_host.so, the host side of adamw.py and lookup.py (trips_amd/csrc/torch_shim/trips_host.cpp)."""
+"""Loads _trips_host.so, the host side of adamw.py, lookup.py, table_loss.py and dropout.py (trips_amd/csrc/torch_shim/trips_host.cpp)."""
 import functools
 
 from . import _lib

@@ -28,6 +28,8 @@ OPTIM_SYMBOLS = ["trips_adamw_workspace_size", "trips_adamw_step", "trips_grad_n
 # every symbol include/trips_lookup.h declares
 LOOKUP_SYMBOLS = ["trips_lookup_workspace_size", "trips_lookup_forward", "trips_lookup_plan_workspace_size",
                   "trips_lookup_plan", "trips_lookup_backward_workspace_size", "trips_lookup_backward"]
+# every symbol include/trips_loss.h declares
+LOSS_SYMBOLS = ["trips_table_loss_workspace_size", "trips_table_loss_forward", "trips_table_loss_backward", "trips_dropout"]
 
 
 class TripsError(RuntimeError):
@@ -91,6 +93,10 @@ def load():
     lib.trips_lookup_plan.argtypes = [vp, i64, i64, vp, i32, vp, vp, vp, C.c_size_t, vp]
     lib.trips_lookup_backward_workspace_size.argtypes = [C.POINTER(abi.TripsLookupDesc), C.POINTER(C.c_size_t)]
     lib.trips_lookup_backward.argtypes = [vp, C.POINTER(abi.TripsLookupDesc), vp, vp, vp, vp, vp, C.c_size_t, vp]
+    lib.trips_table_loss_workspace_size.argtypes = [C.POINTER(abi.TripsTableLossDesc), i32, C.POINTER(C.c_size_t)]
+    lib.trips_table_loss_forward.argtypes = [vp, C.POINTER(abi.TripsTableLossDesc), vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+    lib.trips_table_loss_backward.argtypes = [vp, C.POINTER(abi.TripsTableLossDesc), vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+    lib.trips_dropout.argtypes = [vp, C.POINTER(abi.TripsDropoutDesc), vp, vp, vp, vp, vp, vp]
     lib.trips_profile_enable.argtypes = [vp, i32]
     lib.trips_splat_pair_rows_mode.argtypes = [vp, i32]
     lib.trips_profile_read.argtypes = [vp, C.POINTER(i32), C.POINTER(C.c_char_p), C.POINTER(C.c_float),

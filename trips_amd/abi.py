@@ -34,6 +34,9 @@ TRIPS_TABLE_COLUMNS = 0
 TRIPS_TABLE_ROWS = 1
 TRIPS_INDEX_I64 = 0
 TRIPS_INDEX_I32 = 1
+TRIPS_REDUCE_NONE = 0
+TRIPS_REDUCE_SUM = 1
+TRIPS_REDUCE_MEAN = 2
 
 
 class TripsView(C.Structure):
@@ -225,6 +228,37 @@ class TripsLookupDesc(C.Structure):
         ("table_stride", C.c_int64),
         ("values_stride", C.c_int64),
         ("scale", C.c_float),
+    ]
+
+
+class TripsTableLossDesc(C.Structure):
+    """include/trips_loss.h"""
+    _fields_ = [
+        ("abi_version", C.c_int32),
+        ("dtype", C.c_int32),
+        ("index_dtype", C.c_int32),
+        ("reduction", C.c_int32),
+        ("num_rows", C.c_int64),
+        ("num_entries", C.c_int64),
+        ("num_channels", C.c_int32),
+        ("scale", C.c_float),
+        ("rows_stride", C.c_int64),
+        ("table_stride", C.c_int64),
+        ("d_rows_stride", C.c_int64),
+        ("d_table_stride", C.c_int64),
+    ]
+
+
+class TripsDropoutDesc(C.Structure):
+    """include/trips_loss.h"""
+    _fields_ = [
+        ("abi_version", C.c_int32),
+        ("dtype", C.c_int32),
+        ("n", C.c_int64),
+        ("p", C.c_double),
+        ("seed", C.c_uint64),
+        ("call", C.c_uint32),
+        ("step", C.c_uint32),
     ]
 
 

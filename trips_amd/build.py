@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtrips_splat.so")
 SOURCES = ["trips_splat_abi.hip", "splat_forward.hip", "splat_backward.hip", "misc_kernels.hip", "unet_forward.hip",
-           "unet_backward.hip", "adamw_kernels.hip", "lookup_kernels.hip"]
+           "unet_backward.hip", "adamw_kernels.hip", "lookup_kernels.hip", "loss_kernels.hip", "dropout_kernels.hip"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
     # packed FP32 instructions are kept out of the generated code on purpose
@@ -26,7 +26,7 @@ def hipcc():
 
 HEADERS = ["splat_internal.h", "trips_math.h", "row16.h", "unet_common.h", "abi_common.h", os.path.join("..", "..", "include", "trips_splat.h"),
            os.path.join("..", "..", "include", "trips_unet.h"), os.path.join("..", "..", "include", "trips_optim.h"),
-           os.path.join("..", "..", "include", "trips_lookup.h")]
+           os.path.join("..", "..", "include", "trips_lookup.h"), os.path.join("..", "..", "include", "trips_loss.h")]
 
 
 def build(verbose=False, incremental=False):
@@ -113,7 +113,7 @@ def _build_torch_extension(name, sources, lib, verbose, incremental=False):
 
 
 def build_host(verbose=False, incremental=False):
-    """Builds _trips_host.so, the host side of trips_amd/adamw.py; after build(), whose library it links."""
+    """Builds _trips_host.so, the host side of trips_amd/adamw.py, lookup.py, table_loss.py and dropout.py; after build(), whose library it links."""
     return _build_torch_extension("_trips_host", ("trips_host.cpp",), HOST_LIB, verbose, incremental)
 
 
@@ -129,6 +129,6 @@ if __name__ == "__main__":
     if _has_torch():
         print(build_host(verbose=True, incremental="--incremental" in sys.argv))
     else:
-        print("no torch: _trips_host.so, which adamw.py and lookup.py need, is left out")
+        print("no torch: _trips_host.so, which adamw.py, lookup.py, table_loss.py and dropout.py need, is left out")
     if "--shim" in sys.argv:
         print(build_torch_shim(verbose=True))

@@ -1,4 +1,4 @@
-// The host side of trips_amd/adamw.py and trips_amd/lookup.py: what the C ABI takes of each tensor, collected from the objects
+// The host side of trips_amd/adamw.py, lookup.py, table_loss.py and dropout.py: what the C ABI takes of each tensor, collected from the objects
 // that torch keeps. In Python a tensor's score of attributes and checks took 1.3 to 2 us, more than its share of the kernels'
 // time in a step over a net (18 tensors 32 us a step and 17 so, 40 with copies 68 and 29), and a lookup 10 us.
 #include <torch/csrc/DynamicTypes.h>
@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "../../../include/trips_lookup.h"
+#include "../../../include/trips_loss.h"
 #include "../../../include/trips_optim.h"
 
 namespace py = pybind11;
@@ -325,6 +326,88 @@ at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& gr
     if (out && !d_table.is_inference()) d_table.unsafeGetTensorImpl()->bump_version();
     return d_table;
 }
+
+// ---- a table's cross entropy ----
+
+TripsTableLossDesc loss_desc(const at::Tensor& rows, const at::Tensor& table, const at::Tensor& target, float scale, int reduction)
+{
+    TripsTableLossDesc d{};
+    d.abi_version = TRIPS_ABI_VERSION, d.dtype = dtype_of(rows), d.index_dtype = index_dtype_of(target), d.reduction = reduction, d.scale = scale;
+    if (table.scalar_type() != rows.scalar_type() || table.size(1) != rows.size(1))
+        throw py::value_error("rows and table: matrices of one type and as many channels expected, got " + std::to_string(rows.size(1)) + " and " + std::to_string(table.size(1)) + " channels");
+    if (target.numel() != rows.size(0)) throw py::value_error("target: " + std::to_string(target.numel()) + " entries for " + std::to_string(rows.size(0)) + " rows");
+    d.num_rows = rows.size(0), d.num_entries = table.size(0), d.num_channels = (int32_t)std::min<int64_t>(rows.size(1), INT32_MAX);
+    return d;
+}
+
+// {loss, state}
+std::pair<at::Tensor, at::Tensor> table_loss(uintptr_t ctx, uintptr_t stream, const at::Tensor& rows, const at::Tensor& table, const at::Tensor& target, float scale, int reduction)
+{
+    index_dtype_of(target);
+    int64_t rows_stride, table_stride;
+    const at::Tensor x = rows_of("rows", rows, target, rows_stride), w = rows_of("table", table, target, table_stride);
+    TripsTableLossDesc d = loss_desc(x, w, target, scale, reduction);
+    d.rows_stride = rows_stride, d.table_stride = table_stride;
+    size_t need = 0;
+    check(trips_table_loss_workspace_size(&d, 0, &need));
+    const auto options = x.options().dtype(at::kFloat).requires_grad(false);
+    at::Tensor loss = reduction == TRIPS_REDUCE_NONE ? torch::empty({d.num_rows}, options) : torch::empty({}, options), state = torch::empty({d.num_rows, 2}, options);
+    const at::Tensor workspace = bytes(need, x), t = target.contiguous();
+    check(trips_table_loss_forward(reinterpret_cast<TripsCtx*>(ctx), &d, x.data_ptr(), w.data_ptr(), t.data_ptr(), (float*)loss.data_ptr(), (float*)state.data_ptr(), data(workspace), need,
+                                   reinterpret_cast<void*>(stream)));
+    return {loss, state};
+}
+
+// {d_rows, d_table}, where they are asked for
+std::pair<std::optional<at::Tensor>, std::optional<at::Tensor>> table_loss_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& d_loss, const at::Tensor& rows,
+                                                                                    const at::Tensor& table, const at::Tensor& target, const at::Tensor& state, float scale, int reduction,
+                                                                                    bool want_rows, bool want_table)
+{
+    index_dtype_of(target);
+    int64_t rows_stride, table_stride;
+    const at::Tensor x = rows_of("rows", rows, target, rows_stride), w = rows_of("table", table, target, table_stride);
+    TripsTableLossDesc d = loss_desc(x, w, target, scale, reduction);
+    const int64_t losses = reduction == TRIPS_REDUCE_NONE ? d.num_rows : 1;
+    if (d_loss.scalar_type() != at::kFloat || d_loss.numel() != losses || d_loss.device() != x.device())
+        throw py::value_error("the loss's gradient: " + std::to_string(losses) + " float32 numbers on the rows' device expected");
+    if (state.scalar_type() != at::kFloat || state.numel() != 2 * d.num_rows || state.device() != x.device() || !state.is_contiguous()) throw py::value_error("state is not what the loss left");
+    d.rows_stride = rows_stride, d.table_stride = table_stride, d.d_rows_stride = d.d_table_stride = d.num_channels;
+    const auto options = x.options().requires_grad(false);
+    std::optional<at::Tensor> d_rows, d_table;
+    if (want_rows) d_rows = torch::empty({d.num_rows, d.num_channels}, options);
+    if (want_table) d_table = torch::empty({d.num_entries, d.num_channels}, options);
+    size_t need = 0;
+    check(trips_table_loss_workspace_size(&d, 1, &need));
+    const at::Tensor workspace = bytes(need, x), t = target.contiguous(), g = d_loss.contiguous();
+    check(trips_table_loss_backward(reinterpret_cast<TripsCtx*>(ctx), &d, x.data_ptr(), w.data_ptr(), t.data_ptr(), (const float*)state.data_ptr(), (const float*)g.data_ptr(),
+                                    d_rows ? d_rows->data_ptr() : nullptr, d_table ? d_table->data_ptr() : nullptr, data(workspace), need, reinterpret_cast<void*>(stream)));
+    return {d_rows, d_table};
+}
+
+// ---- dropout ----
+
+// {out, the step that was used (where it was read from the device and is asked for)}
+std::pair<at::Tensor, std::optional<at::Tensor>> dropout(uintptr_t ctx, uintptr_t stream, const at::Tensor& x, double p, uint64_t seed, uint32_t call, uint32_t step,
+                                                         const std::optional<at::Tensor>& step_at, const std::optional<at::Tensor>& residual, bool want_step)
+{
+    if (!(p >= 0.0 && p <= 1.0)) throw py::value_error("p: 0 to 1 expected, got " + std::to_string(p));
+    if (dtype_of(x) < 0 || x.layout() != at::kStrided) throw py::value_error("x: a float32, bfloat16 or float16 tensor expected, got " + std::string(torch::getTHPDtype(x.scalar_type())->name));
+    if (!x.is_cuda()) throw std::runtime_error("dropout needs tensors on a GPU: there is no CPU implementation");
+    if (residual && (residual->scalar_type() != x.scalar_type() || residual->sizes() != x.sizes() || residual->device() != x.device() || residual->layout() != at::kStrided))
+        throw py::value_error("residual: a tensor of x's type and shape on its device expected");
+    if (step_at && ((step_at->scalar_type() != at::kInt && step_at->scalar_type() != at::kLong) || step_at->numel() != 1 || step_at->device() != x.device()))
+        throw py::value_error("step: a number, or one int32 or int64 on x's device, expected");
+    TripsDropoutDesc d{};
+    d.abi_version = TRIPS_ABI_VERSION, d.dtype = dtype_of(x), d.n = x.numel(), d.p = p, d.seed = seed, d.call = call, d.step = step;
+    const at::Tensor from = x.detach().contiguous(), added = residual ? residual->detach().contiguous() : at::Tensor();
+    at::Tensor out = torch::empty(x.sizes(), x.options().requires_grad(false));
+    std::optional<at::Tensor> used;
+    if (step_at && want_step) used = torch::empty({}, x.options().dtype(at::kInt).requires_grad(false));
+    // (the low word of an int64)
+    check(trips_dropout(reinterpret_cast<TripsCtx*>(ctx), &d, from.data_ptr(), data(added), step_at ? (const uint32_t*)step_at->data_ptr() : nullptr,
+                        used ? (uint32_t*)used->data_ptr() : nullptr, out.data_ptr(), reinterpret_cast<void*>(stream)));
+    return {out, used};
+}
 }  // namespace
 
 PYBIND11_MODULE(_trips_host, m)
@@ -334,4 +417,7 @@ PYBIND11_MODULE(_trips_host, m)
     m.def("lookup", &lookup);
     m.def("lookup_plan", &lookup_plan);
     m.def("lookup_backward", &lookup_backward);
+    m.def("table_loss", &table_loss);
+    m.def("table_loss_backward", &table_loss_backward);
+    m.def("dropout", &dropout);
 }

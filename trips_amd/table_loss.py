@@ -1,0 +1,49 @@
+"""Softmax cross entropy of rows against all entries of a table, and its gradients, over the HIP kernels of include/trips_loss.h.
+
+The other end of a table whose rows lookup() reads: which entry a row belongs to, among all of them. The logits are never kept:
+the loss is made in one pass over the table, the gradients from logits that are computed again in pieces of it.
+"""
+import torch
+from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
+
+from . import abi
+from ._host import host as _host
+from .lookup import _transformed, _where
+from .renderer import _untraced
+
+REDUCTIONS = {"none": abi.TRIPS_REDUCE_NONE, "sum": abi.TRIPS_REDUCE_SUM, "mean": abi.TRIPS_REDUCE_MEAN}
+
+
+class _TableCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, table, target, scale, reduction):
+        with _untraced():
+            loss, state = _host().table_loss(*_where(target), rows.detach(), table.detach(), target, scale, reduction)
+        ctx.save_for_backward(rows, table, target, state)
+        ctx.args = (scale, reduction)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        rows, table, target, state = ctx.saved_tensors
+        d_rows, d_table = _host().table_loss_backward(*_where(target), grad, rows.detach(), table.detach(), target, state, *ctx.args,
+                                                      ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return d_rows, d_table, None, None, None
+
+
+def table_cross_entropy(rows, table, target, scale=1.0, reduction="mean"):
+    """What rows [N, C] lose on their targets among the entries of table [T, C]: with logits l = scale <row, entry>, the log of
+    the sum of exp(l) over all entries, minus l of the target. target: N integers (int32 or int64, of any shape, like an index of
+    lookup()); rows whose target is outside the table (padding) count for nothing and get no gradient, whatever they hold.
+
+    reduction: "none" gives [N], "sum" and "mean" one number, the mean over the rows that count (0 where none does); float32
+    whatever the type of rows and table (float32, bfloat16 or float16, the same of both). Differentiable in rows and table, once; gradients
+    have their type. In float16 the gradients of rows whose loss counts 2^-15 as much as another's lose precision."""
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"reduction: 'none', 'sum' or 'mean' expected, got {reduction!r}")
+    graph = torch.is_grad_enabled() and (rows.requires_grad or table.requires_grad)
+    if graph or forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(rows, table, target):
+        return _TableCrossEntropy.apply(rows, table, target, scale, REDUCTIONS[reduction])
+    return _host().table_loss(*_where(target), rows.detach(), table.detach(), target, scale, REDUCTIONS[reduction])[0]
