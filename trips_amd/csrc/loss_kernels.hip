@@ -8,6 +8,7 @@
 // is kept apart: where all entries are masked with the type's lowest value their probabilities are still equal.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "abi_common.h"
 
@@ -222,7 +223,7 @@ constexpr int kTile = 128, kStep = 16, kRow = kTile + 4;
 
 struct ProductParams
 {
-    const void* table;     // of entry 0
+    const void* table;     // the piece's entries
     const void* packed;    // [count][kp]
     const int* count;
     const int* packed_target;
@@ -231,11 +232,12 @@ struct ProductParams
     const float* unscale;
     float2* partial;       // LOGITS: [stripes][rows_pad] {largest product, sum of exponentials}
     float* own_product;    // [rows_pad]
-    float* probs;          // [rows_pad][piece]
+    void* probs;           // [rows_pad][piece], in the tensors' type
     float* slabs;          // D_ROWS: [splits][rows_pad][kp]
     void* d_table;
-    long long table_stride, d_table_stride, entries, first_entry, rows_pad;
-    int channels, kp, piece, stripes, splits, add;
+    long long table_stride, d_table_stride, rows_pad;
+    int held;              // channels that a row of the table holds: those, or with zeros behind them to a multiple of 64
+    int first_entry, in_piece, channels, kp, piece, stripes, first_stripe, splits, add;
     unsigned tiles_x, tiles_y;
     float scale_log2;
 };
@@ -260,7 +262,8 @@ __global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
     // the tile
     const unsigned block_x = blockIdx.x % p.tiles_x, block_y = blockIdx.x / p.tiles_x % p.tiles_y, block_z = blockIdx.x / p.tiles_x / p.tiles_y;
     const long long n0     = (long long)block_y * kTile;
-    const int in_piece = (int)min((long long)p.piece, p.entries - p.first_entry);
+    const int in_piece     = p.in_piece;
+    float* probs           = reinterpret_cast<float*>(p.probs);
     if ((MODE == D_TABLE ? (long long)in_piece : (long long)count) <= n0) return;
     const int rows_up = (count + kStep - 1) / kStep * kStep;
     int k_begin = 0, k_end = MODE == D_TABLE ? rows_up : p.kp;
@@ -272,10 +275,10 @@ __global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
 
     float2 best[2];  // LOGITS: of the wave's rows (a lane: one of 32), in this stripe
     best[0] = best[1] = make_float2(-__builtin_inff(), 0.f);
-    const long long tiles = MODE == LOGITS ? (p.entries + kTile - 1) / kTile : 0;
-    for (long long tile = block_x; tile < (MODE == LOGITS ? tiles : (long long)block_x + 1); tile += MODE == LOGITS ? p.stripes : 1)
+    const int tiles = MODE == LOGITS ? (in_piece + kTile - 1) / kTile : 0;
+    for (int tile = block_x; tile < (MODE == LOGITS ? tiles : (int)block_x + 1); tile += MODE == LOGITS ? p.stripes : 1)
     {
-        const long long m0 = tile * kTile;
+        const int m0 = tile * kTile;
         Acc acc[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -292,18 +295,18 @@ __global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
             for (int e = 0; e < 8; ++e) a[e] = b[e] = 0.f;
             if constexpr (FIRST_ALONG_K)
             {
-                const long long j = (MODE == PROBS ? p.first_entry : 0) + m0 + (threadIdx.x >> 1);
+                const int j       = m0 + (threadIdx.x >> 1);
                 const int k       = k0 + (threadIdx.x & 1) * 8;
                 const T* at       = reinterpret_cast<const T*>(p.table) + j * p.table_stride + k;
-                if (j < p.entries)
+                if (j < in_piece)
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         if (k + e < p.channels) a[e] = E::to_float(at[e]);
             }
             else
             {
-                const int k = k0 + (threadIdx.x >> 4), c = (int)m0 + (threadIdx.x & 15) * 8;
-                const T* at = MODE == D_ROWS ? reinterpret_cast<const T*>(p.table) + (p.first_entry + k) * p.table_stride + c
+                const int k = k0 + (threadIdx.x >> 4), c = m0 + (threadIdx.x & 15) * 8;
+                const T* at = MODE == D_ROWS ? reinterpret_cast<const T*>(p.table) + k * p.table_stride + c
                                              : reinterpret_cast<const T*>(p.packed) + (long long)k * p.kp + c;
                 if (k < (MODE == D_ROWS ? in_piece : count))
 #pragma unroll
@@ -325,14 +328,14 @@ __global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
                 if (r < count)
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (k + e < in_piece) b[e] = p.probs[r * p.piece + k + e];
+                        if (k + e < in_piece) b[e] = probs[r * p.piece + k + e];
             }
             else
             {
                 const int k = k0 + (threadIdx.x >> 4);
                 if (k < count)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) b[e] = p.probs[(long long)k * p.piece + n0 + (threadIdx.x & 15) * 8 + e];
+                    for (int e = 0; e < 8; ++e) b[e] = probs[(long long)k * p.piece + n0 + (threadIdx.x & 15) * 8 + e];
             }
         };
         auto put = [&](int buffer)
@@ -387,18 +390,18 @@ __global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
             const long long n = n0 + wn + j * 32 + (lane & 31);
             if constexpr (MODE == LOGITS)
             {
-                const int own = n < count ? p.packed_target[n] : -1;
+                const int own = n < count ? p.packed_target[n] - p.first_entry : -1;
                 float top     = -__builtin_inff();
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                     {
-                        const long long m = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                        const float l     = m < p.entries ? acc[i][j][e] : -__builtin_inff();
-                        if (m == own) p.own_product[n] = l;
-                        acc[i][j][e] = l;
-                        top          = fmaxf(top, l);
+                        const int m   = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                        const float l = m < in_piece ? acc[i][j][e] : -__builtin_inff();
+                        if (m == own && m < in_piece) p.own_product[n] = l;
+                        acc[i][j][e]  = l;
+                        top           = fmaxf(top, l);
                     }
                 top              = fmaxf(top, __shfl_xor(top, 32));
                 const float now  = fmaxf(best[j].x, top);
@@ -414,7 +417,7 @@ __global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
             else if constexpr (MODE == PROBS)
             {
                 const bool in   = n < count;
-                const int own   = in ? p.packed_target[n] : -1;
+                const int own   = in ? p.packed_target[n] - p.first_entry : -1;
                 const float2 state = in ? p.packed_state[n] : make_float2(0.f, 0.f);
                 const float factor = in ? p.packed_factor[n] : 0.f;
 #pragma unroll
@@ -422,11 +425,10 @@ __global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                     {
-                        const int in_tile = (int)m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                        const long long m = p.first_entry + in_tile;
-                        float q           = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - state.x, p.scale_log2, -state.y));
+                        const int m = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                        float q     = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - state.x, p.scale_log2, -state.y));
                         if (m == own) q -= 1.f;
-                        if (in && in_tile < p.piece) p.probs[n * p.piece + in_tile] = in_tile < in_piece ? q * factor : 0.f;
+                        if (in && m < p.piece) probs[n * p.piece + m] = m < in_piece ? q * factor : 0.f;
                     }
             }
             else
@@ -437,7 +439,7 @@ __global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                     {
-                        const int c = (int)m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                        const int c = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
                         if constexpr (MODE == D_ROWS)
                         {
                             float* at = p.slabs + ((long long)block_z * p.rows_pad + n) * p.kp + c;
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
                         else
                         {
                             if (n < in_piece && c < p.channels)
-                                reinterpret_cast<T*>(p.d_table)[(p.first_entry + n) * p.d_table_stride + c] = E::from_float(acc[i][j][e] * unscale);
+                                reinterpret_cast<T*>(p.d_table)[n * p.d_table_stride + c] = E::from_float(acc[i][j][e] * unscale);
                         }
                     }
             }
@@ -463,7 +465,399 @@ __global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
         {
             const float2 a = joined[0][threadIdx.x], b = joined[1][threadIdx.x];
             const float top = fmaxf(a.x, b.x), base = top == -__builtin_inff() ? 0.f : top;
-            p.partial[block_x * p.rows_pad + n0 + threadIdx.x] = make_float2(top, a.y * part_of(a.x, base, p.scale_log2) + b.y * part_of(b.x, base, p.scale_log2));
+            p.partial[(p.first_stripe + block_x) * p.rows_pad + n0 + threadIdx.x] = make_float2(top, a.y * part_of(a.x, base, p.scale_log2) + b.y * part_of(b.x, base, p.scale_log2));
+        }
+    }
+}
+
+// Entries one behind the other in rows of kp elements, zeros from the channels on: for tables whose rows the direct loads cannot take.
+__global__ __launch_bounds__(256) void copy_entries_kernel(const unsigned short* table, long long stride, unsigned short* to, long long entries, int channels, int kp)
+{
+    using Wide          = Pack<unsigned short, 8>::type;
+    const int pieces    = kp / 8;
+    const long long all = entries * pieces;
+    for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < all; q += (long long)gridDim.x * 256)
+    {
+        const long long j          = q / pieces;
+        const int c                = (int)(q % pieces) * 8;
+        const unsigned short* from = table + j * stride + c;
+        Wide x;
+        if (c + 8 <= channels)
+            x = *reinterpret_cast<const Wide*>(from);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = c + e < channels ? from[e] : (unsigned short)0;
+        *reinterpret_cast<Wide*>(to + q * 8) = x;
+    }
+}
+
+// ---- products of 16-bit types ----
+
+// Tiles of BM x BN in steps of BK along k, both operands by direct loads to LDS, STAGES steps of them at a time; WM x WN wavefronts.
+template <int BM_, int BN_, int WM_, int WN_, int BK_, int STAGES_>
+struct Shape
+{
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, STAGES = STAGES_;
+    static constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+    static constexpr int FIRST_BYTES = BM * BK * 2, STAGE_BYTES = (BM + BN) * BK * 2;
+    static constexpr int FIRST_LOADS = FIRST_BYTES / 1024 / WAVES, SECOND_LOADS = BN * BK * 2 / 1024 / WAVES;
+    static_assert(FIRST_LOADS * WAVES * 1024 == FIRST_BYTES && SECOND_LOADS * WAVES * 1024 == BN * BK * 2, "whole loads of a wavefront");
+};
+
+typedef int Words4 __attribute__((ext_vector_type(4)));
+typedef short Half4 __attribute__((ext_vector_type(4)));
+typedef short Half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 Bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 F8 __attribute__((ext_vector_type(8)));
+
+template <int D>
+__device__ __forceinline__ Acc mfma16(Half8 a, Half8 b, Acc c)
+{
+    if constexpr (D == TRIPS_DTYPE_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf8, a), __builtin_bit_cast(Bf8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(F8, a), __builtin_bit_cast(F8, b), c, 0, 0, 0);
+}
+
+// 64 lanes' 16 bytes from a buffer, each at its own offset, to LDS one behind the other; zeros from beyond the buffer's end.
+// (By itself: of a builtin the compiler would wait for the last load before any read of LDS.)
+__device__ __forceinline__ void load_to_lds(const Words4& buffer, unsigned offset, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
+}
+__device__ __forceinline__ Words4 buffer_of(const void* base, long long bytes)
+{
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    const int n      = (int)min(max(bytes, 0ll), 0x7fffffffll);
+    return Words4{__builtin_amdgcn_readfirstlane((int)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xFFFF)), __builtin_amdgcn_readfirstlane(n), 0x00020000};
+}
+template <int LOADS>
+__device__ __forceinline__ void wait_and_meet()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+}
+
+constexpr unsigned kBeyond = 0x80000000u;  // an offset beyond any buffer
+
+// An operand whose rows run along k: LDS rows of BK elements, their pieces of 16 bytes in an order that depends on the row, so that
+// eight lanes that read the same piece of eight rows meet eight different places of the 128 bytes that LDS gives a cycle.
+template <int ROWS, int BK, int LOADS>
+struct AlongK
+{
+    static constexpr int PIECES = BK / 8;
+    unsigned offset[LOADS];
+    int k_of[LOADS];
+    const char* base;
+    long long bytes;
+    static __device__ __forceinline__ int turn(int row) { return PIECES == 8 ? row & 7 : (row >> 1) & 3; }
+    __device__ __forceinline__ void begin(const void* at, long long stride_bytes, long long size, int wave, int lane)
+    {
+        base = reinterpret_cast<const char*>(at), bytes = size;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+        {
+            const int row   = (wave * LOADS + i) * (64 / PIECES) + lane / PIECES;
+            const int piece = (lane % PIECES) ^ turn(row);
+            offset[i] = (unsigned)(row * stride_bytes) + piece * 16, k_of[i] = piece * 8;
+        }
+    }
+    __device__ __forceinline__ void load(int k0, int k_end, unsigned lds, int wave) const
+    {
+        const Words4 buffer = buffer_of(base, bytes);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load_to_lds(buffer, k0 + k_of[i] < k_end ? offset[i] + 2 * k0 : kBeyond, lds + (wave * LOADS + i) * 1024);
+    }
+    // fragment f of the wavefront's rows from `row` on: 32 rows, 16 elements from 16 kk on, eight a lane
+    static __device__ __forceinline__ Half8 read(const char* lds, int row, int f, int kk, int lane)
+    {
+        const int r = row + (lane & 31);
+        return *reinterpret_cast<const Half8*>(lds + (r + f * 32) * (BK * 2) + (((kk * 2 + (lane >> 5)) ^ turn(r)) * 16));
+    }
+};
+
+// An operand whose rows run along the tile: LDS rows of ROWS elements, one of each k, read through the transposing loads (of 16 lanes'
+// four elements: lane i gets element i % 4 of lanes i / 4, i / 4 + 4, ...). Their pieces of 64 bytes are in an order that depends on k, so that
+// the four rows of 16 lanes lie apart.
+template <int ROWS, int BK, int LOADS>
+struct AcrossK
+{
+    static constexpr int PIECES = ROWS / 8, TURNS = PIECES / 4;
+    unsigned offset[LOADS];
+    const char* base;
+    long long stride, bytes;
+    static __device__ __forceinline__ int turn(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) & (TURNS - 1); }
+    __device__ __forceinline__ void begin(const void* at, long long stride_bytes, long long size, int wave, int lane)
+    {
+        base = reinterpret_cast<const char*>(at), stride = stride_bytes, bytes = size;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+        {
+            const int k     = (wave * LOADS + i) * (64 / PIECES) + lane / PIECES, piece = lane % PIECES;
+            offset[i] = (unsigned)(k * stride_bytes) + ((((piece >> 2) ^ turn(k)) << 2) | (piece & 3)) * 16;
+        }
+    }
+    __device__ __forceinline__ void load(int k0, int, unsigned lds, int wave) const
+    {
+        const Words4 buffer = buffer_of(base + k0 * stride, bytes - k0 * stride);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load_to_lds(buffer, offset[i], lds + (wave * LOADS + i) * 1024);
+    }
+    static __device__ __forceinline__ Half8 read(const char* lds, int row, int f, int kk, int lane)
+    {
+        const int k    = kk * 16 + (lane >> 5) * 8 + ((lane >> 2) & 3);
+        const char* at = lds + k * (ROWS * 2) + (((row >> 5) + f) ^ turn(k)) * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+        using P        = __attribute__((address_space(3))) Half4*;
+        const Half4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 4 * ROWS * 2));
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+template <bool ALONG, int ROWS, int BK, int LOADS>
+using Operand = std::conditional_t<ALONG, AlongK<ROWS, BK, LOADS>, AcrossK<ROWS, BK, LOADS>>;
+
+// Workgroups as they start go around the eight XCDs; here each XCD takes a run of tiles, in which eight of the second operand's share one
+// of the first's at a time.
+__device__ __forceinline__ void tile_of(unsigned id, unsigned all, unsigned across, unsigned down, unsigned& x, unsigned& y, unsigned& z)
+{
+    const unsigned each = all >> 3;
+    if (id < each * 8) id = (id & 7) * each + (id >> 3);
+    z                  = id / (across * down);
+    id                 = id % (across * down);
+    const unsigned g = id / (across * 8), in = id % (across * 8), high = min(8u, down - g * 8);
+    x = in / high, y = g * 8 + in % high;
+}
+
+// f(fragment, element of it, row of a lane's first fragment) for each of a lane's elements of one column of fragments
+template <int FM, typename F>
+__device__ __forceinline__ void each_element(F f)
+{
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f(i, e, i * 32 + 8 * (e >> 2) + (e & 3));
+}
+
+template <int D, int MODE, typename S>
+__global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const ProductParams p)
+{
+    using E = Element<D>;
+    using T = typename E::type;
+    constexpr bool FIRST_ALONG = MODE == LOGITS || MODE == PROBS, SECOND_ALONG = MODE != D_TABLE;
+    using First  = Operand<FIRST_ALONG, S::BM, S::BK, S::FIRST_LOADS>;
+    using Second = Operand<SECOND_ALONG, S::BN, S::BK, S::SECOND_LOADS>;
+    constexpr int LOADS = S::FIRST_LOADS + S::SECOND_LOADS;
+    __shared__ __attribute__((aligned(1024))) char lds[S::STAGES * S::STAGE_BYTES];
+    const unsigned lds_at = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave % S::WM * S::TM, wn = wave / S::WM * S::TN;
+    const int count = *p.count;
+
+    unsigned block_x, block_y, block_z;
+    tile_of(blockIdx.x, gridDim.x, p.tiles_x, p.tiles_y, block_x, block_y, block_z);
+    const long long n0 = (long long)block_y * S::BN;
+    if ((MODE == D_TABLE ? (long long)p.in_piece : (long long)count) <= n0) return;
+    int k_begin = 0, k_end = MODE == D_TABLE ? count : p.held;
+    if (MODE == D_ROWS)
+    {
+        const int steps = (p.in_piece + S::BK - 1) / S::BK, each = (steps + p.splits - 1) / p.splits;
+        k_begin = min(p.in_piece, (int)block_z * each * S::BK), k_end = min(p.in_piece, k_begin + each * S::BK);
+    }
+    const int steps = (k_end - k_begin + S::BK - 1) / S::BK;
+
+    First first;
+    Second second;
+    const char* packed = reinterpret_cast<const char*>(p.packed);
+    const char* probs  = reinterpret_cast<const char*>(p.probs);
+    if constexpr (MODE == LOGITS || MODE == PROBS)
+        second.begin(packed + n0 * p.kp * 2, p.kp * 2, (count - n0) * p.kp * 2, wave, lane);
+    else if constexpr (MODE == D_ROWS)
+        second.begin(probs + n0 * p.piece * 2, (long long)p.piece * 2, (p.rows_pad - n0) * p.piece * 2, wave, lane);
+    else
+        second.begin(probs + n0 * 2, (long long)p.piece * 2, ((long long)count * p.piece - n0) * 2, wave, lane);
+
+    float2 best[S::FN];
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) best[j] = make_float2(-__builtin_inff(), 0.f);
+
+    const int tiles = MODE == LOGITS ? (p.in_piece + S::BM - 1) / S::BM : 0;
+    for (int tile = block_x; tile < (MODE == LOGITS ? tiles : (int)block_x + 1); tile += MODE == LOGITS ? p.stripes : 1)
+    {
+        const int m0 = tile * S::BM;
+        if constexpr (FIRST_ALONG)
+            first.begin(reinterpret_cast<const T*>(p.table) + m0 * p.table_stride, p.table_stride * 2, ((long long)(min(p.in_piece - m0, S::BM) - 1) * p.table_stride + p.held) * 2, wave, lane);
+        else if constexpr (MODE == D_ROWS)
+            first.begin(reinterpret_cast<const T*>(p.table) + m0, p.table_stride * 2, ((p.in_piece - 1ll) * p.table_stride + p.held - m0) * 2, wave, lane);
+        else
+            first.begin(packed + m0 * 2, p.kp * 2, ((long long)count * p.kp - m0) * 2, wave, lane);
+
+        Acc acc[S::FM][S::FN];
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+        auto issue = [&](int step, int stage)
+        {
+            const int k0 = k_begin + step * S::BK;
+            first.load(k0, k_end, lds_at + stage * S::STAGE_BYTES, wave);
+            second.load(k0, SECOND_ALONG && MODE != D_ROWS ? p.kp : k0 + S::BK, lds_at + stage * S::STAGE_BYTES + S::FIRST_BYTES, wave);
+        };
+        // (beyond the last step the loads go on, with nothing behind them, so that the waits count alike)
+#pragma unroll
+        for (int s = 0; s < S::STAGES - 1; ++s) issue(s, s);
+        int stage = 0;
+        for (int step = 0; step < steps; ++step)
+        {
+            wait_and_meet<(S::STAGES - 2) * LOADS>();
+            const int next = stage == 0 ? S::STAGES - 1 : stage - 1;
+            issue(step + S::STAGES - 1, next);
+            const char* a = lds + stage * S::STAGE_BYTES;
+            const char* b = a + S::FIRST_BYTES;
+#pragma unroll
+            for (int kk = 0; kk < S::BK / 16; ++kk)
+            {
+                Half8 x[S::FM], y[S::FN];
+#pragma unroll
+                for (int i = 0; i < S::FM; ++i) x[i] = First::read(a, wm, i, kk, lane);
+#pragma unroll
+                for (int j = 0; j < S::FN; ++j) y[j] = Second::read(b, wn, j, kk, lane);
+#pragma unroll
+                for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma16<D>(x[i], y[j], acc[i][j]);
+            }
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+        }
+        wait_and_meet<0>();  // (nothing is on its way to LDS behind this)
+
+        // a lane's elements: of row n0 + wn + 32 j + lane % 32, of the first operand's rows m0 + wm + 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j)
+        {
+            const long long n = n0 + wn + j * 32 + (lane & 31);
+            const int m_lane  = m0 + wm + 4 * (lane >> 5);
+            if constexpr (MODE == LOGITS)
+            {
+                const int own = n < count ? p.packed_target[n] - p.first_entry - m_lane : -1;  // (of the lane's own elements)
+                float top     = -__builtin_inff();
+                if (m0 + S::BM > p.in_piece)
+                    each_element<S::FM>([&](int i, int e, int m)
+                    {
+                        if (m_lane + m >= p.in_piece) acc[i][j][e] = -__builtin_inff();
+                    });
+                if (__any(own >= 0 && own < S::TM))
+                {
+                    float product = 0.f;
+                    bool here     = false;
+                    each_element<S::FM>([&](int i, int e, int m)
+                    {
+                        if (m == own) product = acc[i][j][e], here = m_lane + m < p.in_piece;
+                    });
+                    if (here) p.own_product[n] = product;
+                }
+                each_element<S::FM>([&](int i, int e, int) { top = fmaxf(top, acc[i][j][e]); });
+                top              = fmaxf(top, __shfl_xor(top, 32));
+                const float now  = fmaxf(best[j].x, top);
+                const float base = now == -__builtin_inff() ? 0.f : now;
+                float sum        = 0.f;
+                each_element<S::FM>([&](int i, int e, int) { sum += part_of(acc[i][j][e], base, p.scale_log2); });
+                sum += __shfl_xor(sum, 32);
+                best[j] = make_float2(now, best[j].y * part_of(best[j].x, base, p.scale_log2) + sum);
+            }
+            else
+            {
+                float2 state = make_float2(0.f, 0.f);
+                float factor = MODE == D_TABLE ? p.unscale[1] : 1.f;
+                int own      = -1;
+                if (MODE == PROBS && n < count) state = p.packed_state[n], factor = p.packed_factor[n], own = p.packed_target[n] - p.first_entry - m_lane;
+                if constexpr (MODE == PROBS)
+                {
+                    each_element<S::FM>([&](int i, int e, int)
+                                        { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - state.x, p.scale_log2, -state.y)) * factor; });
+                    if (__any(own >= 0 && own < S::TM))
+                        each_element<S::FM>([&](int i, int e, int m)
+                        {
+                            if (m == own) acc[i][j][e] -= factor;
+                        });
+                    if (m0 + S::BM > p.in_piece)
+                        each_element<S::FM>([&](int i, int e, int m)
+                        {
+                            if (m_lane + m >= p.in_piece) acc[i][j][e] = 0.f;
+                        });
+                }
+#pragma unroll
+                for (int i = 0; i < S::FM; ++i)
+                {
+                    if constexpr (MODE == D_ROWS)
+                    {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g)
+                        {
+                            const int c = m_lane + i * 32 + 8 * g;
+                            using F4    = Pack<float, 4>::type;
+                            if (n < count && c < p.kp)
+                            {
+                                F4* at = reinterpret_cast<F4*>(p.slabs + ((long long)block_z * p.rows_pad + n) * p.kp + c);
+                                F4 v   = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                                if (p.add) v += *at;
+                                *at = v;
+                            }
+                        }
+                    }
+                    else
+                    {
+                        // two lanes' fours to eight of one lane: 16 bytes
+#pragma unroll
+                        for (int g = 0; g < 4; g += 2)
+                        {
+                            unsigned w[4];
+#pragma unroll
+                            for (int h = 0; h < 4; ++h)
+                                w[h] = (unsigned)E::from_float(acc[i][j][4 * g + 2 * h] * (MODE == D_TABLE ? factor : 1.f)) |
+                                       (unsigned)E::from_float(acc[i][j][4 * g + 2 * h + 1] * (MODE == D_TABLE ? factor : 1.f)) << 16;
+                            const auto low = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), high = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+                            const Words4 eight = {(int)low[0], (int)high[0], (int)low[1], (int)high[1]};
+                            const int m        = m0 + wm + i * 32 + 8 * (g + (lane >> 5));
+                            if constexpr (MODE == PROBS)
+                            {
+                                if (n < count) *reinterpret_cast<Words4*>(reinterpret_cast<T*>(p.probs) + n * p.piece + m) = eight;
+                            }
+                            else if (n < p.in_piece && m < p.channels)
+                            {
+                                T* at = reinterpret_cast<T*>(p.d_table) + n * p.d_table_stride + m;
+                                using T8 = typename Pack<T, 8>::type;
+                                const T8 v = __builtin_bit_cast(T8, eight);
+                                if (m + 8 <= p.channels)
+                                    *reinterpret_cast<T8*>(at) = v;
+                                else
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e)
+                                        if (m + e < p.channels) at[e] = v[e];
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (MODE == LOGITS)
+    {
+        float2* joined = reinterpret_cast<float2*>(lds);  // [WM][BN]
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j)
+            if (lane < 32) joined[wave % S::WM * S::BN + wn + j * 32 + lane] = best[j];
+        __syncthreads();
+        for (int n = threadIdx.x; n < S::BN; n += S::WAVES * 64)
+        {
+            float top = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < S::WM; ++w) top = fmaxf(top, joined[w * S::BN + n].x);
+            const float base = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+            for (int w = 0; w < S::WM; ++w) sum += joined[w * S::BN + n].y * part_of(joined[w * S::BN + n].x, base, p.scale_log2);
+            p.partial[(p.first_stripe + block_x) * p.rows_pad + n0 + n] = make_float2(top, sum);
         }
     }
 }
@@ -569,54 +963,85 @@ __global__ __launch_bounds__(256) void rows_out_kernel(const float* slabs, const
 
 // ---- host ----
 
-constexpr int64_t kPieceBytes = 256ll << 20;
+constexpr int64_t kPieceBytes = 256ll << 20;  // of d_ij
+constexpr int64_t kCopyBytes = 64ll << 20, kLeastCopyBytes = 16ll << 20;  // of copied entries
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+unsigned tiles_of(int64_t n, int tile) { return (unsigned)((n + tile - 1) / tile); }
 
+// Whether the direct loads take the table's rows as they are: 16 bytes at a time, 256 rows within 31 bits.
+bool rows_in_place(const TripsTableLossDesc& d) { return d.num_channels % 8 == 0 && d.table_stride % 8 == 0 && d.table_stride < 1 << 21; }
+
+// Steps of a call over the table; what each takes of the workspace.
 struct Layout
 {
     int64_t rows_pad, chunks, piece, pieces;
     int kp, stripes, splits;
-    size_t packed, place, target, state, factor, count, chunk_count, chunk_top, partial, own_product, sums, probs, slabs, bytes;
+    bool copies;
+    size_t packed, place, target, state, factor, count, chunk_count, chunk_top, partial, own_product, sums, probs, slabs, copy, bytes;
 };
 
-Layout layout_of(const TripsTableLossDesc& d, bool backward)
+struct Big : Shape<256, 256, 2, 4, 64, 2>
+{
+};
+
+// copies: the table's entries are copied, a piece at a time, before the products read them.
+Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
 {
     Layout l{};
-    l.rows_pad = up(d.num_rows, 256), l.chunks = d.num_rows > kCountedBy ? up(d.num_rows, kChunk) / kChunk : 0;
-    l.kp       = (int)up(d.num_channels, 64);
-    size_t at  = 0;
-    auto take  = [&](size_t bytes)
+    const bool wide      = d.dtype == TRIPS_DTYPE_F32;
+    const int size       = dtype_bytes(d.dtype), tile = wide ? kTile : 256;
+    l.rows_pad           = up(d.num_rows, 256), l.chunks = d.num_rows > kCountedBy ? up(d.num_rows, kChunk) / kChunk : 0;
+    l.kp                 = (int)up(d.num_channels, 64);
+    l.copies             = copies;
+    size_t at            = 0;
+    auto take            = [&](size_t bytes)
     {
         const size_t here = at;
         at += (bytes + 255) & ~(size_t)255;
         return here;
     };
     l.count  = take(256);
-    l.packed = take((size_t)d.num_rows * l.kp * dtype_bytes(d.dtype));
+    l.packed = take((size_t)d.num_rows * l.kp * size);
     l.place = take(d.num_rows * 4), l.target = take(d.num_rows * 4);
     l.chunk_count = take(l.chunks * 4), l.chunk_top = take(l.chunks * 4);
-    const int64_t row_tiles = up(d.num_rows, kTile) / kTile, tiles = up(d.num_entries, kTile) / kTile;
+    int64_t most = up(std::max<int64_t>(d.num_entries, 1), 256);
+    if (copies)
+    {
+        most   = std::min(most, std::max<int64_t>((rows_in_place(d) ? kLeastCopyBytes : kCopyBytes) / (l.kp * 2) / 256, 1) * 256);
+        l.copy = take((size_t)most * l.kp * 2);
+    }
+    if (backward) most = std::min(most, std::max<int64_t>(kPieceBytes / (std::max<int64_t>(l.rows_pad, 1) * size) / 256, 1) * 256);
+    l.pieces = std::max<int64_t>(1, (d.num_entries + most - 1) / most);
+    l.piece  = up((d.num_entries + l.pieces - 1) / l.pieces, 256);
+    const int64_t row_tiles = up(d.num_rows, tile) / tile;
     if (!backward)
     {
-        l.stripes   = (int)std::max<int64_t>(1, std::min(tiles, std::max<int64_t>(1, 4096 / std::max<int64_t>(row_tiles, 1))));
-        l.partial   = take((size_t)l.stripes * l.rows_pad * sizeof(float2));
+        const int64_t tiles = up(l.piece, tile) / tile;
+        l.stripes     = (int)std::max<int64_t>(1, std::min(tiles, 4096 / std::max<int64_t>(row_tiles, 1)));
+        l.partial     = take((size_t)l.stripes * l.pieces * l.rows_pad * sizeof(float2));
         l.own_product = take(l.rows_pad * 4);
-        l.sums      = take((d.num_rows / 16 + 1) * 8);
+        l.sums        = take((d.num_rows / 16 + 1) * 8);
     }
     else
     {
         l.state = take(d.num_rows * 8), l.factor = take(d.num_rows * 4);
-        const int64_t most = std::max<int64_t>(kPieceBytes / (std::max<int64_t>(l.rows_pad, 1) * 4) / 256, 1) * 256;
-        l.pieces = std::max<int64_t>(1, (d.num_entries + most - 1) / most);
-        l.piece  = up((d.num_entries + l.pieces - 1) / l.pieces, 256);
-        l.probs  = take((size_t)l.rows_pad * l.piece * 4);
-        const int64_t out_tiles = std::max<int64_t>(1, row_tiles * (up(d.num_channels, kTile) / kTile));
+        l.probs = take((size_t)l.rows_pad * l.piece * size);
+        const int64_t out_tiles = std::max<int64_t>(1, row_tiles * (up(d.num_channels, tile) / tile));
         l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({1024 / out_tiles, l.piece / 256, 64}));
         l.slabs  = take((size_t)l.splits * l.rows_pad * l.kp * 4);
     }
     l.bytes = at;
     return l;
+}
+
+bool copies_of(const TripsTableLossDesc& d, const void* table) { return d.dtype != TRIPS_DTYPE_F32 && !(rows_in_place(d) && aligned(table, 16)); }
+
+// For any address of the table.
+size_t workspace_of(const TripsTableLossDesc& d, bool backward)
+{
+    const size_t copied = d.dtype == TRIPS_DTYPE_F32 ? 0 : layout_of(d, backward, true).bytes;
+    return copies_of(d, nullptr) ? copied : std::max(copied, layout_of(d, backward, false).bytes);
 }
 
 // (not 0: 0 times minus infinity, which stands for entries that are not there, is no number)
@@ -645,40 +1070,72 @@ hipError_t gather(const TripsTableLossDesc& d, const Layout& l, const void* rows
     return hipGetLastError();
 }
 
-ProductParams product_params(const TripsTableLossDesc& d, const Layout& l, const void* table, char* w)
+ProductParams product_params(const TripsTableLossDesc& d, const Layout& l, char* w)
 {
     ProductParams p{};
-    p.table = table, p.packed = w + l.packed, p.count = (int*)(w + l.count), p.packed_target = (int*)(w + l.target);
+    p.packed = w + l.packed, p.count = (int*)(w + l.count), p.packed_target = (int*)(w + l.target);
     p.packed_state = (float2*)(w + l.state), p.packed_factor = (float*)(w + l.factor), p.unscale = (float*)(w + l.count) + 2;
-    p.partial = (float2*)(w + l.partial), p.own_product = (float*)(w + l.own_product), p.probs = (float*)(w + l.probs), p.slabs = (float*)(w + l.slabs);
-    p.table_stride = d.table_stride, p.d_table_stride = d.d_table_stride, p.entries = d.num_entries, p.rows_pad = l.rows_pad;
+    p.partial = (float2*)(w + l.partial), p.own_product = (float*)(w + l.own_product), p.probs = w + l.probs, p.slabs = (float*)(w + l.slabs);
+    p.d_table_stride = d.d_table_stride, p.rows_pad = l.rows_pad;
     p.channels = d.num_channels, p.kp = l.kp, p.piece = (int)l.piece, p.stripes = l.stripes, p.splits = l.splits;
     p.scale_log2 = scale_log2(d);
     return p;
 }
 
-unsigned tiles_of(int64_t n) { return (unsigned)((n + kTile - 1) / kTile); }
+// The entries of piece `piece` as the products read them.
+template <int D>
+hipError_t take_piece(const TripsTableLossDesc& d, const Layout& l, int64_t piece, const void* table, void* d_table, char* w, ProductParams& p, hipStream_t stream, Profiler* prof)
+{
+    using T          = typename Element<D>::type;
+    const T* entries = reinterpret_cast<const T*>(table) + piece * l.piece * d.table_stride;
+    p.first_entry = (int)(piece * l.piece), p.in_piece = (int)std::min(l.piece, d.num_entries - piece * l.piece);
+    p.first_stripe = (int)(piece * l.stripes), p.add = piece > 0;
+    p.table = entries, p.table_stride = d.table_stride, p.held = d.num_channels;
+    p.d_table = d_table ? reinterpret_cast<T*>(d_table) + piece * l.piece * d.d_table_stride : nullptr;
+    if (!l.copies) return hipSuccess;
+    p.table = w + l.copy, p.table_stride = p.held = l.kp;
+    ProfScope scope(prof, "loss_copy", stream);
+    const int64_t pieces = (int64_t)p.in_piece * l.kp / 8;
+    copy_entries_kernel<<<(unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 16), 256, 0, stream>>>(reinterpret_cast<const unsigned short*>(entries), d.table_stride,
+                                                                                                       reinterpret_cast<unsigned short*>(w + l.copy), p.in_piece, d.num_channels, l.kp);
+    return hipGetLastError();
+}
 
 template <int D, int MODE>
-hipError_t launch_product(const char* name, ProductParams p, unsigned x, unsigned y, unsigned z, hipStream_t stream, Profiler* prof)
+hipError_t launch_product(const TripsTableLossDesc& d, ProductParams p, hipStream_t stream, Profiler* prof)
 {
-    if (x == 0 || y == 0) return hipSuccess;
-    p.tiles_x = x, p.tiles_y = y;
-    ProfScope scope(prof, name, stream);
-    product_kernel<D, MODE><<<x * y * z, 256, 0, stream>>>(p);
-    return hipGetLastError();
+    static constexpr const char* NAMES[] = {"loss_logits", "loss_probs", "loss_d_rows", "loss_d_table"};
+    const int64_t along_m = MODE == LOGITS || MODE == PROBS ? p.in_piece : d.num_channels, along_n = MODE == D_TABLE ? p.in_piece : d.num_rows;
+    ProfScope scope(prof, NAMES[MODE], stream);
+    auto launch = [&](auto kernel, int bm, int bn, int threads)
+    {
+        p.tiles_x = MODE == LOGITS ? (unsigned)p.stripes : tiles_of(along_m, bm), p.tiles_y = tiles_of(along_n, bn);
+        kernel<<<p.tiles_x * p.tiles_y * (MODE == D_ROWS ? p.splits : 1), threads, 0, stream>>>(p);
+        return hipGetLastError();
+    };
+    if (along_m == 0 || along_n == 0) return hipSuccess;
+    if constexpr (D == TRIPS_DTYPE_F32)
+        return launch(product_kernel<D, MODE>, kTile, kTile, 256);
+    else
+        return launch(product16_kernel<D, MODE, Big>, Big::BM, Big::BN, Big::WAVES * 64);
 }
 
 template <int D>
 hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* table, const void* target, float* loss, float* state, char* w, hipStream_t stream, Profiler* prof)
 {
-    const Layout l = layout_of(d, false);
+    const Layout l = layout_of(d, false, copies_of(d, table));
     if (hipError_t e = gather<D>(d, l, rows, target, false, nullptr, nullptr, w, stream, prof)) return e;
-    if (hipError_t e = launch_product<D, LOGITS>("loss_logits", product_params(d, l, table, w), l.stripes, tiles_of(d.num_rows), 1, stream, prof)) return e;
+    ProductParams p = product_params(d, l, w);
+    int64_t piece   = 0;
+    for (; piece * l.piece < d.num_entries; ++piece)
+    {
+        if (hipError_t e = take_piece<D>(d, l, piece, table, nullptr, w, p, stream, prof)) return e;
+        if (hipError_t e = launch_product<D, LOGITS>(d, p, stream, prof)) return e;
+    }
     JoinParams j{};
-    j.partial = (float2*)(w + l.partial), j.own_product = (float*)(w + l.own_product), j.place = (int*)(w + l.place), j.count = (int*)(w + l.count);
-    j.loss = loss, j.state = (float2*)state, j.scale = std::fabs(d.scale), j.scale_log2 = scale_log2(d), j.sums = (double*)(w + l.sums), j.ticket = (unsigned*)(w + l.count) + 1;
-    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.stripes = l.stripes, j.reduction = d.reduction;
+    j.partial = p.partial, j.own_product = p.own_product, j.place = (int*)(w + l.place), j.count = p.count;
+    j.loss = loss, j.state = (float2*)state, j.scale = std::fabs(d.scale), j.scale_log2 = p.scale_log2, j.sums = (double*)(w + l.sums), j.ticket = (unsigned*)(w + l.count) + 1;
+    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.stripes = (int)(piece * l.stripes), j.reduction = d.reduction;
     ProfScope scope(prof, "loss_join", stream);
     join_kernel<<<std::max(1u, (unsigned)((d.num_rows + 15) / 16)), 256, 0, stream>>>(j);
     return hipGetLastError();
@@ -688,20 +1145,17 @@ template <int D>
 hipError_t backward(const TripsTableLossDesc& d, const void* rows, const void* table, const void* target, const float* state, const float* d_loss, void* d_rows, void* d_table, char* w,
                     hipStream_t stream, Profiler* prof)
 {
-    const Layout l = layout_of(d, true);
+    const Layout l = layout_of(d, true, copies_of(d, table));
     if (hipError_t e = gather<D>(d, l, rows, target, true, d_loss, state, w, stream, prof)) return e;
-    ProductParams p = product_params(d, l, table, w);
-    p.d_table       = d_table;
-    for (int64_t piece = 0; piece < l.pieces; ++piece)
+    ProductParams p = product_params(d, l, w);
+    for (int64_t piece = 0; piece * l.piece < d.num_entries; ++piece)
     {
-        p.first_entry = piece * l.piece, p.add = piece > 0;
-        if (p.first_entry >= d.num_entries) break;
-        const unsigned row_tiles = tiles_of(d.num_rows), channel_tiles = tiles_of(d.num_channels), entry_tiles = (unsigned)(l.piece / kTile);
-        if (hipError_t e = launch_product<D, PROBS>("loss_probs", p, entry_tiles, row_tiles, 1, stream, prof)) return e;
+        if (hipError_t e = take_piece<D>(d, l, piece, table, d_table, w, p, stream, prof)) return e;
+        if (hipError_t e = launch_product<D, PROBS>(d, p, stream, prof)) return e;
         if (d_rows)
-            if (hipError_t e = launch_product<D, D_ROWS>("loss_d_rows", p, channel_tiles, row_tiles, l.splits, stream, prof)) return e;
+            if (hipError_t e = launch_product<D, D_ROWS>(d, p, stream, prof)) return e;
         if (d_table)
-            if (hipError_t e = launch_product<D, D_TABLE>("loss_d_table", p, channel_tiles, entry_tiles, 1, stream, prof)) return e;
+            if (hipError_t e = launch_product<D, D_TABLE>(d, p, stream, prof)) return e;
     }
     if (!d_rows || d.num_rows == 0) return hipSuccess;
     ProfScope scope(prof, "loss_rows_out", stream);
@@ -747,7 +1201,7 @@ int check_call(TripsCtx* ctx, const TripsTableLossDesc* d, bool backward, const 
     if (int e = check_pointer("table", table, size, d->num_entries > 0)) return e;
     if (int e = check_pointer("target", target, d->index_dtype == TRIPS_INDEX_I32 ? 4 : 8, d->num_rows > 0)) return e;
     if (!workspace || !aligned(workspace, 256)) return set_error(TRIPS_ERR_INVALID_ARG, "workspace must be a 256-byte aligned device pointer");
-    const size_t need = layout_of(*d, backward).bytes;
+    const size_t need = workspace_of(*d, backward);
     if (bytes < need) return set_error(TRIPS_ERR_WORKSPACE_SMALL, "workspace has %zu bytes, %zu needed", bytes, need);
     return TRIPS_OK;
 }
@@ -762,7 +1216,7 @@ int trips_table_loss_workspace_size(const TripsTableLossDesc* desc, int backward
 {
     if (!bytes) return set_error(TRIPS_ERR_INVALID_ARG, "bytes is NULL");
     if (int e = check_desc(desc)) return e;
-    *bytes = layout_of(*desc, backward != 0).bytes;
+    *bytes = workspace_of(*desc, backward != 0);
     return TRIPS_OK;
 }
 
