@@ -217,7 +217,8 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
 //   PROBS   the same again: d_ij, [rows][piece]
 //   D_ROWS  channels x rows, over the piece's entries
 //   D_TABLE channels x entries, over the rows
-enum { LOGITS, PROBS, D_ROWS, D_TABLE };
+//   GRADS   both of those
+enum { LOGITS, PROBS, D_ROWS, D_TABLE, GRADS };
 
 constexpr int kTile = 128, kStep = 16, kRow = kTile + 4;
 
@@ -234,6 +235,7 @@ struct ProductParams
     float* own_product;    // [rows_pad]
     void* probs;           // [rows_pad][piece], in the tensors' type
     float* slabs;          // D_ROWS: [splits][rows_pad][kp]
+    const void* d_rows;    // whether they are wanted
     void* d_table;
     long long table_stride, d_table_stride, rows_pad;
     int held;              // channels that a row of the table holds: those, or with zeros behind them to a multiple of 64
@@ -537,35 +539,43 @@ __device__ __forceinline__ void wait_and_meet()
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
 }
 
+// (of LDS; the loads under way stay so)
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 constexpr unsigned kBeyond = 0x80000000u;  // an offset beyond any buffer
 
+// Where a wavefront's loads of an operand's steps come from: each lane's offsets, the same for all tiles, and the operand's elements from the
+// next step on.
+template <int LOADS>
+struct Source
+{
+    unsigned offset[LOADS];
+    const char* base;
+    long long bytes, step;
+    __device__ __forceinline__ void at(const void* from, long long size) { base = reinterpret_cast<const char*>(from), bytes = size; }
+    __device__ __forceinline__ void next() { base += step, bytes -= step; }
+    __device__ __forceinline__ void load(int i, unsigned lds, int wave) const { load_to_lds(buffer_of(base, bytes), offset[i], lds + (wave * LOADS + i) * 1024); }
+    // of rows along k, of which `left` elements are left: zeros behind them
+    __device__ __forceinline__ void load(int i, unsigned lds, int wave, int k, int left) const
+    {
+        load_to_lds(buffer_of(base, bytes), k < left ? offset[i] : kBeyond, lds + (wave * LOADS + i) * 1024);
+    }
+};
+
 // An operand whose rows run along k: LDS rows of BK elements, their pieces of 16 bytes in an order that depends on the row, so that
-// eight lanes that read the same piece of eight rows meet eight different places of the 128 bytes that LDS gives a cycle.
+// 16 lanes that read the same piece of 16 rows meet 16 different places of the 256 bytes that the banks of LDS are wide.
 template <int ROWS, int BK, int LOADS>
 struct AlongK
 {
     static constexpr int PIECES = BK / 8;
-    unsigned offset[LOADS];
-    int k_of[LOADS];
-    const char* base;
-    long long bytes;
-    static __device__ __forceinline__ int turn(int row) { return PIECES == 8 ? row & 7 : (row >> 1) & 3; }
-    __device__ __forceinline__ void begin(const void* at, long long stride_bytes, long long size, int wave, int lane)
+    static __device__ __forceinline__ int turn(int row) { return PIECES == 8 ? (row >> 1) & 7 : (row >> 2) & 3; }
+    static __device__ __forceinline__ int row_of(int i, int wave, int lane) { return (wave * LOADS + i) * (64 / PIECES) + lane / PIECES; }
+    static __device__ __forceinline__ int k_of(int i, int wave, int lane) { return ((lane % PIECES) ^ turn(row_of(i, wave, lane))) * 8; }
+    static __device__ __forceinline__ void begin(Source<LOADS>& s, long long stride_bytes, int wave, int lane)
     {
-        base = reinterpret_cast<const char*>(at), bytes = size;
+        s.step = BK * 2;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-        {
-            const int row   = (wave * LOADS + i) * (64 / PIECES) + lane / PIECES;
-            const int piece = (lane % PIECES) ^ turn(row);
-            offset[i] = (unsigned)(row * stride_bytes) + piece * 16, k_of[i] = piece * 8;
-        }
-    }
-    __device__ __forceinline__ void load(int k0, int k_end, unsigned lds, int wave) const
-    {
-        const Words4 buffer = buffer_of(base, bytes);
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) load_to_lds(buffer, k0 + k_of[i] < k_end ? offset[i] + 2 * k0 : kBeyond, lds + (wave * LOADS + i) * 1024);
+        for (int i = 0; i < LOADS; ++i) s.offset[i] = (unsigned)(row_of(i, wave, lane) * stride_bytes) + k_of(i, wave, lane) * 2;
     }
     // fragment f of the wavefront's rows from `row` on: 32 rows, 16 elements from 16 kk on, eight a lane
     static __device__ __forceinline__ Half8 read(const char* lds, int row, int f, int kk, int lane)
@@ -582,25 +592,16 @@ template <int ROWS, int BK, int LOADS>
 struct AcrossK
 {
     static constexpr int PIECES = ROWS / 8, TURNS = PIECES / 4;
-    unsigned offset[LOADS];
-    const char* base;
-    long long stride, bytes;
     static __device__ __forceinline__ int turn(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) & (TURNS - 1); }
-    __device__ __forceinline__ void begin(const void* at, long long stride_bytes, long long size, int wave, int lane)
+    static __device__ __forceinline__ void begin(Source<LOADS>& s, long long stride_bytes, int wave, int lane)
     {
-        base = reinterpret_cast<const char*>(at), stride = stride_bytes, bytes = size;
+        s.step = BK * stride_bytes;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
         {
-            const int k     = (wave * LOADS + i) * (64 / PIECES) + lane / PIECES, piece = lane % PIECES;
-            offset[i] = (unsigned)(k * stride_bytes) + ((((piece >> 2) ^ turn(k)) << 2) | (piece & 3)) * 16;
+            const int k = (wave * LOADS + i) * (64 / PIECES) + lane / PIECES, piece = lane % PIECES;
+            s.offset[i] = (unsigned)(k * stride_bytes) + ((((piece >> 2) ^ turn(k)) << 2) | (piece & 3)) * 16;
         }
-    }
-    __device__ __forceinline__ void load(int k0, int, unsigned lds, int wave) const
-    {
-        const Words4 buffer = buffer_of(base + k0 * stride, bytes - k0 * stride);
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) load_to_lds(buffer, offset[i], lds + (wave * LOADS + i) * 1024);
     }
     static __device__ __forceinline__ Half8 read(const char* lds, int row, int f, int kk, int lane)
     {
@@ -612,21 +613,6 @@ struct AcrossK
     }
 };
 
-template <bool ALONG, int ROWS, int BK, int LOADS>
-using Operand = std::conditional_t<ALONG, AlongK<ROWS, BK, LOADS>, AcrossK<ROWS, BK, LOADS>>;
-
-// Workgroups as they start go around the eight XCDs; here each XCD takes a run of tiles, in which eight of the second operand's share one
-// of the first's at a time.
-__device__ __forceinline__ void tile_of(unsigned id, unsigned all, unsigned across, unsigned down, unsigned& x, unsigned& y, unsigned& z)
-{
-    const unsigned each = all >> 3;
-    if (id < each * 8) id = (id & 7) * each + (id >> 3);
-    z                  = id / (across * down);
-    id                 = id % (across * down);
-    const unsigned g = id / (across * 8), in = id % (across * 8), high = min(8u, down - g * 8);
-    x = in / high, y = g * 8 + in % high;
-}
-
 // f(fragment, element of it, row of a lane's first fragment) for each of a lane's elements of one column of fragments
 template <int FM, typename F>
 __device__ __forceinline__ void each_element(F f)
@@ -637,218 +623,286 @@ __device__ __forceinline__ void each_element(F f)
         for (int e = 0; e < 16; ++e) f(i, e, i * 32 + 8 * (e >> 2) + (e & 3));
 }
 
-template <int D, int MODE, typename S>
+// A workgroup's share of a launch: its tiles, one after the other.
+struct Unit
+{
+    int mode;  // of the tile, -1: there is no further one
+    int x, y, z, steps;
+};
+
+// Eight tiles along y share one along x at a time: consecutive tiles go to one XCD, whose L2 holds what they share.
+__device__ __forceinline__ void place(Unit& u, int id, int across, int down)
+{
+    u.z         = id / (across * down);
+    id          = id % (across * down);
+    const int g = id / (across * 8), in = id % (across * 8), high = min(8, down - g * 8);
+    u.x = in / high, u.y = g * 8 + in % high;
+}
+
+// The units of worker w of `all`: unit w, w + all, ... of the larger kind (a of them, size_a steps each), then those of the smaller kind: workers
+// that have one of the larger kind less take so many smaller ones first.
+struct Share
+{
+    int a, size_a, b, size_b;
+};
+__device__ __forceinline__ int share_of(const Share& s, int ordinal, int w, int all, bool& second)
+{
+    const int own = w < s.a ? (s.a - w + all - 1) / all : 0;
+    second        = ordinal >= own;
+    if (!second) return w + ordinal * all;
+    const int rest = s.a % all, early = rest == 0 ? 0 : all - rest, more = early && s.size_b > 0 ? s.size_a / s.size_b : 0;
+    int j = ordinal - own;
+    if (early && w >= rest)
+    {
+        if (j < more) return w - rest + j * early;
+        j -= more;
+    }
+    return early * more + (w >= rest ? w - rest : w + early) + j * all;
+}
+
+// LOGITS, PROBS, or GRADS: D_ROWS and D_TABLE in one launch. One workgroup a CU, which goes through its units; the loads run STAGES steps
+// ahead of the products and go on into the next unit, so that they are under way while a unit's results are written.
+template <int D, int KIND, typename S>
 __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const ProductParams p)
 {
     using E = Element<D>;
     using T = typename E::type;
-    constexpr bool FIRST_ALONG = MODE == LOGITS || MODE == PROBS, SECOND_ALONG = MODE != D_TABLE;
-    using First  = Operand<FIRST_ALONG, S::BM, S::BK, S::FIRST_LOADS>;
-    using Second = Operand<SECOND_ALONG, S::BN, S::BK, S::SECOND_LOADS>;
-    constexpr int LOADS = S::FIRST_LOADS + S::SECOND_LOADS;
+    using FirstAlong   = AlongK<S::BM, S::BK, S::FIRST_LOADS>;
+    using FirstAcross  = AcrossK<S::BM, S::BK, S::FIRST_LOADS>;
+    using SecondAlong  = AlongK<S::BN, S::BK, S::SECOND_LOADS>;
+    using SecondAcross = AcrossK<S::BN, S::BK, S::SECOND_LOADS>;
+    constexpr int LOADS = S::FIRST_LOADS + S::SECOND_LOADS, ROUNDS = S::BK / 16;
+    static_assert(ROUNDS % 2 == 0 && S::STAGES >= 2, "two sets of fragments");
     __shared__ __attribute__((aligned(1024))) char lds[S::STAGES * S::STAGE_BYTES];
+    __shared__ float2 joined[KIND == LOGITS ? S::WM * S::BN : 1];
     const unsigned lds_at = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % S::WM * S::TM, wn = wave / S::WM * S::TN;
     const int count = *p.count;
 
-    unsigned block_x, block_y, block_z;
-    tile_of(blockIdx.x, gridDim.x, p.tiles_x, p.tiles_y, block_x, block_y, block_z);
-    const long long n0 = (long long)block_y * S::BN;
-    if ((MODE == D_TABLE ? (long long)p.in_piece : (long long)count) <= n0) return;
-    int k_begin = 0, k_end = MODE == D_TABLE ? count : p.held;
-    if (MODE == D_ROWS)
+    // workgroups as they start go around the eight XCDs: workers by XCD
+    const int all = gridDim.x, worker = all % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (all / 8) + blockIdx.x / 8);
+    const int row_tiles = (count + S::BN - 1) / S::BN, entry_tiles = (p.in_piece + (KIND == GRADS ? S::BN : S::BM) - 1) / (KIND == GRADS ? S::BN : S::BM);
+    const int channel_tiles = (p.channels + S::BM - 1) / S::BM;
+    const int piece_steps   = (p.in_piece + S::BK - 1) / S::BK;
+    Share share{};
+    bool rows_first = true;
+    if constexpr (KIND == GRADS)
     {
-        const int steps = (p.in_piece + S::BK - 1) / S::BK, each = (steps + p.splits - 1) / p.splits;
-        k_begin = min(p.in_piece, (int)block_z * each * S::BK), k_end = min(p.in_piece, k_begin + each * S::BK);
+        const int rows = p.d_rows ? channel_tiles * row_tiles * p.splits : 0, table = p.d_table ? channel_tiles * entry_tiles : 0;
+        const int rows_size = piece_steps / p.splits, table_size = (count + S::BK - 1) / S::BK;
+        rows_first = rows_size >= table_size;
+        share      = rows_first ? Share{rows, rows_size, table, table_size} : Share{table, table_size, rows, rows_size};
     }
-    const int steps = (k_end - k_begin + S::BK - 1) / S::BK;
+    else
+        share = Share{entry_tiles * row_tiles, 1, 0, 1};
+    auto unit_of = [&](int ordinal)
+    {
+        Unit u{};
+        bool second;
+        const int id = share_of(share, ordinal, worker, all, second);
+        if (id >= (second ? share.b : share.a))
+        {
+            u.mode = -1;
+            return u;
+        }
+        if constexpr (KIND == GRADS)
+        {
+            u.mode = second == rows_first ? D_TABLE : D_ROWS;
+            if (u.mode == D_ROWS)
+            {
+                place(u, id, channel_tiles, row_tiles);
+                u.steps = (int)((long long)(u.z + 1) * piece_steps / p.splits) - (int)((long long)u.z * piece_steps / p.splits);
+            }
+            else
+            {
+                place(u, id, channel_tiles, entry_tiles);
+                u.steps = (count + S::BK - 1) / S::BK;
+            }
+        }
+        else
+        {
+            u.mode = KIND, u.steps = (p.held + S::BK - 1) / S::BK;
+            place(u, id, entry_tiles, row_tiles);
+        }
+        return u;
+    };
 
-    First first;
-    Second second;
+    // ---- the loads, ahead ----
+    const char* table  = reinterpret_cast<const char*>(p.table);
     const char* packed = reinterpret_cast<const char*>(p.packed);
     const char* probs  = reinterpret_cast<const char*>(p.probs);
-    if constexpr (MODE == LOGITS || MODE == PROBS)
-        second.begin(packed + n0 * p.kp * 2, p.kp * 2, (count - n0) * p.kp * 2, wave, lane);
-    else if constexpr (MODE == D_ROWS)
-        second.begin(probs + n0 * p.piece * 2, (long long)p.piece * 2, (p.rows_pad - n0) * p.piece * 2, wave, lane);
-    else
-        second.begin(probs + n0 * 2, (long long)p.piece * 2, ((long long)count * p.piece - n0) * 2, wave, lane);
-
-    float2 best[S::FN];
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) best[j] = make_float2(-__builtin_inff(), 0.f);
-
-    const int tiles = MODE == LOGITS ? (p.in_piece + S::BM - 1) / S::BM : 0;
-    for (int tile = block_x; tile < (MODE == LOGITS ? tiles : (int)block_x + 1); tile += MODE == LOGITS ? p.stripes : 1)
+    Source<S::FIRST_LOADS> first;
+    Source<S::SECOND_LOADS> second;
+    int ahead_ordinal = 0, ahead_mode = -1, ahead_steps = 0, left = 0;
+    auto open = [&]()
     {
-        const int m0 = tile * S::BM;
-        if constexpr (FIRST_ALONG)
-            first.begin(reinterpret_cast<const T*>(p.table) + m0 * p.table_stride, p.table_stride * 2, ((long long)(min(p.in_piece - m0, S::BM) - 1) * p.table_stride + p.held) * 2, wave, lane);
-        else if constexpr (MODE == D_ROWS)
-            first.begin(reinterpret_cast<const T*>(p.table) + m0, p.table_stride * 2, ((p.in_piece - 1ll) * p.table_stride + p.held - m0) * 2, wave, lane);
+        Unit u = unit_of(ahead_ordinal);
+        while (u.mode >= 0 && u.steps == 0) u = unit_of(++ahead_ordinal);
+        ahead_steps = u.mode < 0 ? 0x7fffffff : u.steps;
+        if (u.mode < 0)
+        {
+            first.at(table, 0), second.at(table, 0);  // (zeros, so that the waits count alike)
+            first.step = second.step = 0;
+            return;
+        }
+        const long long stride = p.table_stride * 2, wide = (long long)p.kp * 2, piece = (long long)p.piece * 2;
+        if constexpr (KIND != GRADS)
+        {
+            if (ahead_mode != u.mode) FirstAlong::begin(first, stride, wave, lane), SecondAlong::begin(second, wide, wave, lane);
+            const long long m0 = (long long)u.x * S::BM, n0 = (long long)u.y * S::BN;
+            first.at(table + m0 * stride, (min(p.in_piece - m0, (long long)S::BM) - 1) * stride + p.held * 2);
+            second.at(packed + n0 * wide, (count - n0) * wide);
+            left = p.held;
+        }
+        else if (u.mode == D_ROWS)
+        {
+            if (ahead_mode != u.mode) FirstAcross::begin(first, stride, wave, lane), SecondAlong::begin(second, piece, wave, lane);
+            const long long k = (long long)u.z * piece_steps / p.splits * S::BK, m0 = (long long)u.x * S::BM * 2, n0 = (long long)u.y * S::BN;
+            first.at(table + k * stride + m0, (p.in_piece - 1 - k) * stride + p.held * 2 - m0);
+            second.at(probs + n0 * piece + k * 2, (p.rows_pad - n0) * piece - k * 2);
+        }
         else
-            first.begin(packed + m0 * 2, p.kp * 2, ((long long)count * p.kp - m0) * 2, wave, lane);
+        {
+            if (ahead_mode != u.mode) FirstAcross::begin(first, wide, wave, lane), SecondAcross::begin(second, piece, wave, lane);
+            const long long m0 = (long long)u.x * S::BM * 2, n0 = (long long)u.y * S::BN * 2;
+            first.at(packed + m0, count * wide - m0);
+            second.at(probs + n0, count * piece - n0);
+        }
+        ahead_mode = u.mode;
+    };
+    auto load = [&](int i, int stage)
+    {
+        const unsigned to = lds_at + stage * S::STAGE_BYTES;
+        if (i < S::FIRST_LOADS)
+        {
+            if (KIND != GRADS)
+                first.load(i, to, wave, FirstAlong::k_of(i, wave, lane), left);
+            else
+                first.load(i, to, wave);
+        }
+        else
+            second.load(i - S::FIRST_LOADS, to + S::FIRST_BYTES, wave);
+    };
+    auto loaded_step = [&]()
+    {
+        first.next(), second.next();
+        left -= S::BK;
+        if (--ahead_steps == 0) ++ahead_ordinal, open();
+    };
+    open();
+#pragma unroll
+    for (int s = 0; s < S::STAGES; ++s)
+    {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load(i, s);
+        loaded_step();
+    }
+    wait_and_meet<(S::STAGES - 1) * LOADS>();
+    int stage = 0;
 
-        Acc acc[S::FM][S::FN];
+    // ---- a unit's products ----
+    Acc acc[S::FM][S::FN];
+    auto products = [&](auto along, int steps)
+    {
+        using First  = std::conditional_t<KIND == GRADS, FirstAcross, FirstAlong>;
+        using Second = std::conditional_t<decltype(along)::value, SecondAlong, SecondAcross>;
 #pragma unroll
         for (int i = 0; i < S::FM; ++i)
 #pragma unroll
             for (int j = 0; j < S::FN; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-
-        auto issue = [&](int step, int stage)
+        // Fragments are read a round of the matrix instructions ahead of their use, those of the next step's first round behind the one
+        // meeting of a step, which says that every wavefront has read what the next loads replace, and that the next step is there. The
+        // loads go out between the last round's instructions.
+        Half8 x[2][S::FM], y[2][S::FN];
+        auto read = [&](int set, int from, int kk)
         {
-            const int k0 = k_begin + step * S::BK;
-            first.load(k0, k_end, lds_at + stage * S::STAGE_BYTES, wave);
-            second.load(k0, SECOND_ALONG && MODE != D_ROWS ? p.kp : k0 + S::BK, lds_at + stage * S::STAGE_BYTES + S::FIRST_BYTES, wave);
-        };
-        // (beyond the last step the loads go on, with nothing behind them, so that the waits count alike)
+            const char* a = lds + from * S::STAGE_BYTES;
 #pragma unroll
-        for (int s = 0; s < S::STAGES - 1; ++s) issue(s, s);
-        int stage = 0;
+            for (int i = 0; i < S::FM; ++i) x[set][i] = First::read(a, wm, i, kk, lane);
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) y[set][j] = Second::read(a + S::FIRST_BYTES, wn, j, kk, lane);
+        };
+        if (steps > 0) read(0, stage, 0);
         for (int step = 0; step < steps; ++step)
         {
-            wait_and_meet<(S::STAGES - 2) * LOADS>();
-            const int next = stage == 0 ? S::STAGES - 1 : stage - 1;
-            issue(step + S::STAGES - 1, next);
-            const char* a = lds + stage * S::STAGE_BYTES;
-            const char* b = a + S::FIRST_BYTES;
+            const int next = stage + 1 == S::STAGES ? 0 : stage + 1;
 #pragma unroll
-            for (int kk = 0; kk < S::BK / 16; ++kk)
+            for (int kk = 0; kk < ROUNDS; ++kk)
             {
-                Half8 x[S::FM], y[S::FN];
-#pragma unroll
-                for (int i = 0; i < S::FM; ++i) x[i] = First::read(a, wm, i, kk, lane);
-#pragma unroll
-                for (int j = 0; j < S::FN; ++j) y[j] = Second::read(b, wn, j, kk, lane);
+                if (kk + 1 < ROUNDS)
+                    read((kk + 1) & 1, stage, kk + 1);
+                else
+                {
+                    wait_and_meet<(S::STAGES - 2) * LOADS>();
+                    read(0, next, 0);  // (behind the last step: of the next unit, which reads it again)
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                int loaded = 0;
 #pragma unroll
                 for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-                    for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma16<D>(x[i], y[j], acc[i][j]);
+                    for (int j = 0; j < S::FN; ++j)
+                    {
+                        acc[i][j] = mfma16<D>(x[kk & 1][i], y[kk & 1][j], acc[i][j]);
+                        if (kk + 1 == ROUNDS)
+                        {
+                            constexpr int PAIRS = S::FM * S::FN, EACH = (LOADS + PAIRS - 1) / PAIRS;
+#pragma unroll
+                            for (int q = 0; q < EACH; ++q)
+                                if (loaded < LOADS) load(loaded++, stage);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+            loaded_step();
+            stage = next;
         }
-        wait_and_meet<0>();  // (nothing is on its way to LDS behind this)
+    };
 
-        // a lane's elements: of row n0 + wn + 32 j + lane % 32, of the first operand's rows m0 + wm + 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4
+    // ---- a unit's results ----
+    // a lane's elements: of row n0 + wn + 32 j + lane % 32, of the first operand's rows m0 + wm + 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4
+    auto sums = [&](const Unit& u)
+    {
+        const long long n0 = (long long)u.y * S::BN;
+        const int m0 = u.x * S::BM, m_lane = m0 + wm + 4 * (lane >> 5);
+        float2 best[S::FN];
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
         {
             const long long n = n0 + wn + j * 32 + (lane & 31);
-            const int m_lane  = m0 + wm + 4 * (lane >> 5);
-            if constexpr (MODE == LOGITS)
+            const int own     = n < count ? p.packed_target[n] - p.first_entry - m_lane : -1;  // (of the lane's own elements)
+            float top         = -__builtin_inff();
+            if (m0 + S::BM > p.in_piece)
+                each_element<S::FM>([&](int i, int e, int m)
+                {
+                    if (m_lane + m >= p.in_piece) acc[i][j][e] = -__builtin_inff();
+                });
+            if (__any(own >= 0 && own < S::TM))
             {
-                const int own = n < count ? p.packed_target[n] - p.first_entry - m_lane : -1;  // (of the lane's own elements)
-                float top     = -__builtin_inff();
-                if (m0 + S::BM > p.in_piece)
-                    each_element<S::FM>([&](int i, int e, int m)
-                    {
-                        if (m_lane + m >= p.in_piece) acc[i][j][e] = -__builtin_inff();
-                    });
-                if (__any(own >= 0 && own < S::TM))
+                float product = 0.f;
+                bool here     = false;
+                each_element<S::FM>([&](int i, int e, int m)
                 {
-                    float product = 0.f;
-                    bool here     = false;
-                    each_element<S::FM>([&](int i, int e, int m)
-                    {
-                        if (m == own) product = acc[i][j][e], here = m_lane + m < p.in_piece;
-                    });
-                    if (here) p.own_product[n] = product;
-                }
-                each_element<S::FM>([&](int i, int e, int) { top = fmaxf(top, acc[i][j][e]); });
-                top              = fmaxf(top, __shfl_xor(top, 32));
-                const float now  = fmaxf(best[j].x, top);
-                const float base = now == -__builtin_inff() ? 0.f : now;
-                float sum        = 0.f;
-                each_element<S::FM>([&](int i, int e, int) { sum += part_of(acc[i][j][e], base, p.scale_log2); });
-                sum += __shfl_xor(sum, 32);
-                best[j] = make_float2(now, best[j].y * part_of(best[j].x, base, p.scale_log2) + sum);
+                    if (m == own) product = acc[i][j][e], here = m_lane + m < p.in_piece;
+                });
+                if (here) p.own_product[n] = product;
             }
-            else
-            {
-                float2 state = make_float2(0.f, 0.f);
-                float factor = MODE == D_TABLE ? p.unscale[1] : 1.f;
-                int own      = -1;
-                if (MODE == PROBS && n < count) state = p.packed_state[n], factor = p.packed_factor[n], own = p.packed_target[n] - p.first_entry - m_lane;
-                if constexpr (MODE == PROBS)
-                {
-                    each_element<S::FM>([&](int i, int e, int)
-                                        { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - state.x, p.scale_log2, -state.y)) * factor; });
-                    if (__any(own >= 0 && own < S::TM))
-                        each_element<S::FM>([&](int i, int e, int m)
-                        {
-                            if (m == own) acc[i][j][e] -= factor;
-                        });
-                    if (m0 + S::BM > p.in_piece)
-                        each_element<S::FM>([&](int i, int e, int m)
-                        {
-                            if (m_lane + m >= p.in_piece) acc[i][j][e] = 0.f;
-                        });
-                }
-#pragma unroll
-                for (int i = 0; i < S::FM; ++i)
-                {
-                    if constexpr (MODE == D_ROWS)
-                    {
-#pragma unroll
-                        for (int g = 0; g < 4; ++g)
-                        {
-                            const int c = m_lane + i * 32 + 8 * g;
-                            using F4    = Pack<float, 4>::type;
-                            if (n < count && c < p.kp)
-                            {
-                                F4* at = reinterpret_cast<F4*>(p.slabs + ((long long)block_z * p.rows_pad + n) * p.kp + c);
-                                F4 v   = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                                if (p.add) v += *at;
-                                *at = v;
-                            }
-                        }
-                    }
-                    else
-                    {
-                        // two lanes' fours to eight of one lane: 16 bytes
-#pragma unroll
-                        for (int g = 0; g < 4; g += 2)
-                        {
-                            unsigned w[4];
-#pragma unroll
-                            for (int h = 0; h < 4; ++h)
-                                w[h] = (unsigned)E::from_float(acc[i][j][4 * g + 2 * h] * (MODE == D_TABLE ? factor : 1.f)) |
-                                       (unsigned)E::from_float(acc[i][j][4 * g + 2 * h + 1] * (MODE == D_TABLE ? factor : 1.f)) << 16;
-                            const auto low = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), high = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-                            const Words4 eight = {(int)low[0], (int)high[0], (int)low[1], (int)high[1]};
-                            const int m        = m0 + wm + i * 32 + 8 * (g + (lane >> 5));
-                            if constexpr (MODE == PROBS)
-                            {
-                                if (n < count) *reinterpret_cast<Words4*>(reinterpret_cast<T*>(p.probs) + n * p.piece + m) = eight;
-                            }
-                            else if (n < p.in_piece && m < p.channels)
-                            {
-                                T* at = reinterpret_cast<T*>(p.d_table) + n * p.d_table_stride + m;
-                                using T8 = typename Pack<T, 8>::type;
-                                const T8 v = __builtin_bit_cast(T8, eight);
-                                if (m + 8 <= p.channels)
-                                    *reinterpret_cast<T8*>(at) = v;
-                                else
-#pragma unroll
-                                    for (int e = 0; e < 8; ++e)
-                                        if (m + e < p.channels) at[e] = v[e];
-                            }
-                        }
-                    }
-                }
-            }
+            each_element<S::FM>([&](int i, int e, int) { top = fmaxf(top, acc[i][j][e]); });
+            top              = fmaxf(top, __shfl_xor(top, 32));
+            const float base = top == -__builtin_inff() ? 0.f : top;
+            float sum        = 0.f;
+            each_element<S::FM>([&](int i, int e, int) { sum += part_of(acc[i][j][e], base, p.scale_log2); });
+            best[j] = make_float2(top, sum + __shfl_xor(sum, 32));
         }
-    }
-    if constexpr (MODE == LOGITS)
-    {
-        float2* joined = reinterpret_cast<float2*>(lds);  // [WM][BN]
+        meet();  // (the last unit's have been read)
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
             if (lane < 32) joined[wave % S::WM * S::BN + wn + j * 32 + lane] = best[j];
-        __syncthreads();
+        meet();
         for (int n = threadIdx.x; n < S::BN; n += S::WAVES * 64)
         {
             float top = -__builtin_inff(), sum = 0.f;
@@ -857,9 +911,118 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
             const float base = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
             for (int w = 0; w < S::WM; ++w) sum += joined[w * S::BN + n].y * part_of(joined[w * S::BN + n].x, base, p.scale_log2);
-            p.partial[(p.first_stripe + block_x) * p.rows_pad + n0 + n] = make_float2(top, sum);
+            p.partial[(p.first_stripe + u.x) * p.rows_pad + n0 + n] = make_float2(top, sum);
+        }
+    };
+    auto written = [&](auto mode, const Unit& u)
+    {
+        constexpr int MODE = decltype(mode)::value;
+        const long long n0 = (long long)u.y * S::BN;
+        const int m0 = u.x * S::BM, m_lane = m0 + wm + 4 * (lane >> 5);
+        const float unscale = MODE == D_TABLE ? p.unscale[1] : 1.f;
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j)
+        {
+            const long long n = n0 + wn + j * 32 + (lane & 31);
+            if constexpr (MODE == PROBS)
+            {
+                float2 state = make_float2(0.f, 0.f);
+                float factor = 0.f;
+                int own      = -1;
+                if (n < count) state = p.packed_state[n], factor = p.packed_factor[n], own = p.packed_target[n] - p.first_entry - m_lane;
+                each_element<S::FM>([&](int i, int e, int)
+                                    { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - state.x, p.scale_log2, -state.y)) * factor; });
+                if (__any(own >= 0 && own < S::TM))
+                    each_element<S::FM>([&](int i, int e, int m)
+                    {
+                        if (m == own) acc[i][j][e] -= factor;
+                    });
+                if (m0 + S::BM > p.in_piece)
+                    each_element<S::FM>([&](int i, int e, int m)
+                    {
+                        if (m_lane + m >= p.in_piece) acc[i][j][e] = 0.f;
+                    });
+            }
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+            {
+                if constexpr (MODE == D_ROWS)
+                {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                    {
+                        const int c = m_lane + i * 32 + 8 * g;
+                        using F4    = Pack<float, 4>::type;
+                        if (n < count && c < p.kp)
+                        {
+                            F4* at = reinterpret_cast<F4*>(p.slabs + ((long long)u.z * p.rows_pad + n) * p.kp + c);
+                            F4 v   = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                            if (p.add) v += *at;
+                            *at = v;
+                        }
+                    }
+                }
+                else
+                {
+                    // two lanes' fours to eight of one lane: 16 bytes
+#pragma unroll
+                    for (int g = 0; g < 4; g += 2)
+                    {
+                        unsigned w[4];
+#pragma unroll
+                        for (int h = 0; h < 4; ++h)
+                            w[h] = (unsigned)E::from_float(acc[i][j][4 * g + 2 * h] * unscale) | (unsigned)E::from_float(acc[i][j][4 * g + 2 * h + 1] * unscale) << 16;
+                        const auto low = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), high = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+                        const Words4 eight = {(int)low[0], (int)high[0], (int)low[1], (int)high[1]};
+                        const int m        = m0 + wm + i * 32 + 8 * (g + (lane >> 5));
+                        if constexpr (MODE == PROBS)
+                        {
+                            if (n < count) *reinterpret_cast<Words4*>(reinterpret_cast<T*>(p.probs) + n * p.piece + m) = eight;
+                        }
+                        else if (n < p.in_piece && m < p.channels)
+                        {
+                            T* at      = reinterpret_cast<T*>(p.d_table) + n * p.d_table_stride + m;
+                            using T8   = typename Pack<T, 8>::type;
+                            const T8 v = __builtin_bit_cast(T8, eight);
+                            if (m + 8 <= p.channels)
+                                *reinterpret_cast<T8*>(at) = v;
+                            else
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    if (m + e < p.channels) at[e] = v[e];
+                        }
+                    }
+                }
+            }
+        }
+    };
+
+    for (int ordinal = 0;; ++ordinal)
+    {
+        const Unit u = unit_of(ordinal);
+        if (u.mode < 0) break;
+        if constexpr (KIND == LOGITS)
+        {
+            products(std::true_type{}, u.steps);
+            sums(u);
+        }
+        else if constexpr (KIND == PROBS)
+        {
+            products(std::true_type{}, u.steps);
+            written(std::integral_constant<int, PROBS>{}, u);
+        }
+        else if (u.mode == D_ROWS)
+        {
+            products(std::true_type{}, u.steps);
+            written(std::integral_constant<int, D_ROWS>{}, u);
+        }
+        else
+        {
+            products(std::false_type{}, u.steps);
+            written(std::integral_constant<int, D_TABLE>{}, u);
         }
     }
+    wait_and_meet<0>();  // (nothing is on its way to LDS when the workgroup ends)
 }
 
 // ---- joins ----
@@ -963,7 +1126,8 @@ __global__ __launch_bounds__(256) void rows_out_kernel(const float* slabs, const
 
 // ---- host ----
 
-constexpr int64_t kPieceBytes = 256ll << 20;  // of d_ij
+constexpr int64_t kPieceBytes = 1ll << 30;  // of d_ij
+constexpr int kCus            = 256;
 constexpr int64_t kCopyBytes = 64ll << 20, kLeastCopyBytes = 16ll << 20;  // of copied entries
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -981,9 +1145,40 @@ struct Layout
     size_t packed, place, target, state, factor, count, chunk_count, chunk_top, partial, own_product, sums, probs, slabs, copy, bytes;
 };
 
-struct Big : Shape<256, 256, 2, 4, 64, 2>
+#ifndef BIG
+#define BIG 256, 256, 2, 4, 64, 2
+#endif
+struct Big : Shape<BIG>
 {
 };
+
+// Into how many parts the rows' gradients are cut along the entries, so that they and the table's gradients (units of `steps` and
+// `table_steps`) keep all CUs busy to the end. A part costs its sums' way to memory and back, about 16 steps' time.
+int splits_of(int64_t units, int64_t steps, int64_t table_units, int64_t table_steps)
+{
+    int best      = 1;
+    int64_t least = INT64_MAX;
+    for (int s = 1; s <= 16 && (s == 1 || steps / s >= 16); ++s)
+    {
+        // the larger units first, each to the first CU that is free
+        int64_t a = units * s, size_a = (steps + s - 1) / s + 16, b = table_units, size_b = table_steps + 8;
+        if (size_a < size_b) std::swap(a, b), std::swap(size_a, size_b);
+        const int64_t rest = a % kCus, full = a / kCus * size_a;
+        int64_t end = full + (rest ? size_a : 0);
+        for (int64_t k = 0;; ++k)
+        {
+            const int64_t t = full + k * size_b, by_late = t - full - size_a;
+            const int64_t done = (kCus - rest) * k + (rest && by_late > 0 ? rest * (by_late / size_b) : 0);
+            if (done >= b)
+            {
+                end = std::max(end, t);
+                break;
+            }
+        }
+        if (end < least) best = s, least = end;
+    }
+    return best;
+}
 
 // copies: the table's entries are copied, a piece at a time, before the products read them.
 Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
@@ -1017,8 +1212,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     const int64_t row_tiles = up(d.num_rows, tile) / tile;
     if (!backward)
     {
-        const int64_t tiles = up(l.piece, tile) / tile;
-        l.stripes     = (int)std::max<int64_t>(1, std::min(tiles, 4096 / std::max<int64_t>(row_tiles, 1)));
+        l.stripes     = (int)(up(l.piece, tile) / tile);
         l.partial     = take((size_t)l.stripes * l.pieces * l.rows_pad * sizeof(float2));
         l.own_product = take(l.rows_pad * 4);
         l.sums        = take((d.num_rows / 16 + 1) * 8);
@@ -1027,8 +1221,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     {
         l.state = take(d.num_rows * 8), l.factor = take(d.num_rows * 4);
         l.probs = take((size_t)l.rows_pad * l.piece * size);
-        const int64_t out_tiles = std::max<int64_t>(1, row_tiles * (up(d.num_channels, tile) / tile));
-        l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({1024 / out_tiles, l.piece / 256, 64}));
+        l.splits = splits_of(row_tiles * (up(d.num_channels, tile) / tile), up(l.piece, 64) / 64, up(l.piece, tile) / tile * (up(d.num_channels, tile) / tile), up(d.num_rows, 64) / 64);
         l.slabs  = take((size_t)l.splits * l.rows_pad * l.kp * 4);
     }
     l.bytes = at;
@@ -1104,20 +1297,23 @@ hipError_t take_piece(const TripsTableLossDesc& d, const Layout& l, int64_t piec
 template <int D, int MODE>
 hipError_t launch_product(const TripsTableLossDesc& d, ProductParams p, hipStream_t stream, Profiler* prof)
 {
-    static constexpr const char* NAMES[] = {"loss_logits", "loss_probs", "loss_d_rows", "loss_d_table"};
-    const int64_t along_m = MODE == LOGITS || MODE == PROBS ? p.in_piece : d.num_channels, along_n = MODE == D_TABLE ? p.in_piece : d.num_rows;
+    static constexpr const char* NAMES[] = {"loss_logits", "loss_probs", "loss_d_rows", "loss_d_table", "loss_grads"};
+    if (p.in_piece == 0 || (d.num_rows == 0 && MODE != D_TABLE && MODE != GRADS)) return hipSuccess;
     ProfScope scope(prof, NAMES[MODE], stream);
-    auto launch = [&](auto kernel, int bm, int bn, int threads)
-    {
-        p.tiles_x = MODE == LOGITS ? (unsigned)p.stripes : tiles_of(along_m, bm), p.tiles_y = tiles_of(along_n, bn);
-        kernel<<<p.tiles_x * p.tiles_y * (MODE == D_ROWS ? p.splits : 1), threads, 0, stream>>>(p);
-        return hipGetLastError();
-    };
-    if (along_m == 0 || along_n == 0) return hipSuccess;
     if constexpr (D == TRIPS_DTYPE_F32)
-        return launch(product_kernel<D, MODE>, kTile, kTile, 256);
+    {
+        const int64_t along_m = MODE == LOGITS || MODE == PROBS ? p.in_piece : d.num_channels, along_n = MODE == D_TABLE ? p.in_piece : d.num_rows;
+        p.tiles_x = tiles_of(along_m, kTile), p.tiles_y = tiles_of(along_n, kTile);
+        product_kernel<D, MODE><<<p.tiles_x * p.tiles_y * (MODE == D_ROWS ? p.splits : 1), 256, 0, stream>>>(p);
+    }
     else
-        return launch(product16_kernel<D, MODE, Big>, Big::BM, Big::BN, Big::WAVES * 64);
+    {
+        const int64_t row_tiles = tiles_of(d.num_rows, Big::BN), channel_tiles = tiles_of(d.num_channels, Big::BM);
+        const int64_t units = MODE == GRADS ? channel_tiles * ((p.d_rows ? row_tiles * p.splits : 0) + (p.d_table ? tiles_of(p.in_piece, Big::BN) : 0)) : tiles_of(p.in_piece, Big::BM) * row_tiles;
+        if (units == 0) return hipSuccess;
+        product16_kernel<D, MODE, Big><<<(unsigned)std::min<int64_t>(units, kCus), Big::WAVES * 64, 0, stream>>>(p);
+    }
+    return hipGetLastError();
 }
 
 template <int D>
@@ -1135,7 +1331,7 @@ hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* ta
     JoinParams j{};
     j.partial = p.partial, j.own_product = p.own_product, j.place = (int*)(w + l.place), j.count = p.count;
     j.loss = loss, j.state = (float2*)state, j.scale = std::fabs(d.scale), j.scale_log2 = p.scale_log2, j.sums = (double*)(w + l.sums), j.ticket = (unsigned*)(w + l.count) + 1;
-    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.stripes = (int)(piece * l.stripes), j.reduction = d.reduction;
+    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.stripes = (int)tiles_of(d.num_entries, D == TRIPS_DTYPE_F32 ? kTile : Big::BM), j.reduction = d.reduction;
     ProfScope scope(prof, "loss_join", stream);
     join_kernel<<<std::max(1u, (unsigned)((d.num_rows + 15) / 16)), 256, 0, stream>>>(j);
     return hipGetLastError();
@@ -1148,14 +1344,22 @@ hipError_t backward(const TripsTableLossDesc& d, const void* rows, const void* t
     const Layout l = layout_of(d, true, copies_of(d, table));
     if (hipError_t e = gather<D>(d, l, rows, target, true, d_loss, state, w, stream, prof)) return e;
     ProductParams p = product_params(d, l, w);
+    p.d_rows        = d_rows;
     for (int64_t piece = 0; piece * l.piece < d.num_entries; ++piece)
     {
         if (hipError_t e = take_piece<D>(d, l, piece, table, d_table, w, p, stream, prof)) return e;
         if (hipError_t e = launch_product<D, PROBS>(d, p, stream, prof)) return e;
-        if (d_rows)
-            if (hipError_t e = launch_product<D, D_ROWS>(d, p, stream, prof)) return e;
-        if (d_table)
-            if (hipError_t e = launch_product<D, D_TABLE>(d, p, stream, prof)) return e;
+        if constexpr (D != TRIPS_DTYPE_F32)
+        {
+            if (hipError_t e = launch_product<D, GRADS>(d, p, stream, prof)) return e;
+        }
+        else
+        {
+            if (d_rows && d.num_rows > 0)
+                if (hipError_t e = launch_product<D, D_ROWS>(d, p, stream, prof)) return e;
+            if (d_table)
+                if (hipError_t e = launch_product<D, D_TABLE>(d, p, stream, prof)) return e;
+        }
     }
     if (!d_rows || d.num_rows == 0) return hipSuccess;
     ProfScope scope(prof, "loss_rows_out", stream);
