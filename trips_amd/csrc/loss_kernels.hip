@@ -47,7 +47,6 @@ struct GatherParams
     float* packed_factor;    // backward: what its gradients are multiplied by in d_ij
     int* count;              // [1]
     float* unscale;          // [2]: what undoes the scaling of d_ij, times scale and times |scale|
-    unsigned* ticket;        // cleared for the kernels behind
     long long n, entries, stride;
     int channels, kp, i32, reduction, backward;
     float scale;
@@ -135,13 +134,19 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
         for (long long i = own_chunk * kChunk + threadIdx.x; i < first; i += 256) before += counts<I32>(p.target, i, p.entries);
     }
     else
-        for (long long i = threadIdx.x; i < p.n; i += 256)
-            if (counts<I32>(p.target, i, p.entries))
+        // (eight targets of a thread on their way at a time)
+        for (long long i0 = threadIdx.x; i0 < p.n; i0 += 2048)
+        {
+            bool in[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) in[e] = counts<I32>(p.target, min(i0 + e * 256, p.n - 1), p.entries) && i0 + e * 256 < p.n;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
             {
-                ++all;
-                if (i < first) ++before;
-                if (tops) top = fmaxf(top, size_of(p.d_loss[i]));
+                all += in[e], before += in[e] && i0 + e * 256 < first;
+                if (tops && in[e]) top = fmaxf(top, size_of(p.d_loss[i0 + e * 256]));
             }
+        }
     before = wave_sum(before), all = wave_sum(all), top = wave_max(top);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     if (lane == 0) before_w[wave] = before, all_w[wave] = all, top_w[wave] = top;
@@ -177,8 +182,7 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
     }
     if (blockIdx.x == 0 && threadIdx.x == 0)
     {
-        *p.count  = all;
-        *p.ticket = 0u;
+        *p.count = all;
         if (p.backward)
         {
             const float one = D == TRIPS_DTYPE_F16 ? 1.f / 32768.f : 1.f;
@@ -220,8 +224,6 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
 //   GRADS   both of those
 enum { LOGITS, PROBS, D_ROWS, D_TABLE, GRADS };
 
-constexpr int kTile = 128, kStep = 16, kRow = kTile + 4;
-
 struct ProductParams
 {
     const void* table;     // the piece's entries
@@ -239,8 +241,7 @@ struct ProductParams
     void* d_table;
     long long table_stride, d_table_stride, rows_pad;
     int held;              // channels that a row of the table holds: those, or with zeros behind them to a multiple of 64
-    int first_entry, in_piece, channels, kp, piece, stripes, first_stripe, splits, add;
-    unsigned tiles_x, tiles_y;
+    int first_entry, in_piece, channels, kp, piece, first_stripe, splits, add;
     float scale_log2;
 };
 
@@ -249,261 +250,39 @@ typedef float Acc __attribute__((ext_vector_type(16)));
 // exp(scale (x - base)); 0 for an x of minus infinity.
 __device__ __forceinline__ float part_of(float x, float base, float scale_log2) { return __builtin_amdgcn_exp2f((x - base) * scale_log2); }
 
-template <int D, int MODE>
-__global__ __launch_bounds__(256) void product_kernel(const ProductParams p)
-{
-    using E = Element<D>;
-    using T = typename E::type;
-    __shared__ float first[2][kStep][kRow], second[2][kStep][kRow];
-    __shared__ float2 joined[2][kTile];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    const int count = *p.count;
-    constexpr bool FIRST_ALONG_K  = MODE == LOGITS || MODE == PROBS;
-    constexpr bool SECOND_ALONG_K = MODE != D_TABLE;
-
-    // the tile
-    const unsigned block_x = blockIdx.x % p.tiles_x, block_y = blockIdx.x / p.tiles_x % p.tiles_y, block_z = blockIdx.x / p.tiles_x / p.tiles_y;
-    const long long n0     = (long long)block_y * kTile;
-    const int in_piece     = p.in_piece;
-    float* probs           = reinterpret_cast<float*>(p.probs);
-    if ((MODE == D_TABLE ? (long long)in_piece : (long long)count) <= n0) return;
-    const int rows_up = (count + kStep - 1) / kStep * kStep;
-    int k_begin = 0, k_end = MODE == D_TABLE ? rows_up : p.kp;
-    if (MODE == D_ROWS)
-    {
-        const int steps = (in_piece + kStep - 1) / kStep, each = (steps + p.splits - 1) / p.splits;
-        k_begin = min(in_piece, (int)block_z * each * kStep), k_end = min(in_piece, k_begin + each * kStep);
-    }
-
-    float2 best[2];  // LOGITS: of the wave's rows (a lane: one of 32), in this stripe
-    best[0] = best[1] = make_float2(-__builtin_inff(), 0.f);
-    const int tiles = MODE == LOGITS ? (in_piece + kTile - 1) / kTile : 0;
-    for (int tile = block_x; tile < (MODE == LOGITS ? tiles : (int)block_x + 1); tile += MODE == LOGITS ? p.stripes : 1)
-    {
-        const int m0 = tile * kTile;
-        Acc acc[2][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-
-        // eight elements a thread of each operand: along k, or along the tile
-        float a[8], b[8];
-        auto fetch = [&](int k0)
-        {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) a[e] = b[e] = 0.f;
-            if constexpr (FIRST_ALONG_K)
-            {
-                const int j       = m0 + (threadIdx.x >> 1);
-                const int k       = k0 + (threadIdx.x & 1) * 8;
-                const T* at       = reinterpret_cast<const T*>(p.table) + j * p.table_stride + k;
-                if (j < in_piece)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (k + e < p.channels) a[e] = E::to_float(at[e]);
-            }
-            else
-            {
-                const int k = k0 + (threadIdx.x >> 4), c = m0 + (threadIdx.x & 15) * 8;
-                const T* at = MODE == D_ROWS ? reinterpret_cast<const T*>(p.table) + k * p.table_stride + c
-                                             : reinterpret_cast<const T*>(p.packed) + (long long)k * p.kp + c;
-                if (k < (MODE == D_ROWS ? in_piece : count))
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c + e < p.channels) a[e] = E::to_float(at[e]);
-            }
-            if constexpr (MODE == LOGITS || MODE == PROBS)
-            {
-                const long long r = n0 + (threadIdx.x >> 1);
-                const T* at       = reinterpret_cast<const T*>(p.packed) + r * p.kp + k0 + (threadIdx.x & 1) * 8;
-                if (r < count)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) b[e] = E::to_float(at[e]);
-            }
-            else if constexpr (MODE == D_ROWS)
-            {
-                const long long r = n0 + (threadIdx.x >> 1);
-                const int k       = k0 + (threadIdx.x & 1) * 8;
-                if (r < count)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (k + e < in_piece) b[e] = probs[r * p.piece + k + e];
-            }
-            else
-            {
-                const int k = k0 + (threadIdx.x >> 4);
-                if (k < count)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) b[e] = probs[(long long)k * p.piece + n0 + (threadIdx.x & 15) * 8 + e];
-            }
-        };
-        auto put = [&](int buffer)
-        {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-            {
-                if constexpr (FIRST_ALONG_K)
-                    first[buffer][(threadIdx.x & 1) * 8 + e][threadIdx.x >> 1] = a[e];
-                else
-                    first[buffer][threadIdx.x >> 4][(threadIdx.x & 15) * 8 + e] = a[e];
-                if constexpr (SECOND_ALONG_K)
-                    second[buffer][(threadIdx.x & 1) * 8 + e][threadIdx.x >> 1] = b[e];
-                else
-                    second[buffer][threadIdx.x >> 4][(threadIdx.x & 15) * 8 + e] = b[e];
-            }
-        };
-        int buffer = 0;
-        if (k_begin < k_end)
-        {
-            fetch(k_begin);
-            __syncthreads();
-            put(0);
-        }
-        for (int k0 = k_begin; k0 < k_end; k0 += kStep)
-        {
-            __syncthreads();
-            if (k0 + kStep < k_end) fetch(k0 + kStep);
-#pragma unroll
-            for (int k = 0; k < kStep; k += 2)
-            {
-                float x[2], y[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                {
-                    x[i] = first[buffer][k + (lane >> 5)][wm + i * 32 + (lane & 31)];
-                    y[i] = second[buffer][k + (lane >> 5)][wn + i * 32 + (lane & 31)];
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[j], acc[i][j], 0, 0, 0);
-            }
-            buffer ^= 1;
-            if (k0 + kStep < k_end) put(buffer);
-        }
-
-        // a lane's elements: of row n0 + wn + 32 j + lane % 32, of the first operand's rows m0 + wm + 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-        {
-            const long long n = n0 + wn + j * 32 + (lane & 31);
-            if constexpr (MODE == LOGITS)
-            {
-                const int own = n < count ? p.packed_target[n] - p.first_entry : -1;
-                float top     = -__builtin_inff();
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                    {
-                        const int m   = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                        const float l = m < in_piece ? acc[i][j][e] : -__builtin_inff();
-                        if (m == own && m < in_piece) p.own_product[n] = l;
-                        acc[i][j][e]  = l;
-                        top           = fmaxf(top, l);
-                    }
-                top              = fmaxf(top, __shfl_xor(top, 32));
-                const float now  = fmaxf(best[j].x, top);
-                const float base = now == -__builtin_inff() ? 0.f : now;
-                float sum        = 0.f;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) sum += part_of(acc[i][j][e], base, p.scale_log2);
-                sum += __shfl_xor(sum, 32);
-                best[j] = make_float2(now, best[j].y * part_of(best[j].x, base, p.scale_log2) + sum);
-            }
-            else if constexpr (MODE == PROBS)
-            {
-                const bool in   = n < count;
-                const int own   = in ? p.packed_target[n] - p.first_entry : -1;
-                const float2 state = in ? p.packed_state[n] : make_float2(0.f, 0.f);
-                const float factor = in ? p.packed_factor[n] : 0.f;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                    {
-                        const int m = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                        float q     = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - state.x, p.scale_log2, -state.y));
-                        if (m == own) q -= 1.f;
-                        if (in && m < p.piece) probs[n * p.piece + m] = m < in_piece ? q * factor : 0.f;
-                    }
-            }
-            else
-            {
-                const float unscale = MODE == D_TABLE ? p.unscale[1] : 1.f;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                    {
-                        const int c = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                        if constexpr (MODE == D_ROWS)
-                        {
-                            float* at = p.slabs + ((long long)block_z * p.rows_pad + n) * p.kp + c;
-                            if (n < count && c < p.channels) *at = p.add ? *at + acc[i][j][e] : acc[i][j][e];
-                        }
-                        else
-                        {
-                            if (n < in_piece && c < p.channels)
-                                reinterpret_cast<T*>(p.d_table)[n * p.d_table_stride + c] = E::from_float(acc[i][j][e] * unscale);
-                        }
-                    }
-            }
-        }
-    }
-    if constexpr (MODE == LOGITS)
-    {
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (lane < 32) joined[wave & 1][wn + j * 32 + lane] = best[j];
-        __syncthreads();
-        if (threadIdx.x < kTile)
-        {
-            const float2 a = joined[0][threadIdx.x], b = joined[1][threadIdx.x];
-            const float top = fmaxf(a.x, b.x), base = top == -__builtin_inff() ? 0.f : top;
-            p.partial[(p.first_stripe + block_x) * p.rows_pad + n0 + threadIdx.x] = make_float2(top, a.y * part_of(a.x, base, p.scale_log2) + b.y * part_of(b.x, base, p.scale_log2));
-        }
-    }
-}
-
 // Entries one behind the other in rows of kp elements, zeros from the channels on: for tables whose rows the direct loads cannot take.
-__global__ __launch_bounds__(256) void copy_entries_kernel(const unsigned short* table, long long stride, unsigned short* to, long long entries, int channels, int kp)
+template <typename T>
+__global__ __launch_bounds__(256) void copy_entries_kernel(const T* table, long long stride, T* to, long long entries, int channels, int kp)
 {
-    using Wide          = Pack<unsigned short, 8>::type;
+    using Wide          = typename Pack<T, 8>::type;
     const int pieces    = kp / 8;
     const long long all = entries * pieces;
     for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < all; q += (long long)gridDim.x * 256)
     {
-        const long long j          = q / pieces;
-        const int c                = (int)(q % pieces) * 8;
-        const unsigned short* from = table + j * stride + c;
+        const long long j = q / pieces;
+        const int c       = (int)(q % pieces) * 8;
+        const T* from     = table + j * stride + c;
         Wide x;
         if (c + 8 <= channels)
             x = *reinterpret_cast<const Wide*>(from);
         else
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = c + e < channels ? from[e] : (unsigned short)0;
+            for (int e = 0; e < 8; ++e) x[e] = c + e < channels ? from[e] : T(0);
         *reinterpret_cast<Wide*>(to + q * 8) = x;
     }
 }
 
-// ---- products of 16-bit types ----
+constexpr int kStepBytes = 128, kRounds = 4;  // of a row along k in a step; a round of the matrix instructions takes a quarter of them
 
-// Tiles of BM x BN in steps of BK along k, both operands by direct loads to LDS, STAGES steps of them at a time; WM x WN wavefronts.
-template <int BM_, int BN_, int WM_, int WN_, int BK_, int STAGES_>
+// Tiles of BM x BN in steps along k, both operands by direct loads to LDS, STAGES steps of them at a time; WM x WN wavefronts, PER_CU such workgroups.
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int PER_CU_>
 struct Shape
 {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, STAGES = STAGES_;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_, PER_CU = PER_CU_;
     static constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
-    static constexpr int FIRST_BYTES = BM * BK * 2, STAGE_BYTES = (BM + BN) * BK * 2;
-    static constexpr int FIRST_LOADS = FIRST_BYTES / 1024 / WAVES, SECOND_LOADS = BN * BK * 2 / 1024 / WAVES;
-    static_assert(FIRST_LOADS * WAVES * 1024 == FIRST_BYTES && SECOND_LOADS * WAVES * 1024 == BN * BK * 2, "whole loads of a wavefront");
+    static constexpr int FIRST_BYTES = BM * kStepBytes, SECOND_BYTES = BN * kStepBytes, STAGE_BYTES = FIRST_BYTES + SECOND_BYTES;
+    static constexpr int FIRST_LOADS = FIRST_BYTES / 1024 / WAVES, SECOND_LOADS = SECOND_BYTES / 1024 / WAVES;
+    static_assert(FIRST_LOADS * WAVES * 1024 == FIRST_BYTES && SECOND_LOADS * WAVES * 1024 == SECOND_BYTES, "whole loads of a wavefront");
 };
 
 typedef int Words4 __attribute__((ext_vector_type(4)));
@@ -511,14 +290,24 @@ typedef short Half4 __attribute__((ext_vector_type(4)));
 typedef short Half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 Bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 F8 __attribute__((ext_vector_type(8)));
+typedef float Float4 __attribute__((ext_vector_type(4)));
 
+// 16 bytes a lane of either operand: 32 rows, the lane's element of it and those that follow along k, 16 (of 16 bits) or 8 in two halves of the
+// wavefront. Which elements a half has does not matter, as long as it has the same ones of both operands.
 template <int D>
-__device__ __forceinline__ Acc mfma16(Half8 a, Half8 b, Acc c)
+__device__ __forceinline__ Acc product(Half8 a, Half8 b, Acc c)
 {
     if constexpr (D == TRIPS_DTYPE_BF16)
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf8, a), __builtin_bit_cast(Bf8, b), c, 0, 0, 0);
-    else
+    else if constexpr (D == TRIPS_DTYPE_F16)
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(F8, a), __builtin_bit_cast(F8, b), c, 0, 0, 0);
+    else
+    {
+        const Float4 x = __builtin_bit_cast(Float4, a), y = __builtin_bit_cast(Float4, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
+        return c;
+    }
 }
 
 // 64 lanes' 16 bytes from a buffer, each at its own offset, to LDS one behind the other; zeros from beyond the buffer's end.
@@ -562,54 +351,63 @@ struct Source
     }
 };
 
-// An operand whose rows run along k: LDS rows of BK elements, their pieces of 16 bytes in an order that depends on the row, so that
-// 16 lanes that read the same piece of 16 rows meet 16 different places of the 256 bytes that the banks of LDS are wide.
-template <int ROWS, int BK, int LOADS>
+// An operand whose rows run along k: LDS rows of 128 bytes, their pieces of 16 in an order that depends on the row, so that 16 lanes that
+// read the same piece of 16 rows meet 16 different places of the 256 bytes that the banks of LDS are wide.
+template <int ROWS, int LOADS>
 struct AlongK
 {
-    static constexpr int PIECES = BK / 8;
-    static __device__ __forceinline__ int turn(int row) { return PIECES == 8 ? (row >> 1) & 7 : (row >> 2) & 3; }
+    static constexpr int PIECES = kStepBytes / 16;
+    static __device__ __forceinline__ int turn(int row) { return (row >> 1) & 7; }
     static __device__ __forceinline__ int row_of(int i, int wave, int lane) { return (wave * LOADS + i) * (64 / PIECES) + lane / PIECES; }
-    static __device__ __forceinline__ int k_of(int i, int wave, int lane) { return ((lane % PIECES) ^ turn(row_of(i, wave, lane))) * 8; }
+    static __device__ __forceinline__ int piece_of(int i, int wave, int lane) { return (lane % PIECES) ^ turn(row_of(i, wave, lane)); }
     static __device__ __forceinline__ void begin(Source<LOADS>& s, long long stride_bytes, int wave, int lane)
     {
-        s.step = BK * 2;
+        s.step = kStepBytes;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) s.offset[i] = (unsigned)(row_of(i, wave, lane) * stride_bytes) + k_of(i, wave, lane) * 2;
+        for (int i = 0; i < LOADS; ++i) s.offset[i] = (unsigned)(row_of(i, wave, lane) * stride_bytes) + piece_of(i, wave, lane) * 16;
     }
-    // fragment f of the wavefront's rows from `row` on: 32 rows, 16 elements from 16 kk on, eight a lane
+    // fragment f of the wavefront's rows from `row` on, round kk
     static __device__ __forceinline__ Half8 read(const char* lds, int row, int f, int kk, int lane)
     {
         const int r = row + (lane & 31);
-        return *reinterpret_cast<const Half8*>(lds + (r + f * 32) * (BK * 2) + (((kk * 2 + (lane >> 5)) ^ turn(r)) * 16));
+        return *reinterpret_cast<const Half8*>(lds + (r + f * 32) * kStepBytes + (((kk * 2 + (lane >> 5)) ^ turn(r)) * 16));
     }
 };
 
-// An operand whose rows run along the tile: LDS rows of ROWS elements, one of each k, read through the transposing loads (of 16 lanes'
-// four elements: lane i gets element i % 4 of lanes i / 4, i / 4 + 4, ...). Their pieces of 64 bytes are in an order that depends on k, so that
-// the four rows of 16 lanes lie apart.
-template <int ROWS, int BK, int LOADS>
+// An operand whose rows run along the tile: LDS rows of ROWS elements, one of each k. Of 16 bits they are read through the transposing loads (of
+// 16 lanes' four elements: lane i gets element i % 4 of lanes i / 4, i / 4 + 4, ...). A row's pieces of 64 bytes (32 bits: 128) are in an order
+// that depends on k, so that the four (two) rows that are read at once lie apart.
+template <int SIZE, int ROWS, int LOADS>
 struct AcrossK
 {
-    static constexpr int PIECES = ROWS / 8, TURNS = PIECES / 4;
-    static __device__ __forceinline__ int turn(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) & (TURNS - 1); }
+    static constexpr int PIECES = ROWS * SIZE / 16, GROUP = SIZE == 2 ? 4 : 8, TURNS = PIECES / GROUP;
+    static __device__ __forceinline__ int turn(int k) { return (SIZE == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 1) & (TURNS - 1); }
     static __device__ __forceinline__ void begin(Source<LOADS>& s, long long stride_bytes, int wave, int lane)
     {
-        s.step = BK * stride_bytes;
+        s.step = kStepBytes / SIZE * stride_bytes;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
         {
-            const int k = (wave * LOADS + i) * (64 / PIECES) + lane / PIECES, piece = lane % PIECES;
-            s.offset[i] = (unsigned)(k * stride_bytes) + ((((piece >> 2) ^ turn(k)) << 2) | (piece & 3)) * 16;
+            const int at = (wave * LOADS + i) * 64 + lane, k = at / PIECES, piece = at % PIECES;
+            s.offset[i]  = (unsigned)(k * stride_bytes) + (((piece / GROUP) ^ turn(k)) * GROUP + piece % GROUP) * 16;
         }
     }
     static __device__ __forceinline__ Half8 read(const char* lds, int row, int f, int kk, int lane)
     {
-        const int k    = kk * 16 + (lane >> 5) * 8 + ((lane >> 2) & 3);
-        const char* at = lds + k * (ROWS * 2) + (((row >> 5) + f) ^ turn(k)) * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
-        using P        = __attribute__((address_space(3))) Half4*;
-        const Half4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 4 * ROWS * 2));
-        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        if constexpr (SIZE == 2)
+        {
+            const int k    = kk * 16 + (lane >> 5) * 8 + ((lane >> 2) & 3);
+            const char* at = lds + k * (ROWS * 2) + (((row >> 5) + f) ^ turn(k)) * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+            using P        = __attribute__((address_space(3))) Half4*;
+            const Half4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 4 * ROWS * 2));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        else
+        {
+            const int k     = kk * 8 + (lane >> 5) * 4;
+            const float* at = reinterpret_cast<const float*>(lds + k * (ROWS * 4) + (((row >> 5) + f) ^ turn(k)) * 128) + (lane & 31);
+            return __builtin_bit_cast(Half8, Float4{at[0], at[ROWS], at[2 * ROWS], at[3 * ROWS]});
+        }
     }
 };
 
@@ -660,19 +458,18 @@ __device__ __forceinline__ int share_of(const Share& s, int ordinal, int w, int 
     return early * more + (w >= rest ? w - rest : w + early) + j * all;
 }
 
-// LOGITS, PROBS, or GRADS: D_ROWS and D_TABLE in one launch. One workgroup a CU, which goes through its units; the loads run STAGES steps
+// LOGITS, PROBS, or GRADS: D_ROWS and D_TABLE in one launch. S::PER_CU workgroups a CU, each goes through its units; the loads run STAGES steps
 // ahead of the products and go on into the next unit, so that they are under way while a unit's results are written.
 template <int D, int KIND, typename S>
-__global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const ProductParams p)
+__global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void product_kernel(const ProductParams p)
 {
     using E = Element<D>;
     using T = typename E::type;
-    using FirstAlong   = AlongK<S::BM, S::BK, S::FIRST_LOADS>;
-    using FirstAcross  = AcrossK<S::BM, S::BK, S::FIRST_LOADS>;
-    using SecondAlong  = AlongK<S::BN, S::BK, S::SECOND_LOADS>;
-    using SecondAcross = AcrossK<S::BN, S::BK, S::SECOND_LOADS>;
-    constexpr int LOADS = S::FIRST_LOADS + S::SECOND_LOADS, ROUNDS = S::BK / 16;
-    static_assert(ROUNDS % 2 == 0 && S::STAGES >= 2, "two sets of fragments");
+        constexpr int SIZE = sizeof(T), BK = kStepBytes / SIZE, LOADS = S::FIRST_LOADS + S::SECOND_LOADS, LATE = LOADS / 2;
+    using FirstAlong   = AlongK<S::BM, S::FIRST_LOADS>;
+    using FirstAcross  = AcrossK<SIZE, S::BM, S::FIRST_LOADS>;
+    using SecondAlong  = AlongK<S::BN, S::SECOND_LOADS>;
+    using SecondAcross = AcrossK<SIZE, S::BN, S::SECOND_LOADS>;
     __shared__ __attribute__((aligned(1024))) char lds[S::STAGES * S::STAGE_BYTES];
     __shared__ float2 joined[KIND == LOGITS ? S::WM * S::BN : 1];
     const unsigned lds_at = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds);
@@ -684,13 +481,13 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
     const int all = gridDim.x, worker = all % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (all / 8) + blockIdx.x / 8);
     const int row_tiles = (count + S::BN - 1) / S::BN, entry_tiles = (p.in_piece + (KIND == GRADS ? S::BN : S::BM) - 1) / (KIND == GRADS ? S::BN : S::BM);
     const int channel_tiles = (p.channels + S::BM - 1) / S::BM;
-    const int piece_steps   = (p.in_piece + S::BK - 1) / S::BK;
+    const int piece_steps   = (p.in_piece + BK - 1) / BK;
     Share share{};
     bool rows_first = true;
     if constexpr (KIND == GRADS)
     {
         const int rows = p.d_rows ? channel_tiles * row_tiles * p.splits : 0, table = p.d_table ? channel_tiles * entry_tiles : 0;
-        const int rows_size = piece_steps / p.splits, table_size = (count + S::BK - 1) / S::BK;
+        const int rows_size = piece_steps / p.splits, table_size = (count + BK - 1) / BK;
         rows_first = rows_size >= table_size;
         share      = rows_first ? Share{rows, rows_size, table, table_size} : Share{table, table_size, rows, rows_size};
     }
@@ -717,12 +514,12 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
             else
             {
                 place(u, id, channel_tiles, entry_tiles);
-                u.steps = (count + S::BK - 1) / S::BK;
+                u.steps = (count + BK - 1) / BK;
             }
         }
         else
         {
-            u.mode = KIND, u.steps = (p.held + S::BK - 1) / S::BK;
+            u.mode = KIND, u.steps = (p.held + BK - 1) / BK;
             place(u, id, entry_tiles, row_tiles);
         }
         return u;
@@ -746,26 +543,26 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
             first.step = second.step = 0;
             return;
         }
-        const long long stride = p.table_stride * 2, wide = (long long)p.kp * 2, piece = (long long)p.piece * 2;
+        const long long stride = p.table_stride * SIZE, wide = (long long)p.kp * SIZE, piece = (long long)p.piece * SIZE, held = (long long)p.held * SIZE;
         if constexpr (KIND != GRADS)
         {
             if (ahead_mode != u.mode) FirstAlong::begin(first, stride, wave, lane), SecondAlong::begin(second, wide, wave, lane);
             const long long m0 = (long long)u.x * S::BM, n0 = (long long)u.y * S::BN;
-            first.at(table + m0 * stride, (min(p.in_piece - m0, (long long)S::BM) - 1) * stride + p.held * 2);
+            first.at(table + m0 * stride, (min(p.in_piece - m0, (long long)S::BM) - 1) * stride + held);
             second.at(packed + n0 * wide, (count - n0) * wide);
             left = p.held;
         }
         else if (u.mode == D_ROWS)
         {
             if (ahead_mode != u.mode) FirstAcross::begin(first, stride, wave, lane), SecondAlong::begin(second, piece, wave, lane);
-            const long long k = (long long)u.z * piece_steps / p.splits * S::BK, m0 = (long long)u.x * S::BM * 2, n0 = (long long)u.y * S::BN;
-            first.at(table + k * stride + m0, (p.in_piece - 1 - k) * stride + p.held * 2 - m0);
-            second.at(probs + n0 * piece + k * 2, (p.rows_pad - n0) * piece - k * 2);
+            const long long k = (long long)u.z * piece_steps / p.splits * BK, m0 = (long long)u.x * S::BM * SIZE, n0 = (long long)u.y * S::BN;
+            first.at(table + k * stride + m0, (p.in_piece - 1 - k) * stride + held - m0);
+            second.at(probs + n0 * piece + k * SIZE, (p.rows_pad - n0) * piece - k * SIZE);
         }
         else
         {
             if (ahead_mode != u.mode) FirstAcross::begin(first, wide, wave, lane), SecondAcross::begin(second, piece, wave, lane);
-            const long long m0 = (long long)u.x * S::BM * 2, n0 = (long long)u.y * S::BN * 2;
+            const long long m0 = (long long)u.x * S::BM * SIZE, n0 = (long long)u.y * S::BN * SIZE;
             first.at(packed + m0, count * wide - m0);
             second.at(probs + n0, count * piece - n0);
         }
@@ -777,7 +574,7 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
         if (i < S::FIRST_LOADS)
         {
             if (KIND != GRADS)
-                first.load(i, to, wave, FirstAlong::k_of(i, wave, lane), left);
+                first.load(i, to, wave, FirstAlong::piece_of(i, wave, lane) * (16 / SIZE), left);
             else
                 first.load(i, to, wave);
         }
@@ -787,7 +584,7 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
     auto loaded_step = [&]()
     {
         first.next(), second.next();
-        left -= S::BK;
+        left -= BK;
         if (--ahead_steps == 0) ++ahead_ordinal, open();
     };
     open();
@@ -795,10 +592,10 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
     for (int s = 0; s < S::STAGES; ++s)
     {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) load(i, s);
-        loaded_step();
+        for (int i = 0; i < (s + 1 < S::STAGES ? LOADS : LOADS - LATE); ++i) load(i, s);
+        if (s + 1 < S::STAGES || LATE == 0) loaded_step();
     }
-    wait_and_meet<(S::STAGES - 1) * LOADS>();
+    wait_and_meet<(S::STAGES - 1) * LOADS - LATE>();
     int stage = 0;
 
     // ---- a unit's products ----
@@ -828,11 +625,11 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
         if (steps > 0) read(0, stage, 0);
         for (int step = 0; step < steps; ++step)
         {
-            const int next = stage + 1 == S::STAGES ? 0 : stage + 1;
+            const int next = stage + 1 == S::STAGES ? 0 : stage + 1, free = stage == 0 ? S::STAGES - 1 : stage - 1;
 #pragma unroll
-            for (int kk = 0; kk < ROUNDS; ++kk)
+            for (int kk = 0; kk < kRounds; ++kk)
             {
-                if (kk + 1 < ROUNDS)
+                if (kk + 1 < kRounds)
                     read((kk + 1) & 1, stage, kk + 1);
                 else
                 {
@@ -840,25 +637,27 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
                     read(0, next, 0);  // (behind the last step: of the next unit, which reads it again)
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                int loaded = 0;
+                // of `of` loads from `from` on, the share behind product q of the round
+                auto loads = [&](int q, int from, int of, int to)
+                {
+                    constexpr int PAIRS = S::FM * S::FN;
+#pragma unroll
+                    for (int i = from + q * of / PAIRS; i < from + (q + 1) * of / PAIRS; ++i) load(i, to);
+                };
 #pragma unroll
                 for (int i = 0; i < S::FM; ++i)
 #pragma unroll
                     for (int j = 0; j < S::FN; ++j)
                     {
-                        acc[i][j] = mfma16<D>(x[kk & 1][i], y[kk & 1][j], acc[i][j]);
-                        if (kk + 1 == ROUNDS)
-                        {
-                            constexpr int PAIRS = S::FM * S::FN, EACH = (LOADS + PAIRS - 1) / PAIRS;
-#pragma unroll
-                            for (int q = 0; q < EACH; ++q)
-                                if (loaded < LOADS) load(loaded++, stage);
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
+                        acc[i][j] = product<D>(x[kk & 1][i], y[kk & 1][j], acc[i][j]);
+                        if (kk == 0 && LATE > 0) loads(i * S::FN + j, LOADS - LATE, LATE, free);
+                        if (kk + 1 == kRounds) loads(i * S::FN + j, 0, LOADS - LATE, stage);
+                        if (kk == 0 || kk + 1 == kRounds) __builtin_amdgcn_sched_barrier(0);
                     }
                 __builtin_amdgcn_sched_barrier(0);
+                if (LATE > 0 && kk == 0) loaded_step();
             }
-            loaded_step();
+            if (LATE == 0) loaded_step();
             stage = next;
         }
     };
@@ -962,6 +761,30 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
                         }
                     }
                 }
+                else if constexpr (D == TRIPS_DTYPE_F32)
+                {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                    {
+                        const int m = m_lane + i * 32 + 8 * g;
+                        using F4    = Pack<float, 4>::type;
+                        const F4 v  = {acc[i][j][4 * g] * unscale, acc[i][j][4 * g + 1] * unscale, acc[i][j][4 * g + 2] * unscale, acc[i][j][4 * g + 3] * unscale};
+                        if constexpr (MODE == PROBS)
+                        {
+                            if (n < count) *reinterpret_cast<F4*>(reinterpret_cast<float*>(p.probs) + n * p.piece + m) = v;
+                        }
+                        else if (n < p.in_piece && m < p.channels)
+                        {
+                            float* at = reinterpret_cast<float*>(p.d_table) + n * p.d_table_stride + m;
+                            if (m + 4 <= p.channels)
+                                *reinterpret_cast<F4*>(at) = v;
+                            else
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (m + e < p.channels) at[e] = v[e];
+                        }
+                    }
+                }
                 else
                 {
                     // two lanes' fours to eight of one lane: 16 bytes
@@ -1027,7 +850,7 @@ __global__ __launch_bounds__(S::WAVES * 64, 2) void product16_kernel(const Produ
 
 // ---- joins ----
 
-// 16 rows a workgroup, 16 lanes a row over the stripes: state and loss; the last workgroup adds the workgroups' sums up, in their order.
+// 1 << lanes_log2 lanes a row over the stripes of tiles: state and loss, and the workgroup's sum of losses.
 struct JoinParams
 {
     const float2* partial;
@@ -1037,44 +860,49 @@ struct JoinParams
     float* loss;
     float2* state;
     double* sums;
-    unsigned* ticket;
     long long n, rows_pad;
-    int stripes, reduction;
+    int stripes, reduction, lanes_log2;
     float scale, scale_log2;
 };
 __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
 {
-    __shared__ float2 part[16][17];
-    __shared__ float losses[16];
-    __shared__ bool last;
-    __shared__ double sums[256];
-    const int lane = threadIdx.x & 15, share = threadIdx.x >> 4;
-    const long long i = (long long)blockIdx.x * 16 + lane;
+    __shared__ float2 part[256];
+    __shared__ double sums[4];
+    const int rows_log2 = 8 - p.lanes_log2, row = threadIdx.x & ((1 << rows_log2) - 1), lanes = 1 << p.lanes_log2;
+    const long long i = ((long long)blockIdx.x << rows_log2) + row;
     const int at      = i < p.n ? p.place[i] : -1;
     float2 own        = make_float2(-__builtin_inff(), 0.f);
     if (at >= 0)
-        for (int s = share; s < p.stripes; s += 16)
+    {
+        const float product = p.own_product[at];
+#pragma unroll 4
+        for (int s = threadIdx.x >> rows_log2; s < p.stripes; s += lanes)
         {
             const float2 x  = p.partial[s * p.rows_pad + at];
             const float top = fmaxf(own.x, x.x), base = top == -__builtin_inff() ? 0.f : top;
             own = make_float2(top, own.y * part_of(own.x, base, p.scale_log2) + x.y * part_of(x.x, base, p.scale_log2));
         }
-    part[share][lane] = own;
+        part[threadIdx.x] = own;
+        own.y             = product;
+    }
     __syncthreads();
-    if (threadIdx.x < 16)
+    float loss = 0.f;
+    if (threadIdx.x >> rows_log2 == 0)
     {
-        float top = -__builtin_inff(), sum = 0.f;
-        for (int s = 0; s < 16; ++s) top = fmaxf(top, part[s][lane].x);
-        const float base = top == -__builtin_inff() ? 0.f : top;
-        for (int s = 0; s < 16; ++s) sum += part[s][lane].y * part_of(part[s][lane].x, base, p.scale_log2);
-        float loss = 0.f, log_sum = 0.f;
+        float top = -__builtin_inff(), sum = 0.f, log_sum = 0.f;
         if (at >= 0)
         {
+            for (int s = 0; s < lanes; ++s) top = fmaxf(top, part[(s << rows_log2) + row].x);
+            const float base = top == -__builtin_inff() ? 0.f : top;
+            for (int s = 0; s < lanes; ++s)
+            {
+                const float2 x = part[(s << rows_log2) + row];
+                sum += x.y * part_of(x.x, base, p.scale_log2);
+            }
             const double log = log2((double)sum);
-            loss    = (float)(((double)top - (double)p.own_product[at]) * (double)p.scale + log * kLog2);
+            loss    = (float)(((double)top - (double)own.y) * (double)p.scale + log * kLog2);
             log_sum = (float)log;
         }
-        losses[lane] = loss;
         if (i < p.n)
         {
             p.state[i] = make_float2(at >= 0 ? top : 0.f, log_sum);
@@ -1082,26 +910,35 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
         }
     }
     if (p.reduction == TRIPS_REDUCE_NONE) return;
+    double sum = (double)loss;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
     __syncthreads();
     if (threadIdx.x == 0)
     {
-        double sum = 0.0;
-        for (int l = 0; l < 16; ++l) sum += (double)losses[l];
-        __hip_atomic_store(&p.sums[blockIdx.x], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        if (gridDim.x == 1)
+            *p.loss = (float)(p.reduction == TRIPS_REDUCE_MEAN ? sum / (double)max(*p.count, 1) : sum);
+        else
+            p.sums[blockIdx.x] = sum;
     }
-    __syncthreads();
-    if (!last) return;
+}
+
+// The workgroups' sums, in an order that their number alone determines.
+__global__ __launch_bounds__(1024) void sum_kernel(const double* from, int n, const int* count, int reduction, float* loss)
+{
+    __shared__ double sums[16];
     double sum = 0.0;
-    for (unsigned b = threadIdx.x; b < gridDim.x; b += 256) sum += __hip_atomic_load(&p.sums[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    sums[threadIdx.x] = sum;
+    for (int b = threadIdx.x; b < n; b += 1024) sum += from[b];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
     __syncthreads();
-    for (int o = 128; o > 0; o >>= 1)
-    {
-        if ((int)threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) *p.loss = (float)(p.reduction == TRIPS_REDUCE_MEAN ? sums[0] / (double)max(*p.count, 1) : sums[0]);
+    if (threadIdx.x > 0) return;
+    sum = 0.0;
+    for (int w = 0; w < 16; ++w) sum += sums[w];
+    *loss = (float)(reduction == TRIPS_REDUCE_MEAN ? sum / (double)max(*count, 1) : sum);
 }
 
 // d_rows: the splits' sums, in their order, at their rows' own places.
@@ -1134,7 +971,11 @@ int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 unsigned tiles_of(int64_t n, int tile) { return (unsigned)((n + tile - 1) / tile); }
 
 // Whether the direct loads take the table's rows as they are: 16 bytes at a time, 256 rows within 31 bits.
-bool rows_in_place(const TripsTableLossDesc& d) { return d.num_channels % 8 == 0 && d.table_stride % 8 == 0 && d.table_stride < 1 << 21; }
+bool rows_in_place(const TripsTableLossDesc& d)
+{
+    const int64_t size = dtype_bytes(d.dtype);
+    return d.num_channels * size % 16 == 0 && d.table_stride * size % 16 == 0 && d.table_stride < 1 << 20;
+}
 
 // Steps of a call over the table; what each takes of the workspace.
 struct Layout
@@ -1145,16 +986,19 @@ struct Layout
     size_t packed, place, target, state, factor, count, chunk_count, chunk_top, partial, own_product, sums, probs, slabs, copy, bytes;
 };
 
-#ifndef BIG
-#define BIG 256, 256, 2, 4, 64, 2
-#endif
-struct Big : Shape<BIG>
+using Big   = Shape<256, 256, 2, 4, 2, 1>;
+using Small = Shape<128, 128, 2, 2, 2, 2>;
+
+// Large tiles where they are enough for the CUs; always small ones in 32 bits, whose products take so long that the loads do not count.
+bool big_tiles(const TripsTableLossDesc& d)
 {
-};
+    if (d.dtype == TRIPS_DTYPE_F32) return false;
+    return (int64_t)tiles_of(d.num_rows, 256) * tiles_of(d.num_entries, 256) >= kCus;
+}
 
 // Into how many parts the rows' gradients are cut along the entries, so that they and the table's gradients (units of `steps` and
 // `table_steps`) keep all CUs busy to the end. A part costs its sums' way to memory and back, about 16 steps' time.
-int splits_of(int64_t units, int64_t steps, int64_t table_units, int64_t table_steps)
+int splits_of(int workers, int64_t units, int64_t steps, int64_t table_units, int64_t table_steps)
 {
     int best      = 1;
     int64_t least = INT64_MAX;
@@ -1163,12 +1007,12 @@ int splits_of(int64_t units, int64_t steps, int64_t table_units, int64_t table_s
         // the larger units first, each to the first CU that is free
         int64_t a = units * s, size_a = (steps + s - 1) / s + 16, b = table_units, size_b = table_steps + 8;
         if (size_a < size_b) std::swap(a, b), std::swap(size_a, size_b);
-        const int64_t rest = a % kCus, full = a / kCus * size_a;
+        const int64_t rest = a % workers, full = a / workers * size_a;
         int64_t end = full + (rest ? size_a : 0);
         for (int64_t k = 0;; ++k)
         {
             const int64_t t = full + k * size_b, by_late = t - full - size_a;
-            const int64_t done = (kCus - rest) * k + (rest && by_late > 0 ? rest * (by_late / size_b) : 0);
+            const int64_t done = (workers - rest) * k + (rest && by_late > 0 ? rest * (by_late / size_b) : 0);
             if (done >= b)
             {
                 end = std::max(end, t);
@@ -1184,8 +1028,8 @@ int splits_of(int64_t units, int64_t steps, int64_t table_units, int64_t table_s
 Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
 {
     Layout l{};
-    const bool wide      = d.dtype == TRIPS_DTYPE_F32;
-    const int size       = dtype_bytes(d.dtype), tile = wide ? kTile : 256;
+    const bool big       = big_tiles(d);
+    const int size       = dtype_bytes(d.dtype), tile = big ? 256 : 128, steps = kStepBytes / size;
     l.rows_pad           = up(d.num_rows, 256), l.chunks = d.num_rows > kCountedBy ? up(d.num_rows, kChunk) / kChunk : 0;
     l.kp                 = (int)up(d.num_channels, 64);
     l.copies             = copies;
@@ -1203,8 +1047,8 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     int64_t most = up(std::max<int64_t>(d.num_entries, 1), 256);
     if (copies)
     {
-        most   = std::min(most, std::max<int64_t>((rows_in_place(d) ? kLeastCopyBytes : kCopyBytes) / (l.kp * 2) / 256, 1) * 256);
-        l.copy = take((size_t)most * l.kp * 2);
+        most   = std::min(most, std::max<int64_t>((rows_in_place(d) ? kLeastCopyBytes : kCopyBytes) / (l.kp * size) / 256, 1) * 256);
+        l.copy = take((size_t)most * l.kp * size);
     }
     if (backward) most = std::min(most, std::max<int64_t>(kPieceBytes / (std::max<int64_t>(l.rows_pad, 1) * size) / 256, 1) * 256);
     l.pieces = std::max<int64_t>(1, (d.num_entries + most - 1) / most);
@@ -1212,28 +1056,28 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     const int64_t row_tiles = up(d.num_rows, tile) / tile;
     if (!backward)
     {
-        l.stripes     = (int)(up(l.piece, tile) / tile);
+        l.stripes     = (int)(l.piece / tile);
         l.partial     = take((size_t)l.stripes * l.pieces * l.rows_pad * sizeof(float2));
         l.own_product = take(l.rows_pad * 4);
-        l.sums        = take((d.num_rows / 16 + 1) * 8);
+        l.sums        = take((d.num_rows / 4 + 1) * 8);
     }
     else
     {
         l.state = take(d.num_rows * 8), l.factor = take(d.num_rows * 4);
         l.probs = take((size_t)l.rows_pad * l.piece * size);
-        l.splits = splits_of(row_tiles * (up(d.num_channels, tile) / tile), up(l.piece, 64) / 64, up(l.piece, tile) / tile * (up(d.num_channels, tile) / tile), up(d.num_rows, 64) / 64);
+        l.splits = splits_of(big ? kCus : 2 * kCus, row_tiles * (up(d.num_channels, tile) / tile), l.piece / steps, l.piece / tile * (up(d.num_channels, tile) / tile), up(d.num_rows, steps) / steps);
         l.slabs  = take((size_t)l.splits * l.rows_pad * l.kp * 4);
     }
     l.bytes = at;
     return l;
 }
 
-bool copies_of(const TripsTableLossDesc& d, const void* table) { return d.dtype != TRIPS_DTYPE_F32 && !(rows_in_place(d) && aligned(table, 16)); }
+bool copies_of(const TripsTableLossDesc& d, const void* table) { return !(rows_in_place(d) && aligned(table, 16)); }
 
 // For any address of the table.
 size_t workspace_of(const TripsTableLossDesc& d, bool backward)
 {
-    const size_t copied = d.dtype == TRIPS_DTYPE_F32 ? 0 : layout_of(d, backward, true).bytes;
+    const size_t copied = layout_of(d, backward, true).bytes;
     return copies_of(d, nullptr) ? copied : std::max(copied, layout_of(d, backward, false).bytes);
 }
 
@@ -1247,7 +1091,7 @@ hipError_t gather(const TripsTableLossDesc& d, const Layout& l, const void* rows
     p.rows = rows, p.target = target, p.d_loss = d_loss, p.state = (const float2*)state;
     p.packed = w + l.packed, p.place = (int*)(w + l.place), p.packed_target = (int*)(w + l.target);
     p.packed_state = (float2*)(w + l.state), p.packed_factor = (float*)(w + l.factor);
-    p.count = (int*)(w + l.count), p.unscale = (float*)(w + l.count) + 2, p.ticket = (unsigned*)(w + l.count) + 1;
+    p.count = (int*)(w + l.count), p.unscale = (float*)(w + l.count) + 2;
     p.n = d.num_rows, p.entries = d.num_entries, p.stride = d.rows_stride;
     p.channels = d.num_channels, p.kp = l.kp, p.i32 = d.index_dtype == TRIPS_INDEX_I32, p.reduction = d.reduction, p.backward = backward, p.scale = d.scale;
     if (l.chunks)
@@ -1270,7 +1114,7 @@ ProductParams product_params(const TripsTableLossDesc& d, const Layout& l, char*
     p.packed_state = (float2*)(w + l.state), p.packed_factor = (float*)(w + l.factor), p.unscale = (float*)(w + l.count) + 2;
     p.partial = (float2*)(w + l.partial), p.own_product = (float*)(w + l.own_product), p.probs = w + l.probs, p.slabs = (float*)(w + l.slabs);
     p.d_table_stride = d.d_table_stride, p.rows_pad = l.rows_pad;
-    p.channels = d.num_channels, p.kp = l.kp, p.piece = (int)l.piece, p.stripes = l.stripes, p.splits = l.splits;
+    p.channels = d.num_channels, p.kp = l.kp, p.piece = (int)l.piece, p.splits = l.splits;
     p.scale_log2 = scale_log2(d);
     return p;
 }
@@ -1289,31 +1133,27 @@ hipError_t take_piece(const TripsTableLossDesc& d, const Layout& l, int64_t piec
     p.table = w + l.copy, p.table_stride = p.held = l.kp;
     ProfScope scope(prof, "loss_copy", stream);
     const int64_t pieces = (int64_t)p.in_piece * l.kp / 8;
-    copy_entries_kernel<<<(unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 16), 256, 0, stream>>>(reinterpret_cast<const unsigned short*>(entries), d.table_stride,
-                                                                                                       reinterpret_cast<unsigned short*>(w + l.copy), p.in_piece, d.num_channels, l.kp);
+    copy_entries_kernel<T><<<(unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 16), 256, 0, stream>>>(entries, d.table_stride, reinterpret_cast<T*>(w + l.copy), p.in_piece,
+                                                                                                          d.num_channels, l.kp);
     return hipGetLastError();
 }
 
-template <int D, int MODE>
-hipError_t launch_product(const TripsTableLossDesc& d, ProductParams p, hipStream_t stream, Profiler* prof)
+template <int D, int KIND>
+hipError_t launch_product(const TripsTableLossDesc& d, const ProductParams& p, hipStream_t stream, Profiler* prof)
 {
-    static constexpr const char* NAMES[] = {"loss_logits", "loss_probs", "loss_d_rows", "loss_d_table", "loss_grads"};
-    if (p.in_piece == 0 || (d.num_rows == 0 && MODE != D_TABLE && MODE != GRADS)) return hipSuccess;
-    ProfScope scope(prof, NAMES[MODE], stream);
-    if constexpr (D == TRIPS_DTYPE_F32)
+    auto launch = [&](auto shape)
     {
-        const int64_t along_m = MODE == LOGITS || MODE == PROBS ? p.in_piece : d.num_channels, along_n = MODE == D_TABLE ? p.in_piece : d.num_rows;
-        p.tiles_x = tiles_of(along_m, kTile), p.tiles_y = tiles_of(along_n, kTile);
-        product_kernel<D, MODE><<<p.tiles_x * p.tiles_y * (MODE == D_ROWS ? p.splits : 1), 256, 0, stream>>>(p);
-    }
-    else
-    {
-        const int64_t row_tiles = tiles_of(d.num_rows, Big::BN), channel_tiles = tiles_of(d.num_channels, Big::BM);
-        const int64_t units = MODE == GRADS ? channel_tiles * ((p.d_rows ? row_tiles * p.splits : 0) + (p.d_table ? tiles_of(p.in_piece, Big::BN) : 0)) : tiles_of(p.in_piece, Big::BM) * row_tiles;
+        using S = decltype(shape);
+        const int64_t row_tiles = tiles_of(d.num_rows, S::BN), channel_tiles = tiles_of(d.num_channels, S::BM);
+        const int64_t units = KIND == GRADS ? channel_tiles * ((p.d_rows ? row_tiles * p.splits : 0) + (p.d_table ? tiles_of(p.in_piece, S::BN) : 0)) : tiles_of(p.in_piece, S::BM) * row_tiles;
         if (units == 0) return hipSuccess;
-        product16_kernel<D, MODE, Big><<<(unsigned)std::min<int64_t>(units, kCus), Big::WAVES * 64, 0, stream>>>(p);
-    }
-    return hipGetLastError();
+        ProfScope scope(prof, KIND == LOGITS ? "loss_logits" : KIND == PROBS ? "loss_probs" : "loss_grads", stream);
+        product_kernel<D, KIND, S><<<(unsigned)std::min<int64_t>(units, S::PER_CU * kCus), S::WAVES * 64, 0, stream>>>(p);
+        return hipGetLastError();
+    };
+    if constexpr (D != TRIPS_DTYPE_F32)
+        if (big_tiles(d)) return launch(Big{});
+    return launch(Small{});
 }
 
 template <int D>
@@ -1330,10 +1170,18 @@ hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* ta
     }
     JoinParams j{};
     j.partial = p.partial, j.own_product = p.own_product, j.place = (int*)(w + l.place), j.count = p.count;
-    j.loss = loss, j.state = (float2*)state, j.scale = std::fabs(d.scale), j.scale_log2 = p.scale_log2, j.sums = (double*)(w + l.sums), j.ticket = (unsigned*)(w + l.count) + 1;
-    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.stripes = (int)tiles_of(d.num_entries, D == TRIPS_DTYPE_F32 ? kTile : Big::BM), j.reduction = d.reduction;
-    ProfScope scope(prof, "loss_join", stream);
-    join_kernel<<<std::max(1u, (unsigned)((d.num_rows + 15) / 16)), 256, 0, stream>>>(j);
+    j.loss = loss, j.state = (float2*)state, j.scale = std::fabs(d.scale), j.scale_log2 = p.scale_log2, j.sums = (double*)(w + l.sums);
+    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.stripes = (int)tiles_of(d.num_entries, big_tiles(d) ? 256 : 128), j.reduction = d.reduction;
+    while (j.lanes_log2 < 6 && 8 << j.lanes_log2 < j.stripes) ++j.lanes_log2;
+    const int64_t rows_each = 256 >> j.lanes_log2, groups = std::max<int64_t>(1, (d.num_rows + rows_each - 1) / rows_each);
+    {
+        ProfScope scope(prof, "loss_join", stream);
+        join_kernel<<<(unsigned)groups, 256, 0, stream>>>(j);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    if (d.reduction == TRIPS_REDUCE_NONE || groups == 1) return hipSuccess;
+    ProfScope scope(prof, "loss_sum", stream);
+    sum_kernel<<<1, 1024, 0, stream>>>(j.sums, (int)groups, j.count, d.reduction, loss);
     return hipGetLastError();
 }
 
@@ -1349,17 +1197,7 @@ hipError_t backward(const TripsTableLossDesc& d, const void* rows, const void* t
     {
         if (hipError_t e = take_piece<D>(d, l, piece, table, d_table, w, p, stream, prof)) return e;
         if (hipError_t e = launch_product<D, PROBS>(d, p, stream, prof)) return e;
-        if constexpr (D != TRIPS_DTYPE_F32)
-        {
-            if (hipError_t e = launch_product<D, GRADS>(d, p, stream, prof)) return e;
-        }
-        else
-        {
-            if (d_rows && d.num_rows > 0)
-                if (hipError_t e = launch_product<D, D_ROWS>(d, p, stream, prof)) return e;
-            if (d_table)
-                if (hipError_t e = launch_product<D, D_TABLE>(d, p, stream, prof)) return e;
-        }
+        if (hipError_t e = launch_product<D, GRADS>(d, p, stream, prof)) return e;
     }
     if (!d_rows || d.num_rows == 0) return hipSuccess;
     ProfScope scope(prof, "loss_rows_out", stream);
