@@ -941,29 +941,46 @@ __global__ __launch_bounds__(1024) void sum_kernel(const double* from, int n, co
     *loss = (float)(reduction == TRIPS_REDUCE_MEAN ? sum / (double)max(*count, 1) : sum);
 }
 
-// d_rows: the splits' sums, in their order, at their rows' own places.
+// d_rows: the splits' sums, in their order, at their rows' own places; four channels a lane.
 template <int D>
 __global__ __launch_bounds__(256) void rows_out_kernel(const float* slabs, const int* place, const float* unscale, void* d_rows, long long n, long long rows_pad,
                                                        long long stride, int channels, int kp, int splits)
 {
-    using E       = Element<D>;
-    const float f = *unscale;
-    for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (long long)gridDim.x * 4)
+    using E  = Element<D>;
+    using T  = typename E::type;
+    using F4 = Pack<float, 4>::type;
+    using T4 = typename Pack<T, 4>::type;
+    const float f       = *unscale;
+    const int quads     = (channels + 3) >> 2;
+    const long long all = n * quads, slab = rows_pad * kp;
+    for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < all; q += (long long)gridDim.x * 256)
     {
-    const int at = place[i];
-    for (int c = threadIdx.x & 63; c < channels; c += 64)
-    {
-        float sum = 0.f;
+        const long long i = q / quads;
+        const int c = (int)(q - i * quads) * 4, at = place[i];
+        F4 sum = {0.f, 0.f, 0.f, 0.f};
         if (at >= 0)
-            for (int s = 0; s < splits; ++s) sum += slabs[((long long)s * rows_pad + at) * kp + c];
-        reinterpret_cast<typename E::type*>(d_rows)[i * stride + c] = E::from_float(at >= 0 ? sum * f : 0.f);
-    }
+        {
+            const float* from = slabs + (long long)at * kp + c;
+#pragma unroll 4
+            for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const F4*>(from + s * slab);
+        }
+        T* to = reinterpret_cast<T*>(d_rows) + i * stride + c;
+        T4 out;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = E::from_float(at >= 0 ? sum[e] * f : 0.f);
+        if (c + 4 <= channels)
+            *reinterpret_cast<T4*>(to) = out;
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < channels) to[e] = out[e];
     }
 }
 
 // ---- host ----
 
 constexpr int64_t kPieceBytes = 1ll << 30;  // of d_ij
+constexpr int64_t kSlabBytes  = 256ll << 20;  // of the parts of the rows' gradients
 constexpr int kCus            = 256;
 constexpr int64_t kCopyBytes = 64ll << 20, kLeastCopyBytes = 16ll << 20;  // of copied entries
 
@@ -988,48 +1005,74 @@ struct Layout
 
 using Big   = Shape<256, 256, 2, 4, 2, 1>;
 using Small = Shape<128, 128, 2, 2, 2, 2>;
+using Tiny  = Shape<64, 64, 2, 2, 4, 2>;
 
-// Large tiles where they are enough for the CUs; always small ones in 32 bits, whose products take so long that the loads do not count.
-bool big_tiles(const TripsTableLossDesc& d)
+// f(a shape): the largest tiles of which a product of `down` x `across` makes one for each CU at least; never the largest in 32 bits, whose
+// products take so long that the loads do not count.
+template <typename F>
+auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
 {
-    if (d.dtype == TRIPS_DTYPE_F32) return false;
-    return (int64_t)tiles_of(d.num_rows, 256) * tiles_of(d.num_entries, 256) >= kCus;
+    auto units = [&](int64_t tile)
+    {
+        const int64_t rows = up(d.num_rows, tile) / tile, entries = up(d.num_entries, tile) / tile, channels = up(d.num_channels, tile) / tile;
+        return grads ? channels * entries : rows * entries;
+    };
+    if (d.dtype != TRIPS_DTYPE_F32 && units(256) >= kCus) return f(Big{});
+    if (units(128) >= kCus) return f(Small{});
+    return f(Tiny{});
+}
+// Entries of a tile of the logits.
+int entries_of_tile(const TripsTableLossDesc& d)
+{
+    return with_shape(d, false, [](auto shape) { return decltype(shape)::BM; });
 }
 
-// Into how many parts the rows' gradients are cut along the entries, so that they and the table's gradients (units of `steps` and
-// `table_steps`) keep all CUs busy to the end. A part costs its sums' way to memory and back, about 16 steps' time.
-int splits_of(int workers, int64_t units, int64_t steps, int64_t table_units, int64_t table_steps)
+// Into how many parts the rows' gradients are cut along the entries, so that they and the table's gradients keep all CUs busy to the end,
+// by what a step and a unit's results take, and the parts' way to memory and back.
+int splits_of(const TripsTableLossDesc& d, int64_t rows_pad, int64_t piece, int kp)
 {
-    int best      = 1;
-    int64_t least = INT64_MAX;
-    for (int s = 1; s <= 16 && (s == 1 || steps / s >= 16); ++s)
+    return with_shape(d, true, [&](auto shape)
     {
-        // the larger units first, each to the first CU that is free
-        int64_t a = units * s, size_a = (steps + s - 1) / s + 16, b = table_units, size_b = table_steps + 8;
-        if (size_a < size_b) std::swap(a, b), std::swap(size_a, size_b);
-        const int64_t rest = a % workers, full = a / workers * size_a;
-        int64_t end = full + (rest ? size_a : 0);
-        for (int64_t k = 0;; ++k)
+        using S = decltype(shape);
+        const bool wide       = d.dtype == TRIPS_DTYPE_F32;
+        const int step_k      = kStepBytes / dtype_bytes(d.dtype), workers = kCus * S::PER_CU;
+        const double step     = (wide ? 4.0 : S::BM == 256 ? 1.6 : 0.8) * (S::BM == 64 ? 0.25 : 1.0);  // microseconds
+        const double results  = S::BM == 256 ? 10.0 : S::BM == 128 ? 4.0 : 2.0, slab = (double)rows_pad * kp * 4;
+        const int64_t units = up(d.num_rows, S::BN) / S::BN * (up(d.num_channels, S::BM) / S::BM), steps = piece / step_k;
+        const int64_t table_units = piece / S::BN * (up(d.num_channels, S::BM) / S::BM), table_steps = up(d.num_rows, step_k) / step_k;
+        int best     = 1;
+        double least = 1e300;
+        for (int s = 1; s <= 64 && (s == 1 || (steps / s >= 4 && slab * s <= (double)kSlabBytes)); ++s)
         {
-            const int64_t t = full + k * size_b, by_late = t - full - size_a;
-            const int64_t done = (workers - rest) * k + (rest && by_late > 0 ? rest * (by_late / size_b) : 0);
-            if (done >= b)
+            // the larger units first, each to the first workgroup that is free
+            int64_t a = units * s, b = table_units;
+            double size_a = (double)((steps + s - 1) / s) * step + results, size_b = (double)table_steps * step + results;
+            if (size_a < size_b) std::swap(a, b), std::swap(size_a, size_b);
+            const int64_t rest = a % workers;
+            const double full  = (double)(a / workers) * size_a;
+            double end         = full + (rest ? size_a : 0.0);
+            for (int64_t k = b / workers;; ++k)
             {
-                end = std::max(end, t);
-                break;
+                const double t     = full + (double)k * size_b, late = t - full - size_a;
+                const int64_t done = (workers - rest) * k + (rest && late > 0 ? rest * (int64_t)(late / size_b) : 0);
+                if (done >= b)
+                {
+                    end = std::max(end, t);
+                    break;
+                }
             }
+            end += s * slab / 3.5e6;
+            if (end < least) best = s, least = end;
         }
-        if (end < least) best = s, least = end;
-    }
-    return best;
+        return best;
+    });
 }
 
 // copies: the table's entries are copied, a piece at a time, before the products read them.
 Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
 {
     Layout l{};
-    const bool big       = big_tiles(d);
-    const int size       = dtype_bytes(d.dtype), tile = big ? 256 : 128, steps = kStepBytes / size;
+    const int size       = dtype_bytes(d.dtype);
     l.rows_pad           = up(d.num_rows, 256), l.chunks = d.num_rows > kCountedBy ? up(d.num_rows, kChunk) / kChunk : 0;
     l.kp                 = (int)up(d.num_channels, 64);
     l.copies             = copies;
@@ -1053,10 +1096,9 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     if (backward) most = std::min(most, std::max<int64_t>(kPieceBytes / (std::max<int64_t>(l.rows_pad, 1) * size) / 256, 1) * 256);
     l.pieces = std::max<int64_t>(1, (d.num_entries + most - 1) / most);
     l.piece  = up((d.num_entries + l.pieces - 1) / l.pieces, 256);
-    const int64_t row_tiles = up(d.num_rows, tile) / tile;
     if (!backward)
     {
-        l.stripes     = (int)(l.piece / tile);
+        l.stripes     = (int)(l.piece / entries_of_tile(d));
         l.partial     = take((size_t)l.stripes * l.pieces * l.rows_pad * sizeof(float2));
         l.own_product = take(l.rows_pad * 4);
         l.sums        = take((d.num_rows / 4 + 1) * 8);
@@ -1065,7 +1107,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     {
         l.state = take(d.num_rows * 8), l.factor = take(d.num_rows * 4);
         l.probs = take((size_t)l.rows_pad * l.piece * size);
-        l.splits = splits_of(big ? kCus : 2 * kCus, row_tiles * (up(d.num_channels, tile) / tile), l.piece / steps, l.piece / tile * (up(d.num_channels, tile) / tile), up(d.num_rows, steps) / steps);
+        l.splits = splits_of(d, l.rows_pad, l.piece, l.kp);
         l.slabs  = take((size_t)l.splits * l.rows_pad * l.kp * 4);
     }
     l.bytes = at;
@@ -1141,19 +1183,16 @@ hipError_t take_piece(const TripsTableLossDesc& d, const Layout& l, int64_t piec
 template <int D, int KIND>
 hipError_t launch_product(const TripsTableLossDesc& d, const ProductParams& p, hipStream_t stream, Profiler* prof)
 {
-    auto launch = [&](auto shape)
+    return with_shape(d, KIND == GRADS, [&](auto shape)
     {
-        using S = decltype(shape);
+        using S = std::conditional_t<D == TRIPS_DTYPE_F32 && decltype(shape)::BM == 256, Small, decltype(shape)>;
         const int64_t row_tiles = tiles_of(d.num_rows, S::BN), channel_tiles = tiles_of(d.num_channels, S::BM);
         const int64_t units = KIND == GRADS ? channel_tiles * ((p.d_rows ? row_tiles * p.splits : 0) + (p.d_table ? tiles_of(p.in_piece, S::BN) : 0)) : tiles_of(p.in_piece, S::BM) * row_tiles;
         if (units == 0) return hipSuccess;
         ProfScope scope(prof, KIND == LOGITS ? "loss_logits" : KIND == PROBS ? "loss_probs" : "loss_grads", stream);
         product_kernel<D, KIND, S><<<(unsigned)std::min<int64_t>(units, S::PER_CU * kCus), S::WAVES * 64, 0, stream>>>(p);
         return hipGetLastError();
-    };
-    if constexpr (D != TRIPS_DTYPE_F32)
-        if (big_tiles(d)) return launch(Big{});
-    return launch(Small{});
+    });
 }
 
 template <int D>
@@ -1171,7 +1210,7 @@ hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* ta
     JoinParams j{};
     j.partial = p.partial, j.own_product = p.own_product, j.place = (int*)(w + l.place), j.count = p.count;
     j.loss = loss, j.state = (float2*)state, j.scale = std::fabs(d.scale), j.scale_log2 = p.scale_log2, j.sums = (double*)(w + l.sums);
-    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.stripes = (int)tiles_of(d.num_entries, big_tiles(d) ? 256 : 128), j.reduction = d.reduction;
+    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.stripes = (int)tiles_of(d.num_entries, entries_of_tile(d)), j.reduction = d.reduction;
     while (j.lanes_log2 < 6 && 8 << j.lanes_log2 < j.stripes) ++j.lanes_log2;
     const int64_t rows_each = 256 >> j.lanes_log2, groups = std::max<int64_t>(1, (d.num_rows + rows_each - 1) / rows_each);
     {
@@ -1201,7 +1240,7 @@ hipError_t backward(const TripsTableLossDesc& d, const void* rows, const void* t
     }
     if (!d_rows || d.num_rows == 0) return hipSuccess;
     ProfScope scope(prof, "loss_rows_out", stream);
-    rows_out_kernel<D><<<(unsigned)std::min<int64_t>((d.num_rows + 3) / 4, 1 << 20), 256, 0, stream>>>((float*)(w + l.slabs), (int*)(w + l.place), p.unscale, d_rows, d.num_rows, l.rows_pad, d.d_rows_stride,
+    rows_out_kernel<D><<<(unsigned)std::min<int64_t>((d.num_rows * ((d.num_channels + 3) / 4) + 255) / 256, 1 << 16), 256, 0, stream>>>((float*)(w + l.slabs), (int*)(w + l.place), p.unscale, d_rows, d.num_rows, l.rows_pad, d.d_rows_stride,
                                                                            d.num_channels, l.kp, l.splits);
     return hipGetLastError();
 }
