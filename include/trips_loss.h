@@ -43,20 +43,21 @@ typedef struct TripsTableLossDesc {
     int64_t d_table_stride; /* backward */
 } TripsTableLossDesc;
 
-/* state: [N, 2], 8-byte aligned, what the backward call takes: the largest |scale| / scale <rows_i, table_j> of all j, and the log2 of the sum of
- * exp(l_ij) over that of the largest; zeros for rows that do not count. Logits and sums are held in 32 bits.
+/* kept: trips_table_loss_kept_size bytes, 256-byte aligned, what the backward call takes: the rows that count, one behind the other, and
+ * of each its target, its largest product with an entry and the sum of exponentials. Logits and sums are held in 32 bits.
  * `workspace`: trips_table_loss_workspace_size bytes (backward: 0 for the forward call), 256-byte aligned, of any content;
  * calls that share one must not overlap. */
+int trips_table_loss_kept_size(const TripsTableLossDesc* desc, size_t* bytes);
 int trips_table_loss_workspace_size(const TripsTableLossDesc* desc, int backward, size_t* bytes);
-int trips_table_loss_forward(TripsCtx* ctx, const TripsTableLossDesc* desc, const void* rows, const void* table, const void* target,
-                             float* loss, float* state, void* workspace, size_t workspace_bytes, void* stream);
+int trips_table_loss_forward(TripsCtx* ctx, const TripsTableLossDesc* desc, const void* rows, const void* table, const void* target, float* loss,
+                             void* kept, size_t kept_bytes, void* workspace, size_t workspace_bytes, void* stream);
 
-/* d_loss: [N], or [1], as the loss. d_rows [N, C] and d_table [T, C] are written, rows that do not count with zeros; either may
- * be NULL. The logits are computed again, in pieces of the table; their gradient is held in the tensors' type within a
- * piece, sums over it in 32 bits, in an order that the sizes alone determine. */
-int trips_table_loss_backward(TripsCtx* ctx, const TripsTableLossDesc* desc, const void* rows, const void* table, const void* target,
-                              const float* state, const float* d_loss, void* d_rows, void* d_table, void* workspace, size_t workspace_bytes,
-                              void* stream);
+/* The same desc (but for the strides, those of what is written among them) and table as the forward call that filled `kept`, which is
+ * only read and may be used again. d_loss: [N], or [1], as the loss. d_rows [N, C] and d_table [T, C] are written, rows that do not count with
+ * zeros; either may be NULL. The logits are computed again, in pieces of the table; their gradient is held in the tensors' type
+ * within a piece, sums over it in 32 bits, in an order that the sizes and the number of rows that count alone determine. */
+int trips_table_loss_backward(TripsCtx* ctx, const TripsTableLossDesc* desc, const void* table, const void* kept, size_t kept_bytes, const float* d_loss,
+                              void* d_rows, void* d_table, void* workspace, size_t workspace_bytes, void* stream);
 
 /* out_i = (kept_i ? x_i factor : 0) + residual_i, factor = 65536 / (65536 - border), border = round(65536 p) (ties to even): of
  * element i, half i % 2 (0: the low one) of word i % 8 / 2 of Philox-4x32-10 is its 16 random bits, and it is kept where those

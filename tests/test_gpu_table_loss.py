@@ -325,14 +325,19 @@ def test_two_graphs_and_eager_calls():
         assert all(torch.equal(got, x) for (_, got), x in zip(graphs, want))
 
 
-def test_saved_tensors_that_changed_are_refused():
+def test_what_changed_before_the_gradients():
+    """The rows that count and their targets are kept; the table is not, and refused where it was written to."""
     x, w, target = _inputs(20, 50, 16, "f32")
-    for t in (x, w, target):
-        loss = table_cross_entropy(x, w, target)
-        with torch.no_grad():
-            t.add_(0)
-        with pytest.raises(RuntimeError, match="modified"):
-            loss.backward()
+    want = torch.autograd.grad(table_cross_entropy(x, w, target), (x, w))
+    loss = table_cross_entropy(x, w, target)
+    with torch.no_grad():
+        x.zero_(), target.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (x, w), retain_graph=True), want))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (x, w), retain_graph=True), want))  # (and again)
+    with torch.no_grad():
+        w.add_(0)
+    with pytest.raises(RuntimeError, match="modified"):
+        loss.backward()
 
 
 def test_gradients_once():

@@ -47,8 +47,11 @@ def _loss(**kw):
     return d
 
 
-def _bytes(backward):
+def _bytes(backward=None):
     n = C.c_size_t(0)
+    if backward is None:
+        assert _lib.load().trips_table_loss_kept_size(C.byref(_loss()), C.byref(n)) == 0
+        return n.value
     assert _lib.load().trips_table_loss_workspace_size(C.byref(_loss()), backward, C.byref(n)) == 0
     return n.value
 
@@ -56,17 +59,16 @@ def _bytes(backward):
 BAD_DESC = [dict(abi_version=1), dict(dtype=1), dict(dtype=9), dict(index_dtype=2), dict(reduction=3), dict(reduction=-1), dict(num_rows=-1), dict(num_rows=1 << 28),
             dict(num_entries=-1), dict(num_entries=1 << 31), dict(num_channels=0), dict(num_channels=1 << 17), dict(scale=NAN), dict(scale=float("inf")), dict(rows_stride=-1),
             dict(table_stride=-1), dict(table_stride=1 << 41)]
-BAD_CALL = [dict(ctx=None), dict(rows=None), dict(rows=AT + 2), dict(table=None), dict(table=AT + 1), dict(target=None), dict(target=AT + 2), dict(state=None), dict(state=AT + 4),
-            dict(workspace=None), dict(workspace=AT + 128)]
+BAD_CALL = [dict(ctx=None), dict(table=None), dict(table=AT + 1), dict(kept=None), dict(kept=AT + 128), dict(kept_size=_bytes() - 1), dict(workspace=None), dict(workspace=AT + 128)]
 
 
 @pytest.mark.parametrize("desc,call", [(d, {}) for d in BAD_DESC] + [({}, c) for c in BAD_CALL] + [
-    ({}, dict(loss=None)), ({}, dict(loss=AT + 2)), ({}, dict(size=_bytes(0) - 1)), (dict(index_dtype=0), dict(target=AT + 4)), (dict(dtype=2), dict(rows=AT + 1)),
+    ({}, dict(rows=None)), ({}, dict(rows=AT + 2)), ({}, dict(target=None)), ({}, dict(target=AT + 2)), ({}, dict(loss=None)), ({}, dict(loss=AT + 2)), ({}, dict(size=_bytes(0) - 1)), (dict(index_dtype=0), dict(target=AT + 4)), (dict(dtype=2), dict(rows=AT + 1)),
     (dict(num_rows=0, reduction=1), dict(loss=None))])
 def test_loss_refuses(desc, call):
     lib = _lib.load()
     rc = lib.trips_table_loss_forward(call.get("ctx", C.addressof(CTX)), C.byref(_loss(**desc)), call.get("rows", AT), call.get("table", AT), call.get("target", AT),
-                                      call.get("loss", AT), call.get("state", AT), call.get("workspace", AT), call.get("size", 1 << 40), None)
+                                      call.get("loss", AT), call.get("kept", AT), call.get("kept_size", 1 << 40), call.get("workspace", AT), call.get("size", 1 << 40), None)
     assert rc in ERR and lib.trips_last_error_string()
 
 
@@ -75,8 +77,8 @@ def test_loss_refuses(desc, call):
     (dict(d_rows_stride=15), {}), (dict(d_table_stride=0), {}), (dict(d_table_stride=-1), {})])
 def test_loss_backward_refuses(desc, call):
     lib = _lib.load()
-    rc = lib.trips_table_loss_backward(call.get("ctx", C.addressof(CTX)), C.byref(_loss(**desc)), call.get("rows", AT), call.get("table", AT), call.get("target", AT),
-                                       call.get("state", AT), call.get("d_loss", AT), call.get("d_rows", AT), call.get("d_table", AT), call.get("workspace", AT),
+    rc = lib.trips_table_loss_backward(call.get("ctx", C.addressof(CTX)), C.byref(_loss(**desc)), call.get("table", AT), call.get("kept", AT), call.get("kept_size", 1 << 40),
+                                       call.get("d_loss", AT), call.get("d_rows", AT), call.get("d_table", AT), call.get("workspace", AT),
                                        call.get("size", 1 << 40), None)
     assert rc in ERR and lib.trips_last_error_string()
 

@@ -29,7 +29,7 @@ OPTIM_SYMBOLS = ["trips_adamw_workspace_size", "trips_adamw_step", "trips_grad_n
 LOOKUP_SYMBOLS = ["trips_lookup_workspace_size", "trips_lookup_forward", "trips_lookup_plan_workspace_size",
                   "trips_lookup_plan", "trips_lookup_backward_workspace_size", "trips_lookup_backward"]
 # every symbol include/trips_loss.h declares
-LOSS_SYMBOLS = ["trips_table_loss_workspace_size", "trips_table_loss_forward", "trips_table_loss_backward", "trips_dropout"]
+LOSS_SYMBOLS = ["trips_table_loss_kept_size", "trips_table_loss_workspace_size", "trips_table_loss_forward", "trips_table_loss_backward", "trips_dropout"]
 
 
 class TripsError(RuntimeError):
@@ -94,8 +94,9 @@ def load():
     lib.trips_lookup_backward_workspace_size.argtypes = [C.POINTER(abi.TripsLookupDesc), C.POINTER(C.c_size_t)]
     lib.trips_lookup_backward.argtypes = [vp, C.POINTER(abi.TripsLookupDesc), vp, vp, vp, vp, vp, C.c_size_t, vp]
     lib.trips_table_loss_workspace_size.argtypes = [C.POINTER(abi.TripsTableLossDesc), i32, C.POINTER(C.c_size_t)]
-    lib.trips_table_loss_forward.argtypes = [vp, C.POINTER(abi.TripsTableLossDesc), vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
-    lib.trips_table_loss_backward.argtypes = [vp, C.POINTER(abi.TripsTableLossDesc), vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+    lib.trips_table_loss_kept_size.argtypes = [C.POINTER(abi.TripsTableLossDesc), C.POINTER(C.c_size_t)]
+    lib.trips_table_loss_forward.argtypes = [vp, C.POINTER(abi.TripsTableLossDesc), vp, vp, vp, vp, vp, C.c_size_t, vp, C.c_size_t, vp]
+    lib.trips_table_loss_backward.argtypes = [vp, C.POINTER(abi.TripsTableLossDesc), vp, vp, C.c_size_t, vp, vp, vp, vp, C.c_size_t, vp]
     lib.trips_dropout.argtypes = [vp, C.POINTER(abi.TripsDropoutDesc), vp, vp, vp, vp, vp, vp]
     lib.trips_profile_enable.argtypes = [vp, i32]
     lib.trips_splat_pair_rows_mode.argtypes = [vp, i32]

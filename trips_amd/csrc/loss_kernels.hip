@@ -32,24 +32,25 @@ constexpr int kGatherRows = 16;     // rows of a workgroup
 constexpr int kChunk      = 1024;   // targets of a chunk that count_kernel counts
 constexpr int kCountedBy  = 8192;   // rows from which the chunks are counted beforehand
 
+// What the forward call leaves for the backward call; "packed" is an index among the rows that count.
+struct Kept
+{
+    int* count;            // [1]
+    int* place;            // [n]: where a row went, -1 if it does not count
+    int* row;              // [packed]: where it comes from
+    int* target;           // [packed]
+    float2* state;         // [packed]: {largest product, log2 of the sum of exponentials over its own}
+    void* packed;          // [packed][kp], zeros from the channels on; negated where scale is, so that the products need only |scale|
+};
+
 struct GatherParams
 {
     const void* rows;
     const void* target;
-    const float* d_loss;     // backward: [n] or [1]
-    const float2* state;     // backward: [n]
-    const int* chunk_count;  // valid targets of each chunk, or NULL: every workgroup looks at all targets
-    const float* chunk_top;  // largest |d_loss| among them
-    void* packed;            // [count][kp], zeros from C on; negated where scale is, so that the products behind need only |scale|
-    int* place;              // [n]: where a row went, -1 if it does not count
-    int* packed_target;
-    float2* packed_state;
-    float* packed_factor;    // backward: what its gradients are multiplied by in d_ij
-    int* count;              // [1]
-    float* unscale;          // [2]: what undoes the scaling of d_ij, times scale and times |scale|
+    const int* chunk_count;  // targets that count of each chunk, or NULL: every workgroup looks at all targets
+    Kept kept;
     long long n, entries, stride;
-    int channels, kp, i32, reduction, backward;
-    float scale;
+    int channels, kp, negate;
 };
 
 template <bool I32>
@@ -65,44 +66,22 @@ __device__ __forceinline__ int wave_sum(int x)
     for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
     return x;
 }
-__device__ __forceinline__ float wave_max(float x)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
-}
-
-// |g|, 0 where it is not finite: such a row's factor is g itself, the others' go by the largest that is.
-__device__ __forceinline__ float size_of(float g)
-{
-    const float a = fabsf(g);
-    return a <= 3.4028234663852886e38f ? a : 0.f;
-}
 
 template <bool I32>
-__global__ __launch_bounds__(256) void count_kernel(const void* target, const float* d_loss, long long n, long long entries, int* chunk_count, float* chunk_top)
+__global__ __launch_bounds__(256) void count_kernel(const void* target, long long n, long long entries, int* chunk_count)
 {
     __shared__ int sums[4];
-    __shared__ float tops[4];
-    int own     = 0;
-    float top   = 0.f;
+    int own = 0;
+#pragma unroll
     for (int e = 0; e < kChunk / 256; ++e)
     {
         const long long i = (long long)blockIdx.x * kChunk + e * 256 + threadIdx.x;
-        if (i < n && counts<I32>(target, i, entries))
-        {
-            ++own;
-            if (d_loss) top = fmaxf(top, size_of(d_loss[i]));
-        }
+        own += i < n && counts<I32>(target, i, entries);
     }
-    own = wave_sum(own), top = wave_max(top);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = own, tops[threadIdx.x >> 6] = top;
+    own = wave_sum(own);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = own;
     __syncthreads();
-    if (threadIdx.x == 0)
-    {
-        chunk_count[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
-        chunk_top[blockIdx.x]   = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    }
+    if (threadIdx.x == 0) chunk_count[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
 __device__ __forceinline__ float negative(float x) { return -x; }
@@ -113,14 +92,12 @@ __device__ __forceinline__ unsigned short negative(unsigned short x) { return x 
 template <int D, bool I32>
 __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
 {
-    using T = typename Element<D>::type;
+    using T         = typename Element<D>::type;
+    constexpr int V = 16 / sizeof(T);
     __shared__ int before_w[4], all_w[4];
-    __shared__ float top_w[4];
     __shared__ int own_place[kGatherRows];
     const long long first = (long long)blockIdx.x * kGatherRows;
     int before = 0, all = 0;
-    float top = 0.f;
-    const bool tops = p.backward && p.reduction == TRIPS_REDUCE_NONE;
     if (p.chunk_count)
     {
         const long long chunks = (p.n + kChunk - 1) / kChunk, own_chunk = first / kChunk;
@@ -129,7 +106,6 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
             const int k = p.chunk_count[c];
             all += k;
             if (c < own_chunk) before += k;
-            if (tops) top = fmaxf(top, p.chunk_top[c]);
         }
         for (long long i = own_chunk * kChunk + threadIdx.x; i < first; i += 256) before += counts<I32>(p.target, i, p.entries);
     }
@@ -141,21 +117,15 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
 #pragma unroll
             for (int e = 0; e < 8; ++e) in[e] = counts<I32>(p.target, min(i0 + e * 256, p.n - 1), p.entries) && i0 + e * 256 < p.n;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-            {
-                all += in[e], before += in[e] && i0 + e * 256 < first;
-                if (tops && in[e]) top = fmaxf(top, size_of(p.d_loss[i0 + e * 256]));
-            }
+            for (int e = 0; e < 8; ++e) all += in[e], before += in[e] && i0 + e * 256 < first;
         }
-    before = wave_sum(before), all = wave_sum(all), top = wave_max(top);
+    before = wave_sum(before), all = wave_sum(all);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    if (lane == 0) before_w[wave] = before, all_w[wave] = all, top_w[wave] = top;
+    if (lane == 0) before_w[wave] = before, all_w[wave] = all;
     __syncthreads();
-    before = before_w[0] + before_w[1] + before_w[2] + before_w[3];
-    all    = all_w[0] + all_w[1] + all_w[2] + all_w[3];
-    top    = fmaxf(fmaxf(top_w[0], top_w[1]), fmaxf(top_w[2], top_w[3]));
     if (wave == 0)
     {
+        before              = before_w[0] + before_w[1] + before_w[2] + before_w[3];
         const long long i   = first + lane;
         const bool in       = lane < kGatherRows && i < p.n && counts<I32>(p.target, i, p.entries);
         const uint64_t mask = __ballot(in);
@@ -163,55 +133,92 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
         {
             const int at    = in ? before + __popcll(mask & ((1ull << lane) - 1)) : -1;
             own_place[lane] = at;
-            if (i < p.n) p.place[i] = at;
+            if (i < p.n) p.kept.place[i] = at;
             if (in)
             {
-                p.packed_target[at] = I32 ? reinterpret_cast<const int32_t*>(p.target)[i] : (int)reinterpret_cast<const int64_t*>(p.target)[i];
-                if (p.backward)
-                {
-                    p.packed_state[at] = p.state[i];
-                    // Largest factor: 1 in 32 bits and bfloat16, 2^15 in float16, whose range is short (probabilities from 2^-29 on then
-                    // are normal numbers); d_ij has those for bounds.
-                    const float one = D == TRIPS_DTYPE_F16 ? 32768.f : 1.f;
-                    float f         = one;
-                    if (p.reduction == TRIPS_REDUCE_NONE) f = top > 0.f ? p.d_loss[i] / top * one : p.d_loss[i];
-                    p.packed_factor[at] = f;
-                }
+                p.kept.row[at]    = (int)i;
+                p.kept.target[at] = I32 ? reinterpret_cast<const int32_t*>(p.target)[i] : (int)reinterpret_cast<const int64_t*>(p.target)[i];
             }
         }
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0)
-    {
-        *p.count = all;
-        if (p.backward)
-        {
-            const float one = D == TRIPS_DTYPE_F16 ? 1.f / 32768.f : 1.f;
-            const float g   = p.reduction == TRIPS_REDUCE_NONE ? (top > 0.f ? top : 1.f) : p.reduction == TRIPS_REDUCE_SUM ? p.d_loss[0] : p.d_loss[0] / (float)max(all, 1);
-            p.unscale[0]    = g * one * p.scale;
-            p.unscale[1]    = g * one * fabsf(p.scale);
-        }
+        if (blockIdx.x == 0 && lane == 0) *p.kept.count = all_w[0] + all_w[1] + all_w[2] + all_w[3];
     }
     __syncthreads();
-    for (int r = wave; r < kGatherRows; r += 4)
+    using Wide       = typename Pack<T, V>::type;
+    const int pieces = p.kp / V;
+    for (int q = threadIdx.x; q < kGatherRows * pieces; q += 256)
     {
-        const int at = own_place[r];
+        const int r = q / pieces, c = (q - r * pieces) * V, at = own_place[r];
         if (at < 0) continue;
-        const T* from = reinterpret_cast<const T*>(p.rows) + (first + r) * p.stride;
-        T* to         = reinterpret_cast<T*>(p.packed) + (long long)at * p.kp;
-        for (int c = lane * 8; c < p.kp; c += 512)
+        const T* from = reinterpret_cast<const T*>(p.rows) + (first + r) * p.stride + c;
+        Wide x;
+        if (c + V <= p.channels)
+            x = *reinterpret_cast<const Wide*>(from);
+        else
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = c + e < p.channels ? from[e] : T(0);
+        if (p.negate)
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = negative(x[e]);
+        *reinterpret_cast<Wide*>(reinterpret_cast<T*>(p.kept.packed) + (long long)at * p.kp + c) = x;
+    }
+}
+
+// ---- the loss's gradient ----
+
+// d_ij is held for float16, whose range is short, 2^15 times as large and divided by the largest gradient of a row's loss: probabilities from
+// 2^-29 on are normal numbers then. In the other types it is what it is, or without the gradient where that is the same of all rows.
+template <int D>
+constexpr float kHeld = D == TRIPS_DTYPE_F16 ? 32768.f : 1.f;
+
+// The largest |gradient| of the rows that count, finite ones only: the others are left as they are.
+__global__ __launch_bounds__(1024) void top_kernel(const float* d_loss, const int* place, long long n, float* top)
+{
+    __shared__ float tops[16];
+    float own = 0.f;
+    for (long long i0 = threadIdx.x; i0 < n; i0 += 8192)
+    {
+        float g[8];
+        int at[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = d_loss[min(i0 + e * 1024, n - 1)], at[e] = place[min(i0 + e * 1024, n - 1)];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
         {
-            typename Pack<T, 8>::type x;
-            if (c + 8 <= p.channels)
-                x = *reinterpret_cast<const typename Pack<T, 8>::type*>(from + c);
-            else
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = c + e < p.channels ? from[c + e] : T(0);
-            if (p.scale < 0.f)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = negative(x[e]);
-            *reinterpret_cast<typename Pack<T, 8>::type*>(to + c) = x;
+            const float size = fabsf(g[e]);
+            if (at[e] >= 0 && size <= 3.4028234663852886e38f) own = fmaxf(own, size);
         }
     }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) own = fmaxf(own, __shfl_xor(own, o));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = own;
+    __syncthreads();
+    if (threadIdx.x > 0) return;
+    for (int w = 0; w < 16; ++w) own = fmaxf(own, tops[w]);
+    *top = own > 0.f ? own : 1.f;
+}
+
+struct Upstream
+{
+    const float* d_loss;  // [n] or [1]
+    const float* top;     // float16 and a gradient of each row
+    int reduction;
+    float scale;
+};
+// What a row's probabilities are multiplied by to be held, and what undoes that.
+template <int D>
+__device__ __forceinline__ float held_factor(const Upstream& u, int row)
+{
+    if (u.reduction != TRIPS_REDUCE_NONE) return kHeld<D>;
+    return D == TRIPS_DTYPE_F16 ? u.d_loss[row] / *u.top * kHeld<D> : u.d_loss[row];
+}
+template <int D>
+__device__ __forceinline__ float unheld(const Upstream& u, const int* count)
+{
+    float g = 1.f;
+    if (u.reduction == TRIPS_REDUCE_SUM) g = u.d_loss[0];
+    if (u.reduction == TRIPS_REDUCE_MEAN) g = u.d_loss[0] / (float)max(*count, 1);
+    if (D == TRIPS_DTYPE_F16 && u.reduction == TRIPS_REDUCE_NONE) g = *u.top;
+    return g / kHeld<D>;
 }
 
 // ---- products ----
@@ -226,22 +233,18 @@ enum { LOGITS, PROBS, D_ROWS, D_TABLE, GRADS };
 
 struct ProductParams
 {
-    const void* table;     // the piece's entries
-    const void* packed;    // [count][kp]
-    const int* count;
-    const int* packed_target;
-    const float2* packed_state;  // {largest product, log2 of the sum}
-    const float* packed_factor;
-    const float* unscale;
-    float2* partial;       // LOGITS: [stripes][rows_pad] {largest product, sum of exponentials}
-    float* own_product;    // [rows_pad]
-    void* probs;           // [rows_pad][piece], in the tensors' type
-    float* slabs;          // D_ROWS: [splits][rows_pad][kp]
-    const void* d_rows;    // whether they are wanted
+    const void* table;  // the piece's entries
+    Kept kept;
+    Upstream upstream;
+    float2* partial;     // LOGITS: [tiles of entries][rows_pad] {largest product, sum of exponentials}
+    float* own_product;  // [rows_pad]
+    void* probs;         // [rows_pad][piece], in the tensors' type
+    float* slabs;        // D_ROWS: [splits][rows_pad][kp]
+    const void* d_rows;  // whether they are wanted
     void* d_table;
     long long table_stride, d_table_stride, rows_pad;
-    int held;              // channels that a row of the table holds: those, or with zeros behind them to a multiple of 64
-    int first_entry, in_piece, channels, kp, piece, first_stripe, splits, add;
+    int held;  // channels that a row of the table holds: those, or with zeros behind them to 16 bytes
+    int first_entry, in_piece, channels, kp, piece, first_tile, splits, add;
     float scale_log2;
 };
 
@@ -254,21 +257,22 @@ __device__ __forceinline__ float part_of(float x, float base, float scale_log2) 
 template <typename T>
 __global__ __launch_bounds__(256) void copy_entries_kernel(const T* table, long long stride, T* to, long long entries, int channels, int kp)
 {
-    using Wide          = typename Pack<T, 8>::type;
-    const int pieces    = kp / 8;
+    constexpr int V     = 16 / sizeof(T);
+    using Wide          = typename Pack<T, V>::type;
+    const int pieces    = kp / V;
     const long long all = entries * pieces;
     for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < all; q += (long long)gridDim.x * 256)
     {
         const long long j = q / pieces;
-        const int c       = (int)(q % pieces) * 8;
+        const int c       = (int)(q % pieces) * V;
         const T* from     = table + j * stride + c;
         Wide x;
-        if (c + 8 <= channels)
+        if (c + V <= channels)
             x = *reinterpret_cast<const Wide*>(from);
         else
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = c + e < channels ? from[e] : T(0);
-        *reinterpret_cast<Wide*>(to + q * 8) = x;
+            for (int e = 0; e < V; ++e) x[e] = c + e < channels ? from[e] : T(0);
+        *reinterpret_cast<Wide*>(to + q * V) = x;
     }
 }
 
@@ -475,7 +479,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
     const unsigned lds_at = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % S::WM * S::TM, wn = wave / S::WM * S::TN;
-    const int count = *p.count;
+    const int count = *p.kept.count;
 
     // workgroups as they start go around the eight XCDs: workers by XCD
     const int all = gridDim.x, worker = all % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (all / 8) + blockIdx.x / 8);
@@ -527,7 +531,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
 
     // ---- the loads, ahead ----
     const char* table  = reinterpret_cast<const char*>(p.table);
-    const char* packed = reinterpret_cast<const char*>(p.packed);
+    const char* packed = reinterpret_cast<const char*>(p.kept.packed);
     const char* probs  = reinterpret_cast<const char*>(p.probs);
     Source<S::FIRST_LOADS> first;
     Source<S::SECOND_LOADS> second;
@@ -579,7 +583,13 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                 first.load(i, to, wave);
         }
         else
-            second.load(i - S::FIRST_LOADS, to + S::FIRST_BYTES, wave);
+        {
+            const int q = i - S::FIRST_LOADS;
+            if (KIND != GRADS)
+                second.load(q, to + S::FIRST_BYTES, wave, SecondAlong::piece_of(q, wave, lane) * (16 / SIZE), left);
+            else
+                second.load(q, to + S::FIRST_BYTES, wave);
+        }
     };
     auto loaded_step = [&]()
     {
@@ -673,7 +683,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         for (int j = 0; j < S::FN; ++j)
         {
             const long long n = n0 + wn + j * 32 + (lane & 31);
-            const int own     = n < count ? p.packed_target[n] - p.first_entry - m_lane : -1;  // (of the lane's own elements)
+            const int own     = n < count ? p.kept.target[n] - p.first_entry - m_lane : -1;  // (of the lane's own elements)
             float top         = -__builtin_inff();
             if (m0 + S::BM > p.in_piece)
                 each_element<S::FM>([&](int i, int e, int m)
@@ -710,7 +720,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             const float base = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
             for (int w = 0; w < S::WM; ++w) sum += joined[w * S::BN + n].y * part_of(joined[w * S::BN + n].x, base, p.scale_log2);
-            p.partial[(p.first_stripe + u.x) * p.rows_pad + n0 + n] = make_float2(top, sum);
+            p.partial[(p.first_tile + u.x) * p.rows_pad + n0 + n] = make_float2(top, sum);
         }
     };
     auto written = [&](auto mode, const Unit& u)
@@ -718,7 +728,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         constexpr int MODE = decltype(mode)::value;
         const long long n0 = (long long)u.y * S::BN;
         const int m0 = u.x * S::BM, m_lane = m0 + wm + 4 * (lane >> 5);
-        const float unscale = MODE == D_TABLE ? p.unscale[1] : 1.f;
+        const float unscale = MODE == D_TABLE ? unheld<D>(p.upstream, p.kept.count) * fabsf(p.upstream.scale) : 1.f;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
         {
@@ -728,7 +738,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                 float2 state = make_float2(0.f, 0.f);
                 float factor = 0.f;
                 int own      = -1;
-                if (n < count) state = p.packed_state[n], factor = p.packed_factor[n], own = p.packed_target[n] - p.first_entry - m_lane;
+                if (n < count) state = p.kept.state[n], factor = held_factor<D>(p.upstream, p.upstream.reduction == TRIPS_REDUCE_NONE ? p.kept.row[n] : 0), own = p.kept.target[n] - p.first_entry - m_lane;
                 each_element<S::FM>([&](int i, int e, int)
                                     { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - state.x, p.scale_log2, -state.y)) * factor; });
                 if (__any(own >= 0 && own < S::TM))
@@ -850,18 +860,16 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
 
 // ---- joins ----
 
-// 1 << lanes_log2 lanes a row over the stripes of tiles: state and loss, and the workgroup's sum of losses.
+// 1 << lanes_log2 lanes a row over the tiles: state and loss, and the workgroup's sum of losses.
 struct JoinParams
 {
     const float2* partial;
     const float* own_product;
-    const int* place;
-    const int* count;
+    Kept kept;
     float* loss;
-    float2* state;
     double* sums;
     long long n, rows_pad;
-    int stripes, reduction, lanes_log2;
+    int tiles, reduction, lanes_log2;
     float scale, scale_log2;
 };
 __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
@@ -870,13 +878,13 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
     __shared__ double sums[4];
     const int rows_log2 = 8 - p.lanes_log2, row = threadIdx.x & ((1 << rows_log2) - 1), lanes = 1 << p.lanes_log2;
     const long long i = ((long long)blockIdx.x << rows_log2) + row;
-    const int at      = i < p.n ? p.place[i] : -1;
+    const int at      = i < p.n ? p.kept.place[i] : -1;
     float2 own        = make_float2(-__builtin_inff(), 0.f);
     if (at >= 0)
     {
         const float product = p.own_product[at];
 #pragma unroll 4
-        for (int s = threadIdx.x >> rows_log2; s < p.stripes; s += lanes)
+        for (int s = threadIdx.x >> rows_log2; s < p.tiles; s += lanes)
         {
             const float2 x  = p.partial[s * p.rows_pad + at];
             const float top = fmaxf(own.x, x.x), base = top == -__builtin_inff() ? 0.f : top;
@@ -903,11 +911,8 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
             loss    = (float)(((double)top - (double)own.y) * (double)p.scale + log * kLog2);
             log_sum = (float)log;
         }
-        if (i < p.n)
-        {
-            p.state[i] = make_float2(at >= 0 ? top : 0.f, log_sum);
-            if (p.reduction == TRIPS_REDUCE_NONE) p.loss[i] = loss;
-        }
+        if (at >= 0) p.kept.state[at] = make_float2(top, log_sum);
+        if (i < p.n && p.reduction == TRIPS_REDUCE_NONE) p.loss[i] = loss;
     }
     if (p.reduction == TRIPS_REDUCE_NONE) return;
     double sum = (double)loss;
@@ -919,7 +924,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
     {
         sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
         if (gridDim.x == 1)
-            *p.loss = (float)(p.reduction == TRIPS_REDUCE_MEAN ? sum / (double)max(*p.count, 1) : sum);
+            *p.loss = (float)(p.reduction == TRIPS_REDUCE_MEAN ? sum / (double)max(*p.kept.count, 1) : sum);
         else
             p.sums[blockIdx.x] = sum;
     }
@@ -943,20 +948,20 @@ __global__ __launch_bounds__(1024) void sum_kernel(const double* from, int n, co
 
 // d_rows: the splits' sums, in their order, at their rows' own places; four channels a lane.
 template <int D>
-__global__ __launch_bounds__(256) void rows_out_kernel(const float* slabs, const int* place, const float* unscale, void* d_rows, long long n, long long rows_pad,
+__global__ __launch_bounds__(256) void rows_out_kernel(const float* slabs, const Kept kept, const Upstream upstream, void* d_rows, long long n, long long rows_pad,
                                                        long long stride, int channels, int kp, int splits)
 {
     using E  = Element<D>;
     using T  = typename E::type;
     using F4 = Pack<float, 4>::type;
     using T4 = typename Pack<T, 4>::type;
-    const float f       = *unscale;
+    const float f       = unheld<D>(upstream, kept.count) * upstream.scale;
     const int quads     = (channels + 3) >> 2;
     const long long all = n * quads, slab = rows_pad * kp;
     for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < all; q += (long long)gridDim.x * 256)
     {
         const long long i = q / quads;
-        const int c = (int)(q - i * quads) * 4, at = place[i];
+        const int c = (int)(q - i * quads) * 4, at = kept.place[i];
         F4 sum = {0.f, 0.f, 0.f, 0.f};
         if (at >= 0)
         {
@@ -994,13 +999,46 @@ bool rows_in_place(const TripsTableLossDesc& d)
     return d.num_channels * size % 16 == 0 && d.table_stride * size % 16 == 0 && d.table_stride < 1 << 20;
 }
 
+int packed_channels(const TripsTableLossDesc& d)
+{
+    const int v = 16 / dtype_bytes(d.dtype);
+    return (d.num_channels + v - 1) / v * v;
+}
+
+struct Taker
+{
+    size_t at = 0;
+    size_t operator()(size_t bytes)
+    {
+        const size_t here = at;
+        at += (bytes + 255) & ~(size_t)255;
+        return here;
+    }
+};
+
+// Where what is kept lies; its size where kept is NULL.
+size_t kept_of(const TripsTableLossDesc& d, void* kept, Kept* k)
+{
+    Taker take;
+    char* at = reinterpret_cast<char*>(kept);
+    Kept got;
+    got.count  = (int*)(at + take(4));
+    got.place  = (int*)(at + take(d.num_rows * 4));
+    got.row    = (int*)(at + take(d.num_rows * 4));
+    got.target = (int*)(at + take(d.num_rows * 4));
+    got.state  = (float2*)(at + take(d.num_rows * 8));
+    got.packed = at + take((size_t)d.num_rows * packed_channels(d) * dtype_bytes(d.dtype));
+    if (k) *k = got;
+    return take.at;
+}
+
 // Steps of a call over the table; what each takes of the workspace.
 struct Layout
 {
     int64_t rows_pad, chunks, piece, pieces;
-    int kp, stripes, splits;
+    int kp, tiles, splits;
     bool copies;
-    size_t packed, place, target, state, factor, count, chunk_count, chunk_top, partial, own_product, sums, probs, slabs, copy, bytes;
+    size_t chunk_count, top, partial, own_product, sums, probs, slabs, copy, bytes;
 };
 
 using Big   = Shape<256, 256, 2, 4, 2, 1>;
@@ -1072,21 +1110,11 @@ int splits_of(const TripsTableLossDesc& d, int64_t rows_pad, int64_t piece, int 
 Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
 {
     Layout l{};
-    const int size       = dtype_bytes(d.dtype);
-    l.rows_pad           = up(d.num_rows, 256), l.chunks = d.num_rows > kCountedBy ? up(d.num_rows, kChunk) / kChunk : 0;
-    l.kp                 = (int)up(d.num_channels, 64);
-    l.copies             = copies;
-    size_t at            = 0;
-    auto take            = [&](size_t bytes)
-    {
-        const size_t here = at;
-        at += (bytes + 255) & ~(size_t)255;
-        return here;
-    };
-    l.count  = take(256);
-    l.packed = take((size_t)d.num_rows * l.kp * size);
-    l.place = take(d.num_rows * 4), l.target = take(d.num_rows * 4);
-    l.chunk_count = take(l.chunks * 4), l.chunk_top = take(l.chunks * 4);
+    const int size = dtype_bytes(d.dtype);
+    l.rows_pad = up(d.num_rows, 256), l.chunks = d.num_rows > kCountedBy ? up(d.num_rows, kChunk) / kChunk : 0;
+    l.kp     = packed_channels(d);
+    l.copies = copies;
+    Taker take;
     int64_t most = up(std::max<int64_t>(d.num_entries, 1), 256);
     if (copies)
     {
@@ -1098,19 +1126,20 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     l.piece  = up((d.num_entries + l.pieces - 1) / l.pieces, 256);
     if (!backward)
     {
-        l.stripes     = (int)(l.piece / entries_of_tile(d));
-        l.partial     = take((size_t)l.stripes * l.pieces * l.rows_pad * sizeof(float2));
+        l.chunk_count = take(l.chunks * 4);
+        l.tiles       = (int)(l.piece / entries_of_tile(d));
+        l.partial     = take((size_t)l.tiles * l.pieces * l.rows_pad * sizeof(float2));
         l.own_product = take(l.rows_pad * 4);
         l.sums        = take((d.num_rows / 4 + 1) * 8);
     }
     else
     {
-        l.state = take(d.num_rows * 8), l.factor = take(d.num_rows * 4);
+        l.top   = take(4);
         l.probs = take((size_t)l.rows_pad * l.piece * size);
         l.splits = splits_of(d, l.rows_pad, l.piece, l.kp);
         l.slabs  = take((size_t)l.splits * l.rows_pad * l.kp * 4);
     }
-    l.bytes = at;
+    l.bytes = take.at;
     return l;
 }
 
@@ -1127,33 +1156,30 @@ size_t workspace_of(const TripsTableLossDesc& d, bool backward)
 float scale_log2(const TripsTableLossDesc& d) { return std::max((float)(std::fabs((double)d.scale) * kLog2e), 1.2e-38f); }
 
 template <int D>
-hipError_t gather(const TripsTableLossDesc& d, const Layout& l, const void* rows, const void* target, bool backward, const float* d_loss, const float* state, char* w, hipStream_t stream, Profiler* prof)
+hipError_t gather(const TripsTableLossDesc& d, const Layout& l, const void* rows, const void* target, const Kept& kept, char* w, hipStream_t stream, Profiler* prof)
 {
     GatherParams p{};
-    p.rows = rows, p.target = target, p.d_loss = d_loss, p.state = (const float2*)state;
-    p.packed = w + l.packed, p.place = (int*)(w + l.place), p.packed_target = (int*)(w + l.target);
-    p.packed_state = (float2*)(w + l.state), p.packed_factor = (float*)(w + l.factor);
-    p.count = (int*)(w + l.count), p.unscale = (float*)(w + l.count) + 2;
+    p.rows = rows, p.target = target, p.kept = kept;
     p.n = d.num_rows, p.entries = d.num_entries, p.stride = d.rows_stride;
-    p.channels = d.num_channels, p.kp = l.kp, p.i32 = d.index_dtype == TRIPS_INDEX_I32, p.reduction = d.reduction, p.backward = backward, p.scale = d.scale;
+    p.channels = d.num_channels, p.kp = l.kp, p.negate = d.scale < 0.f;
+    const bool i32 = d.index_dtype == TRIPS_INDEX_I32;
     if (l.chunks)
     {
-        p.chunk_count = (int*)(w + l.chunk_count), p.chunk_top = (float*)(w + l.chunk_top);
+        int* chunk_count = (int*)(w + l.chunk_count);
+        p.chunk_count    = chunk_count;
         ProfScope scope(prof, "loss_count", stream);
-        (p.i32 ? count_kernel<true> : count_kernel<false>)<<<(unsigned)l.chunks, 256, 0, stream>>>(target, d.reduction == TRIPS_REDUCE_NONE ? d_loss : nullptr, d.num_rows, d.num_entries,
-                                                                                                  (int*)(w + l.chunk_count), (float*)(w + l.chunk_top));
+        (i32 ? count_kernel<true> : count_kernel<false>)<<<(unsigned)l.chunks, 256, 0, stream>>>(target, d.num_rows, d.num_entries, chunk_count);
         if (hipError_t e = hipGetLastError()) return e;
     }
     ProfScope scope(prof, "loss_gather", stream);
-    (p.i32 ? gather_kernel<D, true> : gather_kernel<D, false>)<<<std::max(1u, (unsigned)((d.num_rows + kGatherRows - 1) / kGatherRows)), 256, 0, stream>>>(p);
+    (i32 ? gather_kernel<D, true> : gather_kernel<D, false>)<<<std::max(1u, (unsigned)((d.num_rows + kGatherRows - 1) / kGatherRows)), 256, 0, stream>>>(p);
     return hipGetLastError();
 }
 
-ProductParams product_params(const TripsTableLossDesc& d, const Layout& l, char* w)
+ProductParams product_params(const TripsTableLossDesc& d, const Layout& l, const Kept& kept, char* w)
 {
     ProductParams p{};
-    p.packed = w + l.packed, p.count = (int*)(w + l.count), p.packed_target = (int*)(w + l.target);
-    p.packed_state = (float2*)(w + l.state), p.packed_factor = (float*)(w + l.factor), p.unscale = (float*)(w + l.count) + 2;
+    p.kept = kept;
     p.partial = (float2*)(w + l.partial), p.own_product = (float*)(w + l.own_product), p.probs = w + l.probs, p.slabs = (float*)(w + l.slabs);
     p.d_table_stride = d.d_table_stride, p.rows_pad = l.rows_pad;
     p.channels = d.num_channels, p.kp = l.kp, p.piece = (int)l.piece, p.splits = l.splits;
@@ -1168,13 +1194,13 @@ hipError_t take_piece(const TripsTableLossDesc& d, const Layout& l, int64_t piec
     using T          = typename Element<D>::type;
     const T* entries = reinterpret_cast<const T*>(table) + piece * l.piece * d.table_stride;
     p.first_entry = (int)(piece * l.piece), p.in_piece = (int)std::min(l.piece, d.num_entries - piece * l.piece);
-    p.first_stripe = (int)(piece * l.stripes), p.add = piece > 0;
+    p.first_tile = (int)(piece * l.tiles), p.add = piece > 0;
     p.table = entries, p.table_stride = d.table_stride, p.held = d.num_channels;
     p.d_table = d_table ? reinterpret_cast<T*>(d_table) + piece * l.piece * d.d_table_stride : nullptr;
     if (!l.copies) return hipSuccess;
     p.table = w + l.copy, p.table_stride = p.held = l.kp;
     ProfScope scope(prof, "loss_copy", stream);
-    const int64_t pieces = (int64_t)p.in_piece * l.kp / 8;
+    const int64_t pieces = (int64_t)p.in_piece * l.kp * (int64_t)sizeof(T) / 16;
     copy_entries_kernel<T><<<(unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 16), 256, 0, stream>>>(entries, d.table_stride, reinterpret_cast<T*>(w + l.copy), p.in_piece,
                                                                                                           d.num_channels, l.kp);
     return hipGetLastError();
@@ -1196,11 +1222,11 @@ hipError_t launch_product(const TripsTableLossDesc& d, const ProductParams& p, h
 }
 
 template <int D>
-hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* table, const void* target, float* loss, float* state, char* w, hipStream_t stream, Profiler* prof)
+hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* table, const void* target, float* loss, const Kept& kept, char* w, hipStream_t stream, Profiler* prof)
 {
     const Layout l = layout_of(d, false, copies_of(d, table));
-    if (hipError_t e = gather<D>(d, l, rows, target, false, nullptr, nullptr, w, stream, prof)) return e;
-    ProductParams p = product_params(d, l, w);
+    if (hipError_t e = gather<D>(d, l, rows, target, kept, w, stream, prof)) return e;
+    ProductParams p = product_params(d, l, kept, w);
     int64_t piece   = 0;
     for (; piece * l.piece < d.num_entries; ++piece)
     {
@@ -1208,10 +1234,12 @@ hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* ta
         if (hipError_t e = launch_product<D, LOGITS>(d, p, stream, prof)) return e;
     }
     JoinParams j{};
-    j.partial = p.partial, j.own_product = p.own_product, j.place = (int*)(w + l.place), j.count = p.count;
-    j.loss = loss, j.state = (float2*)state, j.scale = std::fabs(d.scale), j.scale_log2 = p.scale_log2, j.sums = (double*)(w + l.sums);
-    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.stripes = (int)tiles_of(d.num_entries, entries_of_tile(d)), j.reduction = d.reduction;
-    while (j.lanes_log2 < 6 && 8 << j.lanes_log2 < j.stripes) ++j.lanes_log2;
+    j.partial = p.partial, j.own_product = p.own_product, j.kept = kept;
+    j.loss = loss, j.scale = std::fabs(d.scale), j.scale_log2 = p.scale_log2, j.sums = (double*)(w + l.sums);
+    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.tiles = (int)tiles_of(d.num_entries, entries_of_tile(d)), j.reduction = d.reduction;
+    while (j.lanes_log2 < 6 && 8 << j.lanes_log2 < j.tiles) ++j.lanes_log2;
+    // (the rows of few in one workgroup, whose sum is the loss then)
+    while (j.lanes_log2 > 2 && d.num_rows > 256 >> j.lanes_log2 && d.num_rows <= 64) --j.lanes_log2;
     const int64_t rows_each = 256 >> j.lanes_log2, groups = std::max<int64_t>(1, (d.num_rows + rows_each - 1) / rows_each);
     {
         ProfScope scope(prof, "loss_join", stream);
@@ -1220,18 +1248,23 @@ hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* ta
     }
     if (d.reduction == TRIPS_REDUCE_NONE || groups == 1) return hipSuccess;
     ProfScope scope(prof, "loss_sum", stream);
-    sum_kernel<<<1, 1024, 0, stream>>>(j.sums, (int)groups, j.count, d.reduction, loss);
+    sum_kernel<<<1, 1024, 0, stream>>>(j.sums, (int)groups, kept.count, d.reduction, loss);
     return hipGetLastError();
 }
 
 template <int D>
-hipError_t backward(const TripsTableLossDesc& d, const void* rows, const void* table, const void* target, const float* state, const float* d_loss, void* d_rows, void* d_table, char* w,
-                    hipStream_t stream, Profiler* prof)
+hipError_t backward(const TripsTableLossDesc& d, const void* table, const Kept& kept, const float* d_loss, void* d_rows, void* d_table, char* w, hipStream_t stream, Profiler* prof)
 {
-    const Layout l = layout_of(d, true, copies_of(d, table));
-    if (hipError_t e = gather<D>(d, l, rows, target, true, d_loss, state, w, stream, prof)) return e;
-    ProductParams p = product_params(d, l, w);
+    const Layout l  = layout_of(d, true, copies_of(d, table));
+    ProductParams p = product_params(d, l, kept, w);
     p.d_rows        = d_rows;
+    p.upstream      = Upstream{d_loss, (float*)(w + l.top), d.reduction, d.scale};
+    if (D == TRIPS_DTYPE_F16 && d.reduction == TRIPS_REDUCE_NONE && d.num_rows > 0)
+    {
+        ProfScope scope(prof, "loss_top", stream);
+        top_kernel<<<1, 1024, 0, stream>>>(d_loss, kept.place, d.num_rows, (float*)(w + l.top));
+        if (hipError_t e = hipGetLastError()) return e;
+    }
     for (int64_t piece = 0; piece * l.piece < d.num_entries; ++piece)
     {
         if (hipError_t e = take_piece<D>(d, l, piece, table, d_table, w, p, stream, prof)) return e;
@@ -1240,8 +1273,8 @@ hipError_t backward(const TripsTableLossDesc& d, const void* rows, const void* t
     }
     if (!d_rows || d.num_rows == 0) return hipSuccess;
     ProfScope scope(prof, "loss_rows_out", stream);
-    rows_out_kernel<D><<<(unsigned)std::min<int64_t>((d.num_rows * ((d.num_channels + 3) / 4) + 255) / 256, 1 << 16), 256, 0, stream>>>((float*)(w + l.slabs), (int*)(w + l.place), p.unscale, d_rows, d.num_rows, l.rows_pad, d.d_rows_stride,
-                                                                           d.num_channels, l.kp, l.splits);
+    rows_out_kernel<D><<<(unsigned)std::min<int64_t>((d.num_rows * ((d.num_channels + 3) / 4) + 255) / 256, 1 << 16), 256, 0, stream>>>(
+        (float*)(w + l.slabs), kept, p.upstream, d_rows, d.num_rows, l.rows_pad, d.d_rows_stride, d.num_channels, l.kp, l.splits);
     return hipGetLastError();
 }
 
@@ -1273,18 +1306,24 @@ int check_pointer(const char* name, const void* p, size_t align, bool needed)
     return TRIPS_OK;
 }
 
-int check_call(TripsCtx* ctx, const TripsTableLossDesc* d, bool backward, const void* rows, const void* table, const void* target, const void* workspace, size_t bytes)
+int check_call(TripsCtx* ctx, const TripsTableLossDesc* d, bool backward, const void* table, const void* kept, size_t kept_bytes, const void* workspace, size_t bytes)
 {
     if (!ctx) return set_error(TRIPS_ERR_INVALID_ARG, "ctx is NULL");
     if (int e = check_desc(d)) return e;
-    const size_t size = dtype_bytes(d->dtype);
-    if (int e = check_pointer("rows", rows, size, d->num_rows > 0)) return e;
-    if (int e = check_pointer("table", table, size, d->num_entries > 0)) return e;
-    if (int e = check_pointer("target", target, d->index_dtype == TRIPS_INDEX_I32 ? 4 : 8, d->num_rows > 0)) return e;
+    if (int e = check_pointer("table", table, dtype_bytes(d->dtype), d->num_entries > 0)) return e;
+    if (!kept || !aligned(kept, 256)) return set_error(TRIPS_ERR_INVALID_ARG, "kept must be a 256-byte aligned device pointer");
+    if (kept_bytes < kept_of(*d, nullptr, nullptr)) return set_error(TRIPS_ERR_WORKSPACE_SMALL, "kept has %zu bytes, %zu needed", kept_bytes, kept_of(*d, nullptr, nullptr));
     if (!workspace || !aligned(workspace, 256)) return set_error(TRIPS_ERR_INVALID_ARG, "workspace must be a 256-byte aligned device pointer");
     const size_t need = workspace_of(*d, backward);
     if (bytes < need) return set_error(TRIPS_ERR_WORKSPACE_SMALL, "workspace has %zu bytes, %zu needed", bytes, need);
     return TRIPS_OK;
+}
+
+template <typename F>
+int with_dtype(int dtype, F f)
+{
+    if (dtype == TRIPS_DTYPE_F32) return f(std::integral_constant<int, TRIPS_DTYPE_F32>{});
+    return dtype == TRIPS_DTYPE_BF16 ? f(std::integral_constant<int, TRIPS_DTYPE_BF16>{}) : f(std::integral_constant<int, TRIPS_DTYPE_F16>{});
 }
 }  // namespace
 }  // namespace trips
@@ -1292,6 +1331,14 @@ int check_call(TripsCtx* ctx, const TripsTableLossDesc* d, bool backward, const 
 using namespace trips;
 
 extern "C" {
+
+int trips_table_loss_kept_size(const TripsTableLossDesc* desc, size_t* bytes)
+{
+    if (!bytes) return set_error(TRIPS_ERR_INVALID_ARG, "bytes is NULL");
+    if (int e = check_desc(desc)) return e;
+    *bytes = kept_of(*desc, nullptr, nullptr);
+    return TRIPS_OK;
+}
 
 int trips_table_loss_workspace_size(const TripsTableLossDesc* desc, int backward, size_t* bytes)
 {
@@ -1301,26 +1348,29 @@ int trips_table_loss_workspace_size(const TripsTableLossDesc* desc, int backward
     return TRIPS_OK;
 }
 
-int trips_table_loss_forward(TripsCtx* ctx, const TripsTableLossDesc* desc, const void* rows, const void* table, const void* target,
-                             float* loss, float* state, void* workspace, size_t workspace_bytes, void* stream)
+int trips_table_loss_forward(TripsCtx* ctx, const TripsTableLossDesc* desc, const void* rows, const void* table, const void* target, float* loss,
+                             void* kept, size_t kept_bytes, void* workspace, size_t workspace_bytes, void* stream)
 {
-    if (int e = check_call(ctx, desc, false, rows, table, target, workspace, workspace_bytes)) return e;
+    if (int e = check_call(ctx, desc, false, table, kept, kept_bytes, workspace, workspace_bytes)) return e;
+    if (int e = check_pointer("rows", rows, dtype_bytes(desc->dtype), desc->num_rows > 0)) return e;
+    if (int e = check_pointer("target", target, desc->index_dtype == TRIPS_INDEX_I32 ? 4 : 8, desc->num_rows > 0)) return e;
     if (int e = check_pointer("loss", loss, 4, desc->num_rows > 0 || desc->reduction != TRIPS_REDUCE_NONE)) return e;
-    if (int e = check_pointer("state", state, 8, desc->num_rows > 0)) return e;
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_error(scope.error, "hipSetDevice");
-    const auto call    = desc->dtype == TRIPS_DTYPE_F32 ? forward<TRIPS_DTYPE_F32> : desc->dtype == TRIPS_DTYPE_BF16 ? forward<TRIPS_DTYPE_BF16> : forward<TRIPS_DTYPE_F16>;
-    const hipError_t e = call(*desc, rows, table, target, loss, state, (char*)workspace, reinterpret_cast<hipStream_t>(stream), profiler(ctx));
-    return e == hipSuccess ? TRIPS_OK : hip_error(e, "table loss launch");
+    Kept k;
+    kept_of(*desc, kept, &k);
+    return with_dtype(desc->dtype, [&](auto dtype)
+    {
+        const hipError_t e = forward<decltype(dtype)::value>(*desc, rows, table, target, loss, k, (char*)workspace, reinterpret_cast<hipStream_t>(stream), profiler(ctx));
+        return e == hipSuccess ? (int)TRIPS_OK : hip_error(e, "table loss launch");
+    });
 }
 
-int trips_table_loss_backward(TripsCtx* ctx, const TripsTableLossDesc* desc, const void* rows, const void* table, const void* target,
-                              const float* state, const float* d_loss, void* d_rows, void* d_table, void* workspace, size_t workspace_bytes,
-                              void* stream)
+int trips_table_loss_backward(TripsCtx* ctx, const TripsTableLossDesc* desc, const void* table, const void* kept, size_t kept_bytes, const float* d_loss,
+                              void* d_rows, void* d_table, void* workspace, size_t workspace_bytes, void* stream)
 {
-    if (int e = check_call(ctx, desc, true, rows, table, target, workspace, workspace_bytes)) return e;
+    if (int e = check_call(ctx, desc, true, table, kept, kept_bytes, workspace, workspace_bytes)) return e;
     const size_t size = dtype_bytes(desc->dtype);
-    if (int e = check_pointer("state", state, 8, desc->num_rows > 0)) return e;
     if (int e = check_pointer("d_loss", d_loss, 4, desc->num_rows > 0 || desc->reduction != TRIPS_REDUCE_NONE)) return e;
     if (int e = check_pointer("d_rows", d_rows, size, false)) return e;
     if (int e = check_pointer("d_table", d_table, size, false)) return e;
@@ -1331,9 +1381,13 @@ int trips_table_loss_backward(TripsCtx* ctx, const TripsTableLossDesc* desc, con
     if (!d_rows && !d_table) return TRIPS_OK;
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_error(scope.error, "hipSetDevice");
-    const auto call    = desc->dtype == TRIPS_DTYPE_F32 ? backward<TRIPS_DTYPE_F32> : desc->dtype == TRIPS_DTYPE_BF16 ? backward<TRIPS_DTYPE_BF16> : backward<TRIPS_DTYPE_F16>;
-    const hipError_t e = call(*desc, rows, table, target, state, d_loss, d_rows, d_table, (char*)workspace, reinterpret_cast<hipStream_t>(stream), profiler(ctx));
-    return e == hipSuccess ? TRIPS_OK : hip_error(e, "table loss launch");
+    Kept k;
+    kept_of(*desc, const_cast<void*>(kept), &k);  // (only read here)
+    return with_dtype(desc->dtype, [&](auto dtype)
+    {
+        const hipError_t e = backward<decltype(dtype)::value>(*desc, table, k, d_loss, d_rows, d_table, (char*)workspace, reinterpret_cast<hipStream_t>(stream), profiler(ctx));
+        return e == hipSuccess ? (int)TRIPS_OK : hip_error(e, "table loss launch");
+    });
 }
 
 }  // extern "C"

@@ -1,8 +1,10 @@
 // The host side of trips_amd/adamw.py, lookup.py, table_loss.py and dropout.py: what the C ABI takes of each tensor, collected from the objects
 // that torch keeps. In Python a tensor's score of attributes and checks took 1.3 to 2 us, more than its share of the kernels'
 // time in a step over a net (18 tensors 32 us a step and 17 so, 40 with copies 68 and 29), and a lookup 10 us.
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <string>
@@ -192,7 +194,9 @@ class NormTable
 
 void check(int rc)
 {
-    if (rc != TRIPS_OK) py::module_::import("trips_amd._lib").attr("check")(rc);
+    if (rc == TRIPS_OK) return;
+    py::gil_scoped_acquire gil;  // (a backward pass runs without it)
+    py::module_::import("trips_amd._lib").attr("check")(rc);
 }
 
 int index_dtype_of(const at::Tensor& index)
@@ -329,84 +333,176 @@ at::Tensor lookup_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& gr
 
 // ---- a table's cross entropy ----
 
-TripsTableLossDesc loss_desc(const at::Tensor& rows, const at::Tensor& table, const at::Tensor& target, float scale, int reduction)
+int64_t stream_of(const at::Tensor& t) { return (int64_t)(uintptr_t)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+TripsTableLossDesc loss_desc(const at::Tensor& table, int64_t rows, double scale, int64_t reduction)
 {
     TripsTableLossDesc d{};
-    d.abi_version = TRIPS_ABI_VERSION, d.dtype = dtype_of(rows), d.index_dtype = index_dtype_of(target), d.reduction = reduction, d.scale = scale;
-    if (table.scalar_type() != rows.scalar_type() || table.size(1) != rows.size(1))
-        throw py::value_error("rows and table: matrices of one type and as many channels expected, got " + std::to_string(rows.size(1)) + " and " + std::to_string(table.size(1)) + " channels");
-    if (target.numel() != rows.size(0)) throw py::value_error("target: " + std::to_string(target.numel()) + " entries for " + std::to_string(rows.size(0)) + " rows");
-    d.num_rows = rows.size(0), d.num_entries = table.size(0), d.num_channels = (int32_t)std::min<int64_t>(rows.size(1), INT32_MAX);
+    d.abi_version = TRIPS_ABI_VERSION, d.dtype = dtype_of(table), d.reduction = (int32_t)reduction, d.scale = (float)scale;
+    d.num_rows = rows, d.num_entries = table.size(0), d.num_channels = (int32_t)std::min<int64_t>(table.size(1), INT32_MAX);
     return d;
 }
 
-// {loss, state}
-std::pair<at::Tensor, at::Tensor> table_loss(uintptr_t ctx, uintptr_t stream, const at::Tensor& rows, const at::Tensor& table, const at::Tensor& target, float scale, int reduction)
+// {loss, what the gradients need}
+std::pair<at::Tensor, at::Tensor> table_loss(int64_t ctx, int64_t stream, const at::Tensor& rows, const at::Tensor& table, const at::Tensor& target, double scale, int64_t reduction)
 {
-    index_dtype_of(target);
+    const int index_dtype = index_dtype_of(target);
     int64_t rows_stride, table_stride;
     const at::Tensor x = rows_of("rows", rows, target, rows_stride), w = rows_of("table", table, target, table_stride);
-    TripsTableLossDesc d = loss_desc(x, w, target, scale, reduction);
-    d.rows_stride = rows_stride, d.table_stride = table_stride;
-    size_t need = 0;
+    if (w.scalar_type() != x.scalar_type() || w.size(1) != x.size(1))
+        throw py::value_error("rows and table: matrices of one type and as many channels expected, got " + std::to_string(x.size(1)) + " and " + std::to_string(w.size(1)) + " channels");
+    if (target.numel() != x.size(0)) throw py::value_error("target: " + std::to_string(target.numel()) + " entries for " + std::to_string(x.size(0)) + " rows");
+    TripsTableLossDesc d = loss_desc(w, x.size(0), scale, reduction);
+    d.index_dtype = index_dtype, d.rows_stride = rows_stride, d.table_stride = table_stride;
+    size_t need = 0, keep = 0;
     check(trips_table_loss_workspace_size(&d, 0, &need));
+    check(trips_table_loss_kept_size(&d, &keep));
     const auto options = x.options().dtype(at::kFloat).requires_grad(false);
-    at::Tensor loss = reduction == TRIPS_REDUCE_NONE ? torch::empty({d.num_rows}, options) : torch::empty({}, options), state = torch::empty({d.num_rows, 2}, options);
+    at::Tensor loss = reduction == TRIPS_REDUCE_NONE ? torch::empty({d.num_rows}, options) : torch::empty({}, options), kept = bytes(keep, x);
     const at::Tensor workspace = bytes(need, x), t = target.contiguous();
-    check(trips_table_loss_forward(reinterpret_cast<TripsCtx*>(ctx), &d, x.data_ptr(), w.data_ptr(), t.data_ptr(), (float*)loss.data_ptr(), (float*)state.data_ptr(), data(workspace), need,
+    check(trips_table_loss_forward(reinterpret_cast<TripsCtx*>(ctx), &d, x.data_ptr(), w.data_ptr(), t.data_ptr(), (float*)loss.data_ptr(), kept.data_ptr(), keep, data(workspace), need,
                                    reinterpret_cast<void*>(stream)));
-    return {loss, state};
+    return {loss, kept};
 }
 
-// {d_rows, d_table}, where they are asked for
-std::pair<std::optional<at::Tensor>, std::optional<at::Tensor>> table_loss_backward(uintptr_t ctx, uintptr_t stream, const at::Tensor& d_loss, const at::Tensor& rows,
-                                                                                    const at::Tensor& table, const at::Tensor& target, const at::Tensor& state, float scale, int reduction,
-                                                                                    bool want_rows, bool want_table)
+// {d_rows, d_table}, undefined where they are not asked for
+std::pair<at::Tensor, at::Tensor> table_loss_gradients(int64_t ctx, int64_t stream, const at::Tensor& d_loss, const at::Tensor& table, const at::Tensor& kept, int64_t rows, double scale,
+                                                       int64_t reduction, bool want_rows, bool want_table)
 {
-    index_dtype_of(target);
-    int64_t rows_stride, table_stride;
-    const at::Tensor x = rows_of("rows", rows, target, rows_stride), w = rows_of("table", table, target, table_stride);
-    TripsTableLossDesc d = loss_desc(x, w, target, scale, reduction);
+    int64_t table_stride;
+    const at::Tensor w   = rows_of("table", table, kept, table_stride);
+    TripsTableLossDesc d = loss_desc(w, rows, scale, reduction);
     const int64_t losses = reduction == TRIPS_REDUCE_NONE ? d.num_rows : 1;
-    if (d_loss.scalar_type() != at::kFloat || d_loss.numel() != losses || d_loss.device() != x.device())
+    if (d_loss.scalar_type() != at::kFloat || d_loss.numel() != losses || d_loss.device() != w.device())
         throw py::value_error("the loss's gradient: " + std::to_string(losses) + " float32 numbers on the rows' device expected");
-    if (state.scalar_type() != at::kFloat || state.numel() != 2 * d.num_rows || state.device() != x.device() || !state.is_contiguous()) throw py::value_error("state is not what the loss left");
-    d.rows_stride = rows_stride, d.table_stride = table_stride, d.d_rows_stride = d.d_table_stride = d.num_channels;
-    const auto options = x.options().requires_grad(false);
-    std::optional<at::Tensor> d_rows, d_table;
+    if (kept.scalar_type() != at::kByte || !kept.is_contiguous()) throw py::value_error("kept is not what the loss left");
+    d.table_stride = table_stride, d.d_rows_stride = d.d_table_stride = d.num_channels;
+    const auto options = w.options().requires_grad(false);
+    at::Tensor d_rows, d_table;
     if (want_rows) d_rows = torch::empty({d.num_rows, d.num_channels}, options);
     if (want_table) d_table = torch::empty({d.num_entries, d.num_channels}, options);
     size_t need = 0;
     check(trips_table_loss_workspace_size(&d, 1, &need));
-    const at::Tensor workspace = bytes(need, x), t = target.contiguous(), g = d_loss.contiguous();
-    check(trips_table_loss_backward(reinterpret_cast<TripsCtx*>(ctx), &d, x.data_ptr(), w.data_ptr(), t.data_ptr(), (const float*)state.data_ptr(), (const float*)g.data_ptr(),
-                                    d_rows ? d_rows->data_ptr() : nullptr, d_table ? d_table->data_ptr() : nullptr, data(workspace), need, reinterpret_cast<void*>(stream)));
+    const at::Tensor workspace = bytes(need, w), g = d_loss.contiguous();
+    check(trips_table_loss_backward(reinterpret_cast<TripsCtx*>(ctx), &d, w.data_ptr(), kept.data_ptr(), kept.nbytes(), (const float*)g.data_ptr(), data(d_rows), data(d_table),
+                                    data(workspace), need, reinterpret_cast<void*>(stream)));
     return {d_rows, d_table};
+}
+std::pair<std::optional<at::Tensor>, std::optional<at::Tensor>> table_loss_backward(int64_t ctx, int64_t stream, const at::Tensor& d_loss, const at::Tensor& table, const at::Tensor& kept,
+                                                                                    int64_t rows, double scale, int64_t reduction, bool want_rows, bool want_table)
+{
+    auto [d_rows, d_table] = table_loss_gradients(ctx, stream, d_loss, table, kept, rows, scale, reduction, want_rows, want_table);
+    return {d_rows.defined() ? std::optional<at::Tensor>(d_rows) : std::nullopt, d_table.defined() ? std::optional<at::Tensor>(d_table) : std::nullopt};
+}
+
+// Gradients that cannot be differentiated again: where that could be asked for, it raises.
+void only_once(torch::autograd::variable_list& grads, const at::Tensor& upstream)
+{
+    if (!at::GradMode::is_enabled() || !upstream.requires_grad()) return;
+    torch::autograd::variable_list in;
+    for (at::Tensor& g : grads)
+        if (g.defined()) g = g.detach().set_requires_grad(true), in.push_back(g);
+    if (in.empty()) return;
+    auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that has its gradients once", (int64_t)in.size());
+    auto out   = (*error)(std::move(in));
+    size_t at  = 0;
+    for (at::Tensor& g : grads)
+        if (g.defined()) g = out[at++];
+}
+
+// The function that a graph records (in Python, its two ways through the interpreter would take as long as the kernels of a small problem: 25 rows
+// of 5000 entries 104 us a pass, so 79).
+struct TableLoss : torch::autograd::Function<TableLoss>
+{
+    static at::Tensor forward(torch::autograd::AutogradContext* own, const at::Tensor& rows, const at::Tensor& table, const at::Tensor& target, int64_t ctx, int64_t stream, double scale,
+                              int64_t reduction)
+    {
+        auto [loss, kept] = table_loss(ctx, stream, rows.detach(), table.detach(), target, scale, reduction);
+        own->save_for_backward({table, kept});
+        own->saved_data["ctx"] = ctx, own->saved_data["scale"] = scale, own->saved_data["reduction"] = reduction, own->saved_data["rows"] = rows.size(0);
+        return loss;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* own, torch::autograd::variable_list upstream)
+    {
+        const auto saved = own->get_saved_variables();
+        const at::Tensor d_loss = upstream[0], &table = saved[0], &kept = saved[1];
+        torch::autograd::variable_list grads(7);
+        if (!d_loss.defined()) return grads;
+        auto [d_rows, d_table] = table_loss_gradients(own->saved_data["ctx"].toInt(), stream_of(kept), d_loss.detach(), table.detach(), kept, own->saved_data["rows"].toInt(),
+                                                      own->saved_data["scale"].toDouble(), own->saved_data["reduction"].toInt(), own->needs_input_grad(0), own->needs_input_grad(1));
+        grads[0] = d_rows, grads[1] = d_table;
+        only_once(grads, d_loss);
+        return grads;
+    }
+};
+at::Tensor table_loss_graph(int64_t ctx, int64_t stream, const at::Tensor& rows, const at::Tensor& table, const at::Tensor& target, double scale, int64_t reduction)
+{
+    return TableLoss::apply(rows, table, target, ctx, stream, scale, reduction);
 }
 
 // ---- dropout ----
 
-// {out, the step that was used (where it was read from the device and is asked for)}
-std::pair<at::Tensor, std::optional<at::Tensor>> dropout(uintptr_t ctx, uintptr_t stream, const at::Tensor& x, double p, uint64_t seed, uint32_t call, uint32_t step,
-                                                         const std::optional<at::Tensor>& step_at, const std::optional<at::Tensor>& residual, bool want_step)
+// {out, the step that was used (undefined where it was not read from the device, or is not asked for)}
+std::pair<at::Tensor, at::Tensor> dropped(int64_t ctx, int64_t stream, const at::Tensor& x, double p, int64_t seed, int64_t call, int64_t step, const std::optional<at::Tensor>& step_at,
+                                          const std::optional<at::Tensor>& residual, bool want_step)
 {
     if (!(p >= 0.0 && p <= 1.0)) throw py::value_error("p: 0 to 1 expected, got " + std::to_string(p));
-    if (dtype_of(x) < 0 || x.layout() != at::kStrided) throw py::value_error("x: a float32, bfloat16 or float16 tensor expected, got " + std::string(torch::getTHPDtype(x.scalar_type())->name));
+    if (dtype_of(x) < 0 || x.layout() != at::kStrided) throw py::value_error("x: a float32, bfloat16 or float16 tensor expected");
     if (!x.is_cuda()) throw std::runtime_error("dropout needs tensors on a GPU: there is no CPU implementation");
     if (residual && (residual->scalar_type() != x.scalar_type() || residual->sizes() != x.sizes() || residual->device() != x.device() || residual->layout() != at::kStrided))
         throw py::value_error("residual: a tensor of x's type and shape on its device expected");
     if (step_at && ((step_at->scalar_type() != at::kInt && step_at->scalar_type() != at::kLong) || step_at->numel() != 1 || step_at->device() != x.device()))
         throw py::value_error("step: a number, or one int32 or int64 on x's device, expected");
     TripsDropoutDesc d{};
-    d.abi_version = TRIPS_ABI_VERSION, d.dtype = dtype_of(x), d.n = x.numel(), d.p = p, d.seed = seed, d.call = call, d.step = step;
+    d.abi_version = TRIPS_ABI_VERSION, d.dtype = dtype_of(x), d.n = x.numel(), d.p = p, d.seed = (uint64_t)seed, d.call = (uint32_t)call, d.step = (uint32_t)step;
     const at::Tensor from = x.detach().contiguous(), added = residual ? residual->detach().contiguous() : at::Tensor();
-    at::Tensor out = torch::empty(x.sizes(), x.options().requires_grad(false));
-    std::optional<at::Tensor> used;
+    at::Tensor out = torch::empty(x.sizes(), x.options().requires_grad(false)), used;
     if (step_at && want_step) used = torch::empty({}, x.options().dtype(at::kInt).requires_grad(false));
     // (the low word of an int64)
-    check(trips_dropout(reinterpret_cast<TripsCtx*>(ctx), &d, from.data_ptr(), data(added), step_at ? (const uint32_t*)step_at->data_ptr() : nullptr,
-                        used ? (uint32_t*)used->data_ptr() : nullptr, out.data_ptr(), reinterpret_cast<void*>(stream)));
+    check(trips_dropout(reinterpret_cast<TripsCtx*>(ctx), &d, from.data_ptr(), data(added), step_at ? (const uint32_t*)step_at->data_ptr() : nullptr, (uint32_t*)data(used), out.data_ptr(),
+                        reinterpret_cast<void*>(stream)));
     return {out, used};
+}
+std::pair<at::Tensor, std::optional<at::Tensor>> dropout(int64_t ctx, int64_t stream, const at::Tensor& x, double p, int64_t seed, int64_t call, int64_t step,
+                                                         const std::optional<at::Tensor>& step_at, const std::optional<at::Tensor>& residual, bool want_step)
+{
+    auto [out, used] = dropped(ctx, stream, x, p, seed, call, step, step_at, residual, want_step);
+    return {out, used.defined() ? std::optional<at::Tensor>(used) : std::nullopt};
+}
+
+struct Dropout : torch::autograd::Function<Dropout>
+{
+    static at::Tensor forward(torch::autograd::AutogradContext* own, const at::Tensor& x, const std::optional<at::Tensor>& residual, int64_t ctx, int64_t stream, double p, int64_t seed,
+                              int64_t call, int64_t step, const std::optional<at::Tensor>& step_at)
+    {
+        // (the step may have gone on when the gradient is made: what was used is kept)
+        auto [out, used] = dropped(ctx, stream, x, p, seed, call, step, step_at, residual, true);
+        if (used.defined()) own->save_for_backward({used});
+        own->saved_data["ctx"] = ctx, own->saved_data["p"] = p, own->saved_data["seed"] = seed, own->saved_data["call"] = call, own->saved_data["step"] = step;
+        own->saved_data["used"] = used.defined(), own->saved_data["residual"] = residual.has_value();
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* own, torch::autograd::variable_list upstream)
+    {
+        torch::autograd::variable_list grads(9);
+        const at::Tensor g = upstream[0];
+        if (!g.defined()) return grads;
+        if (own->needs_input_grad(0))
+        {
+            const std::optional<at::Tensor> used = own->saved_data["used"].toBool() ? std::optional<at::Tensor>(own->get_saved_variables()[0]) : std::nullopt;
+            grads[0] = dropped(own->saved_data["ctx"].toInt(), stream_of(g), g, own->saved_data["p"].toDouble(), own->saved_data["seed"].toInt(), own->saved_data["call"].toInt(),
+                               own->saved_data["step"].toInt(), used, std::nullopt, false)
+                           .first;
+            only_once(grads, g);
+        }
+        if (own->saved_data["residual"].toBool() && own->needs_input_grad(1)) grads[1] = g;  // (an edge of its own where there is one)
+        return grads;
+    }
+};
+at::Tensor dropout_graph(int64_t ctx, int64_t stream, const at::Tensor& x, const std::optional<at::Tensor>& residual, double p, int64_t seed, int64_t call, int64_t step,
+                         const std::optional<at::Tensor>& step_at)
+{
+    return Dropout::apply(x, residual, ctx, stream, p, seed, call, step, step_at);
 }
 }  // namespace
 
@@ -419,5 +515,7 @@ PYBIND11_MODULE(_trips_host, m)
     m.def("lookup_backward", &lookup_backward);
     m.def("table_loss", &table_loss);
     m.def("table_loss_backward", &table_loss_backward);
+    m.def("table_loss_graph", &table_loss_graph);
     m.def("dropout", &dropout);
+    m.def("dropout_graph", &dropout_graph);
 }

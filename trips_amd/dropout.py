@@ -17,6 +17,7 @@ def _run(x, p, seed, call, step, residual, want_step):
 
 
 class _Dropout(torch.autograd.Function):
+    """For modes that have to see a call: traces record it, forward-mode levels and functional transforms refuse it."""
     @staticmethod
     def forward(ctx, x, p, seed, call, step, residual):
         with _untraced():
@@ -44,11 +45,13 @@ def dropout(x, p, seed, call=0, step=0, residual=None):
     `step`: a number below 2^32, or one int32 or int64 on x's device, of which the kernel reads the low 32 bits, for steps that are captured
     into a graph (a parameter's step count of AdamW, for instance). Differentiable in x and residual, once; the gradient of x is this
     function of the gradient, with the step that was used."""
-    seed &= 0xFFFFFFFFFFFFFFFF
+    seed = (seed + (1 << 63)) % (1 << 64) - (1 << 63)  # (64 bits, as the extension takes them)
     if not 0 <= call < 1 << 32 or not (torch.is_tensor(step) or 0 <= step < 1 << 32):
         raise ValueError(f"call and step: 32 bits expected, got {call} and {step}")
-    graph = torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))
-    tensors = [t for t in (x, residual, step) if torch.is_tensor(t)]
-    if graph or forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(*tensors):
+    if forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(*(t for t in (x, residual, step) if torch.is_tensor(t))):
         return _Dropout.apply(x, p, seed, call, step, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        ctx, stream = _where(x)
+        number, at = (0, step) if torch.is_tensor(step) else (step, None)
+        return _host().dropout_graph(ctx, stream, x, residual, p, seed, call, number, at)
     return _run(x.detach(), p, seed, call, step, None if residual is None else residual.detach(), False)[0]

@@ -16,20 +16,20 @@ REDUCTIONS = {"none": abi.TRIPS_REDUCE_NONE, "sum": abi.TRIPS_REDUCE_SUM, "mean"
 
 
 class _TableCrossEntropy(torch.autograd.Function):
+    """For modes that have to see a call: traces record it, forward-mode levels and functional transforms refuse it."""
     @staticmethod
     def forward(ctx, rows, table, target, scale, reduction):
         with _untraced():
-            loss, state = _host().table_loss(*_where(target), rows.detach(), table.detach(), target, scale, reduction)
-        ctx.save_for_backward(rows, table, target, state)
-        ctx.args = (scale, reduction)
+            loss, kept = _host().table_loss(*_where(target), rows.detach(), table.detach(), target, scale, reduction)
+        ctx.save_for_backward(table, kept)
+        ctx.args = (rows.shape[0], scale, reduction)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        rows, table, target, state = ctx.saved_tensors
-        d_rows, d_table = _host().table_loss_backward(*_where(target), grad, rows.detach(), table.detach(), target, state, *ctx.args,
-                                                      ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        table, kept = ctx.saved_tensors
+        d_rows, d_table = _host().table_loss_backward(*_where(kept), grad, table.detach(), kept, *ctx.args, *ctx.needs_input_grad[:2])
         return d_rows, d_table, None, None, None
 
 
@@ -40,10 +40,14 @@ def table_cross_entropy(rows, table, target, scale=1.0, reduction="mean"):
 
     reduction: "none" gives [N], "sum" and "mean" one number, the mean over the rows that count (0 where none does); float32
     whatever the type of rows and table (float32, bfloat16 or float16, the same of both). Differentiable in rows and table, once; gradients
-    have their type. In float16 the gradients of rows whose loss counts 2^-15 as much as another's lose precision."""
+    have their type. What the gradients need of the rows is a copy of those that count, kept with the graph; they may be written to
+    meanwhile, the table may not. In float16 the gradients of rows whose loss counts 2^-15 as much as another's lose precision."""
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction: 'none', 'sum' or 'mean' expected, got {reduction!r}")
-    graph = torch.is_grad_enabled() and (rows.requires_grad or table.requires_grad)
-    if graph or forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(rows, table, target):
-        return _TableCrossEntropy.apply(rows, table, target, scale, REDUCTIONS[reduction])
-    return _host().table_loss(*_where(target), rows.detach(), table.detach(), target, scale, REDUCTIONS[reduction])[0]
+    reduction = REDUCTIONS[reduction]
+    if forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(rows, table, target):
+        return _TableCrossEntropy.apply(rows, table, target, scale, reduction)
+    if torch.is_grad_enabled() and (rows.requires_grad or table.requires_grad):
+        ctx, stream = _where(target)
+        return _host().table_loss_graph(ctx, stream, rows, table, target, scale, reduction)
+    return _host().table_loss(*_where(target), rows.detach(), table.detach(), target, scale, reduction)[0]
