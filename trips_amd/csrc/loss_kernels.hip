@@ -335,6 +335,10 @@ __device__ __forceinline__ void wait_and_meet()
 // (of LDS; the loads under way stay so)
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Logits up to which the distance from the largest may be taken after the scaling, in one operation (their own rounding is as much), in types of
+// 16 bits. Products masked with the lowest value lie beyond it.
+constexpr float kFar = 65536.f;
+
 constexpr unsigned kBeyond = 0x80000000u;  // an offset beyond any buffer
 
 // Where a wavefront's loads of an operand's steps come from: each lane's offsets, the same for all tiles, and the operand's elements from the
@@ -481,8 +485,9 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
     const int wm = wave % S::WM * S::TM, wn = wave / S::WM * S::TN;
     const int count = *p.kept.count;
 
-    // workgroups as they start go around the eight XCDs: workers by XCD
-    const int all = gridDim.x, worker = all % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (all / 8) + blockIdx.x / 8);
+    // Workgroups as they start go around the eight XCDs: of each 256, which take a CU each, workers by XCD.
+    const int all = gridDim.x, run = (int)blockIdx.x & ~255, runs = min(256, all - run), in_run = (int)blockIdx.x & 255;
+    const int worker = run + (runs % 8 ? in_run : in_run % 8 * (runs / 8) + in_run / 8);
     const int row_tiles = (count + S::BN - 1) / S::BN, entry_tiles = (p.in_piece + (KIND == GRADS ? S::BN : S::BM) - 1) / (KIND == GRADS ? S::BN : S::BM);
     const int channel_tiles = (p.channels + S::BM - 1) / S::BM;
     const int piece_steps   = (p.in_piece + BK - 1) / BK;
@@ -700,11 +705,17 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                 });
                 if (here) p.own_product[n] = product;
             }
-            each_element<S::FM>([&](int i, int e, int) { top = fmaxf(top, acc[i][j][e]); });
+            each_element<S::FM>([&](int i, int e, int)
+            {
+                if (e % 2) top = fmaxf(top, fmaxf(acc[i][j][e - 1], acc[i][j][e]));
+            });
             top              = fmaxf(top, __shfl_xor(top, 32));
-            const float base = top == -__builtin_inff() ? 0.f : top;
+            const float base = top == -__builtin_inff() ? 0.f : top, less = -base * p.scale_log2;
             float sum        = 0.f;
-            each_element<S::FM>([&](int i, int e, int) { sum += part_of(acc[i][j][e], base, p.scale_log2); });
+            if (D != TRIPS_DTYPE_F32 && fabsf(less) < kFar)  // (each lane by itself: a row's bits do not depend on other rows)
+                each_element<S::FM>([&](int i, int e, int) { sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], p.scale_log2, less)); });
+            else
+                each_element<S::FM>([&](int i, int e, int) { sum += part_of(acc[i][j][e], base, p.scale_log2); });
             best[j] = make_float2(top, sum + __shfl_xor(sum, 32));
         }
         meet();  // (the last unit's have been read)
@@ -739,8 +750,12 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                 float factor = 0.f;
                 int own      = -1;
                 if (n < count) state = p.kept.state[n], factor = held_factor<D>(p.upstream, p.upstream.reduction == TRIPS_REDUCE_NONE ? p.kept.row[n] : 0), own = p.kept.target[n] - p.first_entry - m_lane;
-                each_element<S::FM>([&](int i, int e, int)
-                                    { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - state.x, p.scale_log2, -state.y)) * factor; });
+                const float less = -state.x * p.scale_log2, held = D == TRIPS_DTYPE_F16 ? factor : 1.f;
+                if (D != TRIPS_DTYPE_F32 && fabsf(less) < kFar)
+                    each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], p.scale_log2, less - state.y)) * held; });
+                else
+                    each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - state.x, p.scale_log2, -state.y)) * held; });
+                if (D != TRIPS_DTYPE_F16 && p.upstream.reduction == TRIPS_REDUCE_NONE) each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] *= factor; });
                 if (__any(own >= 0 && own < S::TM))
                     each_element<S::FM>([&](int i, int e, int m)
                     {
@@ -893,27 +908,25 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
         part[threadIdx.x] = own;
         own.y             = product;
     }
-    __syncthreads();
-    float loss = 0.f;
-    if (threadIdx.x >> rows_log2 == 0)
+    for (int o = lanes >> 1; o > 0; o >>= 1)
     {
-        float top = -__builtin_inff(), sum = 0.f, log_sum = 0.f;
-        if (at >= 0)
+        __syncthreads();
+        if (threadIdx.x >> rows_log2 < o && at >= 0)
         {
-            for (int s = 0; s < lanes; ++s) top = fmaxf(top, part[(s << rows_log2) + row].x);
-            const float base = top == -__builtin_inff() ? 0.f : top;
-            for (int s = 0; s < lanes; ++s)
-            {
-                const float2 x = part[(s << rows_log2) + row];
-                sum += x.y * part_of(x.x, base, p.scale_log2);
-            }
-            const double log = log2((double)sum);
-            loss    = (float)(((double)top - (double)own.y) * (double)p.scale + log * kLog2);
-            log_sum = (float)log;
+            const float2 x = part[threadIdx.x], y = part[threadIdx.x + (o << rows_log2)];
+            const float top = fmaxf(x.x, y.x), base = top == -__builtin_inff() ? 0.f : top;
+            part[threadIdx.x] = make_float2(top, x.y * part_of(x.x, base, p.scale_log2) + y.y * part_of(y.x, base, p.scale_log2));
         }
-        if (at >= 0) p.kept.state[at] = make_float2(top, log_sum);
-        if (i < p.n && p.reduction == TRIPS_REDUCE_NONE) p.loss[i] = loss;
     }
+    float loss = 0.f;
+    if (threadIdx.x >> rows_log2 == 0 && at >= 0)  // (what a thread reads it wrote itself)
+    {
+        const float2 all = part[threadIdx.x];
+        const double log = log2((double)all.y);
+        loss             = (float)(((double)all.x - (double)own.y) * (double)p.scale + log * kLog2);
+        p.kept.state[at] = make_float2(all.x, (float)log);
+    }
+    if (threadIdx.x >> rows_log2 == 0 && i < p.n && p.reduction == TRIPS_REDUCE_NONE) p.loss[i] = loss;
     if (p.reduction == TRIPS_REDUCE_NONE) return;
     double sum = (double)loss;
 #pragma unroll
@@ -1042,11 +1055,13 @@ struct Layout
 };
 
 using Big   = Shape<256, 256, 2, 4, 2, 1>;
+using Wide  = Shape<256, 256, 2, 2, 2, 1>;  // four wavefronts of 128 x 128: fewer reads of LDS, and nothing beside a wavefront's exponentials
 using Small = Shape<128, 128, 2, 2, 2, 2>;
 using Tiny  = Shape<64, 64, 2, 2, 4, 2>;
 
 // f(a shape): the largest tiles of which a product of `down` x `across` makes one for each CU at least; never the largest in 32 bits, whose
-// products take so long that the loads do not count.
+// products take so long that the loads do not count. (Wide for the gradients: 8191 rows of 50,000 entries of 1024 bfloat16 channels 1575 us with
+// Big and 1522 so; the logits 870 with Big, 1084 so.)
 template <typename F>
 auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
 {
@@ -1055,7 +1070,7 @@ auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
         const int64_t rows = up(d.num_rows, tile) / tile, entries = up(d.num_entries, tile) / tile, channels = up(d.num_channels, tile) / tile;
         return grads ? channels * entries : rows * entries;
     };
-    if (d.dtype != TRIPS_DTYPE_F32 && units(256) >= kCus) return f(Big{});
+    if (d.dtype != TRIPS_DTYPE_F32 && units(256) >= kCus) return grads ? f(Wide{}) : f(Big{});
     if (units(128) >= kCus) return f(Small{});
     return f(Tiny{});
 }
@@ -1211,7 +1226,9 @@ hipError_t launch_product(const TripsTableLossDesc& d, const ProductParams& p, h
 {
     return with_shape(d, KIND == GRADS, [&](auto shape)
     {
-        using S = std::conditional_t<D == TRIPS_DTYPE_F32 && decltype(shape)::BM == 256, Small, decltype(shape)>;
+        using Given = decltype(shape);
+        // (no code for what with_shape() does not give)
+        using S = std::conditional_t<Given::BM == 256 && (D == TRIPS_DTYPE_F32 || (Given::WAVES == 4) != (KIND == GRADS)), Small, Given>;
         const int64_t row_tiles = tiles_of(d.num_rows, S::BN), channel_tiles = tiles_of(d.num_channels, S::BM);
         const int64_t units = KIND == GRADS ? channel_tiles * ((p.d_rows ? row_tiles * p.splits : 0) + (p.d_table ? tiles_of(p.in_piece, S::BN) : 0)) : tiles_of(p.in_piece, S::BM) * row_tiles;
         if (units == 0) return hipSuccess;
