@@ -120,6 +120,20 @@ def test_unaligned_and_transposed(dtype, shift):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,t,c,pad", [(40, 300, 57, 1), (40, 300, 62, 2), (300, 900, 33, 7), (9, 70, 3, 5), (600, 4000, 66, 2), (50, 200, 129, 3)])
+def test_what_lies_behind_a_row(dtype, n, t, c, pad):
+    """Elements between the rows hold anything; the same gradients as without them."""
+    x, w, target = _inputs(n, t, c, dtype, 0.2)
+    want = _check(x, w, target)
+    wide = [torch.full((m.shape[0], c + pad), float("nan"), dtype=m.dtype, device="cuda") for m in (x, w)]
+    views = [m[:, :c].copy_(a.detach()) for m, a in zip(wide, (x, w))]
+    for m in views:
+        assert m.stride(0) == c + pad
+    for a, b in zip(_check_only(*views, target), want):
+        assert torch.equal(a, b)
+
+
 def test_rows_that_repeat():
     """One row of memory for all rows: read, its gradients summed by torch."""
     x, w, target = _inputs(1, 100, 16, "f32")

@@ -243,7 +243,7 @@ struct ProductParams
     const void* d_rows;  // whether they are wanted
     void* d_table;
     long long table_stride, d_table_stride, rows_pad;
-    int held;  // channels that a row of the table holds: those, or with zeros behind them to 16 bytes
+    int held;  // channels that a row of the table has: those, or of a copy with zeros behind them to 16 bytes
     int first_entry, in_piece, channels, kp, piece, first_tile, splits, add;
     float scale_log2;
 };
@@ -552,7 +552,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             first.step = second.step = 0;
             return;
         }
-        const long long stride = p.table_stride * SIZE, wide = (long long)p.kp * SIZE, piece = (long long)p.piece * SIZE, held = (long long)p.held * SIZE;
+        const long long stride = p.table_stride * SIZE, wide = (long long)p.kp * SIZE, piece = (long long)p.piece * SIZE, held = ((long long)p.held * SIZE + 3) / 4 * 4;
         if constexpr (KIND != GRADS)
         {
             if (ahead_mode != u.mode) FirstAlong::begin(first, stride, wave, lane), SecondAlong::begin(second, wide, wave, lane);
@@ -637,6 +637,20 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
 #pragma unroll
             for (int j = 0; j < S::FN; ++j) y[set][j] = Second::read(a + S::FIRST_BYTES, wn, j, kk, lane);
         };
+        // Of a table whose rows are no whole pieces of 16 bytes, the last one that a row has brings elements of what lies behind the row: they meet
+        // zeros of the second operand, but might be no numbers.
+        constexpr int V = 16 / SIZE;
+        const bool ragged = KIND != GRADS && p.held % V;
+        auto clear_ends = [&](int of)
+        {
+            for (int row = threadIdx.x; row < S::BM; row += S::WAVES * 64)
+            {
+                T* piece = reinterpret_cast<T*>(lds + of * S::STAGE_BYTES + row * kStepBytes + ((p.held % BK / V) ^ FirstAlong::turn(row)) * 16);
+                for (int e = p.held % V; e < V; ++e) piece[e] = 0;
+            }
+            meet();
+        };
+        if (ragged && steps == 1) clear_ends(stage);
         if (steps > 0) read(0, stage, 0);
         for (int step = 0; step < steps; ++step)
         {
@@ -649,6 +663,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                 else
                 {
                     wait_and_meet<(S::STAGES - 2) * LOADS>();
+                    if (ragged && step + 2 == steps) clear_ends(next);
                     read(0, next, 0);  // (behind the last step: of the next unit, which reads it again)
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -1005,12 +1020,8 @@ constexpr int64_t kCopyBytes = 64ll << 20, kLeastCopyBytes = 16ll << 20;  // of 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 unsigned tiles_of(int64_t n, int tile) { return (unsigned)((n + tile - 1) / tile); }
 
-// Whether the direct loads take the table's rows as they are: 16 bytes at a time, 256 rows within 31 bits.
-bool rows_in_place(const TripsTableLossDesc& d)
-{
-    const int64_t size = dtype_bytes(d.dtype);
-    return d.num_channels * size % 16 == 0 && d.table_stride * size % 16 == 0 && d.table_stride < 1 << 20;
-}
+// Whether the direct loads take the table's rows as they are: whole words, 256 rows within 31 bits.
+bool rows_in_place(const TripsTableLossDesc& d) { return d.table_stride * dtype_bytes(d.dtype) % 4 == 0 && d.table_stride < 1 << 20; }
 
 int packed_channels(const TripsTableLossDesc& d)
 {
@@ -1055,13 +1066,12 @@ struct Layout
 };
 
 using Big   = Shape<256, 256, 2, 4, 2, 1>;
-using Wide  = Shape<256, 256, 2, 2, 2, 1>;  // four wavefronts of 128 x 128: fewer reads of LDS, and nothing beside a wavefront's exponentials
 using Small = Shape<128, 128, 2, 2, 2, 2>;
 using Tiny  = Shape<64, 64, 2, 2, 4, 2>;
 
 // f(a shape): the largest tiles of which a product of `down` x `across` makes one for each CU at least; never the largest in 32 bits, whose
-// products take so long that the loads do not count. (Wide for the gradients: 8191 rows of 50,000 entries of 1024 bfloat16 channels 1575 us with
-// Big and 1522 so; the logits 870 with Big, 1084 so.)
+// products take so long that the loads do not count. (With four wavefronts of 128 x 128 the logits of 8191
+// rows and 50,000 entries of 1024 bfloat16 channels took 1084 us where eight take 870, the gradients 1475 and 1434.)
 template <typename F>
 auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
 {
@@ -1070,7 +1080,7 @@ auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
         const int64_t rows = up(d.num_rows, tile) / tile, entries = up(d.num_entries, tile) / tile, channels = up(d.num_channels, tile) / tile;
         return grads ? channels * entries : rows * entries;
     };
-    if (d.dtype != TRIPS_DTYPE_F32 && units(256) >= kCus) return grads ? f(Wide{}) : f(Big{});
+    if (d.dtype != TRIPS_DTYPE_F32 && units(256) >= kCus) return f(Big{});
     if (units(128) >= kCus) return f(Small{});
     return f(Tiny{});
 }
@@ -1158,7 +1168,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     return l;
 }
 
-bool copies_of(const TripsTableLossDesc& d, const void* table) { return !(rows_in_place(d) && aligned(table, 16)); }
+bool copies_of(const TripsTableLossDesc& d, const void* table) { return !(rows_in_place(d) && aligned(table, 4)); }
 
 // For any address of the table.
 size_t workspace_of(const TripsTableLossDesc& d, bool backward)
@@ -1228,7 +1238,7 @@ hipError_t launch_product(const TripsTableLossDesc& d, const ProductParams& p, h
     {
         using Given = decltype(shape);
         // (no code for what with_shape() does not give)
-        using S = std::conditional_t<Given::BM == 256 && (D == TRIPS_DTYPE_F32 || (Given::WAVES == 4) != (KIND == GRADS)), Small, Given>;
+        using S = std::conditional_t<D == TRIPS_DTYPE_F32 && Given::BM == 256, Small, Given>;
         const int64_t row_tiles = tiles_of(d.num_rows, S::BN), channel_tiles = tiles_of(d.num_channels, S::BM);
         const int64_t units = KIND == GRADS ? channel_tiles * ((p.d_rows ? row_tiles * p.splits : 0) + (p.d_table ? tiles_of(p.in_piece, S::BN) : 0)) : tiles_of(p.in_piece, S::BM) * row_tiles;
         if (units == 0) return hipSuccess;
