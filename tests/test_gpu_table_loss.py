@@ -223,27 +223,47 @@ def test_large_logits(dtype):
     _check(*_inputs(60, 200, 64, dtype, spread=60.0))
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-def test_pieces_of_the_table(dtype):
-    """More entries than a piece holds (of 9000 rows). The bound is loss_reference.Loss's, with the largest error of any row's log
-    probabilities: e of them, (terms + 8) 2 U for a sum of so many terms, half a step of the type where d_ij is held in it, half a
-    step of the result."""
-    x, w, target = _inputs(9000, 17_000, 8, dtype, 0.2)
-    loss, d_rows, d_table = _check_only(x, w, target, "sum")
-    inside = (target >= 0) & (target < 17_000)
+def _check_on_the_gpu(x, w, target, reduction="sum"):
+    """For sizes that numpy would take long for: the oracle's products in double precision on the GPU. The bound is loss_reference.Loss's, with the
+    largest error of any row's log probabilities: e of them, (terms + 8) 2 U for a sum of so many terms, half a step of the type where d_ij is held in it,
+    half a step of the result."""
+    (n, c), t = x.shape, w.shape[0]
+    loss, d_rows, d_table = _check_only(x, w, target, reduction)
+    inside = (target >= 0) & (target < t)
     i, u = inside.nonzero()[:, 0], torch.finfo(x.dtype).eps
-    logp = torch.log_softmax(x.detach()[i].double() @ w.detach().double().t(), 1)
-    total = -logp[torch.arange(i.numel()), target[i]].sum()
-    assert abs(float(loss) - float(total)) < 1e-5 * float(total)
-    rows, table = x.detach()[i].double().abs(), w.detach().double().abs()
-    size = float((rows @ table.t()).max())
-    e = (4 * (8 + 2) * size + 8 * size + 320 + 17_000 / 64 + 8) * U
-    p = logp.exp_()
-    p[torch.arange(i.numel()), target[i]] -= 1
+    rows, table = x.detach()[i].double(), w.detach().double()
+    p = rows @ table.t()
+    size = float((rows.abs() @ table.t().abs()).max())
+    at = torch.arange(i.numel(), device="cuda")
+    p = torch.log_softmax(p, 1)
+    total = -p[at, target[i]].sum()
+    e = (4 * (c + 2) * size + 8 * size + 320 + t / 64 + 8) * U
+    assert abs(float(loss) - float(total)) <= i.numel() * e + 4 * U * float(total)
+    p.exp_()
+    p[at, target[i]] -= 1
     p *= 1.5
-    for got, a, b in ((d_rows[i], p, w.detach().double()), (d_table, p.t().contiguous(), x.detach()[i].double())):
-        within(got, (a @ b).cpu().numpy(), ((u + 2 * e + (a.shape[1] + 16) * 2 * U) * (a.abs() @ b.abs()) + 1e-9).cpu().numpy(), "gradients")
+    for got, a, b in ((d_rows[i], p, table), (d_table, p.t(), rows)):
+        want, bound = a @ b, (u + 2 * e + (a.shape[1] + 16) * 2 * U) * (a.abs() @ b.abs()) + 1e-9
+        off = (got.double() - want).abs() > bound
+        assert not off.any() and not got.isnan().any(), f"{int(off.sum())} of {off.numel()} off"
     assert (d_rows[~inside] == 0).all()
+
+
+LARGE = [(9000, 17_000, 8, 0), (300, 40_000, 40, 0), (600, 30_001, 66, 0), (200, 14_000, 1100, 0), (2000, 9000, 257, 0), (2049, 8193, 130, 3), (130, 66_000, 72, 0), (129, 70_000, 513, 1),
+         (513, 33_000, 520, 8)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n,t,c,pad", LARGE)
+def test_large_tiles(n, t, c, pad, dtype):
+    """Tiles of 256 x 256 in 16 bits, for the logits, the gradients or both, and the same sizes in 32."""
+    _check_on_the_gpu(*_inputs(n, t, c, dtype, 0.2, pad=pad))
+
+
+@pytest.mark.parametrize("n,t,c,dtype", [(70_000, 9000, 8, "bf16"), (66_000, 8300, 24, "f16"), (35_000, 8000, 12, "f32"), (150, 40_000, 1001, "bf16"), (140, 66_000, 513, "f16")])
+def test_pieces_of_the_table(n, t, c, dtype):
+    """More rows and entries than the logits' gradient of a piece holds, and (of odd channels) more entries than are copied at a time."""
+    _check_on_the_gpu(*_inputs(n, t, c, dtype, 0.2))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])

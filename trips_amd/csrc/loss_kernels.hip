@@ -170,6 +170,11 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
 template <int D>
 constexpr float kHeld = D == TRIPS_DTYPE_F16 ? 32768.f : 1.f;
 
+// In 16 bits d_ij is off by up to 2^-9 (bfloat16) of itself, and so is what it adds to the gradients, which are rounded as far once more: their
+// error against the exact ones is 1.1 to 1.8 times that of this last rounding alone, the more the fewer entries share a row's probability. Holding the
+// rest of d_ij as well, as a second part of the same type, takes that away and doubles the gradients' products: done where those are few (see
+// parts_of()).
+
 // The largest |gradient| of the rows that count, finite ones only: the others are left as they are.
 __global__ __launch_bounds__(1024) void top_kernel(const float* d_loss, const int* place, long long n, float* top)
 {
@@ -238,13 +243,13 @@ struct ProductParams
     Upstream upstream;
     float2* partial;     // LOGITS: [tiles of entries][rows_pad] {largest product, sum of exponentials}
     float* own_product;  // [rows_pad]
-    void* probs;         // [rows_pad][piece], in the tensors' type
+    void* probs;         // [parts][rows_pad][piece], in the tensors' type
     float* slabs;        // D_ROWS: [splits][rows_pad][kp]
     const void* d_rows;  // whether they are wanted
     void* d_table;
     long long table_stride, d_table_stride, rows_pad;
     int held;  // channels that a row of the table has: those, or of a copy with zeros behind them to 16 bytes
-    int first_entry, in_piece, channels, kp, piece, first_tile, splits, add;
+    int first_entry, in_piece, channels, kp, piece, first_tile, splits, parts, add;
     float scale_log2;
 };
 
@@ -540,7 +545,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
     const char* probs  = reinterpret_cast<const char*>(p.probs);
     Source<S::FIRST_LOADS> first;
     Source<S::SECOND_LOADS> second;
-    int ahead_ordinal = 0, ahead_mode = -1, ahead_steps = 0, left = 0;
+    int ahead_ordinal = 0, ahead_part = 0, ahead_mode = -1, ahead_steps = 0, left = 0;
     auto open = [&]()
     {
         Unit u = unit_of(ahead_ordinal);
@@ -552,6 +557,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             first.step = second.step = 0;
             return;
         }
+        const char* part       = probs + ahead_part * p.rows_pad * p.piece * SIZE;
         const long long stride = p.table_stride * SIZE, wide = (long long)p.kp * SIZE, piece = (long long)p.piece * SIZE, held = ((long long)p.held * SIZE + 3) / 4 * 4;
         if constexpr (KIND != GRADS)
         {
@@ -566,14 +572,14 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             if (ahead_mode != u.mode) FirstAcross::begin(first, stride, wave, lane), SecondAlong::begin(second, piece, wave, lane);
             const long long k = (long long)u.z * piece_steps / p.splits * BK, m0 = (long long)u.x * S::BM * SIZE, n0 = (long long)u.y * S::BN;
             first.at(table + k * stride + m0, (p.in_piece - 1 - k) * stride + held - m0);
-            second.at(probs + n0 * piece + k * SIZE, (p.rows_pad - n0) * piece - k * SIZE);
+            second.at(part + n0 * piece + k * SIZE, (p.rows_pad - n0) * piece - k * SIZE);
         }
         else
         {
             if (ahead_mode != u.mode) FirstAcross::begin(first, wide, wave, lane), SecondAcross::begin(second, piece, wave, lane);
             const long long m0 = (long long)u.x * S::BM * SIZE, n0 = (long long)u.y * S::BN * SIZE;
             first.at(packed + m0, count * wide - m0);
-            second.at(probs + n0, count * piece - n0);
+            second.at(part + n0, count * piece - n0);
         }
         ahead_mode = u.mode;
     };
@@ -600,7 +606,9 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
     {
         first.next(), second.next();
         left -= BK;
-        if (--ahead_steps == 0) ++ahead_ordinal, open();
+        if (--ahead_steps > 0) return;
+        if (KIND != GRADS || ++ahead_part == p.parts) ++ahead_ordinal, ahead_part = 0;
+        open();
     };
     open();
 #pragma unroll
@@ -831,16 +839,25 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
 #pragma unroll
                     for (int g = 0; g < 4; g += 2)
                     {
-                        unsigned w[4];
+                        auto eight_of = [&](auto value)
+                        {
+                            unsigned w[4];
 #pragma unroll
-                        for (int h = 0; h < 4; ++h)
-                            w[h] = (unsigned)E::from_float(acc[i][j][4 * g + 2 * h] * unscale) | (unsigned)E::from_float(acc[i][j][4 * g + 2 * h + 1] * unscale) << 16;
-                        const auto low = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), high = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-                        const Words4 eight = {(int)low[0], (int)high[0], (int)low[1], (int)high[1]};
+                            for (int h = 0; h < 4; ++h) w[h] = (unsigned)value(4 * g + 2 * h) | (unsigned)value(4 * g + 2 * h + 1) << 16;
+                            const auto low = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), high = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+                            return Words4{(int)low[0], (int)high[0], (int)low[1], (int)high[1]};
+                        };
+                        const Words4 eight = eight_of([&](int e) { return E::from_float(acc[i][j][e] * unscale); });
                         const int m        = m0 + wm + i * 32 + 8 * (g + (lane >> 5));
                         if constexpr (MODE == PROBS)
                         {
-                            if (n < count) *reinterpret_cast<Words4*>(reinterpret_cast<T*>(p.probs) + n * p.piece + m) = eight;
+                            T* at = reinterpret_cast<T*>(p.probs) + n * p.piece + m;
+                            if (n < count) *reinterpret_cast<Words4*>(at) = eight;
+                            if (p.parts > 1)
+                            {
+                                const Words4 rest = eight_of([&](int e) { return E::from_float(acc[i][j][e] - E::to_float(E::from_float(acc[i][j][e]))); });
+                                if (n < count) *reinterpret_cast<Words4*>(at + p.rows_pad * p.piece) = rest;
+                            }
                         }
                         else if (n < p.in_piece && m < p.channels)
                         {
@@ -876,12 +893,12 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         }
         else if (u.mode == D_ROWS)
         {
-            products(std::true_type{}, u.steps);
+            products(std::true_type{}, u.steps * p.parts);
             written(std::integral_constant<int, D_ROWS>{}, u);
         }
         else
         {
-            products(std::false_type{}, u.steps);
+            products(std::false_type{}, u.steps * p.parts);
             written(std::integral_constant<int, D_TABLE>{}, u);
         }
     }
@@ -1060,7 +1077,7 @@ size_t kept_of(const TripsTableLossDesc& d, void* kept, Kept* k)
 struct Layout
 {
     int64_t rows_pad, chunks, piece, pieces;
-    int kp, tiles, splits;
+    int kp, tiles, splits, parts;
     bool copies;
     size_t chunk_count, top, partial, own_product, sums, probs, slabs, copy, bytes;
 };
@@ -1070,7 +1087,8 @@ using Small = Shape<128, 128, 2, 2, 2, 2>;
 using Tiny  = Shape<64, 64, 2, 2, 4, 2>;
 
 // f(a shape): the largest tiles of which a product of `down` x `across` makes one for each CU at least; never the largest in 32 bits, whose
-// products take so long that the loads do not count. (With four wavefronts of 128 x 128 the logits of 8191
+// products take so long that the loads do not count, nor for rows that half of one holds (32 rows of 50,000 entries of 1024 channels:
+// gradients with d_ij in two parts 122 us, 98 with Small). (With four wavefronts of 128 x 128 the logits of 8191
 // rows and 50,000 entries of 1024 bfloat16 channels took 1084 us where eight take 870, the gradients 1475 and 1434.)
 template <typename F>
 auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
@@ -1080,7 +1098,7 @@ auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
         const int64_t rows = up(d.num_rows, tile) / tile, entries = up(d.num_entries, tile) / tile, channels = up(d.num_channels, tile) / tile;
         return grads ? channels * entries : rows * entries;
     };
-    if (d.dtype != TRIPS_DTYPE_F32 && units(256) >= kCus) return f(Big{});
+    if (d.dtype != TRIPS_DTYPE_F32 && d.num_rows > 128 && units(256) >= kCus) return f(Big{});
     if (units(128) >= kCus) return f(Small{});
     return f(Tiny{});
 }
@@ -1088,6 +1106,15 @@ auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
 int entries_of_tile(const TripsTableLossDesc& d)
 {
     return with_shape(d, false, [](auto shape) { return decltype(shape)::BM; });
+}
+
+// Parts that d_ij is held in: two where the tiles are the smallest, or the rows and the table, so that launches and latency take most of the time
+// (7 rows of 19 entries of 2696 bfloat16 channels 70 us a pass either way; 3 of 221,303 of 2122 would take 1.24 ms for the gradients and not 0.71).
+int parts_of(const TripsTableLossDesc& d)
+{
+    if (d.dtype == TRIPS_DTYPE_F32) return 1;
+    const bool little = d.num_rows <= 128 && d.num_entries * d.num_channels <= 1 << 22;
+    return little || with_shape(d, true, [](auto shape) { return decltype(shape)::BM == Tiny::BM; }) ? 2 : 1;
 }
 
 // Into how many parts the rows' gradients are cut along the entries, so that they and the table's gradients keep all CUs busy to the end,
@@ -1139,6 +1166,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     l.rows_pad = up(d.num_rows, 256), l.chunks = d.num_rows > kCountedBy ? up(d.num_rows, kChunk) / kChunk : 0;
     l.kp     = packed_channels(d);
     l.copies = copies;
+    l.parts  = parts_of(d);
     Taker take;
     int64_t most = up(std::max<int64_t>(d.num_entries, 1), 256);
     if (copies)
@@ -1146,7 +1174,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
         most   = std::min(most, std::max<int64_t>((rows_in_place(d) ? kLeastCopyBytes : kCopyBytes) / (l.kp * size) / 256, 1) * 256);
         l.copy = take((size_t)most * l.kp * size);
     }
-    if (backward) most = std::min(most, std::max<int64_t>(kPieceBytes / (std::max<int64_t>(l.rows_pad, 1) * size) / 256, 1) * 256);
+    if (backward) most = std::min(most, std::max<int64_t>(kPieceBytes / (std::max<int64_t>(l.rows_pad, 1) * size * l.parts) / 256, 1) * 256);
     l.pieces = std::max<int64_t>(1, (d.num_entries + most - 1) / most);
     l.piece  = up((d.num_entries + l.pieces - 1) / l.pieces, 256);
     if (!backward)
@@ -1160,7 +1188,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     else
     {
         l.top   = take(4);
-        l.probs = take((size_t)l.rows_pad * l.piece * size);
+        l.probs = take((size_t)l.parts * l.rows_pad * l.piece * size);
         l.splits = splits_of(d, l.rows_pad, l.piece, l.kp);
         l.slabs  = take((size_t)l.splits * l.rows_pad * l.kp * 4);
     }
@@ -1207,7 +1235,7 @@ ProductParams product_params(const TripsTableLossDesc& d, const Layout& l, const
     p.kept = kept;
     p.partial = (float2*)(w + l.partial), p.own_product = (float*)(w + l.own_product), p.probs = w + l.probs, p.slabs = (float*)(w + l.slabs);
     p.d_table_stride = d.d_table_stride, p.rows_pad = l.rows_pad;
-    p.channels = d.num_channels, p.kp = l.kp, p.piece = (int)l.piece, p.splits = l.splits;
+    p.channels = d.num_channels, p.kp = l.kp, p.piece = (int)l.piece, p.splits = l.splits, p.parts = l.parts;
     p.scale_log2 = scale_log2(d);
     return p;
 }
