@@ -26,6 +26,7 @@ enum { TRIPS_REDUCE_NONE = 0, TRIPS_REDUCE_SUM = 1, TRIPS_REDUCE_MEAN = 2 };
  *
  *   l_ij = scale <rows_i, table_j>;   lse_i = log sum_j exp l_ij;   loss_i = lse_i - l_i,target_i
  *
+ * N T C is bounded by the units of work of a launch, 2^31 of some 10^4 products: what is refused for it would take minutes.
  * Rows whose target is outside [0, T) do not count: loss 0, gradient 0, whatever they hold. Strides are the elements between
  * two rows of memory; within a row elements are adjacent. A stride may be 0 where the call only reads. */
 typedef struct TripsTableLossDesc {

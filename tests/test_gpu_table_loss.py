@@ -96,7 +96,7 @@ def test_no_rows_and_no_entries():
         nothing = torch.zeros(0, 8, dtype=dtype, device="cuda", requires_grad=True)
         loss = table_cross_entropy(rows, nothing, torch.zeros(3, dtype=torch.int32, device="cuda"))
         d_rows, d_table = torch.autograd.grad(loss, (rows, nothing))
-        assert float(loss) == 0 and (d_rows == 0).all() and d_table.shape == (0, 8)
+        assert float(loss.detach()) == 0 and (d_rows == 0).all() and d_table.shape == (0, 8)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
@@ -238,7 +238,7 @@ def _check_on_the_gpu(x, w, target, reduction="sum"):
     p = torch.log_softmax(p, 1)
     total = -p[at, target[i]].sum()
     e = (4 * (c + 2) * size + 8 * size + 320 + t / 64 + 8) * U
-    assert abs(float(loss) - float(total)) <= i.numel() * e + 4 * U * float(total)
+    assert abs(float(loss.detach()) - float(total)) <= i.numel() * e + 4 * U * float(total)
     p.exp_()
     p[at, target[i]] -= 1
     p *= 1.5
@@ -379,6 +379,49 @@ def test_gradients_once():
     d, = torch.autograd.grad(table_cross_entropy(x, w, target), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(d.sum(), x)
+
+
+def test_gradients_of_a_gradient_that_is_followed_are_refused():
+    x, w, target = _inputs(20, 50, 16, "f32")
+    loss = table_cross_entropy(x, w, target)
+    g = torch.ones_like(loss).requires_grad_()
+    d, = torch.autograd.grad(loss, x, g, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        d.sum().backward()
+
+
+def test_saved_tensors_elsewhere():
+    """Hooks that move what is saved to the host and back."""
+    x, w, target = _inputs(90, 200, 40, "bf16", 0.2)
+    want = torch.autograd.grad(table_cross_entropy(x, w, target), (x, w))
+    with torch.autograd.graph.save_on_cpu():
+        loss = table_cross_entropy(x, w, target)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (x, w)), want))
+
+
+def test_table_of_more_than_4_gib():
+    """Entries whose offsets pass 32 bits, with two rows that belong to the last ones; the oracle in pieces, in double precision."""
+    t, c = 280_000, 8192
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.empty(t, c, dtype=torch.bfloat16, device="cuda").normal_(0, 2 / c ** 0.5, generator=g).requires_grad_()
+    target = torch.tensor([t - 1, 5, -1, t - 2], device="cuda")
+    x = (torch.randn(4, c, device="cuda", generator=g) + 1.5 * w.detach()[target].float()).bfloat16().requires_grad_()
+    loss = table_cross_entropy(x, w, target, reduction="none")
+    d_rows, d_table = torch.autograd.grad(loss, (x, w), torch.ones(4, device="cuda"))
+    rows = x.detach()[[0, 1, 3]].double()
+    logits = torch.cat([rows @ part.double().t() for part in w.detach().split(20_000)], 1)
+    p = torch.log_softmax(logits, 1)
+    own = target[[0, 1, 3]]
+    assert (loss[[0, 1, 3]].double() + p[[0, 1, 2], own]).abs().max() < 1e-3 and float(loss[2].detach()) == 0
+    p = p.exp_()
+    p[[0, 1, 2], own] -= 1
+    for first in (0, 262_144 - 64, t - 128):  # (2^32 bytes are 262,144 entries)
+        part = slice(first, first + 128)
+        want, size = p[:, part].t() @ rows, p[:, part].abs().t() @ rows.abs()
+        assert ((d_table[part].double() - want).abs() <= 2.0 ** -7 * size + 1e-6).all()
+    want = sum(p[:, i:i + 20_000] @ w.detach()[i:i + 20_000].double() for i in range(0, t, 20_000))
+    size = sum(p[:, i:i + 20_000].abs() @ w.detach()[i:i + 20_000].double().abs() for i in range(0, t, 20_000))
+    assert ((d_rows[[0, 1, 3]].double() - want).abs() <= 2.0 ** -7 * size + 1e-6).all() and (d_rows[2] == 0).all()
 
 
 def test_refusals():

@@ -58,7 +58,8 @@ def _bytes(backward=None):
 
 BAD_DESC = [dict(abi_version=1), dict(dtype=1), dict(dtype=9), dict(index_dtype=2), dict(reduction=3), dict(reduction=-1), dict(num_rows=-1), dict(num_rows=1 << 28),
             dict(num_entries=-1), dict(num_entries=1 << 31), dict(num_channels=0), dict(num_channels=1 << 17), dict(scale=NAN), dict(scale=float("inf")), dict(rows_stride=-1),
-            dict(table_stride=-1), dict(table_stride=1 << 41)]
+            dict(table_stride=-1), dict(table_stride=1 << 41),
+            dict(dtype=2, num_rows=20_000_000, num_entries=2_000_000_000)]
 BAD_CALL = [dict(ctx=None), dict(table=None), dict(table=AT + 1), dict(kept=None), dict(kept=AT + 128), dict(kept_size=_bytes() - 1), dict(workspace=None), dict(workspace=AT + 128)]
 
 

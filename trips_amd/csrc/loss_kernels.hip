@@ -1340,6 +1340,22 @@ int check_stride(const char* name, int64_t stride, int64_t row, int64_t rows, bo
     return TRIPS_OK;
 }
 
+// A launch's units are numbered in 31 bits.
+int check_units(const TripsTableLossDesc& d)
+{
+    for (int grads = 0; grads < 2; ++grads)
+    {
+        const double units = with_shape(d, grads, [&](auto shape)
+        {
+            using S = decltype(shape);
+            const double rows = (double)(up(d.num_rows, S::BN) / S::BN), entries = (double)(up(d.num_entries, S::BN) / S::BN), channels = (double)(up(d.num_channels, S::BM) / S::BM);
+            return grads ? channels * (rows * 64.0 + entries) : rows * entries;
+        });
+        if (units >= 2147000000.0) return set_error(TRIPS_ERR_UNSUPPORTED, "%lld rows and %lld entries are too many for one call", (long long)d.num_rows, (long long)d.num_entries);
+    }
+    return TRIPS_OK;
+}
+
 int check_desc(const TripsTableLossDesc* d)
 {
     if (!d) return set_error(TRIPS_ERR_INVALID_ARG, "desc is NULL");
@@ -1352,7 +1368,8 @@ int check_desc(const TripsTableLossDesc* d)
     if (d->num_channels < 1 || d->num_channels >= kMostChannels) return set_error(TRIPS_ERR_INVALID_ARG, "num_channels = %d", d->num_channels);
     if (!(d->scale - d->scale == 0.f)) return set_error(TRIPS_ERR_INVALID_ARG, "scale is not finite");
     if (int e = check_stride("rows_stride", d->rows_stride, d->num_channels, d->num_rows, false)) return e;
-    return check_stride("table_stride", d->table_stride, d->num_channels, d->num_entries, false);
+    if (int e = check_stride("table_stride", d->table_stride, d->num_channels, d->num_entries, false)) return e;
+    return check_units(*d);
 }
 
 int check_pointer(const char* name, const void* p, size_t align, bool needed)
