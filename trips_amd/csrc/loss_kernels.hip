@@ -623,6 +623,29 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
 
     // ---- a unit's products ----
     Acc acc[S::FM][S::FN];
+    // Of the lane's rows of the second operand (LOGITS, PROBS): asked for before a unit's first step and there behind its first meeting. (A wait for
+    // a load waits for all that went before it, and as the compiler counts them for those behind it too: when the results are written, the next unit's.)
+    int target[S::FN];
+    float2 state[S::FN];
+    auto ask = [&](const Unit& u)
+    {
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j)
+        {
+            const long long n = min((long long)u.y * S::BN + wn + j * 32 + (lane & 31), count - 1ll);
+            target[j]         = p.kept.target[n];
+            if (KIND == PROBS) state[j] = p.kept.state[n];
+        }
+    };
+    auto receive = [&]()
+    {
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j)
+        {
+            asm volatile("" : "+v"(target[j]));
+            if (KIND == PROBS) asm volatile("" : "+v"(state[j].x), "+v"(state[j].y));
+        }
+    };
     auto products = [&](auto along, int steps)
     {
         using First  = std::conditional_t<KIND == GRADS, FirstAcross, FirstAlong>;
@@ -671,6 +694,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                 else
                 {
                     wait_and_meet<(S::STAGES - 2) * LOADS>();
+                    if (KIND != GRADS && step == 0) receive();
                     if (ragged && step + 2 == steps) clear_ends(next);
                     read(0, next, 0);  // (behind the last step: of the next unit, which reads it again)
                 }
@@ -711,7 +735,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         for (int j = 0; j < S::FN; ++j)
         {
             const long long n = n0 + wn + j * 32 + (lane & 31);
-            const int own     = n < count ? p.kept.target[n] - p.first_entry - m_lane : -1;  // (of the lane's own elements)
+            const int own     = n < count ? target[j] - p.first_entry - m_lane : -1;  // (of the lane's own elements)
             float top         = -__builtin_inff();
             if (m0 + S::BM > p.in_piece)
                 each_element<S::FM>([&](int i, int e, int m)
@@ -769,15 +793,14 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             const long long n = n0 + wn + j * 32 + (lane & 31);
             if constexpr (MODE == PROBS)
             {
-                float2 state = make_float2(0.f, 0.f);
-                float factor = 0.f;
-                int own      = -1;
-                if (n < count) state = p.kept.state[n], factor = held_factor<D>(p.upstream, p.upstream.reduction == TRIPS_REDUCE_NONE ? p.kept.row[n] : 0), own = p.kept.target[n] - p.first_entry - m_lane;
-                const float less = -state.x * p.scale_log2, held = D == TRIPS_DTYPE_F16 ? factor : 1.f;
+                const float2 of = state[j];
+                const int own      = n < count ? target[j] - p.first_entry - m_lane : -1;
+                const float factor = held_factor<D>(p.upstream, p.upstream.reduction == TRIPS_REDUCE_NONE ? p.kept.row[min(n, count - 1ll)] : 0);
+                const float less   = -of.x * p.scale_log2, held = D == TRIPS_DTYPE_F16 ? factor : 1.f;
                 if (D != TRIPS_DTYPE_F32 && fabsf(less) < kFar)
-                    each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], p.scale_log2, less - state.y)) * held; });
+                    each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], p.scale_log2, less - of.y)) * held; });
                 else
-                    each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - state.x, p.scale_log2, -state.y)) * held; });
+                    each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - of.x, p.scale_log2, -of.y)) * held; });
                 if (D != TRIPS_DTYPE_F16 && p.upstream.reduction == TRIPS_REDUCE_NONE) each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] *= factor; });
                 if (__any(own >= 0 && own < S::TM))
                     each_element<S::FM>([&](int i, int e, int m)
@@ -883,11 +906,13 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         if (u.mode < 0) break;
         if constexpr (KIND == LOGITS)
         {
+            ask(u);
             products(std::true_type{}, u.steps);
             sums(u);
         }
         else if constexpr (KIND == PROBS)
         {
+            ask(u);
             products(std::true_type{}, u.steps);
             written(std::integral_constant<int, PROBS>{}, u);
         }
