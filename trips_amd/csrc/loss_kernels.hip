@@ -434,6 +434,16 @@ __device__ __forceinline__ void each_element(F f)
         for (int e = 0; e < 16; ++e) f(i, e, i * 32 + 8 * (e >> 2) + (e & 3));
 }
 
+// Two numbers rounded to 16 bits, side by side.
+template <int D>
+__device__ __forceinline__ unsigned pair_of(float a, float b)
+{
+    using Type = std::conditional_t<D == TRIPS_DTYPE_BF16, __bf16, _Float16>;
+    typedef Type Two __attribute__((ext_vector_type(2)));
+    typedef float Floats __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(Floats{a, b}, Two));
+}
+
 // A workgroup's share of a launch: its tiles, one after the other.
 struct Unit
 {
@@ -752,10 +762,8 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                 });
                 if (here) p.own_product[n] = product;
             }
-            each_element<S::FM>([&](int i, int e, int)
-            {
-                if (e % 2) top = fmaxf(top, fmaxf(acc[i][j][e - 1], acc[i][j][e]));
-            });
+            // (the larger: fmaxf would first quiet each product's NaN by an operation of its own)
+            each_element<S::FM>([&](int i, int e, int) { top = __builtin_amdgcn_fmed3f(top, acc[i][j][e], __builtin_inff()); });
             top              = fmaxf(top, __shfl_xor(top, 32));
             const float base = top == -__builtin_inff() ? 0.f : top, less = -base * p.scale_log2;
             float sum        = 0.f;
@@ -832,7 +840,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                         }
                     }
                 }
-                else if constexpr (D == TRIPS_DTYPE_F32)
+                if constexpr (MODE != D_ROWS && D == TRIPS_DTYPE_F32)
                 {
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
@@ -856,46 +864,43 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                         }
                     }
                 }
-                else
+            }
+            if constexpr (D != TRIPS_DTYPE_F32 && MODE != D_ROWS)
+            {
+                // Two lanes' fours to eight of one lane: 16 bytes, 32 of each of 32 rows at a time. (Turned in LDS to runs of 128 bytes before they were stored,
+                // the logits' gradient took 999 us where it takes 857 so: its wavefronts have nothing to do while they wait for LDS.)
+                using T8 = Pack<unsigned short, 8>::type;
+                auto out = [&](auto value, T* to, long long stride, long long rows, int columns)
                 {
-                    // two lanes' fours to eight of one lane: 16 bytes
 #pragma unroll
-                    for (int g = 0; g < 4; g += 2)
-                    {
-                        auto eight_of = [&](auto value)
+                    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                        for (int g = 0; g < 4; g += 2)
                         {
                             unsigned w[4];
 #pragma unroll
-                            for (int h = 0; h < 4; ++h) w[h] = (unsigned)value(4 * g + 2 * h) | (unsigned)value(4 * g + 2 * h + 1) << 16;
+                            for (int h = 0; h < 4; ++h) w[h] = pair_of<D>(value(acc[i][j][4 * g + 2 * h]), value(acc[i][j][4 * g + 2 * h + 1]));
                             const auto low = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), high = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-                            return Words4{(int)low[0], (int)high[0], (int)low[1], (int)high[1]};
-                        };
-                        const Words4 eight = eight_of([&](int e) { return E::from_float(acc[i][j][e] * unscale); });
-                        const int m        = m0 + wm + i * 32 + 8 * (g + (lane >> 5));
-                        if constexpr (MODE == PROBS)
-                        {
-                            T* at = reinterpret_cast<T*>(p.probs) + n * p.piece + m;
-                            if (n < count) *reinterpret_cast<Words4*>(at) = eight;
-                            if (p.parts > 1)
-                            {
-                                const Words4 rest = eight_of([&](int e) { return E::from_float(acc[i][j][e] - E::to_float(E::from_float(acc[i][j][e]))); });
-                                if (n < count) *reinterpret_cast<Words4*>(at + p.rows_pad * p.piece) = rest;
-                            }
-                        }
-                        else if (n < p.in_piece && m < p.channels)
-                        {
-                            T* at      = reinterpret_cast<T*>(p.d_table) + n * p.d_table_stride + m;
-                            using T8   = typename Pack<T, 8>::type;
-                            const T8 v = __builtin_bit_cast(T8, eight);
-                            if (m + 8 <= p.channels)
-                                *reinterpret_cast<T8*>(at) = v;
+                            const T8 v  = __builtin_bit_cast(T8, Words4{(int)low[0], (int)high[0], (int)low[1], (int)high[1]});
+                            const int m = m0 + wm + i * 32 + 8 * (g + (lane >> 5));
+                            T* x        = to + n * stride + m;
+                            if (n >= rows || m >= columns) continue;
+                            if (m + 8 <= columns)
+                                *reinterpret_cast<T8*>(x) = v;
                             else
 #pragma unroll
                                 for (int e = 0; e < 8; ++e)
-                                    if (m + e < p.channels) at[e] = v[e];
+                                    if (m + e < columns) x[e] = v[e];
                         }
-                    }
+                };
+                if constexpr (MODE == PROBS)
+                {
+                    T* to = reinterpret_cast<T*>(p.probs);
+                    out([](float x) { return x; }, to, p.piece, count, 0x7fffffff);
+                    if (p.parts > 1) out([](float x) { return x - E::to_float(E::from_float(x)); }, to + p.rows_pad * p.piece, p.piece, count, 0x7fffffff);
                 }
+                else
+                    out([&](float x) { return x * unscale; }, reinterpret_cast<T*>(p.d_table), p.d_table_stride, p.in_piece, p.channels);
             }
         }
     };
