@@ -78,7 +78,7 @@ def test_scales(dtype, scale):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("n", [16_384, 16_400, 9_000])
+@pytest.mark.parametrize("n", [16_384, 16_400, 9_000, 20_480, 20_481, 21_530])
 def test_many_rows(n, dtype):
     _check(*_inputs(n, 60, 24, dtype, 0.4), reduction="mean")
 

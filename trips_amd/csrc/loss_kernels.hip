@@ -30,7 +30,7 @@ constexpr double kLog2  = 0.6931471805599453;
 
 constexpr int kGatherRows = 16;     // rows of a workgroup
 constexpr int kChunk      = 1024;   // targets of a chunk that count_kernel counts
-constexpr int kCountedBy  = 8192;   // rows from which the chunks are counted beforehand
+constexpr int kCountedBy  = 8192;   // rows from which the chunks are counted beforehand (losses of 8191 rows of 16 floats 15.7 us without, 16.8 with; of 12,000 19.5 and 18.2)
 
 // What the forward call leaves for the backward call; "packed" is an index among the rows that count.
 struct Kept
