@@ -83,6 +83,13 @@ def test_many_rows(n, dtype):
     _check(*_inputs(n, 60, 24, dtype, 0.4), reduction="mean")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,t,c,pad", [(20_000, 150, 16, 0), (16_384, 2, 100, 3), (12_001, 65, 33, 0), (3000, 7, 700, 1), (9000, 129, 257, 0)])
+def test_few_entries_of_many_rows(n, t, c, pad, dtype):
+    """The table's gradient is a sum over many rows: cut into parts."""
+    _check(*_inputs(n, t, c, dtype, 0.3, pad=pad), scale=-0.7, reduction="none" if t == 65 else "mean")
+
+
 def test_no_rows_and_no_entries():
     for dtype in TYPES.values():
         x, w = torch.zeros(0, 8, dtype=dtype, device="cuda", requires_grad=True), torch.randn(5, 8, device="cuda").to(dtype).requires_grad_()

@@ -245,11 +245,12 @@ struct ProductParams
     float* own_product;  // [rows_pad]
     void* probs;         // [parts][rows_pad][piece], in the tensors' type
     float* slabs;        // D_ROWS: [splits][rows_pad][kp]
+    float* table_slabs;  // D_TABLE, where table_splits > 1: [table_splits][piece][kp]
     const void* d_rows;  // whether they are wanted
     void* d_table;
     long long table_stride, d_table_stride, rows_pad;
     int held;  // channels that a row of the table has: those, or of a copy with zeros behind them to 16 bytes
-    int first_entry, in_piece, channels, kp, piece, first_tile, splits, parts, add;
+    int first_entry, in_piece, channels, kp, piece, first_tile, splits, table_splits, parts, add;
     float scale_log2;
 };
 
@@ -293,6 +294,10 @@ struct Shape
     static constexpr int FIRST_LOADS = FIRST_BYTES / 1024 / WAVES, SECOND_LOADS = SECOND_BYTES / 1024 / WAVES;
     static_assert(FIRST_LOADS * WAVES * 1024 == FIRST_BYTES && SECOND_LOADS * WAVES * 1024 == SECOND_BYTES, "whole loads of a wavefront");
 };
+
+using Big   = Shape<256, 256, 2, 4, 2, 1>;
+using Small = Shape<128, 128, 2, 2, 2, 2>;
+using Tiny  = Shape<64, 64, 2, 2, 4, 2>;
 
 typedef int Words4 __attribute__((ext_vector_type(4)));
 typedef short Half4 __attribute__((ext_vector_type(4)));
@@ -460,6 +465,9 @@ __device__ __forceinline__ void place(Unit& u, int id, int across, int down)
     u.x = in / high, u.y = g * 8 + in % high;
 }
 
+// Where part z of `steps` in `parts` begins.
+__device__ __forceinline__ int part_begin(int z, int steps, int parts) { return (int)((long long)z * steps / parts); }
+
 // The units of worker w of `all`: unit w, w + all, ... of the larger kind (a of them, size_a steps each), then those of the smaller kind: workers
 // that have one of the larger kind less take so many smaller ones first.
 struct Share
@@ -505,13 +513,15 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
     const int worker = run + (runs % 8 ? in_run : in_run % 8 * (runs / 8) + in_run / 8);
     const int row_tiles = (count + S::BN - 1) / S::BN, entry_tiles = (p.in_piece + (KIND == GRADS ? S::BN : S::BM) - 1) / (KIND == GRADS ? S::BN : S::BM);
     const int channel_tiles = (p.channels + S::BM - 1) / S::BM;
-    const int piece_steps   = (p.in_piece + BK - 1) / BK;
+    const int piece_steps = (p.in_piece + BK - 1) / BK, row_steps = (count + BK - 1) / BK;
+    constexpr bool TABLE_SPLITS = KIND == GRADS && S::BM < Big::BM;  // (tiles of 256 make units enough by themselves)
+    const int table_splits      = TABLE_SPLITS ? p.table_splits : 1;
     Share share{};
     bool rows_first = true;
     if constexpr (KIND == GRADS)
     {
-        const int rows = p.d_rows ? channel_tiles * row_tiles * p.splits : 0, table = p.d_table ? channel_tiles * entry_tiles : 0;
-        const int rows_size = piece_steps / p.splits, table_size = (count + BK - 1) / BK;
+        const int rows = p.d_rows ? channel_tiles * row_tiles * p.splits : 0, table = p.d_table ? channel_tiles * entry_tiles * table_splits : 0;
+        const int rows_size = piece_steps / p.splits, table_size = row_steps / table_splits;
         rows_first = rows_size >= table_size;
         share      = rows_first ? Share{rows, rows_size, table, table_size} : Share{table, table_size, rows, rows_size};
     }
@@ -533,12 +543,12 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             if (u.mode == D_ROWS)
             {
                 place(u, id, channel_tiles, row_tiles);
-                u.steps = (int)((long long)(u.z + 1) * piece_steps / p.splits) - (int)((long long)u.z * piece_steps / p.splits);
+                u.steps = part_begin(u.z + 1, piece_steps, p.splits) - part_begin(u.z, piece_steps, p.splits);
             }
             else
             {
                 place(u, id, channel_tiles, entry_tiles);
-                u.steps = (count + BK - 1) / BK;
+                u.steps = part_begin(u.z + 1, row_steps, table_splits) - part_begin(u.z, row_steps, table_splits);
             }
         }
         else
@@ -580,16 +590,16 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         else if (u.mode == D_ROWS)
         {
             if (ahead_mode != u.mode) FirstAcross::begin(first, stride, wave, lane), SecondAlong::begin(second, piece, wave, lane);
-            const long long k = (long long)u.z * piece_steps / p.splits * BK, m0 = (long long)u.x * S::BM * SIZE, n0 = (long long)u.y * S::BN;
+            const long long k = (long long)part_begin(u.z, piece_steps, p.splits) * BK, m0 = (long long)u.x * S::BM * SIZE, n0 = (long long)u.y * S::BN;
             first.at(table + k * stride + m0, (p.in_piece - 1 - k) * stride + held - m0);
             second.at(part + n0 * piece + k * SIZE, (p.rows_pad - n0) * piece - k * SIZE);
         }
         else
         {
             if (ahead_mode != u.mode) FirstAcross::begin(first, wide, wave, lane), SecondAcross::begin(second, piece, wave, lane);
-            const long long m0 = (long long)u.x * S::BM * SIZE, n0 = (long long)u.y * S::BN * SIZE;
-            first.at(packed + m0, count * wide - m0);
-            second.at(part + n0, count * piece - n0);
+            const long long k = (long long)part_begin(u.z, row_steps, table_splits) * BK, m0 = (long long)u.x * S::BM * SIZE, n0 = (long long)u.y * S::BN * SIZE;
+            first.at(packed + k * wide + m0, (count - k) * wide - m0);
+            second.at(part + k * piece + n0, (count - k) * piece - n0);
         }
         ahead_mode = u.mode;
     };
@@ -794,6 +804,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         constexpr int MODE = decltype(mode)::value;
         const long long n0 = (long long)u.y * S::BN;
         const int m0 = u.x * S::BM, m_lane = m0 + wm + 4 * (lane >> 5);
+        const bool in_slabs = TABLE_SPLITS && MODE == D_TABLE && table_splits > 1;
         const float unscale = MODE == D_TABLE ? unheld<D>(p.upstream, p.kept.count) * fabsf(p.upstream.scale) : 1.f;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
@@ -824,21 +835,23 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
 #pragma unroll
             for (int i = 0; i < S::FM; ++i)
             {
-                if constexpr (MODE == D_ROWS)
+                if (MODE == D_ROWS || in_slabs)
                 {
+                    float* slab = MODE == D_ROWS ? p.slabs + ((long long)u.z * p.rows_pad + n) * p.kp : p.table_slabs + ((long long)u.z * p.piece + n) * p.kp;
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
                     {
                         const int c = m_lane + i * 32 + 8 * g;
                         using F4    = Pack<float, 4>::type;
-                        if (n < count && c < p.kp)
+                        if (n < (MODE == D_ROWS ? count : p.in_piece) && c < p.kp)
                         {
-                            F4* at = reinterpret_cast<F4*>(p.slabs + ((long long)u.z * p.rows_pad + n) * p.kp + c);
+                            F4* at = reinterpret_cast<F4*>(slab + c);
                             F4 v   = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                            if (p.add) v += *at;
+                            if (MODE == D_ROWS && p.add) v += *at;
                             *at = v;
                         }
                     }
+                    continue;
                 }
                 if constexpr (MODE != D_ROWS && D == TRIPS_DTYPE_F32)
                 {
@@ -867,6 +880,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             }
             if constexpr (D != TRIPS_DTYPE_F32 && MODE != D_ROWS)
             {
+                if (in_slabs) continue;
                 // Two lanes' fours to eight of one lane: 16 bytes, 32 of each of 32 rows at a time. (Turned in LDS to runs of 128 bytes before they were stored,
                 // the logits' gradient took 999 us where it takes 857 so: its wavefronts have nothing to do while they wait for LDS.)
                 using T8 = Pack<unsigned short, 8>::type;
@@ -1021,22 +1035,23 @@ __global__ __launch_bounds__(1024) void sum_kernel(const double* from, int n, co
     *loss = (float)(reduction == TRIPS_REDUCE_MEAN ? sum / (double)max(*count, 1) : sum);
 }
 
-// d_rows: the splits' sums, in their order, at their rows' own places; four channels a lane.
+// d_rows: the splits' sums, in their order, at their rows' own places (place; NULL for d_table's splits, whose entries are where they belong);
+// four channels a lane.
 template <int D>
-__global__ __launch_bounds__(256) void rows_out_kernel(const float* slabs, const Kept kept, const Upstream upstream, void* d_rows, long long n, long long rows_pad,
-                                                       long long stride, int channels, int kp, int splits)
+__global__ __launch_bounds__(256) void slabs_out_kernel(const float* slabs, const int* place, const int* count, const Upstream upstream, float scale, void* out_rows, long long n,
+                                                        long long rows_pad, long long stride, int channels, int kp, int splits)
 {
     using E  = Element<D>;
     using T  = typename E::type;
     using F4 = Pack<float, 4>::type;
     using T4 = typename Pack<T, 4>::type;
-    const float f       = unheld<D>(upstream, kept.count) * upstream.scale;
+    const float f       = unheld<D>(upstream, count) * scale;
     const int quads     = (channels + 3) >> 2;
     const long long all = n * quads, slab = rows_pad * kp;
     for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < all; q += (long long)gridDim.x * 256)
     {
         const long long i = q / quads;
-        const int c = (int)(q - i * quads) * 4, at = kept.place[i];
+        const int c = (int)(q - i * quads) * 4, at = place ? place[i] : (int)i;
         F4 sum = {0.f, 0.f, 0.f, 0.f};
         if (at >= 0)
         {
@@ -1044,7 +1059,7 @@ __global__ __launch_bounds__(256) void rows_out_kernel(const float* slabs, const
 #pragma unroll 4
             for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const F4*>(from + s * slab);
         }
-        T* to = reinterpret_cast<T*>(d_rows) + i * stride + c;
+        T* to = reinterpret_cast<T*>(out_rows) + i * stride + c;
         T4 out;
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = E::from_float(at >= 0 ? sum[e] * f : 0.f);
@@ -1062,6 +1077,7 @@ __global__ __launch_bounds__(256) void rows_out_kernel(const float* slabs, const
 constexpr int64_t kPieceBytes = 1ll << 30;  // of d_ij
 constexpr int64_t kSlabBytes  = 256ll << 20;  // of the parts of the rows' gradients
 constexpr int kCus            = 256;
+constexpr int kMostSplits     = 64;
 constexpr int64_t kCopyBytes = 64ll << 20, kLeastCopyBytes = 16ll << 20;  // of copied entries
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -1107,14 +1123,10 @@ size_t kept_of(const TripsTableLossDesc& d, void* kept, Kept* k)
 struct Layout
 {
     int64_t rows_pad, chunks, piece, pieces;
-    int kp, tiles, splits, parts;
+    int kp, tiles, splits, table_splits, parts;
     bool copies;
-    size_t chunk_count, top, partial, own_product, sums, probs, slabs, copy, bytes;
+    size_t chunk_count, top, partial, own_product, sums, probs, slabs, table_slabs, copy, bytes;
 };
-
-using Big   = Shape<256, 256, 2, 4, 2, 1>;
-using Small = Shape<128, 128, 2, 2, 2, 2>;
-using Tiny  = Shape<64, 64, 2, 2, 4, 2>;
 
 // f(a shape): the largest tiles of which a product of `down` x `across` makes one for each CU at least; never the largest in 32 bits, whose
 // products take so long that the loads do not count, nor for rows that half of one holds (32 rows of 50,000 entries of 1024 channels:
@@ -1147,9 +1159,13 @@ int parts_of(const TripsTableLossDesc& d)
     return little || with_shape(d, true, [](auto shape) { return decltype(shape)::BM == Tiny::BM; }) ? 2 : 1;
 }
 
-// Into how many parts the rows' gradients are cut along the entries, so that they and the table's gradients keep all CUs busy to the end,
-// by what a step and a unit's results take, and the parts' way to memory and back.
-int splits_of(const TripsTableLossDesc& d, int64_t rows_pad, int64_t piece, int kp)
+// Into how many parts the rows' gradients are cut along the entries, and the table's along the rows where its tiles are few, so that they keep all
+// CUs busy to the end, by what a step and a unit's results take, and the parts' way to memory and back.
+struct Splits
+{
+    int rows, table;
+};
+Splits splits_of(const TripsTableLossDesc& d, int64_t rows_pad, int64_t piece, int kp)
 {
     return with_shape(d, true, [&](auto shape)
     {
@@ -1157,16 +1173,27 @@ int splits_of(const TripsTableLossDesc& d, int64_t rows_pad, int64_t piece, int 
         const bool wide       = d.dtype == TRIPS_DTYPE_F32;
         const int step_k      = kStepBytes / dtype_bytes(d.dtype), workers = kCus * S::PER_CU;
         const double step     = (wide ? 4.0 : S::BM == 256 ? 1.6 : 0.8) * (S::BM == 64 ? 0.25 : 1.0);  // microseconds
-        const double results  = S::BM == 256 ? 10.0 : S::BM == 128 ? 4.0 : 2.0, slab = (double)rows_pad * kp * 4;
-        const int64_t units = up(d.num_rows, S::BN) / S::BN * (up(d.num_channels, S::BM) / S::BM), steps = piece / step_k;
-        const int64_t table_units = piece / S::BN * (up(d.num_channels, S::BM) / S::BM), table_steps = up(d.num_rows, step_k) / step_k;
-        int best     = 1;
+        const double results  = S::BM == 256 ? 10.0 : S::BM == 128 ? 4.0 : 2.0, slab = (double)rows_pad * kp * 4, table_slab = (double)piece * kp * 4;
+        const int64_t channel_tiles = up(d.num_channels, S::BM) / S::BM, units = up(d.num_rows, S::BN) / S::BN * channel_tiles, steps = piece / step_k;
+        const int64_t table_tiles = up(std::min(piece, d.num_entries), S::BN) / S::BN * channel_tiles, table_steps = up(d.num_rows, step_k) / step_k;
+        int table    = 1;
         double least = 1e300;
-        for (int s = 1; s <= 64 && (s == 1 || (steps / s >= 4 && slab * s <= (double)kSlabBytes)); ++s)
+        for (int s = 1; s <= kMostSplits && (s == 1 || (S::BM < Big::BM && table_tiles * (s - 1) < workers && table_steps / s >= 4 && table_slab * s <= (double)kSlabBytes)); ++s)
+        {
+            // a unit's time, no less than a share of everything; the parts' way to memory and back
+            const double unit = (double)((table_steps + s - 1) / s) * step + results;
+            const double all  = ((double)(units * steps + table_tiles * table_steps) * step + (double)table_tiles * s * results) / workers;
+            const double end  = std::max(unit, all) + (s > 1 ? 3.0 + s * table_slab / 3.5e6 : 0.0);
+            if (end < least) table = s, least = end;
+        }
+        const int64_t table_units = table_tiles * table;
+        int best = 1;
+        least    = 1e300;
+        for (int s = 1; s <= kMostSplits && (s == 1 || (steps / s >= 4 && slab * s <= (double)kSlabBytes)); ++s)
         {
             // the larger units first, each to the first workgroup that is free
             int64_t a = units * s, b = table_units;
-            double size_a = (double)((steps + s - 1) / s) * step + results, size_b = (double)table_steps * step + results;
+            double size_a = (double)((steps + s - 1) / s) * step + results, size_b = (double)((table_steps + table - 1) / table) * step + results;
             if (size_a < size_b) std::swap(a, b), std::swap(size_a, size_b);
             const int64_t rest = a % workers;
             const double full  = (double)(a / workers) * size_a;
@@ -1184,7 +1211,7 @@ int splits_of(const TripsTableLossDesc& d, int64_t rows_pad, int64_t piece, int 
             end += s * slab / 3.5e6;
             if (end < least) best = s, least = end;
         }
-        return best;
+        return Splits{best, table};
     });
 }
 
@@ -1219,8 +1246,10 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     {
         l.top   = take(4);
         l.probs = take((size_t)l.parts * l.rows_pad * l.piece * size);
-        l.splits = splits_of(d, l.rows_pad, l.piece, l.kp);
-        l.slabs  = take((size_t)l.splits * l.rows_pad * l.kp * 4);
+        const Splits s = splits_of(d, l.rows_pad, l.piece, l.kp);
+        l.splits = s.rows, l.table_splits = s.table;
+        l.slabs = take((size_t)l.splits * l.rows_pad * l.kp * 4);
+        if (l.table_splits > 1) l.table_slabs = take((size_t)l.table_splits * l.piece * l.kp * 4);
     }
     l.bytes = take.at;
     return l;
@@ -1263,9 +1292,9 @@ ProductParams product_params(const TripsTableLossDesc& d, const Layout& l, const
 {
     ProductParams p{};
     p.kept = kept;
-    p.partial = (float2*)(w + l.partial), p.own_product = (float*)(w + l.own_product), p.probs = w + l.probs, p.slabs = (float*)(w + l.slabs);
+    p.partial = (float2*)(w + l.partial), p.own_product = (float*)(w + l.own_product), p.probs = w + l.probs, p.slabs = (float*)(w + l.slabs), p.table_slabs = (float*)(w + l.table_slabs);
     p.d_table_stride = d.d_table_stride, p.rows_pad = l.rows_pad;
-    p.channels = d.num_channels, p.kp = l.kp, p.piece = (int)l.piece, p.splits = l.splits, p.parts = l.parts;
+    p.channels = d.num_channels, p.kp = l.kp, p.piece = (int)l.piece, p.splits = l.splits, p.table_splits = l.table_splits, p.parts = l.parts;
     p.scale_log2 = scale_log2(d);
     return p;
 }
@@ -1298,7 +1327,7 @@ hipError_t launch_product(const TripsTableLossDesc& d, const ProductParams& p, h
         // (no code for what with_shape() does not give)
         using S = std::conditional_t<D == TRIPS_DTYPE_F32 && Given::BM == 256, Small, Given>;
         const int64_t row_tiles = tiles_of(d.num_rows, S::BN), channel_tiles = tiles_of(d.num_channels, S::BM);
-        const int64_t units = KIND == GRADS ? channel_tiles * ((p.d_rows ? row_tiles * p.splits : 0) + (p.d_table ? tiles_of(p.in_piece, S::BN) : 0)) : tiles_of(p.in_piece, S::BM) * row_tiles;
+        const int64_t units = KIND == GRADS ? channel_tiles * ((p.d_rows ? row_tiles * p.splits : 0) + (p.d_table ? tiles_of(p.in_piece, S::BN) * p.table_splits : 0)) : tiles_of(p.in_piece, S::BM) * row_tiles;
         if (units == 0) return hipSuccess;
         ProfScope scope(prof, KIND == LOGITS ? "loss_logits" : KIND == PROBS ? "loss_probs" : "loss_grads", stream);
         product_kernel<D, KIND, S><<<(unsigned)std::min<int64_t>(units, S::PER_CU * kCus), S::WAVES * 64, 0, stream>>>(p);
@@ -1338,6 +1367,16 @@ hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* ta
 }
 
 template <int D>
+hipError_t slabs_out(const TripsTableLossDesc& d, const Layout& l, const char* name, const float* slabs, const Kept& kept, const Upstream& upstream, float scale, bool placed, void* out,
+                     int64_t n, int64_t rows_pad, int64_t stride, int splits, hipStream_t stream, Profiler* prof)
+{
+    ProfScope scope(prof, name, stream);
+    slabs_out_kernel<D><<<(unsigned)std::min<int64_t>((n * ((d.num_channels + 3) / 4) + 255) / 256, 1 << 16), 256, 0, stream>>>(
+        slabs, placed ? kept.place : nullptr, kept.count, upstream, scale, out, n, rows_pad, stride, d.num_channels, l.kp, splits);
+    return hipGetLastError();
+}
+
+template <int D>
 hipError_t backward(const TripsTableLossDesc& d, const void* table, const Kept& kept, const float* d_loss, void* d_rows, void* d_table, char* w, hipStream_t stream, Profiler* prof)
 {
     const Layout l  = layout_of(d, true, copies_of(d, table));
@@ -1355,12 +1394,13 @@ hipError_t backward(const TripsTableLossDesc& d, const void* table, const Kept& 
         if (hipError_t e = take_piece<D>(d, l, piece, table, d_table, w, p, stream, prof)) return e;
         if (hipError_t e = launch_product<D, PROBS>(d, p, stream, prof)) return e;
         if (hipError_t e = launch_product<D, GRADS>(d, p, stream, prof)) return e;
+        if (!d_table || l.table_splits == 1) continue;
+        if (hipError_t e = slabs_out<D>(d, l, "loss_table_out", p.table_slabs, kept, p.upstream, std::fabs(d.scale), false, p.d_table, p.in_piece, l.piece, d.d_table_stride,
+                                        l.table_splits, stream, prof))
+            return e;
     }
     if (!d_rows || d.num_rows == 0) return hipSuccess;
-    ProfScope scope(prof, "loss_rows_out", stream);
-    rows_out_kernel<D><<<(unsigned)std::min<int64_t>((d.num_rows * ((d.num_channels + 3) / 4) + 255) / 256, 1 << 16), 256, 0, stream>>>(
-        (float*)(w + l.slabs), kept, p.upstream, d_rows, d.num_rows, l.rows_pad, d.d_rows_stride, d.num_channels, l.kp, l.splits);
-    return hipGetLastError();
+    return slabs_out<D>(d, l, "loss_rows_out", (float*)(w + l.slabs), kept, p.upstream, d.scale, true, d_rows, d.num_rows, l.rows_pad, d.d_rows_stride, l.splits, stream, prof);
 }
 
 int check_stride(const char* name, int64_t stride, int64_t row, int64_t rows, bool written)
@@ -1379,7 +1419,7 @@ int check_units(const TripsTableLossDesc& d)
         {
             using S = decltype(shape);
             const double rows = (double)(up(d.num_rows, S::BN) / S::BN), entries = (double)(up(d.num_entries, S::BN) / S::BN), channels = (double)(up(d.num_channels, S::BM) / S::BM);
-            return grads ? channels * (rows * 64.0 + entries) : rows * entries;
+            return grads ? channels * (rows * kMostSplits + entries) + kCus * S::PER_CU : rows * entries;  // (see splits_of())
         });
         if (units >= 2147000000.0) return set_error(TRIPS_ERR_UNSUPPORTED, "%lld rows and %lld entries are too many for one call", (long long)d.num_rows, (long long)d.num_entries);
     }
