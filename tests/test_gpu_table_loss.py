@@ -84,6 +84,13 @@ def test_many_rows(n, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,t,c,pad", [(3, 17_000, 500, 0), (32, 9000, 70, 1), (33, 9001, 70, 0), (64, 9000, 140, 0), (65, 8500, 130, 5), (600, 33, 1000, 0), (40, 97, 2000, 1), (500, 31, 700, 0),
+                                       (2, 65, 9, 0)])
+def test_few_rows_or_few_tiles(n, t, c, pad, dtype):
+    _check(*_inputs(n, t, c, dtype, 0.2 if n > 3 else 0, pad=pad), scale=0.7, reduction="sum")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n,t,c,pad", [(20_000, 150, 16, 0), (16_384, 2, 100, 3), (12_001, 65, 33, 0), (3000, 7, 700, 1), (9000, 129, 257, 0)])
 def test_few_entries_of_many_rows(n, t, c, pad, dtype):
     """The table's gradient is a sum over many rows: cut into parts."""

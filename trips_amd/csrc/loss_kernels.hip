@@ -284,20 +284,28 @@ __global__ __launch_bounds__(256) void copy_entries_kernel(const T* table, long 
 
 constexpr int kStepBytes = 128, kRounds = 4;  // of a row along k in a step; a round of the matrix instructions takes a quarter of them
 
-// Tiles of BM x BN in steps along k, both operands by direct loads to LDS, STAGES steps of them at a time; WM x WN wavefronts, PER_CU such workgroups.
-template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int PER_CU_>
+// Tiles of BM x BN in steps along k, both operands by direct loads to LDS, STAGES steps of them at a time; WM x WN wavefronts, WK of them along a step's
+// rounds, whose sums are joined behind the last step; PER_CU such workgroups.
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int PER_CU_, int WK_ = 1>
 struct Shape
 {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_, PER_CU = PER_CU_;
-    static constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_, PER_CU = PER_CU_, WK = WK_;
+    static constexpr int WAVES = WM * WN * WK, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
     static constexpr int FIRST_BYTES = BM * kStepBytes, SECOND_BYTES = BN * kStepBytes, STAGE_BYTES = FIRST_BYTES + SECOND_BYTES;
     static constexpr int FIRST_LOADS = FIRST_BYTES / 1024 / WAVES, SECOND_LOADS = SECOND_BYTES / 1024 / WAVES;
+    static_assert(WK == 1 || (WK == kRounds && WM * WN == 1), "a round of each step for each wavefront");
     static_assert(FIRST_LOADS * WAVES * 1024 == FIRST_BYTES && SECOND_LOADS * WAVES * 1024 == SECOND_BYTES, "whole loads of a wavefront");
 };
 
 using Big   = Shape<256, 256, 2, 4, 2, 1>;
 using Small = Shape<128, 128, 2, 2, 2, 2>;
 using Tiny  = Shape<64, 64, 2, 2, 4, 2>;
+// Of the gradients, whose units are many and may be of a few steps: a wavefront's waits for loads wait for the results stored before them too, which more
+// workgroups hide and deeper loads do not (8000 rows of 90 entries of 4000 bfloat16 channels 168 us with Tiny, 108 so; 130 with three of each).
+using Tight = Shape<64, 64, 2, 2, 2, 4>;
+// Of the logits where tiles of 64 leave CUs without one, or rows are few: the wavefronts share each step's products, not the tile (4000 rows of 10 entries
+// of 4000 floats 41 us, 89 with Tiny; 644 of 487 of 1596 28 and 40).
+using Deep = Shape<32, 32, 1, 1, 4, 3, 4>;
 
 typedef int Words4 __attribute__((ext_vector_type(4)));
 typedef short Half4 __attribute__((ext_vector_type(4)));
@@ -503,9 +511,11 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
     using SecondAcross = AcrossK<SIZE, S::BN, S::SECOND_LOADS>;
     __shared__ __attribute__((aligned(1024))) char lds[S::STAGES * S::STAGE_BYTES];
     __shared__ float2 joined[KIND == LOGITS ? S::WM * S::BN : 1];
+    __shared__ Acc others[S::WK > 1 ? S::WK - 1 : 1][S::WK > 1 ? 64 : 1];
     const unsigned lds_at = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave % S::WM * S::TM, wn = wave / S::WM * S::TN;
+    const bool writes = S::WK == 1 || wave == 0;
+    const int wm = wave % S::WM * S::TM, wn = wave / S::WM % S::WN * S::TN;
     const int count = *p.kept.count;
 
     // Workgroups as they start go around the eight XCDs: of each 256, which take a CU each, workers by XCD.
@@ -702,10 +712,25 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             meet();
         };
         if (ragged && steps == 1) clear_ends(stage);
-        if (steps > 0) read(0, stage, 0);
+        if (steps > 0) read(0, stage, S::WK > 1 ? wave : 0);
         for (int step = 0; step < steps; ++step)
         {
             const int next = stage + 1 == S::STAGES ? 0 : stage + 1, free = stage == 0 ? S::STAGES - 1 : stage - 1;
+            if constexpr (S::WK > 1)
+            {
+                // (each wavefront its own round of every step)
+#pragma unroll
+                for (int i = LOADS - LATE; i < LOADS; ++i) load(i, free);
+                if (LATE > 0) loaded_step();
+                acc[0][0] = product<D>(x[0][0], y[0][0], acc[0][0]);
+                wait_and_meet<(S::STAGES - 2) * LOADS>();
+                if (KIND != GRADS && step == 0) receive();
+                if (ragged && step + 2 == steps) clear_ends(next);
+                read(0, next, wave);
+#pragma unroll
+                for (int i = 0; i < LOADS - LATE; ++i) load(i, stage);
+            }
+            else
 #pragma unroll
             for (int kk = 0; kk < kRounds; ++kk)
             {
@@ -742,6 +767,14 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             if (LATE == 0) loaded_step();
             stage = next;
         }
+        if constexpr (S::WK > 1)
+        {
+            if (wave > 0) others[wave - 1][lane] = acc[0][0];
+            meet();
+            if (wave == 0)
+#pragma unroll
+                for (int w = 0; w < S::WK - 1; ++w) acc[0][0] += others[w][lane];
+        }
     };
 
     // ---- a unit's results ----
@@ -754,6 +787,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
         {
+            if (!writes) break;
             const long long n = n0 + wn + j * 32 + (lane & 31);
             const int own     = n < count ? target[j] - p.first_entry - m_lane : -1;  // (of the lane's own elements)
             float top         = -__builtin_inff();
@@ -786,7 +820,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         meet();  // (the last unit's have been read)
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
-            if (lane < 32) joined[wave % S::WM * S::BN + wn + j * 32 + lane] = best[j];
+            if (lane < 32 && writes) joined[wave % S::WM * S::BN + wn + j * 32 + lane] = best[j];
         meet();
         for (int n = threadIdx.x; n < S::BN; n += S::WAVES * 64)
         {
@@ -805,7 +839,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         const long long n0 = (long long)u.y * S::BN;
         const int m0 = u.x * S::BM, m_lane = m0 + wm + 4 * (lane >> 5);
         const bool in_slabs = TABLE_SPLITS && MODE == D_TABLE && table_splits > 1;
-        const float unscale = MODE == D_TABLE ? unheld<D>(p.upstream, p.kept.count) * fabsf(p.upstream.scale) : 1.f;
+        const float unscale = MODE == D_TABLE && !in_slabs ? unheld<D>(p.upstream, p.kept.count) * fabsf(p.upstream.scale) : 1.f;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
         {
@@ -933,7 +967,17 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         {
             ask(u);
             products(std::true_type{}, u.steps);
-            written(std::integral_constant<int, PROBS>{}, u);
+            if (writes) written(std::integral_constant<int, PROBS>{}, u);
+            // (zeros behind the piece's last entry to a whole step of the gradients)
+            if (S::BM < BK && wave == 1 && u.x + 1 == entry_tiles && entry_tiles % (BK / S::BM) != 0)
+            {
+                const long long n = (long long)u.y * S::BN + (lane & 31);
+                if (n < count)
+                    for (int part = 0; part < p.parts; ++part)
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            *reinterpret_cast<Words4*>(reinterpret_cast<T*>(p.probs) + (part * p.rows_pad + n) * p.piece + (u.x + 1) * S::BM + ((lane >> 5) * 2 + q) * 8) = Words4{};
+            }
         }
         else if (u.mode == D_ROWS)
         {
@@ -1130,8 +1174,11 @@ struct Layout
 
 // f(a shape): the largest tiles of which a product of `down` x `across` makes one for each CU at least; never the largest in 32 bits, whose
 // products take so long that the loads do not count, nor for rows that half of one holds (32 rows of 50,000 entries of 1024 channels:
-// gradients with d_ij in two parts 122 us, 98 with Small). (With four wavefronts of 128 x 128 the logits of 8191
-// rows and 50,000 entries of 1024 bfloat16 channels took 1084 us where eight take 870, the gradients 1475 and 1434.)
+// gradients with d_ij in two parts 122 us, 98 with Small). Few rows take smaller ones where a tile's products would be of rows that are not there: in
+// 32 bits (3 rows of 200,000 entries of 2000 floats, logits 848 us with Small, 388 with Deep, gradients 1451 and 1157 with Tight; 40 of 200,000 of 100,
+// gradients 238 and 101), in 16 the logits of up to 32 rows (one of 100,000 entries of 4000 channels 165 and 141; of 33 rows of 60,000 entries of 2000
+// 53 and 73). (With four wavefronts of 128 x 128 the logits of 8191 rows and 50,000 entries of 1024 bfloat16 channels took 1084 us where eight
+// take 870, the gradients 1475 and 1434.)
 template <typename F>
 auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
 {
@@ -1141,7 +1188,10 @@ auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
         return grads ? channels * entries : rows * entries;
     };
     if (d.dtype != TRIPS_DTYPE_F32 && d.num_rows > 128 && units(256) >= kCus) return f(Big{});
-    if (units(128) >= kCus) return f(Small{});
+    const bool wide = d.dtype == TRIPS_DTYPE_F32;
+    if (units(128) >= kCus && (grads || d.num_rows > 32) && (!wide || d.num_rows > 64)) return f(Small{});
+    if (grads) return f(Tight{});
+    if (d.num_rows <= 32 || units(64) < kCus) return f(Deep{});
     return f(Tiny{});
 }
 // Entries of a tile of the logits.
@@ -1172,7 +1222,7 @@ Splits splits_of(const TripsTableLossDesc& d, int64_t rows_pad, int64_t piece, i
         using S = decltype(shape);
         const bool wide       = d.dtype == TRIPS_DTYPE_F32;
         const int step_k      = kStepBytes / dtype_bytes(d.dtype), workers = kCus * S::PER_CU;
-        const double step     = (wide ? 4.0 : S::BM == 256 ? 1.6 : 0.8) * (S::BM == 64 ? 0.25 : 1.0);  // microseconds
+        const double step     = (wide ? 4.0 : S::BM == 256 ? 1.6 : 0.8) * (S::BM == 64 ? 0.5 : 1.0);  // microseconds
         const double results  = S::BM == 256 ? 10.0 : S::BM == 128 ? 4.0 : 2.0, slab = (double)rows_pad * kp * 4, table_slab = (double)piece * kp * 4;
         const int64_t channel_tiles = up(d.num_channels, S::BM) / S::BM, units = up(d.num_rows, S::BN) / S::BN * channel_tiles, steps = piece / step_k;
         const int64_t table_tiles = up(std::min(piece, d.num_entries), S::BN) / S::BN * channel_tiles, table_steps = up(d.num_rows, step_k) / step_k;
@@ -1325,7 +1375,7 @@ hipError_t launch_product(const TripsTableLossDesc& d, const ProductParams& p, h
     {
         using Given = decltype(shape);
         // (no code for what with_shape() does not give)
-        using S = std::conditional_t<D == TRIPS_DTYPE_F32 && Given::BM == 256, Small, Given>;
+        using S = std::conditional_t<D == TRIPS_DTYPE_F32 && Given::BM == 256, Small, std::conditional_t<KIND == GRADS && Given::BM <= Tiny::BM, Tight, std::conditional_t<KIND != GRADS && std::is_same<Given, Tight>::value, Tiny, Given>>>;
         const int64_t row_tiles = tiles_of(d.num_rows, S::BN), channel_tiles = tiles_of(d.num_channels, S::BM);
         const int64_t units = KIND == GRADS ? channel_tiles * ((p.d_rows ? row_tiles * p.splits : 0) + (p.d_table ? tiles_of(p.in_piece, S::BN) * p.table_splits : 0)) : tiles_of(p.in_piece, S::BM) * row_tiles;
         if (units == 0) return hipSuccess;
