@@ -1187,8 +1187,8 @@ struct Layout
 // products take so long that the loads do not count, nor for rows that half of one holds (32 rows of 50,000 entries of 1024 channels:
 // gradients with d_ij in two parts 122 us, 98 with Small). Few rows take smaller ones where a tile's products would be of rows that are not there: in
 // 32 bits (3 rows of 200,000 entries of 2000 floats, logits 848 us with Small, 388 with Deep, gradients 1451 and 1157 with Tight; 40 of 200,000 of 100,
-// gradients 238 and 101), in 16 the logits of up to 32 rows (one of 100,000 entries of 4000 channels 165 and 141; of 33 rows of 60,000 entries of 2000
-// 53 and 73). (With four wavefronts of 128 x 128 the logits of 8191 rows and 50,000 entries of 1024 bfloat16 channels took 1084 us where eight
+// gradients 238 and 101), in 16 the logits of up to 32 wide rows (one of 100,000 entries of 4000 channels 165 and 141, of 50,000 of 1024 21.0 and 21.8; 33 rows of
+// 60,000 entries of 2000 53 and 73). (With four wavefronts of 128 x 128 the logits of 8191 rows and 50,000 entries of 1024 bfloat16 channels took 1084 us where eight
 // take 870, the gradients 1475 and 1434.)
 template <typename F>
 auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
@@ -1200,9 +1200,10 @@ auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
     };
     if (d.dtype != TRIPS_DTYPE_F32 && d.num_rows > 128 && units(256) >= kCus) return f(Big{});
     const bool wide = d.dtype == TRIPS_DTYPE_F32;
-    if (units(128) >= kCus && (grads || d.num_rows > 32) && (!wide || d.num_rows > 64)) return f(Small{});
+    const bool few  = !grads && d.num_rows <= 32 && (wide || d.num_channels >= 2048);
+    if (units(128) >= kCus && !few && (!wide || d.num_rows > 64)) return f(Small{});
     if (grads) return f(Tight{});
-    if (d.num_rows <= 32 || units(64) < kCus) return f(Deep{});
+    if (few || units(64) < kCus) return f(Deep{});
     return f(Tiny{});
 }
 // Entries of a tile of the logits.
