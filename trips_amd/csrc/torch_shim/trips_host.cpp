@@ -411,7 +411,7 @@ void only_once(torch::autograd::variable_list& grads, const at::Tensor& upstream
 }
 
 // The function that a graph records (in Python, its two ways through the interpreter would take as long as the kernels of a small problem: 25 rows
-// of 5000 entries 104 us a pass, so 79).
+// of 5000 entries 104 us a pass, so 70).
 struct TableLoss : torch::autograd::Function<TableLoss>
 {
     static at::Tensor forward(torch::autograd::AutogradContext* own, const at::Tensor& rows, const at::Tensor& table, const at::Tensor& target, int64_t ctx, int64_t stream, double scale,
