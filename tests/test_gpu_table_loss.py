@@ -91,6 +91,13 @@ def test_few_rows_or_few_tiles(n, t, c, pad, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,t,c", [(1, 70_001, 8), (3, 300_000, 4), (30, 66_000, 5), (64, 140_000, 4), (65, 140_000, 4)])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_few_rows_of_very_many_entries(n, t, c, dtype, reduction):
+    _check(*_inputs(n, t, c, dtype, 0.3 if n > 3 else 0), reduction=reduction)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n,t,c,pad", [(20_000, 150, 16, 0), (16_384, 2, 100, 3), (12_001, 65, 33, 0), (3000, 7, 700, 1), (9000, 129, 257, 0)])
 def test_few_entries_of_many_rows(n, t, c, pad, dtype):
     """The table's gradient is a sum over many rows: cut into parts."""

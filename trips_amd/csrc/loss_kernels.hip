@@ -253,14 +253,14 @@ struct ProductParams
     const void* table;  // the piece's entries
     Kept kept;
     Upstream upstream;
-    float2* partial;     // LOGITS: [tiles of entries][rows_pad] {largest product, sum of exponentials}
+    float2* partial;     // LOGITS: [tiles of entries][partial_pad] {largest product, sum of exponentials}
     float* own_product;  // [rows_pad]
     void* probs;         // [parts][rows_pad][piece], in the tensors' type
     float* slabs;        // D_ROWS: [splits][rows_pad][kp]
     float* table_slabs;  // D_TABLE, where table_splits > 1: [table_splits][piece][kp]
     const void* d_rows;  // whether they are wanted
     void* d_table;
-    long long table_stride, d_table_stride, rows_pad;
+    long long table_stride, d_table_stride, rows_pad, partial_pad;
     int held;  // channels that a row of the table has: those, or of a copy with zeros behind them to 16 bytes
     int first_entry, in_piece, channels, kp, piece, first_tile, splits, table_splits, parts, add;
     float scale_log2;
@@ -848,7 +848,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             const float base = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
             for (int w = 0; w < S::WM; ++w) sum += joined[w * S::BN + n].y * part_of(joined[w * S::BN + n].x, base, p.scale_log2);
-            p.partial[(p.first_tile + u.x) * p.rows_pad + n0 + n] = make_float2(top, sum);
+            p.partial[(p.first_tile + u.x) * p.partial_pad + n0 + n] = make_float2(top, sum);
         }
     };
     auto written = [&](auto mode, const Unit& u)
@@ -1022,7 +1022,7 @@ struct JoinParams
     Kept kept;
     float* loss;
     double* sums;
-    long long n, rows_pad;
+    long long n, partial_pad;
     int tiles, reduction, lanes_log2;
     float scale, scale_log2;
 };
@@ -1040,7 +1040,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
 #pragma unroll 4
         for (int s = threadIdx.x >> rows_log2; s < p.tiles; s += lanes)
         {
-            const float2 x  = p.partial[s * p.rows_pad + at];
+            const float2 x  = p.partial[s * p.partial_pad + at];
             const float top = fmaxf(own.x, x.x), base = top == -__builtin_inff() ? 0.f : top;
             own = make_float2(top, own.y * part_of(own.x, base, p.scale_log2) + x.y * part_of(x.x, base, p.scale_log2));
         }
@@ -1142,6 +1142,7 @@ constexpr int64_t kPieceBytes = 1ll << 30;  // of d_ij
 constexpr int64_t kSlabBytes  = 256ll << 20;  // of the parts of the rows' gradients
 constexpr int kCus            = 256;
 constexpr int kMostSplits     = 64;
+constexpr int64_t kFewRows    = 64;
 constexpr int64_t kCopyBytes = 64ll << 20, kLeastCopyBytes = 16ll << 20;  // of copied entries
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -1186,7 +1187,7 @@ size_t kept_of(const TripsTableLossDesc& d, void* kept, Kept* k)
 // Steps of a call over the table; what each takes of the workspace.
 struct Layout
 {
-    int64_t rows_pad, chunks, piece, pieces;
+    int64_t rows_pad, partial_pad, chunks, piece, pieces;
     int kp, tiles, splits, table_splits, parts;
     bool copies;
     size_t chunk_count, top, partial, own_product, sums, probs, slabs, table_slabs, copy, bytes;
@@ -1215,8 +1216,8 @@ auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
     if (few || units(64) < kCus) return f(Deep{});
     return f(Tiny{});
 }
-// Entries of a tile of the logits.
-int entries_of_tile(const TripsTableLossDesc& d)
+// Entries, and rows, of a tile of the logits.
+int tile_of_logits(const TripsTableLossDesc& d)
 {
     return with_shape(d, false, [](auto shape) { return decltype(shape)::BM; });
 }
@@ -1308,10 +1309,11 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     if (!backward)
     {
         l.chunk_count = take(l.chunks * 4);
-        l.tiles       = (int)(l.piece / entries_of_tile(d));
-        l.partial     = take((size_t)l.tiles * l.pieces * l.rows_pad * sizeof(float2));
+        l.tiles       = (int)(l.piece / tile_of_logits(d));
+        l.partial_pad = up(d.num_rows, tile_of_logits(d));
+        l.partial     = take((size_t)l.tiles * l.pieces * l.partial_pad * sizeof(float2));
         l.own_product = take(l.rows_pad * 4);
-        l.sums        = take((d.num_rows / 4 + 1) * 8);
+        l.sums        = take((std::max(d.num_rows / 4, kFewRows) + 1) * 8);
     }
     else
     {
@@ -1367,7 +1369,7 @@ ProductParams product_params(const TripsTableLossDesc& d, const Layout& l, const
     ProductParams p{};
     p.kept = kept;
     p.partial = (float2*)(w + l.partial), p.own_product = (float*)(w + l.own_product), p.probs = w + l.probs, p.slabs = (float*)(w + l.slabs), p.table_slabs = (float*)(w + l.table_slabs);
-    p.d_table_stride = d.d_table_stride, p.rows_pad = l.rows_pad;
+    p.d_table_stride = d.d_table_stride, p.rows_pad = l.rows_pad, p.partial_pad = l.partial_pad;
     p.channels = d.num_channels, p.kp = l.kp, p.piece = (int)l.piece, p.splits = l.splits, p.table_splits = l.table_splits, p.parts = l.parts;
     p.scale_log2 = scale_log2(d);
     return p;
@@ -1424,10 +1426,13 @@ hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* ta
     JoinParams j{};
     j.partial = p.partial, j.own_product = p.own_product, j.kept = kept;
     j.loss = loss, j.scale = std::fabs(d.scale), j.scale_log2 = p.scale_log2, j.sums = (double*)(w + l.sums);
-    j.n = d.num_rows, j.rows_pad = l.rows_pad, j.tiles = (int)tiles_of(d.num_entries, entries_of_tile(d)), j.reduction = d.reduction;
+    j.n = d.num_rows, j.partial_pad = l.partial_pad, j.tiles = (int)tiles_of(d.num_entries, tile_of_logits(d)), j.reduction = d.reduction;
     while (j.lanes_log2 < 6 && 8 << j.lanes_log2 < j.tiles) ++j.lanes_log2;
-    // (the rows of few in one workgroup, whose sum is the loss then)
-    while (j.lanes_log2 > 2 && d.num_rows > 256 >> j.lanes_log2 && d.num_rows <= 64) --j.lanes_log2;
+    // (the rows of few in one workgroup, whose sum is the loss then, or of very many tiles in one each)
+    if (d.num_rows <= kFewRows && j.tiles > 2048)
+        while (j.lanes_log2 < 8 && 16 << j.lanes_log2 < j.tiles) ++j.lanes_log2;
+    else
+        while (j.lanes_log2 > 2 && d.num_rows > 256 >> j.lanes_log2 && d.num_rows <= kFewRows) --j.lanes_log2;
     const int64_t rows_each = 256 >> j.lanes_log2, groups = std::max<int64_t>(1, (d.num_rows + rows_each - 1) / rows_each);
     {
         ProfScope scope(prof, "loss_join", stream);
