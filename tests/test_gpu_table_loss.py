@@ -104,6 +104,11 @@ def test_few_entries_of_many_rows(n, t, c, pad, dtype):
     _check(*_inputs(n, t, c, dtype, 0.3, pad=pad), scale=-0.7, reduction="none" if t == 65 else "mean")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_more_than_a_million_rows(dtype):
+    _check(*_inputs(1_100_000, 40, 6, dtype, 0.3), reduction="mean")
+
+
 def test_no_rows_and_no_entries():
     for dtype in TYPES.values():
         x, w = torch.zeros(0, 8, dtype=dtype, device="cuda", requires_grad=True), torch.randn(5, 8, device="cuda").to(dtype).requires_grad_()
