@@ -485,8 +485,9 @@ __device__ __forceinline__ void place(Unit& u, int id, int across, int down)
     u.x = in / high, u.y = g * 8 + in % high;
 }
 
-// Where part z of `steps` in `parts` begins.
-__device__ __forceinline__ int part_begin(int z, int steps, int parts) { return (int)((long long)z * steps / parts); }
+// Where part z of `steps` in `parts` begins (steps are below 2^26, parts at most 64). Units of one step are made faster than they are worked out: no
+// division where there is one part.
+__device__ __forceinline__ int part_begin(int z, int steps, int parts) { return parts == 1 ? z * steps : (int)((unsigned)z * (unsigned)steps / (unsigned)parts); }
 
 // The units of worker w of `all`: unit w, w + all, ... of the larger kind (a of them, size_a steps each), then those of the smaller kind: workers
 // that have one of the larger kind less take so many smaller ones first.
