@@ -332,6 +332,38 @@ def test_same_bits_every_time_and_on_another_stream():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,t,c", [(20_000, 150, 16), (40, 97, 2000), (30, 66_000, 5), (500, 31, 700), (300, 3000, 70), (600, 9000, 300)])
+def test_same_bits_two_at_once(n, t, c, dtype):
+    """Two calls on two streams at the same time, each with its own tensors, and again alone."""
+    sets = [_inputs(n, t, c, dtype, 0.2, seed=s) for s in (1, 2)]
+    alone = [(loss, *torch.autograd.grad(loss, (x, w))) for x, w, target in sets for loss in [table_cross_entropy(x, w, target)]]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        got = []
+        for stream, (x, w, target) in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                loss = table_cross_entropy(x, w, target)
+                got.append((loss, *torch.autograd.grad(loss, (x, w))))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for one, other in zip(got, alone) for a, b in zip(one, other))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,t,c", [(600, 33, 1000), (500, 31, 700), (4000, 20, 100), (40, 97, 2000), (65, 8500, 130), (20_000, 150, 16), (3, 17_000, 500), (300, 3000, 70), (700, 9001, 300),
+                                   (7, 19, 2696)])
+def test_workspaces_of_any_content(n, t, c, dtype):
+    """What the allocator hands out for workspaces and results holds no numbers."""
+    x, w, target = _inputs(n, t, c, dtype, 0.2)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    del [torch.full((1 << 27,), float("nan"), device="cuda")][:]
+    for size in (1 << 8, 1 << 12, 1 << 16):  # (small blocks come from a pool of their own)
+        del [torch.full((size,), float("nan"), device="cuda") for _ in range(64)][:]
+    _check(x, w, target, reduction="mean")
+
+
 def test_only_one_gradient():
     x, w, target = _inputs(100, 300, 32, "bf16", 0.2)
     _, d_rows, d_table = _check_only(x, w, target, "mean")
