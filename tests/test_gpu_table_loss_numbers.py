@@ -1,0 +1,40 @@
+"""A table's cross entropy where its numbers are at an end: rows that are sure of their target, scales near zero, gradients without a number."""
+import numpy as np
+import pytest
+import torch
+
+from tests.loss_reference import U, half_step
+from trips_amd.table_loss import table_cross_entropy
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _signs(n, t, c, seed):
+    """A table of signs and a target of each row: products of whole numbers, exact in every type."""
+    rng = np.random.default_rng(seed)
+    w, target = rng.choice([-1.0, 1.0], size=(t, c)), rng.integers(0, t, n)
+    return w, target
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,t,c", [(1, 300, 64), (30, 3000, 64), (500, 2000, 64), (700, 300, 128), (3000, 20_000, 64)])
+@pytest.mark.parametrize("size,scale", [(4, 1.0), (3, -0.7), (11, 0.7), (100, 1.0), (300, 0.9)])
+def test_rows_that_are_sure_of_their_target(n, t, c, size, scale, dtype):
+    """The target's logit is so far ahead that its probability is 1 in double precision: a loss is no less than 0, and what rounding leaves of it and of the
+    gradients does not grow with the logits. An exponential is off by 2^-23 of itself and so is the correction of a sum, their product by U: 5 U; its logarithm as
+    much again; in the gradients the probability's own two, 16 U of the target's weight in all, half a step of what is held of it and half a step of the result."""
+    w, target = _signs(n, t, c, n + t)
+    x = size * np.sign(scale) * w[target]
+    near = np.array([np.partition(row, -2)[-2] for row in w[target[:500]] @ w.T])
+    assert ((c - near) * size * abs(scale) > 40).all()
+    x, w, target = (torch.as_tensor(a, device="cuda") for a in (x, w, target))
+    x, w = (a.to(TYPES[dtype]).requires_grad_() for a in (x, w))
+    loss = table_cross_entropy(x, w, target, scale=scale, reduction="none")
+    assert (loss >= 0).all() and float(loss.max()) <= 16 * U
+    d_rows, d_table = torch.autograd.grad(loss.sum(), (x, w))
+    off = 16 * U * abs(scale)
+    assert float(d_rows.abs().max()) <= off * (1 + 2.0 ** -8) + float(half_step(x.dtype, np.float64(off)))
+    times = torch.bincount(target, minlength=t)[:, None]
+    bound = (times * size * off * (1 + 2.0 ** -7)).cpu().numpy() + 1e-12
+    assert (d_table.detach().double().abs().cpu().numpy() <= bound + half_step(x.dtype, bound)).all()

@@ -271,6 +271,13 @@ typedef float Acc __attribute__((ext_vector_type(16)));
 // exp(scale (x - base)); 0 for an x of minus infinity.
 __device__ __forceinline__ float part_of(float x, float base, float scale_log2) { return __builtin_amdgcn_exp2f((x - base) * scale_log2); }
 
+// What -scale_log2 base - minus is beyond less - minus, for less = -scale_log2 base as rounded.
+__device__ __forceinline__ float rest_of(float base, float scale_log2, float less, float minus)
+{
+    const float sum = less - minus, back = sum - less;
+    return __builtin_fmaf(-base, scale_log2, -less) + ((less - (sum - back)) + (-minus - back));
+}
+
 // Entries one behind the other in rows of kp elements, zeros from the channels on: for tables whose rows the direct loads cannot take.
 template <typename T>
 __global__ __launch_bounds__(256) void copy_entries_kernel(const T* table, long long stride, T* to, long long entries, int channels, int kp)
@@ -365,9 +372,11 @@ __device__ __forceinline__ void wait_and_meet()
 // (of LDS; the loads under way stay so)
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Logits up to which the distance from the largest may be taken after the scaling, in one operation (their own rounding is as much), in types of
-// 16 bits. Products masked with the lowest value lie beyond it.
-constexpr float kFar = 65536.f;
+// Up to which |base| scale_log2 the distance from the largest product is taken behind the scaling, scale x + less in one operation with less = -scale base, in
+// types of 16 bits. Products masked with the lowest value lie beyond it. The rounding of `less` is the same for all of a row's products and known
+// (rest_of()): the sums are corrected by it, without which a row whose target is far ahead lost less than nothing (-3e-4 at logits of 10^4). Of d_ij only
+// the target's, a difference of two numbers near 1, is corrected; for the others it stays below 2^-16 of them, less than d_ij in 16 bits shows.
+constexpr float kFar = 65536.f, kFarOfOne = 256.f;
 
 constexpr unsigned kBeyond = 0x80000000u;  // an offset beyond any buffer
 
@@ -830,11 +839,18 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
             top              = fmaxf(top, __shfl_xor(top, 32));
             const float base = top == -__builtin_inff() ? 0.f : top, less = -base * p.scale_log2;
             float sum        = 0.f;
-            if (D != TRIPS_DTYPE_F32 && fabsf(less) < kFar)  // (each lane by itself: a row's bits do not depend on other rows)
+            const bool near  = D != TRIPS_DTYPE_F32 && fabsf(less) < kFar;  // (each lane by itself: a row's bits do not depend on other rows)
+            if (near)
                 each_element<S::FM>([&](int i, int e, int) { sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], p.scale_log2, less)); });
             else
                 each_element<S::FM>([&](int i, int e, int) { sum += part_of(acc[i][j][e], base, p.scale_log2); });
-            best[j] = make_float2(top, sum + __shfl_xor(sum, 32));
+            sum += __shfl_xor(sum, 32);
+            if (near)
+            {
+                sum *= __builtin_amdgcn_exp2f(rest_of(base, p.scale_log2, less, 0.f));
+                if (top > -__builtin_inff() && sum < 1.f) sum = 1.f;  // (the largest one's own)
+            }
+            best[j] = make_float2(top, sum);
         }
         meet();  // (the last unit's have been read)
 #pragma unroll
@@ -869,16 +885,20 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                 const int own      = n < count ? target[j] - p.first_entry - m_lane : -1;
                 const float factor = held_factor<D>(p.upstream, p.upstream.reduction == TRIPS_REDUCE_NONE ? p.kept.row[min(n, count - 1ll)] : 0);
                 const float less   = -of.x * p.scale_log2, held = D == TRIPS_DTYPE_F16 ? factor : 1.f;
-                if (D != TRIPS_DTYPE_F32 && fabsf(less) < kFar)
+                const bool near = D != TRIPS_DTYPE_F32 && fabsf(less) < kFarOfOne;
+                if (near)
                     each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], p.scale_log2, less - of.y)) * held; });
                 else
                     each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e] - of.x, p.scale_log2, -of.y)) * held; });
                 if (D != TRIPS_DTYPE_F16 && p.upstream.reduction == TRIPS_REDUCE_NONE) each_element<S::FM>([&](int i, int e, int) { acc[i][j][e] *= factor; });
                 if (__any(own >= 0 && own < S::TM))
+                {
+                    const float rest = near ? __builtin_amdgcn_exp2f(rest_of(of.x, p.scale_log2, less, of.y)) : 1.f;
                     each_element<S::FM>([&](int i, int e, int m)
                     {
-                        if (m == own) acc[i][j][e] -= factor;
+                        if (m == own) acc[i][j][e] = acc[i][j][e] * rest - factor;
                     });
+                }
                 if (m0 + S::BM > p.in_piece)
                     each_element<S::FM>([&](int i, int e, int m)
                     {
