@@ -38,3 +38,20 @@ def test_rows_that_are_sure_of_their_target(n, t, c, size, scale, dtype):
     times = torch.bincount(target, minlength=t)[:, None]
     bound = (times * size * off * (1 + 2.0 ** -7)).cpu().numpy() + 1e-12
     assert (d_table.detach().double().abs().cpu().numpy() <= bound + half_step(x.dtype, bound)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-45, 1e-41])
+@pytest.mark.parametrize("n,t", [(4, 10), (70, 300), (300, 900)])
+def test_scales_near_zero_beside_the_lowest_value(n, t, scale, dtype):
+    """Logits are 0 whatever the products are, the largest numbers of the type among them: off by at most 2^-20 of a power of two at 0, by scale
+    max |product| (2^-8 in float32 and bfloat16 at 1e-41) otherwise, and by the sum's and the logarithm's (320 + t / 64 + 8) U."""
+    x, w = (torch.zeros(m, 8, dtype=TYPES[dtype], device="cuda") for m in (n, t))
+    x[:, 0] = 1
+    w[t // 2:, 0] = torch.finfo(w.dtype).min
+    target = torch.arange(n, device="cuda") % t
+    loss = table_cross_entropy(x.requires_grad_(), w.requires_grad_(), target, scale=scale, reduction="none")
+    off = max(2.0 ** -19, 2 * scale * 3.5e38) + (328 + t / 64) * U
+    assert np.abs(loss.detach().double().cpu().numpy() - np.log(t)).max() <= off + U * np.log(t)
+    d_table, = torch.autograd.grad(loss.sum(), w)
+    assert float(d_table.abs().max()) <= 2 * scale * n + 1e-30

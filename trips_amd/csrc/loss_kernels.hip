@@ -8,6 +8,7 @@
 // is kept apart: where all entries are masked with the type's lowest value their probabilities are still equal.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "abi_common.h"
@@ -1358,8 +1359,9 @@ size_t workspace_of(const TripsTableLossDesc& d, bool backward)
     return copies_of(d, nullptr) ? copied : std::max(copied, layout_of(d, backward, false).bytes);
 }
 
-// (not 0: 0 times minus infinity, which stands for entries that are not there, is no number)
-float scale_log2(const TripsTableLossDesc& d) { return std::max((float)(std::fabs((double)d.scale) * kLog2e), 1.2e-38f); }
+// (not 0: 0 times minus infinity, which stands for entries that are not there, is no number. The smallest number there is: times the distance of two of the
+// largest, where entries are masked with the lowest value, it is 2^-20.)
+float scale_log2(const TripsTableLossDesc& d) { return std::max((float)(std::fabs((double)d.scale) * kLog2e), std::numeric_limits<float>::denorm_min()); }
 
 template <int D>
 hipError_t gather(const TripsTableLossDesc& d, const Layout& l, const void* rows, const void* target, const Kept& kept, char* w, hipStream_t stream, Profiler* prof)
