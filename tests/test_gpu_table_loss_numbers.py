@@ -55,3 +55,15 @@ def test_scales_near_zero_beside_the_lowest_value(n, t, scale, dtype):
     assert np.abs(loss.detach().double().cpu().numpy() - np.log(t)).max() <= off + U * np.log(t)
     d_table, = torch.autograd.grad(loss.sum(), w)
     assert float(d_table.abs().max()) <= 2 * scale * n + 1e-30
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("n,t,c", [(0, 5, 8), (4, 10, 8), (150, 333, 48), (9000, 129, 40), (600, 9000, 300)])
+def test_no_row_that_counts_and_a_gradient_without_a_number(n, t, c, reduction, dtype):
+    """Gradients are sums over the rows that count: 0 over none of them."""
+    x, w = (torch.randn(m, c, device="cuda").to(TYPES[dtype]).requires_grad_() for m in (n, t))
+    loss = table_cross_entropy(x, w, torch.full((n,), -1, device="cuda"), reduction=reduction)
+    for bad in (float("nan"), float("inf")):
+        for d in torch.autograd.grad(loss, (x, w), torch.full_like(loss, bad), retain_graph=True):
+            assert (d == 0).all()

@@ -233,8 +233,11 @@ template <int D>
 __device__ __forceinline__ float unheld(const Upstream& u, const int* count)
 {
     float g = 1.f;
-    if (u.reduction == TRIPS_REDUCE_SUM) g = u.d_loss[0];
-    if (u.reduction == TRIPS_REDUCE_MEAN) g = u.d_loss[0] / (float)max(*count, 1);
+    if (u.reduction != TRIPS_REDUCE_NONE)
+    {
+        const int rows = *count;
+        g              = rows == 0 ? 0.f : u.reduction == TRIPS_REDUCE_MEAN ? u.d_loss[0] / (float)rows : u.d_loss[0];  // (no row, no gradient, whatever the loss's is)
+    }
     if (D == TRIPS_DTYPE_F16 && u.reduction == TRIPS_REDUCE_NONE) g = *u.top;
     return g / kHeld<D>;
 }
