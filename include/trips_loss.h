@@ -37,7 +37,7 @@ typedef struct TripsTableLossDesc {
     int64_t num_rows;     /* N, below 2^28 */
     int64_t num_entries;  /* T, below 2^31 - 256 */
     int32_t num_channels; /* C, below 2^17 */
-    float scale;
+    float scale;          /* up to 2.3e38 either way: times log2 e it is a number of 32 bits too */
     int64_t rows_stride;
     int64_t table_stride;
     int64_t d_rows_stride;  /* backward */

@@ -1541,7 +1541,7 @@ int check_desc(const TripsTableLossDesc* d)
     if (d->num_rows < 0 || d->num_rows >= kMostRows) return set_error(TRIPS_ERR_INVALID_ARG, "num_rows = %lld", (long long)d->num_rows);
     if (d->num_entries < 0 || d->num_entries >= kMostEntries) return set_error(TRIPS_ERR_INVALID_ARG, "num_entries = %lld", (long long)d->num_entries);
     if (d->num_channels < 1 || d->num_channels >= kMostChannels) return set_error(TRIPS_ERR_INVALID_ARG, "num_channels = %d", d->num_channels);
-    if (!(d->scale - d->scale == 0.f)) return set_error(TRIPS_ERR_INVALID_ARG, "scale is not finite");
+    if (!(std::fabs((double)d->scale) * kLog2e <= (double)std::numeric_limits<float>::max())) return set_error(TRIPS_ERR_INVALID_ARG, "scale = %g", (double)d->scale);
     if (int e = check_stride("rows_stride", d->rows_stride, d->num_channels, d->num_rows, false)) return e;
     if (int e = check_stride("table_stride", d->table_stride, d->num_channels, d->num_entries, false)) return e;
     return check_units(*d);
