@@ -39,13 +39,16 @@ def table_cross_entropy(rows, table, target, scale=1.0, reduction="mean"):
     lookup()); rows whose target is outside the table (padding) count for nothing and get no gradient, whatever they hold.
 
     reduction: "none" gives [N], "sum" and "mean" one number, the mean over the rows that count (0 where none does); float32
-    whatever the type of rows and table (float32, bfloat16 or float16, the same of both). Differentiable in rows and table, once; gradients
+    whatever the type of rows and table (float32, bfloat16 or float16, the same of both). Differentiable in rows and table, once, and
+    not in scale; gradients
     have their type. What the gradients need of the rows is a copy of those that count, kept with the graph; they may be written to
     meanwhile, the table may not. In float16 the gradients of rows whose loss counts 2^-15 as much as another's lose precision."""
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction: 'none', 'sum' or 'mean' expected, got {reduction!r}")
     reduction = REDUCTIONS[reduction]
-    if forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(rows, table, target):
+    if torch.is_tensor(scale) and scale.requires_grad and torch.is_grad_enabled():
+        raise ValueError("scale: it gets no gradient; scale the rows where it is learned")
+    if forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(*(t for t in (rows, table, target, scale) if torch.is_tensor(t))):
         return _TableCrossEntropy.apply(rows, table, target, scale, reduction)
     if torch.is_grad_enabled() and (rows.requires_grad or table.requires_grad):
         ctx, stream = _where(target)
