@@ -2,6 +2,7 @@
 import ctypes as C
 
 import pytest
+import torch
 
 from trips_amd import _lib, abi
 
@@ -24,3 +25,20 @@ def test_scales(scale, taken):
     rc, _ = _workspace(0, 10, 10, 8, scale=scale)
     assert rc == (abi.TRIPS_OK if taken else abi.TRIPS_ERR_INVALID_ARG)
     assert taken or b"scale" in _lib.load().trips_last_error_string()
+
+
+def test_refusals_name_what_they_refuse():
+    """The targets and the cross entropy, not an index and lookups."""
+    from trips_amd.table_loss import table_cross_entropy
+    x, w, target = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(3, dtype=torch.int32)
+    for grad in (False, True):
+        x.requires_grad_(grad)
+        with pytest.raises(ValueError, match="^target: int32 or int64"):
+            table_cross_entropy(x, w, target.float())
+        with pytest.raises(RuntimeError, match="^the cross entropy needs tensors on a GPU"):
+            table_cross_entropy(x, w, target)
+    from trips_amd.lookup import lookup
+    with pytest.raises(ValueError, match="^index: int32 or int64"):
+        lookup(w, target.float())
+    with pytest.raises(RuntimeError, match="^lookups need tensors on a GPU"):
+        lookup(w, target)

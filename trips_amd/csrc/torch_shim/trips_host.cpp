@@ -199,19 +199,19 @@ void check(int rc)
     py::module_::import("trips_amd._lib").attr("check")(rc);
 }
 
-int index_dtype_of(const at::Tensor& index)
+int index_dtype_of(const at::Tensor& index, const char* name = "index", const char* what = "lookups need")
 {
     if (index.scalar_type() != at::kInt && index.scalar_type() != at::kLong)
-        throw py::value_error("index: int32 or int64 expected, got " + std::string(torch::getTHPDtype(index.scalar_type())->name));
-    if (!index.is_cuda()) throw std::runtime_error("lookups need tensors on a GPU: there is no CPU implementation");
+        throw py::value_error(std::string(name) + ": int32 or int64 expected, got " + std::string(torch::getTHPDtype(index.scalar_type())->name));
+    if (!index.is_cuda()) throw std::runtime_error(std::string(what) + " tensors on a GPU: there is no CPU implementation");
     return index.scalar_type() == at::kInt ? TRIPS_INDEX_I32 : TRIPS_INDEX_I64;
 }
 
 // A matrix on the index's device with adjacent elements in a row (a copy of it, if need be), and the distance of its rows.
-at::Tensor rows_of(const char* name, const at::Tensor& t, const at::Tensor& index, int64_t& stride)
+at::Tensor rows_of(const char* name, const at::Tensor& t, const at::Tensor& index, int64_t& stride, const char* where = "index's")
 {
     if (t.dim() != 2 || dtype_of(t) < 0 || t.layout() != at::kStrided || t.device() != index.device())
-        throw py::value_error(std::string(name) + ": a float32, bfloat16 or float16 matrix on the index's device expected");
+        throw py::value_error(std::string(name) + ": a float32, bfloat16 or float16 matrix on the " + where + " device expected");
     const at::Tensor m = t.stride(1) != 1 && t.size(1) > 1 ? t.detach().contiguous() : t;
     stride             = m.size(0) > 1 ? m.stride(0) : m.size(1);
     return m;
@@ -346,9 +346,9 @@ TripsTableLossDesc loss_desc(const at::Tensor& table, int64_t rows, double scale
 // {loss, what the gradients need}
 std::pair<at::Tensor, at::Tensor> table_loss(int64_t ctx, int64_t stream, const at::Tensor& rows, const at::Tensor& table, const at::Tensor& target, double scale, int64_t reduction)
 {
-    const int index_dtype = index_dtype_of(target);
+    const int index_dtype = index_dtype_of(target, "target", "the cross entropy needs");
     int64_t rows_stride, table_stride;
-    const at::Tensor x = rows_of("rows", rows, target, rows_stride), w = rows_of("table", table, target, table_stride);
+    const at::Tensor x = rows_of("rows", rows, target, rows_stride, "target's"), w = rows_of("table", table, target, table_stride, "target's");
     if (w.scalar_type() != x.scalar_type() || w.size(1) != x.size(1))
         throw py::value_error("rows and table: matrices of one type and as many channels expected, got " + std::to_string(x.size(1)) + " and " + std::to_string(w.size(1)) + " channels");
     if (target.numel() != x.size(0)) throw py::value_error("target: " + std::to_string(target.numel()) + " entries for " + std::to_string(x.size(0)) + " rows");
@@ -370,7 +370,7 @@ std::pair<at::Tensor, at::Tensor> table_loss_gradients(int64_t ctx, int64_t stre
                                                        int64_t reduction, bool want_rows, bool want_table)
 {
     int64_t table_stride;
-    const at::Tensor w   = rows_of("table", table, kept, table_stride);
+    const at::Tensor w   = rows_of("table", table, kept, table_stride, "rows'");
     TripsTableLossDesc d = loss_desc(w, rows, scale, reduction);
     const int64_t losses = reduction == TRIPS_REDUCE_NONE ? d.num_rows : 1;
     if (d_loss.scalar_type() != at::kFloat || d_loss.numel() != losses || d_loss.device() != w.device())
