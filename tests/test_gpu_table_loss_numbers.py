@@ -67,3 +67,28 @@ def test_no_row_that_counts_and_a_gradient_without_a_number(n, t, c, reduction, 
     for bad in (float("nan"), float("inf")):
         for d in torch.autograd.grad(loss, (x, w), torch.full_like(loss, bad), retain_graph=True):
             assert (d == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("n", [(1 << 19) - 1, 1 << 19, (1 << 19) + 1, 5_000_000])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_where_the_rows_of_many_go(n, dtype, index):
+    """Around the number of rows from which the counts of their chunks are summed beforehand, and beyond 4096 chunks: logits are whole numbers of one channel, so a
+    row's loss and gradient follow from its target and its number alone."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    target = torch.randint(-2, 6, (n,), device="cuda", generator=g, dtype=index)
+    target[n // 2:n // 2 + 5000] = -1
+    number = torch.randint(0, 3, (n,), device="cuda", generator=g)
+    x = number[:, None].to(TYPES[dtype]).requires_grad_()
+    w = torch.tensor([[0.0], [1.0], [2.0], [-1.0]], dtype=TYPES[dtype], device="cuda", requires_grad=True)
+    logp = torch.log_softmax(number[:, None].double() * w.detach()[:, 0].double(), 1)
+    inside = (target >= 0) & (target < 4)
+    own = target.long().clamp(0, 3)[:, None]
+    want = torch.where(inside, -logp.gather(1, own)[:, 0], 0.0)
+    loss = table_cross_entropy(x, w, target, reduction="none")
+    assert float((loss.double() - want).abs().max()) <= 64 * U
+    d = logp.exp().scatter_add_(1, own, torch.full_like(own, -1.0, dtype=torch.float64)) * inside[:, None]
+    d_rows, = torch.autograd.grad(loss.sum(), (x,))
+    half = torch.finfo(x.dtype).eps / 2
+    assert float((d_rows.double()[:, 0] - d @ w.detach()[:, 0].double()).abs().max()) <= 4 * (half + 32 * U)
+    assert (d_rows[~inside] == 0).all()

@@ -33,6 +33,8 @@ constexpr int kGatherRows = 16;     // rows of a workgroup
 constexpr int kChunk      = 1024;   // targets of a chunk that count_kernel counts
 constexpr int kAhead      = 4;      // pieces of 16 bytes that a thread asks for before it stores the first (8000 rows of 4000 floats 68 us one by one, 52 so)
 constexpr int kCountedBy  = 8192;   // rows from which the chunks are counted beforehand (losses of 8191 rows of 16 floats 15.7 us without, 16.8 with; of 12,000 19.5 and 18.2)
+constexpr int64_t kScannedBy = 1 << 19;  // rows from which the chunks' counts are summed beforehand, once for all workgroups, whose work would grow with the square of the rows (gathering 16 floats:
+                                         // 262,144 rows 30 us without, 34 with; a million 119 and 110; 6M 1438 and 794)
 
 // What the forward call leaves for the backward call; "packed" is an index among the rows that count.
 struct Kept
@@ -50,6 +52,7 @@ struct GatherParams
     const void* rows;
     const void* target;
     const int* chunk_count;  // targets that count of each chunk, or NULL: every workgroup looks at all targets
+    int scanned;             // whether they are those of the chunks before instead, and of all chunks behind the last one
     Kept kept;
     long long n, entries, stride;
     int channels, kp, negate;
@@ -86,6 +89,46 @@ __global__ __launch_bounds__(256) void count_kernel(const void* target, long lon
     if (threadIdx.x == 0) chunk_count[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
+// Each chunk's count becomes that of the chunks before it; all of them behind the last. One workgroup: bound by latency, 1.5 us for each 4096 chunks.
+__global__ __launch_bounds__(1024) void scan_kernel(int* count, long long chunks)
+{
+    __shared__ int sums[16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int carry = 0;
+    for (long long first = 0; first < chunks; first += 4096)
+    {
+        const long long i = first + threadIdx.x * 4;
+        int own[4], sum = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) own[e] = i + e < chunks ? count[i + e] : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += own[e];
+        int up_to = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1)
+        {
+            const int x = __shfl_up(up_to, o);
+            if (lane >= o) up_to += x;
+        }
+        if (lane == 63) sums[wave] = up_to;
+        __syncthreads();
+        int before = carry + up_to - sum;
+        for (int w = 0; w < 16; ++w)
+        {
+            if (w < wave) before += sums[w];
+            carry += sums[w];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+        {
+            if (i + e < chunks) count[i + e] = before;
+            before += own[e];
+        }
+        __syncthreads();  // (the sums are written again)
+    }
+    if (threadIdx.x == 0) count[chunks] = carry;
+}
+
 __device__ __forceinline__ float negative(float x) { return -x; }
 __device__ __forceinline__ unsigned short negative(unsigned short x) { return x ^ 0x8000u; }
 
@@ -104,12 +147,17 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
     if (p.chunk_count)
     {
         const long long chunks = (p.n + kChunk - 1) / kChunk, own_chunk = first / kChunk;
-        for (long long c = threadIdx.x; c < chunks; c += 256)
+        if (p.scanned)
         {
-            const int k = p.chunk_count[c];
-            all += k;
-            if (c < own_chunk) before += k;
+            if (threadIdx.x == 0) before = p.chunk_count[own_chunk], all = p.chunk_count[chunks];
         }
+        else
+            for (long long c = threadIdx.x; c < chunks; c += 256)
+            {
+                const int k = p.chunk_count[c];
+                all += k;
+                if (c < own_chunk) before += k;
+            }
         for (long long i = own_chunk * kChunk + threadIdx.x; i < first; i += 256) before += counts<I32>(p.target, i, p.entries);
     }
     else
@@ -1333,7 +1381,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     l.piece  = up((d.num_entries + l.pieces - 1) / l.pieces, 256);
     if (!backward)
     {
-        l.chunk_count = take(l.chunks * 4);
+        l.chunk_count = take((l.chunks + 1) * 4);
         l.tiles       = (int)(l.piece / tile_of_logits(d));
         l.partial_pad = up(d.num_rows, tile_of_logits(d));
         l.partial     = take((size_t)l.tiles * l.pieces * l.partial_pad * sizeof(float2));
@@ -1381,6 +1429,13 @@ hipError_t gather(const TripsTableLossDesc& d, const Layout& l, const void* rows
         ProfScope scope(prof, "loss_count", stream);
         (i32 ? count_kernel<true> : count_kernel<false>)<<<(unsigned)l.chunks, 256, 0, stream>>>(target, d.num_rows, d.num_entries, chunk_count);
         if (hipError_t e = hipGetLastError()) return e;
+        p.scanned = d.num_rows > kScannedBy;
+        if (p.scanned)
+        {
+            ProfScope scope(prof, "loss_scan", stream);
+            scan_kernel<<<1, 1024, 0, stream>>>(chunk_count, l.chunks);
+            if (hipError_t e = hipGetLastError()) return e;
+        }
     }
     ProfScope scope(prof, "loss_gather", stream);
     const unsigned groups = std::max(1u, (unsigned)((d.num_rows + kGatherRows - 1) / kGatherRows));
