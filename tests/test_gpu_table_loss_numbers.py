@@ -92,3 +92,24 @@ def test_where_the_rows_of_many_go(n, dtype, index):
     half = torch.finfo(x.dtype).eps / 2
     assert float((d_rows.double()[:, 0] - d @ w.detach()[:, 0].double()).abs().max()) <= 4 * (half + 32 * U)
     assert (d_rows[~inside] == 0).all()
+
+
+@pytest.mark.parametrize("n", [65_536, 65_537, 70_001, 2_200_000])
+def test_the_largest_gradient_of_many_rows(n):
+    """float16 is held over the largest gradient of a row that counts, wherever that stands: one missed would leave the row's probability infinite, one of a row
+    that does not count taken would leave the others' zero."""
+    x = torch.ones(n, 1, dtype=torch.float16, device="cuda", requires_grad=True)
+    w = torch.tensor([[0.0], [0.5], [2.0]], dtype=torch.float16, device="cuda")
+    p = torch.softmax(w.double()[:, 0], 0)
+    slope = float(p @ w.double()[:, 0]) - 0.5
+    target = torch.ones(n, dtype=torch.int64, device="cuda")
+    target[7], target[n - 9] = -1, 3
+    loss = table_cross_entropy(x, w, target, reduction="none")
+    for at in (0, 8191, 8192, n // 2, n - 8193, n - 1):
+        g = torch.ones(n, device="cuda")
+        g[at], g[7], g[n - 9] = 1e4, 1e30, float("inf")
+        want = g.double() * slope
+        want[7] = want[n - 9] = 0
+        got, = torch.autograd.grad(loss, x, g, retain_graph=True)
+        # (half a step of the result, of each of three d_ij, and the smallest step of those, 2^-25 of 10^4 / 2^15)
+        assert ((got[:, 0].double() - want).abs() <= want.abs() * 2.0 ** -10 * 4 + 3 * 2 * 2.0 ** -25 * 1e4 / 32768).all()

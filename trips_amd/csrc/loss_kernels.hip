@@ -236,17 +236,22 @@ constexpr float kHeld = D == TRIPS_DTYPE_F16 ? 32768.f : 1.f;
 // rest of d_ij as well, as a second part of the same type, takes that away and doubles the gradients' products: done where those are few (see
 // parts_of()).
 
-// The largest |gradient| of the rows that count, finite ones only: the others are left as they are.
+constexpr int64_t kTopBy = 65536;  // rows from which several workgroups look for the largest gradient (with one 40,000 rows 6.5 us, with several 5.1 in two launches; 70,000 10 and 5.5, 6M 831 and 14)
+constexpr int kTops      = 256;
+
+// The largest |gradient| of the rows that count (not PLACED: of all), finite ones only: the others are left as they are. Of several workgroups each its own, which a second
+// launch takes together.
+template <bool PLACED>
 __global__ __launch_bounds__(1024) void top_kernel(const float* d_loss, const int* place, long long n, float* top)
 {
     __shared__ float tops[16];
     float own = 0.f;
-    for (long long i0 = threadIdx.x; i0 < n; i0 += 8192)
+    for (long long i0 = blockIdx.x * 8192ll + threadIdx.x; i0 < n; i0 += gridDim.x * 8192ll)
     {
         float g[8];
         int at[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = d_loss[min(i0 + e * 1024, n - 1)], at[e] = place[min(i0 + e * 1024, n - 1)];
+        for (int e = 0; e < 8; ++e) g[e] = d_loss[min(i0 + e * 1024, n - 1)], at[e] = PLACED ? place[min(i0 + e * 1024, n - 1)] : 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
         {
@@ -260,7 +265,7 @@ __global__ __launch_bounds__(1024) void top_kernel(const float* d_loss, const in
     __syncthreads();
     if (threadIdx.x > 0) return;
     for (int w = 0; w < 16; ++w) own = fmaxf(own, tops[w]);
-    *top = own > 0.f ? own : 1.f;
+    top[blockIdx.x] = gridDim.x > 1 || own > 0.f ? own : 1.f;
 }
 
 struct Upstream
@@ -1390,7 +1395,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     }
     else
     {
-        l.top   = take(4);
+        l.top   = take((1 + kTops) * 4);
         l.probs = take((size_t)l.parts * l.rows_pad * l.piece * size);
         const Splits s = splits_of(d, l.rows_pad, l.piece, l.kp);
         l.splits = s.rows, l.table_splits = s.table;
@@ -1546,8 +1551,15 @@ hipError_t backward(const TripsTableLossDesc& d, const void* table, const Kept& 
     if (D == TRIPS_DTYPE_F16 && d.reduction == TRIPS_REDUCE_NONE && d.num_rows > 0)
     {
         ProfScope scope(prof, "loss_top", stream);
-        top_kernel<<<1, 1024, 0, stream>>>(d_loss, kept.place, d.num_rows, (float*)(w + l.top));
+        float* top       = (float*)(w + l.top);
+        const int groups = d.num_rows > kTopBy ? (int)std::min<int64_t>((d.num_rows + 8191) / 8192, kTops) : 1;
+        top_kernel<true><<<groups, 1024, 0, stream>>>(d_loss, kept.place, d.num_rows, groups > 1 ? top + 1 : top);
         if (hipError_t e = hipGetLastError()) return e;
+        if (groups > 1)
+        {
+            top_kernel<false><<<1, 1024, 0, stream>>>(top + 1, nullptr, groups, top);
+            if (hipError_t e = hipGetLastError()) return e;
+        }
     }
     for (int64_t piece = 0; piece * l.piece < d.num_entries; ++piece)
     {
