@@ -34,7 +34,7 @@ typedef struct TripsTableLossDesc {
     int32_t dtype;        /* of rows, table and their gradients: TRIPS_DTYPE_F32, _BF16 or _F16 */
     int32_t index_dtype;  /* TRIPS_INDEX_* */
     int32_t reduction;    /* TRIPS_REDUCE_*: loss is [N], or [1]: the sum, or the mean over the rows that count (0 if none does) */
-    int64_t num_rows;     /* N, below 2^28 */
+    int64_t num_rows;     /* N, at most 2^28 - 16 */
     int64_t num_entries;  /* T, below 2^31 - 256 */
     int32_t num_channels; /* C, below 2^17 */
     float scale;          /* up to 2.3e38 either way: times log2 e it is a number of 32 bits too */

@@ -42,3 +42,9 @@ def test_refusals_name_what_they_refuse():
         lookup(w, target.float())
     with pytest.raises(RuntimeError, match="^lookups need tensors on a GPU"):
         lookup(w, target)
+
+
+@pytest.mark.parametrize("n,taken", [((1 << 28) - 16, True), ((1 << 28) - 15, False), ((1 << 28) - 1, False)])
+def test_rows(n, taken):
+    """A launch of 16 threads a row has fewer than 2^32."""
+    assert _workspace(0, n, 2, 1)[0] == (abi.TRIPS_OK if taken else abi.TRIPS_ERR_INVALID_ARG)

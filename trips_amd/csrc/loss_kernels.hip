@@ -21,7 +21,7 @@ namespace trips
 {
 namespace
 {
-constexpr int64_t kMostRows    = 1ll << 28;  // threads of a launch
+constexpr int64_t kMostRows    = (1ll << 28) - 16;  // gather_kernel's threads, 16 a row, stay below 2^32
 constexpr int64_t kMostEntries = 0x7fffffffll - 256;
 constexpr int kMostChannels    = 1 << 17;
 constexpr double kLog2e = 1.4426950408889634;
@@ -1605,7 +1605,7 @@ int check_desc(const TripsTableLossDesc* d)
     if (!dtype_ok(d->dtype)) return set_error(TRIPS_ERR_UNSUPPORTED, "dtype %d", d->dtype);
     if (d->index_dtype != TRIPS_INDEX_I64 && d->index_dtype != TRIPS_INDEX_I32) return set_error(TRIPS_ERR_UNSUPPORTED, "index_dtype %d", d->index_dtype);
     if (d->reduction != TRIPS_REDUCE_NONE && d->reduction != TRIPS_REDUCE_SUM && d->reduction != TRIPS_REDUCE_MEAN) return set_error(TRIPS_ERR_INVALID_ARG, "reduction %d", d->reduction);
-    if (d->num_rows < 0 || d->num_rows >= kMostRows) return set_error(TRIPS_ERR_INVALID_ARG, "num_rows = %lld", (long long)d->num_rows);
+    if (d->num_rows < 0 || d->num_rows > kMostRows) return set_error(TRIPS_ERR_INVALID_ARG, "num_rows = %lld", (long long)d->num_rows);
     if (d->num_entries < 0 || d->num_entries >= kMostEntries) return set_error(TRIPS_ERR_INVALID_ARG, "num_entries = %lld", (long long)d->num_entries);
     if (d->num_channels < 1 || d->num_channels >= kMostChannels) return set_error(TRIPS_ERR_INVALID_ARG, "num_channels = %d", d->num_channels);
     if (!(std::fabs((double)d->scale) * kLog2e <= (double)std::numeric_limits<float>::max())) return set_error(TRIPS_ERR_INVALID_ARG, "scale = %g", (double)d->scale);
