@@ -113,3 +113,44 @@ def test_the_largest_gradient_of_many_rows(n):
         got, = torch.autograd.grad(loss, x, g, retain_graph=True)
         # (half a step of the result, of each of three d_ij, and the smallest step of those, 2^-25 of 10^4 / 2^15)
         assert ((got[:, 0].double() - want).abs() <= want.abs() * 2.0 ** -10 * 4 + 3 * 2 * 2.0 ** -25 * 1e4 / 32768).all()
+
+
+def _one_channel(n, t, dtype, c=1):
+    """Rows of four kinds over a table that rises along its entries, so that for some the largest logits come first and for others last; their losses and gradients
+    follow from the kind and the target alone. Products are exact."""
+    g = torch.Generator(device="cuda").manual_seed(n + t)
+    kinds = torch.tensor([1.0, -1.0, 0.5, 0.0], device="cuda")
+    kind = torch.randint(0, 4, (n,), device="cuda", generator=g)
+    target = torch.randint(0, t, (n,), device="cuda", generator=g, dtype=torch.int32)
+    target[torch.rand(n, device="cuda", generator=g) < 0.1] = -1
+    x, w = torch.zeros(n, c, dtype=TYPES[dtype], device="cuda"), torch.zeros(t, c, dtype=TYPES[dtype], device="cuda")
+    x[:, 0], w[:, 0] = kinds[kind].to(x.dtype), (torch.arange(t, device="cuda") * (16.0 / t) - 8).to(w.dtype)
+    logp = torch.log_softmax(kinds[:, None].double() * w[:, 0].double(), 1)
+    inside, own = target >= 0, target.long().clamp(min=0)
+    loss = torch.where(inside, -logp[kind, own], 0.0)
+    d_rows = torch.where(inside, (logp.exp() @ w[:, 0].double())[kind] - w[own, 0].double(), 0.0)
+    return x.requires_grad_(), w.requires_grad_(), target, loss, d_rows
+
+
+@pytest.mark.parametrize("dtype,n,t,c", [("f32", 66_000, 300_000, 1), ("bf16", 140_000, 262_500, 2), ("f16", 140_000, 262_500, 2), ("bf16", 140_001, 263_000, 1), ("f32", 40, 3_700_000, 1)])
+def test_tiles_that_are_joined_in_rounds(dtype, n, t, c):
+    """More maxima and sums of tiles than are held at once (and one case of few rows, which holds them). Off by the roundings of logits up to 8, of an exponential
+    (2^-22), of sums in chains of 320 + t / 64 terms at most; gradients by as much of 16, the spread of the table, and half a step of d_ij and of the result."""
+    x, w, target, want, want_rows = _one_channel(n, t, dtype, c)
+    loss = table_cross_entropy(x, w, target, reduction="none")
+    off = (8 * 8 + 4 + 320 + t / 64) * U
+    assert float((loss.double() - want).abs().max()) <= off
+    d_rows, = torch.autograd.grad(loss.sum(), (x,))
+    step = torch.finfo(x.dtype).eps
+    assert float((d_rows[:, 0].double() - want_rows).abs().max()) <= 16 * (2 * off + step + t * 2.0 ** -25 / 32768)
+    assert (d_rows[:, 1:] == 0).all() if c == 1 else True
+    mean = table_cross_entropy(x.detach(), w.detach(), target)
+    assert abs(float(mean) - float(want.sum() / (target >= 0).sum())) <= off
+
+
+def test_very_many_rows_of_many_entries():
+    """2^26 rows and more than 256 tiles of entries: no launch has more threads than there may be."""
+    x, w, target, want, _ = _one_channel((1 << 26) + 9, 66_000, "bf16", 2)
+    with torch.no_grad():
+        loss = table_cross_entropy(x, w, target, reduction="none")
+    assert float((loss - want).abs().max()) <= (68 + 320 + 66_000 / 64) * U

@@ -48,3 +48,14 @@ def test_refusals_name_what_they_refuse():
 def test_rows(n, taken):
     """A launch of 16 threads a row has fewer than 2^32."""
     assert _workspace(0, n, 2, 1)[0] == (abi.TRIPS_OK if taken else abi.TRIPS_ERR_INVALID_ARG)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,t", [(131_072, 262_144), (262_144, 262_144), (8191, 2_000_000_000), (300_000, 20_000_000), (1 << 26, 66_000), (1 << 26, 33_000), (5, 2_000_000_000), (1, 1), (0, 0), (0, 5), (5, 0)])
+@pytest.mark.parametrize("c", [1, 8, 1000])
+def test_the_losss_workspace_does_not_grow_with_rows_times_entries(n, t, c, dtype):
+    """Maxima and sums of a GiB of tiles at once, or of 256 entries (four tiles at most, of 8 bytes a row each); 64 MiB of entries that are copied, or 256 of
+    them; 8 bytes a row besides."""
+    rc, got = _workspace(0, n, t, c, dtype)
+    assert rc == abi.TRIPS_OK
+    assert got <= max(1 << 30, n * 4 * 8) + max(64 << 20, 256 * 4 * (c + 8)) + 8 * n + (1 << 20), got / 2 ** 30

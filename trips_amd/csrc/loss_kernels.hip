@@ -1091,7 +1091,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
 
 // ---- joins ----
 
-// 1 << lanes_log2 lanes a row over the tiles: state and loss, and the workgroup's sum of losses. Bound by latency: 4 us for few tiles and rows, 10 for 7782 rows and
+// 1 << lanes_log2 lanes a row over the tiles: state and loss, and the workgroup's sum of losses; of tiles that are not all, the sum of exponentials in the place of its logarithm. Bound by latency: 4 us for few tiles and rows, 10 for 7782 rows and
 // 196 tiles (12 MB).
 struct JoinParams
 {
@@ -1102,6 +1102,7 @@ struct JoinParams
     double* sums;
     long long n, partial_pad;
     int tiles, reduction, lanes_log2;
+    int more, last;  // whether earlier tiles are in the state; whether there are no further ones
     float scale, scale_log2;
 };
 __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
@@ -1115,6 +1116,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
     if (at >= 0)
     {
         const float product = p.own_product[at];
+        if (p.more && threadIdx.x >> rows_log2 == 0) own = p.kept.state[at];
 #pragma unroll 4
         for (int s = threadIdx.x >> rows_log2; s < p.tiles; s += lanes)
         {
@@ -1134,6 +1136,11 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinParams p)
             const float top = fmaxf(x.x, y.x), base = top == -__builtin_inff() ? 0.f : top;
             part[threadIdx.x] = make_float2(top, x.y * part_of(x.x, base, p.scale_log2) + y.y * part_of(y.x, base, p.scale_log2));
         }
+    }
+    if (!p.last)
+    {
+        if (threadIdx.x >> rows_log2 == 0 && at >= 0) p.kept.state[at] = part[threadIdx.x];
+        return;
     }
     float loss = 0.f;
     if (threadIdx.x >> rows_log2 == 0 && at >= 0)  // (what a thread reads it wrote itself)
@@ -1217,6 +1224,7 @@ __global__ __launch_bounds__(256) void slabs_out_kernel(const float* slabs, cons
 // ---- host ----
 
 constexpr int64_t kPieceBytes = 1ll << 30;  // of d_ij
+constexpr int64_t kPartialBytes = 1ll << 30;  // of the maxima and sums of the rows' tiles that are joined at once
 constexpr int64_t kSlabBytes  = 256ll << 20;  // of the parts of the rows' gradients
 constexpr int kCus            = 256;
 constexpr int kMostSplits     = 64;
@@ -1267,6 +1275,7 @@ struct Layout
 {
     int64_t rows_pad, partial_pad, chunks, piece, pieces;
     int kp, tiles, splits, table_splits, parts;
+    int at_once;  // pieces whose tiles are joined at once
     bool copies;
     size_t chunk_count, top, partial, own_product, sums, probs, slabs, table_slabs, copy, bytes;
 };
@@ -1381,6 +1390,11 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
         most   = std::min(most, std::max<int64_t>((rows_in_place(d) ? kLeastCopyBytes : kCopyBytes) / (l.kp * size) / 256, 1) * 256);
         l.copy = take((size_t)most * l.kp * size);
     }
+    if (!backward)
+    {
+        const int64_t tile = tile_of_logits(d), tiles = kPartialBytes / (std::max<int64_t>(up(d.num_rows, tile), 1) * (int64_t)sizeof(float2));
+        most               = std::min(most, std::max<int64_t>(tiles * tile / 256, 1) * 256);
+    }
     if (backward) most = std::min(most, std::max<int64_t>(kPieceBytes / (std::max<int64_t>(l.rows_pad, 1) * size * l.parts) / 256, 1) * 256);
     l.pieces = std::max<int64_t>(1, (d.num_entries + most - 1) / most);
     l.piece  = up((d.num_entries + l.pieces - 1) / l.pieces, 256);
@@ -1389,7 +1403,8 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
         l.chunk_count = take((l.chunks + 1) * 4);
         l.tiles       = (int)(l.piece / tile_of_logits(d));
         l.partial_pad = up(d.num_rows, tile_of_logits(d));
-        l.partial     = take((size_t)l.tiles * l.pieces * l.partial_pad * sizeof(float2));
+        l.at_once     = (int)std::min(l.pieces, std::max<int64_t>(1, kPartialBytes / (std::max<int64_t>(l.partial_pad * l.tiles, 1) * (int64_t)sizeof(float2))));
+        l.partial     = take((size_t)l.tiles * l.at_once * l.partial_pad * sizeof(float2));
         l.own_product = take(l.rows_pad * 4);
         l.sums        = take((std::max(d.num_rows / 4, kFewRows) + 1) * 8);
     }
@@ -1468,7 +1483,7 @@ hipError_t take_piece(const TripsTableLossDesc& d, const Layout& l, int64_t piec
     using T          = typename Element<D>::type;
     const T* entries = reinterpret_cast<const T*>(table) + piece * l.piece * d.table_stride;
     p.first_entry = (int)(piece * l.piece), p.in_piece = (int)std::min(l.piece, d.num_entries - piece * l.piece);
-    p.first_tile = (int)(piece * l.tiles), p.add = piece > 0;
+    p.first_tile = l.at_once ? (int)(piece % l.at_once * l.tiles) : 0, p.add = piece > 0;
     p.table = entries, p.table_stride = d.table_stride, p.held = d.num_channels;
     p.d_table = d_table ? reinterpret_cast<T*>(d_table) + piece * l.piece * d.d_table_stride : nullptr;
     if (!l.copies) return hipSuccess;
@@ -1503,24 +1518,30 @@ hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* ta
     const Layout l = layout_of(d, false, copies_of(d, table));
     if (hipError_t e = gather<D>(d, l, rows, target, kept, w, stream, prof)) return e;
     ProductParams p = product_params(d, l, kept, w);
-    int64_t piece   = 0;
-    for (; piece * l.piece < d.num_entries; ++piece)
-    {
-        if (hipError_t e = take_piece<D>(d, l, piece, table, nullptr, w, p, stream, prof)) return e;
-        if (hipError_t e = launch_product<D, LOGITS>(d, p, stream, prof)) return e;
-    }
     JoinParams j{};
     j.partial = p.partial, j.own_product = p.own_product, j.kept = kept;
     j.loss = loss, j.scale = std::fabs(d.scale), j.scale_log2 = p.scale_log2, j.sums = (double*)(w + l.sums);
-    j.n = d.num_rows, j.partial_pad = l.partial_pad, j.tiles = (int)tiles_of(d.num_entries, tile_of_logits(d)), j.reduction = d.reduction;
-    while (j.lanes_log2 < 6 && 8 << j.lanes_log2 < j.tiles) ++j.lanes_log2;
-    // (the rows of few in one workgroup, whose sum is the loss then, or of very many tiles in one each)
-    if (d.num_rows <= kFewRows && j.tiles > 2048)
-        while (j.lanes_log2 < 8 && 16 << j.lanes_log2 < j.tiles) ++j.lanes_log2;
-    else
-        while (j.lanes_log2 > 2 && d.num_rows > 256 >> j.lanes_log2 && d.num_rows <= kFewRows) --j.lanes_log2;
-    const int64_t rows_each = 256 >> j.lanes_log2, groups = std::max<int64_t>(1, (d.num_rows + rows_each - 1) / rows_each);
+    j.n = d.num_rows, j.partial_pad = l.partial_pad, j.reduction = d.reduction;
+    int64_t groups = 1;
+    for (int64_t piece = 0; !j.last;)
     {
+        const int64_t first = piece * l.piece;
+        for (int k = 0; k < l.at_once && piece * l.piece < d.num_entries; ++k, ++piece)
+        {
+            if (hipError_t e = take_piece<D>(d, l, piece, table, nullptr, w, p, stream, prof)) return e;
+            if (hipError_t e = launch_product<D, LOGITS>(d, p, stream, prof)) return e;
+        }
+        j.tiles = (int)tiles_of(std::min(piece * l.piece, d.num_entries) - first, tile_of_logits(d));
+        j.more = first > 0, j.last = piece * l.piece >= d.num_entries;
+        j.lanes_log2 = 0;
+        while (j.lanes_log2 < 6 && 8 << j.lanes_log2 < j.tiles) ++j.lanes_log2;
+        // (the rows of few in one workgroup, whose sum is the loss then, or of very many tiles in one each)
+        if (d.num_rows <= kFewRows && j.tiles > 2048)
+            while (j.lanes_log2 < 8 && 16 << j.lanes_log2 < j.tiles) ++j.lanes_log2;
+        else
+            while (j.lanes_log2 > 2 && d.num_rows > 256 >> j.lanes_log2 && d.num_rows <= kFewRows) --j.lanes_log2;
+        const int64_t rows_each = 256 >> j.lanes_log2;  // (a launch's threads stay below 2^32: rows of many tiles are few, see kPartialBytes)
+        groups                  = std::max<int64_t>(1, (d.num_rows + rows_each - 1) / rows_each);
         ProfScope scope(prof, "loss_join", stream);
         join_kernel<<<(unsigned)groups, 256, 0, stream>>>(j);
         if (hipError_t e = hipGetLastError()) return e;
