@@ -59,3 +59,21 @@ def test_the_losss_workspace_does_not_grow_with_rows_times_entries(n, t, c, dtyp
     rc, got = _workspace(0, n, t, c, dtype)
     assert rc == abi.TRIPS_OK
     assert got <= max(1 << 30, n * 4 * 8) + max(64 << 20, 256 * 4 * (c + 8)) + 8 * n + (1 << 20), got / 2 ** 30
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,t,c", [(6_000_000, 150, 16), (6_000_000, 2, 16), (1_000_000, 2, 16), (1_100_000, 40, 6), (1 << 21, 256, 1000), (100_000_000, 33, 3), (1 << 27, 100_000, 16),
+                                   (16_384, 262_143, 1024), (500_000, 70_000, 64), (3, 200_000, 2000), (5, 1, 1)])
+def test_the_gradients_workspace_is_bounded(n, t, c, dtype):
+    """A GiB of d_ij, a quarter of that of a gradient's parts or one part of it in 32 bits (of a million rows at most, of the table where there are more rows than that, else of a
+    piece of it), copied entries, and small things: whatever the rows times the entries are."""
+    rc, got = _workspace(1, n, t, c, dtype)
+    assert rc == abi.TRIPS_OK
+    padded = 4 * (c + 8)
+    rows, table = (min(n, 1 << 20) + 256) * padded, (t + 65536) * padded
+    assert got <= (1 << 30) + max(256 << 20, rows) + max(256 << 20, table) + max(64 << 20, 256 * padded) + (1 << 20), got / 2 ** 30
+
+
+def test_few_entries_take_no_more_than_whole_tiles():
+    """1000 rows and two entries: d_ij in 64 columns (the least step of the gradients), not in 256."""
+    assert _workspace(1, 1000, 2, 16)[1] < _workspace(1, 1000, 200, 16)[1] - 1024 * 64 * 4

@@ -314,12 +314,14 @@ struct ProductParams
     float* own_product;  // [rows_pad]
     void* probs;         // [parts][rows_pad][piece], in the tensors' type
     float* slabs;        // D_ROWS: [splits][rows_pad][kp]
-    float* table_slabs;  // D_TABLE, where table_splits > 1: [table_splits][piece][kp]
+    float* table_slabs;  // D_TABLE, where in_table_slabs: [table_splits][piece][kp]
     const void* d_rows;  // whether they are wanted
     void* d_table;
     long long table_stride, d_table_stride, rows_pad, partial_pad;
     int held;  // channels that a row of the table has: those, or of a copy with zeros behind them to 16 bytes
     int first_entry, in_piece, channels, kp, piece, first_tile, splits, table_splits, parts, add;
+    int first_row, most_rows;         // of the rows that count, those of the launch: kept is theirs (but for the count)
+    int in_table_slabs, add_to_table;  // D_TABLE: whether its results are parts of sums, of the rows' (table_splits) or of the blocks of rows, and whether those have begun
     float scale_log2;
 };
 
@@ -601,7 +603,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool writes = S::WK == 1 || wave == 0;
     const int wm = wave % S::WM * S::TM, wn = wave / S::WM % S::WN * S::TN;
-    const int count = *p.kept.count;
+    const int count = min(max(*p.kept.count - p.first_row, 0), p.most_rows);
 
     // Workgroups as they start go around the eight XCDs: of each 256, which take a CU each, workers by XCD.
     const int all = gridDim.x, run = (int)blockIdx.x & ~255, runs = min(256, all - run), in_run = (int)blockIdx.x & 255;
@@ -930,7 +932,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
         constexpr int MODE = decltype(mode)::value;
         const long long n0 = (long long)u.y * S::BN;
         const int m0 = u.x * S::BM, m_lane = m0 + wm + 4 * (lane >> 5);
-        const bool in_slabs = TABLE_SPLITS && MODE == D_TABLE && table_splits > 1;
+        const bool in_slabs = TABLE_SPLITS && MODE == D_TABLE && p.in_table_slabs;
         const float unscale = MODE == D_TABLE && !in_slabs ? unheld<D>(p.upstream, p.kept.count) * fabsf(p.upstream.scale) : 1.f;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j)
@@ -977,7 +979,7 @@ __global__ __launch_bounds__(S::WAVES * 64, S::PER_CU * S::WAVES / 4) void produ
                         {
                             F4* at = reinterpret_cast<F4*>(slab + c);
                             F4 v   = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-                            if (MODE == D_ROWS && p.add) v += *at;
+                            if (MODE == D_ROWS ? p.add : p.add_to_table) v += *at;
                             *at = v;
                         }
                     }
@@ -1184,46 +1186,60 @@ __global__ __launch_bounds__(1024) void sum_kernel(const double* from, int n, co
     *loss = (float)(reduction == TRIPS_REDUCE_MEAN ? sum / (double)max(*count, 1) : sum);
 }
 
-// d_rows: the splits' sums, in their order, at their rows' own places (place; NULL for d_table's splits, whose entries are where they belong);
-// four channels a lane. Bound by memory: 7 parts of 7782 rows of 1024 channels 43 us, 5.4 TB/s.
+// What a slab's rows are of: entries (d_table's splits and blocks, which are where they belong), all rows (whose places say which of the slab's they are; zeros
+// for those that do not count), or a block of the rows that count, which `row` says the places of; the others are written by a launch of their own then.
+enum { ENTRIES, ALL_ROWS, BLOCK_ROWS, OTHER_ROWS };
+struct SlabsOut
+{
+    const float* slabs;
+    Kept kept;  // BLOCK_ROWS: the block's
+    Upstream upstream;
+    void* out;
+    long long n, rows_pad, stride;
+    int what, first_row, channels, kp, splits;
+    float scale;
+};
+// The splits' sums, in their order; four channels a lane. Bound by memory: 7 parts of 7782 rows of 1024 channels 43 us, 5.4 TB/s.
 template <int D>
-__global__ __launch_bounds__(256) void slabs_out_kernel(const float* slabs, const int* place, const int* count, const Upstream upstream, float scale, void* out_rows, long long n,
-                                                        long long rows_pad, long long stride, int channels, int kp, int splits)
+__global__ __launch_bounds__(256) void slabs_out_kernel(const SlabsOut p)
 {
     using E  = Element<D>;
     using T  = typename E::type;
     using F4 = Pack<float, 4>::type;
     using T4 = typename Pack<T, 4>::type;
-    const float f       = unheld<D>(upstream, count) * scale;
-    const int quads     = (channels + 3) >> 2;
-    const long long all = n * quads, slab = rows_pad * kp;
+    const float f       = unheld<D>(p.upstream, p.kept.count) * p.scale;
+    const int quads     = (p.channels + 3) >> 2;
+    const long long n   = p.what == BLOCK_ROWS ? min(p.n, *p.kept.count - (long long)p.first_row) : p.n;
+    const long long all = n * quads, slab = p.rows_pad * p.kp;
     for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < all; q += (long long)gridDim.x * 256)
     {
         const long long i = q / quads;
-        const int c = (int)(q - i * quads) * 4, at = place ? place[i] : (int)i;
+        const int c = (int)(q - i * quads) * 4, at = p.what == ALL_ROWS || p.what == OTHER_ROWS ? p.kept.place[i] : (int)i;
+        if (p.what == OTHER_ROWS && at >= 0) continue;
         F4 sum = {0.f, 0.f, 0.f, 0.f};
         if (at >= 0)
         {
-            const float* from = slabs + (long long)at * kp + c;
+            const float* from = p.slabs + (long long)at * p.kp + c;
 #pragma unroll 4
-            for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const F4*>(from + s * slab);
+            for (int s = 0; s < p.splits; ++s) sum += *reinterpret_cast<const F4*>(from + s * slab);
         }
-        T* to = reinterpret_cast<T*>(out_rows) + i * stride + c;
+        T* to = reinterpret_cast<T*>(p.out) + (p.what == BLOCK_ROWS ? (long long)p.kept.row[i] : i) * p.stride + c;
         T4 out;
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[e] = E::from_float(at >= 0 ? sum[e] * f : 0.f);
-        if (c + 4 <= channels)
+        if (c + 4 <= p.channels)
             *reinterpret_cast<T4*>(to) = out;
         else
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (c + e < channels) to[e] = out[e];
+                if (c + e < p.channels) to[e] = out[e];
     }
 }
 
 // ---- host ----
 
 constexpr int64_t kPieceBytes = 1ll << 30;  // of d_ij
+constexpr int64_t kBlockRows  = 1ll << 20;  // rows that d_ij is held of at once: 256 entries of them are kPieceBytes (in 32 bits, or in two parts)
 constexpr int64_t kPartialBytes = 1ll << 30;  // of the maxima and sums of the rows' tiles that are joined at once
 constexpr int64_t kSlabBytes  = 256ll << 20;  // of the parts of the rows' gradients
 constexpr int kCus            = 256;
@@ -1275,7 +1291,8 @@ struct Layout
 {
     int64_t rows_pad, partial_pad, chunks, piece, pieces;
     int kp, tiles, splits, table_splits, parts;
-    int at_once;  // pieces whose tiles are joined at once
+    int at_once;            // pieces whose tiles are joined at once
+    int64_t block, blocks;  // backward: rows taken at a time
     bool copies;
     size_t chunk_count, top, partial, own_product, sums, probs, slabs, table_slabs, copy, bytes;
 };
@@ -1295,7 +1312,8 @@ auto with_shape(const TripsTableLossDesc& d, bool grads, F f)
         const int64_t rows = up(d.num_rows, tile) / tile, entries = up(d.num_entries, tile) / tile, channels = up(d.num_channels, tile) / tile;
         return grads ? channels * entries : rows * entries;
     };
-    if (d.dtype != TRIPS_DTYPE_F32 && d.num_rows > 128 && units(256) >= kCus) return f(Big{});
+    // (the largest leave no parts of the table's gradient, which blocks of rows are)
+    if (d.dtype != TRIPS_DTYPE_F32 && d.num_rows > 128 && units(256) >= kCus && !(grads && d.num_rows > kBlockRows)) return f(Big{});
     const bool wide = d.dtype == TRIPS_DTYPE_F32;
     const bool few  = !grads && d.num_rows <= 32 && (wide || d.num_channels >= 2048);
     if (units(128) >= kCus && !few && (!wide || d.num_rows > 64)) return f(Small{});
@@ -1319,12 +1337,13 @@ int parts_of(const TripsTableLossDesc& d)
 }
 
 // Into how many parts the rows' gradients are cut along the entries, and the table's along the rows where its tiles are few, so that they keep all
-// CUs busy to the end, by what a step and a unit's results take, and the parts' way to memory and back.
+// CUs busy to the end, by what a step and a unit's results take, and the parts' way to memory and back. (rows: of a block; in_slabs: entries whose
+// gradients' parts are held at once.)
 struct Splits
 {
     int rows, table;
 };
-Splits splits_of(const TripsTableLossDesc& d, int64_t rows_pad, int64_t piece, int kp)
+Splits splits_of(const TripsTableLossDesc& d, int64_t rows, int64_t rows_pad, int64_t piece, int64_t in_slabs, int kp)
 {
     return with_shape(d, true, [&](auto shape)
     {
@@ -1332,9 +1351,9 @@ Splits splits_of(const TripsTableLossDesc& d, int64_t rows_pad, int64_t piece, i
         const bool wide       = d.dtype == TRIPS_DTYPE_F32;
         const int step_k      = kStepBytes / dtype_bytes(d.dtype), workers = kCus * S::PER_CU;
         const double step     = (wide ? 4.0 : S::BM == 256 ? 1.6 : 0.8) * (S::BM == 64 ? 0.5 : 1.0);  // microseconds
-        const double results  = S::BM == 256 ? 10.0 : S::BM == 128 ? 4.0 : 2.0, slab = (double)rows_pad * kp * 4, table_slab = (double)piece * kp * 4;
-        const int64_t channel_tiles = up(d.num_channels, S::BM) / S::BM, units = up(d.num_rows, S::BN) / S::BN * channel_tiles, steps = piece / step_k;
-        const int64_t table_tiles = up(std::min(piece, d.num_entries), S::BN) / S::BN * channel_tiles, table_steps = up(d.num_rows, step_k) / step_k;
+        const double results  = S::BM == 256 ? 10.0 : S::BM == 128 ? 4.0 : 2.0, slab = (double)rows_pad * kp * 4, table_slab = (double)in_slabs * kp * 4;
+        const int64_t channel_tiles = up(d.num_channels, S::BM) / S::BM, units = up(rows, S::BN) / S::BN * channel_tiles, steps = piece / step_k;
+        const int64_t table_tiles = up(std::min(piece, d.num_entries), S::BN) / S::BN * channel_tiles, table_steps = up(rows, step_k) / step_k;
         int table    = 1;
         double least = 1e300;
         for (int s = 1; s <= kMostSplits && (s == 1 || (S::BM < Big::BM && table_tiles * (s - 1) < workers && table_steps / s >= 4 && table_slab * s <= (double)kSlabBytes)); ++s)
@@ -1383,8 +1402,15 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     l.kp     = packed_channels(d);
     l.copies = copies;
     l.parts  = parts_of(d);
+    if (backward)
+    {
+        l.blocks   = std::max<int64_t>(1, (d.num_rows + kBlockRows - 1) / kBlockRows);
+        l.block    = l.blocks > 1 ? up((d.num_rows + l.blocks - 1) / l.blocks, 256) : d.num_rows;
+        l.rows_pad = up(l.block, 256);
+    }
     Taker take;
-    int64_t most = up(std::max<int64_t>(d.num_entries, 1), 256);
+    const int64_t grain = std::max(tile_of_logits(d), 64);  // (whole tiles of the logits, whole steps of the gradients)
+    int64_t most        = up(std::max<int64_t>(d.num_entries, 1), grain);
     if (copies)
     {
         most   = std::min(most, std::max<int64_t>((rows_in_place(d) ? kLeastCopyBytes : kCopyBytes) / (l.kp * size) / 256, 1) * 256);
@@ -1397,7 +1423,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     }
     if (backward) most = std::min(most, std::max<int64_t>(kPieceBytes / (std::max<int64_t>(l.rows_pad, 1) * size * l.parts) / 256, 1) * 256);
     l.pieces = std::max<int64_t>(1, (d.num_entries + most - 1) / most);
-    l.piece  = up((d.num_entries + l.pieces - 1) / l.pieces, 256);
+    l.piece  = up((d.num_entries + l.pieces - 1) / l.pieces, grain);
     if (!backward)
     {
         l.chunk_count = take((l.chunks + 1) * 4);
@@ -1412,10 +1438,11 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
     {
         l.top   = take((1 + kTops) * 4);
         l.probs = take((size_t)l.parts * l.rows_pad * l.piece * size);
-        const Splits s = splits_of(d, l.rows_pad, l.piece, l.kp);
+        const int64_t in_slabs = l.blocks > 1 ? l.pieces * l.piece : l.piece;  // (of several blocks the whole table's)
+        const Splits s         = splits_of(d, l.block, l.rows_pad, l.piece, in_slabs, l.kp);
         l.splits = s.rows, l.table_splits = s.table;
         l.slabs = take((size_t)l.splits * l.rows_pad * l.kp * 4);
-        if (l.table_splits > 1) l.table_slabs = take((size_t)l.table_splits * l.piece * l.kp * 4);
+        if (l.table_splits > 1 || l.blocks > 1) l.table_slabs = take((size_t)l.table_splits * in_slabs * l.kp * 4);
     }
     l.bytes = take.at;
     return l;
@@ -1472,6 +1499,7 @@ ProductParams product_params(const TripsTableLossDesc& d, const Layout& l, const
     p.partial = (float2*)(w + l.partial), p.own_product = (float*)(w + l.own_product), p.probs = w + l.probs, p.slabs = (float*)(w + l.slabs), p.table_slabs = (float*)(w + l.table_slabs);
     p.d_table_stride = d.d_table_stride, p.rows_pad = l.rows_pad, p.partial_pad = l.partial_pad;
     p.channels = d.num_channels, p.kp = l.kp, p.piece = (int)l.piece, p.splits = l.splits, p.table_splits = l.table_splits, p.parts = l.parts;
+    p.most_rows = 0x7fffffff, p.in_table_slabs = l.table_splits > 1 || l.blocks > 1;
     p.scale_log2 = scale_log2(d);
     return p;
 }
@@ -1553,12 +1581,10 @@ hipError_t forward(const TripsTableLossDesc& d, const void* rows, const void* ta
 }
 
 template <int D>
-hipError_t slabs_out(const TripsTableLossDesc& d, const Layout& l, const char* name, const float* slabs, const Kept& kept, const Upstream& upstream, float scale, bool placed, void* out,
-                     int64_t n, int64_t rows_pad, int64_t stride, int splits, hipStream_t stream, Profiler* prof)
+hipError_t slabs_out(const char* name, const SlabsOut& p, hipStream_t stream, Profiler* prof)
 {
     ProfScope scope(prof, name, stream);
-    slabs_out_kernel<D><<<(unsigned)std::min<int64_t>((n * ((d.num_channels + 3) / 4) + 255) / 256, 1 << 16), 256, 0, stream>>>(
-        slabs, placed ? kept.place : nullptr, kept.count, upstream, scale, out, n, rows_pad, stride, d.num_channels, l.kp, splits);
+    slabs_out_kernel<D><<<(unsigned)std::min<int64_t>((p.n * ((p.channels + 3) / 4) + 255) / 256, 1 << 16), 256, 0, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -1582,18 +1608,39 @@ hipError_t backward(const TripsTableLossDesc& d, const void* table, const Kept& 
             if (hipError_t e = hipGetLastError()) return e;
         }
     }
-    for (int64_t piece = 0; piece * l.piece < d.num_entries; ++piece)
+    SlabsOut entries{}, out{};
+    entries.kept = kept, entries.upstream = p.upstream, entries.rows_pad = l.piece, entries.stride = d.d_table_stride, entries.what = ENTRIES;
+    entries.channels = d.num_channels, entries.kp = l.kp, entries.splits = l.table_splits, entries.scale = std::fabs(d.scale);
+    out          = entries;
+    out.slabs = p.slabs, out.out = d_rows, out.n = d.num_rows, out.rows_pad = l.rows_pad, out.stride = d.d_rows_stride, out.splits = l.splits, out.scale = d.scale;
+    const bool rows_out = d_rows && d.num_rows > 0;
+    if (l.blocks > 1 && rows_out)
     {
-        if (hipError_t e = take_piece<D>(d, l, piece, table, d_table, w, p, stream, prof)) return e;
-        if (hipError_t e = launch_product<D, PROBS>(d, p, stream, prof)) return e;
-        if (hipError_t e = launch_product<D, GRADS>(d, p, stream, prof)) return e;
-        if (!d_table || l.table_splits == 1) continue;
-        if (hipError_t e = slabs_out<D>(d, l, "loss_table_out", p.table_slabs, kept, p.upstream, std::fabs(d.scale), false, p.d_table, p.in_piece, l.piece, d.d_table_stride,
-                                        l.table_splits, stream, prof))
-            return e;
+        out.what = OTHER_ROWS;
+        if (hipError_t e = slabs_out<D>("loss_rows_out", out, stream, prof)) return e;
     }
-    if (!d_rows || d.num_rows == 0) return hipSuccess;
-    return slabs_out<D>(d, l, "loss_rows_out", (float*)(w + l.slabs), kept, p.upstream, d.scale, true, d_rows, d.num_rows, l.rows_pad, d.d_rows_stride, l.splits, stream, prof);
+    for (int64_t block = 0; block < l.blocks; ++block)
+    {
+        const int64_t first = block * l.block;
+        p.first_row = (int)first, p.most_rows = (int)l.block, p.add_to_table = block > 0;
+        p.kept.row = kept.row + first, p.kept.target = kept.target + first, p.kept.state = kept.state + first;
+        p.kept.packed = reinterpret_cast<char*>(kept.packed) + first * l.kp * dtype_bytes(d.dtype);
+        for (int64_t piece = 0; piece * l.piece < d.num_entries; ++piece)
+        {
+            if (hipError_t e = take_piece<D>(d, l, piece, table, d_table, w, p, stream, prof)) return e;
+            p.table_slabs = (float*)(w + l.table_slabs) + (l.blocks > 1 ? piece * l.table_splits * l.piece * l.kp : 0);
+            if (hipError_t e = launch_product<D, PROBS>(d, p, stream, prof)) return e;
+            if (hipError_t e = launch_product<D, GRADS>(d, p, stream, prof)) return e;
+            if (!d_table || !p.in_table_slabs || block + 1 < l.blocks) continue;
+            entries.slabs = p.table_slabs, entries.out = p.d_table, entries.n = p.in_piece;
+            if (hipError_t e = slabs_out<D>("loss_table_out", entries, stream, prof)) return e;
+        }
+        if (!rows_out) continue;
+        if (l.blocks > 1) out.what = BLOCK_ROWS, out.kept = p.kept, out.first_row = p.first_row, out.n = l.block;
+        else out.what = ALL_ROWS;
+        if (hipError_t e = slabs_out<D>("loss_rows_out", out, stream, prof)) return e;
+    }
+    return hipSuccess;
 }
 
 int check_stride(const char* name, int64_t stride, int64_t row, int64_t rows, bool written)
@@ -1611,7 +1658,7 @@ int check_units(const TripsTableLossDesc& d)
         const double units = with_shape(d, grads, [&](auto shape)
         {
             using S = decltype(shape);
-            const double rows = (double)(up(d.num_rows, S::BN) / S::BN), entries = (double)(up(d.num_entries, S::BN) / S::BN), channels = (double)(up(d.num_channels, S::BM) / S::BM);
+            const double rows = (double)(up(grads ? std::min(d.num_rows, kBlockRows) : d.num_rows, S::BN) / S::BN), entries = (double)(up(d.num_entries, S::BN) / S::BN), channels = (double)(up(d.num_channels, S::BM) / S::BM);
             return grads ? channels * (rows * kMostSplits + entries) + kCus * S::PER_CU : rows * entries;  // (see splits_of())
         });
         if (units >= 2147000000.0) return set_error(TRIPS_ERR_UNSUPPORTED, "%lld rows and %lld entries are too many for one call", (long long)d.num_rows, (long long)d.num_entries);
