@@ -414,7 +414,7 @@ __device__ __forceinline__ Acc product(Half8 a, Half8 b, Acc c)
 // (By itself: of a builtin the compiler would wait for the last load before any read of LDS.)
 __device__ __forceinline__ void load_to_lds(const Words4& buffer, unsigned offset, unsigned lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory", "m0");
 }
 __device__ __forceinline__ Words4 buffer_of(const void* base, long long bytes)
 {
