@@ -39,8 +39,8 @@ class Loss:
     """The cross entropy of rows against a table, in double precision, and how far the kernels may be off.
 
     e_i, the products of a row: a sum of C products in float32 in any order, each addition off by at most 2^-23 of the sum of
-    magnitudes (the matrix instructions may cut where others round), so C 2^-23 max_j sum_c |x_ic w_jc| |scale|. In float32 the products
-    of three parts of a number each (of eight bits) leave out what is below 2^-23 of a product: two more. Both the products and what
+    magnitudes (the matrix instructions may cut where others round), so C 2^-23 max_j sum_c |x_ic w_jc| |scale|, for C + 2 of them here (two
+    more than there are). Both the products and what
     they are compared with are off by e_i; the difference and its scaling add 4 U of their size (at most 2 max_j |l_ij|).
     The exponential is off by 2^-22 of itself, its sum, in chains of at most 320 + T / 64 terms, by as many U."""
 

@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherParams p)
 template <int D>
 constexpr float kHeld = D == TRIPS_DTYPE_F16 ? 32768.f : 1.f;
 
-// In 16 bits d_ij is off by up to 2^-9 (bfloat16) of itself, and so is what it adds to the gradients, which are rounded as far once more: their
+// In 16 bits d_ij is off by up to 2^-8 (bfloat16) or 2^-11 (float16) of itself, and so is what it adds to the gradients, which are rounded as far once more: their
 // error against the exact ones is 1.1 to 1.8 times that of this last rounding alone, the more the fewer entries share a row's probability. Holding the
 // rest of d_ij as well, as a second part of the same type, takes that away and doubles the gradients' products: done where those are few (see
 // parts_of()).
@@ -578,11 +578,11 @@ __device__ __forceinline__ int share_of(const Share& s, int ordinal, int w, int 
     return early * more + (w >= rest ? w - rest : w + early) + j * all;
 }
 
-// Large problems of 16 bits are bound by the card's power: the matrix instructions fill 53 to 68 % of a busy CU's cycles at 1.6 to 1.8 GHz of 2.4, no bank
+// Large problems of 16 bits are bound by the card's power and by the tiles' results: the matrix instructions fill 52 to 66 % of a busy CU's cycles at 1.6 to 1.9 GHz of 2.4, no bank
 // of LDS conflicts, and fewer waits lower the clock. What is left of the cycles goes to the results: of 772 and 830 us for the logits of 7782 rows and 50,000 entries of
-// 1024 bfloat16 channels and their gradient 637 and 633 are without them. There: logits 755 us (1.06 PFLOP/s), their gradient 830 (0.96), both gradients 1420
-// (1.12; a library's product of 16384 a side reaches 1.58, of these sizes 1.20). In 32 bits the matrix instructions fill 80 to 87 % at 2.2 GHz (1023 rows, 20,000 entries
-// of 384: 145, 151 and 291 us, 108 TFLOP/s of 154). Few rows are bound by the table's way in: one row and 50,000 entries of 1024 bfloat16 channels 21 us, 5.0 TB/s.
+// 1024 bfloat16 channels and their gradient 637 and 633 are without them. There: logits 731 to 774 us (1.06 PFLOP/s), their gradient 813 to 837 (0.97), both gradients 1395 to 1408
+// (1.14; a library's product of 16384 a side reaches 1.58, of these sizes 1.20). In 32 bits the matrix instructions fill 80 to 87 % at 2.2 GHz (1023 rows, 20,000 entries
+// of 384: 144, 152 and 289 us, 108 TFLOP/s of 154). Few rows are bound by the table's way in: one row and 50,000 entries of 1024 bfloat16 channels 21.3 us, 4.8 TB/s.
 //
 // LOGITS, PROBS, or GRADS: D_ROWS and D_TABLE in one launch. S::PER_CU workgroups a CU, each goes through its units; the loads run STAGES steps
 // ahead of the products and go on into the next unit, so that they are under way while a unit's results are written.
@@ -1409,7 +1409,7 @@ Layout layout_of(const TripsTableLossDesc& d, bool backward, bool copies)
         l.rows_pad = up(l.block, 256);
     }
     Taker take;
-    const int64_t grain = std::max(tile_of_logits(d), 64);  // (whole tiles of the logits, whole steps of the gradients)
+    const int64_t grain = d.num_entries < 256 ? std::max(tile_of_logits(d), 64) : 256;  // (whole tiles of the logits, whole steps of the gradients; few entries are not padded to more)
     int64_t most        = up(std::max<int64_t>(d.num_entries, 1), grain);
     if (copies)
     {
