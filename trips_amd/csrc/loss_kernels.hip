@@ -1376,16 +1376,20 @@ Splits splits_of(const TripsTableLossDesc& d, int64_t rows, int64_t rows_pad, in
             const int64_t rest = a % workers;
             const double full  = (double)(a / workers) * size_a;
             double end         = full + (rest ? size_a : 0.0);
-            for (int64_t k = b / workers;; ++k)
+            // (the least number of rounds of b by whose end all of it is done, which is found by doubling and halving: what is done grows with the rounds)
+            auto enough = [&](int64_t k)
             {
-                const double t     = full + (double)k * size_b, late = t - full - size_a;
-                const int64_t done = (workers - rest) * k + (rest && late > 0 ? rest * (int64_t)(late / size_b) : 0);
-                if (done >= b)
-                {
-                    end = std::max(end, t);
-                    break;
-                }
+                const double late = (double)k * size_b - size_a;
+                return (workers - rest) * k + (rest && late > 0 ? rest * (int64_t)(late / size_b) : 0) >= b;
+            };
+            int64_t low = b / workers, high = low;
+            for (int64_t by = 1; !enough(high); by *= 2) low = high + 1, high += by;
+            while (low < high)
+            {
+                const int64_t k = (low + high) / 2;
+                if (enough(k)) high = k; else low = k + 1;
             }
+            end = std::max(end, full + (double)low * size_b);
             end += s * slab / 3.5e6;
             if (end < least) best = s, least = end;
         }
