@@ -2,6 +2,8 @@
 call, the step and an element's place, so the mask is made again for the gradient and never stored, and is the same on every
 device, in every type and however the elements are split over launches.
 """
+import operator
+
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
@@ -41,11 +43,11 @@ def dropout(x, p, seed, call=0, step=0, residual=None):
     """x with each element dropped (0, whatever it was) with probability p and the others scaled by 1 / (1 - p), plus `residual` (of x's
     shape and type) if there is one. p is rounded to a multiple of 2^-16, and the scale is that of the rounded one.
 
-    The generator's counter is the element's place in x (as if it were contiguous), `call`, which tells the dropouts of a step apart, and
+    The generator's key is the low 64 bits of `seed`, its counter the element's place in x (as if it were contiguous), `call`, which tells the dropouts of a step apart, and
     `step`: a number below 2^32, or one int32 or int64 on x's device, of which the kernel reads the low 32 bits, for steps that are captured
     into a graph (a parameter's step count of AdamW, for instance). Differentiable in x and residual, once; the gradient of x is this
     function of the gradient, with the step that was used."""
-    seed = (seed + (1 << 63)) % (1 << 64) - (1 << 63)  # (64 bits, as the extension takes them)
+    seed = (operator.index(seed) + (1 << 63)) % (1 << 64) - (1 << 63)  # (64 bits, as the extension takes them; numpy's whole numbers too)
     if not 0 <= call < 1 << 32 or not (torch.is_tensor(step) or 0 <= step < 1 << 32):
         raise ValueError(f"call and step: 32 bits expected, got {call} and {step}")
     if forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(*(t for t in (x, residual, step) if torch.is_tensor(t))):
