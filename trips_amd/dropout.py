@@ -50,7 +50,9 @@ def dropout(x, p, seed, call=0, step=0, residual=None):
     seed = (operator.index(seed) + (1 << 63)) % (1 << 64) - (1 << 63)  # (64 bits, as the extension takes them; numpy's whole numbers too)
     if not 0 <= call < 1 << 32 or not (torch.is_tensor(step) or 0 <= step < 1 << 32):
         raise ValueError(f"call and step: 32 bits expected, got {call} and {step}")
-    if forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(*(t for t in (x, residual, step) if torch.is_tensor(t))):
+    if torch.is_tensor(p) and p.requires_grad and torch.is_grad_enabled():
+        raise ValueError("p: it gets no gradient")
+    if forward_ad._current_level >= 0 or torch.jit.is_tracing() or _transformed(*(t for t in (x, residual, step, p) if torch.is_tensor(t))):
         return _Dropout.apply(x, p, seed, call, step, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         ctx, stream = _where(x)
